@@ -23,6 +23,7 @@ ERR_UNSUPPORTED = -5
 
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+DTYPE_F16 = 2
 EMPTY_ROW_ZEROS = 0
 EMPTY_ROW_UNIFORM = 1
 
@@ -120,6 +121,30 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "b200ta_mask_lengths": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "b200ta_mask_bits": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "b200ta_layer_norm": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int, c_int64, c_int, c_float, c_void_p],
+    ),
+    "b200ta_layer_norm_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "b200ta_layer_norm_backward": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+         c_size_t, c_int, c_int64, c_int, c_void_p],
+    ),
+    "b200ta_dense_few_rows": (c_int, []),
+    "b200ta_dense": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int,
+         c_int, c_int64, c_int, c_int, c_void_p],
+    ),
+    "b200ta_dense_keeps": (c_int, [c_int, c_int, c_int]),
+    "b200ta_dense_backward_workspace_bytes": (c_size_t, [c_int, c_int, c_int64, c_int, c_int]),
+    "b200ta_dense_backward": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+         c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int64, c_int, c_int, c_void_p],
+    ),
+    "b200ta_copy_rows": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
 }
 
 

@@ -22,9 +22,11 @@ PKG = CSRC.parent
 LIB = PKG / "libb200ta.so"
 HOST = PKG / "_host.so"
 OBJ_DIR = CSRC / "build"
+HOST_SOURCES = [CSRC / "torch_host.cpp", CSRC / "torch_training.cpp"]
 HOST_MADE_FOR = "host_made_for.txt"
 SOURCES = ["host.cu", "pack.cu", "rowgemm.cu", "attention.cu", "node.cu", "transition.cu", "trimul_project.cu",
-           "trimul_contract.cu", "trimul_output.cu", "linear.cu", "pair_bias.cu", "masks.cu"]
+           "trimul_contract.cu", "trimul_output.cu", "linear.cu", "pair_bias.cu", "masks.cu",
+           "layer_norm.cu", "dense.cu", "matmul_forward.cu", "matmul_grad.cu", "matmul_product.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo", "--use_fast_math",
@@ -61,12 +63,12 @@ def _host_made_for() -> str:
 def _host_stale() -> bool:
     """Whether _host.so is missing, older than its sources or made for another PyTorch, interpreter or toolkit."""
     made_for = OBJ_DIR / HOST_MADE_FOR
-    return (_stale(HOST, [CSRC / "torch_host.cpp", PKG.parent / "include" / "b200ta.h"])
+    return (_stale(HOST, [*HOST_SOURCES, CSRC / "torch_host.h", PKG.parent / "include" / "b200ta.h"])
             or not made_for.exists() or made_for.read_text() != _host_made_for())
 
 
 def _build_host(force: bool) -> None:
-    """_host.so from torch_host.cpp against the headers of the installed PyTorch; it links none of the kernels."""
+    """_host.so from its sources against the headers of the installed PyTorch; it links none of the kernels."""
     if not (force or _host_stale()):
         return
     import sysconfig
@@ -79,7 +81,7 @@ def _build_host(force: bool) -> None:
            "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_host",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *(f"-I{p}" for p in include_paths()), f"-I{sysconfig.get_paths()['include']}", f"-I{cuda / 'include'}",
-           str(CSRC / "torch_host.cpp"), "-o", str(HOST), *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           *map(str, HOST_SOURCES), "-o", str(HOST), *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu",
            "-ltorch_python", f"-L{cuda / 'lib64'}", "-lcudart", "-ldl"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:

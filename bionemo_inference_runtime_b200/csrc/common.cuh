@@ -44,12 +44,12 @@ struct DeviceState {
   int device = -1;
   int num_sms = 0;
   int* status_dev = nullptr;  // device word kernels write when they abandon a bounded wait
-  std::atomic<uint32_t> configured{0};  // bit per KernelId: its shared-memory limit has been raised on this device
+  std::atomic<uint64_t> configured{0};  // bit per KernelId: its shared-memory limit has been raised on this device
 };
 enum KernelId {
   kKernelPrologue, kKernelEpilogue, kKernelAttention, kKernelAttentionMasked, kKernelTransition, kKernelTransitionRelu,
   kKernelProject, kKernelContract, kKernelOutput, kKernelOutputF32, kKernelLinear, kKernelPairBias, kKernelRowStats,
-  kKernelMaskRows
+  kKernelMaskRows, kKernelNorm, kKernelDenseHelpers, kKernelMatmul  // and one for each of the matmul kernels after it
 };
 int get_device_state(DeviceState** out);
 
@@ -60,7 +60,7 @@ int get_device_state(DeviceState** out);
 template <typename... P, typename... A>
 int launch_kernel(DeviceState* st, KernelId id, void (*kernel)(P...), dim3 grid, int threads, int smem_bytes, void* stream,
                   A&&... args) {
-  const uint32_t bit = 1u << id;
+  const uint64_t bit = 1ull << id;
   if (smem_bytes > 0 && !(st->configured.load(std::memory_order_relaxed) & bit)) {
     B200TA_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
     st->configured.fetch_or(bit, std::memory_order_relaxed);

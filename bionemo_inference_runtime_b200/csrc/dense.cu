@@ -1,0 +1,609 @@
+// The trainable dense layers around their products: argument checks, tensor maps and tiles of the products, and the small
+// kernels beside them (few rows, dz from stored pre-activations, sums over rows, joining of parts, aligned copies).
+#include "matmul.cuh"
+
+namespace b200ta {
+
+namespace {
+
+int map_of(CUtensorMap* map, const Plane& t, int bytes, uint32_t columns, uint32_t rows, uint32_t outer, SwizzleMode swz, const char* what) {
+  const uint64_t dims[3] = {uint64_t(t.columns), uint64_t(t.rows), uint64_t(t.outer)};
+  const uint64_t strides[2] = {uint64_t(t.pitch) * bytes, uint64_t(t.outer > 1 ? t.outer_stride : t.pitch) * bytes};
+  const uint32_t box[3] = {columns, rows, outer};
+  return encode_tensor_map(map, t.base, bytes, 3, dims, strides, box, swz, what);
+}
+
+// Columns of a tile's accumulator.  A tile costs the larger of its MMAs (a [128 x n x 64] block takes 4 * max(40, n * 0.54)
+// clocks), its operands' way from L2 (46 bytes a clock and SM) and its finishing (some 7 clocks a column), and all blocks
+// take as many tiles as the busiest: wide tiles where there are enough of them, narrow ones to give every SM work.  Each of
+// the finishing warps' two halves takes whole groups of 32 result columns, which sets the least width.
+int choose_tile_n(int64_t tiles_m, int64_t columns, int kblocks, int least_n, int num_sms) {
+  int best = 256;
+  double least = 1e300;
+  for (int n = 256; n >= least_n; n /= 2) {
+    const double tiles = double(tiles_m) * double((columns + n - 1) / n);
+    const double mma = 4.0 * (n * 0.54 > 40 ? n * 0.54 : 40), load = (16384.0 + n * 128.0) / 46;
+    double tile = kblocks * (mma > load ? mma : load);
+    if (tile < 7.0 * n) tile = 7.0 * n;
+    const double waves = double(int64_t((tiles + num_sms - 1) / num_sms));
+    const double cost = waves * tile;
+    if (cost < least * 0.98) least = cost, best = n;
+  }
+  return best;
+}
+
+}  // namespace
+
+int run_matmul(const Matmul& m, void* stream) {
+  DeviceState* st = nullptr;
+  int rc = get_device_state(&st);
+  if (rc != B200TA_OK) return rc;
+  const bool two = m.form == kGated || m.form == kGatedGrad;
+  MatmulParams p{};
+  const int64_t rows = m.a_mn ? m.a.columns : m.a.rows, columns = m.b_mn ? m.b.columns : m.b.rows;
+  const int64_t k = m.a_mn ? m.a.rows : m.a.columns, m_outer = m.a_mn ? m.a.outer : 1, k_outer = m.a_mn ? 1 : m.a.outer;
+  constexpr int64_t kMost = int64_t(1) << 31;
+  B200TA_REQUIRE(rows < kMost - 512 && columns < kMost - 512 && k < kMost - 512, "%s: a size is past 2^31", m.what);
+  p.tiles_m_inner = int((rows + matmul::kBM - 1) / matmul::kBM);
+  p.tiles_m = int(p.tiles_m_inner * m_outer);
+  p.kblocks_inner = int((k + matmul::kBK - 1) / matmul::kBK);
+  p.kblocks = int(p.kblocks_inner * k_outer);
+  p.kblocks_split = m.kblocks_split > 0 && m.kblocks_split < p.kblocks ? m.kblocks_split : p.kblocks;
+  p.splits = (p.kblocks + p.kblocks_split - 1) / p.kblocks_split;
+  p.rows_inner = int(rows), p.columns = int(columns);
+  p.tile_n = choose_tile_n(int64_t(p.tiles_m) * p.splits, two ? columns * 2 : columns, p.kblocks_split, two ? 128 : 64, st->num_sms);
+  const int units = two ? p.tile_n / 2 : p.tile_n;
+  p.tiles_n = int((columns + units - 1) / units);
+  const int64_t work = int64_t(p.tiles_m) * p.tiles_n * p.splits;
+  B200TA_REQUIRE(work < kMost - 1024, "%s: too many tiles", m.what);
+  p.work = int(work);
+  p.group_m = 16;
+  const int stage = matmul::kABytes + p.tile_n * matmul::kBK * 2;
+  p.stages = matmul::kRingBytes / stage < matmul::kMaxStages ? matmul::kRingBytes / stage : matmul::kMaxStages;
+  p.bias = m.bias;
+  p.activation = m.activation;
+  p.has_aux = m.aux.base != nullptr, p.has_saved = m.saved.base != nullptr, p.accumulate = m.accumulate;
+  p.status = st->status_dev;
+
+  MatmulMaps maps{};
+  rc = m.a_mn ? map_of(&maps.a, m.a, 2, 64, 64, 1, SWZ_128, m.what) : map_of(&maps.a, m.a, 2, 64, matmul::kBM, 1, SWZ_128, m.what);
+  if (rc != B200TA_OK) return rc;
+  rc = m.b_mn ? map_of(&maps.b, m.b, 2, 64, 64, 1, SWZ_128, m.what)
+              : map_of(&maps.b, m.b, 2, 64, uint32_t(units), two ? 2 : 1, SWZ_128, m.what);
+  if (rc != B200TA_OK) return rc;
+  const bool f32 = m.form == kPartial;
+  rc = map_of(&maps.out, m.out, f32 ? 4 : 2, 32, 32, 1, f32 ? SWZ_128 : SWZ_64, m.what);
+  if (rc != B200TA_OK) return rc;
+  if (p.has_aux && (rc = map_of(&maps.aux, m.aux, 2, 32, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
+  if (p.has_saved && (rc = map_of(&maps.saved, m.saved, 2, 32, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
+  const int grid = p.work < st->num_sms ? p.work : st->num_sms;
+  if (m.form == kDenseGrad || m.form == kGatedGrad) return launch_matmul_grad(st, m, maps, p, grid, stream);
+  if (m.b_mn) return launch_matmul_product(st, m, maps, p, grid, stream);
+  return launch_matmul_forward(st, m, maps, p, grid, stream);
+}
+
+namespace {
+
+// ---- few rows ---------------------------------------------------------------------------------------------------
+//
+// Up to 16 rows: the weights are read once and that bounds the call, or its latency does.  A warp takes one result column (a
+// value and a gate row of W for kGated), its lanes run along k with 16-byte loads, the rows' sums are exchanged so that each
+// row's ends in a lane of its own.  128-row tiles of the tensor cores would leave all but N / 64 SMs idle.
+constexpr int kFewRows = 16;
+
+struct FewParams {
+  const void *x, *w, *bias, *residual;
+  void *y, *saved;
+  long long xs, ws, rs, ys, ss;
+  int rows, K, N, activation, gated, f16;
+};
+
+template <typename T, int kVec>
+__device__ __forceinline__ void load_vec(const T* p, float* v) {
+  if constexpr (kVec == 1) {
+    v[0] = static_cast<float>(*p);
+  } else {
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack2<T>(w[e]);
+      v[2 * e] = f.x, v[2 * e + 1] = f.y;
+    }
+  }
+}
+
+__device__ __forceinline__ void activate_any(int activation, float z, float& a, float& s) {
+  float a1, s1;
+  switch (activation) {
+    case kActNone: return activate2<kActNone, true>(z, z, a, a1, s, s1);
+    case kActRelu: return activate2<kActRelu, true>(z, z, a, a1, s, s1);
+    case kActSilu: return activate2<kActSilu, true>(z, z, a, a1, s, s1);
+    case kActGelu: return activate2<kActGelu, true>(z, z, a, a1, s, s1);
+    case kActGeluTanh: return activate2<kActGeluTanh, true>(z, z, a, a1, s, s1);
+    default: return activate2<kActSigmoid, true>(z, z, a, a1, s, s1);
+  }
+}
+
+// The sums over a warp of kRows values: lane l ends with that of row (l >> (5 - log2 kRows)).
+template <int kRows>
+__device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
+  int o = 16;
+#pragma unroll
+  for (int n = kRows; n > 1; n >>= 1, o >>= 1) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const float keep = upper ? v[i + n / 2] : v[i], give = upper ? v[i] : v[i + n / 2];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  for (; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  return v[0];
+}
+
+template <typename T, int kRows, int kVec, bool kTwo>
+__global__ void __launch_bounds__(128)
+few_rows_kernel(const FewParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, n = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (n >= p.N) return;
+  const T* x = static_cast<const T*>(p.x);
+  const T* w = static_cast<const T*>(p.w) + n * p.ws;
+  const T* wg = static_cast<const T*>(p.w) + (long long)(n + p.N) * p.ws;
+  float acc[kRows], gate[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) acc[r] = 0.f, gate[r] = 0.f;
+#pragma unroll 2
+  for (int k = lane * kVec; k < p.K; k += 32 * kVec) {
+    float a[kVec], b[kVec], c[kVec];
+    load_vec<T, kVec>(w + k, a);
+    if constexpr (kTwo) load_vec<T, kVec>(wg + k, b);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (r < p.rows) {
+        load_vec<T, kVec>(x + r * p.xs + k, c);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          acc[r] = fmaf(a[e], c[e], acc[r]);
+          if constexpr (kTwo) gate[r] = fmaf(b[e], c[e], gate[r]);
+        }
+      }
+    }
+  }
+  constexpr int kShift = kRows == 16 ? 1 : kRows == 8 ? 2 : kRows == 4 ? 3 : kRows == 2 ? 4 : 5;
+  float v = sum_rows<kRows>(acc, lane), g = 0.f;
+  if constexpr (kTwo) g = sum_rows<kRows>(gate, lane);
+  const int row = lane >> kShift;
+  if ((lane & ((1 << kShift) - 1)) != 0 || row >= p.rows) return;
+  const T* bias = static_cast<const T*>(p.bias);
+  if (bias != nullptr) {
+    v += static_cast<float>(bias[n]);
+    if (kTwo) g += static_cast<float>(bias[n + p.N]);
+  }
+  if (p.saved != nullptr) {
+    T* s = static_cast<T*>(p.saved) + row * p.ss + n;
+    s[0] = static_cast<T>(v);
+    if (kTwo) s[p.ss / 2] = static_cast<T>(g);
+  }
+  float a, slope;
+  activate_any(p.activation, kTwo ? g : v, a, slope);
+  if (kTwo) a *= v;
+  if (p.residual != nullptr) a += static_cast<float>(static_cast<const T*>(p.residual)[row * p.rs + n]);
+  static_cast<T*>(p.y)[row * p.ys + n] = static_cast<T>(a);
+}
+
+template <typename T, int kVec, bool kTwo>
+auto pick_few(int rows) {
+  if (rows <= 1) return &few_rows_kernel<T, 1, kVec, kTwo>;
+  if (rows <= 2) return &few_rows_kernel<T, 2, kVec, kTwo>;
+  if (rows <= 4) return &few_rows_kernel<T, 4, kVec, kTwo>;
+  return rows <= 8 ? &few_rows_kernel<T, 8, kVec, kTwo> : &few_rows_kernel<T, 16, kVec, kTwo>;
+}
+template <typename T>
+auto pick_few(int rows, bool vec, bool two) {
+  if (two) return vec ? pick_few<T, 8, true>(rows) : pick_few<T, 1, true>(rows);
+  return vec ? pick_few<T, 8, false>(rows) : pick_few<T, 1, false>(rows);
+}
+
+// ---- dz from stored pre-activations ---------------------------------------------------------------------------------
+//
+// dz = dy act'(z), or [dy act(g) | dy v act'(g)]: reads 2 (3) and writes 1 (2) planes, bound by HBM.  Eight columns a thread.
+struct SlopeParams {
+  const void *dy, *saved;
+  void* dz;
+  long long dys, ss, zs, rows;
+  int N;
+};
+template <typename T, int kAct, bool kTwo>
+__global__ void __launch_bounds__(256)
+slope_kernel(const SlopeParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int vectors = (p.N + 7) / 8;
+  const long long total = p.rows * vectors;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long row = i / vectors;
+    const int c = int(i - row * vectors) * 8;
+    const T* dy = static_cast<const T*>(p.dy) + row * p.dys + c;
+    const T* z = static_cast<const T*>(p.saved) + row * p.ss + c;
+    T* dz = static_cast<T*>(p.dz) + row * p.zs + c;
+    float d[8], v[8], g[8];
+    if (c + 8 <= p.N) {
+      load_vec<T, 8>(dy, d);
+      load_vec<T, 8>(z, v);
+      if constexpr (kTwo) load_vec<T, 8>(z + p.ss / 2, g);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool in = c + j < p.N;
+        d[j] = in ? static_cast<float>(dy[j]) : 0.f, v[j] = in ? static_cast<float>(z[j]) : 0.f;
+        if constexpr (kTwo) g[j] = in ? static_cast<float>(z[p.ss / 2 + j]) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      float a0, a1, s0, s1;
+      if constexpr (kTwo) {
+        activate2<kAct, true>(g[j], g[j + 1], a0, a1, s0, s1);
+        g[j] = d[j] * v[j] * s0, g[j + 1] = d[j + 1] * v[j + 1] * s1;
+        v[j] = d[j] * a0, v[j + 1] = d[j + 1] * a1;
+      } else {
+        activate2<kAct, true>(v[j], v[j + 1], a0, a1, s0, s1);
+        v[j] = d[j] * s0, v[j + 1] = d[j + 1] * s1;
+      }
+    }
+    // (dz's rows are padded to eight columns: its last vector is stored whole)
+    *reinterpret_cast<uint4*>(dz) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    if constexpr (kTwo)
+      *reinterpret_cast<uint4*>(dz + p.zs / 2) =
+          make_uint4(pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3]), pack2<T>(g[4], g[5]), pack2<T>(g[6], g[7]));
+  }
+}
+template <typename T, bool kTwo>
+auto pick_slope(int activation) {
+  switch (activation) {
+    case kActNone: return &slope_kernel<T, kActNone, kTwo>;
+    case kActRelu: return &slope_kernel<T, kActRelu, kTwo>;
+    case kActSilu: return &slope_kernel<T, kActSilu, kTwo>;
+    case kActGelu: return &slope_kernel<T, kActGelu, kTwo>;
+    case kActGeluTanh: return &slope_kernel<T, kActGeluTanh, kTwo>;
+    default: return &slope_kernel<T, kActSigmoid, kTwo>;
+  }
+}
+
+// ---- sums over rows -------------------------------------------------------------------------------------------------
+//
+// part[block.y][n] (+)= sum over a block's rows of dz[., n].  32 lanes of eight columns, eight rows at a time.
+template <typename T>
+__global__ void __launch_bounds__(256)
+row_sum_kernel(const T* dz, long long pitch, long long rows, int N, long long part_pitch, int rows_block, int accumulate, float* part) {
+  __shared__ float joined[8][256 + 4];
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 256 + lane * 8;
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const long long r0 = (long long)blockIdx.y * rows_block, r1 = r0 + rows_block < rows ? r0 + rows_block : rows;
+  if (c < N) {
+#pragma unroll 4
+    for (long long r = r0 + k; r < r1; r += 8) {
+      float v[8];
+      if (c + 8 <= N) {
+        load_vec<T, 8>(dz + r * pitch + c, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < N ? static_cast<float>(dz[r * pitch + c + j]) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) joined[k][lane * 8 + j] = s[j];
+  __syncthreads();
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n < N) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += joined[i][threadIdx.x];
+    float* dst = part + (long long)blockIdx.y * part_pitch + n;
+    *dst = accumulate ? *dst + sum : sum;
+  }
+}
+
+// out[r][c] = sum over the parts, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+join_kernel(const float* part, int parts, long long part_stride, long long pitch, long long rows, int columns, T* out, long long out_pitch) {
+  pdl_trigger();
+  pdl_wait();
+  const long long total = rows * columns;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long r = i / columns, c = i - r * columns;
+    const float* src = part + r * pitch + c;
+    float sum = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < parts; ++s) sum += __ldg(src + s * part_stride);
+    out[r * out_pitch + c] = static_cast<T>(sum);
+  }
+}
+
+// ---- aligned copies ---------------------------------------------------------------------------------------------------
+//
+// dst[r][c] = src[r * rs + c * cs] for 16-bit elements: tensors whose rows a TMA load or store cannot address (a pitch or
+// base that is no multiple of 16 bytes, columns that are not contiguous) pass through a padded copy.  [32 x 32] tiles turned
+// in shared memory where the rows are contiguous instead of the columns.
+__global__ void __launch_bounds__(256)
+copy_rows_kernel(const uint16_t* src, long long rs, long long cs, uint16_t* dst, long long pitch, long long rows, int columns) {
+  __shared__ uint16_t tile[32][34];
+  pdl_trigger();
+  pdl_wait();
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int tiles_c = (columns + 31) / 32;
+  const long long tiles = (rows + 31) / 32 * tiles_c;
+  const bool turn = cs != 1;
+  for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const long long r0 = t / tiles_c * 32;
+    const int c0 = int(t % tiles_c) * 32;
+    if (!turn) {
+      for (int i = ty; i < 32; i += 8)
+        if (r0 + i < rows && c0 + tx < columns) dst[(r0 + i) * pitch + c0 + tx] = src[(r0 + i) * rs + c0 + tx];
+    } else {
+      for (int i = ty; i < 32; i += 8)
+        if (r0 + tx < rows && c0 + i < columns) tile[i][tx] = src[(r0 + tx) * rs + (c0 + i) * cs];
+      __syncthreads();
+      for (int i = ty; i < 32; i += 8)
+        if (r0 + i < rows && c0 + tx < columns) dst[(r0 + i) * pitch + c0 + tx] = tile[tx][i];
+      __syncthreads();
+    }
+  }
+}
+
+bool rows_aligned(const void* p, int64_t pitch) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && pitch % 8 == 0; }
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+int64_t pad4(int64_t n) { return (n + 3) / 4 * 4; }
+
+int check_layer(const char* what, int dtype, int activation, int64_t rows, int K, int N) {
+  B200TA_REQUIRE(dtype == B200TA_DTYPE_BF16 || dtype == B200TA_DTYPE_F16, "%s: activations and weights are bf16 or fp16 (dtype %d)", what, dtype);
+  B200TA_REQUIRE(activation >= 0 && activation < kActCount, "%s: unknown activation %d", what, activation);
+  B200TA_REQUIRE(rows > 0 && K > 0 && N > 0 && rows < (int64_t(1) << 31) - 512 && N < (1 << 30), "%s: rows=%lld, K=%d, N=%d", what,
+                 (long long)rows, K, N);
+  return B200TA_OK;
+}
+
+// How dW = dz^T x is cut along the rows: enough parts to give every SM a tile, few enough that reading them again stays
+// small.  A tile takes some 550 clocks per 64 rows and 256 columns, its store and start some 3000; parts are written and read
+// once at some 3400 bytes a clock.
+struct Split {
+  int kblocks, parts;  // of a part; in all
+};
+Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns, int num_sms) {
+  const int64_t kblocks = (rows + matmul::kBK - 1) / matmul::kBK;
+  const int64_t tiles_m = (n_rows + 127) / 128 * n_outer;
+  const int tile_n = columns > 128 ? 256 : columns > 64 ? 128 : 64;
+  const int64_t tiles = tiles_m * ((columns + tile_n - 1) / tile_n);
+  Split best{int(kblocks), 1};
+  double least = 1e300;
+  for (int64_t parts = 1; parts <= 256 && parts <= kblocks; ++parts) {
+    const int64_t per = (kblocks + parts - 1) / parts;
+    if ((kblocks + per - 1) / per != parts) continue;
+    const double waves = double((tiles * parts + num_sms - 1) / num_sms);
+    const double bytes = parts == 1 ? 0 : 8.0 * double(parts) * double(n_rows * n_outer) * double(columns);
+    const double cost = waves * (double(per) * 550 * tile_n / 256 + 3000) + bytes / 3400;
+    if (cost < least) least = cost, best = {int(per), int(parts)};
+  }
+  return best;
+}
+constexpr int kSumRows = 1024;  // rows of a partial sum of db
+
+// The backward pass: how many rows at a time, and where its intermediates lie in the workspace.
+struct BackwardPlan {
+  int64_t chunk;      // rows of dz at a time
+  int64_t dz_pitch;   // 0: dz is dy
+  Split split;        // of a chunk's rows for dW
+  bool direct;        // dW is written by its product
+  int64_t dz, parts, sums, bytes;  // offsets, total
+};
+BackwardPlan plan_backward(bool gated, bool slope, int64_t rows, int K, int N, int num_sms) {
+  BackwardPlan p{};
+  const int64_t outer = gated ? 2 : 1;
+  p.dz_pitch = gated || slope ? outer * pad8(N) : 0;
+  p.chunk = rows;
+  if (p.dz_pitch != 0) {
+    // Narrow layers are bound by HBM: dz of a chunk is read back from L2 if it fits there, and the next chunk overwrites it.
+    // Wide layers are bound by the tensor cores: their chunks only keep the workspace small.
+    const int64_t most = (K <= 256 ? int64_t(48) : int64_t(1024)) << 20;
+    const int64_t fit = most / (p.dz_pitch * 2) / kSumRows * kSumRows;
+    const int64_t chunk = fit < kSumRows ? kSumRows : fit;
+    if (chunk < rows) {
+      const int64_t chunks = (rows + chunk - 1) / chunk, even = (rows + chunks - 1) / chunks;
+      p.chunk = (even + kSumRows - 1) / kSumRows * kSumRows;
+    }
+  }
+  p.split = split_rows(p.chunk, N, outer, K, num_sms);
+  p.direct = p.chunk >= rows && p.split.parts == 1 && K % 8 == 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t at = p.bytes;
+    p.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  p.dz = take(p.dz_pitch * (p.chunk < rows ? p.chunk : rows) * 2);
+  p.parts = take(p.direct ? 0 : p.split.parts * outer * N * pad4(K) * int64_t(sizeof(float)));
+  p.sums = take((p.chunk + kSumRows - 1) / kSumRows * outer * pad8(N) * int64_t(sizeof(float)));
+  return p;
+}
+
+}  // namespace
+}  // namespace b200ta
+
+extern "C" {
+
+int b200ta_dense_few_rows(void) { return b200ta::kFewRows; }
+
+int b200ta_dense(const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* residual, int64_t rs, void* y,
+                 int64_t ys, void* saved, int64_t ss, int dtype, int activation, int gated, int64_t rows, int K, int N, void* stream) {
+  using namespace b200ta;
+  int rc = check_layer("dense", dtype, activation, rows, K, N);
+  if (rc != B200TA_OK) return rc;
+  B200TA_REQUIRE(x && w && y, "dense: NULL pointer");
+  B200TA_REQUIRE(!gated || residual == nullptr, "dense: a gated layer has no residual");
+  B200TA_REQUIRE(!gated || saved == nullptr || ss % 16 == 0, "dense: the pitch of a gated layer's saved values must be a multiple of 16");
+  if (rows <= kFewRows) {
+    DeviceState* st = nullptr;
+    rc = get_device_state(&st);
+    if (rc != B200TA_OK) return rc;
+    const FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation, gated, dtype == B200TA_DTYPE_F16};
+    const bool vec = K % 8 == 0 && rows_aligned(x, xs) && rows_aligned(w, ws);
+    return launch_kernel(st, kKernelDenseHelpers, p.f16 ? pick_few<__half>(int(rows), vec, gated) : pick_few<__nv_bfloat16>(int(rows), vec, gated),
+                         dim3(unsigned((N + 3) / 4)), 128, 0, stream, p);
+  }
+  B200TA_REQUIRE(rows_aligned(x, xs) && rows_aligned(w, ws) && rows_aligned(y, ys) && (!residual || rows_aligned(residual, rs)) &&
+                     (!saved || rows_aligned(saved, ss)),
+                 "dense: tensors must be 16-byte aligned with row strides that are multiples of 8 elements");
+  Matmul m;
+  m.form = gated ? kGated : kDense;
+  m.f16 = dtype == B200TA_DTYPE_F16;
+  m.a = {x, rows, K, xs};
+  m.b = {w, N, K, ws, gated ? 2 : 1, int64_t(N) * ws};
+  m.out = {y, rows, N, ys};
+  if (residual) m.aux = {residual, rows, N, rs};
+  if (saved) m.saved = {saved, rows, N, ss, gated ? 2 : 1, ss / 2};
+  m.bias = bias, m.activation = activation, m.what = gated ? "gated dense" : "dense";
+  return run_matmul(m, stream);
+}
+
+int b200ta_dense_keeps(int activation, int gated, int K) {
+  // Kept values are written and read at 2 bytes each (and dz formed from them in a pass of its own), computed ones cost 2 K
+  // operations each on the tensor cores.
+  return (gated || activation != b200ta::kActNone) && K >= 512;
+}
+
+size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int64_t rows, int K, int N) {
+  using namespace b200ta;
+  DeviceState* st = nullptr;
+  if (rows <= 0 || K <= 0 || N <= 0 || get_device_state(&st) != B200TA_OK) return 0;
+  return size_t(plan_backward(gated, activation != kActNone, rows, K, N, st->num_sms).bytes);
+}
+
+int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias,
+                          const void* saved, int64_t ss, void* dx, int64_t dxs, void* dw, void* dbias, void* workspace,
+                          size_t workspace_bytes, int dtype, int activation, int gated, int64_t rows, int K, int N, void* stream) {
+  using namespace b200ta;
+  int rc = check_layer("dense_backward", dtype, activation, rows, K, N);
+  if (rc != B200TA_OK) return rc;
+  B200TA_REQUIRE(dy && x && w, "dense_backward: NULL pointer");
+  B200TA_REQUIRE(rows_aligned(dy, dys) && rows_aligned(x, xs) && rows_aligned(w, ws) && (!dx || rows_aligned(dx, dxs)) &&
+                     (!saved || (rows_aligned(saved, ss) && (!gated || ss % 16 == 0))),
+                 "dense_backward: tensors must be 16-byte aligned with row strides that are multiples of 8 elements");
+  DeviceState* st = nullptr;
+  rc = get_device_state(&st);
+  if (rc != B200TA_OK) return rc;
+  const BackwardPlan plan = plan_backward(gated, activation != kActNone, rows, K, N, st->num_sms);
+  B200TA_REQUIRE(plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
+                                     workspace_bytes >= size_t(plan.bytes)),
+                 "dense_backward: the workspace must be 256-byte aligned and of %lld bytes", (long long)plan.bytes);
+  const bool f16 = dtype == B200TA_DTYPE_F16, own_dz = plan.dz_pitch != 0;
+  const int64_t outer = gated ? 2 : 1;
+  char* ws_base = static_cast<char*>(workspace);
+  float* parts = reinterpret_cast<float*>(ws_base + plan.parts);
+  float* sums = reinterpret_cast<float*>(ws_base + plan.sums);
+  const int64_t sum_pitch = own_dz ? plan.dz_pitch : pad8(N);  // columns of dz that are summed, padding included
+  const int sum_columns = int(own_dz ? plan.dz_pitch : N);
+  const bool direct = plan.direct && dw != nullptr && rows_aligned(dw, K);
+
+  for (int64_t r0 = 0; r0 < rows; r0 += plan.chunk) {
+    const int64_t n = rows - r0 < plan.chunk ? rows - r0 : plan.chunk;
+    const char* dy_c = static_cast<const char*>(dy) + r0 * dys * 2;
+    const char* x_c = static_cast<const char*>(x) + r0 * xs * 2;
+    const void* dz = dy_c;
+    int64_t zs = dys;
+    if (own_dz) {
+      void* dst = ws_base + plan.dz;
+      dz = dst, zs = plan.dz_pitch;
+      if (saved != nullptr) {
+        const SlopeParams p{dy_c, static_cast<const char*>(saved) + r0 * ss * 2, dst, dys, ss, zs, n, N};
+        const int64_t need = (n * ((N + 7) / 8) + 255) / 256, most = int64_t(st->num_sms) * 16;
+        void (*kernel)(SlopeParams);
+        if (f16) kernel = gated ? pick_slope<__half, true>(activation) : pick_slope<__half, false>(activation);
+        else kernel = gated ? pick_slope<__nv_bfloat16, true>(activation) : pick_slope<__nv_bfloat16, false>(activation);
+        rc = launch_kernel(st, kKernelDenseHelpers, kernel, dim3(unsigned(need < most ? need : most)), 256, 0, stream, p);
+      } else {
+        Matmul m;
+        m.form = gated ? kGatedGrad : kDenseGrad, m.f16 = f16;
+        m.a = {x_c, n, K, xs};
+        m.b = {w, N, K, ws, outer, int64_t(N) * ws};
+        m.out = {dst, n, N, zs, outer, zs / 2};
+        m.aux = {dy_c, n, N, dys};
+        m.bias = bias, m.activation = activation, m.what = "dense_backward dz";
+        rc = run_matmul(m, stream);
+      }
+      if (rc != B200TA_OK) return rc;
+    }
+    if (dx != nullptr) {
+      Matmul m;
+      m.form = kDense, m.b_mn = true, m.f16 = f16;
+      m.a = {dz, n, N, zs, outer, zs / 2};
+      m.b = {w, N, K, ws, outer, int64_t(N) * ws};
+      m.out = {static_cast<char*>(dx) + r0 * dxs * 2, n, K, dxs};
+      m.what = "dense_backward dx";
+      if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
+    }
+    if (dw != nullptr) {
+      Matmul m;
+      m.form = direct ? kDense : kPartial, m.a_mn = m.b_mn = true, m.f16 = f16;
+      m.a = {dz, n, N, zs, outer, zs / 2};
+      m.b = {x_c, n, K, xs};
+      if (direct) {
+        m.out = {dw, N, K, K, outer, int64_t(N) * K};
+      } else {
+        m.out = {parts, N, K, pad4(K), plan.split.parts * outer, N * pad4(K)};
+        m.kblocks_split = plan.split.kblocks;
+        m.accumulate = r0 > 0;  // each part is added to by one block at a time, the chunks in their order
+      }
+      m.what = "dense_backward dW";
+      if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
+    }
+    if (dbias != nullptr) {
+      const dim3 grid{unsigned((sum_columns + 255) / 256), unsigned((n + kSumRows - 1) / kSumRows)};
+      if (f16)
+        rc = launch_kernel(st, kKernelDenseHelpers, row_sum_kernel<__half>, grid, 256, 0, stream, static_cast<const __half*>(dz), zs, n,
+                           sum_columns, sum_pitch, kSumRows, int(r0 > 0), sums);
+      else
+        rc = launch_kernel(st, kKernelDenseHelpers, row_sum_kernel<__nv_bfloat16>, grid, 256, 0, stream,
+                           static_cast<const __nv_bfloat16*>(dz), zs, n, sum_columns, sum_pitch, kSumRows, int(r0 > 0), sums);
+      if (rc != B200TA_OK) return rc;
+    }
+  }
+  auto join = [&](const float* part, int64_t count, int64_t stride, int64_t pitch, int64_t n_rows, int columns, void* out) {
+    const int64_t need = (n_rows * columns + 255) / 256, most = int64_t(st->num_sms) * 16;
+    const dim3 grid{unsigned(need < most ? need : most)};
+    if (f16)
+      return launch_kernel(st, kKernelDenseHelpers, join_kernel<__half>, grid, 256, 0, stream, part, int(count), stride, pitch, n_rows,
+                           columns, static_cast<__half*>(out), int64_t(columns));
+    return launch_kernel(st, kKernelDenseHelpers, join_kernel<__nv_bfloat16>, grid, 256, 0, stream, part, int(count), stride, pitch,
+                         n_rows, columns, static_cast<__nv_bfloat16*>(out), int64_t(columns));
+  };
+  const int64_t chunk = plan.chunk < rows ? plan.chunk : rows;
+  if (dw != nullptr && !direct) {
+    rc = join(parts, plan.split.parts, outer * N * pad4(K), pad4(K), outer * N, K, dw);
+    if (rc != B200TA_OK) return rc;
+  }
+  if (dbias != nullptr) rc = join(sums, (chunk + kSumRows - 1) / kSumRows, sum_pitch, sum_pitch / outer, outer, N, dbias);
+  return rc;
+}
+
+int b200ta_copy_rows(const void* src, int64_t row_stride, int64_t column_stride, void* dst, int64_t pitch, int64_t rows, int columns,
+                     void* stream) {
+  using namespace b200ta;
+  B200TA_REQUIRE(src && dst, "copy_rows: NULL pointer");
+  B200TA_REQUIRE(rows > 0 && columns > 0, "copy_rows: rows=%lld, columns=%d", (long long)rows, columns);
+  DeviceState* st = nullptr;
+  const int rc = get_device_state(&st);
+  if (rc != B200TA_OK) return rc;
+  const int64_t tiles = (rows + 31) / 32 * ((columns + 31) / 32), most = int64_t(st->num_sms) * 8;
+  return launch_kernel(st, kKernelDenseHelpers, copy_rows_kernel, dim3(unsigned(tiles < most ? tiles : most)), 256, 0, stream,
+                       static_cast<const uint16_t*>(src), row_stride, column_stride, static_cast<uint16_t*>(dst), pitch, rows, columns);
+}
+
+}  // extern "C"

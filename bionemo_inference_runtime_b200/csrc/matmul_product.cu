@@ -1,0 +1,12 @@
+// The two products behind dz: dx = dz W (W with its rows along k) and dW = dz^T x (both with their rows along k), the
+// latter at once or in parts of the rows.
+#include "matmul.cuh"
+
+namespace b200ta {
+int launch_matmul_product(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, int grid, void* stream) {
+  if (m.form == kDense && !m.a_mn) return matmul::launch<kDense, false, true>(st, 4, m, maps, p, grid, stream);
+  if (m.form == kDense) return matmul::launch<kDense, true, true>(st, 5, m, maps, p, grid, stream);
+  if (m.form == kPartial) return matmul::launch<kPartial, true, true>(st, 6, m, maps, p, grid, stream);
+  return fail(B200TA_ERR_UNSUPPORTED, "%s: not a product of gradients", m.what);
+}
+}  // namespace b200ta

@@ -19,6 +19,7 @@
 #include <string>
 
 #include "../../include/b200ta.h"
+#include "torch_host.h"
 
 namespace py = pybind11;
 
@@ -45,9 +46,13 @@ void bind(const std::string& path, py::object error) {
   B200TA_ENTRIES(B200TA_LOAD)
 #undef B200TA_LOAD
   error_type = std::move(error);
+  b200ta_host::bind_training(handle);
 }
 
-// Raises what _lib.call raises for a non-zero status.
+}  // namespace
+
+namespace b200ta_host {
+
 void check(int code, const char* fn) {
   if (code == B200TA_OK) return;
   const std::string reason = lib.last_error();
@@ -56,13 +61,20 @@ void check(int code, const char* fn) {
   throw py::error_already_set();
 }
 
-void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
-
 std::string shape_of(const at::Tensor& t) {
   std::string s = "(";
   for (int64_t d : t.sizes()) s += std::to_string(d) + ", ";
   return s + ")";
 }
+
+}  // namespace b200ta_host
+
+namespace {
+
+using b200ta_host::check;
+using b200ta_host::shape_of;
+
+void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
 void require_bf16(const char* name, const at::Tensor& t) {
   if (!t.is_cuda()) throw py::value_error(std::string(name) + " must be a CUDA tensor (this package has no CPU path)");
@@ -710,6 +722,7 @@ bool more_than_its_class(PyObject* module) {
 
 PYBIND11_MODULE(_host, m) {
   m.doc() = "Native host path of the layers (see csrc/torch_host.cpp).";
+  b200ta_host::define_training(m);
   m.def("bind", &bind);
   m.def("node", &node);
   m.def("node_masked", &node_masked);

@@ -12,7 +12,7 @@ import math
 
 import torch
 
-from . import _lib
+from . import _host, _lib
 
 C = 128
 HEADS = 4
@@ -488,3 +488,72 @@ def linear(a: torch.Tensor, w: torch.Tensor, sc: torch.Tensor, mode: int, *, B: 
     _lib.call("b200ta_linear", a.data_ptr(), *a_strides, w.data_ptr(), sc.data_ptr(), _ptr(stats), _ptr(residual),
               0 if residual is None else shape[-1], out.data_ptr(), os_row, plane_stride, mode, B, rows, K, N, _stream())
     return out
+
+
+# ------------------------------------------------------------------------------------------ trainable layers
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "sigmoid": 5}
+
+
+def _activation(name: str) -> int:
+    code = ACTIVATIONS.get(name)
+    if code is None:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {name!r}")
+    return code
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5, *,
+               want_stats: bool = False, out: torch.Tensor | None = None):
+    """Layer norm over the last axis (1 to 16384 wide) of a bf16, fp16 or fp32 tensor of any leading shape and strides.
+
+    ``weight`` and ``bias`` are in the dtype of ``x`` or fp32.  With ``want_stats`` returns ``(y, stats)``, ``stats``
+    being the fp32 ``[rows, 2]`` pairs ``{rstd, -mean * rstd}`` that :func:`layer_norm_backward` takes.
+    """
+    y, stats = _host.layer_norm(x, weight, bias, float(eps), want_stats, out)
+    return (y, stats) if want_stats else y
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weight: torch.Tensor | None = None, *,
+                        want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
+    """``(dx, dweight, dbias)`` of :func:`layer_norm`; the parameters' gradients (sums over all rows, in fp32 and in a fixed
+    order) are in the dtype of ``weight``.  What is not wanted is not computed, and None."""
+    return _host.layer_norm_backward(dy, x, stats, weight, want_dx, want_dweight, want_dbias)
+
+
+def dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str = "none",
+          residual: torch.Tensor | None = None, want_saved: bool = False, out: torch.Tensor | None = None):
+    """``activation(x @ weight.T + bias) + residual`` in one kernel, for bf16 or fp16 ``x [..., K]`` and ``weight [N, K]`` of
+    any sizes and strides; sums in fp32, one rounding at the end.
+
+    With ``want_saved`` returns ``(y, saved)`` for :func:`dense_backward`: the values before the activation where a training
+    step is faster with them than by computing them again, otherwise None.
+    """
+    y, saved = _host.dense(x, weight, bias, residual, _activation(activation), False, want_saved, out)
+    return (y, saved) if want_saved else y
+
+
+def dense_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                   activation: str = "none", saved: torch.Tensor | None = None, want_dx: bool = True,
+                   want_dweight: bool = True, want_dbias: bool | None = None):
+    """``(dx, dweight, dbias)`` of :func:`dense` (the gradient of its residual is ``dy``).  ``dbias`` is computed where the
+    layer has a bias unless ``want_dbias`` says otherwise.  Without ``saved`` the values before the activation are computed
+    again.  The gradient before the activation is rounded to the dtype of ``x`` between the kernels."""
+    return _host.dense_backward(dy, x, weight, bias, saved, _activation(activation), False, want_dx, want_dweight,
+                                           bias is not None if want_dbias is None else want_dbias)
+
+
+def gated_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str = "silu",
+                want_saved: bool = False, out: torch.Tensor | None = None):
+    """``value * activation(gate)`` with ``[value | gate] = x @ weight.T + bias`` in one kernel: ``weight [2 * hidden, K]``
+    holds the value rows, then the gate rows (the order of the transitions' ``fused_fc2_fc1``).  Types, sizes and
+    ``want_saved`` as for :func:`dense`."""
+    y, saved = _host.dense(x, weight, bias, None, _activation(activation), True, want_saved, out)
+    return (y, saved) if want_saved else y
+
+
+def gated_dense_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                         activation: str = "silu", saved: torch.Tensor | None = None, want_dx: bool = True,
+                         want_dweight: bool = True, want_dbias: bool | None = None):
+    """``(dx, dweight, dbias)`` of :func:`gated_dense`; see :func:`dense_backward`."""
+    return _host.dense_backward(dy, x, weight, bias, saved, _activation(activation), True, want_dx, want_dweight,
+                                           bias is not None if want_dbias is None else want_dbias)

@@ -43,6 +43,7 @@ extern "C" {
 
 #define B200TA_DTYPE_BF16 0
 #define B200TA_DTYPE_F32 1
+#define B200TA_DTYPE_F16 2
 
 #define B200TA_EMPTY_ROW_ZEROS 0   /* rows with no valid key produce 0 (fused reference kernels) */
 #define B200TA_EMPTY_ROW_UNIFORM 1 /* rows with no valid key average V over all keys (eager reference) */
@@ -404,6 +405,60 @@ int b200ta_mask_lengths(const float* mask, int64_t s_b, int64_t s_r, int64_t s_s
                         int B, int R, int S, void* stream);
 int b200ta_mask_bits(const float* mask, int64_t s_b, int64_t s_r, int64_t s_s, int additive, int32_t* lengths,
                      uint32_t* bits, int B, int R, int S, void* stream);
+
+/* ---- trainable dense layers ---------------------------------------------------
+ *
+ * Layer norm, dense and gated dense layers with their gradients: what a transition is trained with (the modules of the
+ * reference's bionemo_ir/_torch/layers/transition.py:187-336 are forward only).  Weights are plain row-major matrices, read
+ * as they are; rows are addressed by strides in elements.  `dtype` is that of activations and weights.
+ */
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over rows of 1 to 16384 elements in bf16, fp16 or fp32.  `weight` and
+ * `bias` (either may be NULL) are in `dtype` or fp32 (`param_dtype`).  `stats` (may be NULL): [rows] pairs of floats
+ * {rstd, -mean * rstd} for the backward pass. */
+int b200ta_layer_norm(const void* x, int64_t x_row_stride, const void* weight, const void* bias, int param_dtype, void* y,
+                      int64_t y_row_stride, void* stats, int dtype, int64_t rows, int width, float eps, void* stream);
+
+/* Gradients of the same: dx (may be NULL), dweight and dbias (each may be NULL; in `param_dtype`).  The workspace is needed
+ * for the latter two. */
+size_t b200ta_layer_norm_workspace_bytes(int64_t rows, int width);
+int b200ta_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void* x, int64_t x_row_stride, const void* stats,
+                               const void* weight, int param_dtype, void* dx, int64_t dx_row_stride, void* dweight, void* dbias,
+                               void* workspace, size_t workspace_bytes, int dtype, int64_t rows, int width, void* stream);
+
+#define B200TA_ACT_NONE 0
+#define B200TA_ACT_RELU 1
+#define B200TA_ACT_SILU 2
+#define B200TA_ACT_GELU 3
+#define B200TA_ACT_GELU_TANH 4
+#define B200TA_ACT_SIGMOID 5
+
+/* y[rows, N] = act(x w^T + bias) + residual, x [rows, K], w [N, K]; or with `gated`, w [2 N, K] (value rows, then gate rows),
+ * y = value * act(gate), [value | gate] = x w^T + bias.  bf16 or fp16.  bias and residual (not for a gated layer) may be NULL.
+ * `saved` (may be NULL) receives x w^T + bias for the backward pass, [rows, N] or [rows, 2, saved_row_stride / 2].
+ * Up to b200ta_dense_few_rows() rows, any strides and alignment; otherwise base addresses are 16-byte aligned and row strides
+ * multiples of 8 elements (sizes are free). */
+int b200ta_dense_few_rows(void);
+int b200ta_dense(const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride, const void* bias, const void* residual,
+                 int64_t residual_row_stride, void* y, int64_t y_row_stride, void* saved, int64_t saved_row_stride, int dtype,
+                 int activation, int gated, int64_t rows, int K, int N, void* stream);
+
+/* Whether a training step is faster with `saved` than with the pre-activations computed again. */
+int b200ta_dense_keeps(int activation, int gated, int K);
+
+/* Gradients of the same: dx [rows, K], dw [N or 2 N, K] and dbias [N or 2 N], both dense; each may be NULL.  The
+ * pre-activations are taken from `saved`, or computed again from x, w and bias if it is NULL.  Alignment as above, dw and
+ * dbias free; the workspace is 256-byte aligned. */
+size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int64_t rows, int K, int N);
+int b200ta_dense_backward(const void* dy, int64_t dy_row_stride, const void* x, int64_t x_row_stride, const void* w,
+                          int64_t w_row_stride, const void* bias, const void* saved, int64_t saved_row_stride, void* dx,
+                          int64_t dx_row_stride, void* dw, void* dbias, void* workspace, size_t workspace_bytes, int dtype,
+                          int activation, int gated, int64_t rows, int K, int N, void* stream);
+
+/* dst[r, c] = src[r * row_stride + c * column_stride] for 16-bit elements, dst with rows `dst_row_stride` apart: aligned
+ * copies of what the entry points above cannot take as it lies, and the way back. */
+int b200ta_copy_rows(const void* src, int64_t row_stride, int64_t column_stride, void* dst, int64_t dst_row_stride, int64_t rows,
+                     int columns, void* stream);
 
 #ifdef __cplusplus
 }
