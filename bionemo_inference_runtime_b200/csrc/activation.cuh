@@ -1,10 +1,11 @@
 // Activations of the dense layers and their slopes, for pairs of values in 32 bits.
 //
 // Functions of the logistic kind cost two special-function operations a value (one exponential, one reciprocal), and that
-// unit does 16 a clock and SM: with one reciprocal for a pair, 1 / (p q) times q and p, they cost one and a half.
-// The exponent is held below 62, so that the product of two terms stays finite; past it the result is below 2^-62 and
-// taken as zero, which also keeps z * sigmoid(z) zero where z is large.  Results agree with the formulas to a few units of
-// the last place of 32 bits.
+// unit does 16 a clock and SM: with one reciprocal for a pair, 1 / (p q) times q and p, they cost one and a half.  The
+// exponent is held below 62, so that the product of two terms stays finite, and what multiplies a sigmoid that small is held
+// above -44: the products are below 2^-56 where the formulas give zero.  NaN stays in its own value (the exponent's bound
+// drops it, the other factor keeps it).  Sums and products are made in packed pairs, which halves their issue slots.
+// Results agree with the formulas to a few units of the last place of 32 bits.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -23,17 +24,33 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// sigmoid(z) of two values.  A NaN gives some number between 0 and 1; what is made of it here is multiplied by z or passed
-// through keep_nan().
-__device__ __forceinline__ void sigmoid2(float z0, float z1, float& s0, float& s1) {
-  constexpr float kLog2e = 1.4426950408889634f, kMost = 62.f;
-  const float t0 = -kLog2e * z0, t1 = -kLog2e * z1;
-  const float p = 1.f + ex2_approx(fminf(t0, kMost)), q = 1.f + ex2_approx(fminf(t1, kMost));
-  const float r = rcp_approx(p * q);
-  s0 = t0 >= kMost ? 0.f : r * q;
-  s1 = t1 >= kMost ? 0.f : r * p;
+__device__ __forceinline__ float max_nan(float a, float b) {  // the larger one, NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
 }
 __device__ __forceinline__ float keep_nan(float z, float value) { return z == z ? value : z; }
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2(float a, float b) : v(pack_f32x2(a, b)) {}
+  __device__ __forceinline__ explicit F2(float a) : v(pack_f32x2(a, a)) {}
+  __device__ __forceinline__ explicit F2(uint64_t x) : v(x) {}
+  __device__ __forceinline__ void to(float& a, float& b) const { unpack_f32x2(v, a, b); }
+};
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) { return F2(mul_f32x2(a.v, b.v)); }
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) { return F2(add_f32x2(a.v, b.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { return F2(fma_f32x2(a.v, b.v, c.v)); }
+
+// sigmoid(z) of two values; a NaN gives a number between 0 and 1.
+__device__ __forceinline__ F2 sigmoid2(F2 z) {
+  constexpr float kLog2e = 1.4426950408889634f, kMost = 62.f;
+  float t0, t1, p, q;
+  (z * F2(-kLog2e)).to(t0, t1);
+  (F2(ex2_approx(fminf(t0, kMost)), ex2_approx(fminf(t1, kMost))) + F2(1.f)).to(p, q);
+  const float r = rcp_approx(p * q);
+  return F2(r * q, r * p);
+}
+__device__ __forceinline__ F2 held(float z0, float z1) { return F2(max_nan(z0, -44.f), max_nan(z1, -44.f)); }
 
 // a = act(z) and, with kSlope, s = act'(z), for two values.
 template <int kAct, bool kSlope>
@@ -42,17 +59,17 @@ __device__ __forceinline__ void activate2(float z0, float z1, float& a0, float& 
     a0 = z0, a1 = z1;
     if (kSlope) s0 = 1.f, s1 = 1.f;
   } else if constexpr (kAct == kActRelu) {
-    a0 = z0 < 0.f ? 0.f : z0, a1 = z1 < 0.f ? 0.f : z1;  // a NaN stays
+    a0 = max_nan(z0, 0.f), a1 = max_nan(z1, 0.f);
     if (kSlope) s0 = z0 > 0.f ? 1.f : 0.f, s1 = z1 > 0.f ? 1.f : 0.f;
   } else if constexpr (kAct == kActSigmoid) {
-    sigmoid2(z0, z1, a0, a1);
+    const F2 p = sigmoid2(F2(z0, z1));
+    p.to(a0, a1);
     a0 = keep_nan(z0, a0), a1 = keep_nan(z1, a1);
-    if (kSlope) s0 = a0 * (1.f - a0), s1 = a1 * (1.f - a1);
+    if (kSlope) s0 = fmaf(-a0, a0, a0), s1 = fmaf(-a1, a1, a1);
   } else if constexpr (kAct == kActSilu) {
-    float p0, p1;
-    sigmoid2(z0, z1, p0, p1);
-    a0 = z0 * p0, a1 = z1 * p1;
-    if (kSlope) s0 = fmaf(a0, 1.f - p0, p0), s1 = fmaf(a1, 1.f - p1, p1);
+    const F2 p = sigmoid2(F2(z0, z1)), a = held(z0, z1) * p;
+    a.to(a0, a1);
+    if (kSlope) fma2(a, fma2(p, F2(-1.f), F2(1.f)), p).to(s0, s1);
   } else if constexpr (kAct == kActGelu) {
     constexpr float kRsqrt2 = 0.70710678118654752f, kDensity = 0.39894228040143268f, kHalfLog2e = 0.72134752044448170f;
     const float p0 = fmaf(0.5f, erff(z0 * kRsqrt2), 0.5f), p1 = fmaf(0.5f, erff(z1 * kRsqrt2), 0.5f);
@@ -66,14 +83,13 @@ __device__ __forceinline__ void activate2(float z0, float z1, float& a0, float& 
   } else {
     // 0.5 (1 + tanh u) = sigmoid(2 u), u = c (z + k z^3)
     constexpr float kTwoC = 1.5957691216057308f, kK = 0.044715f;
-    float p0, p1;
-    sigmoid2(z0 * fmaf(kTwoC * kK * z0, z0, kTwoC), z1 * fmaf(kTwoC * kK * z1, z1, kTwoC), p0, p1);
-    a0 = z0 * p0, a1 = z1 * p1;
+    const F2 z(z0, z1), p = sigmoid2(z * fma2(z * F2(kTwoC * kK), z, F2(kTwoC)));
+    (held(z0, z1) * p).to(a0, a1);
     if (kSlope) {
       // beyond 10 the slope is 0 or 1: p (1 - p) is zero there, and its factor is kept finite
-      const float c0 = fminf(fmaxf(z0, -10.f), 10.f), c1 = fminf(fmaxf(z1, -10.f), 10.f);
-      s0 = keep_nan(z0, fmaf(c0 * fmaf(3.f * kTwoC * kK * c0, c0, kTwoC), p0 * (1.f - p0), p0));
-      s1 = keep_nan(z1, fmaf(c1 * fmaf(3.f * kTwoC * kK * c1, c1, kTwoC), p1 * (1.f - p1), p1));
+      const F2 c(fminf(fmaxf(z0, -10.f), 10.f), fminf(fmaxf(z1, -10.f), 10.f));
+      fma2(c * fma2(c * F2(3.f * kTwoC * kK), c, F2(kTwoC)), fma2(p * F2(-1.f), p, p), p).to(s0, s1);
+      s0 = keep_nan(z0, s0), s1 = keep_nan(z1, s1);
     }
   }
 }

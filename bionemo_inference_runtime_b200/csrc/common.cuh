@@ -57,26 +57,34 @@ int get_device_state(DeviceState** out);
 // Launches a kernel that begins with pdl_wait(): the stream may start its blocks while the last blocks of the kernel
 // before it still run (programmatic dependent launch), so that barrier and tensor-memory set-up and the launch latency
 // itself hide behind them.  A block's set-up takes 2-3 us of the 5-12 us a kernel needs at small token counts.
+// launch_clusters: in clusters of `cluster` blocks (1: none).
 template <typename... P, typename... A>
-int launch_kernel(DeviceState* st, KernelId id, void (*kernel)(P...), dim3 grid, int threads, int smem_bytes, void* stream,
-                  A&&... args) {
+int launch_clusters(DeviceState* st, KernelId id, void (*kernel)(P...), dim3 grid, unsigned cluster, int threads, int smem_bytes,
+                    void* stream, A&&... args) {
   const uint64_t bit = 1ull << id;
   if (smem_bytes > 0 && !(st->configured.load(std::memory_order_relaxed) & bit)) {
     B200TA_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
     st->configured.fetch_or(bit, std::memory_order_relaxed);
   }
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster, attrs[1].val.clusterDim.y = 1, attrs[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = dim3(unsigned(threads));
   config.dynamicSmemBytes = size_t(smem_bytes);
   config.stream = static_cast<cudaStream_t>(stream);
-  config.attrs = &attr;
-  config.numAttrs = 1;
+  config.attrs = attrs;
+  config.numAttrs = cluster > 1 ? 2 : 1;
   B200TA_CHECK_CUDA(cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...));
   return B200TA_OK;
+}
+template <typename... P, typename... A>
+int launch_kernel(DeviceState* st, KernelId id, void (*kernel)(P...), dim3 grid, int threads, int smem_bytes, void* stream,
+                  A&&... args) {
+  return launch_clusters(st, id, kernel, grid, 1, threads, smem_bytes, stream, static_cast<A&&>(args)...);
 }
 #endif
 

@@ -1,5 +1,7 @@
 // The trainable dense layers around their products: argument checks, tensor maps and tiles of the products, and the small
 // kernels beside them (few rows, dz from stored pre-activations, sums over rows, joining of parts, aligned copies).
+#include <algorithm>
+
 #include "matmul.cuh"
 
 namespace b200ta {
@@ -13,21 +15,37 @@ int map_of(CUtensorMap* map, const Plane& t, int bytes, uint32_t columns, uint32
   return encode_tensor_map(map, t.base, bytes, 3, dims, strides, box, swz, what);
 }
 
-// Columns of a tile's accumulator.  A tile costs the larger of its MMAs (a [128 x n x 64] block takes 4 * max(40, n * 0.54)
-// clocks), its operands' way from L2 (46 bytes a clock and SM) and its finishing (some 7 clocks a column), and all blocks
-// take as many tiles as the busiest: wide tiles where there are enough of them, narrow ones to give every SM work.  Each of
-// the finishing warps' two halves takes whole groups of 32 result columns, which sets the least width.
-int choose_tile_n(int64_t tiles_m, int64_t columns, int kblocks, int least_n, int num_sms) {
-  int best = 256;
+// How the blocks share a product.  The costs are in clocks: a block of 64 along k costs its MMAs (4 * max(40, n * 0.54)) or its
+// operands' way from L2 (46 bytes a clock and SM), a tile of 256 columns with its two stages waits for its loads besides, and
+// a tile costs its finishing if that is more; all blocks take as many tiles as the busiest.
+struct Tiling {
+  int tile_n, pair, resident;
+};
+Tiling choose_tiling(const Matmul& m, int64_t rows, int64_t m_outer, int64_t columns, int kblocks, int splits, int num_sms) {
+  const bool two = m.form == kGated || m.form == kGatedGrad;
+  const int64_t accumulated = two ? columns * 2 : columns;
+  const double finish = m.form == kGatedGrad ? 12 : two ? 8 : 6.5;  // clocks for an accumulator column of 128 rows
+  Tiling best{128, 0, 0};
   double least = 1e300;
-  for (int n = 256; n >= least_n; n /= 2) {
-    const double tiles = double(tiles_m) * double((columns + n - 1) / n);
-    const double mma = 4.0 * (n * 0.54 > 40 ? n * 0.54 : 40), load = (16384.0 + n * 128.0) / 46;
-    double tile = kblocks * (mma > load ? mma : load);
-    if (tile < 7.0 * n) tile = 7.0 * n;
-    const double waves = double(int64_t((tiles + num_sms - 1) / num_sms));
-    const double cost = waves * tile;
-    if (cost < least * 0.98) least = cost, best = n;
+  auto consider = [&](Tiling t, double waves, double main, double columns_of_tile) {
+    const double cost = waves * std::max(main, finish * columns_of_tile) + std::min(main, finish * columns_of_tile) + 1500;
+    if (cost < least * 0.98) least = cost, best = t;
+  };
+  auto waves_of = [](int64_t items, int64_t blocks) { return double((items + blocks - 1) / blocks); };
+  if (rows > matmul::kBM && accumulated > 128) {
+    const int64_t tiles = (rows + 255) / 256 * m_outer * splits * ((accumulated + 255) / 256);
+    consider({256, 1, 0}, waves_of(tiles, num_sms / 2), kblocks * 712.0, 256);
+  }
+  for (int n = 256; n >= 64; n /= 2) {
+    if (n > 64 && n / 2 >= accumulated) continue;
+    const int64_t tiles_m = (rows + 127) / 128 * m_outer, tiles_n = (accumulated + n - 1) / n;
+    const double mma = 4.0 * std::max(40.0, n * 0.54);
+    if (!m.a_mn && splits == 1 && kblocks * n * matmul::kBK * 2 <= matmul::kResidentBytes && tiles_n <= num_sms) {
+      const int64_t lanes = std::min(tiles_m, num_sms / tiles_n);
+      consider({n, 0, int(lanes)}, waves_of(tiles_m, lanes), kblocks * std::max(mma, 356.0), n);
+    } else {
+      consider({n, 0, 0}, waves_of(tiles_m * tiles_n * splits, num_sms), kblocks * std::max(mma, (n == 256 ? 1.2 : 1.0) * (16384 + n * 128) / 46), n);
+    }
   }
   return best;
 }
@@ -44,22 +62,26 @@ int run_matmul(const Matmul& m, void* stream) {
   const int64_t k = m.a_mn ? m.a.rows : m.a.columns, m_outer = m.a_mn ? m.a.outer : 1, k_outer = m.a_mn ? 1 : m.a.outer;
   constexpr int64_t kMost = int64_t(1) << 31;
   B200TA_REQUIRE(rows < kMost - 512 && columns < kMost - 512 && k < kMost - 512, "%s: a size is past 2^31", m.what);
-  p.tiles_m_inner = int((rows + matmul::kBM - 1) / matmul::kBM);
-  p.tiles_m = int(p.tiles_m_inner * m_outer);
   p.kblocks_inner = int((k + matmul::kBK - 1) / matmul::kBK);
   p.kblocks = int(p.kblocks_inner * k_outer);
   p.kblocks_split = m.kblocks_split > 0 && m.kblocks_split < p.kblocks ? m.kblocks_split : p.kblocks;
   p.splits = (p.kblocks + p.kblocks_split - 1) / p.kblocks_split;
   p.rows_inner = int(rows), p.columns = int(columns);
-  p.tile_n = choose_tile_n(int64_t(p.tiles_m) * p.splits, two ? columns * 2 : columns, p.kblocks_split, two ? 128 : 64, st->num_sms);
+  const Tiling tiling = choose_tiling(m, rows, m_outer, columns, p.kblocks_split, p.splits, st->num_sms);
+  p.tile_n = tiling.tile_n, p.pair = tiling.pair, p.resident = tiling.resident;
+  const int tile_m = p.pair ? 2 * matmul::kBM : matmul::kBM;
+  p.tiles_m_inner = int((rows + tile_m - 1) / tile_m);
+  p.tiles_m = int(p.tiles_m_inner * m_outer);
   const int units = two ? p.tile_n / 2 : p.tile_n;
   p.tiles_n = int((columns + units - 1) / units);
   const int64_t work = int64_t(p.tiles_m) * p.tiles_n * p.splits;
   B200TA_REQUIRE(work < kMost - 1024, "%s: too many tiles", m.what);
   p.work = int(work);
-  p.group_m = 16;
-  const int stage = matmul::kABytes + p.tile_n * matmul::kBK * 2;
-  p.stages = matmul::kRingBytes / stage < matmul::kMaxStages ? matmul::kRingBytes / stage : matmul::kMaxStages;
+  p.group_m = p.pair ? 8 : 16;
+  const int b_rows = p.pair ? p.tile_n / 2 : p.tile_n;
+  p.stages = p.resident ? (matmul::kRingBytes - matmul::kResidentBytes) / matmul::kABytes
+                        : matmul::kRingBytes / (matmul::kABytes + b_rows * matmul::kBK * 2);
+  if (p.stages > matmul::kMaxStages) p.stages = matmul::kMaxStages;
   p.bias = m.bias;
   p.activation = m.activation;
   p.has_aux = m.aux.base != nullptr, p.has_saved = m.saved.base != nullptr, p.accumulate = m.accumulate;
@@ -69,14 +91,15 @@ int run_matmul(const Matmul& m, void* stream) {
   rc = m.a_mn ? map_of(&maps.a, m.a, 2, 64, 64, 1, SWZ_128, m.what) : map_of(&maps.a, m.a, 2, 64, matmul::kBM, 1, SWZ_128, m.what);
   if (rc != B200TA_OK) return rc;
   rc = m.b_mn ? map_of(&maps.b, m.b, 2, 64, 64, 1, SWZ_128, m.what)
-              : map_of(&maps.b, m.b, 2, 64, uint32_t(units), two ? 2 : 1, SWZ_128, m.what);
+              : map_of(&maps.b, m.b, 2, 64, uint32_t(p.pair || !two ? b_rows : units), two && !p.pair ? 2 : 1, SWZ_128, m.what);
   if (rc != B200TA_OK) return rc;
   const bool f32 = m.form == kPartial;
-  rc = map_of(&maps.out, m.out, f32 ? 4 : 2, 32, 32, 1, f32 ? SWZ_128 : SWZ_64, m.what);
+  rc = map_of(&maps.out, m.out, f32 ? 4 : 2, f32 ? 16 : 32, 32, 1, SWZ_64, m.what);
   if (rc != B200TA_OK) return rc;
   if (p.has_aux && (rc = map_of(&maps.aux, m.aux, 2, 32, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
   if (p.has_saved && (rc = map_of(&maps.saved, m.saved, 2, 32, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
-  const int grid = p.work < st->num_sms ? p.work : st->num_sms;
+  const int blocks = p.resident ? p.resident * p.tiles_n : std::min(p.work, p.pair ? st->num_sms / 2 : st->num_sms);
+  const int grid = p.pair ? 2 * blocks : blocks;
   if (m.form == kDenseGrad || m.form == kGatedGrad) return launch_matmul_grad(st, m, maps, p, grid, stream);
   if (m.b_mn) return launch_matmul_product(st, m, maps, p, grid, stream);
   return launch_matmul_forward(st, m, maps, p, grid, stream);
@@ -395,7 +418,7 @@ Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns,
   }
   return best;
 }
-constexpr int kSumRows = 1024;  // rows of a partial sum of db
+constexpr int kSumRows = 256;  // rows of a partial sum of db
 
 // The backward pass: how many rows at a time, and where its intermediates lie in the workspace.
 struct BackwardPlan {
@@ -412,14 +435,11 @@ BackwardPlan plan_backward(bool gated, bool slope, int64_t rows, int K, int N, i
   p.chunk = rows;
   if (p.dz_pitch != 0) {
     // Narrow layers are bound by HBM: dz of a chunk is read back from L2 if it fits there, and the next chunk overwrites it.
-    // Wide layers are bound by the tensor cores: their chunks only keep the workspace small.
-    const int64_t most = (K <= 256 ? int64_t(48) : int64_t(1024)) << 20;
-    const int64_t fit = most / (p.dz_pitch * 2) / kSumRows * kSumRows;
-    const int64_t chunk = fit < kSumRows ? kSumRows : fit;
-    if (chunk < rows) {
-      const int64_t chunks = (rows + chunk - 1) / chunk, even = (rows + chunks - 1) / chunks;
-      p.chunk = (even + kSumRows - 1) / kSumRows * kSumRows;
-    }
+    // A chunk is a row tile for every SM, or several.  Wide layers are bound by the tensor cores: their chunks only keep the
+    // workspace small.
+    const int64_t wave = (int64_t(num_sms) * matmul::kBM + kSumRows - 1) / kSumRows * kSumRows;
+    const int64_t fit = (K <= 256 ? int64_t(48) << 20 : int64_t(1) << 30) / (p.dz_pitch * 2) / wave;
+    p.chunk = std::min(rows, std::max<int64_t>(fit, 1) * wave);
   }
   p.split = split_rows(p.chunk, N, outer, K, num_sms);
   p.direct = p.chunk >= rows && p.split.parts == 1 && K % 8 == 0;
@@ -542,7 +562,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
     }
     if (dx != nullptr) {
       Matmul m;
-      m.form = kDense, m.b_mn = true, m.f16 = f16;
+      m.form = kPlain, m.b_mn = true, m.f16 = f16;
       m.a = {dz, n, N, zs, outer, zs / 2};
       m.b = {w, N, K, ws, outer, int64_t(N) * ws};
       m.out = {static_cast<char*>(dx) + r0 * dxs * 2, n, K, dxs};
@@ -551,7 +571,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
     }
     if (dw != nullptr) {
       Matmul m;
-      m.form = direct ? kDense : kPartial, m.a_mn = m.b_mn = true, m.f16 = f16;
+      m.form = direct ? kPlain : kPartial, m.a_mn = m.b_mn = true, m.f16 = f16;
       m.a = {dz, n, N, zs, outer, zs / 2};
       m.b = {x_c, n, K, xs};
       if (direct) {

@@ -1,29 +1,35 @@
 // The tensor-core products of the trainable dense layers (sm_100a): D[m, n] = sum_k A[m, k] B[n, k], finished in one of
-// five forms, for bf16 or fp16 operands with accumulators in 32 bits.
+// six forms, for bf16 or fp16 operands with accumulators in 32 bits.
 //
 //   kDense      y = act(D + bias) + residual, and D + bias itself where the backward pass is to have it
 //   kGated      value and gate columns in one tile: y = (value + b) act(gate + b')
 //   kDenseGrad  dz = dy act'(D + bias)                                  D computed again from the layer's input
 //   kGatedGrad  dz = [dy act(gate) | dy value act'(gate)]
+//   kPlain      D                                                       products of gradients
 //   kPartial    D in 32 bits, over one of several parts of k            weight gradients, joined by another kernel
 //
 // An operand lies with k contiguous (K-major) or with its rows contiguous (MN-major): x and W as they are make the forward
 // product, dz and W that of dx, dz and x that of dW; nothing is transposed in memory.  Sizes are free (tiles past the edge
 // are zero-filled by the loads and clipped by the stores); base addresses and row pitches are multiples of 16 bytes.
 //
-// A persistent block walks [128 x tile_n] tiles.  Warp roles (320 threads): warps 0-7 finish tiles (TMEM lane = row, two
-// halves of the columns), warp 8 loads [128 x 64] and [tile_n x 64] operand blocks by TMA into a ring, warp 9 issues
-// tcgen05.mma into two accumulators of 256 columns, one filled while the other is finished.  The finishing warps fetch what
-// they read beside the accumulators (residual, dy) by TMA two groups of 32 columns ahead and store by TMA from a ring of
-// slabs: a lane's own accesses to 32 rows occupy the load-store unit for some 56 clocks.
+// A persistent block walks [128 x tile_n] tiles; with kPair two blocks of a cluster walk [256 x 256] tiles together, each
+// with its 128 rows of A and half of B (cta_group::2), which halves what a tile of B costs in shared memory and from L2.
+// Warp roles (576 threads): warps 0-15 finish tiles (TMEM lane = row; each takes every fourth group of 32 columns), warp 16
+// loads [128 x 64] and [tile_n x 64] operand blocks by TMA into a ring, warp 17 issues tcgen05.mma into two accumulators of
+// 256 columns, one filled while the other is finished.  Where all of a column tile of B fits in half of the ring (64 KiB: 128
+// wide layers), it is loaded once and only A passes through the ring.  The finishing warps fetch what they read beside the
+// accumulators (residual, dy) by TMA a group ahead and store by TMA: a lane's own accesses to 32 rows occupy the load-store
+// unit for some 56 clocks.
 #pragma once
+
+#include <type_traits>
 
 #include "activation.cuh"
 #include "common.cuh"
 
 namespace b200ta {
 
-enum MatmulForm { kDense, kGated, kDenseGrad, kGatedGrad, kPartial };
+enum MatmulForm { kDense, kGated, kDenseGrad, kGatedGrad, kPlain, kPartial };
 
 struct MatmulParams {
   int tiles_m, tiles_n, splits, work;  // work = tiles_m * tiles_n * splits items
@@ -35,6 +41,8 @@ struct MatmulParams {
   int columns;                         // valid result columns (kGated*: hidden units)
   int tile_n;                          // accumulator columns of a tile: 64, 128 or 256
   int stages;
+  int pair;                            // two blocks on [256 x 256] tiles (tiles_m counts those)
+  int resident;                        // blocks keep their column tile of B (and walk the row tiles in steps of resident)
   const void* bias;                    // [columns] (kGated*: value biases, then gate biases), or NULL
   int activation;
   int has_aux;                         // kDense: a residual
@@ -47,16 +55,18 @@ struct MatmulParams {
 
 namespace matmul {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 576, kFinishers = 16;
 constexpr int kBM = 128, kBK = 64;
 constexpr int kABytes = kBM * kBK * 2;
-constexpr int kRingBytes = 147456;     // operand stages
-constexpr int kMaxStages = 6;
-constexpr int kSmSlabs = kRingBytes;   // 8 warps x 8 KiB
-constexpr int kWarpSlabs = 8192;
-constexpr int kSmBars = kSmSlabs + 8 * kWarpSlabs;
+constexpr int kRingBytes = 131072;         // operand stages
+constexpr int kResidentBytes = 65536;      // of them for a resident B
+constexpr int kMaxStages = 7;
+constexpr int kSlab = 2048;                // 32 rows of 64 bytes
+constexpr int kSmSlabs = kRingBytes;       // three for each finishing warp
+constexpr int kSmBars = kSmSlabs + kFinishers * 3 * kSlab;
 enum Bar {
-  FULL = 0, EMPTY = kMaxStages, ACC_FULL = 2 * kMaxStages, ACC_EMPTY = ACC_FULL + 2, AUX = ACC_EMPTY + 2, NUM_BARS = AUX + 16
+  FULL = 0, EMPTY = kMaxStages, ACC_FULL = 2 * kMaxStages, ACC_EMPTY = ACC_FULL + 2, B_FULL = ACC_EMPTY + 2, AUX = B_FULL + 1,
+  NUM_BARS = AUX + kFinishers
 };
 constexpr int kSmTotal = kSmBars + NUM_BARS * 8 + 32;
 constexpr int kSmDynamic = kSmTotal + 1024;
@@ -65,71 +75,106 @@ static_assert(kSmDynamic <= 232448, "shared memory of a block");
 struct Item {
   int split, m_outer, m0, n0, kb0, kb1;
 };
-__device__ __forceinline__ Item decode(const MatmulParams& p, int t, int units) {
+// Item i of a block (of a cluster with kPair): rows from m0, result columns from n0, blocks kb0 to kb1 along k.
+template <bool kPair, bool kOuter>
+__device__ __forceinline__ Item item_of(const MatmulParams& p, int i, int units) {
+  constexpr int kRows = kPair ? 2 * kBM : kBM;
+  const int block = kPair ? blockIdx.x >> 1 : blockIdx.x, blocks = kPair ? gridDim.x >> 1 : gridDim.x;
   Item r;
+  r.m_outer = 0;
+  if (p.resident) {
+    r.split = 0, r.kb0 = 0, r.kb1 = p.kblocks;
+    const int m = block / p.tiles_n;
+    r.n0 = (block - m * p.tiles_n) * units;
+    r.m0 = (m + i * p.resident) * kRows;
+    return r;
+  }
+  int t = block + i * blocks;
   const int tiles = p.tiles_m * p.tiles_n;
-  r.split = t / tiles;
-  t -= r.split * tiles;
+  r.split = 0;
+  if (p.splits > 1) r.split = t / tiles, t -= r.split * tiles;
   // groups of row tiles, all columns of a group before the next: what the blocks of a wave read stays in L2
   const int per_group = p.group_m * p.tiles_n, g = t / per_group, first = g * p.group_m;
   const int rows = p.tiles_m - first < p.group_m ? p.tiles_m - first : p.group_m;
   t -= g * per_group;
-  const int nt = t / rows, mt = first + (t - nt * rows);
-  r.m_outer = mt / p.tiles_m_inner;
-  r.m0 = (mt - r.m_outer * p.tiles_m_inner) * kBM;
+  const int nt = t / rows;
+  int mt = first + (t - nt * rows);
+  if (kOuter) r.m_outer = mt / p.tiles_m_inner, mt -= r.m_outer * p.tiles_m_inner;
+  r.m0 = mt * kRows;
   r.n0 = nt * units;
   r.kb0 = r.split * p.kblocks_split;
   const int end = r.kb0 + p.kblocks_split;
   r.kb1 = end < p.kblocks ? end : p.kblocks;
   return r;
 }
+template <bool kPair>
+__device__ __forceinline__ int items_of(const MatmulParams& p) {
+  const int block = kPair ? blockIdx.x >> 1 : blockIdx.x, blocks = kPair ? gridDim.x >> 1 : gridDim.x;
+  if (p.resident) return (p.tiles_m - 1 - block / p.tiles_n) / p.resident + 1;
+  return (p.work - 1 - block) / blocks + 1;
+}
 
 __host__ __device__ constexpr uint32_t idesc(bool f16, int m, int n, bool a_mn, bool b_mn) {
   return make_idesc_bf16(m, n, a_mn, b_mn) & ~(f16 ? (1u << 7 | 1u << 10) : 0u);
 }
 
-// y / dz of 32 columns of one row.  v: accumulators (kGated*: of the values), g: of the gates, aux: residual or dy.
-// Results replace v (and g).
-template <MatmulForm kForm, int kAct>
-__device__ __forceinline__ void finish(float (&v)[32], float (&g)[32], const float (&aux)[32]) {
+// y / dz of kN of a group's 32 columns, from column kFirst, of one row, as 16-bit pairs.  v: accumulators (kGated*: of the values), g: of the gates, aux: residual
+// (with has_aux) or dy; kGatedGrad: y the gradients of the values, yg those of the gates.
+template <typename T, MatmulForm kForm, int kAct, int kFirst, int kN>
+__device__ __forceinline__ void finish(const float (&v)[kN], const float (&g)[kN], bool has_aux, const uint32_t (&aux)[16],
+                                       uint32_t (&y)[16], uint32_t (&yg)[16]) {
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) {
+  for (int i = 0; i < kN / 2; ++i) {
+    const int j = kFirst / 2 + i;
     float a0, a1, s0, s1;
+    const float v0 = v[2 * i], v1 = v[2 * i + 1], g0 = g[2 * i], g1 = g[2 * i + 1];
     if constexpr (kForm == kDense) {
-      activate2<kAct, false>(v[j], v[j + 1], a0, a1, s0, s1);
-      v[j] = a0 + aux[j], v[j + 1] = a1 + aux[j + 1];
+      activate2<kAct, false>(v0, v1, a0, a1, s0, s1);
+      if (has_aux) {
+        const float2 x = unpack2<T>(aux[j]);
+        (F2(a0, a1) + F2(x.x, x.y)).to(a0, a1);
+      }
+      y[j] = pack2<T>(a0, a1);
     } else if constexpr (kForm == kGated) {
-      activate2<kAct, false>(g[j], g[j + 1], a0, a1, s0, s1);
-      v[j] *= a0, v[j + 1] *= a1;
-    } else if constexpr (kForm == kDenseGrad) {
-      activate2<kAct, true>(v[j], v[j + 1], a0, a1, s0, s1);
-      v[j] = aux[j] * s0, v[j + 1] = aux[j + 1] * s1;
+      activate2<kAct, false>(g0, g1, a0, a1, s0, s1);
+      (F2(v0, v1) * F2(a0, a1)).to(a0, a1);
+      y[j] = pack2<T>(a0, a1);
     } else {
-      activate2<kAct, true>(g[j], g[j + 1], a0, a1, s0, s1);
-      g[j] = aux[j] * v[j] * s0, g[j + 1] = aux[j + 1] * v[j + 1] * s1;
-      v[j] = aux[j] * a0, v[j + 1] = aux[j + 1] * a1;
+      const float2 x = unpack2<T>(aux[j]);
+      const F2 d(x.x, x.y);
+      activate2<kAct, true>(kForm == kDenseGrad ? v0 : g0, kForm == kDenseGrad ? v1 : g1, a0, a1, s0, s1);
+      if constexpr (kForm == kDenseGrad) {
+        (d * F2(s0, s1)).to(s0, s1);
+        y[j] = pack2<T>(s0, s1);
+      } else {
+        (d * F2(a0, a1)).to(a0, a1);
+        (d * F2(v0, v1) * F2(s0, s1)).to(s0, s1);
+        y[j] = pack2<T>(a0, a1);
+        yg[j] = pack2<T>(s0, s1);
+      }
     }
   }
 }
-template <MatmulForm kForm>
-__device__ __forceinline__ void finish_any(int activation, float (&v)[32], float (&g)[32], const float (&aux)[32]) {
+template <typename T, MatmulForm kForm, int kFirst, int kN>
+__device__ __forceinline__ void finish_any(int activation, const float (&v)[kN], const float (&g)[kN], bool has_aux,
+                                           const uint32_t (&aux)[16], uint32_t (&y)[16], uint32_t (&yg)[16]) {
   switch (activation) {
-    case kActNone: return finish<kForm, kActNone>(v, g, aux);
-    case kActRelu: return finish<kForm, kActRelu>(v, g, aux);
-    case kActSilu: return finish<kForm, kActSilu>(v, g, aux);
-    case kActGelu: return finish<kForm, kActGelu>(v, g, aux);
-    case kActGeluTanh: return finish<kForm, kActGeluTanh>(v, g, aux);
-    default: return finish<kForm, kActSigmoid>(v, g, aux);
+    case kActNone: return finish<T, kForm, kActNone, kFirst, kN>(v, g, has_aux, aux, y, yg);
+    case kActRelu: return finish<T, kForm, kActRelu, kFirst, kN>(v, g, has_aux, aux, y, yg);
+    case kActSilu: return finish<T, kForm, kActSilu, kFirst, kN>(v, g, has_aux, aux, y, yg);
+    case kActGelu: return finish<T, kForm, kActGelu, kFirst, kN>(v, g, has_aux, aux, y, yg);
+    case kActGeluTanh: return finish<T, kForm, kActGeluTanh, kFirst, kN>(v, g, has_aux, aux, y, yg);
+    default: return finish<T, kForm, kActSigmoid, kFirst, kN>(v, g, has_aux, aux, y, yg);
   }
 }
 
-// Adds biases n .. n + 31 (those below `columns`) to v; every lane reads the same addresses.
-template <typename T>
-__device__ __forceinline__ void add_bias(float (&v)[32], const T* bias, int n, int columns) {
+// Adds biases n .. n + kN - 1 (those below `columns`) to v; every lane reads the same addresses.
+template <typename T, int kN>
+__device__ __forceinline__ void add_bias(float (&v)[kN], const T* bias, int n, int columns) {
   const T* b = bias + n;
-  if (n + 32 <= columns && (reinterpret_cast<uintptr_t>(b) & 15u) == 0) {
+  if (n + kN <= columns && (reinterpret_cast<uintptr_t>(b) & 15u) == 0) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < kN / 8; ++c) {
       const uint4 x = __ldg(reinterpret_cast<const uint4*>(b) + c);
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -140,9 +185,17 @@ __device__ __forceinline__ void add_bias(float (&v)[32], const T* bias, int n, i
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
+    for (int j = 0; j < kN; ++j)
       if (n + j < columns) v[j] += static_cast<float>(b[j]);
   }
+}
+template <int kN>
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[kN]) {
+  uint32_t r[kN];
+  if constexpr (kN == 32) tmem_ld32(addr, r);
+  else tmem_ld16(addr, r);
+#pragma unroll
+  for (int j = 0; j < kN; ++j) v[j] = __uint_as_float(r[j]);
 }
 
 __device__ __forceinline__ void tma_add_3d(const CUtensorMap* m, uint32_t src, int c0, int c1, int c2) {
@@ -151,15 +204,67 @@ __device__ __forceinline__ void tma_add_3d(const CUtensorMap* m, uint32_t src, i
                : "memory");
 }
 
-template <typename T, MatmulForm kForm, bool kAMn, bool kBMn>
+// ---- two blocks on one tile -------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of the first block's copy of a shared-memory variable.
+__device__ __forceinline__ uint32_t in_first_block(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t slot_smem, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_smem), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+// A load into this block's shared memory that is counted by a barrier of either block.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(m), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ss_pair_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, e;\nsetp.ne.b32 p, %4, 0;\nelect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives on the barrier at this address in both blocks once all MMAs issued so far have completed.
+__device__ __forceinline__ void umma_commit_pair_warp(uint32_t bar) {
+  asm volatile(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster_warp(uint32_t bar) {
+  asm volatile(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e mbarrier.arrive.shared::cluster.b64 _, [%0];\n}" ::"r"(bar)
+      : "memory");
+}
+
+template <typename T, MatmulForm kForm, bool kAMn, bool kBMn, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
               const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ CUtensorMap tm_aux,
               const __grid_constant__ CUtensorMap tm_saved, const MatmulParams p) {
   constexpr bool kTwo = kForm == kGated || kForm == kGatedGrad;  // value and gate columns in a tile
   constexpr bool kGrad = kForm == kDenseGrad || kForm == kGatedGrad;
-  constexpr int kRing = kForm == kGated ? 4 : 2;                 // output slabs of a warp
-  constexpr int kSlab = kForm == kPartial ? 4096 : 2048;
+  constexpr bool kAux = kGrad || kForm == kDense;                // a warp's first slab receives residual or dy
+  constexpr int kRing = kAux ? 2 : 3;                            // the others hold results
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -168,6 +273,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + kSmBars + NUM_BARS * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kSmBars + NUM_BARS * 8 + 8);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = kPair ? cluster_rank() : 0;
 
   if (threadIdx.x == 0) {
     abort_flag[0] = 0, abort_flag[1] = 0;
@@ -177,143 +283,177 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bars + (ACC_FULL + i) * 8, 1);
-      mbar_init(bars + (ACC_EMPTY + i) * 8, 8);
+      mbar_init(bars + (ACC_EMPTY + i) * 8, kPair ? 2 * kFinishers : kFinishers);
     }
-    for (int i = 0; i < 16; ++i) mbar_init(bars + (AUX + i) * 8, 1);
+    mbar_init(bars + B_FULL * 8, 1);
+    for (int i = 0; i < kFinishers; ++i) mbar_init(bars + (AUX + i) * 8, 1);
     fence_mbar_init();
   }
-  if (warp == 9) {
-    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+  if (warp == 17) {
+    if constexpr (kPair) tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    else tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
     pdl_trigger();
   }
   tc_fence_before();
-  __syncthreads();
+  if constexpr (kPair) cluster_sync();
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  const int items = (p.work - 1 - int(blockIdx.x)) / int(gridDim.x) + 1;
-  const int units = kTwo ? p.tile_n / 2 : p.tile_n;  // result columns of a tile
-  const int stage_bytes = kABytes + p.tile_n * kBK * 2;
+  const int items = items_of<kPair>(p);
+  const int units = kTwo ? p.tile_n / 2 : p.tile_n;           // result columns of a tile
+  const int b_rows = kPair ? p.tile_n / 2 : p.tile_n;         // rows of B that this block loads
+  const int b_bytes = b_rows * kBK * 2;
+  const int stage_bytes = p.resident ? kABytes : kABytes + b_bytes;
+  const uint32_t ring = base + (p.resident ? kResidentBytes : 0);
 
-  if (warp == 8) {
+  if (warp == 16) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
       tma_prefetch_desc(&tm_a);
       tma_prefetch_desc(&tm_b);
       pdl_wait();
+      auto load = [&](uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
+        if constexpr (kPair) tma_load_3d_pair(dst, m, bar, c0, c1, c2);
+        else tma_load_3d(dst, m, bar, c0, c1, c2);
+      };
+      auto load_b = [&](uint32_t sb, uint32_t bar, int n0, int k0, int ko) {
+        if constexpr (kBMn) {
+          for (int n = 0; n < b_rows; n += 64) load(sb + n * kBK * 2, &tm_b, bar, n0 + int(rank) * b_rows + n, k0, ko);
+        } else if constexpr (kTwo && kPair) {
+          load(sb, &tm_b, bar, k0, n0, int(rank));  // the first block has the values, the second the gates
+        } else {
+          load(sb, &tm_b, bar, k0, n0 + int(rank) * b_rows, 0);  // kTwo: a box of value rows and a box of gate rows in one
+        }
+      };
+      if (p.resident) {
+        const Item t = item_of<kPair, kAMn>(p, 0, units);
+        mbar_expect_tx(bars + B_FULL * 8, p.kblocks * b_bytes);
+        for (int kb = 0, ko = 0, ki = 0; kb < p.kblocks; ++kb) {
+          load_b(base + kb * b_bytes, bars + B_FULL * 8, t.n0, ki * kBK, ko);
+          if (++ki == p.kblocks_inner) ki = 0, ++ko;
+        }
+      }
       int stage = 0, issued = 0;
       uint32_t phase = 1;
       bool ok = true;
       for (int i = 0; ok && i < items; ++i) {
-        const Item t = decode(p, blockIdx.x + i * gridDim.x, units);
+        Item t = item_of<kPair, kAMn>(p, i, units);
+        t.m0 += int(rank) * kBM;
         int ko = t.kb0 / p.kblocks_inner, ki = t.kb0 - ko * p.kblocks_inner;
         for (int kb = t.kb0; kb < t.kb1; ++kb) {
           ok = mbar_wait(bars + (EMPTY + stage) * 8, phase, abort_flag);
           if (!ok) break;
-          const uint32_t full = bars + (FULL + stage) * 8;
-          const uint32_t sa = base + stage * stage_bytes, sb = sa + kABytes;
+          uint32_t full = bars + (FULL + stage) * 8;
+          // the first block's barrier counts the loads of both
+          if (kPair) {
+            if (rank == 0) mbar_expect_tx(full, 2 * stage_bytes);
+            full = in_first_block(full);
+          } else {
+            mbar_expect_tx(full, stage_bytes);
+          }
+          const uint32_t sa = ring + stage * stage_bytes;
           const int k0 = ki * kBK;
-          mbar_expect_tx(full, stage_bytes);
           if constexpr (kAMn) {
-            tma_load_3d(sa, &tm_a, full, t.m0, k0, t.m_outer);
-            tma_load_3d(sa + kABytes / 2, &tm_a, full, t.m0 + 64, k0, t.m_outer);
+            load(sa, &tm_a, full, t.m0, k0, t.m_outer);
+            load(sa + kABytes / 2, &tm_a, full, t.m0 + 64, k0, t.m_outer);
           } else {
-            tma_load_3d(sa, &tm_a, full, k0, t.m0, ko);
+            load(sa, &tm_a, full, k0, t.m0, ko);
           }
-          if constexpr (kBMn) {
-            for (int n = 0; n < p.tile_n; n += 64) tma_load_3d(sb + n * kBK * 2, &tm_b, full, t.n0 + n, k0, ko);
-          } else {
-            tma_load_3d(sb, &tm_b, full, k0, t.n0, 0);  // kTwo: a box of value rows and a box of gate rows in one
-          }
+          if (!p.resident) load_b(sa + kABytes, full, t.n0, k0, ko);
           ++issued;
           if (++stage == p.stages) stage = 0, phase ^= 1u;
           if (++ki == p.kblocks_inner) ki = 0, ++ko;
         }
       }
-      // If the loop was abandoned, give copies still in flight a bounded chance to land.
-      if (*abort_flag)
-        for (int j = issued > p.stages ? issued - p.stages : 0; j < issued; ++j)
-          mbar_wait(bars + (FULL + j % p.stages) * 8, (j / p.stages) & 1, abort_flag + 1);
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ MMA issuer (whole warp, one lane issues)
-    const uint32_t id = idesc(__is_same(T, __half), kBM, p.tile_n, kAMn, kBMn);
-    const uint32_t tb = __shfl_sync(0xffffffffu, tmem_base, 0);
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int i = 0; ok && i < items; ++i) {
-      const Item t = decode(p, blockIdx.x + i * gridDim.x, units);
-      const uint32_t acc = tb + (i & 1) * 256;
-      ok = mbar_wait_warp(bars + (ACC_EMPTY + (i & 1)) * 8, ((i >> 1) & 1) ^ 1, abort_flag);
-      for (int kb = t.kb0; ok && kb < t.kb1; ++kb) {
-        ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t sa = base + stage * stage_bytes;
-        // K-major: rows of 128 bytes, groups of 8 rows 1 KiB apart, a step of 16 k is 32 bytes.  MN-major: rows (k) of 64
-        // elements, blocks of 64 elements 8 KiB apart, a step of 16 k is 2 KiB.
-        const uint64_t da = kAMn ? smem_desc<8192, 1024, kLayoutSw128>(sa) : smem_desc<16, 1024, kLayoutSw128>(sa);
-        const uint64_t db = kBMn ? smem_desc<8192, 1024, kLayoutSw128>(sa + kABytes) : smem_desc<16, 1024, kLayoutSw128>(sa + kABytes);
-#pragma unroll
-        for (int k = 0; k < kBK / 16; ++k)
-          umma_ss_warp(acc, da + k * (kAMn ? 128 : 2), db + k * (kBMn ? 128 : 2), id, (kb > t.kb0 || k > 0) ? 1u : 0u);
-        umma_commit_warp(bars + (EMPTY + stage) * 8);
-        if (++stage == p.stages) stage = 0, phase ^= 1u;
+      // If the loop was abandoned, give copies still in flight a bounded chance to land (of a pair's first block: those of
+      // both; its second block's copies are waited for there).
+      if (*abort_flag) {
+        if (p.resident) mbar_wait(bars + B_FULL * 8, 0, abort_flag + 1);
+        if (rank == 0)
+          for (int j = issued > p.stages ? issued - p.stages : 0; j < issued; ++j)
+            mbar_wait(bars + (FULL + j % p.stages) * 8, (j / p.stages) & 1, abort_flag + 1);
       }
-      if (ok) umma_commit_warp(bars + (ACC_FULL + (i & 1)) * 8);
+    }
+  } else if (warp == 17) {
+    // ------------------------------------------------------------------ MMA issuer (whole warp, one lane issues)
+    if (rank == 0) {
+      const uint32_t id = idesc(__is_same(T, __half), kPair ? 2 * kBM : kBM, p.tile_n, kAMn, kBMn);
+      const uint32_t tb = __shfl_sync(0xffffffffu, tmem_base, 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      if (p.resident) ok = mbar_wait_warp(bars + B_FULL * 8, 0, abort_flag);
+      for (int i = 0; ok && i < items; ++i) {
+        const Item t = item_of<kPair, kAMn>(p, i, units);
+        const uint32_t acc = tb + (i & 1) * 256;
+        ok = mbar_wait_warp(bars + (ACC_EMPTY + (i & 1)) * 8, ((i >> 1) & 1) ^ 1, abort_flag);
+        for (int kb = t.kb0; ok && kb < t.kb1; ++kb) {
+          ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = ring + stage * stage_bytes, sb = p.resident ? base + kb * b_bytes : sa + kABytes;
+          // K-major: rows of 128 bytes, groups of 8 rows 1 KiB apart, a step of 16 k is 32 bytes.  MN-major: rows (k) of 64
+          // elements, blocks of 64 elements 8 KiB apart, a step of 16 k is 2 KiB.
+          const uint64_t da = kAMn ? smem_desc<8192, 1024, kLayoutSw128>(sa) : smem_desc<16, 1024, kLayoutSw128>(sa);
+          const uint64_t db = kBMn ? smem_desc<8192, 1024, kLayoutSw128>(sb) : smem_desc<16, 1024, kLayoutSw128>(sb);
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k) {
+            const uint64_t dak = da + k * (kAMn ? 128 : 2), dbk = db + k * (kBMn ? 128 : 2);
+            const uint32_t add = (kb > t.kb0 || k > 0) ? 1u : 0u;
+            if constexpr (kPair) umma_ss_pair_warp(acc, dak, dbk, id, add);
+            else umma_ss_warp(acc, dak, dbk, id, add);
+          }
+          if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + stage) * 8);
+          else umma_commit_warp(bars + (EMPTY + stage) * 8);
+          if (++stage == p.stages) stage = 0, phase ^= 1u;
+        }
+        if (!ok) break;
+        if constexpr (kPair) umma_commit_pair_warp(bars + (ACC_FULL + (i & 1)) * 8);
+        else umma_commit_warp(bars + (ACC_FULL + (i & 1)) * 8);
+      }
     }
   } else {
     // ------------------------------------------------------------------ finishing warps
     pdl_wait();
-    const int half = warp >> 2, m = (warp & 3) * 32, c0 = half * (units / 2);
-    const uint32_t lane_acc = tmem_base + (uint32_t(m) << 16);
-    const uint32_t slabs = base + kSmSlabs + warp * kWarpSlabs;
-    const uint32_t out_slabs = slabs + (kForm == kDense || kGrad ? 4096 : 0);
-    const uint32_t aux_bar = bars + (AUX + warp * 2) * 8;
+    const int quarter = warp >> 2, m = (warp & 3) * 32 + int(rank) * kBM;
+    const uint32_t lane_acc = tmem_base + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t slabs = base + kSmSlabs + warp * 3 * kSlab, out_slabs = slabs + (kAux ? kSlab : 0);
+    const uint32_t aux_bar = bars + (AUX + warp) * 8;
     const bool has_aux = kGrad || (kForm == kDense && p.has_aux);
     const T* bias = static_cast<const T*>(p.bias);
-    // groups of 32 columns that this warp has in an item
+    // groups of 32 result columns of an item; this warp takes every fourth
     auto groups_of = [&](const Item& t) {
       if (t.m0 + m >= p.rows_inner) return 0;
-      const int left = p.columns - t.n0 - c0, most = units / 2;
-      return left <= 0 ? 0 : ((left < most ? left : most) + 31) / 32;
+      const int left = p.columns - t.n0;
+      return ((left < units ? left : units) + 31) / 32;
     };
-    // residual or dy: the loads run two groups ahead
-    int next_i = 0, next_g = 0, next_groups = -1;
+    // residual or dy: the load of the next group runs while this one is finished
+    int next_i = 0, next_g = quarter, next_groups = -1;
     Item next{};
     uint32_t loads = 0, taken = 0;
     auto load_aux = [&]() {
-      for (; next_i < items; ++next_i, next_g = 0, next_groups = -1) {
-        if (next_groups < 0) next = decode(p, blockIdx.x + next_i * gridDim.x, units), next_groups = groups_of(next);
+      for (; next_i < items; ++next_i, next_g = quarter, next_groups = -1) {
+        if (next_groups < 0) next = item_of<kPair, kAMn>(p, next_i, units), next_groups = groups_of(next);
         if (next_g >= next_groups) continue;
         if (lane == 0) {
-          const uint32_t bar = aux_bar + (loads & 1) * 8;
-          mbar_expect_tx(bar, 2048);
-          tma_load_3d(slabs + (loads & 1) * 2048, &tm_aux, bar, next.n0 + c0 + next_g * 32, next.m0 + m, 0);
+          mbar_expect_tx(aux_bar, kSlab);
+          tma_load_3d(slabs, &tm_aux, aux_bar, next.n0 + next_g * 32, next.m0 + m, 0);
         }
-        ++loads, ++next_g;
+        ++loads, next_g += 4;
         return;
       }
     };
-    if (has_aux) load_aux(), load_aux();
+    if (has_aux) load_aux();
 
-    uint32_t stores = 0;
-    auto store = [&](const CUtensorMap& map, const float (&x)[32], int column, int row, int outer) {
-      const uint32_t slab = out_slabs + (stores & (kRing - 1)) * kSlab;
+    uint32_t slot = 0;
+    // writes a slab (32 columns in 16 bits or 16 in 32 bits, of the 32 rows) and stores it
+    auto store = [&](const CUtensorMap& map, const uint32_t (&x)[16], int column, int row, int outer) {
+      const uint32_t slab = out_slabs + slot * kSlab;
       if (lane == 0) tma_store_wait_read<kRing - 1>();  // the store that used this slab before has read it
       __syncwarp();
-      if constexpr (kForm == kPartial) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          sts128(slab + sw128_offset(lane, j), make_uint4(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]),
-                                                          __float_as_uint(x[4 * j + 2]), __float_as_uint(x[4 * j + 3])));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          sts128(slab + sw64_offset(lane, j), make_uint4(pack2<T>(x[8 * j], x[8 * j + 1]), pack2<T>(x[8 * j + 2], x[8 * j + 3]),
-                                                         pack2<T>(x[8 * j + 4], x[8 * j + 5]), pack2<T>(x[8 * j + 6], x[8 * j + 7])));
-      }
+      for (int j = 0; j < 4; ++j) sts128(slab + sw64_offset(lane, j), make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -321,91 +461,101 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         else tma_store_3d(&map, slab, column, row, outer);
         tma_store_commit();
       }
-      ++stores;
+      if (++slot == kRing) slot = 0;
+    };
+    auto release = [&](int i) {  // the accumulator is in registers
+      tc_fence_before();
+      __syncwarp();
+      const uint32_t bar = bars + (ACC_EMPTY + (i & 1)) * 8;
+      if (kPair) mbar_arrive_cluster_warp(in_first_block(bar));
+      else mbar_arrive_warp(bar);
     };
 
     bool ok = true;
     for (int i = 0; ok && i < items; ++i) {
-      const Item t = decode(p, blockIdx.x + i * gridDim.x, units);
-      const int groups = groups_of(t);
+      const Item t = item_of<kPair, kAMn>(p, i, units);
+      const int groups = groups_of(t), row = t.m0 + m;
       ok = mbar_wait_warp(bars + (ACC_FULL + (i & 1)) * 8, (i >> 1) & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t acc = lane_acc + (i & 1) * 256 + c0;
-      for (int g = 0; g < groups; ++g) {
-        uint32_t r[32], q[32];
-        tmem_ld32(acc + g * 32, r);
-        if constexpr (kTwo) tmem_ld32(acc + units + g * 32, q);
-        const int n = t.n0 + c0 + g * 32, row = t.m0 + m;
-        float aux[32];
-        if constexpr (kGrad || kForm == kDense) {
+      const uint32_t acc = lane_acc + (i & 1) * 256;
+      if (quarter >= groups) release(i);
+      for (int g = quarter; g < groups; g += 4) {
+        const int n = t.n0 + g * 32;
+        uint32_t aux[16];
+        if constexpr (kAux) {
           if (has_aux) {
-            ok = mbar_wait_warp(aux_bar + (taken & 1) * 8, (taken >> 1) & 1, abort_flag);
+            ok = mbar_wait_warp(aux_bar, taken & 1, abort_flag);
             if (!ok) break;
-            const uint32_t slab = slabs + (taken & 1) * 2048;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const uint4 x = lds128(slab + sw64_offset(lane, j));
-              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack2<T>(w[e]);
-                aux[j * 8 + 2 * e] = f.x, aux[j * 8 + 2 * e + 1] = f.y;
-              }
+              const uint4 x = lds128(slabs + sw64_offset(lane, j));
+              aux[4 * j] = x.x, aux[4 * j + 1] = x.y, aux[4 * j + 2] = x.z, aux[4 * j + 3] = x.w;
             }
             ++taken;
             __threadfence_block();  // the reads are complete before the next load may overwrite the slab
             __syncwarp();
             load_aux();
+          }
+        }
+        // Accumulators are taken 16 columns at a time (kDense, kPlain: 32), to stay within the registers that 18 warps leave a thread.
+        constexpr int kStep = kForm == kDense || kForm == kPlain ? 32 : 16;
+        uint32_t y[16], yg[16], z[16], zg[16];
+        auto step = [&](auto first) {
+          constexpr int kFirst = decltype(first)::value;
+          float v[kStep], gate[kStep];
+          tmem_load(acc + g * 32 + kFirst, v);
+          if constexpr (kTwo) tmem_load(acc + units + g * 32 + kFirst, gate);
+          tmem_ld_wait();
+          if (kFirst + kStep == 32 && g + 4 >= groups) release(i);
+          if constexpr (kForm == kPartial) {
+            uint32_t x[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(v[j]);
+            if (n + kFirst < p.columns) store(tm_out, x, n + kFirst, row, t.split * (p.tiles_m / p.tiles_m_inner) + t.m_outer);
+          } else if constexpr (kForm == kPlain) {
+#pragma unroll
+            for (int j = 0; j < kStep / 2; ++j) y[kFirst / 2 + j] = pack2<T>(v[2 * j], v[2 * j + 1]);
           } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) aux[j] = 0.f;
-          }
-        }
-        tmem_ld_wait();
-        if (g == groups - 1) {  // the accumulator is in registers
-          tc_fence_before();
-          __syncwarp();
-          mbar_arrive_warp(bars + (ACC_EMPTY + (i & 1)) * 8);
-        }
-        float v[32], gate[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]), gate[j] = kTwo ? __uint_as_float(q[j]) : 0.f;
-        if constexpr (kForm == kPartial) {
-          store(tm_out, v, n, row, t.split * (p.tiles_m / p.tiles_m_inner) + t.m_outer);
-        } else {
-          if (bias != nullptr) {
-            add_bias(v, bias, n, p.columns);
-            if (kTwo) add_bias(gate, bias + p.columns, n, p.columns);
-          }
-          if constexpr (kForm == kDense || kForm == kGated) {
-            if (p.has_saved) {
-              store(tm_saved, v, n, row, 0);
-              if (kTwo) store(tm_saved, gate, n, row, 1);
+            if (bias != nullptr) {
+              add_bias(v, bias, n + kFirst, p.columns);
+              if constexpr (kTwo) add_bias(gate, bias + p.columns, n + kFirst, p.columns);
             }
+            if ((kForm == kDense || kForm == kGated) && p.has_saved) {
+#pragma unroll
+              for (int j = 0; j < kStep / 2; ++j) {
+                z[kFirst / 2 + j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+                if (kTwo) zg[kFirst / 2 + j] = pack2<T>(gate[2 * j], gate[2 * j + 1]);
+              }
+            }
+            finish_any<T, kForm, kFirst, kStep>(p.activation, v, gate, has_aux, aux, y, yg);
           }
-          finish_any<kForm>(p.activation, v, gate, aux);
-          store(tm_out, v, n, row, kForm == kDense ? t.m_outer : 0);
-          if (kForm == kGatedGrad) store(tm_out, gate, n, row, 1);
+        };
+        step(std::integral_constant<int, 0>());
+        if constexpr (kStep == 16) step(std::integral_constant<int, 16>());
+        if constexpr (kForm != kPartial) {
+          if ((kForm == kDense || kForm == kGated) && p.has_saved) {
+            store(tm_saved, z, n, row, 0);
+            if (kTwo) store(tm_saved, zg, n, row, 1);
+          }
+          store(tm_out, y, n, row, kForm == kPlain ? t.m_outer : 0);
+          if (kForm == kGatedGrad) store(tm_out, yg, n, row, 1);
         }
-      }
-      if (ok && groups == 0) {
-        tc_fence_before();
-        __syncwarp();
-        mbar_arrive_warp(bars + (ACC_EMPTY + (i & 1)) * 8);
       }
     }
-    if (!ok)  // loads of the residual or of dy still in flight
-      for (uint32_t j = taken; j < loads; ++j) mbar_wait(aux_bar + (j & 1) * 8, (j >> 1) & 1, abort_flag + 1);
+    if (!ok && taken < loads) mbar_wait(aux_bar, taken & 1, abort_flag + 1);  // a load still in flight
     if (lane == 0) tma_store_wait_all();
   }
 
   __syncwarp();
   tc_fence_before();
-  __syncthreads();
-  if (warp == 9) {
+  // a pair's blocks stay until the other no longer arrives on their barriers or reads their operands
+  if constexpr (kPair) cluster_sync();
+  else __syncthreads();
+  if (warp == 17) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    if constexpr (kPair) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
   }
   if (threadIdx.x == 0 && *abort_flag) *p.status = B200TA_ERR_DEVICE_WAIT;
 }
@@ -447,9 +597,11 @@ int launch_matmul_product(DeviceState* st, const Matmul& m, const MatmulMaps& ma
 namespace matmul {
 template <MatmulForm kForm, bool kAMn, bool kBMn>
 int launch(DeviceState* st, int id, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, int grid, void* stream) {
-  const KernelId kernel = KernelId(kKernelMatmul + 2 * id + (m.f16 ? 1 : 0));
-  return launch_kernel(st, kernel, m.f16 ? matmul_kernel<__half, kForm, kAMn, kBMn> : matmul_kernel<__nv_bfloat16, kForm, kAMn, kBMn>,
-                       dim3(unsigned(grid)), kThreads, kSmDynamic, stream, maps.a, maps.b, maps.out, maps.aux, maps.saved, p);
+  const KernelId kernel = KernelId(kKernelMatmul + 4 * id + (m.f16 ? 2 : 0) + (p.pair ? 1 : 0));
+  auto* function = p.pair ? (m.f16 ? matmul_kernel<__half, kForm, kAMn, kBMn, true> : matmul_kernel<__nv_bfloat16, kForm, kAMn, kBMn, true>)
+                          : (m.f16 ? matmul_kernel<__half, kForm, kAMn, kBMn, false> : matmul_kernel<__nv_bfloat16, kForm, kAMn, kBMn, false>);
+  return launch_clusters(st, kernel, function, dim3(unsigned(grid)), p.pair ? 2 : 1, kThreads, kSmDynamic, stream, maps.a, maps.b,
+                         maps.out, maps.aux, maps.saved, p);
 }
 }  // namespace matmul
 #endif
