@@ -10,6 +10,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace b200ta {
@@ -32,6 +34,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // the larger one,
 __device__ __forceinline__ float keep_nan(float z, float value) { return z == z ? value : z; }
 struct F2 {
   uint64_t v;
+  F2() = default;
   __device__ __forceinline__ F2(float a, float b) : v(pack_f32x2(a, b)) {}
   __device__ __forceinline__ explicit F2(float a) : v(pack_f32x2(a, a)) {}
   __device__ __forceinline__ explicit F2(uint64_t x) : v(x) {}

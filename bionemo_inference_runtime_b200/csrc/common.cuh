@@ -62,7 +62,7 @@ template <typename... P, typename... A>
 int launch_clusters(DeviceState* st, KernelId id, void (*kernel)(P...), dim3 grid, unsigned cluster, int threads, int smem_bytes,
                     void* stream, A&&... args) {
   const uint64_t bit = 1ull << id;
-  if (smem_bytes > 0 && !(st->configured.load(std::memory_order_relaxed) & bit)) {
+  if (smem_bytes > 48 * 1024 && !(st->configured.load(std::memory_order_relaxed) & bit)) {
     B200TA_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
     st->configured.fetch_or(bit, std::memory_order_relaxed);
   }

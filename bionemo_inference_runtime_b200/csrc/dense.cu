@@ -32,10 +32,6 @@ Tiling choose_tiling(const Matmul& m, int64_t rows, int64_t m_outer, int64_t col
     if (cost < least * 0.98) least = cost, best = t;
   };
   auto waves_of = [](int64_t items, int64_t blocks) { return double((items + blocks - 1) / blocks); };
-  if (rows > matmul::kBM && accumulated > 128) {
-    const int64_t tiles = (rows + 255) / 256 * m_outer * splits * ((accumulated + 255) / 256);
-    consider({256, 1, 0}, waves_of(tiles, num_sms / 2), kblocks * 712.0, 256);
-  }
   for (int n = 256; n >= 64; n /= 2) {
     if (n > 64 && n / 2 >= accumulated) continue;
     const int64_t tiles_m = (rows + 127) / 128 * m_outer, tiles_n = (accumulated + n - 1) / n;
@@ -46,6 +42,10 @@ Tiling choose_tiling(const Matmul& m, int64_t rows, int64_t m_outer, int64_t col
     } else {
       consider({n, 0, 0}, waves_of(tiles_m * tiles_n * splits, num_sms), kblocks * std::max(mma, (n == 256 ? 1.2 : 1.0) * (16384 + n * 128) / 46), n);
     }
+  }
+  if (rows > matmul::kBM && accumulated > 128) {
+    const int64_t tiles = (rows + 255) / 256 * m_outer * splits * ((accumulated + 255) / 256);
+    consider({256, 1, 0}, waves_of(tiles, num_sms / 2), kblocks * 712.0, 256);
   }
   return best;
 }
@@ -434,12 +434,11 @@ BackwardPlan plan_backward(bool gated, bool slope, int64_t rows, int K, int N, i
   p.dz_pitch = gated || slope ? outer * pad8(N) : 0;
   p.chunk = rows;
   if (p.dz_pitch != 0) {
-    // Narrow layers are bound by HBM: dz of a chunk is read back from L2 if it fits there, and the next chunk overwrites it.
-    // A chunk is a row tile for every SM, or several.  Wide layers are bound by the tensor cores: their chunks only keep the
-    // workspace small.
+    // At most half a gigabyte of dz, in whole waves of row tiles.  (Chunks that L2 keeps do not pay: a gated layer 128 -> 512
+    // over 147456 rows took 347 us in chunks of 39 MB, 300 us of 116 MB and 241 us in one, which writes dz to HBM and reads
+    // it twice; each launch's first loads and last stores cost more.)
     const int64_t wave = (int64_t(num_sms) * matmul::kBM + kSumRows - 1) / kSumRows * kSumRows;
-    const int64_t fit = (K <= 256 ? int64_t(48) << 20 : int64_t(1) << 30) / (p.dz_pitch * 2) / wave;
-    p.chunk = std::min(rows, std::max<int64_t>(fit, 1) * wave);
+    p.chunk = std::min(rows, std::max<int64_t>((int64_t(1) << 29) / (p.dz_pitch * 2) / wave, 1) * wave);
   }
   p.split = split_rows(p.chunk, N, outer, K, num_sms);
   p.direct = p.chunk >= rows && p.split.parts == 1 && K % 8 == 0;

@@ -1,0 +1,268 @@
+// Layer norm over the last axis and its gradients (sm_100a), for bf16, fp16 or fp32 rows:
+//
+//   y  = (x - mean) rstd w + b                          rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   dx = rstd (g - mean(g) - xh mean(g xh))             g = dy w, xh = (x - mean) rstd
+//   dw = sum over rows of dy xh,  db = sum over rows of dy
+//
+// Bound: HBM.  Forward reads x and writes y, backward reads x and dy and writes dx, each once: a row is held in the
+// registers of the 2 to 1024 threads that share it, and its mean and variance, or its two sums, are taken there in 32 bits,
+// the variance from centred values.  Issue slots come next (a first version with 64-bit index arithmetic and unpacked sums
+// needed 200 instructions for 16 values a lane and stayed at half the bandwidth), so addresses advance by constants, sums
+// and products are made in packed pairs, and groups of lanes have a size known at compile time.  Blocks are persistent; a
+// thread keeps its columns, and with them their parameters in registers (of up to 16 columns), and copies the next rows' vectors into its own slots
+// of shared memory while it works on one (registers alone hold too few bytes in flight).
+//
+// Rows that are not 16-byte aligned (odd widths, odd pitches) take the same path with aligned loads that are shifted into
+// place in registers and stores that are shifted back between neighbouring lanes; only the ends of a warp's segment are
+// stored by elements.  (A 16-byte vector with a byte of the row in it lies in the row's allocation.)
+#pragma once
+
+#include "activation.cuh"
+#include "common.cuh"
+
+namespace b200ta {
+
+struct NormParams {
+  const void *x, *dy, *w, *b;
+  void *y, *dx;
+  float2* stats;   // {rstd, -mean * rstd} per row: written by the forward pass (if not NULL), read by the backward pass
+  float* partial;  // [blocks][2][width]
+  long long xs, ys, dys, dxs, rows;
+  int width;
+  int lanes;           // threads that share a row, a power of two
+  int params_aligned;  // the parameters may be read by vectors
+  float eps;
+};
+
+struct NormShape {
+  int lanes, items, threads;
+  bool shifted;
+};
+constexpr int kNormThreads = 256;  // of a block, unless a row takes more
+constexpr int kNormMaxWidth = 16384;
+// Threads that share a row: a warp or less (from 2), or up to `most_lanes` of them, as long as 16 values a thread hold the row;
+// up to 512 with 32 values for what is wider.
+inline NormShape norm_shape(int width, int vec, int most_lanes, bool shifted) {
+  NormShape s;
+  s.shifted = shifted;
+  const int n = (width + vec - 1) / vec, most = (n > most_lanes * 16 / vec ? 32 : 16) / vec;
+  s.lanes = 2;
+  while (s.lanes < 32 && s.lanes < n) s.lanes *= 2;
+  while (s.lanes * most < n) s.lanes *= 2;
+  s.items = (n + s.lanes - 1) / s.lanes;
+  // the kernels are made for 1, 2 and all items of 16 values, and for those of 32
+  s.items = s.items <= 2 ? s.items : s.items * vec <= 16 ? 16 / vec : 32 / vec;
+  s.threads = s.lanes > kNormThreads ? s.lanes : kNormThreads;
+  return s;
+}
+inline int norm_element_bytes(int dtype) { return dtype == B200TA_DTYPE_F32 ? 4 : 2; }
+inline bool norm_aligned(const void* p, int64_t stride, int bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride * bytes % 16 == 0;
+}
+
+#ifdef __CUDACC__
+namespace norm {
+
+// kVec values of 16 bytes in packed pairs.
+template <typename T>
+struct Values {
+  static constexpr int kVec = 16 / int(sizeof(T));
+  F2 p[kVec / 2];
+  __device__ __forceinline__ explicit Values(uint4 x) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < kVec / 2; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        p[j] = F2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+      } else {
+        const float2 f = unpack2<T>(w[j]);
+        p[j] = F2(f.x, f.y);
+      }
+    }
+  }
+};
+template <typename T>
+__device__ __forceinline__ uint4 bits_of(const F2* p) {
+  float a[8];
+  if constexpr (sizeof(T) == 4) {
+    p[0].to(a[0], a[1]), p[1].to(a[2], a[3]);
+    return make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j].to(a[2 * j], a[2 * j + 1]);
+    return make_uint4(pack2<T>(a[0], a[1]), pack2<T>(a[2], a[3]), pack2<T>(a[4], a[5]), pack2<T>(a[6], a[7]));
+  }
+}
+
+// Bytes `at` .. `at` + 15 of the 32 bytes of lo and hi (0 <= at < 16, a multiple of the element size).
+template <typename T>
+__device__ __forceinline__ uint4 window(uint4 lo, uint4 hi, uint32_t at) {
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  if (at & 8u) w[0] = w[2], w[1] = w[3], w[2] = w[4], w[3] = w[5], w[4] = w[6], w[5] = w[7];
+  if (at & 4u) w[0] = w[1], w[1] = w[2], w[2] = w[3], w[3] = w[4], w[4] = w[5];
+  if (sizeof(T) == 2 && (at & 2u)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The first `valid` elements of a vector, zeros behind them.
+template <typename T>
+__device__ __forceinline__ uint4 first(uint4 x, int valid) {
+  constexpr int kPer = 4 / int(sizeof(T));
+  uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int left = valid - j * kPer;
+    w[j] = left >= kPer ? w[j] : left <= 0 ? 0u : w[j] & 0xFFFFu;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Rows that a group of threads works on at a time: two where a thread holds 16 values, so that a row's sums over the group
+// (shuffles, and a barrier beyond a warp) cost half.
+__host__ __device__ constexpr int rows_at_a_time(int values, bool shifted) { return values == 16 && !shifted ? 2 : 1; }
+// Slots of shared memory for rows of `vectors` vectors a thread, those that are worked on included.
+__host__ __device__ constexpr int stages_of(int vectors, int threads, int blocks) {
+  const int by_bytes = 196608 / blocks / (vectors * threads * 16);
+  return by_bytes < 4 ? by_bytes : 4;
+}
+__device__ __forceinline__ void copy_ahead(uint32_t slot, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// A vector of a row from `p` on, `valid` elements of which are in the row.
+template <typename T, bool kShifted>
+__device__ __forceinline__ uint4 load(const T* p, int valid) {
+  if constexpr (!kShifted) {
+    return __ldg(reinterpret_cast<const uint4*>(p));
+  } else {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), base = a & ~uintptr_t(15);
+    const uint32_t at = uint32_t(a & 15u), bytes = (valid < Values<T>::kVec ? valid : Values<T>::kVec) * uint32_t(sizeof(T));
+    const uint4 lo = __ldg(reinterpret_cast<const uint4*>(base));
+    uint4 hi = make_uint4(0u, 0u, 0u, 0u);
+    if (at + bytes > 16u) hi = __ldg(reinterpret_cast<const uint4*>(base) + 1);
+    const uint4 x = window<T>(lo, hi, at);
+    return valid >= Values<T>::kVec ? x : first<T>(x, valid);
+  }
+}
+// Stores a vector of a row at `p`, the `index`-th of the `lanes` vectors that neighbouring lanes of this warp store, all of
+// which call this; valid <= 0: nothing of it is in the row.
+template <typename T, bool kShifted>
+__device__ __forceinline__ void store(T* p, uint4 x, int valid, int index, int lanes) {
+  constexpr int kVec = Values<T>::kVec;
+  if constexpr (!kShifted) {
+    if (valid > 0) *reinterpret_cast<uint4*>(p) = x;
+  } else {
+    const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>(p) & 15u);
+    const int own = at == 0 ? kVec : int((16u - at) / sizeof(T));  // elements up to the next 16-byte boundary
+    uint4 before;
+    before.x = __shfl_up_sync(0xffffffffu, x.x, 1), before.y = __shfl_up_sync(0xffffffffu, x.y, 1);
+    before.z = __shfl_up_sync(0xffffffffu, x.z, 1), before.w = __shfl_up_sync(0xffffffffu, x.w, 1);
+    // the aligned vector that ends in this lane's first elements; the one behind it is the next lane's
+    const bool whole = valid >= own && (at == 0 || index > 0);
+    const bool next = at == 0 || (index + 1 < lanes && valid - kVec >= own);
+    if (whole) *reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(p) - at) = at == 0 ? x : window<T>(before, x, 16u - at);
+    if (!(whole && next)) {
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        if (e < valid && !(e < own ? whole : next)) {
+          if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[e] = w[e];
+          else reinterpret_cast<uint16_t*>(p)[e] = uint16_t(w[e / 2] >> (16 * (e & 1)));
+        }
+      }
+    }
+  }
+}
+
+// The parameters of kVec columns from c on, `valid` of them in the row, or `none` where there are none.
+template <typename T, typename W, bool kShifted>
+__device__ __forceinline__ void load_param(const NormParams& p, const void* param, int c, int valid, float none, F2* v) {
+  constexpr int kVec = Values<T>::kVec;
+  if (param == nullptr) {
+#pragma unroll
+    for (int j = 0; j < kVec / 2; ++j) v[j] = F2(none);
+  } else if (!kShifted || (p.params_aligned && valid >= kVec)) {
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const W*>(param) + c);
+    if constexpr (sizeof(W) == sizeof(T)) {
+      const Values<W> x(__ldg(q));
+#pragma unroll
+      for (int j = 0; j < kVec / 2; ++j) v[j] = x.p[j];
+    } else {
+      const Values<float> lo(__ldg(q)), hi(__ldg(q + 1));
+      v[0] = lo.p[0], v[1] = lo.p[1], v[2] = hi.p[0], v[3] = hi.p[1];
+    }
+  } else {
+    const W* q = static_cast<const W*>(param) + c;
+#pragma unroll
+    for (int j = 0; j < kVec / 2; ++j)
+      v[j] = F2(2 * j < valid ? static_cast<float>(q[2 * j]) : none, 2 * j + 1 < valid ? static_cast<float>(q[2 * j + 1]) : none);
+  }
+}
+
+__device__ __forceinline__ float sum_of(F2 p) {
+  float a, b;
+  p.to(a, b);
+  return a + b;
+}
+
+// The sums over the threads that share a row; every one of them gets the result.  Rows of more than a warp go through one of
+// two halves of `scratch` in turn (32 warps each): all threads of the block call this equally often.
+template <int kLanes, int kSums>
+__device__ __forceinline__ void row_sums(float (&s)[kSums], int lanes, float* scratch, int& turn) {
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+  if (kLanes == 32 && lanes > 32) {
+    const int warp = threadIdx.x >> 5, warps = lanes >> 5, first = warp / warps * warps;
+    float* half = scratch + turn * 32 * kSums;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int i = 0; i < kSums; ++i) half[warp * kSums + i] = s[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) s[i] = 0.f;
+    for (int w = first; w < first + warps; ++w)
+#pragma unroll
+      for (int i = 0; i < kSums; ++i) s[i] += half[w * kSums + i];
+  }
+}
+
+// Launches one kernel; its shared-memory limit is raised once on each device.
+template <auto kKernel>
+int launch_one(DeviceState* st, int blocks, int threads, int smem, void* stream, const NormParams& p) {
+  static std::atomic<uint64_t> raised{0};
+  const uint64_t bit = 1ull << st->device;
+  if (smem > 40 * 1024 && !(raised.load(std::memory_order_relaxed) & bit)) {
+    B200TA_CHECK_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    raised.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return launch_kernel(st, kKernelNorm, kKernel, dim3(unsigned(blocks)), threads, smem, stream, p);
+}
+
+// The launch of a shape's kernel<T, W, kShifted, kItems, kLanes, kMost>: 2, 4, 8, 16 or (at least) 32 lanes, blocks of at most
+// kMost threads.
+#define B200TA_NORM_PICK(kernel, T, W, kShifted, s)                                  \
+  (s.threads > 256 && s.items > int(sizeof(T))                                       \
+       ? &norm::launch_one<kernel<T, W, kShifted, 2 * int(sizeof(T)), 32, 512>>      \
+   : s.threads > 256     ? &norm::launch_one<kernel<T, W, kShifted, int(sizeof(T)), 32, 512>>         \
+   : s.lanes == 2        ? &norm::launch_one<kernel<T, W, kShifted, 1, 2, 256>>                       \
+   : s.lanes == 4        ? &norm::launch_one<kernel<T, W, kShifted, 1, 4, 256>>                       \
+   : s.lanes == 8        ? &norm::launch_one<kernel<T, W, kShifted, 1, 8, 256>>                       \
+   : s.lanes == 16       ? &norm::launch_one<kernel<T, W, kShifted, 1, 16, 256>>                      \
+   : s.items == 1        ? &norm::launch_one<kernel<T, W, kShifted, 1, 32, 256>>                      \
+   : s.items == 2        ? &norm::launch_one<kernel<T, W, kShifted, 2, 32, 256>>                      \
+   : s.items <= sizeof(T) ? &norm::launch_one<kernel<T, W, kShifted, int(sizeof(T)), 32, 256>>        \
+                         : &norm::launch_one<kernel<T, W, kShifted, 2 * int(sizeof(T)), 32, 256>>)
+
+}  // namespace norm
+#endif  // __CUDACC__
+}  // namespace b200ta

@@ -1,0 +1,262 @@
+// Gradients of the layer norm; see layer_norm.cuh for the mathematics and what bounds it.
+//
+// A thread keeps its columns, so dw and db add up in its registers over all of its rows, are joined over the block in shared
+// memory, and one row of partial sums per block goes to the workspace, which a second kernel adds up.  The order is fixed:
+// results repeat bit by bit.
+#include "layer_norm.cuh"
+
+namespace b200ta {
+namespace {
+
+// Blocks of a multiprocessor: 8 values a thread leave room for three of 256 threads, more for two.
+__host__ __device__ constexpr int grad_blocks_of(int threads, int values) { return threads > 256 ? 1 : values <= 8 ? 3 : 2; }
+
+template <typename T, typename W, bool kShifted, int kItems, int kLanes, int kMost>
+__global__ void __launch_bounds__(kMost, grad_blocks_of(kMost, kItems * norm::Values<T>::kVec))
+norm_grad_kernel(const NormParams p) {
+  constexpr int kVec = norm::Values<T>::kVec, kPairs = kVec / 2;
+  constexpr int kRows = norm::rows_at_a_time(kItems * kVec, kShifted);
+  constexpr int kStages = norm::stages_of(2 * kItems, kMost, grad_blocks_of(kMost, kItems * kVec));
+  constexpr bool kHold = kItems * kVec <= 16;
+  constexpr bool kKeep = kRows == 1 && kHold;  // xh and g stay in registers between the two passes over a row
+  extern __shared__ uint4 slots[];    // [stage][x items, dy items][thread] (not for shifted rows); joined sums at the end
+  float* joined = reinterpret_cast<float*>(slots);  // [groups / 2][2][width]
+  __shared__ float scratch[128 * kRows];
+  pdl_trigger();
+  pdl_wait();
+  const int lanes = kLanes == 32 ? p.lanes : kLanes, lane = threadIdx.x & (lanes - 1);
+  const int per_block = blockDim.x / lanes, group = threadIdx.x / lanes;
+  const float inv = 1.f / float(p.width);
+  int turn = 0, valid[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) valid[i] = p.width - (i * lanes + lane) * kVec;
+  const long long row0 = (long long)blockIdx.x * per_block + group, step = (long long)gridDim.x * per_block;
+  const T* x = static_cast<const T*>(p.x) + row0 * p.xs + lane * kVec;
+  const T* dy = static_cast<const T*>(p.dy) + row0 * p.dys + lane * kVec;
+  T* dx = static_cast<T*>(p.dx) + row0 * p.dxs + lane * kVec;
+  const float2* stats = p.stats + row0;
+  long long left = p.rows - row0, block_left = p.rows - (long long)blockIdx.x * per_block;
+  const uint32_t slot0 = smem_u32(slots) + threadIdx.x * 16, item_bytes = blockDim.x * 16, stage_bytes = 2 * kItems * item_bytes;
+  long long ahead = left;
+  int fill = 0, take = 0;
+  auto fetch = [&]() {
+    if (ahead > 0)
+#pragma unroll
+      for (int i = 0; i < kItems; ++i)
+        if (valid[i] > 0) {
+          norm::copy_ahead(slot0 + fill * stage_bytes + i * item_bytes, x + i * lanes * kVec);
+          norm::copy_ahead(slot0 + fill * stage_bytes + (kItems + i) * item_bytes, dy + i * lanes * kVec);
+        }
+    norm::copy_commit();
+    x += step * p.xs, dy += step * p.dys, ahead -= step;
+    if (++fill == kStages) fill = 0;
+  };
+  if constexpr (!kShifted)
+    for (int i = 0; i < kStages - kRows; ++i) fetch();
+  F2 dw[kItems][kPairs] = {}, db[kItems][kPairs] = {}, w[kHold ? kItems : 1][kPairs] = {};
+#pragma unroll
+  for (int i = 0; i < kItems; ++i)
+    if (kHold && valid[i] > 0) norm::load_param<T, W, kShifted>(p, p.w, (i * lanes + lane) * kVec, valid[i], 1.f, w[kHold ? i : 0]);
+  float2 next[kRows];
+  auto fetch_stats = [&](long long rows_left) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) next[r] = rows_left > r * step ? __ldg(stats + r * step) : make_float2(0.f, 0.f);
+    stats += kRows * step;
+  };
+  fetch_stats(left);
+  for (; block_left > 0; block_left -= kRows * step, left -= kRows * step) {
+    F2 xh[kKeep ? kItems : 1][kPairs], g[kKeep ? kItems : 1][kPairs];
+    float2 st[kRows];
+    float s[2 * kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) st[r] = next[r];
+    fetch_stats(left - kRows * step);
+    if constexpr (!kShifted) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) fetch();
+      norm::copy_wait<kStages - kRows>();
+    }
+    // xh and g = dy w of item i of a row; with kSum also dw and db
+    auto load = [&](int i, int r, int stage, auto sum) {
+      uint4 raw_x = make_uint4(0u, 0u, 0u, 0u), raw_dy = raw_x;
+      if (left > r * step && valid[i] > 0) {
+        if constexpr (kShifted) {
+          raw_x = norm::load<T, kShifted>(x + i * lanes * kVec, valid[i]);
+          raw_dy = norm::load<T, kShifted>(dy + i * lanes * kVec, valid[i]);
+        } else {
+          raw_x = lds128(slot0 + stage * stage_bytes + i * item_bytes);
+          raw_dy = lds128(slot0 + stage * stage_bytes + (kItems + i) * item_bytes);
+        }
+      }
+      const norm::Values<T> vx(raw_x), vd(raw_dy);
+      const int k = kKeep ? i : 0, kw = kHold ? i : 0;
+      if (!kHold && valid[i] > 0) norm::load_param<T, W, kShifted>(p, p.w, (i * lanes + lane) * kVec, valid[i], 1.f, w[0]);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        // (behind the row dy is zero, and what xh is there does not count)
+        xh[k][j] = fma2(vx.p[j], F2(st[r].x), F2(st[r].y));
+        if constexpr (decltype(sum)::value) {
+          dw[i][j] = fma2(vd.p[j], xh[k][j], dw[i][j]);
+          db[i][j] = db[i][j] + vd.p[j];
+        }
+        g[k][j] = vd.p[j] * w[kw][j];
+      }
+    };
+    int stage = take;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      F2 s0(0.f), s1(0.f);
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        load(i, r, stage, std::true_type());
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) s0 = s0 + g[kKeep ? i : 0][j], s1 = fma2(g[kKeep ? i : 0][j], xh[kKeep ? i : 0][j], s1);
+      }
+      s[2 * r] = norm::sum_of(s0), s[2 * r + 1] = norm::sum_of(s1);
+      if (++stage == kStages) stage = 0;
+    }
+    if (p.dx != nullptr) {
+      norm::row_sums<kLanes>(s, lanes, scratch, turn);
+      stage = take;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const F2 a(st[r].x), b(-s[2 * r] * inv * st[r].x), c(-s[2 * r + 1] * inv * st[r].x);
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          if constexpr (!kKeep) load(i, r, stage, std::false_type());
+          F2 out[kPairs];
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) out[j] = fma2(xh[kKeep ? i : 0][j], c, fma2(g[kKeep ? i : 0][j], a, b));
+          norm::store<T, kShifted>(dx + i * lanes * kVec, norm::bits_of<T>(out), left > r * step ? valid[i] : 0, lane & (kLanes - 1), kLanes);
+        }
+        dx += step * p.dxs;
+        if (++stage == kStages) stage = 0;
+      }
+    }
+    if (kShifted) x += step * p.xs, dy += step * p.dys;
+    take = stage;
+  }
+  if (p.partial == nullptr) return;
+  norm::copy_wait<0>();
+  __syncthreads();  // the slots are free
+  // the groups' sums, joined in pairs: half of the groups that are left hand theirs to the other half
+  auto each = [&](float* at, bool add) {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        const int c = (i * lanes + lane) * kVec + 2 * j;
+        float w0, w1, b0, b1;
+        dw[i][j].to(w0, w1), db[i][j].to(b0, b1);
+        if (add) {
+          if (c < p.width) w0 += at[c], b0 += at[p.width + c];
+          if (c + 1 < p.width) w1 += at[c + 1], b1 += at[p.width + c + 1];
+          dw[i][j] = F2(w0, w1), db[i][j] = F2(b0, b1);
+        } else {
+          if (c < p.width) at[c] = w0, at[p.width + c] = b0;
+          if (c + 1 < p.width) at[c + 1] = w1, at[p.width + c + 1] = b1;
+        }
+      }
+  };
+  for (int left_groups = per_block; left_groups > 1; left_groups >>= 1) {
+    const int half = left_groups >> 1;
+    if (group >= half && group < left_groups) each(joined + (group - half) * 2 * p.width, false);
+    __syncthreads();
+    if (group < half) each(joined + group * 2 * p.width, true);
+    __syncthreads();
+  }
+  if (group == 0) each(p.partial + (long long)blockIdx.x * 2 * p.width, false);
+}
+
+// dw and db: column sums of the blocks' partial sums.  A block takes 32 of the 2 * width columns, 32 threads a column.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+norm_join_kernel(const float* partial, int blocks, int width, T* dw, T* db) {
+  __shared__ float part[32][33];
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float sum = 0.f;
+  if (c < 2 * width)
+#pragma unroll 8
+    for (int b = k; b < blocks; b += 32) sum += __ldg(partial + (long long)b * 2 * width + c);
+  part[k][lane] = sum;
+  __syncthreads();
+  if (k == 0 && c < 2 * width) {
+#pragma unroll
+    for (int i = 1; i < 32; ++i) sum += part[i][lane];
+    T* dst = c < width ? dw : db;
+    if (dst != nullptr) dst[c < width ? c : c - width] = static_cast<T>(sum);
+  }
+}
+
+template <typename T, typename W>
+auto pick(const NormShape& s) {
+  return s.shifted ? B200TA_NORM_PICK(norm_grad_kernel, T, W, true, s) : B200TA_NORM_PICK(norm_grad_kernel, T, W, false, s);
+}
+
+}  // namespace
+}  // namespace b200ta
+
+extern "C" {
+
+size_t b200ta_layer_norm_workspace_bytes(int64_t rows, int width) {
+  // a row of partial sums for each block; at most three blocks run on a multiprocessor
+  using namespace b200ta;
+  DeviceState* st = nullptr;
+  if (rows <= 0 || width <= 0 || get_device_state(&st) != B200TA_OK) return 0;
+  const int64_t most = int64_t(st->num_sms) * 3;
+  return size_t(rows < most ? rows : most) * 2 * size_t(width) * sizeof(float);
+}
+
+int b200ta_layer_norm_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const void* stats, const void* weight,
+                               int param_dtype, void* dx, int64_t dxs, void* dweight, void* dbias, void* workspace,
+                               size_t workspace_bytes, int dtype, int64_t rows, int width, void* stream) {
+  using namespace b200ta;
+  B200TA_REQUIRE(dy && x && stats, "layer_norm_backward: NULL pointer");
+  B200TA_REQUIRE(dtype >= 0 && dtype <= B200TA_DTYPE_F16, "layer_norm_backward: unknown dtype %d", dtype);
+  B200TA_REQUIRE(param_dtype == dtype || param_dtype == B200TA_DTYPE_F32,
+                 "layer_norm_backward: parameters are in the dtype of x or in float32");
+  B200TA_REQUIRE(rows > 0 && width > 0 && width <= kNormMaxWidth, "layer_norm_backward: rows=%lld, width=%d (1 to %d)",
+                 (long long)rows, width, kNormMaxWidth);
+  const bool sums = dweight != nullptr || dbias != nullptr;
+  B200TA_REQUIRE(!sums || (workspace != nullptr && workspace_bytes >= b200ta_layer_norm_workspace_bytes(rows, width)),
+                 "layer_norm_backward: the workspace is too small");
+  if (!sums && dx == nullptr) return B200TA_OK;
+  DeviceState* st = nullptr;
+  int rc = get_device_state(&st);
+  if (rc != B200TA_OK) return rc;
+  NormParams p{};
+  p.x = x, p.dy = dy, p.w = weight, p.dx = dx, p.stats = static_cast<float2*>(const_cast<void*>(stats));
+  p.partial = sums ? static_cast<float*>(workspace) : nullptr;
+  p.xs = xs, p.dys = dys, p.dxs = dxs, p.rows = rows, p.width = width;
+  p.params_aligned = norm_aligned(weight, 0, 4);
+  const int bytes = norm_element_bytes(dtype), vec = 16 / bytes;
+  const bool whole = width % vec == 0 && norm_aligned(x, xs, bytes) && norm_aligned(dy, dys, bytes) &&
+                     (!dx || norm_aligned(dx, dxs, bytes)) && p.params_aligned;
+  const NormShape s = norm_shape(width, vec, 512, !whole);
+  p.lanes = s.lanes;
+  const int groups = s.threads / s.lanes, resident = grad_blocks_of(s.threads, s.items * vec);
+  const int joined = sums && groups > 1 ? groups / 2 * 2 * width * int(sizeof(float)) : 0;
+  const int ring = whole ? norm::stages_of(2 * s.items, s.threads, resident) * 2 * s.items * s.threads * 16 : 0;
+  const int smem = joined > ring ? joined : ring;
+  const int64_t need = (rows + groups - 1) / groups, most = int64_t(st->num_sms) * resident;
+  const int blocks = int(need < most ? need : most);
+  const bool f32 = param_dtype == B200TA_DTYPE_F32;
+  int (*launch)(DeviceState*, int, int, int, void*, const NormParams&);
+  if (dtype == B200TA_DTYPE_BF16) launch = f32 ? pick<__nv_bfloat16, float>(s) : pick<__nv_bfloat16, __nv_bfloat16>(s);
+  else if (dtype == B200TA_DTYPE_F16) launch = f32 ? pick<__half, float>(s) : pick<__half, __half>(s);
+  else launch = pick<float, float>(s);
+  rc = launch(st, blocks, s.threads, smem, stream, p);
+  if (rc != B200TA_OK || !sums) return rc;
+  const dim3 grid{unsigned((2 * width + 31) / 32)};
+  auto join = [&](auto* dw, auto* db) {
+    return launch_kernel(st, kKernelNorm, norm_join_kernel<std::remove_pointer_t<decltype(dw)>>, grid, 1024, 0, stream, p.partial, blocks,
+                         width, dw, db);
+  };
+  if (f32) return join(static_cast<float*>(dweight), static_cast<float*>(dbias));
+  if (param_dtype == B200TA_DTYPE_F16) return join(static_cast<__half*>(dweight), static_cast<__half*>(dbias));
+  return join(static_cast<__nv_bfloat16*>(dweight), static_cast<__nv_bfloat16*>(dbias));
+}
+
+}  // extern "C"

@@ -87,7 +87,7 @@ def check_norm(x, w, b, dy, eps=1e-5):
     within(db, want_db, 1.01 * pu * want_db.abs() + SUM * dy.double().abs().sum(0) + 1e-30, "dbias")
 
 
-NORM_SHAPES = [(1, 1), (1, 384), (2, 3), (3, 16), (7, 100), (5, 128), (300, 128), (65, 257), (33, 384), (17, 1001), (40, 1024),
+NORM_SHAPES = [(1, 1), (1, 384), (2, 3), (3, 16), (7, 100), (5, 128), (300, 128), (21, 40), (30, 200), (30, 203), (65, 257), (33, 384), (17, 1001), (40, 1024),
                (9, 2000), (6, 4100), (5, 8192), (3, 12288), (2, 16384), (2, 16383), (5000, 64), (1, 16384)]
 
 
@@ -279,9 +279,9 @@ def test_kept_and_computed_pre_activations(gated):
     check_layer(activation="gelu", keep=False, **given)
 
 
-@pytest.mark.parametrize("rows,K,N,gated", [(150000, 128, 512, True), (40000, 64, 1024, False), (120001, 24, 700, True)])
+@pytest.mark.parametrize("rows,K,N,gated", [(150000, 128, 512, True), (270001, 16, 1024, True), (300001, 24, 1000, False)])
 def test_rows_in_chunks(rows, K, N, gated):
-    """Enough rows that the backward pass of a narrow layer takes them in several chunks."""
+    """The last two have so many rows that the backward pass takes them in several chunks."""
     check_layer(activation="silu", **layer_inputs(rows, K, N, torch.bfloat16, gated, True, False))
 
 
