@@ -144,7 +144,7 @@ SIGNATURES: dict[str, tuple] = {
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
          c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int64, c_int, c_int, c_void_p],
     ),
-    "b200ta_copy_rows": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
+    "b200ta_copy_rows": (c_int, [c_void_p, c_int, c_void_p]),
 }
 
 

@@ -2,6 +2,7 @@
 // kernels beside them (few rows, dz from stored pre-activations, sums over rows, joining of parts, aligned copies).
 #include <algorithm>
 
+#include "layer_norm.cuh"
 #include "matmul.cuh"
 
 namespace b200ta {
@@ -84,7 +85,7 @@ int run_matmul(const Matmul& m, void* stream) {
   if (p.stages > matmul::kMaxStages) p.stages = matmul::kMaxStages;
   p.bias = m.bias;
   p.activation = m.activation;
-  p.has_aux = m.aux.base != nullptr, p.has_saved = m.saved.base != nullptr, p.accumulate = m.accumulate;
+  p.has_aux = m.aux.base != nullptr, p.has_saved = m.saved.base != nullptr, p.accumulate = m.accumulate, p.beside = m.beside;
   p.status = st->status_dev;
 
   MatmulMaps maps{};
@@ -94,8 +95,14 @@ int run_matmul(const Matmul& m, void* stream) {
               : map_of(&maps.b, m.b, 2, 64, uint32_t(p.pair || !two ? b_rows : units), two && !p.pair ? 2 : 1, SWZ_128, m.what);
   if (rc != B200TA_OK) return rc;
   const bool f32 = m.form == kPartial;
-  rc = map_of(&maps.out, m.out, f32 ? 4 : 2, f32 ? 16 : 32, 32, 1, SWZ_64, m.what);
-  if (rc != B200TA_OK) return rc;
+  const bool stored = f32 || ((reinterpret_cast<uintptr_t>(m.out.base) & 15u) == 0 && m.out.pitch % 8 == 0 &&
+                              (m.out.outer == 1 || m.out.outer_stride % 8 == 0));
+  if (!stored) {
+    B200TA_REQUIRE(m.form == kDense || m.form == kGated || m.form == kPlain, "%s: the result must be aligned", m.what);
+    p.direct = const_cast<void*>(m.out.base), p.direct_pitch = m.out.pitch, p.direct_outer = m.out.outer_stride;
+  } else if ((rc = map_of(&maps.out, m.out, f32 ? 4 : 2, f32 ? 16 : 32, 32, 1, SWZ_64, m.what)) != B200TA_OK) {
+    return rc;
+  }
   if (p.has_aux && (rc = map_of(&maps.aux, m.aux, 2, 32, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
   if (p.has_saved && (rc = map_of(&maps.saved, m.saved, 2, 32, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
   const int blocks = p.resident ? p.resident * p.tiles_n : std::min(p.work, p.pair ? st->num_sms / 2 : st->num_sms);
@@ -335,50 +342,69 @@ row_sum_kernel(const T* dz, long long pitch, long long rows, int N, long long pa
   }
 }
 
-// out[r][c] = sum over the parts, in their order.
+// out[r][c] = sum over the parts, in their order; two such results (dW and db) in one launch, either of which may be empty.
+struct JoinParams {
+  const float* part;
+  void* out;  // rows of `columns`, dense
+  long long part_stride, pitch, rows;
+  int parts, columns, blocks;
+};
 template <typename T>
 __global__ void __launch_bounds__(256)
-join_kernel(const float* part, int parts, long long part_stride, long long pitch, long long rows, int columns, T* out, long long out_pitch) {
+join_kernel(const JoinParams a, const JoinParams b) {
   pdl_trigger();
   pdl_wait();
-  const long long total = rows * columns;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long r = i / columns, c = i - r * columns;
-    const float* src = part + r * pitch + c;
+  const bool second = int(blockIdx.x) >= a.blocks;
+  const JoinParams& p = second ? b : a;
+  const long long total = p.rows * p.columns, first = (blockIdx.x - (second ? a.blocks : 0)) * 256LL + threadIdx.x;
+  for (long long i = first; i < total; i += p.blocks * 256LL) {
+    const long long r = i / p.columns, c = i - r * p.columns;
+    const float* src = p.part + r * p.pitch + c;
     float sum = 0.f;
 #pragma unroll 8
-    for (int s = 0; s < parts; ++s) sum += __ldg(src + s * part_stride);
-    out[r * out_pitch + c] = static_cast<T>(sum);
+    for (int s = 0; s < p.parts; ++s) sum += __ldg(src + s * p.part_stride);
+    static_cast<T*>(p.out)[i] = static_cast<T>(sum);
   }
 }
 
 // ---- aligned copies ---------------------------------------------------------------------------------------------------
 //
-// dst[r][c] = src[r * rs + c * cs] for 16-bit elements: tensors whose rows a TMA load or store cannot address (a pitch or
-// base that is no multiple of 16 bytes, columns that are not contiguous) pass through a padded copy.  [32 x 32] tiles turned
-// in shared memory where the rows are contiguous instead of the columns.
+// dst[r][c] = src[r * rs + c * cs] for 16-bit elements: tensors whose rows a TMA load cannot address (a pitch or base that is
+// no multiple of 16 bytes, columns that are not contiguous) pass through a padded copy, up to four in one launch.  A thread
+// makes a vector of eight columns, from two aligned loads shifted into place if they are contiguous, otherwise from eight
+// loads with neighbouring threads in neighbouring rows.  (An aligned 16-byte vector with a byte of the source in it lies in
+// the source's allocation.)
+struct CopyParams {
+  b200ta_copy job[B200TA_COPIES];
+  long long end[B200TA_COPIES];  // vectors up to and with this job
+  int jobs;
+};
 __global__ void __launch_bounds__(256)
-copy_rows_kernel(const uint16_t* src, long long rs, long long cs, uint16_t* dst, long long pitch, long long rows, int columns) {
-  __shared__ uint16_t tile[32][34];
+copy_rows_kernel(const CopyParams p) {
   pdl_trigger();
   pdl_wait();
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int tiles_c = (columns + 31) / 32;
-  const long long tiles = (rows + 31) / 32 * tiles_c;
-  const bool turn = cs != 1;
-  for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const long long r0 = t / tiles_c * 32;
-    const int c0 = int(t % tiles_c) * 32;
-    if (!turn) {
-      for (int i = ty; i < 32; i += 8)
-        if (r0 + i < rows && c0 + tx < columns) dst[(r0 + i) * pitch + c0 + tx] = src[(r0 + i) * rs + c0 + tx];
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < p.end[p.jobs - 1]; i += gridDim.x * 256LL) {
+    int k = 0;
+    while (i >= p.end[k]) ++k;
+    const b200ta_copy& job = p.job[k];
+    const long long v = i - (k == 0 ? 0 : p.end[k - 1]);
+    const int vectors = (job.columns + 7) / 8;
+    uint16_t* dst = static_cast<uint16_t*>(job.dst);
+    const uint16_t* src = static_cast<const uint16_t*>(job.src);
+    if (job.column_stride == 1) {
+      const long long r = v / vectors;
+      const int c = int(v - r * vectors) * 8, valid = job.columns - c;
+      *reinterpret_cast<uint4*>(dst + r * job.dst_row_stride + c) = norm::load<__half, true>(reinterpret_cast<const __half*>(src + r * job.row_stride + c), valid);
     } else {
-      for (int i = ty; i < 32; i += 8)
-        if (r0 + tx < rows && c0 + i < columns) tile[i][tx] = src[(r0 + tx) * rs + (c0 + i) * cs];
-      __syncthreads();
-      for (int i = ty; i < 32; i += 8)
-        if (r0 + i < rows && c0 + tx < columns) dst[(r0 + i) * pitch + c0 + tx] = tile[tx][i];
-      __syncthreads();
+      const long long c = v / job.rows * 8, r = v - v / job.rows * job.rows;
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = c + 2 * j < job.columns ? src[r * job.row_stride + (c + 2 * j) * job.column_stride] : 0u;
+        const uint32_t hi = c + 2 * j + 1 < job.columns ? src[r * job.row_stride + (c + 2 * j + 1) * job.column_stride] : 0u;
+        w[j] = lo | hi << 16;
+      }
+      *reinterpret_cast<uint4*>(dst + r * job.dst_row_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
@@ -418,7 +444,12 @@ Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns,
   }
   return best;
 }
-constexpr int kSumRows = 256;  // rows of a partial sum of db
+constexpr int kChunkRows = 256;  // chunks of the backward pass are multiples of this
+// Rows of a partial sum of db: enough blocks of 256 columns to fill the device a few times, at least 32 rows each.
+int sum_rows(int64_t rows, int64_t columns, int num_sms) {
+  const int64_t blocks = std::max<int64_t>(4 * num_sms / ((columns + 255) / 256), 1), each = (rows + blocks - 1) / blocks;
+  return int(std::min<int64_t>(std::max<int64_t>((each + 7) / 8 * 8, 32), 1024));
+}
 
 // The backward pass: how many rows at a time, and where its intermediates lie in the workspace.
 struct BackwardPlan {
@@ -426,6 +457,7 @@ struct BackwardPlan {
   int64_t dz_pitch;   // 0: dz is dy
   Split split;        // of a chunk's rows for dW
   bool direct;        // dW is written by its product
+  int rows_sum;       // rows of a partial sum of db
   int64_t dz, parts, sums, bytes;  // offsets, total
 };
 BackwardPlan plan_backward(bool gated, bool slope, int64_t rows, int K, int N, int num_sms) {
@@ -437,11 +469,11 @@ BackwardPlan plan_backward(bool gated, bool slope, int64_t rows, int K, int N, i
     // At most half a gigabyte of dz, in whole waves of row tiles.  (Chunks that L2 keeps do not pay: a gated layer 128 -> 512
     // over 147456 rows took 347 us in chunks of 39 MB, 300 us of 116 MB and 241 us in one, which writes dz to HBM and reads
     // it twice; each launch's first loads and last stores cost more.)
-    const int64_t wave = (int64_t(num_sms) * matmul::kBM + kSumRows - 1) / kSumRows * kSumRows;
+    const int64_t wave = (int64_t(num_sms) * matmul::kBM + kChunkRows - 1) / kChunkRows * kChunkRows;
     p.chunk = std::min(rows, std::max<int64_t>((int64_t(1) << 29) / (p.dz_pitch * 2) / wave, 1) * wave);
   }
   p.split = split_rows(p.chunk, N, outer, K, num_sms);
-  p.direct = p.chunk >= rows && p.split.parts == 1 && K % 8 == 0;
+  p.direct = p.chunk >= rows && p.split.parts == 1;
   auto take = [&](int64_t bytes) {
     const int64_t at = p.bytes;
     p.bytes += (bytes + 255) / 256 * 256;
@@ -449,7 +481,8 @@ BackwardPlan plan_backward(bool gated, bool slope, int64_t rows, int K, int N, i
   };
   p.dz = take(p.dz_pitch * (p.chunk < rows ? p.chunk : rows) * 2);
   p.parts = take(p.direct ? 0 : p.split.parts * outer * N * pad4(K) * int64_t(sizeof(float)));
-  p.sums = take((p.chunk + kSumRows - 1) / kSumRows * outer * pad8(N) * int64_t(sizeof(float)));
+  p.rows_sum = sum_rows(p.chunk, outer * N, num_sms);
+  p.sums = take((p.chunk + p.rows_sum - 1) / p.rows_sum * outer * pad8(N) * int64_t(sizeof(float)));
   return p;
 }
 
@@ -477,9 +510,9 @@ int b200ta_dense(const void* x, int64_t xs, const void* w, int64_t ws, const voi
     return launch_kernel(st, kKernelDenseHelpers, p.f16 ? pick_few<__half>(int(rows), vec, gated) : pick_few<__nv_bfloat16>(int(rows), vec, gated),
                          dim3(unsigned((N + 3) / 4)), 128, 0, stream, p);
   }
-  B200TA_REQUIRE(rows_aligned(x, xs) && rows_aligned(w, ws) && rows_aligned(y, ys) && (!residual || rows_aligned(residual, rs)) &&
+  B200TA_REQUIRE(rows_aligned(x, xs) && rows_aligned(w, ws) && (!residual || rows_aligned(residual, rs)) &&
                      (!saved || rows_aligned(saved, ss)),
-                 "dense: tensors must be 16-byte aligned with row strides that are multiples of 8 elements");
+                 "dense: what is read must be 16-byte aligned with row strides that are multiples of 8 elements");
   Matmul m;
   m.form = gated ? kGated : kDense;
   m.f16 = dtype == B200TA_DTYPE_F16;
@@ -512,9 +545,9 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
   int rc = check_layer("dense_backward", dtype, activation, rows, K, N);
   if (rc != B200TA_OK) return rc;
   B200TA_REQUIRE(dy && x && w, "dense_backward: NULL pointer");
-  B200TA_REQUIRE(rows_aligned(dy, dys) && rows_aligned(x, xs) && rows_aligned(w, ws) && (!dx || rows_aligned(dx, dxs)) &&
+  B200TA_REQUIRE(rows_aligned(dy, dys) && rows_aligned(x, xs) && rows_aligned(w, ws) &&
                      (!saved || (rows_aligned(saved, ss) && (!gated || ss % 16 == 0))),
-                 "dense_backward: tensors must be 16-byte aligned with row strides that are multiples of 8 elements");
+                 "dense_backward: what is read must be 16-byte aligned with row strides that are multiples of 8 elements");
   DeviceState* st = nullptr;
   rc = get_device_state(&st);
   if (rc != B200TA_OK) return rc;
@@ -529,7 +562,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
   float* sums = reinterpret_cast<float*>(ws_base + plan.sums);
   const int64_t sum_pitch = own_dz ? plan.dz_pitch : pad8(N);  // columns of dz that are summed, padding included
   const int sum_columns = int(own_dz ? plan.dz_pitch : N);
-  const bool direct = plan.direct && dw != nullptr && rows_aligned(dw, K);
+  const bool direct = plan.direct;
 
   for (int64_t r0 = 0; r0 < rows; r0 += plan.chunk) {
     const int64_t n = rows - r0 < plan.chunk ? rows - r0 : plan.chunk;
@@ -565,6 +598,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       m.a = {dz, n, N, zs, outer, zs / 2};
       m.b = {w, N, K, ws, outer, int64_t(N) * ws};
       m.out = {static_cast<char*>(dx) + r0 * dxs * 2, n, K, dxs};
+      if (dw != nullptr) m.beside = kBesideFirst;
       m.what = "dense_backward dx";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
     }
@@ -580,49 +614,53 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
         m.kblocks_split = plan.split.kblocks;
         m.accumulate = r0 > 0;  // each part is added to by one block at a time, the chunks in their order
       }
+      if (dx != nullptr) m.beside = kBesideSecond;
       m.what = "dense_backward dW";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
     }
     if (dbias != nullptr) {
-      const dim3 grid{unsigned((sum_columns + 255) / 256), unsigned((n + kSumRows - 1) / kSumRows)};
+      const dim3 grid{unsigned((sum_columns + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
       if (f16)
         rc = launch_kernel(st, kKernelDenseHelpers, row_sum_kernel<__half>, grid, 256, 0, stream, static_cast<const __half*>(dz), zs, n,
-                           sum_columns, sum_pitch, kSumRows, int(r0 > 0), sums);
+                           sum_columns, sum_pitch, plan.rows_sum, int(r0 > 0), sums);
       else
         rc = launch_kernel(st, kKernelDenseHelpers, row_sum_kernel<__nv_bfloat16>, grid, 256, 0, stream,
-                           static_cast<const __nv_bfloat16*>(dz), zs, n, sum_columns, sum_pitch, kSumRows, int(r0 > 0), sums);
+                           static_cast<const __nv_bfloat16*>(dz), zs, n, sum_columns, sum_pitch, plan.rows_sum, int(r0 > 0), sums);
       if (rc != B200TA_OK) return rc;
     }
   }
-  auto join = [&](const float* part, int64_t count, int64_t stride, int64_t pitch, int64_t n_rows, int columns, void* out) {
-    const int64_t need = (n_rows * columns + 255) / 256, most = int64_t(st->num_sms) * 16;
-    const dim3 grid{unsigned(need < most ? need : most)};
-    if (f16)
-      return launch_kernel(st, kKernelDenseHelpers, join_kernel<__half>, grid, 256, 0, stream, part, int(count), stride, pitch, n_rows,
-                           columns, static_cast<__half*>(out), int64_t(columns));
-    return launch_kernel(st, kKernelDenseHelpers, join_kernel<__nv_bfloat16>, grid, 256, 0, stream, part, int(count), stride, pitch,
-                         n_rows, columns, static_cast<__nv_bfloat16*>(out), int64_t(columns));
-  };
+  const bool parts_left = dw != nullptr && !direct;
+  if (!parts_left && dbias == nullptr) return B200TA_OK;
   const int64_t chunk = plan.chunk < rows ? plan.chunk : rows;
-  if (dw != nullptr && !direct) {
-    rc = join(parts, plan.split.parts, outer * N * pad4(K), pad4(K), outer * N, K, dw);
-    if (rc != B200TA_OK) return rc;
-  }
-  if (dbias != nullptr) rc = join(sums, (chunk + kSumRows - 1) / kSumRows, sum_pitch, sum_pitch / outer, outer, N, dbias);
-  return rc;
+  auto join_of = [&](bool wanted, const float* part, int64_t count, int64_t stride, int64_t pitch, int64_t n_rows, int columns, void* out) {
+    const int64_t need = (n_rows * columns + 255) / 256, most = int64_t(st->num_sms) * 16;
+    return JoinParams{part, out, stride, pitch, n_rows, int(count), columns, wanted ? int(std::min(need, most)) : 0};
+  };
+  const JoinParams a = join_of(parts_left, parts, plan.split.parts, outer * N * pad4(K), pad4(K), outer * N, K, dw);
+  const JoinParams b = join_of(dbias != nullptr, sums, (chunk + plan.rows_sum - 1) / plan.rows_sum, sum_pitch, sum_pitch / outer, outer, N, dbias);
+  return launch_kernel(st, kKernelDenseHelpers, f16 ? join_kernel<__half> : join_kernel<__nv_bfloat16>, dim3(unsigned(a.blocks + b.blocks)),
+                       256, 0, stream, a, b);
 }
 
-int b200ta_copy_rows(const void* src, int64_t row_stride, int64_t column_stride, void* dst, int64_t pitch, int64_t rows, int columns,
-                     void* stream) {
+int b200ta_copy_rows(const b200ta_copy* jobs, int count, void* stream) {
   using namespace b200ta;
-  B200TA_REQUIRE(src && dst, "copy_rows: NULL pointer");
-  B200TA_REQUIRE(rows > 0 && columns > 0, "copy_rows: rows=%lld, columns=%d", (long long)rows, columns);
+  B200TA_REQUIRE(jobs != nullptr && count > 0 && count <= B200TA_COPIES, "copy_rows: 1 to %d copies", B200TA_COPIES);
+  CopyParams p{};
+  p.jobs = count;
+  for (int i = 0; i < count; ++i) {
+    const b200ta_copy& job = p.job[i] = jobs[i];
+    B200TA_REQUIRE(job.src && job.dst, "copy_rows: NULL pointer");
+    B200TA_REQUIRE(job.rows > 0 && job.columns > 0, "copy_rows: rows=%lld, columns=%d", (long long)job.rows, job.columns);
+    B200TA_REQUIRE(rows_aligned(job.dst, job.dst_row_stride) && job.dst_row_stride >= pad8(job.columns),
+                   "copy_rows: dst must be 16-byte aligned with rows of at least %lld elements, a multiple of 8",
+                   (long long)pad8(job.columns));
+    p.end[i] = (i == 0 ? 0 : p.end[i - 1]) + job.rows * ((job.columns + 7) / 8);
+  }
   DeviceState* st = nullptr;
   const int rc = get_device_state(&st);
   if (rc != B200TA_OK) return rc;
-  const int64_t tiles = (rows + 31) / 32 * ((columns + 31) / 32), most = int64_t(st->num_sms) * 8;
-  return launch_kernel(st, kKernelDenseHelpers, copy_rows_kernel, dim3(unsigned(tiles < most ? tiles : most)), 256, 0, stream,
-                       static_cast<const uint16_t*>(src), row_stride, column_stride, static_cast<uint16_t*>(dst), pitch, rows, columns);
+  const int64_t need = (p.end[count - 1] + 255) / 256, most = int64_t(st->num_sms) * 16;
+  return launch_kernel(st, kKernelDenseHelpers, copy_rows_kernel, dim3(unsigned(need < most ? need : most)), 256, 0, stream, p);
 }
 
 }  // extern "C"

@@ -10,7 +10,8 @@
 //
 // An operand lies with k contiguous (K-major) or with its rows contiguous (MN-major): x and W as they are make the forward
 // product, dz and W that of dx, dz and x that of dW; nothing is transposed in memory.  Sizes are free (tiles past the edge
-// are zero-filled by the loads and clipped by the stores); base addresses and row pitches are multiples of 16 bytes.
+// are zero-filled by the loads and clipped by the stores); base addresses and row pitches of what is read are multiples of 16
+// bytes.
 //
 // A persistent block walks [128 x tile_n] tiles; with kPair two blocks of a cluster walk [256 x 256] tiles together, each
 // with its 128 rows of A and half of B (cta_group::2), which halves what a tile of B costs in shared memory and from L2.
@@ -19,7 +20,7 @@
 // 256 columns, one filled while the other is finished.  Where all of a column tile of B fits in half of the ring (64 KiB: 128
 // wide layers), it is loaded once and only A passes through the ring.  The finishing warps fetch what they read beside the
 // accumulators (residual, dy) by TMA a group ahead and store by TMA: a lane's own accesses to 32 rows occupy the load-store
-// unit for some 56 clocks.
+// unit for some 56 clocks.  Results whose rows TMA cannot address are stored from the same slabs, a row at a time.
 #pragma once
 
 #include <type_traits>
@@ -48,8 +49,15 @@ struct MatmulParams {
   int has_aux;                         // kDense: a residual
   int has_saved;                       // kDense, kGated: D + bias is stored as well
   int accumulate;                      // kPartial: add to what the parts hold
+  int beside;                          // kBesideFirst, kBesideSecond: see there
+  void* direct;                        // results that a TMA store cannot address: base, pitch and distance of the outer planes
+  long long direct_pitch, direct_outer;
   int* status;
 };
+
+// Two products that read the same dz run beside each other: the first lets its successor start only when what came before both
+// is complete, so the second does not wait for it, except at its end (whatever follows them waits for the second alone).
+enum { kBesideNone = 0, kBesideFirst, kBesideSecond };
 
 #ifdef __CUDACC__
 
@@ -198,6 +206,11 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[kN]) {
   for (int j = 0; j < kN; ++j) v[j] = __uint_as_float(r[j]);
 }
 
+__device__ __forceinline__ uint16_t lds16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
 __device__ __forceinline__ void tma_add_3d(const CUtensorMap* m, uint32_t src, int c0, int c1, int c2) {
   asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(m), "r"(src),
                "r"(c0), "r"(c1), "r"(c2)
@@ -292,6 +305,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   if (warp == 17) {
     if constexpr (kPair) tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
     else tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    if (p.beside == kBesideFirst) pdl_wait();
     pdl_trigger();
   }
   tc_fence_before();
@@ -312,7 +326,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     if (lane == 0) {
       tma_prefetch_desc(&tm_a);
       tma_prefetch_desc(&tm_b);
-      pdl_wait();
+      if (p.beside != kBesideSecond) pdl_wait();
       auto load = [&](uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
         if constexpr (kPair) tma_load_3d_pair(dst, m, bar, c0, c1, c2);
         else tma_load_3d(dst, m, bar, c0, c1, c2);
@@ -415,7 +429,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     }
   } else {
     // ------------------------------------------------------------------ finishing warps
-    pdl_wait();
+    if (p.beside != kBesideSecond) pdl_wait();
     const int quarter = warp >> 2, m = (warp & 3) * 32 + int(rank) * kBM;
     const uint32_t lane_acc = tmem_base + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t slabs = base + kSmSlabs + warp * 3 * kSlab, out_slabs = slabs + (kAux ? kSlab : 0);
@@ -454,6 +468,18 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < 4; ++j) sts128(slab + sw64_offset(lane, j), make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
+      if ((kForm == kDense || kForm == kGated || kForm == kPlain) && p.direct != nullptr && &map == &tm_out) {
+        __syncwarp();
+        const int rows = p.rows_inner - row < 32 ? p.rows_inner - row : 32;
+        T* to = static_cast<T*>(p.direct) + outer * p.direct_outer + (long long)row * p.direct_pitch + column + lane;
+        if (column + lane < p.columns)
+#pragma unroll 4
+          for (int i = 0; i < rows; ++i, to += p.direct_pitch)
+            *reinterpret_cast<uint16_t*>(to) = lds16(slab + sw64_offset(i, lane >> 3) + (lane & 7) * 2);
+        __syncwarp();
+        if (++slot == kRing) slot = 0;
+        return;
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -545,6 +571,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     }
     if (!ok && taken < loads) mbar_wait(aux_bar, taken & 1, abort_flag + 1);  // a load still in flight
     if (lane == 0) tma_store_wait_all();
+    if (p.beside == kBesideSecond) pdl_wait();
   }
 
   __syncwarp();
@@ -581,6 +608,7 @@ struct Matmul {
   int activation = kActNone;
   int kblocks_split = 0;  // blocks of 64 of a part (kPartial); 0: all of them
   bool accumulate = false;
+  int beside = kBesideNone;
   const char* what = "matmul";
 };
 int run_matmul(const Matmul& m, void* stream);

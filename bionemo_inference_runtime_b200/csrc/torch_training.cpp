@@ -88,33 +88,30 @@ Rows plain_rows(const at::Tensor& t) {
 bool tma_takes(const void* ptr, int64_t rows, int64_t columns, int64_t stride) {
   return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0 && stride % 8 == 0 && (rows == 1 || stride >= columns);
 }
-// Rows that a TMA load can address; `few`: any alignment will do.
-Rows operand(const at::Tensor& t, bool few) {
+// Collects the aligned copies of a call's operands and makes them in one launch.
+struct Copies {
+  b200ta_copy jobs[B200TA_COPIES];
+  at::Tensor held[B200TA_COPIES];  // the sources, until the launch
+  int count = 0;
+  void make() const {
+    if (count > 0) check(lib.copy_rows(jobs, count, stream()), "b200ta_copy_rows");
+  }
+};
+// Rows that a TMA load can address (`few`: any alignment will do), a copy if they are not.
+Rows operand(const at::Tensor& t, bool few, Copies& copies) {
   Rows r = rows_of(t);
   if (r.column_stride == 1 && (few || tma_takes(r.ptr, r.rows, r.columns, r.stride))) return r;
   const at::Tensor copy = at::empty({r.rows, pad8(r.columns)}, t.options().memory_format(c10::MemoryFormat::Contiguous));
-  check(lib.copy_rows(r.ptr, r.stride, r.column_stride, copy.data_ptr(), copy.stride(0), r.rows, int(r.columns), stream()),
-        "b200ta_copy_rows");
+  copies.jobs[copies.count++] = {r.ptr, r.stride, r.column_stride, copy.data_ptr(), copy.stride(0), r.rows, int(r.columns)};
+  copies.held[copies.count - 1] = r.held;
   return {copy, copy.data_ptr(), r.rows, r.columns, copy.stride(0), 1};
 }
 
-// Where a result goes: the tensor itself, or a padded one that finish() copies from.
-struct Result {
-  at::Tensor out, padded;
-  Rows rows;
-  void finish() const {
-    if (!padded.defined()) return;
-    const Rows r = rows_of(out);
-    check(lib.copy_rows(padded.data_ptr(), padded.stride(0), 1, r.ptr, r.stride, r.rows, int(r.columns), stream()), "b200ta_copy_rows");
-  }
-};
-Result result_in(const at::Tensor& out, bool few) {
+// Where a result goes: contiguous columns, rows with one stride.
+Rows result_in(const at::Tensor& out) {
   Rows r = rows_of(out);
   if (r.held.data_ptr() != out.data_ptr() || r.column_stride != 1) refuse("out must have contiguous columns and rows with one stride");
-  if (r.rows == 1) r.stride = pad8(r.columns);
-  if (few || tma_takes(r.ptr, r.rows, r.columns, r.stride)) return {out, {}, r};
-  const at::Tensor padded = at::empty({r.rows, pad8(r.columns)}, out.options().memory_format(c10::MemoryFormat::Contiguous));
-  return {out, padded, {padded, padded.data_ptr(), r.rows, r.columns, padded.stride(0), 1}};
+  return r;
 }
 at::Tensor empty_rows(const at::Tensor& x, int64_t columns) {
   std::vector<int64_t> shape = x.sizes().vec();
@@ -161,9 +158,9 @@ std::pair<at::Tensor, Maybe> layer_norm(const at::Tensor& x, const Maybe& weight
   if (want_stats) stats = at::empty({rows, 2}, x.options().dtype(at::kFloat).memory_format(c10::MemoryFormat::Contiguous));
   if (rows == 0) return {y, stats};
   const Rows r = plain_rows(x);
-  const Result to = result_in(y, true);
+  const Rows to = result_in(y);
   const Maybe w = weight ? Maybe(weight->contiguous()) : Maybe(), b = bias ? Maybe(bias->contiguous()) : Maybe();
-  check(lib.layer_norm(r.ptr, r.stride, pointer(w), pointer(b), params, to.rows.ptr, to.rows.stride, pointer(stats), dtype, rows, width,
+  check(lib.layer_norm(r.ptr, r.stride, pointer(w), pointer(b), params, to.ptr, to.stride, pointer(stats), dtype, rows, width,
                        float(eps), stream()),
         "b200ta_layer_norm");
   return {y, stats};
@@ -229,15 +226,15 @@ std::pair<at::Tensor, Maybe> dense(const at::Tensor& x, const at::Tensor& w, con
   if (want_saved && lib.dense_keeps(int(activation), gated, l.K)) saved = at::empty({l.rows, pitch}, x.options().memory_format(c10::MemoryFormat::Contiguous));
   if (l.rows == 0) return {y, saved};
   const bool few = l.rows <= lib.dense_few_rows();
-  const Rows rx = operand(x, few), rw = operand(w, few);
-  const Result to = result_in(y, few);
+  Copies copies;
+  const Rows rx = operand(x, few, copies), rw = operand(w, few, copies), to = result_in(y);
   Rows rr{};
-  if (residual) rr = operand(*residual, few);
+  if (residual) rr = operand(*residual, few, copies);
+  copies.make();
   const Maybe b = bias ? Maybe(bias->contiguous()) : Maybe();
-  check(lib.dense(rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), residual ? rr.ptr : nullptr, rr.stride, to.rows.ptr, to.rows.stride,
+  check(lib.dense(rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), residual ? rr.ptr : nullptr, rr.stride, to.ptr, to.stride,
                   pointer(saved), pitch, l.dtype, int(activation), gated, l.rows, l.K, l.N, stream()),
         "b200ta_dense");
-  to.finish();
   return {y, saved};
 }
 
@@ -263,17 +260,16 @@ std::tuple<Maybe, Maybe, Maybe> dense_backward(const at::Tensor& dy, const at::T
     if (dbias) dbias->zero_();
     return {dx, dweight, dbias};
   }
-  const Rows rdy = operand(dy, false), rx = operand(x, false), rw = operand(w, false);
-  Result to{};
-  if (dx) to = result_in(*dx, false);
+  Copies copies;
+  const Rows rdy = operand(dy, false, copies), rx = operand(x, false, copies), rw = operand(w, false, copies);
+  copies.make();
   const Maybe b = bias ? Maybe(bias->contiguous()) : Maybe();
   const size_t need = lib.dense_backward_workspace_bytes(int(activation), gated, l.rows, l.K, l.N);
   const at::Tensor workspace = bytes(x, need);
   check(lib.dense_backward(rdy.ptr, rdy.stride, rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), pointer(saved), pitch,
-                           dx ? to.rows.ptr : nullptr, to.rows.stride, pointer(dweight), pointer(dbias), workspace.data_ptr(), need,
+                           pointer(dx), l.K, pointer(dweight), pointer(dbias), workspace.data_ptr(), need,
                            l.dtype, int(activation), gated, l.rows, l.K, l.N, stream()),
         "b200ta_dense_backward");
-  if (dx) to.finish();
   return {dx, dweight, dbias};
 }
 

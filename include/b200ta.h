@@ -436,8 +436,8 @@ int b200ta_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void
 /* y[rows, N] = act(x w^T + bias) + residual, x [rows, K], w [N, K]; or with `gated`, w [2 N, K] (value rows, then gate rows),
  * y = value * act(gate), [value | gate] = x w^T + bias.  bf16 or fp16.  bias and residual (not for a gated layer) may be NULL.
  * `saved` (may be NULL) receives x w^T + bias for the backward pass, [rows, N] or [rows, 2, saved_row_stride / 2].
- * Up to b200ta_dense_few_rows() rows, any strides and alignment; otherwise base addresses are 16-byte aligned and row strides
- * multiples of 8 elements (sizes are free). */
+ * Up to b200ta_dense_few_rows() rows, any strides and alignment; otherwise x, w, residual and saved are 16-byte aligned with row
+ * strides that are multiples of 8 elements (sizes are free, and so is y). */
 int b200ta_dense_few_rows(void);
 int b200ta_dense(const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride, const void* bias, const void* residual,
                  int64_t residual_row_stride, void* y, int64_t y_row_stride, void* saved, int64_t saved_row_stride, int dtype,
@@ -447,18 +447,26 @@ int b200ta_dense(const void* x, int64_t x_row_stride, const void* w, int64_t w_r
 int b200ta_dense_keeps(int activation, int gated, int K);
 
 /* Gradients of the same: dx [rows, K], dw [N or 2 N, K] and dbias [N or 2 N], both dense; each may be NULL.  The
- * pre-activations are taken from `saved`, or computed again from x, w and bias if it is NULL.  Alignment as above, dw and
- * dbias free; the workspace is 256-byte aligned. */
+ * pre-activations are taken from `saved`, or computed again from x, w and bias if it is NULL.  Alignment of what is
+ * read as above, results free; the workspace is 256-byte aligned. */
 size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int64_t rows, int K, int N);
 int b200ta_dense_backward(const void* dy, int64_t dy_row_stride, const void* x, int64_t x_row_stride, const void* w,
                           int64_t w_row_stride, const void* bias, const void* saved, int64_t saved_row_stride, void* dx,
                           int64_t dx_row_stride, void* dw, void* dbias, void* workspace, size_t workspace_bytes, int dtype,
                           int activation, int gated, int64_t rows, int K, int N, void* stream);
 
-/* dst[r, c] = src[r * row_stride + c * column_stride] for 16-bit elements, dst with rows `dst_row_stride` apart: aligned
- * copies of what the entry points above cannot take as it lies, and the way back. */
-int b200ta_copy_rows(const void* src, int64_t row_stride, int64_t column_stride, void* dst, int64_t dst_row_stride, int64_t rows,
-                     int columns, void* stream);
+/* dst[r, c] = src[r * row_stride + c * column_stride] for 16-bit elements: aligned copies of what the entry points above cannot
+ * read as it lies, up to B200TA_COPIES of them in one launch.  dst is 16-byte aligned, its rows a multiple of 8 elements apart and
+ * padded to 8 columns (the padding is written). */
+#define B200TA_COPIES 4
+typedef struct {
+  const void* src;
+  int64_t row_stride, column_stride;
+  void* dst;
+  int64_t dst_row_stride, rows;
+  int columns;
+} b200ta_copy;
+int b200ta_copy_rows(const b200ta_copy* jobs, int count, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,8 +15,8 @@ CSRC = Path(build.__file__).resolve().parent
 def test_matmul_kernel_lets_the_next_kernel_start_behind_its_allocation():
     """The rule of the other tensor-memory kernels, for the one that is a template in a header."""
     text = (CSRC / "matmul.cuh").read_text()
-    assert text.count("tmem_alloc(") == 1 and text.count("pdl_trigger()") == 1
-    assert re.search(r"tmem_alloc\(.*\);\s*pdl_trigger\(\);", text)
+    assert text.count("tmem_alloc(") == 1 and text.count("tmem_alloc_pair(") == 2 and text.count("pdl_trigger()") == 1
+    assert re.search(r"tmem_alloc_pair\(.*\);\s*else tmem_alloc\(.*\);\s*if \(.*\) pdl_wait\(\);\s*pdl_trigger\(\);", text)
 
 
 def test_every_wait_of_the_matmul_kernel_is_bounded():
@@ -33,8 +33,8 @@ def test_entry_points_refuse_before_any_cuda_call():
         _lib.call("b200ta_dense", None, 8, None, 8, None, None, 0, None, 8, None, 0, 0, 99, 0, 4, 8, 8, None)
     with pytest.raises(ValueError, match="NULL"):
         _lib.call("b200ta_dense_backward", None, 8, None, 8, None, 8, None, None, 0, None, 8, None, None, None, 0, 0, 0, 0, 4, 8, 8, None)
-    with pytest.raises(ValueError, match="rows"):
-        _lib.call("b200ta_copy_rows", 16, 8, 1, 32, 8, 0, 8, None)
+    with pytest.raises(ValueError, match="copies"):
+        _lib.call("b200ta_copy_rows", None, 0, None)
 
 
 def test_host_tensors_and_unknown_activations_are_refused():
