@@ -21,32 +21,40 @@ int map_of(CUtensorMap* map, const Plane& t, int bytes, uint32_t columns, uint32
 // a tile costs its finishing if that is more; all blocks take as many tiles as the busiest.
 struct Tiling {
   int tile_n, pair, resident;
+  double clocks;
 };
-Tiling choose_tiling(const Matmul& m, int64_t rows, int64_t m_outer, int64_t columns, int kblocks, int splits, int num_sms) {
+struct TilingOf {
+  MatmulForm form;
+  bool a_mn, sums;  // sums of A over k: tiles of up to 128 columns
+  int64_t rows, outer, columns;
+  int kblocks, splits;
+};
+Tiling choose_tiling(const TilingOf& m, int num_sms) {
   const bool two = m.form == kGated || m.form == kGatedGrad;
-  const int64_t accumulated = two ? columns * 2 : columns;
+  const int64_t accumulated = two ? m.columns * 2 : m.columns;
   const double finish = m.form == kGatedGrad ? 12 : two ? 8 : 6.5;  // clocks for an accumulator column of 128 rows
-  Tiling best{128, 0, 0};
-  double least = 1e300;
-  auto consider = [&](Tiling t, double waves, double main, double columns_of_tile) {
-    const double cost = waves * std::max(main, finish * columns_of_tile) + std::min(main, finish * columns_of_tile) + 1500;
-    if (cost < least * 0.98) least = cost, best = t;
+  Tiling best{128, 0, 0, 1e300};
+  auto consider = [&](int n, int pair, int resident, double waves, double main) {
+    const double end = finish * n, cost = waves * std::max(main, end) + std::min(main, end) + 1500;
+    if (cost < best.clocks * 0.98) best = {n, pair, resident, cost};
   };
   auto waves_of = [](int64_t items, int64_t blocks) { return double((items + blocks - 1) / blocks); };
-  for (int n = 256; n >= 64; n /= 2) {
+  const int64_t tiles_m = (m.rows + 127) / 128 * m.outer;
+  for (int n = m.sums ? 128 : 256; n >= 64; n /= 2) {
     if (n > 64 && n / 2 >= accumulated) continue;
-    const int64_t tiles_m = (rows + 127) / 128 * m_outer, tiles_n = (accumulated + n - 1) / n;
+    const int64_t tiles_n = (accumulated + n - 1) / n;
     const double mma = 4.0 * std::max(40.0, n * 0.54);
-    if (!m.a_mn && splits == 1 && kblocks * n * matmul::kBK * 2 <= matmul::kResidentBytes && tiles_n <= num_sms) {
+    if (!m.a_mn && m.splits == 1 && m.kblocks * n * matmul::kBK * 2 <= matmul::kResidentBytes && tiles_n <= num_sms) {
       const int64_t lanes = std::min(tiles_m, num_sms / tiles_n);
-      consider({n, 0, int(lanes)}, waves_of(tiles_m, lanes), kblocks * std::max(mma, 356.0), n);
+      consider(n, 0, int(lanes), waves_of(tiles_m, lanes), m.kblocks * std::max(mma, 356.0));
     } else {
-      consider({n, 0, 0}, waves_of(tiles_m * tiles_n * splits, num_sms), kblocks * std::max(mma, (n == 256 ? 1.2 : 1.0) * (16384 + n * 128) / 46), n);
+      const double load = (n == 256 ? 1.2 : 1.0) * (16384 + n * 128) / 46;
+      consider(n, 0, 0, waves_of(tiles_m * tiles_n * m.splits, num_sms), m.kblocks * std::max(mma, load));
     }
   }
-  if (rows > matmul::kBM && accumulated > 128) {
-    const int64_t tiles = (rows + 255) / 256 * m_outer * splits * ((accumulated + 255) / 256);
-    consider({256, 1, 0}, waves_of(tiles, num_sms / 2), kblocks * 712.0, 256);
+  if (m.rows > matmul::kBM && accumulated > 128 && !m.sums) {
+    const int64_t tiles = (m.rows + 255) / 256 * m.outer * m.splits * ((accumulated + 255) / 256);
+    consider(256, 1, 0, waves_of(tiles, num_sms / 2), m.kblocks * 712.0);
   }
   return best;
 }
@@ -68,7 +76,7 @@ int run_matmul(const Matmul& m, void* stream) {
   p.kblocks_split = m.kblocks_split > 0 && m.kblocks_split < p.kblocks ? m.kblocks_split : p.kblocks;
   p.splits = (p.kblocks + p.kblocks_split - 1) / p.kblocks_split;
   p.rows_inner = int(rows), p.columns = int(columns);
-  const Tiling tiling = choose_tiling(m, rows, m_outer, columns, p.kblocks_split, p.splits, st->num_sms);
+  const Tiling tiling = choose_tiling({m.form, m.a_mn, m.sums != nullptr, rows, m_outer, columns, p.kblocks_split, p.splits}, st->num_sms);
   p.tile_n = tiling.tile_n, p.pair = tiling.pair, p.resident = tiling.resident;
   const int tile_m = p.pair ? 2 * matmul::kBM : matmul::kBM;
   p.tiles_m_inner = int((rows + tile_m - 1) / tile_m);
@@ -85,7 +93,7 @@ int run_matmul(const Matmul& m, void* stream) {
   if (p.stages > matmul::kMaxStages) p.stages = matmul::kMaxStages;
   p.bias = m.bias;
   p.activation = m.activation;
-  p.has_aux = m.aux.base != nullptr, p.has_saved = m.saved.base != nullptr, p.accumulate = m.accumulate, p.beside = m.beside;
+  p.has_aux = m.aux.base != nullptr, p.has_saved = m.saved.base != nullptr, p.accumulate = m.accumulate, p.beside = m.beside, p.sums = m.sums;
   p.status = st->status_dev;
 
   MatmulMaps maps{};
@@ -107,6 +115,9 @@ int run_matmul(const Matmul& m, void* stream) {
   if (p.has_saved && (rc = map_of(&maps.saved, m.saved, 2, 32, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
   const int blocks = p.resident ? p.resident * p.tiles_n : std::min(p.work, p.pair ? st->num_sms / 2 : st->num_sms);
   const int grid = p.pair ? 2 * blocks : blocks;
+  // Two sets of finishing warps are out of step, so that one computes while the other loads and stores, and a warp's waits
+  // serve twice the columns; a block's only tile is for all of them.
+  p.alternate = p.resident ? p.tiles_m > p.resident : p.work > blocks;
   if (m.form == kDenseGrad || m.form == kGatedGrad) return launch_matmul_grad(st, m, maps, p, grid, stream);
   if (m.b_mn) return launch_matmul_product(st, m, maps, p, grid, stream);
   return launch_matmul_forward(st, m, maps, p, grid, stream);
@@ -421,26 +432,26 @@ int check_layer(const char* what, int dtype, int activation, int64_t rows, int K
   return B200TA_OK;
 }
 
-// How dW = dz^T x is cut along the rows: enough parts to give every SM a tile, few enough that reading them again stays
-// small.  A tile takes some 550 clocks per 64 rows and 256 columns, its store and start some 3000; parts are written and read
-// once at some 3400 bytes a clock.
+// How dW = dz^T x is cut along the rows, and whether db comes from the same product (sums of dz by MMAs with ones, which only
+// tiles of up to 128 columns have room for) or from a pass over dz of its own.  Parts are written and read once and sums read
+// dz once more at some 2400 bytes a clock; a launch more costs some 4000 clocks.
 struct Split {
   int kblocks, parts;  // of a part; in all
+  bool sums;           // db from the product
 };
-Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns, int num_sms) {
-  const int64_t kblocks = (rows + matmul::kBK - 1) / matmul::kBK;
-  const int64_t tiles_m = (n_rows + 127) / 128 * n_outer;
-  const int tile_n = columns > 128 ? 256 : columns > 64 ? 128 : 64;
-  const int64_t tiles = tiles_m * ((columns + tile_n - 1) / tile_n);
-  Split best{int(kblocks), 1};
+Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns, bool want_sums, int num_sms) {
+  const int64_t kblocks = (rows + matmul::kBK - 1) / matmul::kBK, values = n_rows * n_outer;
+  Split best{int(kblocks), 1, false};
   double least = 1e300;
-  for (int64_t parts = 1; parts <= 256 && parts <= kblocks; ++parts) {
-    const int64_t per = (kblocks + parts - 1) / parts;
-    if ((kblocks + per - 1) / per != parts) continue;
-    const double waves = double((tiles * parts + num_sms - 1) / num_sms);
-    const double bytes = parts == 1 ? 0 : 8.0 * double(parts) * double(n_rows * n_outer) * double(columns);
-    const double cost = waves * (double(per) * 550 * tile_n / 256 + 3000) + bytes / 3400;
-    if (cost < least) least = cost, best = {int(per), int(parts)};
+  for (int64_t tried = 1; tried <= 256 && tried <= kblocks; tried += tried < 8 ? 1 : tried < 32 ? 4 : tried < 64 ? 8 : 16) {
+    const int64_t per = (kblocks + tried - 1) / tried, parts = (kblocks + per - 1) / per;
+    for (int sums = 0; sums <= int(want_sums); ++sums) {
+      const MatmulForm form = parts > 1 ? kPartial : kPlain;
+      double cost = choose_tiling({form, true, sums != 0, n_rows, n_outer, columns, int(per), int(parts)}, num_sms).clocks;
+      if (parts > 1) cost += 4000 + 8.0 * double(parts) * double(values) * double(columns) / 2400;
+      if (want_sums && !sums) cost += (parts > 1 ? 4000 : 8000) + 2.0 * double(values) * double(rows) / 2400;
+      if (cost < least * 0.98) least = cost, best = {int(per), int(parts), sums != 0};
+    }
   }
   return best;
 }
@@ -460,7 +471,7 @@ struct BackwardPlan {
   int rows_sum;       // rows of a partial sum of db
   int64_t dz, parts, sums, bytes;  // offsets, total
 };
-BackwardPlan plan_backward(bool gated, bool slope, int64_t rows, int K, int N, int num_sms) {
+BackwardPlan make_plan(bool gated, bool slope, bool want_dbias, int64_t rows, int K, int N, int num_sms) {
   BackwardPlan p{};
   const int64_t outer = gated ? 2 : 1;
   p.dz_pitch = gated || slope ? outer * pad8(N) : 0;
@@ -472,7 +483,7 @@ BackwardPlan plan_backward(bool gated, bool slope, int64_t rows, int K, int N, i
     const int64_t wave = (int64_t(num_sms) * matmul::kBM + kChunkRows - 1) / kChunkRows * kChunkRows;
     p.chunk = std::min(rows, std::max<int64_t>((int64_t(1) << 29) / (p.dz_pitch * 2) / wave, 1) * wave);
   }
-  p.split = split_rows(p.chunk, N, outer, K, num_sms);
+  p.split = split_rows(p.chunk, N, outer, K, want_dbias, num_sms);
   p.direct = p.chunk >= rows && p.split.parts == 1;
   auto take = [&](int64_t bytes) {
     const int64_t at = p.bytes;
@@ -482,8 +493,25 @@ BackwardPlan plan_backward(bool gated, bool slope, int64_t rows, int K, int N, i
   p.dz = take(p.dz_pitch * (p.chunk < rows ? p.chunk : rows) * 2);
   p.parts = take(p.direct ? 0 : p.split.parts * outer * N * pad4(K) * int64_t(sizeof(float)));
   p.rows_sum = sum_rows(p.chunk, outer * N, num_sms);
-  p.sums = take((p.chunk + p.rows_sum - 1) / p.rows_sum * outer * pad8(N) * int64_t(sizeof(float)));
+  const int64_t slots = p.split.sums ? p.split.parts : (p.chunk + p.rows_sum - 1) / p.rows_sum;
+  p.sums = take(!want_dbias || (p.split.sums && p.direct) ? 0 : slots * outer * pad8(N) * int64_t(sizeof(float)));
   return p;
+}
+// The plan is a function of the sizes; the last few of a thread are kept, since making one takes longer than a launch.
+const BackwardPlan& plan_backward(bool gated, bool slope, bool want_dbias, int64_t rows, int K, int N, int num_sms) {
+  struct Entry {
+    int64_t rows = -1;
+    int K, N, flags, num_sms;
+    BackwardPlan plan;
+  };
+  thread_local Entry entries[16];
+  const int flags = gated | slope << 1 | want_dbias << 2;
+  Entry& e = entries[(uint64_t(rows) * 31 + uint64_t(K) * 7 + uint64_t(N) * 3 + flags) % 16];
+  if (e.rows != rows || e.K != K || e.N != N || e.flags != flags || e.num_sms != num_sms) {
+    e.plan = make_plan(gated, slope, want_dbias, rows, K, N, num_sms);
+    e.rows = rows, e.K = K, e.N = N, e.flags = flags, e.num_sms = num_sms;
+  }
+  return e.plan;
 }
 
 }  // namespace
@@ -531,11 +559,11 @@ int b200ta_dense_keeps(int activation, int gated, int K) {
   return (gated || activation != b200ta::kActNone) && K >= 512;
 }
 
-size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int64_t rows, int K, int N) {
+size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int want_dbias, int64_t rows, int K, int N) {
   using namespace b200ta;
   DeviceState* st = nullptr;
   if (rows <= 0 || K <= 0 || N <= 0 || get_device_state(&st) != B200TA_OK) return 0;
-  return size_t(plan_backward(gated, activation != kActNone, rows, K, N, st->num_sms).bytes);
+  return size_t(plan_backward(gated, activation != kActNone, want_dbias, rows, K, N, st->num_sms).bytes);
 }
 
 int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias,
@@ -551,7 +579,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
   DeviceState* st = nullptr;
   rc = get_device_state(&st);
   if (rc != B200TA_OK) return rc;
-  const BackwardPlan plan = plan_backward(gated, activation != kActNone, rows, K, N, st->num_sms);
+  const BackwardPlan& plan = plan_backward(gated, activation != kActNone, dbias != nullptr, rows, K, N, st->num_sms);
   B200TA_REQUIRE(plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
                                      workspace_bytes >= size_t(plan.bytes)),
                  "dense_backward: the workspace must be 256-byte aligned and of %lld bytes", (long long)plan.bytes);
@@ -602,6 +630,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       m.what = "dense_backward dx";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
     }
+    const bool product_sums = plan.split.sums && dw != nullptr && dbias != nullptr;
     if (dw != nullptr) {
       Matmul m;
       m.form = direct ? kPlain : kPartial, m.a_mn = m.b_mn = true, m.f16 = f16;
@@ -615,10 +644,11 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
         m.accumulate = r0 > 0;  // each part is added to by one block at a time, the chunks in their order
       }
       if (dx != nullptr) m.beside = kBesideSecond;
+      if (product_sums) m.sums = direct ? dbias : sums;
       m.what = "dense_backward dW";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
     }
-    if (dbias != nullptr) {
+    if (dbias != nullptr && !product_sums) {
       const dim3 grid{unsigned((sum_columns + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
       if (f16)
         rc = launch_kernel(st, kKernelDenseHelpers, row_sum_kernel<__half>, grid, 256, 0, stream, static_cast<const __half*>(dz), zs, n,
@@ -629,15 +659,17 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       if (rc != B200TA_OK) return rc;
     }
   }
-  const bool parts_left = dw != nullptr && !direct;
-  if (!parts_left && dbias == nullptr) return B200TA_OK;
+  const bool product_sums = plan.split.sums && dw != nullptr;
+  const bool parts_left = dw != nullptr && !direct, sums_left = dbias != nullptr && !(product_sums && direct);
+  if (!parts_left && !sums_left) return B200TA_OK;
   const int64_t chunk = plan.chunk < rows ? plan.chunk : rows;
   auto join_of = [&](bool wanted, const float* part, int64_t count, int64_t stride, int64_t pitch, int64_t n_rows, int columns, void* out) {
     const int64_t need = (n_rows * columns + 255) / 256, most = int64_t(st->num_sms) * 16;
     return JoinParams{part, out, stride, pitch, n_rows, int(count), columns, wanted ? int(std::min(need, most)) : 0};
   };
   const JoinParams a = join_of(parts_left, parts, plan.split.parts, outer * N * pad4(K), pad4(K), outer * N, K, dw);
-  const JoinParams b = join_of(dbias != nullptr, sums, (chunk + plan.rows_sum - 1) / plan.rows_sum, sum_pitch, sum_pitch / outer, outer, N, dbias);
+  const JoinParams b = product_sums ? join_of(sums_left, sums, plan.split.parts, outer * N, N, outer, N, dbias)
+                                    : join_of(sums_left, sums, (chunk + plan.rows_sum - 1) / plan.rows_sum, sum_pitch, sum_pitch / outer, outer, N, dbias);
   return launch_kernel(st, kKernelDenseHelpers, f16 ? join_kernel<__half> : join_kernel<__nv_bfloat16>, dim3(unsigned(a.blocks + b.blocks)),
                        256, 0, stream, a, b);
 }

@@ -15,7 +15,7 @@
 //
 // A persistent block walks [128 x tile_n] tiles; with kPair two blocks of a cluster walk [256 x 256] tiles together, each
 // with its 128 rows of A and half of B (cta_group::2), which halves what a tile of B costs in shared memory and from L2.
-// Warp roles (576 threads): warps 0-15 finish tiles (TMEM lane = row; each takes every fourth group of 32 columns), warp 16
+// Warp roles (576 threads): warps 0-15 finish tiles (TMEM lane = row, groups of 32 columns), warp 16
 // loads [128 x 64] and [tile_n x 64] operand blocks by TMA into a ring, warp 17 issues tcgen05.mma into two accumulators of
 // 256 columns, one filled while the other is finished.  Where all of a column tile of B fits in half of the ring (64 KiB: 128
 // wide layers), it is loaded once and only A passes through the ring.  The finishing warps fetch what they read beside the
@@ -49,7 +49,10 @@ struct MatmulParams {
   int has_aux;                         // kDense: a residual
   int has_saved;                       // kDense, kGated: D + bias is stored as well
   int accumulate;                      // kPartial: add to what the parts hold
+  int alternate;                       // the finishing warps take tiles in two sets, in turn
   int beside;                          // kBesideFirst, kBesideSecond: see there
+  void* sums;                          // kPlain, kPartial with MN-major A, tiles of up to 128: sums of A over k, [outer][rows] in
+                                       // the operands' type (kPartial: [split][outer][rows] in 32 bits), or NULL
   void* direct;                        // results that a TMA store cannot address: base, pitch and distance of the outer planes
   long long direct_pitch, direct_outer;
   int* status;
@@ -71,7 +74,8 @@ constexpr int kResidentBytes = 65536;      // of them for a resident B
 constexpr int kMaxStages = 7;
 constexpr int kSlab = 2048;                // 32 rows of 64 bytes
 constexpr int kSmSlabs = kRingBytes;       // three for each finishing warp
-constexpr int kSmBars = kSmSlabs + kFinishers * 3 * kSlab;
+constexpr int kSmOnes = kSmSlabs + kFinishers * 3 * kSlab;  // an operand block of ones, [16 x 16]
+constexpr int kSmBars = kSmOnes + 512;
 enum Bar {
   FULL = 0, EMPTY = kMaxStages, ACC_FULL = 2 * kMaxStages, ACC_EMPTY = ACC_FULL + 2, B_FULL = ACC_EMPTY + 2, AUX = B_FULL + 1,
   NUM_BARS = AUX + kFinishers
@@ -278,6 +282,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   constexpr bool kGrad = kForm == kDenseGrad || kForm == kGatedGrad;
   constexpr bool kAux = kGrad || kForm == kDense;                // a warp's first slab receives residual or dy
   constexpr int kRing = kAux ? 2 : 3;                            // the others hold results
+  constexpr bool kSums = kAMn && !kPair;                         // sums of A over k may be wanted
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -296,11 +301,16 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bars + (ACC_FULL + i) * 8, 1);
-      mbar_init(bars + (ACC_EMPTY + i) * 8, kPair ? 2 * kFinishers : kFinishers);
+      mbar_init(bars + (ACC_EMPTY + i) * 8, (kPair ? 2 * kFinishers : kFinishers) >> p.alternate);
     }
     mbar_init(bars + B_FULL * 8, 1);
     for (int i = 0; i < kFinishers; ++i) mbar_init(bars + (AUX + i) * 8, 1);
     fence_mbar_init();
+  }
+  if (kSums && p.sums != nullptr && threadIdx.x < 128) {
+    const uint32_t one = __is_same(T, __half) ? 0x3C003C00u : 0x3F803F80u;
+    reinterpret_cast<uint32_t*>(gen + kSmOnes)[threadIdx.x] = one;
+    fence_proxy_async_smem();
   }
   if (warp == 17) {
     if constexpr (kPair) tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
@@ -418,6 +428,12 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
             if constexpr (kPair) umma_ss_pair_warp(acc, dak, dbk, id, add);
             else umma_ss_warp(acc, dak, dbk, id, add);
           }
+          if (kSums && p.sums != nullptr && t.n0 == 0) {  // A times a block of ones, into 16 columns of their own
+            const uint32_t id_ones = idesc(__is_same(T, __half), kBM, 16, kAMn, false);
+            const uint64_t ones = smem_desc<16, 256, kLayoutSw32>(base + kSmOnes);
+#pragma unroll
+            for (int k = 0; k < kBK / 16; ++k) umma_ss_warp(acc + 128, da + k * 128, ones, id_ones, (kb > t.kb0 || k > 0) ? 1u : 0u);
+          }
           if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + stage) * 8);
           else umma_commit_warp(bars + (EMPTY + stage) * 8);
           if (++stage == p.stages) stage = 0, phase ^= 1u;
@@ -430,31 +446,35 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   } else {
     // ------------------------------------------------------------------ finishing warps
     if (p.beside != kBesideSecond) pdl_wait();
-    const int quarter = warp >> 2, m = (warp & 3) * 32 + int(rank) * kBM;
+    // All of them on every tile, each with every fourth group of 32 result columns; or (alternate) eight on the even tiles and
+    // eight on the odd ones, with every second group.
+    const int first_i = p.alternate ? warp >> 3 : 0, step_i = 1 + p.alternate;
+    const int first_g = p.alternate ? (warp >> 2) & 1 : warp >> 2, step_g = p.alternate ? 2 : 4;
+    const int m = (warp & 3) * 32 + int(rank) * kBM;
     const uint32_t lane_acc = tmem_base + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t slabs = base + kSmSlabs + warp * 3 * kSlab, out_slabs = slabs + (kAux ? kSlab : 0);
     const uint32_t aux_bar = bars + (AUX + warp) * 8;
     const bool has_aux = kGrad || (kForm == kDense && p.has_aux);
     const T* bias = static_cast<const T*>(p.bias);
-    // groups of 32 result columns of an item; this warp takes every fourth
+    // groups of 32 result columns of an item
     auto groups_of = [&](const Item& t) {
       if (t.m0 + m >= p.rows_inner) return 0;
       const int left = p.columns - t.n0;
       return ((left < units ? left : units) + 31) / 32;
     };
     // residual or dy: the load of the next group runs while this one is finished
-    int next_i = 0, next_g = quarter, next_groups = -1;
+    int next_i = first_i, next_g = first_g, next_groups = -1;
     Item next{};
     uint32_t loads = 0, taken = 0;
     auto load_aux = [&]() {
-      for (; next_i < items; ++next_i, next_g = quarter, next_groups = -1) {
+      for (; next_i < items; next_i += step_i, next_g = first_g, next_groups = -1) {
         if (next_groups < 0) next = item_of<kPair, kAMn>(p, next_i, units), next_groups = groups_of(next);
         if (next_g >= next_groups) continue;
         if (lane == 0) {
           mbar_expect_tx(aux_bar, kSlab);
           tma_load_3d(slabs, &tm_aux, aux_bar, next.n0 + next_g * 32, next.m0 + m, 0);
         }
-        ++loads, next_g += 4;
+        ++loads, next_g += step_g;
         return;
       }
     };
@@ -498,15 +518,29 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     };
 
     bool ok = true;
-    for (int i = 0; ok && i < items; ++i) {
+    for (int i = first_i; ok && i < items; i += step_i) {
       const Item t = item_of<kPair, kAMn>(p, i, units);
       const int groups = groups_of(t), row = t.m0 + m;
       ok = mbar_wait_warp(bars + (ACC_FULL + (i & 1)) * 8, (i >> 1) & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
       const uint32_t acc = lane_acc + (i & 1) * 256;
-      if (quarter >= groups) release(i);
-      for (int g = quarter; g < groups; g += 4) {
+      if (kSums && p.sums != nullptr && t.n0 == 0 && first_g == 0 && groups > 0) {
+        float sum[16];
+        tmem_load(acc + 128, sum);
+        tmem_ld_wait();
+        if (row + lane < p.rows_inner) {
+          if constexpr (kForm == kPartial) {
+            const int outer = t.split * (p.tiles_m / p.tiles_m_inner) + t.m_outer;
+            float* to = static_cast<float*>(p.sums) + (long long)outer * p.rows_inner + row + lane;
+            *to = p.accumulate ? *to + sum[0] : sum[0];
+          } else {
+            static_cast<T*>(p.sums)[(long long)t.m_outer * p.rows_inner + row + lane] = static_cast<T>(sum[0]);
+          }
+        }
+      }
+      if (first_g >= groups) release(i);
+      for (int g = first_g; g < groups; g += step_g) {
         const int n = t.n0 + g * 32;
         uint32_t aux[16];
         if constexpr (kAux) {
@@ -533,7 +567,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           tmem_load(acc + g * 32 + kFirst, v);
           if constexpr (kTwo) tmem_load(acc + units + g * 32 + kFirst, gate);
           tmem_ld_wait();
-          if (kFirst + kStep == 32 && g + 4 >= groups) release(i);
+          if (kFirst + kStep == 32 && g + step_g >= groups) release(i);
           if constexpr (kForm == kPartial) {
             uint32_t x[16];
 #pragma unroll
@@ -609,6 +643,7 @@ struct Matmul {
   int kblocks_split = 0;  // blocks of 64 of a part (kPartial); 0: all of them
   bool accumulate = false;
   int beside = kBesideNone;
+  void* sums = nullptr;  // see MatmulParams
   const char* what = "matmul";
 };
 int run_matmul(const Matmul& m, void* stream);
