@@ -138,7 +138,7 @@ SIGNATURES: dict[str, tuple] = {
          c_int, c_int64, c_int, c_int, c_void_p],
     ),
     "b200ta_dense_keeps": (c_int, [c_int, c_int, c_int]),
-    "b200ta_dense_backward_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int64, c_int, c_int]),
+    "b200ta_dense_backward_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int64, c_int, c_int]),
     "b200ta_dense_backward": (
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,

@@ -250,57 +250,84 @@ auto pick_few(int rows, bool vec, bool two) {
 
 // ---- dz from stored pre-activations ---------------------------------------------------------------------------------
 //
-// dz = dy act'(z), or [dy act(g) | dy v act'(g)]: reads 2 (3) and writes 1 (2) planes, bound by HBM.  Eight columns a thread.
+// dz = dy act'(z), or [dy act(g) | dy v act'(g)]: reads 2 (3) and writes 1 (2) planes, bound by HBM.  A block takes 256 columns
+// of some rows, a thread eight columns of every eighth of them, whose sums (db) it has on the way: part[block.y][column] (+)=
+// theirs, of the values before they are rounded.
 struct SlopeParams {
   const void *dy, *saved;
   void* dz;
-  long long dys, ss, zs, rows;
-  int N;
+  float* part;  // or NULL
+  long long dys, ss, zs, rows, part_pitch;
+  int N, rows_block, accumulate;
 };
+// The sums of the block's threads with the same columns, to the workspace.
+__device__ __forceinline__ void store_sums(const float (&s)[8], float (&joined)[8][256 + 4], float* part, int columns, bool accumulate) {
+  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) joined[k][lane * 8 + j] = s[j];
+  __syncthreads();
+  if (int(threadIdx.x) < columns) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += joined[i][threadIdx.x];
+    part[threadIdx.x] = accumulate ? part[threadIdx.x] + sum : sum;
+  }
+  __syncthreads();
+}
 template <typename T, int kAct, bool kTwo>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, kTwo ? 3 : 4)
 slope_kernel(const SlopeParams p) {
+  __shared__ float joined[8][256 + 4];
   pdl_trigger();
   pdl_wait();
-  const int vectors = (p.N + 7) / 8;
-  const long long total = p.rows * vectors;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long row = i / vectors;
-    const int c = int(i - row * vectors) * 8;
-    const T* dy = static_cast<const T*>(p.dy) + row * p.dys + c;
-    const T* z = static_cast<const T*>(p.saved) + row * p.ss + c;
-    T* dz = static_cast<T*>(p.dz) + row * p.zs + c;
-    float d[8], v[8], g[8];
-    if (c + 8 <= p.N) {
-      load_vec<T, 8>(dy, d);
-      load_vec<T, 8>(z, v);
-      if constexpr (kTwo) load_vec<T, 8>(z + p.ss / 2, g);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool in = c + j < p.N;
-        d[j] = in ? static_cast<float>(dy[j]) : 0.f, v[j] = in ? static_cast<float>(z[j]) : 0.f;
-        if constexpr (kTwo) g[j] = in ? static_cast<float>(z[p.ss / 2 + j]) : 0.f;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      float a0, a1, s0, s1;
-      if constexpr (kTwo) {
-        activate2<kAct, true>(g[j], g[j + 1], a0, a1, s0, s1);
-        g[j] = d[j] * v[j] * s0, g[j + 1] = d[j + 1] * v[j + 1] * s1;
-        v[j] = d[j] * a0, v[j + 1] = d[j + 1] * a1;
+  const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
+  const long long r0 = (long long)blockIdx.y * p.rows_block, r1 = r0 + p.rows_block < p.rows ? r0 + p.rows_block : p.rows;
+  float sv[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sg[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (c < p.N) {
+#pragma unroll 1
+    for (long long row = r0 + (threadIdx.x >> 5); row < r1; row += 8) {
+      const T* dy = static_cast<const T*>(p.dy) + row * p.dys + c;
+      const T* z = static_cast<const T*>(p.saved) + row * p.ss + c;
+      T* dz = static_cast<T*>(p.dz) + row * p.zs + c;
+      float d[8], v[8], g[8];
+      if (c + 8 <= p.N) {
+        load_vec<T, 8>(dy, d);
+        load_vec<T, 8>(z, v);
+        if constexpr (kTwo) load_vec<T, 8>(z + p.ss / 2, g);
       } else {
-        activate2<kAct, true>(v[j], v[j + 1], a0, a1, s0, s1);
-        v[j] = d[j] * s0, v[j + 1] = d[j + 1] * s1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = c + j < p.N;
+          d[j] = in ? static_cast<float>(dy[j]) : 0.f, v[j] = in ? static_cast<float>(z[j]) : 0.f;
+          if constexpr (kTwo) g[j] = in ? static_cast<float>(z[p.ss / 2 + j]) : 0.f;
+        }
       }
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        float a0, a1, s0, s1;
+        if constexpr (kTwo) {
+          activate2<kAct, true>(g[j], g[j + 1], a0, a1, s0, s1);
+          g[j] = d[j] * v[j] * s0, g[j + 1] = d[j + 1] * v[j + 1] * s1;
+          v[j] = d[j] * a0, v[j + 1] = d[j + 1] * a1;
+          sg[j] += g[j], sg[j + 1] += g[j + 1];
+        } else {
+          activate2<kAct, true>(v[j], v[j + 1], a0, a1, s0, s1);
+          v[j] = d[j] * s0, v[j + 1] = d[j + 1] * s1;
+        }
+        sv[j] += v[j], sv[j + 1] += v[j + 1];
+      }
+      // (dz's rows are padded to eight columns: its last vector is stored whole)
+      *reinterpret_cast<uint4*>(dz) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+      if constexpr (kTwo)
+        *reinterpret_cast<uint4*>(dz + p.zs / 2) =
+            make_uint4(pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3]), pack2<T>(g[4], g[5]), pack2<T>(g[6], g[7]));
     }
-    // (dz's rows are padded to eight columns: its last vector is stored whole)
-    *reinterpret_cast<uint4*>(dz) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-    if constexpr (kTwo)
-      *reinterpret_cast<uint4*>(dz + p.zs / 2) =
-          make_uint4(pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3]), pack2<T>(g[4], g[5]), pack2<T>(g[6], g[7]));
   }
+  if (p.part == nullptr) return;
+  float* part = p.part + (long long)blockIdx.y * p.part_pitch + blockIdx.x * 256;
+  const int columns = p.N - int(blockIdx.x) * 256;
+  store_sums(sv, joined, part, columns, p.accumulate);
+  if constexpr (kTwo) store_sums(sg, joined, part + p.zs / 2, columns, p.accumulate);
 }
 template <typename T, bool kTwo>
 auto pick_slope(int activation) {
@@ -323,12 +350,12 @@ row_sum_kernel(const T* dz, long long pitch, long long rows, int N, long long pa
   __shared__ float joined[8][256 + 4];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 256 + lane * 8;
+  const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const long long r0 = (long long)blockIdx.y * rows_block, r1 = r0 + rows_block < rows ? r0 + rows_block : rows;
   if (c < N) {
 #pragma unroll 4
-    for (long long r = r0 + k; r < r1; r += 8) {
+    for (long long r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
       float v[8];
       if (c + 8 <= N) {
         load_vec<T, 8>(dz + r * pitch + c, v);
@@ -340,41 +367,43 @@ row_sum_kernel(const T* dz, long long pitch, long long rows, int N, long long pa
       for (int j = 0; j < 8; ++j) s[j] += v[j];
     }
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) joined[k][lane * 8 + j] = s[j];
-  __syncthreads();
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n < N) {
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum += joined[i][threadIdx.x];
-    float* dst = part + (long long)blockIdx.y * part_pitch + n;
-    *dst = accumulate ? *dst + sum : sum;
-  }
+  store_sums(s, joined, part + (long long)blockIdx.y * part_pitch + blockIdx.x * 256, N - int(blockIdx.x) * 256, accumulate);
 }
 
-// out[r][c] = sum over the parts, in their order; two such results (dW and db) in one launch, either of which may be empty.
+// out[r][c] = sum over the parts, in a fixed order; two such results (dW and db) in one launch, either of which may be empty.
+// A thread sums one value, or eight threads do where there are many parts of few values.
 struct JoinParams {
   const float* part;
   void* out;  // rows of `columns`, dense
   long long part_stride, pitch, rows;
-  int parts, columns, blocks;
+  int parts, columns, slices, blocks;  // slices: threads of a value, 1 or 8
 };
 template <typename T>
 __global__ void __launch_bounds__(256)
 join_kernel(const JoinParams a, const JoinParams b) {
+  __shared__ float joined[8][33];
   pdl_trigger();
   pdl_wait();
   const bool second = int(blockIdx.x) >= a.blocks;
   const JoinParams& p = second ? b : a;
-  const long long total = p.rows * p.columns, first = (blockIdx.x - (second ? a.blocks : 0)) * 256LL + threadIdx.x;
-  for (long long i = first; i < total; i += p.blocks * 256LL) {
-    const long long r = i / p.columns, c = i - r * p.columns;
+  const int values = 256 / p.slices, slice = p.slices == 1 ? 0 : threadIdx.x >> 5, lane = p.slices == 1 ? threadIdx.x : threadIdx.x & 31;
+  const long long total = p.rows * p.columns;
+  for (long long i0 = (blockIdx.x - (second ? a.blocks : 0)) * (long long)values; i0 < total; i0 += (long long)p.blocks * values) {
+    const long long i = i0 + lane, r = i / p.columns, c = i - r * p.columns;
     const float* src = p.part + r * p.pitch + c;
     float sum = 0.f;
+    if (i < total)
 #pragma unroll 8
-    for (int s = 0; s < p.parts; ++s) sum += __ldg(src + s * p.part_stride);
-    static_cast<T*>(p.out)[i] = static_cast<T>(sum);
+      for (int s = slice; s < p.parts; s += p.slices) sum += __ldg(src + s * p.part_stride);
+    if (p.slices > 1) {
+      joined[slice][lane] = sum;
+      __syncthreads();
+      if (slice == 0)
+#pragma unroll
+        for (int s = 1; s < 8; ++s) sum += joined[s][lane];
+      __syncthreads();
+    }
+    if (slice == 0 && i < total) static_cast<T*>(p.out)[i] = static_cast<T>(sum);
   }
 }
 
@@ -433,13 +462,13 @@ int check_layer(const char* what, int dtype, int activation, int64_t rows, int K
 }
 
 // How dW = dz^T x is cut along the rows, and whether db comes from the same product (sums of dz by MMAs with ones, which only
-// tiles of up to 128 columns have room for) or from a pass over dz of its own.  Parts are written and read once and sums read
+// tiles of up to 128 columns have room for) or from a pass over dz: its own, or the one that forms dz from kept values.  Parts are written and read once and sums read
 // dz once more at some 2400 bytes a clock; a launch more costs some 4000 clocks.
 struct Split {
   int kblocks, parts;  // of a part; in all
   bool sums;           // db from the product
 };
-Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns, bool want_sums, int num_sms) {
+Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns, bool want_sums, bool kept, int num_sms) {
   const int64_t kblocks = (rows + matmul::kBK - 1) / matmul::kBK, values = n_rows * n_outer;
   Split best{int(kblocks), 1, false};
   double least = 1e300;
@@ -449,7 +478,7 @@ Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns,
       const MatmulForm form = parts > 1 ? kPartial : kPlain;
       double cost = choose_tiling({form, true, sums != 0, n_rows, n_outer, columns, int(per), int(parts)}, num_sms).clocks;
       if (parts > 1) cost += 4000 + 8.0 * double(parts) * double(values) * double(columns) / 2400;
-      if (want_sums && !sums) cost += (parts > 1 ? 4000 : 8000) + 2.0 * double(values) * double(rows) / 2400;
+      if (want_sums && !sums) cost += (parts > 1 ? 0 : 4000) + (kept ? 0 : 4000 + 2.0 * double(values) * double(rows) / 2400);
       if (cost < least * 0.98) least = cost, best = {int(per), int(parts), sums != 0};
     }
   }
@@ -458,7 +487,7 @@ Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns,
 constexpr int kChunkRows = 256;  // chunks of the backward pass are multiples of this
 // Rows of a partial sum of db: enough blocks of 256 columns to fill the device a few times, at least 32 rows each.
 int sum_rows(int64_t rows, int64_t columns, int num_sms) {
-  const int64_t blocks = std::max<int64_t>(4 * num_sms / ((columns + 255) / 256), 1), each = (rows + blocks - 1) / blocks;
+  const int64_t blocks = std::max<int64_t>(8 * num_sms / ((columns + 255) / 256), 1), each = (rows + blocks - 1) / blocks;
   return int(std::min<int64_t>(std::max<int64_t>((each + 7) / 8 * 8, 32), 1024));
 }
 
@@ -471,7 +500,7 @@ struct BackwardPlan {
   int rows_sum;       // rows of a partial sum of db
   int64_t dz, parts, sums, bytes;  // offsets, total
 };
-BackwardPlan make_plan(bool gated, bool slope, bool want_dbias, int64_t rows, int K, int N, int num_sms) {
+BackwardPlan make_plan(bool gated, bool slope, bool kept, bool want_dbias, int64_t rows, int K, int N, int num_sms) {
   BackwardPlan p{};
   const int64_t outer = gated ? 2 : 1;
   p.dz_pitch = gated || slope ? outer * pad8(N) : 0;
@@ -483,7 +512,7 @@ BackwardPlan make_plan(bool gated, bool slope, bool want_dbias, int64_t rows, in
     const int64_t wave = (int64_t(num_sms) * matmul::kBM + kChunkRows - 1) / kChunkRows * kChunkRows;
     p.chunk = std::min(rows, std::max<int64_t>((int64_t(1) << 29) / (p.dz_pitch * 2) / wave, 1) * wave);
   }
-  p.split = split_rows(p.chunk, N, outer, K, want_dbias, num_sms);
+  p.split = split_rows(p.chunk, N, outer, K, want_dbias, kept, num_sms);
   p.direct = p.chunk >= rows && p.split.parts == 1;
   auto take = [&](int64_t bytes) {
     const int64_t at = p.bytes;
@@ -492,23 +521,23 @@ BackwardPlan make_plan(bool gated, bool slope, bool want_dbias, int64_t rows, in
   };
   p.dz = take(p.dz_pitch * (p.chunk < rows ? p.chunk : rows) * 2);
   p.parts = take(p.direct ? 0 : p.split.parts * outer * N * pad4(K) * int64_t(sizeof(float)));
-  p.rows_sum = sum_rows(p.chunk, outer * N, num_sms);
+  p.rows_sum = sum_rows(p.chunk, N, num_sms);
   const int64_t slots = p.split.sums ? p.split.parts : (p.chunk + p.rows_sum - 1) / p.rows_sum;
   p.sums = take(!want_dbias || (p.split.sums && p.direct) ? 0 : slots * outer * pad8(N) * int64_t(sizeof(float)));
   return p;
 }
 // The plan is a function of the sizes; the last few of a thread are kept, since making one takes longer than a launch.
-const BackwardPlan& plan_backward(bool gated, bool slope, bool want_dbias, int64_t rows, int K, int N, int num_sms) {
+const BackwardPlan& plan_backward(bool gated, bool slope, bool kept, bool want_dbias, int64_t rows, int K, int N, int num_sms) {
   struct Entry {
     int64_t rows = -1;
     int K, N, flags, num_sms;
     BackwardPlan plan;
   };
   thread_local Entry entries[16];
-  const int flags = gated | slope << 1 | want_dbias << 2;
+  const int flags = gated | slope << 1 | want_dbias << 2 | kept << 3;
   Entry& e = entries[(uint64_t(rows) * 31 + uint64_t(K) * 7 + uint64_t(N) * 3 + flags) % 16];
   if (e.rows != rows || e.K != K || e.N != N || e.flags != flags || e.num_sms != num_sms) {
-    e.plan = make_plan(gated, slope, want_dbias, rows, K, N, num_sms);
+    e.plan = make_plan(gated, slope, kept, want_dbias, rows, K, N, num_sms);
     e.rows = rows, e.K = K, e.N = N, e.flags = flags, e.num_sms = num_sms;
   }
   return e.plan;
@@ -559,11 +588,11 @@ int b200ta_dense_keeps(int activation, int gated, int K) {
   return (gated || activation != b200ta::kActNone) && K >= 512;
 }
 
-size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int want_dbias, int64_t rows, int K, int N) {
+size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, int64_t rows, int K, int N) {
   using namespace b200ta;
   DeviceState* st = nullptr;
   if (rows <= 0 || K <= 0 || N <= 0 || get_device_state(&st) != B200TA_OK) return 0;
-  return size_t(plan_backward(gated, activation != kActNone, want_dbias, rows, K, N, st->num_sms).bytes);
+  return size_t(plan_backward(gated, activation != kActNone, kept != 0, want_dbias != 0, rows, K, N, st->num_sms).bytes);
 }
 
 int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias,
@@ -579,7 +608,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
   DeviceState* st = nullptr;
   rc = get_device_state(&st);
   if (rc != B200TA_OK) return rc;
-  const BackwardPlan& plan = plan_backward(gated, activation != kActNone, dbias != nullptr, rows, K, N, st->num_sms);
+  const BackwardPlan& plan = plan_backward(gated, activation != kActNone, saved != nullptr, dbias != nullptr, rows, K, N, st->num_sms);
   B200TA_REQUIRE(plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
                                      workspace_bytes >= size_t(plan.bytes)),
                  "dense_backward: the workspace must be 256-byte aligned and of %lld bytes", (long long)plan.bytes);
@@ -590,7 +619,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
   float* sums = reinterpret_cast<float*>(ws_base + plan.sums);
   const int64_t sum_pitch = own_dz ? plan.dz_pitch : pad8(N);  // columns of dz that are summed, padding included
   const int sum_columns = int(own_dz ? plan.dz_pitch : N);
-  const bool direct = plan.direct;
+  const bool direct = plan.direct, product_sums = plan.split.sums && dw != nullptr && dbias != nullptr;
 
   for (int64_t r0 = 0; r0 < rows; r0 += plan.chunk) {
     const int64_t n = rows - r0 < plan.chunk ? rows - r0 : plan.chunk;
@@ -602,12 +631,13 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       void* dst = ws_base + plan.dz;
       dz = dst, zs = plan.dz_pitch;
       if (saved != nullptr) {
-        const SlopeParams p{dy_c, static_cast<const char*>(saved) + r0 * ss * 2, dst, dys, ss, zs, n, N};
-        const int64_t need = (n * ((N + 7) / 8) + 255) / 256, most = int64_t(st->num_sms) * 16;
+        const SlopeParams p{dy_c, static_cast<const char*>(saved) + r0 * ss * 2, dst, dbias != nullptr && !product_sums ? sums : nullptr, dys, ss, zs, n,
+                            sum_pitch, N, plan.rows_sum, r0 > 0};
+        const dim3 grid{unsigned((N + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
         void (*kernel)(SlopeParams);
         if (f16) kernel = gated ? pick_slope<__half, true>(activation) : pick_slope<__half, false>(activation);
         else kernel = gated ? pick_slope<__nv_bfloat16, true>(activation) : pick_slope<__nv_bfloat16, false>(activation);
-        rc = launch_kernel(st, kKernelDenseHelpers, kernel, dim3(unsigned(need < most ? need : most)), 256, 0, stream, p);
+        rc = launch_kernel(st, kKernelDenseHelpers, kernel, grid, 256, 0, stream, p);
       } else {
         Matmul m;
         m.form = gated ? kGatedGrad : kDenseGrad, m.f16 = f16;
@@ -630,7 +660,6 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       m.what = "dense_backward dx";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
     }
-    const bool product_sums = plan.split.sums && dw != nullptr && dbias != nullptr;
     if (dw != nullptr) {
       Matmul m;
       m.form = direct ? kPlain : kPartial, m.a_mn = m.b_mn = true, m.f16 = f16;
@@ -648,7 +677,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       m.what = "dense_backward dW";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
     }
-    if (dbias != nullptr && !product_sums) {
+    if (dbias != nullptr && !product_sums && saved == nullptr) {
       const dim3 grid{unsigned((sum_columns + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
       if (f16)
         rc = launch_kernel(st, kKernelDenseHelpers, row_sum_kernel<__half>, grid, 256, 0, stream, static_cast<const __half*>(dz), zs, n,
@@ -659,13 +688,13 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       if (rc != B200TA_OK) return rc;
     }
   }
-  const bool product_sums = plan.split.sums && dw != nullptr;
   const bool parts_left = dw != nullptr && !direct, sums_left = dbias != nullptr && !(product_sums && direct);
   if (!parts_left && !sums_left) return B200TA_OK;
   const int64_t chunk = plan.chunk < rows ? plan.chunk : rows;
   auto join_of = [&](bool wanted, const float* part, int64_t count, int64_t stride, int64_t pitch, int64_t n_rows, int columns, void* out) {
-    const int64_t need = (n_rows * columns + 255) / 256, most = int64_t(st->num_sms) * 16;
-    return JoinParams{part, out, stride, pitch, n_rows, int(count), columns, wanted ? int(std::min(need, most)) : 0};
+    const int slices = count > 8 && n_rows * columns < 256 * 1024 ? 8 : 1;
+    const int64_t need = (n_rows * columns * slices + 255) / 256, most = int64_t(st->num_sms) * 16;
+    return JoinParams{part, out, stride, pitch, n_rows, int(count), columns, slices, wanted ? int(std::min(need, most)) : 0};
   };
   const JoinParams a = join_of(parts_left, parts, plan.split.parts, outer * N * pad4(K), pad4(K), outer * N, K, dw);
   const JoinParams b = product_sums ? join_of(sums_left, sums, plan.split.parts, outer * N, N, outer, N, dbias)

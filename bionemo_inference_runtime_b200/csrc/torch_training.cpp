@@ -264,7 +264,7 @@ std::tuple<Maybe, Maybe, Maybe> dense_backward(const at::Tensor& dy, const at::T
   const Rows rdy = operand(dy, false, copies), rx = operand(x, false, copies), rw = operand(w, false, copies);
   copies.make();
   const Maybe b = bias ? Maybe(bias->contiguous()) : Maybe();
-  const size_t need = lib.dense_backward_workspace_bytes(int(activation), gated, want_dbias, l.rows, l.K, l.N);
+  const size_t need = lib.dense_backward_workspace_bytes(int(activation), gated, saved.has_value(), want_dbias, l.rows, l.K, l.N);
   const at::Tensor workspace = bytes(x, need);
   check(lib.dense_backward(rdy.ptr, rdy.stride, rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), pointer(saved), pitch,
                            pointer(dx), l.K, pointer(dweight), pointer(dbias), workspace.data_ptr(), need,
