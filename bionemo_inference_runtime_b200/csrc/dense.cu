@@ -128,15 +128,16 @@ namespace {
 // ---- few rows ---------------------------------------------------------------------------------------------------
 //
 // Up to 16 rows: the weights are read once and that bounds the call, or its latency does.  A warp takes one result column (a
-// value and a gate row of W for kGated), its lanes run along k with 16-byte loads, the rows' sums are exchanged so that each
-// row's ends in a lane of its own.  128-row tiles of the tensor cores would leave all but N / 64 SMs idle.
+// value and a gate row of W for kGated), or two, four or eight warps do where there are few columns; its lanes run along k with
+// 16-byte loads, the rows' sums are exchanged so that each row's ends in a lane of its own.  128-row tiles of the tensor cores
+// would leave all but N / 64 SMs idle.
 constexpr int kFewRows = 16;
 
 struct FewParams {
   const void *x, *w, *bias, *residual;
   void *y, *saved;
   long long xs, ws, rs, ys, ss;
-  int rows, K, N, activation, gated, f16;
+  int rows, K, N, activation, warps;  // warps: of a column
 };
 
 template <typename T, int kVec>
@@ -183,32 +184,37 @@ __device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
   return v[0];
 }
 
+constexpr int kFewWarps = 8;  // of a block
 template <typename T, int kRows, int kVec, bool kTwo>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kFewWarps * 32)
 few_rows_kernel(const FewParams p) {
+  __shared__ float joined[2][kFewWarps][32];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, n = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (n >= p.N) return;
-  const T* x = static_cast<const T*>(p.x);
-  const T* w = static_cast<const T*>(p.w) + n * p.ws;
-  const T* wg = static_cast<const T*>(p.w) + (long long)(n + p.N) * p.ws;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % p.warps;
+  const int n = blockIdx.x * (kFewWarps / p.warps) + warp / p.warps;
+  const bool in = n < p.N;
   float acc[kRows], gate[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) acc[r] = 0.f, gate[r] = 0.f;
+  if (in) {
+    const T* x = static_cast<const T*>(p.x);
+    const T* w = static_cast<const T*>(p.w) + n * p.ws;
+    const T* wg = static_cast<const T*>(p.w) + (long long)(n + p.N) * p.ws;
 #pragma unroll 2
-  for (int k = lane * kVec; k < p.K; k += 32 * kVec) {
-    float a[kVec], b[kVec], c[kVec];
-    load_vec<T, kVec>(w + k, a);
-    if constexpr (kTwo) load_vec<T, kVec>(wg + k, b);
+    for (int k = (part * 32 + lane) * kVec; k < p.K; k += p.warps * 32 * kVec) {
+      float a[kVec], b[kVec], c[kVec];
+      load_vec<T, kVec>(w + k, a);
+      if constexpr (kTwo) load_vec<T, kVec>(wg + k, b);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      if (r < p.rows) {
-        load_vec<T, kVec>(x + r * p.xs + k, c);
+      for (int r = 0; r < kRows; ++r) {
+        if (r < p.rows) {
+          load_vec<T, kVec>(x + r * p.xs + k, c);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          acc[r] = fmaf(a[e], c[e], acc[r]);
-          if constexpr (kTwo) gate[r] = fmaf(b[e], c[e], gate[r]);
+          for (int e = 0; e < kVec; ++e) {
+            acc[r] = fmaf(a[e], c[e], acc[r]);
+            if constexpr (kTwo) gate[r] = fmaf(b[e], c[e], gate[r]);
+          }
         }
       }
     }
@@ -216,8 +222,18 @@ few_rows_kernel(const FewParams p) {
   constexpr int kShift = kRows == 16 ? 1 : kRows == 8 ? 2 : kRows == 4 ? 3 : kRows == 2 ? 4 : 5;
   float v = sum_rows<kRows>(acc, lane), g = 0.f;
   if constexpr (kTwo) g = sum_rows<kRows>(gate, lane);
+  if (p.warps > 1) {
+    joined[0][warp][lane] = v;
+    if (kTwo) joined[1][warp][lane] = g;
+    __syncthreads();
+    if (part != 0) return;
+    for (int i = 1; i < p.warps; ++i) {
+      v += joined[0][warp + i][lane];
+      if (kTwo) g += joined[1][warp + i][lane];
+    }
+  }
   const int row = lane >> kShift;
-  if ((lane & ((1 << kShift) - 1)) != 0 || row >= p.rows) return;
+  if (!in || (lane & ((1 << kShift) - 1)) != 0 || row >= p.rows) return;
   const T* bias = static_cast<const T*>(p.bias);
   if (bias != nullptr) {
     v += static_cast<float>(bias[n]);
@@ -376,8 +392,25 @@ struct JoinParams {
   const float* part;
   void* out;  // rows of `columns`, dense
   long long part_stride, pitch, rows;
-  int parts, columns, slices, blocks;  // slices: threads of a value, 1 or 8
+  int parts, columns, slices, blocks;  // slices: threads of a value, 1 or 8; 0: a thread takes four neighbouring values
 };
+template <typename T>
+__device__ __forceinline__ void join_by_four(const JoinParams& p, long long first) {
+  const int quads = p.columns / 4;
+  for (long long i = first; i < p.rows * quads; i += p.blocks * 256LL) {
+    const long long r = i / quads;
+    const int c = int(i - r * quads) * 4;
+    const float4* src = reinterpret_cast<const float4*>(p.part + r * p.pitch + c);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < p.parts; ++s) {
+      const float4 x = __ldg(src + s * (p.part_stride / 4));
+      sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+    }
+    T* out = static_cast<T*>(p.out) + r * p.columns + c;  // 8-byte aligned: columns are a multiple of four
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(sum.x, sum.y), pack2<T>(sum.z, sum.w));
+  }
+}
 template <typename T>
 __global__ void __launch_bounds__(256)
 join_kernel(const JoinParams a, const JoinParams b) {
@@ -386,6 +419,7 @@ join_kernel(const JoinParams a, const JoinParams b) {
   pdl_wait();
   const bool second = int(blockIdx.x) >= a.blocks;
   const JoinParams& p = second ? b : a;
+  if (p.slices == 0) return join_by_four<T>(p, (blockIdx.x - (second ? a.blocks : 0)) * 256LL + threadIdx.x);
   const int values = 256 / p.slices, slice = p.slices == 1 ? 0 : threadIdx.x >> 5, lane = p.slices == 1 ? threadIdx.x : threadIdx.x & 31;
   const long long total = p.rows * p.columns;
   for (long long i0 = (blockIdx.x - (second ? a.blocks : 0)) * (long long)values; i0 < total; i0 += (long long)p.blocks * values) {
@@ -434,7 +468,8 @@ copy_rows_kernel(const CopyParams p) {
     if (job.column_stride == 1) {
       const long long r = v / vectors;
       const int c = int(v - r * vectors) * 8, valid = job.columns - c;
-      *reinterpret_cast<uint4*>(dst + r * job.dst_row_stride + c) = norm::load<__half, true>(reinterpret_cast<const __half*>(src + r * job.row_stride + c), valid);
+      const __half* from = reinterpret_cast<const __half*>(src + r * job.row_stride + c);
+      *reinterpret_cast<uint4*>(dst + r * job.dst_row_stride + c) = norm::arrived<__half, true>(norm::load<__half, true>(from, valid), from, valid);
     } else {
       const long long c = v / job.rows * 8, r = v - v / job.rows * job.rows;
       uint32_t w[4];
@@ -472,7 +507,7 @@ Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns,
   const int64_t kblocks = (rows + matmul::kBK - 1) / matmul::kBK, values = n_rows * n_outer;
   Split best{int(kblocks), 1, false};
   double least = 1e300;
-  for (int64_t tried = 1; tried <= 256 && tried <= kblocks; tried += tried < 8 ? 1 : tried < 32 ? 4 : tried < 64 ? 8 : 16) {
+  for (int64_t tried = 1; tried <= 256 && tried <= kblocks; tried += tried < 8 ? 1 : tried < 24 ? 2 : tried < 64 ? 8 : 16) {
     const int64_t per = (kblocks + tried - 1) / tried, parts = (kblocks + per - 1) / per;
     for (int sums = 0; sums <= int(want_sums); ++sums) {
       const MatmulForm form = parts > 1 ? kPartial : kPlain;
@@ -562,10 +597,14 @@ int b200ta_dense(const void* x, int64_t xs, const void* w, int64_t ws, const voi
     DeviceState* st = nullptr;
     rc = get_device_state(&st);
     if (rc != B200TA_OK) return rc;
-    const FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation, gated, dtype == B200TA_DTYPE_F16};
-    const bool vec = K % 8 == 0 && rows_aligned(x, xs) && rows_aligned(w, ws);
-    return launch_kernel(st, kKernelDenseHelpers, p.f16 ? pick_few<__half>(int(rows), vec, gated) : pick_few<__nv_bfloat16>(int(rows), vec, gated),
-                         dim3(unsigned((N + 3) / 4)), 128, 0, stream, p);
+    const bool vec = K % 8 == 0 && rows_aligned(x, xs) && rows_aligned(w, ws), f16 = dtype == B200TA_DTYPE_F16;
+    // more warps a column while the device has room for them and each still has a vector a lane
+    int warps = 1;
+    while (warps < kFewWarps && int64_t(N) * warps < int64_t(st->num_sms) * 16 && K > warps * 32 * (vec ? 8 : 1)) warps *= 2;
+    const FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation, warps};
+    const int columns = kFewWarps / warps;
+    return launch_kernel(st, kKernelDenseHelpers, f16 ? pick_few<__half>(int(rows), vec, gated) : pick_few<__nv_bfloat16>(int(rows), vec, gated),
+                         dim3(unsigned((N + columns - 1) / columns)), kFewWarps * 32, 0, stream, p);
   }
   B200TA_REQUIRE(rows_aligned(x, xs) && rows_aligned(w, ws) && (!residual || rows_aligned(residual, rs)) &&
                      (!saved || rows_aligned(saved, ss)),
@@ -692,8 +731,9 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
   if (!parts_left && !sums_left) return B200TA_OK;
   const int64_t chunk = plan.chunk < rows ? plan.chunk : rows;
   auto join_of = [&](bool wanted, const float* part, int64_t count, int64_t stride, int64_t pitch, int64_t n_rows, int columns, void* out) {
-    const int slices = count > 8 && n_rows * columns < 256 * 1024 ? 8 : 1;
-    const int64_t need = (n_rows * columns * slices + 255) / 256, most = int64_t(st->num_sms) * 16;
+    const bool four = columns % 4 == 0 && pitch % 4 == 0 && stride % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0;
+    const int slices = n_rows * columns < 32768 && count > 8 ? 8 : four ? 0 : 1;
+    const int64_t need = (slices == 0 ? n_rows * columns / 4 + 255 : n_rows * columns * slices + 255) / 256, most = int64_t(st->num_sms) * 16;
     return JoinParams{part, out, stride, pitch, n_rows, int(count), columns, slices, wanted ? int(std::min(need, most)) : 0};
   };
   const JoinParams a = join_of(parts_left, parts, plan.split.parts, outer * N * pad4(K), pad4(K), outer * N, K, dw);

@@ -49,10 +49,7 @@ norm_kernel(const NormParams p) {
   uint4 next[kAhead ? kItems : 1];
   auto load_next = [&](bool in) {
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      next[kAhead ? i : 0] = make_uint4(0u, 0u, 0u, 0u);
-      if (in && valid[i] > 0) next[kAhead ? i : 0] = norm::load<T, kShifted>(x + i * lanes * kVec, valid[i]);
-    }
+    for (int i = 0; i < kItems; ++i) next[kAhead ? i : 0] = norm::load_if(in && valid[i] > 0, x + i * lanes * kVec);
     x += x_step;
   };
   if constexpr (kCopies)
@@ -78,15 +75,17 @@ norm_kernel(const NormParams p) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       F2 sum(0.f);
+      norm::Pending pending[kShifted ? kItems : 1];
+      if constexpr (kShifted) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) pending[i] = norm::load<T, true>(x + i * lanes * kVec, left > 0 ? valid[i] : 0);
+      }
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
         uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (kAhead) {
-          raw = next[i];
-        } else if (left > r * step && valid[i] > 0) {
-          if constexpr (kShifted) raw = norm::load<T, kShifted>(x + i * lanes * kVec, valid[i]);
-          else raw = lds128(slot0 + take * stage_bytes + i * blockDim.x * 16);
-        }
+        if constexpr (kAhead) raw = next[i];
+        else if constexpr (kShifted) raw = norm::arrived<T, true>(pending[i], x + i * lanes * kVec, left > 0 ? valid[i] : 0);
+        else if (left > r * step && valid[i] > 0) raw = lds128(slot0 + take * stage_bytes + i * blockDim.x * 16);
         const norm::Values<T> values(raw);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) v[r][i][j] = values.p[j], sum = sum + values.p[j];  // zeros behind the row

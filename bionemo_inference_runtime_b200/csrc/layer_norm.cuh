@@ -136,19 +136,39 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
-// A vector of a row from `p` on, `valid` elements of which are in the row.
+// 16 bytes, or zeros without an access: no branch, so that a thread's loads are on their way together.
+__device__ __forceinline__ uint4 load_if(bool in, const void* p) {
+  uint4 v;
+  asm volatile(
+      "{\n.reg .pred q;\nsetp.ne.u32 q, %5, 0;\nmov.u32 %0, 0;\nmov.u32 %1, 0;\nmov.u32 %2, 0;\nmov.u32 %3, 0;\n"
+      "@q ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"(static_cast<uint32_t>(in)));
+  return v;
+}
+// A vector of a row from `p` on, `valid` elements of which are in the row: the one or two aligned vectors that hold it, and the
+// vector itself once they are there.
+struct Pending {
+  uint4 lo, hi;
+};
 template <typename T, bool kShifted>
-__device__ __forceinline__ uint4 load(const T* p, int valid) {
+__device__ __forceinline__ Pending load(const T* p, int valid) {
   if constexpr (!kShifted) {
-    return __ldg(reinterpret_cast<const uint4*>(p));
+    return {load_if(valid > 0, p), uint4()};
   } else {
     const uintptr_t a = reinterpret_cast<uintptr_t>(p), base = a & ~uintptr_t(15);
     const uint32_t at = uint32_t(a & 15u), bytes = (valid < Values<T>::kVec ? valid : Values<T>::kVec) * uint32_t(sizeof(T));
-    const uint4 lo = __ldg(reinterpret_cast<const uint4*>(base));
-    uint4 hi = make_uint4(0u, 0u, 0u, 0u);
-    if (at + bytes > 16u) hi = __ldg(reinterpret_cast<const uint4*>(base) + 1);
-    const uint4 x = window<T>(lo, hi, at);
-    return valid >= Values<T>::kVec ? x : first<T>(x, valid);
+    return {load_if(valid > 0, reinterpret_cast<const void*>(base)),
+            load_if(valid > 0 && at + bytes > 16u, reinterpret_cast<const void*>(base + 16))};
+  }
+}
+template <typename T, bool kShifted>
+__device__ __forceinline__ uint4 arrived(const Pending& x, const T* p, int valid) {
+  if constexpr (!kShifted) {
+    return x.lo;
+  } else {
+    const uint4 v = window<T>(x.lo, x.hi, uint32_t(reinterpret_cast<uintptr_t>(p) & 15u));
+    return valid >= Values<T>::kVec ? v : first<T>(v, valid);
   }
 }
 // Stores a vector of a row at `p`, the `index`-th of the `lanes` vectors that neighbouring lanes of this warp store, all of
@@ -181,6 +201,20 @@ __device__ __forceinline__ void store(T* p, uint4 x, int valid, int index, int l
   }
 }
 
+template <typename W>
+__device__ __forceinline__ float element_if(bool in, const W* p) {
+  if constexpr (sizeof(W) == 4) {
+    float v;
+    asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\nmov.f32 %0, 0f00000000;\n@q ld.global.nc.f32 %0, [%1];\n}"
+                 : "=&f"(v) : "l"(p), "r"(static_cast<uint32_t>(in)));
+    return v;
+  } else {
+    uint16_t v;
+    asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\nmov.u16 %0, 0;\n@q ld.global.nc.u16 %0, [%1];\n}"
+                 : "=&h"(v) : "l"(p), "r"(static_cast<uint32_t>(in)));
+    return unpack2<W>(uint32_t(v)).x;
+  }
+}
 // The parameters of kVec columns from c on, `valid` of them in the row, or `none` where there are none.
 template <typename T, typename W, bool kShifted>
 __device__ __forceinline__ void load_param(const NormParams& p, const void* param, int c, int valid, float none, F2* v) {
@@ -200,9 +234,11 @@ __device__ __forceinline__ void load_param(const NormParams& p, const void* para
     }
   } else {
     const W* q = static_cast<const W*>(param) + c;
+    float f[kVec];
 #pragma unroll
-    for (int j = 0; j < kVec / 2; ++j)
-      v[j] = F2(2 * j < valid ? static_cast<float>(q[2 * j]) : none, 2 * j + 1 < valid ? static_cast<float>(q[2 * j + 1]) : none);
+    for (int j = 0; j < kVec; ++j) f[j] = element_if(j < valid, q + j);
+#pragma unroll
+    for (int j = 0; j < kVec / 2; ++j) v[j] = F2(f[2 * j], f[2 * j + 1]);
   }
 }
 

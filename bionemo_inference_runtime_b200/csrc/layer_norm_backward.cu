@@ -76,17 +76,26 @@ norm_grad_kernel(const NormParams p) {
       for (int r = 0; r < kRows; ++r) fetch();
       norm::copy_wait<kStages - kRows>();
     }
+    norm::Pending px[kShifted ? kItems : 1], pdy[kShifted ? kItems : 1];
+    auto request = [&]() {
+      if constexpr (kShifted) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          px[i] = norm::load<T, true>(x + i * lanes * kVec, left > 0 ? valid[i] : 0);
+          pdy[i] = norm::load<T, true>(dy + i * lanes * kVec, left > 0 ? valid[i] : 0);
+        }
+      }
+    };
+    request();
     // xh and g = dy w of item i of a row; with kSum also dw and db
     auto load = [&](int i, int r, int stage, auto sum) {
       uint4 raw_x = make_uint4(0u, 0u, 0u, 0u), raw_dy = raw_x;
-      if (left > r * step && valid[i] > 0) {
-        if constexpr (kShifted) {
-          raw_x = norm::load<T, kShifted>(x + i * lanes * kVec, valid[i]);
-          raw_dy = norm::load<T, kShifted>(dy + i * lanes * kVec, valid[i]);
-        } else {
-          raw_x = lds128(slot0 + stage * stage_bytes + i * item_bytes);
-          raw_dy = lds128(slot0 + stage * stage_bytes + (kItems + i) * item_bytes);
-        }
+      if constexpr (kShifted) {
+        raw_x = norm::arrived<T, true>(px[i], x + i * lanes * kVec, left > 0 ? valid[i] : 0);
+        raw_dy = norm::arrived<T, true>(pdy[i], dy + i * lanes * kVec, left > 0 ? valid[i] : 0);
+      } else if (left > r * step && valid[i] > 0) {
+        raw_x = lds128(slot0 + stage * stage_bytes + i * item_bytes);
+        raw_dy = lds128(slot0 + stage * stage_bytes + (kItems + i) * item_bytes);
       }
       const norm::Values<T> vx(raw_x), vd(raw_dy);
       const int k = kKeep ? i : 0, kw = kHold ? i : 0;
@@ -117,6 +126,7 @@ norm_grad_kernel(const NormParams p) {
     }
     if (p.dx != nullptr) {
       norm::row_sums<kLanes>(s, lanes, scratch, turn);
+      if (!kKeep) request();
       stage = take;
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
@@ -168,23 +178,26 @@ norm_grad_kernel(const NormParams p) {
   if (group == 0) each(p.partial + (long long)blockIdx.x * 2 * p.width, false);
 }
 
-// dw and db: column sums of the blocks' partial sums.  A block takes 32 of the 2 * width columns, 32 threads a column.
+// dw and db: column sums of the blocks' partial sums.  A block takes 8 of the 2 * width columns, 128 threads a column.
 template <typename T>
 __global__ void __launch_bounds__(1024)
 norm_join_kernel(const float* partial, int blocks, int width, T* dw, T* db) {
-  __shared__ float part[32][33];
+  __shared__ float part[32][8];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, k = threadIdx.x >> 3, c = blockIdx.x * 8 + (threadIdx.x & 7);
   float sum = 0.f;
   if (c < 2 * width)
-#pragma unroll 8
-    for (int b = k; b < blocks; b += 32) sum += __ldg(partial + (long long)b * 2 * width + c);
-  part[k][lane] = sum;
+#pragma unroll 4
+    for (int b = k; b < blocks; b += 128) sum += __ldg(partial + (long long)b * 2 * width + c);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+  if (lane < 8) part[threadIdx.x >> 5][lane] = sum;
   __syncthreads();
-  if (k == 0 && c < 2 * width) {
+  if (threadIdx.x < 8 && c < 2 * width) {
+    sum = 0.f;
 #pragma unroll
-    for (int i = 1; i < 32; ++i) sum += part[i][lane];
+    for (int i = 0; i < 32; ++i) sum += part[i][threadIdx.x];
     T* dst = c < width ? dw : db;
     if (dst != nullptr) dst[c < width ? c : c - width] = static_cast<T>(sum);
   }
@@ -249,7 +262,7 @@ int b200ta_layer_norm_backward(const void* dy, int64_t dys, const void* x, int64
   else launch = pick<float, float>(s);
   rc = launch(st, blocks, s.threads, smem, stream, p);
   if (rc != B200TA_OK || !sums) return rc;
-  const dim3 grid{unsigned((2 * width + 31) / 32)};
+  const dim3 grid{unsigned((2 * width + 7) / 8)};
   auto join = [&](auto* dw, auto* db) {
     return launch_kernel(st, kKernelNorm, norm_join_kernel<std::remove_pointer_t<decltype(dw)>>, grid, 1024, 0, stream, p.partial, blocks,
                          width, dw, db);
