@@ -95,9 +95,18 @@ int encode_tensor_map(CUtensorMap* map, const void* base, int elem_bytes, int ra
                           : swz == SWZ_64 ? CU_TENSOR_MAP_SWIZZLE_64B
                           : swz == SWZ_32 ? CU_TENSOR_MAP_SWIZZLE_32B
                                           : CU_TENSOR_MAP_SWIZZLE_NONE;
-  CUresult r = g_encode(map, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdims, gstrides, gbox,
-                        estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&]() {
+    return g_encode(map, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdims, gstrides, gbox, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // a thread that has made no runtime call yet (PyTorch runs backward passes on threads of its own) has no context
+    int dev = 0;
+    B200TA_CHECK_CUDA(cudaGetDevice(&dev));
+    B200TA_CHECK_CUDA(cudaSetDevice(dev));
+    r = encode();
+  }
   if (r != CUDA_SUCCESS) return fail(B200TA_ERR_DRIVER, "%s: cuTensorMapEncodeTiled returned %d", what, (int)r);
   return B200TA_OK;
 }

@@ -11,6 +11,7 @@ from .buffers import PreallocatedBuffers, ensure_buffer
 from .linear import Linear, WeightMode, WeightsLoadingConfig
 from .pairformer import (PairformerLayerV1, PairformerLayerV2, PairformerModule, PairformerNoSeqLayer,
                          PairformerNoSeqModule)
+from .training import TrainableTransition, dense, gated_dense, layer_norm
 from .transition import PairTransition, Transition
 from .triangle_multiplication import (TriangleMultiplicationMetadata, TriangleMultiplicationNode,
                                       TriangleMultiplicationNodeType, precompute_trimul_metadata,
@@ -28,5 +29,5 @@ __all__ = [
     "TriangleMultiplicationMetadata", "TriangleMultiplicationNode", "TriangleMultiplicationNodeType",
     "precompute_trimul_metadata", "set_trimul_token_padding", "PairformerNoSeqLayer", "PairformerNoSeqModule",
     "AttentionPairBias", "PairformerLayerV1", "PairformerLayerV2", "PairformerModule", "PrecomputedSingleMasks", "precompute_single_masks",
-    "register_precompute_single_masks",
+    "register_precompute_single_masks", "TrainableTransition", "dense", "gated_dense", "layer_norm",
 ]
