@@ -26,7 +26,7 @@ HOST_SOURCES = [CSRC / "torch_host.cpp", CSRC / "torch_training.cpp"]
 HOST_MADE_FOR = "host_made_for.txt"
 SOURCES = ["host.cu", "pack.cu", "rowgemm.cu", "attention.cu", "node.cu", "transition.cu", "trimul_project.cu",
            "trimul_contract.cu", "trimul_output.cu", "linear.cu", "pair_bias.cu", "masks.cu",
-           "layer_norm.cu", "layer_norm_backward.cu", "dense.cu", "matmul_forward.cu", "matmul_grad.cu", "matmul_product.cu"]
+           "layer_norm.cu", "layer_norm_backward.cu", "dense.cu", "matmul_forward.cu", "matmul_grad.cu", "matmul_product.cu", "narrow.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo", "--use_fast_math",

@@ -49,7 +49,8 @@ struct DeviceState {
 enum KernelId {
   kKernelPrologue, kKernelEpilogue, kKernelAttention, kKernelAttentionMasked, kKernelTransition, kKernelTransitionRelu,
   kKernelProject, kKernelContract, kKernelOutput, kKernelOutputF32, kKernelLinear, kKernelPairBias, kKernelRowStats,
-  kKernelMaskRows, kKernelNorm, kKernelDenseHelpers, kKernelMatmul  // and one for each of the matmul kernels after it
+  kKernelMaskRows, kKernelNorm, kKernelDenseHelpers, kKernelNarrow,
+  kKernelMatmul = kKernelNarrow + 4  // and one for each of the matmul kernels after it
 };
 int get_device_state(DeviceState** out);
 

@@ -4,6 +4,7 @@
 
 #include "layer_norm.cuh"
 #include "matmul.cuh"
+#include "narrow.cuh"
 
 namespace b200ta {
 
@@ -535,6 +536,12 @@ struct BackwardPlan {
   int rows_sum;       // rows of a partial sum of db
   int64_t dz, parts, sums, bytes;  // offsets, total
 };
+// Whether dz and dx come from one kernel (narrow.cuh): its blocks take 256 rows each, so from a row tile for half of the SMs on.
+// (Backward pass of a gated layer 128 -> 512: 6000 rows 46 us so and 40 us otherwise, 16384 rows 50 and 58, 147456 rows 208 and
+// 231; 64 -> 256, 147456 rows: 110 and 126.)
+bool narrow_pays(bool own_dz, bool kept, int64_t rows, int K, const void* dx, int64_t dxs, int num_sms) {
+  return own_dz && !kept && K <= 128 && dx != nullptr && rows_aligned(dx, dxs) && rows >= int64_t(num_sms) * 64;
+}
 BackwardPlan make_plan(bool gated, bool slope, bool kept, bool want_dbias, int64_t rows, int K, int N, int num_sms) {
   BackwardPlan p{};
   const int64_t outer = gated ? 2 : 1;
@@ -660,6 +667,18 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
   const int sum_columns = int(own_dz ? plan.dz_pitch : N);
   const bool direct = plan.direct, product_sums = plan.split.sums && dw != nullptr && dbias != nullptr;
 
+  auto join_of = [&](bool wanted, const float* part, int64_t count, int64_t stride, int64_t pitch, int64_t n_rows, int columns, void* out) {
+    const bool four = columns % 4 == 0 && pitch % 4 == 0 && stride % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0;
+    const int slices = n_rows * columns < 32768 && count > 8 ? 8 : four ? 0 : 1;
+    const int64_t need = (slices == 0 ? n_rows * columns / 4 + 255 : n_rows * columns * slices + 255) / 256, most = int64_t(st->num_sms) * 16;
+    return JoinParams{part, out, stride, pitch, n_rows, int(count), columns, slices, wanted ? int(std::min(need, most)) : 0};
+  };
+  auto join = [&](const JoinParams& a, const JoinParams& b) {
+    return launch_kernel(st, kKernelDenseHelpers, f16 ? join_kernel<__half> : join_kernel<__nv_bfloat16>, dim3(unsigned(a.blocks + b.blocks)),
+                         256, 0, stream, a, b);
+  };
+  const bool narrow = narrow_pays(own_dz, saved != nullptr, rows, K, dx, dxs, st->num_sms);
+
   for (int64_t r0 = 0; r0 < rows; r0 += plan.chunk) {
     const int64_t n = rows - r0 < plan.chunk ? rows - r0 : plan.chunk;
     const char* dy_c = static_cast<const char*>(dy) + r0 * dys * 2;
@@ -669,7 +688,17 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
     if (own_dz) {
       void* dst = ws_base + plan.dz;
       dz = dst, zs = plan.dz_pitch;
-      if (saved != nullptr) {
+      if (narrow) {
+        Narrow m;
+        m.f16 = f16, m.gated = gated != 0;
+        m.x = {x_c, n, K, xs};
+        m.dy = {dy_c, n, N, dys};
+        m.w = {w, N, K, ws, outer, int64_t(N) * ws};
+        m.dx = {static_cast<char*>(dx) + r0 * dxs * 2, n, K, dxs};
+        if (dw != nullptr || dbias != nullptr) m.dz = {dst, n, N, zs, outer, zs / 2};
+        m.bias = bias, m.activation = activation, m.what = "dense_backward dx";
+        rc = run_narrow(m, stream);
+      } else if (saved != nullptr) {
         const SlopeParams p{dy_c, static_cast<const char*>(saved) + r0 * ss * 2, dst, dbias != nullptr && !product_sums ? sums : nullptr, dys, ss, zs, n,
                             sum_pitch, N, plan.rows_sum, r0 > 0};
         const dim3 grid{unsigned((N + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
@@ -689,7 +718,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       }
       if (rc != B200TA_OK) return rc;
     }
-    if (dx != nullptr) {
+    if (dx != nullptr && !narrow) {
       Matmul m;
       m.form = kPlain, m.b_mn = true, m.f16 = f16;
       m.a = {dz, n, N, zs, outer, zs / 2};
@@ -711,7 +740,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
         m.kblocks_split = plan.split.kblocks;
         m.accumulate = r0 > 0;  // each part is added to by one block at a time, the chunks in their order
       }
-      if (dx != nullptr) m.beside = kBesideSecond;
+      if (dx != nullptr && !narrow) m.beside = kBesideSecond;
       if (product_sums) m.sums = direct ? dbias : sums;
       m.what = "dense_backward dW";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
@@ -730,17 +759,10 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
   const bool parts_left = dw != nullptr && !direct, sums_left = dbias != nullptr && !(product_sums && direct);
   if (!parts_left && !sums_left) return B200TA_OK;
   const int64_t chunk = plan.chunk < rows ? plan.chunk : rows;
-  auto join_of = [&](bool wanted, const float* part, int64_t count, int64_t stride, int64_t pitch, int64_t n_rows, int columns, void* out) {
-    const bool four = columns % 4 == 0 && pitch % 4 == 0 && stride % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0;
-    const int slices = n_rows * columns < 32768 && count > 8 ? 8 : four ? 0 : 1;
-    const int64_t need = (slices == 0 ? n_rows * columns / 4 + 255 : n_rows * columns * slices + 255) / 256, most = int64_t(st->num_sms) * 16;
-    return JoinParams{part, out, stride, pitch, n_rows, int(count), columns, slices, wanted ? int(std::min(need, most)) : 0};
-  };
   const JoinParams a = join_of(parts_left, parts, plan.split.parts, outer * N * pad4(K), pad4(K), outer * N, K, dw);
   const JoinParams b = product_sums ? join_of(sums_left, sums, plan.split.parts, outer * N, N, outer, N, dbias)
                                     : join_of(sums_left, sums, (chunk + plan.rows_sum - 1) / plan.rows_sum, sum_pitch, sum_pitch / outer, outer, N, dbias);
-  return launch_kernel(st, kKernelDenseHelpers, f16 ? join_kernel<__half> : join_kernel<__nv_bfloat16>, dim3(unsigned(a.blocks + b.blocks)),
-                       256, 0, stream, a, b);
+  return join(a, b);
 }
 
 int b200ta_copy_rows(const b200ta_copy* jobs, int count, void* stream) {

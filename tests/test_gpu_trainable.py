@@ -285,6 +285,19 @@ def test_rows_in_chunks(rows, K, N, gated):
     check_layer(activation="silu", **layer_inputs(rows, K, N, torch.bfloat16, gated, True, False))
 
 
+@pytest.mark.parametrize("gated", [False, True], ids=["dense", "gated"])
+@pytest.mark.parametrize("rows,K,N", [(9472, 128, 64), (9700, 64, 200), (10001, 128, 512), (12000, 8, 7), (9999, 72, 130)])
+def test_narrow_layers_of_many_rows(rows, K, N, gated):
+    """At most 128 inputs: dz and dx come from one kernel.  Rows and units that fill its tiles of 256 and 64, and do not."""
+    dtype = torch.float16 if N % 4 else torch.bfloat16
+    given = layer_inputs(rows, K, N, dtype, gated, rows % 2 == 0, False)
+    check_layer(activation="silu", **given)
+    x, w, bias, dy = given["x"], given["w"], given["bias"], given["dy"]
+    back = ops.gated_dense_backward if gated else ops.dense_backward
+    both, alone = back(dy, x, w, bias, activation="gelu"), back(dy, x, w, bias, activation="gelu", want_dweight=False, want_dbias=False)
+    assert torch.equal(both[0], alone[0]) and alone[1] is None
+
+
 def test_parts_of_the_weight_gradient():
     """dW in one piece, and in parts of the rows."""
     check_layer(**layer_inputs(256, 2048, 2048, torch.bfloat16, False, True, True))

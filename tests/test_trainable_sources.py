@@ -19,9 +19,16 @@ def test_matmul_kernel_lets_the_next_kernel_start_behind_its_allocation():
     assert re.search(r"tmem_alloc_pair\(.*\);\s*else tmem_alloc\(.*\);\s*if \(.*\) pdl_wait\(\);\s*pdl_trigger\(\);", text)
 
 
-def test_every_wait_of_the_matmul_kernel_is_bounded():
-    text = re.sub(r"//[^\n]*", "", (CSRC / "matmul.cuh").read_text())
-    assert "try_wait" not in text and not re.search(r"while\s*\(", text)
+def test_narrow_kernel_lets_the_next_kernel_start_behind_its_allocation():
+    text = (CSRC / "narrow.cuh").read_text()
+    assert text.count("tmem_alloc(") == 1 and text.count("pdl_trigger()") == 1
+    assert re.search(r"tmem_alloc\(.*\);\s*pdl_trigger\(\);", text)
+
+
+@pytest.mark.parametrize("header", ["matmul.cuh", "narrow.cuh"])
+def test_every_wait_is_bounded(header):
+    text = re.sub(r"//[^\n]*", "", (CSRC / header).read_text())
+    assert "bar.sync" not in text and "try_wait" not in text and not re.search(r"while\s*\(", text)
 
 
 def test_entry_points_refuse_before_any_cuda_call():
