@@ -113,7 +113,7 @@ int run_matmul(const Matmul& m, void* stream) {
     return rc;
   }
   if (p.has_aux && (rc = map_of(&maps.aux, m.aux, 2, 32, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
-  if (p.has_saved && (rc = map_of(&maps.saved, m.saved, 2, 32, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
+  if (p.has_saved && (rc = map_of(&maps.saved, m.saved, 4, 16, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
   const int blocks = p.resident ? p.resident * p.tiles_n : std::min(p.work, p.pair ? st->num_sms / 2 : st->num_sms);
   const int grid = p.pair ? 2 * blocks : blocks;
   // Two sets of finishing warps are out of step, so that one computes while the other loads and stores, and a warp's waits
@@ -241,9 +241,9 @@ few_rows_kernel(const FewParams p) {
     if (kTwo) g += static_cast<float>(bias[n + p.N]);
   }
   if (p.saved != nullptr) {
-    T* s = static_cast<T*>(p.saved) + row * p.ss + n;
-    s[0] = static_cast<T>(v);
-    if (kTwo) s[p.ss / 2] = static_cast<T>(g);
+    float* s = static_cast<float*>(p.saved) + row * p.ss + n;
+    s[0] = v;
+    if (kTwo) s[p.ss / 2] = g;
   }
   float a, slope;
   activate_any(p.activation, kTwo ? g : v, a, slope);
@@ -267,7 +267,7 @@ auto pick_few(int rows, bool vec, bool two) {
 
 // ---- dz from stored pre-activations ---------------------------------------------------------------------------------
 //
-// dz = dy act'(z), or [dy act(g) | dy v act'(g)]: reads 2 (3) and writes 1 (2) planes, bound by HBM.  A block takes 256 columns
+// dz = dy act'(z), or [dy act(g) | dy v act'(g)], z kept in 32 bits: bound by HBM.  A block takes 256 columns
 // of some rows, a thread eight columns of every eighth of them, whose sums (db) it has on the way: part[block.y][column] (+)=
 // theirs, of the values before they are rounded.
 struct SlopeParams {
@@ -277,6 +277,10 @@ struct SlopeParams {
   long long dys, ss, zs, rows, part_pitch;
   int N, rows_block, accumulate;
 };
+__device__ __forceinline__ void load_eight(const float* p, float (&v)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
 // The sums of the block's threads with the same columns, to the workspace.
 __device__ __forceinline__ void store_sums(const float (&s)[8], float (&joined)[8][256 + 4], float* part, int columns, bool accumulate) {
   const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
@@ -304,19 +308,19 @@ slope_kernel(const SlopeParams p) {
 #pragma unroll 1
     for (long long row = r0 + (threadIdx.x >> 5); row < r1; row += 8) {
       const T* dy = static_cast<const T*>(p.dy) + row * p.dys + c;
-      const T* z = static_cast<const T*>(p.saved) + row * p.ss + c;
+      const float* z = static_cast<const float*>(p.saved) + row * p.ss + c;
       T* dz = static_cast<T*>(p.dz) + row * p.zs + c;
       float d[8], v[8], g[8];
       if (c + 8 <= p.N) {
         load_vec<T, 8>(dy, d);
-        load_vec<T, 8>(z, v);
-        if constexpr (kTwo) load_vec<T, 8>(z + p.ss / 2, g);
+        load_eight(z, v);
+        if constexpr (kTwo) load_eight(z + p.ss / 2, g);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const bool in = c + j < p.N;
-          d[j] = in ? static_cast<float>(dy[j]) : 0.f, v[j] = in ? static_cast<float>(z[j]) : 0.f;
-          if constexpr (kTwo) g[j] = in ? static_cast<float>(z[p.ss / 2 + j]) : 0.f;
+          d[j] = in ? static_cast<float>(dy[j]) : 0.f, v[j] = in ? z[j] : 0.f;
+          if constexpr (kTwo) g[j] = in ? z[p.ss / 2 + j] : 0.f;
         }
       }
 #pragma unroll
@@ -563,7 +567,7 @@ BackwardPlan make_plan(bool gated, bool slope, bool kept, bool want_dbias, int64
   };
   p.dz = take(p.dz_pitch * (p.chunk < rows ? p.chunk : rows) * 2);
   p.parts = take(p.direct ? 0 : p.split.parts * outer * N * pad4(K) * int64_t(sizeof(float)));
-  p.rows_sum = sum_rows(p.chunk, N, num_sms);
+  p.rows_sum = sum_rows(p.chunk, kept ? N : outer * N, num_sms);
   const int64_t slots = p.split.sums ? p.split.parts : (p.chunk + p.rows_sum - 1) / p.rows_sum;
   p.sums = take(!want_dbias || (p.split.sums && p.direct) ? 0 : slots * outer * pad8(N) * int64_t(sizeof(float)));
   return p;
@@ -629,9 +633,10 @@ int b200ta_dense(const void* x, int64_t xs, const void* w, int64_t ws, const voi
 }
 
 int b200ta_dense_keeps(int activation, int gated, int K) {
-  // Kept values are written and read at 2 bytes each (and dz formed from them in a pass of its own), computed ones cost 2 K
-  // operations each on the tensor cores.
-  return (gated || activation != b200ta::kActNone) && K >= 512;
+  // Kept values are written and read at 4 bytes each, computed ones cost 2 K operations each on the tensor cores: a training step
+  // of a gated layer takes 399 us either way for 8192 rows, 1024 -> 4096, and 361 us kept, 406 us computed again for 4096 rows,
+  // 2048 -> 4096.  (In 16 bits keeping would pay from 512 inputs on, but its rounding adds a third to the gradients' error.)
+  return (gated || activation != b200ta::kActNone) && K >= 1536;
 }
 
 size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, int64_t rows, int K, int N) {
@@ -699,7 +704,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
         m.bias = bias, m.activation = activation, m.what = "dense_backward dx";
         rc = run_narrow(m, stream);
       } else if (saved != nullptr) {
-        const SlopeParams p{dy_c, static_cast<const char*>(saved) + r0 * ss * 2, dst, dbias != nullptr && !product_sums ? sums : nullptr, dys, ss, zs, n,
+        const SlopeParams p{dy_c, static_cast<const float*>(saved) + r0 * ss, dst, dbias != nullptr && !product_sums ? sums : nullptr, dys, ss, zs, n,
                             sum_pitch, N, plan.rows_sum, r0 > 0};
         const dim3 grid{unsigned((N + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
         void (*kernel)(SlopeParams);

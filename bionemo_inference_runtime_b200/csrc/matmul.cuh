@@ -47,7 +47,7 @@ struct MatmulParams {
   const void* bias;                    // [columns] (kGated*: value biases, then gate biases), or NULL
   int activation;
   int has_aux;                         // kDense: a residual
-  int has_saved;                       // kDense, kGated: D + bias is stored as well
+  int has_saved;                       // kDense, kGated: D + bias is stored as well, in 32 bits
   int accumulate;                      // kPartial: add to what the parts hold
   int alternate;                       // the finishing warps take tiles in two sets, in turn
   int beside;                          // kBesideFirst, kBesideSecond: see there
@@ -180,25 +180,32 @@ __device__ __forceinline__ void finish_any(int activation, const float (&v)[kN],
   }
 }
 
-// Adds biases n .. n + kN - 1 (those below `columns`) to v; every lane reads the same addresses.
+// Biases n .. n + kN - 1 as 16-bit pairs, zeros for those from `columns` on; every lane reads the same addresses.  The forward
+// forms load them before the accumulators they are added to, whose way hides theirs.
 template <typename T, int kN>
-__device__ __forceinline__ void add_bias(float (&v)[kN], const T* bias, int n, int columns) {
-  const T* b = bias + n;
-  if (n + kN <= columns && (reinterpret_cast<uintptr_t>(b) & 15u) == 0) {
+__device__ __forceinline__ void load_bias(uint32_t (&b)[kN / 2], const T* bias, int n, int columns) {
+  const T* p = bias + n;
+  if (n + kN <= columns && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
 #pragma unroll
     for (int c = 0; c < kN / 8; ++c) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(b) + c);
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack2<T>(w[e]);
-        v[c * 8 + 2 * e] += f.x, v[c * 8 + 2 * e + 1] += f.y;
-      }
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + c);
+      b[4 * c] = x.x, b[4 * c + 1] = x.y, b[4 * c + 2] = x.z, b[4 * c + 3] = x.w;
     }
   } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int j = 0; j < kN; ++j)
-      if (n + j < columns) v[j] += static_cast<float>(b[j]);
+    for (int j = 0; j < kN / 2; ++j) {
+      const uint32_t lo = n + 2 * j < columns ? __ldg(q + 2 * j) : 0u, hi = n + 2 * j + 1 < columns ? __ldg(q + 2 * j + 1) : 0u;
+      b[j] = lo | hi << 16;
+    }
+  }
+}
+template <typename T, int kN>
+__device__ __forceinline__ void add_bias(float (&v)[kN], const uint32_t (&b)[kN / 2]) {
+#pragma unroll
+  for (int j = 0; j < kN / 2; ++j) {
+    const float2 f = unpack2<T>(b[j]);
+    (F2(v[2 * j], v[2 * j + 1]) + F2(f.x, f.y)).to(v[2 * j], v[2 * j + 1]);
   }
 }
 template <int kN>
@@ -560,10 +567,15 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         }
         // Accumulators are taken 16 columns at a time (kDense, kPlain: 32), to stay within the registers that 18 warps leave a thread.
         constexpr int kStep = kForm == kDense || kForm == kPlain ? 32 : 16;
-        uint32_t y[16], yg[16], z[16], zg[16];
+        uint32_t y[16], yg[16];
         auto step = [&](auto first) {
           constexpr int kFirst = decltype(first)::value;
           float v[kStep], gate[kStep];
+          uint32_t bv[kStep / 2], bg[kStep / 2];
+          if ((kForm == kDense || kForm == kGated) && bias != nullptr) {  // (the gradients' registers do not suffice)
+            load_bias<T, kStep>(bv, bias, n + kFirst, p.columns);
+            if constexpr (kTwo) load_bias<T, kStep>(bg, bias + p.columns, n + kFirst, p.columns);
+          }
           tmem_load(acc + g * 32 + kFirst, v);
           if constexpr (kTwo) tmem_load(acc + units + g * 32 + kFirst, gate);
           tmem_ld_wait();
@@ -578,14 +590,24 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
             for (int j = 0; j < kStep / 2; ++j) y[kFirst / 2 + j] = pack2<T>(v[2 * j], v[2 * j + 1]);
           } else {
             if (bias != nullptr) {
-              add_bias(v, bias, n + kFirst, p.columns);
-              if constexpr (kTwo) add_bias(gate, bias + p.columns, n + kFirst, p.columns);
+              if constexpr (kGrad) load_bias<T, kStep>(bv, bias, n + kFirst, p.columns);
+              add_bias<T>(v, bv);
+              if constexpr (kGrad && kTwo) load_bias<T, kStep>(bg, bias + p.columns, n + kFirst, p.columns);
+              if constexpr (kTwo) add_bias<T>(gate, bg);
             }
             if ((kForm == kDense || kForm == kGated) && p.has_saved) {
 #pragma unroll
-              for (int j = 0; j < kStep / 2; ++j) {
-                z[kFirst / 2 + j] = pack2<T>(v[2 * j], v[2 * j + 1]);
-                if (kTwo) zg[kFirst / 2 + j] = pack2<T>(gate[2 * j], gate[2 * j + 1]);
+              for (int c = 0; c < kStep; c += 16) {
+                if (n + kFirst + c >= p.columns) break;
+                uint32_t x[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(v[c + j]);
+                store(tm_saved, x, n + kFirst + c, row, 0);
+                if constexpr (kTwo) {
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(gate[c + j]);
+                  store(tm_saved, x, n + kFirst + c, row, 1);
+                }
               }
             }
             finish_any<T, kForm, kFirst, kStep>(p.activation, v, gate, has_aux, aux, y, yg);
@@ -594,10 +616,6 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         step(std::integral_constant<int, 0>());
         if constexpr (kStep == 16) step(std::integral_constant<int, 16>());
         if constexpr (kForm != kPartial) {
-          if ((kForm == kDense || kForm == kGated) && p.has_saved) {
-            store(tm_saved, z, n, row, 0);
-            if (kTwo) store(tm_saved, zg, n, row, 1);
-          }
           store(tm_out, y, n, row, kForm == kPlain ? t.m_outer : 0);
           if (kForm == kGatedGrad) store(tm_out, yg, n, row, 1);
         }

@@ -70,8 +70,13 @@ __device__ __forceinline__ void group_dz(uint32_t v_addr, uint32_t g_addr, int n
     if constexpr (kTwo) matmul::tmem_load(g_addr + kFirst, gate);
     tmem_ld_wait();
     if (bias != nullptr) {
-      matmul::add_bias(v, bias, n + kFirst, p.N);
-      if constexpr (kTwo) matmul::add_bias(gate, bias + p.N, n + kFirst, p.N);
+      uint32_t b[8];
+      matmul::load_bias<T, 16>(b, bias, n + kFirst, p.N);
+      matmul::add_bias<T>(v, b);
+      if constexpr (kTwo) {
+        matmul::load_bias<T, 16>(b, bias + p.N, n + kFirst, p.N);
+        matmul::add_bias<T>(gate, b);
+      }
     }
     matmul::finish_any<T, kForm, kFirst, 16>(p.activation, v, gate, true, aux, y, yg);
   };

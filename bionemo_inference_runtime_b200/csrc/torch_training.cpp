@@ -223,7 +223,7 @@ std::pair<at::Tensor, Maybe> dense(const at::Tensor& x, const at::Tensor& w, con
   if (residual) require_like("residual", *residual, x, y.sizes());
   Maybe saved;
   const int64_t pitch = pad8(l.N) * (gated ? 2 : 1);
-  if (want_saved && lib.dense_keeps(int(activation), gated, l.K)) saved = at::empty({l.rows, pitch}, x.options().memory_format(c10::MemoryFormat::Contiguous));
+  if (want_saved && lib.dense_keeps(int(activation), gated, l.K)) saved = at::empty({l.rows, pitch}, x.options().dtype(at::kFloat).memory_format(c10::MemoryFormat::Contiguous));
   if (l.rows == 0) return {y, saved};
   const bool few = l.rows <= lib.dense_few_rows();
   Copies copies;
@@ -247,8 +247,8 @@ std::tuple<Maybe, Maybe, Maybe> dense_backward(const at::Tensor& dy, const at::T
   require_like("dy", dy, x, shape);
   const int64_t pitch = pad8(l.N) * (gated ? 2 : 1);
   if (saved) {
-    require_like("saved", *saved, x, {l.rows, pitch});
-    if (!saved->is_contiguous()) refuse("saved must be what the forward pass returned");
+    require_like("saved", *saved, x, {l.rows, pitch}, true);
+    if (!saved->is_contiguous() || saved->scalar_type() != at::kFloat) refuse("saved must be what the forward pass returned");
   }
   const c10::cuda::CUDAGuard guard(x.device());
   const at::TensorOptions options = x.options().memory_format(c10::MemoryFormat::Contiguous);

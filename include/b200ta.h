@@ -435,7 +435,7 @@ int b200ta_layer_norm_backward(const void* dy, int64_t dy_row_stride, const void
 
 /* y[rows, N] = act(x w^T + bias) + residual, x [rows, K], w [N, K]; or with `gated`, w [2 N, K] (value rows, then gate rows),
  * y = value * act(gate), [value | gate] = x w^T + bias.  bf16 or fp16.  bias and residual (not for a gated layer) may be NULL.
- * `saved` (may be NULL) receives x w^T + bias for the backward pass, [rows, N] or [rows, 2, saved_row_stride / 2].
+ * `saved` (may be NULL) receives x w^T + bias for the backward pass in fp32, [rows, N] or [rows, 2, saved_row_stride / 2].
  * Up to b200ta_dense_few_rows() rows, any strides and alignment; otherwise x, w, residual and saved are 16-byte aligned with row
  * strides that are multiples of 8 elements (sizes are free, and so is y). */
 int b200ta_dense_few_rows(void);

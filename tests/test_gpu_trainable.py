@@ -3,8 +3,7 @@
 Tolerances are bounds, derived from the roundings that the operators make: with u half the spacing of the type, a result is
 within u * |result| of the formula (one rounding at the end), plus 2^-18 of the sum of the absolute terms for sums in 32 bits
 (up to a few thousand terms), plus, behind a gradient before the activation that is rounded between two kernels, u times its
-absolute terms.  Kept pre-activations are rounded once more; their error passes through the slopes, of at most 1.2 (the first)
-and 0.8 (the second derivative of every activation here).
+absolute terms.  Slopes are at most 1.2 (the first) and 0.8 (the second derivative of every activation here).
 """
 
 import math
@@ -196,12 +195,11 @@ def layer_formula(x, w, bias, residual, activation, gated, dy=None):
     dy = dy.double()
     if gated:
         dz = torch.cat([dy * a, dy * value * slope], 1)
-        kept = torch.cat([1.2 * dy.abs() * gate.abs(), dy.abs() * value.abs() * (1.2 + 0.8 * gate.abs())], 1)
         sums = torch.cat([1.2 * dy.abs() * size[:, n:], dy.abs() * (size[:, :n] * 1.2 + 0.8 * value.abs() * size[:, n:])], 1)
     else:
         dz = dy * slope
-        kept, sums = 0.8 * dy.abs() * z.abs(), 0.8 * dy.abs() * size
-    return y, terms, dz, kept, sums
+        sums = 0.8 * dy.abs() * size
+    return y, terms, dz, sums
 
 
 def check_layer(x, w, bias=None, residual=None, activation="none", gated=False, dy=None, keep=None):
@@ -220,10 +218,10 @@ def check_layer(x, w, bias=None, residual=None, activation="none", gated=False, 
         saved = None
     back = ops.gated_dense_backward if gated else ops.dense_backward
     dx, dw, db = back(dy, x, w, bias, activation=activation, saved=saved, want_dbias=True)
-    _, _, dz, kept, sums = layer_formula(x, w, bias, residual, activation, gated, dy)
+    _, _, dz, sums = layer_formula(x, w, bias, residual, activation, gated, dy)
     # dz is rounded where a kernel hands it to the next one
     plain = activation == "none" and not gated
-    off = SUM * sums + (0 if plain else 1.01 * u * dz.abs() + tiny) + (0 if saved is None else 1.01 * u * kept)
+    off = SUM * sums + (0 if plain else 1.01 * u * dz.abs() + tiny)
     if activation == "relu":  # its slope jumps: where a sum in 32 bits may have the other sign, either is right
         z = x.double() @ w.double().t() + (0 if bias is None else bias.double())
         g = z[:, z.shape[1] // 2:] if gated else z
@@ -252,7 +250,7 @@ def layer_inputs(rows, K, N, dtype, gated, bias, residual, seed=0):
 # rows around the few-rows limit and the tiles of 128, widths around 8, 32, 64 and the tiles of 64, 128 and 256
 SIZES = [(1, 1, 1), (1, 384, 96), (2, 8, 8), (3, 15, 7), (5, 64, 33), (16, 100, 130), (17, 64, 64), (31, 40, 24), (100, 16, 16),
          (128, 128, 128), (129, 72, 65), (200, 515, 129), (257, 128, 512), (300, 384, 200), (500, 1, 40), (333, 1000, 1),
-         (1000, 96, 320), (2500, 520, 136)]
+         (1000, 96, 320), (2500, 520, 136), (700, 1030, 133), (200, 1541, 70)]
 
 
 @pytest.mark.parametrize("gated", [False, True], ids=["dense", "gated"])
@@ -265,7 +263,7 @@ def test_layer_sizes(rows, K, N, gated):
 
 @pytest.mark.parametrize("gated", [False, True], ids=["dense", "gated"])
 @pytest.mark.parametrize("activation", list(ACTS))
-@pytest.mark.parametrize("rows,K", [(6, 64), (150, 64), (150, 520)])
+@pytest.mark.parametrize("rows,K", [(6, 64), (150, 64), (150, 1544)])
 def test_layer_activations(rows, K, activation, gated):
     """Few rows, pre-activations computed again, pre-activations kept."""
     for dtype in (torch.bfloat16, torch.float16):
@@ -274,7 +272,7 @@ def test_layer_activations(rows, K, activation, gated):
 
 @pytest.mark.parametrize("gated", [False, True], ids=["dense", "gated"])
 def test_kept_and_computed_pre_activations(gated):
-    given = layer_inputs(400, 640, 264, torch.bfloat16, gated, True, True)
+    given = layer_inputs(400, 1600, 264, torch.bfloat16, gated, True, True)
     check_layer(activation="gelu", **given)
     check_layer(activation="gelu", keep=False, **given)
 
