@@ -7,19 +7,22 @@ namespace {
 // Rows of more than 4096 are held by 256 threads of 32 values (three blocks, whose barriers fall apart) rather than 512 of 16:
 // 6001 rows of 8192 in fp16 take 43 us and 53 us.  Their parameters are read again for every row, which with the rows' way
 // through shared memory would fill the L1 pipe (51 us), so the next row waits in registers.
-__host__ __device__ constexpr int blocks_of(int threads, int values, bool shifted) {
-  return threads > 256 ? 1 : values <= 8 ? 4 : values == 16 && !shifted ? 2 : 3;
+__host__ __device__ constexpr int rows_of(int values, int bytes, bool shifted) {
+  return !shifted && (values == 16 || (values == 32 && bytes == 2)) ? 2 : 1;
+}
+__host__ __device__ constexpr int blocks_of(int threads, int values, int bytes, bool shifted) {
+  return threads > 256 ? 1 : values <= 8 ? 4 : rows_of(values, bytes, shifted) == 2 ? 2 : 3;
 }
 
 template <typename T, typename W, bool kShifted, int kItems, int kLanes, int kMost>
-__global__ void __launch_bounds__(kMost, blocks_of(kMost, kItems * (16 / int(sizeof(T))), kShifted))
+__global__ void __launch_bounds__(kMost, blocks_of(kMost, kItems * (16 / int(sizeof(T))), sizeof(T), kShifted))
 norm_kernel(const NormParams p) {
   constexpr int kVec = norm::Values<T>::kVec, kPairs = kVec / 2;
-  constexpr int kRows = norm::rows_at_a_time(kItems * kVec, kShifted);
-  constexpr int kStages = norm::stages_of(kItems, kMost, blocks_of(kMost, kItems * kVec, kShifted));
+  constexpr int kRows = rows_of(kItems * kVec, sizeof(T), kShifted);
+  constexpr int kStages = norm::stages_of(kItems, kMost, blocks_of(kMost, kItems * kVec, sizeof(T), kShifted));
   constexpr bool kHold = kItems * kVec <= 16, kCopies = !kShifted && kHold, kAhead = !kShifted && !kHold;
   extern __shared__ uint4 slots[];  // [stage][item][thread] (not for shifted rows)
-  __shared__ float scratch[64 * kRows];
+  __shared__ __align__(8) float scratch[64 * kRows];
   pdl_trigger();
   pdl_wait();
   const int lanes = kLanes == 32 ? p.lanes : kLanes, lane = threadIdx.x & (lanes - 1);
@@ -46,15 +49,18 @@ norm_kernel(const NormParams p) {
     x += x_step, ahead -= step;
     if (++fill == kStages) fill = 0;
   };
-  uint4 next[kAhead ? kItems : 1];
-  auto load_next = [&](bool in) {
+  uint4 next[kRows][kAhead ? kItems : 1];
+  auto load_next = [&](long long from) {  // `from`: rows from the first of them on
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) next[kAhead ? i : 0] = norm::load_if(in && valid[i] > 0, x + i * lanes * kVec);
-    x += x_step;
+    for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) next[r][kAhead ? i : 0] = norm::load_if(from > r * step && valid[i] > 0, x + i * lanes * kVec);
+      x += x_step;
+    }
   };
   if constexpr (kCopies)
     for (int i = 0; i < kStages - kRows; ++i) fetch();
-  if constexpr (kAhead) load_next(left > 0);
+  if constexpr (kAhead) load_next(left);
   F2 w[kHold ? kItems : 1][kPairs] = {}, b[kHold ? kItems : 1][kPairs] = {};
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
@@ -83,7 +89,7 @@ norm_kernel(const NormParams p) {
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
         uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (kAhead) raw = next[i];
+        if constexpr (kAhead) raw = next[r][i];
         else if constexpr (kShifted) raw = norm::arrived<T, true>(pending[i], x + i * lanes * kVec, left > 0 ? valid[i] : 0);
         else if (left > r * step && valid[i] > 0) raw = lds128(slot0 + take * stage_bytes + i * blockDim.x * 16);
         const norm::Values<T> values(raw);
@@ -94,7 +100,7 @@ norm_kernel(const NormParams p) {
       if (++take == kStages) take = 0;
     }
     if (kShifted) x += x_step;
-    if constexpr (kAhead) load_next(left > step);
+    if constexpr (kAhead) load_next(left - kRows * step);
     norm::row_sums<kLanes>(s, lanes, scratch, turn);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
@@ -118,24 +124,28 @@ norm_kernel(const NormParams p) {
       s[r] = norm::sum_of(sq);
     }
     norm::row_sums<kLanes>(s, lanes, scratch, turn);
+    float rstd[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const float rstd = rsqrtf(s[r] * inv + p.eps);
-      const bool in = left > r * step;
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) {
-        if (!kHold && valid[i] > 0) {
-          norm::load_param<T, W, kShifted>(p, p.w, (i * lanes + lane) * kVec, valid[i], 1.f, w[0]);
-          norm::load_param<T, W, kShifted>(p, p.b, (i * lanes + lane) * kVec, valid[i], 0.f, b[0]);
-        }
-        const int k = kHold ? i : 0;
-#pragma unroll
-        for (int j = 0; j < kPairs; ++j) v[r][i][j] = fma2(v[r][i][j] * F2(rstd), w[k][j], b[k][j]);
-        norm::store<T, kShifted>(y + i * lanes * kVec, norm::bits_of<T>(v[r][i]), in ? valid[i] : 0, lane & (kLanes - 1), kLanes);
-      }
-      if (p.stats != nullptr && lane == 0 && in) p.stats[row + r * step] = make_float2(rstd, -mean[r] * rstd);
-      y += y_step;
+      rstd[r] = rsqrtf(s[r] * inv + p.eps);
+      if (p.stats != nullptr && lane == 0 && left > r * step) p.stats[row + r * step] = make_float2(rstd[r], -mean[r] * rstd[r]);
     }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      if (!kHold && valid[i] > 0) {
+        norm::load_param<T, W, kShifted>(p, p.w, (i * lanes + lane) * kVec, valid[i], 1.f, w[0]);
+        norm::load_param<T, W, kShifted>(p, p.b, (i * lanes + lane) * kVec, valid[i], 0.f, b[0]);
+      }
+      const int k = kHold ? i : 0;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) v[r][i][j] = fma2(v[r][i][j] * F2(rstd[r]), w[k][j], b[k][j]);
+        norm::store<T, kShifted>(y + r * y_step + i * lanes * kVec, norm::bits_of<T>(v[r][i]), left > r * step ? valid[i] : 0,
+                                 lane & (kLanes - 1), kLanes);
+      }
+    }
+    y += kRows * y_step;
   }
 }
 
@@ -170,7 +180,7 @@ int b200ta_layer_norm(const void* x, int64_t xs, const void* weight, const void*
   const NormShape s = norm_shape(width, vec, 256, !whole);
   p.lanes = s.lanes;
   const int64_t per_block = s.threads / s.lanes, need = (rows + per_block - 1) / per_block;
-  const int resident = blocks_of(s.threads, s.items * vec, s.shifted);  // blocks that run at once on a multiprocessor
+  const int resident = blocks_of(s.threads, s.items * vec, bytes, s.shifted);  // blocks that run at once on a multiprocessor
   const int64_t most = int64_t(st->num_sms) * resident;
   const int smem = whole && s.items * vec <= 16 ? norm::stages_of(s.items, s.threads, resident) * s.items * s.threads * 16 : 0;
   const bool f32 = param_dtype == B200TA_DTYPE_F32;

@@ -266,9 +266,18 @@ __device__ __forceinline__ void row_sums(float (&s)[kSums], int lanes, float* sc
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kSums; ++i) s[i] = 0.f;
-    for (int w = first; w < first + warps; ++w)
+    for (int w = first; w < first + warps; w += 2)  // two warps' in one access
 #pragma unroll
-      for (int i = 0; i < kSums; ++i) s[i] += half[w * kSums + i];
+      for (int i = 0; i < kSums; i += 2) {
+        if constexpr (kSums == 1) {
+          const float2 x = *reinterpret_cast<const float2*>(half + w);
+          s[0] += x.x + x.y;
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(half + w * kSums + i);
+          const float2 z = *reinterpret_cast<const float2*>(half + (w + 1) * kSums + i);
+          s[i] += x.x + z.x, s[i + 1] += x.y + z.y;
+        }
+      }
   }
 }
 

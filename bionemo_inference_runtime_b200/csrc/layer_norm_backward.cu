@@ -21,7 +21,7 @@ norm_grad_kernel(const NormParams p) {
   constexpr bool kKeep = kRows == 1 && kHold;  // xh and g stay in registers between the two passes over a row
   extern __shared__ uint4 slots[];    // [stage][x items, dy items][thread] (not for shifted rows); joined sums at the end
   float* joined = reinterpret_cast<float*>(slots);  // [groups / 2][2][width]
-  __shared__ float scratch[128 * kRows];
+  __shared__ __align__(8) float scratch[128 * kRows];
   pdl_trigger();
   pdl_wait();
   const int lanes = kLanes == 32 ? p.lanes : kLanes, lane = threadIdx.x & (lanes - 1);
