@@ -473,8 +473,9 @@ copy_rows_kernel(const CopyParams p) {
     if (job.column_stride == 1) {
       const long long r = v / vectors;
       const int c = int(v - r * vectors) * 8, valid = job.columns - c;
-      const __half* from = reinterpret_cast<const __half*>(src + r * job.row_stride + c);
-      *reinterpret_cast<uint4*>(dst + r * job.dst_row_stride + c) = norm::arrived<__half, true>(norm::load<__half, true>(from, valid), from, valid);
+      const __half* row = reinterpret_cast<const __half*>(src + r * job.row_stride);
+      const uint4 x = norm::load_anywhere(row + c, row, job.columns);
+      *reinterpret_cast<uint4*>(dst + r * job.dst_row_stride + c) = valid >= 8 ? x : norm::first<__half>(x, valid);
     } else {
       const long long c = v / job.rows * 8, r = v - v / job.rows * job.rows;
       uint32_t w[4];

@@ -5,16 +5,20 @@
 //   dw = sum over rows of dy xh,  db = sum over rows of dy
 //
 // Bound: HBM.  Forward reads x and writes y, backward reads x and dy and writes dx, each once: a row is held in the
-// registers of the 2 to 1024 threads that share it, and its mean and variance, or its two sums, are taken there in 32 bits,
+// registers of the 2 to 512 threads that share it, and its mean and variance, or its two sums, are taken there in 32 bits,
 // the variance from centred values.  Issue slots come next (a first version with 64-bit index arithmetic and unpacked sums
 // needed 200 instructions for 16 values a lane and stayed at half the bandwidth), so addresses advance by constants, sums
 // and products are made in packed pairs, and groups of lanes have a size known at compile time.  Blocks are persistent; a
 // thread keeps its columns, and with them their parameters in registers (of up to 16 columns), and copies the next rows' vectors into its own slots
 // of shared memory while it works on one (registers alone hold too few bytes in flight).
 //
-// Rows that are not 16-byte aligned (odd widths, odd pitches) take the same path with aligned loads that are shifted into
-// place in registers and stores that are shifted back between neighbouring lanes; only the ends of a warp's segment are
-// stored by elements.  (A 16-byte vector with a byte of the row in it lies in the row's allocation.)
+// Rows that are not 16-byte aligned (odd widths, odd pitches) take the same path: vectors lie on the 16-byte boundaries of the
+// row that is written, and the at most 2 * 7 elements (fp32: 3) before the first and behind the last whole vector are taken by
+// the row's first lanes, an element each.  Blocks step by a multiple of 8 (fp32: 4) rows, after which every pitch is back on
+// the same boundary, so a thread keeps its columns.  A tensor whose rows lie otherwise is read by two aligned vectors that are
+// shifted into place.  (A 16-byte vector with a byte of the row in it lies in the row's allocation.)  Vectors on the boundaries
+// of x's columns instead, shifted on their way in and out, cost three times the instructions: 9000 rows of 1027 in bf16 took 39 us
+// forward and 50 backward, now 16 and 28; 100000 of 127 took 29 and 36, now 18 and 28.
 #pragma once
 
 #include "activation.cuh"
@@ -30,7 +34,6 @@ struct NormParams {
   long long xs, ys, dys, dxs, rows;
   int width;
   int lanes;           // threads that share a row, a power of two
-  int params_aligned;  // the parameters may be read by vectors
   float eps;
 };
 
@@ -40,20 +43,26 @@ struct NormShape {
 };
 constexpr int kNormThreads = 256;  // of a block, unless a row takes more
 constexpr int kNormMaxWidth = 16384;
-// Threads that share a row: a warp or less (from 2), or up to `most_lanes` of them, as long as 16 values a thread hold the row;
+// Threads that share a row: a warp or less (from 2, shifted 8), or up to `most_lanes` of them, as long as 16 values a thread hold the row;
 // up to 512 with 32 values for what is wider.
 inline NormShape norm_shape(int width, int vec, int most_lanes, bool shifted) {
   NormShape s;
   s.shifted = shifted;
-  const int n = (width + vec - 1) / vec, most = (n > most_lanes * 16 / vec ? 32 : 16) / vec;
-  s.lanes = 2;
+  const int n = width / vec, most = (n > most_lanes * 16 / vec ? 32 : 16) / vec;
+  s.lanes = shifted ? 8 : 2;  // (with fewer a lane would take four or eight single elements)
   while (s.lanes < 32 && s.lanes < n) s.lanes *= 2;
   while (s.lanes * most < n) s.lanes *= 2;
-  s.items = (n + s.lanes - 1) / s.lanes;
+  s.items = n > 0 ? (n + s.lanes - 1) / s.lanes : 1;
   // the kernels are made for 1, 2 and all items of 16 values, and for those of 32
   s.items = s.items <= 2 ? s.items : s.items * vec <= 16 ? 16 / vec : 32 / vec;
   s.threads = s.lanes > kNormThreads ? s.lanes : kNormThreads;
   return s;
+}
+// Blocks of a grid, at most `most`: those of shifted rows step by whole periods of their alignment.
+inline int norm_blocks(int64_t rows, int64_t most, int per_block, int vec, bool shifted) {
+  const int64_t need = (rows + per_block - 1) / per_block;
+  if (need <= most) return int(need);
+  return int(shifted && per_block < vec ? most - most % (vec / per_block) : most);
 }
 inline int norm_element_bytes(int dtype) { return dtype == B200TA_DTYPE_F32 ? 4 : 2; }
 inline bool norm_aligned(const void* p, int64_t stride, int bytes) {
@@ -121,7 +130,7 @@ __device__ __forceinline__ uint4 first(uint4 x, int valid) {
 
 // Rows that a group of threads works on at a time: two where a thread holds 16 values, so that a row's sums over the group
 // (shuffles, and a barrier beyond a warp) cost half.
-__host__ __device__ constexpr int rows_at_a_time(int values, bool shifted) { return values == 16 && !shifted ? 2 : 1; }
+__host__ __device__ constexpr int rows_at_a_time(int values) { return values == 16 ? 2 : 1; }
 // Slots of shared memory for rows of `vectors` vectors a thread, those that are worked on included.
 __host__ __device__ constexpr int stages_of(int vectors, int threads, int blocks) {
   const int by_bytes = 196608 / blocks / (vectors * threads * 16);
@@ -146,64 +155,19 @@ __device__ __forceinline__ uint4 load_if(bool in, const void* p) {
       : "l"(p), "r"(static_cast<uint32_t>(in)));
   return v;
 }
-// A vector of a row from `p` on, `valid` elements of which are in the row: the one or two aligned vectors that hold it, and the
-// vector itself once they are there.
-struct Pending {
-  uint4 lo, hi;
-};
-template <typename T, bool kShifted>
-__device__ __forceinline__ Pending load(const T* p, int valid) {
-  if constexpr (!kShifted) {
-    return {load_if(valid > 0, p), uint4()};
-  } else {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(p), base = a & ~uintptr_t(15);
-    const uint32_t at = uint32_t(a & 15u), bytes = (valid < Values<T>::kVec ? valid : Values<T>::kVec) * uint32_t(sizeof(T));
-    return {load_if(valid > 0, reinterpret_cast<const void*>(base)),
-            load_if(valid > 0 && at + bytes > 16u, reinterpret_cast<const void*>(base + 16))};
-  }
+// The vector at `p`, of any alignment, of a row of `width` elements from `row` on: from the two aligned vectors that hold it, as
+// far as they touch the row.
+template <typename T>
+__device__ __forceinline__ uint4 load_anywhere(const T* p, const T* row, int width) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), at = a & 15u, lo = a - at, hi = lo + 16;
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(row), end = begin + width * sizeof(T);
+  const uint4 x = load_if(hi > begin && lo < end, reinterpret_cast<const void*>(lo));
+  const uint4 z = load_if(at != 0 && hi + 16 > begin && hi < end, reinterpret_cast<const void*>(hi));
+  return window<T>(x, z, uint32_t(at));
 }
-template <typename T, bool kShifted>
-__device__ __forceinline__ uint4 arrived(const Pending& x, const T* p, int valid) {
-  if constexpr (!kShifted) {
-    return x.lo;
-  } else {
-    const uint4 v = window<T>(x.lo, x.hi, uint32_t(reinterpret_cast<uintptr_t>(p) & 15u));
-    return valid >= Values<T>::kVec ? v : first<T>(v, valid);
-  }
-}
-// Stores a vector of a row at `p`, the `index`-th of the `lanes` vectors that neighbouring lanes of this warp store, all of
-// which call this; valid <= 0: nothing of it is in the row.
-template <typename T, bool kShifted>
-__device__ __forceinline__ void store(T* p, uint4 x, int valid, int index, int lanes) {
-  constexpr int kVec = Values<T>::kVec;
-  if constexpr (!kShifted) {
-    if (valid > 0) *reinterpret_cast<uint4*>(p) = x;
-  } else {
-    const uint32_t at = uint32_t(reinterpret_cast<uintptr_t>(p) & 15u);
-    const int own = at == 0 ? kVec : int((16u - at) / sizeof(T));  // elements up to the next 16-byte boundary
-    uint4 before;
-    before.x = __shfl_up_sync(0xffffffffu, x.x, 1), before.y = __shfl_up_sync(0xffffffffu, x.y, 1);
-    before.z = __shfl_up_sync(0xffffffffu, x.z, 1), before.w = __shfl_up_sync(0xffffffffu, x.w, 1);
-    // the aligned vector that ends in this lane's first elements; the one behind it is the next lane's
-    const bool whole = valid >= own && (at == 0 || index > 0);
-    const bool next = at == 0 || (index + 1 < lanes && valid - kVec >= own);
-    if (whole) *reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(p) - at) = at == 0 ? x : window<T>(before, x, 16u - at);
-    if (!(whole && next)) {
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        if (e < valid && !(e < own ? whole : next)) {
-          if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[e] = w[e];
-          else reinterpret_cast<uint16_t*>(p)[e] = uint16_t(w[e / 2] >> (16 * (e & 1)));
-        }
-      }
-    }
-  }
-}
-
-template <typename W>
-__device__ __forceinline__ float element_if(bool in, const W* p) {
-  if constexpr (sizeof(W) == 4) {
+template <typename T>
+__device__ __forceinline__ float element_if(bool in, const T* p) {  // zero without an access
+  if constexpr (sizeof(T) == 4) {
     float v;
     asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\nmov.f32 %0, 0f00000000;\n@q ld.global.nc.f32 %0, [%1];\n}"
                  : "=&f"(v) : "l"(p), "r"(static_cast<uint32_t>(in)));
@@ -212,34 +176,54 @@ __device__ __forceinline__ float element_if(bool in, const W* p) {
     uint16_t v;
     asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\nmov.u16 %0, 0;\n@q ld.global.nc.u16 %0, [%1];\n}"
                  : "=&h"(v) : "l"(p), "r"(static_cast<uint32_t>(in)));
-    return unpack2<W>(uint32_t(v)).x;
+    return unpack2<T>(uint32_t(v)).x;
   }
 }
-// The parameters of kVec columns from c on, `valid` of them in the row, or `none` where there are none.
+
+// How a thread's part of a row lies: whole vectors from `column` on, one every lanes * kVec columns, and (kShifted) single
+// elements before the first and behind the last vector of the row, kSingles of them at most.
+template <typename T, bool kShifted, int kLanes>
+struct Place {
+  static constexpr int kVec = Values<T>::kVec;
+  static constexpr int kSingles = !kShifted ? 0 : kLanes >= 2 * kVec ? 1 : 2 * kVec / kLanes, kSlots = kSingles ? kSingles : 1;
+  int vectors;         // of the row, from this lane's first on
+  int column;
+  int single[kSlots];  // their columns, -1: none
+  __device__ __forceinline__ Place(const T* row, int width, int lane, int lanes) {
+    const int before = int((16u - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / int(sizeof(T));
+    const int head = !kShifted ? 0 : before < width ? before : width, all = (width - head) / kVec, rest = head + all * kVec;
+    vectors = all - lane, column = head + lane * kVec;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      const int e = lane + i * lanes, c = e < kVec ? e : rest + e - kVec;
+      single[i] = kShifted && (e < kVec ? e < head : e < 2 * kVec && c < width) ? c : -1;
+    }
+  }
+};
+
+// The parameters of kVec columns from c on, or `none` where there are none.
 template <typename T, typename W, bool kShifted>
-__device__ __forceinline__ void load_param(const NormParams& p, const void* param, int c, int valid, float none, F2* v) {
-  constexpr int kVec = Values<T>::kVec;
+__device__ __forceinline__ void load_param(const NormParams& p, const void* param, int c, float none, F2* v) {
+  constexpr int kVec = Values<T>::kVec, kHalf = Values<W>::kVec;
   if (param == nullptr) {
 #pragma unroll
     for (int j = 0; j < kVec / 2; ++j) v[j] = F2(none);
-  } else if (!kShifted || (p.params_aligned && valid >= kVec)) {
-    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const W*>(param) + c);
-    if constexpr (sizeof(W) == sizeof(T)) {
-      const Values<W> x(__ldg(q));
-#pragma unroll
-      for (int j = 0; j < kVec / 2; ++j) v[j] = x.p[j];
-    } else {
-      const Values<float> lo(__ldg(q)), hi(__ldg(q + 1));
-      v[0] = lo.p[0], v[1] = lo.p[1], v[2] = hi.p[0], v[3] = hi.p[1];
-    }
-  } else {
-    const W* q = static_cast<const W*>(param) + c;
-    float f[kVec];
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) f[j] = element_if(j < valid, q + j);
-#pragma unroll
-    for (int j = 0; j < kVec / 2; ++j) v[j] = F2(f[2 * j], f[2 * j + 1]);
+    return;
   }
+  const W* q = static_cast<const W*>(param) + c;
+#pragma unroll
+  for (int h = 0; h < kVec; h += kHalf) {  // 16-bit rows with 32-bit parameters: two vectors
+    uint4 raw;
+    if constexpr (kShifted) raw = load_anywhere(q + h, static_cast<const W*>(param), p.width);
+    else raw = __ldg(reinterpret_cast<const uint4*>(q + h));
+    const Values<W> x(raw);
+#pragma unroll
+    for (int j = 0; j < kHalf / 2; ++j) v[h / 2 + j] = x.p[j];
+  }
+}
+template <typename W>
+__device__ __forceinline__ float single_param(const void* param, int c, float none) {
+  return param == nullptr ? none : element_if(c >= 0, static_cast<const W*>(param) + c);
 }
 
 __device__ __forceinline__ float sum_of(F2 p) {
@@ -299,8 +283,8 @@ int launch_one(DeviceState* st, int blocks, int threads, int smem, void* stream,
   (s.threads > 256 && s.items > int(sizeof(T))                                       \
        ? &norm::launch_one<kernel<T, W, kShifted, 2 * int(sizeof(T)), 32, 512>>      \
    : s.threads > 256     ? &norm::launch_one<kernel<T, W, kShifted, int(sizeof(T)), 32, 512>>         \
-   : s.lanes == 2        ? &norm::launch_one<kernel<T, W, kShifted, 1, 2, 256>>                       \
-   : s.lanes == 4        ? &norm::launch_one<kernel<T, W, kShifted, 1, 4, 256>>                       \
+   : s.lanes == 2        ? &norm::launch_one<kernel<T, W, kShifted, 1, kShifted ? 8 : 2, 256>>                       \
+   : s.lanes == 4        ? &norm::launch_one<kernel<T, W, kShifted, 1, kShifted ? 8 : 4, 256>>                       \
    : s.lanes == 8        ? &norm::launch_one<kernel<T, W, kShifted, 1, 8, 256>>                       \
    : s.lanes == 16       ? &norm::launch_one<kernel<T, W, kShifted, 1, 16, 256>>                      \
    : s.items == 1        ? &norm::launch_one<kernel<T, W, kShifted, 1, 32, 256>>                      \

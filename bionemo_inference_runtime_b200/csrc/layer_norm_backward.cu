@@ -8,18 +8,21 @@
 namespace b200ta {
 namespace {
 
-// Blocks of a multiprocessor: 8 values a thread leave room for three of 256 threads, more for two.
-__host__ __device__ constexpr int grad_blocks_of(int threads, int values) { return threads > 256 ? 1 : values <= 8 ? 3 : 2; }
+// Blocks of a multiprocessor: 8 values a thread leave room for three of 256 threads, more (or single elements beside
+// them) for two.
+__host__ __device__ constexpr int grad_blocks_of(int threads, int values, bool shifted) {
+  return threads > 256 ? 1 : values <= 8 && !shifted ? 3 : 2;
+}
 
 template <typename T, typename W, bool kShifted, int kItems, int kLanes, int kMost>
-__global__ void __launch_bounds__(kMost, grad_blocks_of(kMost, kItems * norm::Values<T>::kVec))
+__global__ void __launch_bounds__(kMost, grad_blocks_of(kMost, kItems * norm::Values<T>::kVec, kShifted))
 norm_grad_kernel(const NormParams p) {
   constexpr int kVec = norm::Values<T>::kVec, kPairs = kVec / 2;
-  constexpr int kRows = norm::rows_at_a_time(kItems * kVec, kShifted);
-  constexpr int kStages = norm::stages_of(2 * kItems, kMost, grad_blocks_of(kMost, kItems * kVec));
+  constexpr int kRows = norm::rows_at_a_time(kItems * kVec);
+  constexpr int kStages = norm::stages_of(2 * kItems, kMost, grad_blocks_of(kMost, kItems * kVec, kShifted));
   constexpr bool kHold = kItems * kVec <= 16;
   constexpr bool kKeep = kRows == 1 && kHold;  // xh and g stay in registers between the two passes over a row
-  extern __shared__ uint4 slots[];    // [stage][x items, dy items][thread] (not for shifted rows); joined sums at the end
+  extern __shared__ uint4 slots[];    // [stage][x items, dy items][thread]; joined sums at the end
   float* joined = reinterpret_cast<float*>(slots);  // [groups / 2][2][width]
   __shared__ __align__(8) float scratch[128 * kRows];
   pdl_trigger();
@@ -27,13 +30,19 @@ norm_grad_kernel(const NormParams p) {
   const int lanes = kLanes == 32 ? p.lanes : kLanes, lane = threadIdx.x & (lanes - 1);
   const int per_block = blockDim.x / lanes, group = threadIdx.x / lanes;
   const float inv = 1.f / float(p.width);
-  int turn = 0, valid[kItems];
-#pragma unroll
-  for (int i = 0; i < kItems; ++i) valid[i] = p.width - (i * lanes + lane) * kVec;
   const long long row0 = (long long)blockIdx.x * per_block + group, step = (long long)gridDim.x * per_block;
-  const T* x = static_cast<const T*>(p.x) + row0 * p.xs + lane * kVec;
-  const T* dy = static_cast<const T*>(p.dy) + row0 * p.dys + lane * kVec;
-  T* dx = static_cast<T*>(p.dx) + row0 * p.dxs + lane * kVec;
+  const T* x = static_cast<const T*>(p.x) + row0 * p.xs;
+  const T* dy = static_cast<const T*>(p.dy) + row0 * p.dys;
+  T* dx = static_cast<T*>(p.dx) + row0 * p.dxs;
+  const norm::Place<T, kShifted, kLanes> place(p.dx != nullptr ? dx : x, p.width, lane, lanes);
+  constexpr int kSingles = place.kSingles, kSlots = place.kSlots;
+  auto has = [&](int i) { return place.vectors > i * lanes; };
+  int turn = 0;
+  const T *x_row = x, *dy_row = dy;  // of the single elements that are fetched next
+  T* dx_row = dx;
+  x += place.column, dy += place.column, dx += place.column;
+  const bool same_x = !kShifted || (reinterpret_cast<uintptr_t>(x) & 15u) == 0;  // lies as dx does
+  const bool same_dy = !kShifted || (reinterpret_cast<uintptr_t>(dy) & 15u) == 0;
   const float2* stats = p.stats + row0;
   long long left = p.rows - row0, block_left = p.rows - (long long)blockIdx.x * per_block;
   const uint32_t slot0 = smem_u32(slots) + threadIdx.x * 16, item_bytes = blockDim.x * 16, stage_bytes = 2 * kItems * item_bytes;
@@ -43,20 +52,39 @@ norm_grad_kernel(const NormParams p) {
     if (ahead > 0)
 #pragma unroll
       for (int i = 0; i < kItems; ++i)
-        if (valid[i] > 0) {
-          norm::copy_ahead(slot0 + fill * stage_bytes + i * item_bytes, x + i * lanes * kVec);
-          norm::copy_ahead(slot0 + fill * stage_bytes + (kItems + i) * item_bytes, dy + i * lanes * kVec);
+        if (has(i)) {
+          const int c = i * lanes * kVec;
+          const uint32_t to_x = slot0 + fill * stage_bytes + i * item_bytes, to_dy = to_x + kItems * item_bytes;
+          if (same_x) norm::copy_ahead(to_x, x + c);
+          else sts128(to_x, norm::load_anywhere(x + c, x - place.column, p.width));
+          if (same_dy) norm::copy_ahead(to_dy, dy + c);
+          else sts128(to_dy, norm::load_anywhere(dy + c, dy - place.column, p.width));
         }
     norm::copy_commit();
     x += step * p.xs, dy += step * p.dys, ahead -= step;
     if (++fill == kStages) fill = 0;
   };
-  if constexpr (!kShifted)
-    for (int i = 0; i < kStages - kRows; ++i) fetch();
+  for (int i = 0; i < kStages - kRows; ++i) fetch();
+  float2 next_single[kRows][kSlots];  // {x, dy}
+  float single_w[kSlots], single_dw[kSlots] = {}, single_db[kSlots] = {};
+  auto load_singles = [&](long long from) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+      for (int i = 0; i < kSingles; ++i) {
+        const bool in = from > r * step && place.single[i] >= 0;
+        next_single[r][i] = make_float2(norm::element_if(in, x_row + place.single[i]), norm::element_if(in, dy_row + place.single[i]));
+      }
+      x_row += step * p.xs, dy_row += step * p.dys;
+    }
+  };
+  if constexpr (kSingles > 0) load_singles(left);
+#pragma unroll
+  for (int i = 0; i < kSingles; ++i) single_w[i] = norm::single_param<W>(p.w, place.single[i], 1.f);
   F2 dw[kItems][kPairs] = {}, db[kItems][kPairs] = {}, w[kHold ? kItems : 1][kPairs] = {};
 #pragma unroll
   for (int i = 0; i < kItems; ++i)
-    if (kHold && valid[i] > 0) norm::load_param<T, W, kShifted>(p, p.w, (i * lanes + lane) * kVec, valid[i], 1.f, w[kHold ? i : 0]);
+    if (kHold && has(i)) norm::load_param<T, W, kShifted>(p, p.w, place.column + i * lanes * kVec, 1.f, w[kHold ? i : 0]);
   float2 next[kRows];
   auto fetch_stats = [&](long long rows_left) {
 #pragma unroll
@@ -71,35 +99,19 @@ norm_grad_kernel(const NormParams p) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) st[r] = next[r];
     fetch_stats(left - kRows * step);
-    if constexpr (!kShifted) {
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) fetch();
-      norm::copy_wait<kStages - kRows>();
-    }
-    norm::Pending px[kShifted ? kItems : 1], pdy[kShifted ? kItems : 1];
-    auto request = [&]() {
-      if constexpr (kShifted) {
-#pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-          px[i] = norm::load<T, true>(x + i * lanes * kVec, left > 0 ? valid[i] : 0);
-          pdy[i] = norm::load<T, true>(dy + i * lanes * kVec, left > 0 ? valid[i] : 0);
-        }
-      }
-    };
-    request();
+    for (int r = 0; r < kRows; ++r) fetch();
+    norm::copy_wait<kStages - kRows>();
     // xh and g = dy w of item i of a row; with kSum also dw and db
     auto load = [&](int i, int r, int stage, auto sum) {
       uint4 raw_x = make_uint4(0u, 0u, 0u, 0u), raw_dy = raw_x;
-      if constexpr (kShifted) {
-        raw_x = norm::arrived<T, true>(px[i], x + i * lanes * kVec, left > 0 ? valid[i] : 0);
-        raw_dy = norm::arrived<T, true>(pdy[i], dy + i * lanes * kVec, left > 0 ? valid[i] : 0);
-      } else if (left > r * step && valid[i] > 0) {
+      if (left > r * step && has(i)) {
         raw_x = lds128(slot0 + stage * stage_bytes + i * item_bytes);
         raw_dy = lds128(slot0 + stage * stage_bytes + (kItems + i) * item_bytes);
       }
       const norm::Values<T> vx(raw_x), vd(raw_dy);
       const int k = kKeep ? i : 0, kw = kHold ? i : 0;
-      if (!kHold && valid[i] > 0) norm::load_param<T, W, kShifted>(p, p.w, (i * lanes + lane) * kVec, valid[i], 1.f, w[0]);
+      if (!kHold && has(i)) norm::load_param<T, W, kShifted>(p, p.w, place.column + i * lanes * kVec, 1.f, w[0]);
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
         // (behind the row dy is zero, and what xh is there does not count)
@@ -111,6 +123,7 @@ norm_grad_kernel(const NormParams p) {
         g[k][j] = vd.p[j] * w[kw][j];
       }
     };
+    float2 single[kRows][kSlots];  // {xh, g}
     int stage = take;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
@@ -122,11 +135,19 @@ norm_grad_kernel(const NormParams p) {
         for (int j = 0; j < kPairs; ++j) s0 = s0 + g[kKeep ? i : 0][j], s1 = fma2(g[kKeep ? i : 0][j], xh[kKeep ? i : 0][j], s1);
       }
       s[2 * r] = norm::sum_of(s0), s[2 * r + 1] = norm::sum_of(s1);
+#pragma unroll
+      for (int i = 0; i < kSingles; ++i) {
+        const float2 v = next_single[r][i];
+        const float xh_i = fmaf(v.x, st[r].x, st[r].y), g_i = v.y * single_w[i];
+        single_dw[i] = fmaf(v.y, xh_i, single_dw[i]), single_db[i] += v.y;
+        s[2 * r] += g_i, s[2 * r + 1] = fmaf(g_i, xh_i, s[2 * r + 1]);
+        single[r][i] = make_float2(xh_i, g_i);
+      }
       if (++stage == kStages) stage = 0;
     }
+    if constexpr (kSingles > 0) load_singles(left - kRows * step);
     if (p.dx != nullptr) {
       norm::row_sums<kLanes>(s, lanes, scratch, turn);
-      if (!kKeep) request();
       stage = take;
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
@@ -137,36 +158,43 @@ norm_grad_kernel(const NormParams p) {
           F2 out[kPairs];
 #pragma unroll
           for (int j = 0; j < kPairs; ++j) out[j] = fma2(xh[kKeep ? i : 0][j], c, fma2(g[kKeep ? i : 0][j], a, b));
-          norm::store<T, kShifted>(dx + i * lanes * kVec, norm::bits_of<T>(out), left > r * step ? valid[i] : 0, lane & (kLanes - 1), kLanes);
+          if (has(i) && left > r * step) *reinterpret_cast<uint4*>(dx + i * lanes * kVec) = norm::bits_of<T>(out);
         }
+#pragma unroll
+        for (int i = 0; i < kSingles; ++i) {
+          const float out = -(single[r][i].x * s[2 * r + 1] + s[2 * r]) * inv * st[r].x + single[r][i].y * st[r].x;
+          if (place.single[i] >= 0 && left > r * step) dx_row[place.single[i]] = static_cast<T>(out);
+        }
+        dx_row += step * p.dxs;
         dx += step * p.dxs;
         if (++stage == kStages) stage = 0;
       }
     }
-    if (kShifted) x += step * p.xs, dy += step * p.dys;
     take = stage;
   }
   if (p.partial == nullptr) return;
   norm::copy_wait<0>();
   __syncthreads();  // the slots are free
   // the groups' sums, joined in pairs: half of the groups that are left hand theirs to the other half
-  auto each = [&](float* at, bool add) {
+  auto each = [&](float* to, bool add) {
 #pragma unroll
     for (int i = 0; i < kItems; ++i)
 #pragma unroll
       for (int j = 0; j < kPairs; ++j) {
-        const int c = (i * lanes + lane) * kVec + 2 * j;
+        const int c = place.column + i * lanes * kVec + 2 * j;
         float w0, w1, b0, b1;
         dw[i][j].to(w0, w1), db[i][j].to(b0, b1);
-        if (add) {
-          if (c < p.width) w0 += at[c], b0 += at[p.width + c];
-          if (c + 1 < p.width) w1 += at[c + 1], b1 += at[p.width + c + 1];
-          dw[i][j] = F2(w0, w1), db[i][j] = F2(b0, b1);
-        } else {
-          if (c < p.width) at[c] = w0, at[p.width + c] = b0;
-          if (c + 1 < p.width) at[c + 1] = w1, at[p.width + c + 1] = b1;
-        }
+        if (!has(i)) continue;
+        if (add) dw[i][j] = F2(w0 + to[c], w1 + to[c + 1]), db[i][j] = F2(b0 + to[p.width + c], b1 + to[p.width + c + 1]);
+        else to[c] = w0, to[c + 1] = w1, to[p.width + c] = b0, to[p.width + c + 1] = b1;
       }
+#pragma unroll
+    for (int i = 0; i < kSingles; ++i) {
+      const int c = place.single[i];
+      if (c < 0) continue;
+      if (add) single_dw[i] += to[c], single_db[i] += to[p.width + c];
+      else to[c] = single_dw[i], to[p.width + c] = single_db[i];
+    }
   };
   for (int left_groups = per_block; left_groups > 1; left_groups >>= 1) {
     const int half = left_groups >> 1;
@@ -243,18 +271,16 @@ int b200ta_layer_norm_backward(const void* dy, int64_t dys, const void* x, int64
   p.x = x, p.dy = dy, p.w = weight, p.dx = dx, p.stats = static_cast<float2*>(const_cast<void*>(stats));
   p.partial = sums ? static_cast<float*>(workspace) : nullptr;
   p.xs = xs, p.dys = dys, p.dxs = dxs, p.rows = rows, p.width = width;
-  p.params_aligned = norm_aligned(weight, 0, 4);
   const int bytes = norm_element_bytes(dtype), vec = 16 / bytes;
   const bool whole = width % vec == 0 && norm_aligned(x, xs, bytes) && norm_aligned(dy, dys, bytes) &&
-                     (!dx || norm_aligned(dx, dxs, bytes)) && p.params_aligned;
+                     (!dx || norm_aligned(dx, dxs, bytes)) && norm_aligned(weight, 0, 4);
   const NormShape s = norm_shape(width, vec, 512, !whole);
   p.lanes = s.lanes;
-  const int groups = s.threads / s.lanes, resident = grad_blocks_of(s.threads, s.items * vec);
+  const int groups = s.threads / s.lanes, resident = grad_blocks_of(s.threads, s.items * vec, s.shifted);
   const int joined = sums && groups > 1 ? groups / 2 * 2 * width * int(sizeof(float)) : 0;
-  const int ring = whole ? norm::stages_of(2 * s.items, s.threads, resident) * 2 * s.items * s.threads * 16 : 0;
+  const int ring = norm::stages_of(2 * s.items, s.threads, resident) * 2 * s.items * s.threads * 16;
   const int smem = joined > ring ? joined : ring;
-  const int64_t need = (rows + groups - 1) / groups, most = int64_t(st->num_sms) * resident;
-  const int blocks = int(need < most ? need : most);
+  const int blocks = norm_blocks(rows, int64_t(st->num_sms) * resident, groups, vec, s.shifted);
   const bool f32 = param_dtype == B200TA_DTYPE_F32;
   int (*launch)(DeviceState*, int, int, int, void*, const NormParams&);
   if (dtype == B200TA_DTYPE_BF16) launch = f32 ? pick<__nv_bfloat16, float>(s) : pick<__nv_bfloat16, __nv_bfloat16>(s);

@@ -119,6 +119,26 @@ def test_layer_norm_of_rows_with_a_large_mean_and_of_constant_rows():
     assert (y == 0).all() and torch.allclose(stats[:, 0], torch.full((4,), 1e-5 ** -0.5, device=DEV), rtol=1e-5)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,width", [(3000, 1), (2500, 5), (2500, 9), (3001, 15), (2000, 24), (1500, 127), (700, 519), (900, 4093), (310, 8190)])
+def test_layer_norm_rows_on_other_boundaries(rows, width, dtype):
+    """Rows of odd pitches and offsets, more of them than run at once: x, dy and the results each on boundaries of their own."""
+    wide = width + 6
+    x, dy = (randn(rows * wide + 16, seed=s, dtype=dtype, std=d) for s, d in ((1, 1.5), (2, 0.1)))
+    w, b = randn(width + 1, seed=3, dtype=dtype, mean=1.0)[1:], randn(width + 1, seed=4, dtype=dtype)[1:]
+    for x_first, x_pitch, dy_first, dy_pitch in ((0, width, 0, width), (3, width + 1, 1, width), (5, width + 2, 2, width + 5)):
+        xs = x[x_first:].as_strided((rows, width), (x_pitch, 1))
+        dys = dy[dy_first:].as_strided((rows, width), (dy_pitch, 1))
+        check_norm(xs, w, b, dys)
+        held, again = (torch.zeros(rows * wide + 8, device=DEV, dtype=dtype) for _ in range(2))
+        places = [t[1:].as_strided((rows, width), (wide - 1, 1)) for t in (held, again)]
+        ops.layer_norm(xs, w, b, out=places[0])
+        ops.layer_norm(xs.contiguous(), w, b, out=places[1])  # the same rows to the same boundaries: the same sums
+        assert torch.equal(held, again)
+        places[0].zero_()
+        assert not held.any()
+
+
 def test_layer_norm_strides_and_leading_shapes():
     base = randn(6, 5, 3, 160, seed=1)
     for x in (base[..., 7:107], base[:, 1:4, :, ::2], base.transpose(0, 2), base[:, :, 1], base.permute(0, 1, 3, 2), base[:0],
