@@ -3,6 +3,7 @@
 // of what a TMA load cannot address (odd pitches, transposed or broadcast tensors).
 #include "torch_host.h"
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
@@ -56,6 +57,11 @@ void require_like(const char* name, const at::Tensor& t, const at::Tensor& x, at
   }
 }
 
+// Memory from PyTorch's caching allocator without a pass through its dispatcher, which a call of 5 us would notice.
+at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(shape, type, like.device(), at::MemoryFormat::Contiguous));
+}
+
 // A tensor [..., K] as rows of K elements with one stride, copied by PyTorch only where there is no such stride.
 struct Rows {
   at::Tensor held;
@@ -101,7 +107,7 @@ struct Copies {
 Rows operand(const at::Tensor& t, bool few, Copies& copies) {
   Rows r = rows_of(t);
   if (r.column_stride == 1 && (few || tma_takes(r.ptr, r.rows, r.columns, r.stride))) return r;
-  const at::Tensor copy = at::empty({r.rows, pad8(r.columns)}, t.options().memory_format(c10::MemoryFormat::Contiguous));
+  const at::Tensor copy = empty({r.rows, pad8(r.columns)}, t.scalar_type(), t);
   copies.jobs[copies.count++] = {r.ptr, r.stride, r.column_stride, copy.data_ptr(), copy.stride(0), r.rows, int(r.columns)};
   copies.held[copies.count - 1] = r.held;
   return {copy, copy.data_ptr(), r.rows, r.columns, copy.stride(0), 1};
@@ -114,18 +120,18 @@ Rows result_in(const at::Tensor& out) {
   return r;
 }
 at::Tensor empty_rows(const at::Tensor& x, int64_t columns) {
-  std::vector<int64_t> shape = x.sizes().vec();
+  c10::SmallVector<int64_t, 8> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = columns;
-  return at::empty(shape, x.options().memory_format(c10::MemoryFormat::Contiguous));
+  return empty(shape, x.scalar_type(), x);
 }
-at::Tensor bytes(const at::Tensor& x, size_t n) { return at::empty({int64_t(n)}, x.options().dtype(at::kByte)); }
+at::Tensor bytes(const at::Tensor& x, size_t n) { return empty({int64_t(n)}, at::kByte, x); }
 int width_of(const char* what, const at::Tensor& x) {
   if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) >= (int64_t(1) << 30)) refuse(std::string(what) + ": x must be [..., width], got " + shape_of(x));
   return int(x.size(-1));
 }
 at::Tensor or_out(const Maybe& out, const at::Tensor& x, int64_t columns) {
   if (!out) return empty_rows(x, columns);
-  std::vector<int64_t> shape = x.sizes().vec();
+  c10::SmallVector<int64_t, 8> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = columns;
   require_like("out", *out, x, shape);
   return *out;
@@ -155,7 +161,7 @@ std::pair<at::Tensor, Maybe> layer_norm(const at::Tensor& x, const Maybe& weight
   const at::Tensor y = or_out(out, x, width);
   const int64_t rows = x.numel() / width;
   Maybe stats;
-  if (want_stats) stats = at::empty({rows, 2}, x.options().dtype(at::kFloat).memory_format(c10::MemoryFormat::Contiguous));
+  if (want_stats) stats = empty({rows, 2}, at::kFloat, x);
   if (rows == 0) return {y, stats};
   const Rows r = plain_rows(x);
   const Rows to = result_in(y);
@@ -174,9 +180,9 @@ std::tuple<Maybe, Maybe, Maybe> layer_norm_backward(const at::Tensor& dy, const 
   require_like("stats", stats, x, {rows, 2}, true);
   if (stats.scalar_type() != at::kFloat || !stats.is_contiguous()) refuse("stats must be what layer_norm(want_stats=True) returned");
   const c10::cuda::CUDAGuard guard(x.device());
-  const at::TensorOptions kind = weight ? weight->options() : x.options();
+  const at::ScalarType kind = weight ? weight->scalar_type() : x.scalar_type();
   auto param = [&](bool want) {
-    return want ? Maybe(at::empty({width}, kind.memory_format(c10::MemoryFormat::Contiguous))) : Maybe();
+    return want ? Maybe(empty({width}, kind, x)) : Maybe();
   };
   const Maybe dx = want_dx ? Maybe(empty_rows(x, width)) : Maybe(), dweight = param(want_dweight), dbias = param(want_dbias);
   if (rows == 0) {
@@ -223,7 +229,7 @@ std::pair<at::Tensor, Maybe> dense(const at::Tensor& x, const at::Tensor& w, con
   if (residual) require_like("residual", *residual, x, y.sizes());
   Maybe saved;
   const int64_t pitch = pad8(l.N) * (gated ? 2 : 1);
-  if (want_saved && lib.dense_keeps(int(activation), gated, l.K)) saved = at::empty({l.rows, pitch}, x.options().dtype(at::kFloat).memory_format(c10::MemoryFormat::Contiguous));
+  if (want_saved && lib.dense_keeps(int(activation), gated, l.K)) saved = empty({l.rows, pitch}, at::kFloat, x);
   if (l.rows == 0) return {y, saved};
   const bool few = l.rows <= lib.dense_few_rows();
   Copies copies;
@@ -242,7 +248,7 @@ std::tuple<Maybe, Maybe, Maybe> dense_backward(const at::Tensor& dy, const at::T
                                                const Maybe& saved, int64_t activation, bool gated, bool want_dx, bool want_dweight,
                                                bool want_dbias) {
   const Layer l = layer_of(x, w, bias, activation, gated);
-  std::vector<int64_t> shape = x.sizes().vec();
+  c10::SmallVector<int64_t, 8> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = l.N;
   require_like("dy", dy, x, shape);
   const int64_t pitch = pad8(l.N) * (gated ? 2 : 1);
@@ -251,10 +257,9 @@ std::tuple<Maybe, Maybe, Maybe> dense_backward(const at::Tensor& dy, const at::T
     if (!saved->is_contiguous() || saved->scalar_type() != at::kFloat) refuse("saved must be what the forward pass returned");
   }
   const c10::cuda::CUDAGuard guard(x.device());
-  const at::TensorOptions options = x.options().memory_format(c10::MemoryFormat::Contiguous);
   const Maybe dx = want_dx ? Maybe(empty_rows(x, l.K)) : Maybe();
-  const Maybe dweight = want_dweight ? Maybe(at::empty(w.sizes(), options)) : Maybe();
-  const Maybe dbias = want_dbias ? Maybe(at::empty({w.size(0)}, options)) : Maybe();
+  const Maybe dweight = want_dweight ? Maybe(empty(w.sizes(), w.scalar_type(), x)) : Maybe();
+  const Maybe dbias = want_dbias ? Maybe(empty({w.size(0)}, w.scalar_type(), x)) : Maybe();
   if (l.rows == 0) {
     if (dweight) dweight->zero_();
     if (dbias) dbias->zero_();
