@@ -2,7 +2,8 @@
 //
 // A thread keeps its columns, so dw and db add up in its registers over all of its rows, are joined over the block in shared
 // memory, and one row of partial sums per block goes to the workspace, which a second kernel adds up.  The order is fixed:
-// results repeat bit by bit.
+// results repeat bit by bit.  Rows are walked from the last to the first: what came before (the forward pass, or the kernel that
+// made dy) ended with the last ones, which L2 still holds (262144 rows of 128 in bf16, forward and backward: 72 us, so 68).
 #include "layer_norm.cuh"
 
 namespace b200ta {
@@ -31,9 +32,10 @@ norm_grad_kernel(const NormParams p) {
   const int per_block = blockDim.x / lanes, group = threadIdx.x / lanes;
   const float inv = 1.f / float(p.width);
   const long long row0 = (long long)blockIdx.x * per_block + group, step = (long long)gridDim.x * per_block;
-  const T* x = static_cast<const T*>(p.x) + row0 * p.xs;
-  const T* dy = static_cast<const T*>(p.dy) + row0 * p.dys;
-  T* dx = static_cast<T*>(p.dx) + row0 * p.dxs;
+  const long long first = p.rows - 1 - row0;  // row0, left and so on count from the last row
+  const T* x = static_cast<const T*>(p.x) + first * p.xs;
+  const T* dy = static_cast<const T*>(p.dy) + first * p.dys;
+  T* dx = static_cast<T*>(p.dx) + first * p.dxs;
   const norm::Place<T, kShifted, kLanes> place(p.dx != nullptr ? dx : x, p.width, lane, lanes);
   constexpr int kSingles = place.kSingles, kSlots = place.kSlots;
   auto has = [&](int i) { return place.vectors > i * lanes; };
@@ -43,7 +45,7 @@ norm_grad_kernel(const NormParams p) {
   x += place.column, dy += place.column, dx += place.column;
   const bool same_x = !kShifted || (reinterpret_cast<uintptr_t>(x) & 15u) == 0;  // lies as dx does
   const bool same_dy = !kShifted || (reinterpret_cast<uintptr_t>(dy) & 15u) == 0;
-  const float2* stats = p.stats + row0;
+  const float2* stats = p.stats + first;
   long long left = p.rows - row0, block_left = p.rows - (long long)blockIdx.x * per_block;
   const uint32_t slot0 = smem_u32(slots) + threadIdx.x * 16, item_bytes = blockDim.x * 16, stage_bytes = 2 * kItems * item_bytes;
   long long ahead = left;
@@ -61,7 +63,7 @@ norm_grad_kernel(const NormParams p) {
           else sts128(to_dy, norm::load_anywhere(dy + c, dy - place.column, p.width));
         }
     norm::copy_commit();
-    x += step * p.xs, dy += step * p.dys, ahead -= step;
+    x -= step * p.xs, dy -= step * p.dys, ahead -= step;
     if (++fill == kStages) fill = 0;
   };
   for (int i = 0; i < kStages - kRows; ++i) fetch();
@@ -75,7 +77,7 @@ norm_grad_kernel(const NormParams p) {
         const bool in = from > r * step && place.single[i] >= 0;
         next_single[r][i] = make_float2(norm::element_if(in, x_row + place.single[i]), norm::element_if(in, dy_row + place.single[i]));
       }
-      x_row += step * p.xs, dy_row += step * p.dys;
+      x_row -= step * p.xs, dy_row -= step * p.dys;
     }
   };
   if constexpr (kSingles > 0) load_singles(left);
@@ -88,8 +90,8 @@ norm_grad_kernel(const NormParams p) {
   float2 next[kRows];
   auto fetch_stats = [&](long long rows_left) {
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) next[r] = rows_left > r * step ? __ldg(stats + r * step) : make_float2(0.f, 0.f);
-    stats += kRows * step;
+    for (int r = 0; r < kRows; ++r) next[r] = rows_left > r * step ? __ldg(stats - r * step) : make_float2(0.f, 0.f);
+    stats -= kRows * step;
   };
   fetch_stats(left);
   for (; block_left > 0; block_left -= kRows * step, left -= kRows * step) {
@@ -165,8 +167,8 @@ norm_grad_kernel(const NormParams p) {
           const float out = -(single[r][i].x * s[2 * r + 1] + s[2 * r]) * inv * st[r].x + single[r][i].y * st[r].x;
           if (place.single[i] >= 0 && left > r * step) dx_row[place.single[i]] = static_cast<T>(out);
         }
-        dx_row += step * p.dxs;
-        dx += step * p.dxs;
+        dx_row -= step * p.dxs;
+        dx -= step * p.dxs;
         if (++stage == kStages) stage = 0;
       }
     }
