@@ -19,7 +19,9 @@ int map_of(CUtensorMap* map, const Plane& t, int bytes, uint32_t columns, uint32
 
 // How the blocks share a product.  The costs are in clocks: a block of 64 along k costs its MMAs (4 * max(40, n * 0.54)) or its
 // operands' way from L2 (46 bytes a clock and SM), a tile of 256 columns with its two stages waits for its loads besides, and
-// a tile costs its finishing if that is more; all blocks take as many tiles as the busiest.
+// a tile costs its finishing if that is more; all blocks take as many tiles as the busiest.  Pairs on 128 columns save loads of B
+// (dW of 147456 rows, 128 -> 512 gated: 55 us, 58 by single blocks; 262144 rows of 512 -> 128: 71 and 73) and start later (768
+// rows of 384 -> 1536 gated: 7.1 and 6.8).
 struct Tiling {
   int tile_n, pair, resident;
   double clocks;
@@ -36,7 +38,7 @@ Tiling choose_tiling(const TilingOf& m, int num_sms) {
   const double finish = m.form == kGatedGrad ? 12 : two ? 8 : 6.5;  // clocks for an accumulator column of 128 rows
   Tiling best{128, 0, 0, 1e300};
   auto consider = [&](int n, int pair, int resident, double waves, double main) {
-    const double end = finish * n, cost = waves * std::max(main, end) + std::min(main, end) + 1500;
+    const double end = finish * n, cost = waves * std::max(main, end) + std::min(main, end) + (pair && n < 256 ? 3500 : 1500);
     if (cost < best.clocks * 0.98) best = {n, pair, resident, cost};
   };
   auto waves_of = [](int64_t items, int64_t blocks) { return double((items + blocks - 1) / blocks); };
@@ -53,9 +55,10 @@ Tiling choose_tiling(const TilingOf& m, int num_sms) {
       consider(n, 0, 0, waves_of(tiles_m * tiles_n * m.splits, num_sms), m.kblocks * std::max(mma, load));
     }
   }
-  if (m.rows > matmul::kBM && accumulated > 128 && !m.sums) {
-    const int64_t tiles = (m.rows + 255) / 256 * m.outer * m.splits * ((accumulated + 255) / 256);
-    consider(256, 1, 0, waves_of(tiles, num_sms / 2), m.kblocks * 712.0);
+  for (int n = 256; n >= 128 && m.rows > matmul::kBM && !m.sums; n /= 2) {
+    if (n / 2 >= accumulated) continue;
+    const int64_t tiles = (m.rows + 255) / 256 * m.outer * m.splits * ((accumulated + n - 1) / n);
+    consider(n, 1, 0, waves_of(tiles, num_sms / 2), m.kblocks * std::max(4.0 * n * 0.54, (16384 + n * 64) / 46.0));
   }
   return best;
 }
