@@ -28,8 +28,8 @@ int run_narrow(const Narrow& n, void* stream) {
   CUtensorMap x, w, dy, dx, dz{};
   if ((rc = map_of(&x, n.x, 2, 64, 128, 1, SWZ_128, n.what)) != B200TA_OK ||
       (rc = map_of(&w, n.w, 2, 64, 32, n.gated ? 2 : 1, SWZ_128, n.what)) != B200TA_OK ||
-      (rc = map_of(&dy, n.dy, 2, 32, 32, 1, SWZ_64, n.what)) != B200TA_OK || (rc = map_of(&dx, n.dx, 2, 32, 32, 1, SWZ_64, n.what)) != B200TA_OK ||
-      (p.store_dz && (rc = map_of(&dz, n.dz, 2, 32, 32, 1, SWZ_64, n.what)) != B200TA_OK))
+      (rc = map_of(&dy, n.dy, 2, 16, 32, 1, SWZ_32, n.what)) != B200TA_OK || (rc = map_of(&dx, n.dx, 2, 32, 32, 1, SWZ_64, n.what)) != B200TA_OK ||
+      (p.store_dz && (rc = map_of(&dz, n.dz, 2, 16, 32, 1, SWZ_32, n.what)) != B200TA_OK))
     return rc;
   const int grid = std::min((p.rows + 255) / 256, st->num_sms);
   auto* kernel = n.gated ? (n.f16 ? narrow::narrow_kernel<__half, kGatedGrad> : narrow::narrow_kernel<__nv_bfloat16, kGatedGrad>)

@@ -44,51 +44,53 @@ int run_narrow(const Narrow& n, void* stream);
 namespace narrow {
 
 constexpr int kThreads = 576;
-constexpr int kSlab = 2048;  // dy of a group: 32 rows of 64 bytes
+constexpr int kSlab = 2048;       // 32 rows of 64 bytes, or two of 32 rows of 32
+constexpr int kHalf = kSlab / 2;
 
 __device__ __forceinline__ void store_slab(uint32_t slab, int lane, const uint32_t (&x)[16]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) sts128(slab + sw64_offset(lane, j), make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
 }
-__device__ __forceinline__ void load_slab(uint32_t slab, int lane, uint32_t (&aux)[16]) {
+// 32 rows of 16 units; 16-byte vectors swapped in every second group of four rows (SWZ_32), so that lanes meet no bank twice.
+__device__ __forceinline__ uint32_t half_offset(int lane, int j) { return lane * 32u + ((uint32_t(j) ^ ((uint32_t(lane) >> 2) & 1u)) << 4); }
+__device__ __forceinline__ void store_half(uint32_t slab, int lane, const uint32_t (&x)[16]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint4 x = lds128(slab + sw64_offset(lane, j));
+  for (int j = 0; j < 2; ++j) sts128(slab + half_offset(lane, j), make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
+}
+__device__ __forceinline__ void load_half(uint32_t slab, int lane, uint32_t (&aux)[16]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint4 x = lds128(slab + half_offset(lane, j));
     aux[4 * j] = x.x, aux[4 * j + 1] = x.y, aux[4 * j + 2] = x.z, aux[4 * j + 3] = x.w;
   }
 }
-// dz of a group's 32 units: accumulators of the values at `v` and of the gates at `g` (kDenseGrad: only `v`).
+// dz of 16 units (in the first halves of y, yg): accumulators of the values at `v` and of the gates at `g` (kDenseGrad: only `v`).
 template <typename T, MatmulForm kForm>
-__device__ __forceinline__ void group_dz(uint32_t v_addr, uint32_t g_addr, int n, const NarrowParams& p, const uint32_t (&aux)[16],
+__device__ __forceinline__ void units_dz(uint32_t v_addr, uint32_t g_addr, int n, const NarrowParams& p, const uint32_t (&aux)[16],
                                          uint32_t (&y)[16], uint32_t (&yg)[16]) {
   constexpr bool kTwo = kForm == kGatedGrad;
   const T* bias = static_cast<const T*>(p.bias);
-  auto step = [&](auto first) {
-    constexpr int kFirst = decltype(first)::value;
-    float v[16], gate[16];
-    matmul::tmem_load(v_addr + kFirst, v);
-    if constexpr (kTwo) matmul::tmem_load(g_addr + kFirst, gate);
-    tmem_ld_wait();
-    if (bias != nullptr) {
-      uint32_t b[8];
-      matmul::load_bias<T, 16>(b, bias, n + kFirst, p.N);
-      matmul::add_bias<T>(v, b);
-      if constexpr (kTwo) {
-        matmul::load_bias<T, 16>(b, bias + p.N, n + kFirst, p.N);
-        matmul::add_bias<T>(gate, b);
-      }
+  float v[16], gate[16];
+  matmul::tmem_load(v_addr, v);
+  if constexpr (kTwo) matmul::tmem_load(g_addr, gate);
+  tmem_ld_wait();
+  if (bias != nullptr) {
+    uint32_t b[8];
+    matmul::load_bias<T, 16>(b, bias, n, p.N);
+    matmul::add_bias<T>(v, b);
+    if constexpr (kTwo) {
+      matmul::load_bias<T, 16>(b, bias + p.N, n, p.N);
+      matmul::add_bias<T>(gate, b);
     }
-    matmul::finish_any<T, kForm, kFirst, 16>(p.activation, v, gate, true, aux, y, yg);
-  };
-  step(std::integral_constant<int, 0>());
-  step(std::integral_constant<int, 16>());
+  }
+  matmul::finish_any<T, kForm, 0, 16>(p.activation, v, gate, true, aux, y, yg);
 }
 
 constexpr int kStages = 2;
 constexpr int kSmX = 0, kSmW = 65536, kSmOut = kSmW + kStages * 32768, kSmSlabs = kSmOut + 32 * kSlab, kSmBars = kSmSlabs + 16 * kSlab;
 enum Bar {
   X_FULL = 0, X_EMPTY = 2, S_FULL = 4, D_FULL = 6, DX_FULL = 8, DX_EMPTY = 10, W_FULL = 12, W_EMPTY = W_FULL + kStages,
-  AUX = W_EMPTY + kStages, NUM_BARS = AUX + 16
+  AUX = W_EMPTY + kStages, NUM_BARS = AUX + 32
 };
 constexpr int kSmTotal = kSmBars + NUM_BARS * 8 + 32, kSmDynamic = kSmTotal + 1024;
 static_assert(kSmDynamic <= 232448, "shared memory of a block");
@@ -115,11 +117,11 @@ narrow_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ 
     for (int i = 0; i < 2; ++i) {
       mbar_init(bars + (X_FULL + i) * 8, 1), mbar_init(bars + (X_EMPTY + i) * 8, 1);
       mbar_init(bars + (S_FULL + i) * 8, 1);
-      mbar_init(bars + (D_FULL + i) * 8, 8);
-      mbar_init(bars + (DX_FULL + i) * 8, 1), mbar_init(bars + (DX_EMPTY + i) * 8, 8);
+      mbar_init(bars + (D_FULL + i) * 8, 16);
+      mbar_init(bars + (DX_FULL + i) * 8, 1), mbar_init(bars + (DX_EMPTY + i) * 8, 16);
     }
     for (int i = 0; i < kStages; ++i) mbar_init(bars + (W_FULL + i) * 8, 1), mbar_init(bars + (W_EMPTY + i) * 8, 1);
-    for (int i = 0; i < 16; ++i) mbar_init(bars + (AUX + i) * 8, 1);
+    for (int i = 0; i < 32; ++i) mbar_init(bars + (AUX + i) * 8, 1);
     fence_mbar_init();
   }
   if (warp == 17) {
@@ -204,95 +206,112 @@ narrow_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ 
       if (ok && c == 0) ok = mbar_wait_warp(bars + (DX_EMPTY + t) * 8, (i & 1) ^ 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      // dz of a group in the first columns of its part of S; W: rows (hidden units) of 64 inputs, blocks of 64 inputs kWBlock apart
+      // dz of 16 units in the first 8 columns of their part of S; W: rows (hidden units) of 64 inputs, blocks of 64 inputs kWBlock apart
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const uint64_t db = smem_desc<kWBlock, 1024, kLayoutSw128>(base + kSmW + stage * 32768 + g * (kWBlock / 2));
 #pragma unroll
         for (int k = 0; k < kColumns / 32; ++k)
-          umma_ts_warp(tb + 256 + t * 128, tb + t * 128 + g * (kColumns / 2) + k * 8, db + k * 128, id_dx, (c > 0 || g > 0 || k > 0) ? 1u : 0u);
+          umma_ts_warp(tb + 256 + t * 128, tb + t * 128 + g * (kColumns / 2) + k * 16, db + k * 128, id_dx, (c > 0 || g > 0 || k > 0) ? 1u : 0u);
       }
       if (t == 1) umma_commit_warp(bars + (W_EMPTY + stage) * 8);
       if (c == p.chunks - 1) umma_commit_warp(bars + (DX_FULL + t) * 8);
       if (s + 2 < steps) issue_s(s + 2);  // behind the product that reads dz, whose columns it overwrites
     }
   } else {
-    // ------------------------------------------------------------------ finishing warps: eight for each row tile
+    // ------------------------------------------------------------------ finishing warps: all of them on every step
     pdl_wait();
-    const int t = warp >> 3, group = (warp >> 2) & 1, quad = warp & 3;
+    const int quad = warp & 3, part = warp >> 2;  // 32 rows, 16 of the chunk's units
     const uint32_t lane_tmem = tmem_base + (uint32_t(quad * 32) << 16);
-    const uint32_t slab = base + kSmSlabs + warp * kSlab, aux_bar = bars + (AUX + warp) * 8;
-    const uint32_t out = base + kSmOut + warp * 2 * kSlab;
+    const uint32_t slabs = base + kSmSlabs + warp * kSlab, aux_bars = bars + (AUX + warp * 2) * 8;  // one for each row tile
+    const uint32_t outs = base + kSmOut + warp * 2 * kSlab;
+    const uint32_t s_column = (part >> 1) * (kColumns / 2) + (part & 1) * 16;
     const int steps = items * p.chunks;
-    int next_i = 0, next_c = 0;
-    auto load_dy = [&]() {
-      if (next_i >= items) return;
+    auto row_of = [&](int i, int t) { return (int(blockIdx.x) + i * int(gridDim.x)) * 256 + t * 128 + quad * 32; };
+    auto load_dy = [&](int i, int c, int t) {
       if (lane == 0) {
-        mbar_expect_tx(aux_bar, kSlab);
-        tma_load_3d(slab, &tm_dy, aux_bar, next_c * 64 + group * 32, (blockIdx.x + next_i * gridDim.x) * 256 + t * 128 + quad * 32, 0);
+        mbar_expect_tx(aux_bars + t * 8, kHalf);
+        tma_load_3d(slabs + t * kHalf, &tm_dy, aux_bars + t * 8, c * 64 + part * 16, row_of(i, t), 0);
       }
-      if (++next_c == p.chunks) next_c = 0, ++next_i;
     };
-    load_dy();
+    load_dy(0, 0, 0);
+    load_dy(0, 0, 1);
     bool ok = true;
     int i = 0, c = 0;
     for (int w = 0; ok && w < steps; ++w) {
-      uint32_t aux[16], y[16], yg[16];
-      ok = mbar_wait2_warp(bars + (S_FULL + t) * 8, w & 1, aux_bar, w & 1, abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      load_slab(slab, lane, aux);
-      const uint32_t s_addr = lane_tmem + t * 128 + group * (kColumns / 2);
-      group_dz<T, kForm>(s_addr, s_addr + 32, c * 64 + group * 32, p, aux, y, yg);
-      tmem_st16(s_addr, y);
-      if constexpr (kTwo) tmem_st16(s_addr + 16, yg);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      mbar_arrive_warp(bars + (D_FULL + t) * 8);
-      const int row0 = (blockIdx.x + i * gridDim.x) * 256 + t * 128 + quad * 32, unit = c * 64 + group * 32;
-      if (p.store_dz && row0 < p.rows && unit < p.N) {
-        if (lane == 0) tma_store_wait_read<0>();  // the stores of the step before have read the slabs
+      const int unit = c * 64 + part * 16;
+      const bool last = c + 1 == p.chunks;
+#pragma unroll 1
+      for (int t = 0; t < 2; ++t) {
+        uint32_t aux[16], y[16], yg[16];
+        ok = mbar_wait2_warp(bars + (S_FULL + t) * 8, w & 1, aux_bars + t * 8, w & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        load_half(slabs + t * kHalf, lane, aux);
+        const uint32_t s_addr = lane_tmem + t * 128 + s_column;
+        units_dz<T, kForm>(s_addr, s_addr + 32, unit, p, aux, y, yg);
+        // (dz takes the place of accumulators that have been read, by this warp alone)
+        tmem_st8(s_addr, reinterpret_cast<const uint32_t(&)[8]>(y));
+        if constexpr (kTwo) tmem_st8(s_addr + 32, reinterpret_cast<const uint32_t(&)[8]>(yg));
+        tmem_st_wait();
+        tc_fence_before();
         __syncwarp();
-        store_slab(out, lane, y);
-        if constexpr (kTwo) store_slab(out + kSlab, lane, yg);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_3d(&tm_dz, out, unit, row0, 0);
-          if constexpr (kTwo) tma_store_3d(&tm_dz, out + kSlab, unit, row0, 1);
-          tma_store_commit();
+        mbar_arrive_warp(bars + (D_FULL + t) * 8);
+        if (p.store_dz) {
+          const uint32_t out = outs + t * kSlab;
+          if (lane == 0) tma_store_wait_read<1>();  // the stores of this row tile's step before have read the slabs
+          __syncwarp();
+          store_half(out, lane, y);
+          if constexpr (kTwo) store_half(out + kHalf, lane, yg);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (row_of(i, t) < p.rows && unit < p.N) {
+              tma_store_3d(&tm_dz, out, unit, row_of(i, t), 0);
+              if constexpr (kTwo) tma_store_3d(&tm_dz, out + kHalf, unit, row_of(i, t), 1);
+            }
+            tma_store_commit();  // (an empty group as well: they are counted)
+          }
         }
+        // what the slab held has been used
+        if (!last) load_dy(i, c + 1, t);
+        else if (i + 1 < items) load_dy(i + 1, 0, t);
       }
-      load_dy();  // (what the slab held has been used)
+      if (!ok) break;
       if (++c < p.chunks) continue;
-      // dx of the row tile
-      ok = mbar_wait_warp(bars + (DX_FULL + t) * 8, i & 1, abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      for (int n = group * 32; n < p.K; n += 64) {
-        float v[32];
-        uint32_t x[16];
-        matmul::tmem_load(lane_tmem + 256 + t * 128 + n, v);
-        tmem_ld_wait();
+      // dx of the row tiles
+#pragma unroll 1
+      for (int t = 0; ok && t < 2; ++t) {
+        ok = mbar_wait_warp(bars + (DX_FULL + t) * 8, i & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const int n = part * 32;
+        if (n < p.K) {
+          const uint32_t out = outs + t * kSlab;
+          float v[32];
+          uint32_t x[16];
+          matmul::tmem_load(lane_tmem + 256 + t * 128 + n, v);
+          tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
-        if (lane == 0) tma_store_wait_read<0>();
-        __syncwarp();
-        store_slab(out, lane, x);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0 && row0 < p.rows) {
-          tma_store_3d(&tm_dx, out, n, row0, 0);
-          tma_store_commit();
+          for (int j = 0; j < 16; ++j) x[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+          store_slab(out, lane, x);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (row_of(i, t) < p.rows) tma_store_3d(&tm_dx, out, n, row_of(i, t), 0);
+            tma_store_commit();
+          }
         }
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_warp(bars + (DX_EMPTY + t) * 8);
       }
-      tc_fence_before();
-      __syncwarp();
-      mbar_arrive_warp(bars + (DX_EMPTY + t) * 8);
       c = 0, ++i;
     }
-    if (!ok && lane == 0) mbar_wait(aux_bar, 0, abort_flag + 1), mbar_wait(aux_bar, 1, abort_flag + 1);  // a load in flight lands
+    if (!ok && lane == 0)  // loads in flight land
+      for (int t = 0; t < 2; ++t) mbar_wait(aux_bars + t * 8, 0, abort_flag + 1), mbar_wait(aux_bars + t * 8, 1, abort_flag + 1);
     if (lane == 0) tma_store_wait_all();
   }
 
