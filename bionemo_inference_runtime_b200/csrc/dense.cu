@@ -545,8 +545,8 @@ struct BackwardPlan {
   int64_t dz, parts, sums, bytes;  // offsets, total
 };
 // Whether dz and dx come from one kernel (narrow.cuh): its blocks take 256 rows each, so from a row tile for half of the SMs on.
-// (Backward pass of a gated layer 128 -> 512: 6000 rows 46 us so and 40 us otherwise, 16384 rows 50 and 58, 147456 rows 208 and
-// 231; 64 -> 256, 147456 rows: 110 and 126.)
+// (Backward pass of a gated layer 128 -> 512: 6000 rows 44 us so and 41 us otherwise, 9472 rows 46 and 44, 16384 rows 48 and 57,
+// 147456 rows 194 and 229; 64 -> 256, 147456 rows: 101 and 127.)
 bool narrow_pays(bool own_dz, bool kept, int64_t rows, int K, const void* dx, int64_t dxs, int num_sms) {
   return own_dz && !kept && K <= 128 && dx != nullptr && rows_aligned(dx, dxs) && rows >= int64_t(num_sms) * 64;
 }

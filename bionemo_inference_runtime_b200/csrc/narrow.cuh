@@ -7,14 +7,16 @@
 // of this kind for dW = dz^T x took 100 us for 147456 rows, 128 -> 512 gated, where reading dz takes 56: its operands' way
 // through shared memory bounded it.)
 //
-// The finishing warps bound the kernel (activation, its slope and two products a unit: some 500 instructions for 32 units of 32
-// rows).  Two row tiles of 128 share every tile of W; eight finishing warps serve each, half a step apart.  Shared memory: x
-// 2 x 32 KiB, W in two stages of a chunk's value and gate rows (32 KiB each), dy 16 x 2 KiB, results on their way out 16 x 4 KiB.
-// Tensor memory: S 2 x 128 columns, dz in their place as the left operand of the second product (from shared memory its tiles
-// would be written and read again: that pipe bounded the kernel, dx alone 117 us where it now takes 89), dx 2 x 128.
+// The finishing warps bound the kernel (activation, its slope and two products a unit: 250 instructions for 16 units of 32 rows, and
+// one and a half special-function operations a unit).  Two row tiles of 128 share every tile of W and take turns: all sixteen
+// warps finish one while the tensor cores work on the other, and what a step stores has until the tile's next step to leave.
+// (Eight warps for each tile with one buffer for their stores: 147456 rows, 128 -> 512 gated, 135 us, now 125.  Chunks of 32 units
+// with S twice: 147; its MMAs are too small.)  Shared memory: x 2 x 32 KiB, W in two stages of a chunk's value and gate rows (32
+// KiB each), dy 16 x 2 KiB, results on their way out 16 x 4 KiB.  Tensor memory: S 2 x 128 columns, dz in their place as the left
+// operand of the second product (from shared memory its tiles would be written and read again: that pipe bounded the kernel, dx
+// alone 117 us where it now takes 88), dx 2 x 128.
 //
-// Warp roles (576 threads): warps 0-15 finish (TMEM lane = row, groups of 32 units), warp 16 loads by TMA, warp 17 issues
-// tcgen05.mma.
+// Warp roles (576 threads): warps 0-15 finish (TMEM lane = row, 16 units each), warp 16 loads by TMA, warp 17 issues tcgen05.mma.
 #pragma once
 
 #include "matmul.cuh"
