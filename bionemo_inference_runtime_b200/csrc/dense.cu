@@ -367,9 +367,11 @@ auto pick_slope(int activation) {
 
 // ---- sums over rows -------------------------------------------------------------------------------------------------
 //
-// part[block.y][n] (+)= sum over a block's rows of dz[., n].  32 lanes of eight columns, eight rows at a time.
+// part[block.y][n] (+)= sum over a block's rows of dz[., n].  32 lanes of eight columns, eight rows at a time, eight loads of a
+// thread on their way: dz of 5003 rows and 6144 columns takes 14 us (61 MB).  (Blocks of half the rows with four loads: two waves
+// of them, 19 us.)
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 row_sum_kernel(const T* dz, long long pitch, long long rows, int N, long long part_pitch, int rows_block, int accumulate, float* part) {
   __shared__ float joined[8][256 + 4];
   pdl_trigger();
@@ -378,7 +380,7 @@ row_sum_kernel(const T* dz, long long pitch, long long rows, int N, long long pa
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const long long r0 = (long long)blockIdx.y * rows_block, r1 = r0 + rows_block < rows ? r0 + rows_block : rows;
   if (c < N) {
-#pragma unroll 4
+#pragma unroll 8
     for (long long r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
       float v[8];
       if (c + 8 <= N) {
@@ -531,7 +533,7 @@ Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns,
 constexpr int kChunkRows = 256;  // chunks of the backward pass are multiples of this
 // Rows of a partial sum of db: enough blocks of 256 columns to fill the device a few times, at least 32 rows each.
 int sum_rows(int64_t rows, int64_t columns, int num_sms) {
-  const int64_t blocks = std::max<int64_t>(8 * num_sms / ((columns + 255) / 256), 1), each = (rows + blocks - 1) / blocks;
+  const int64_t blocks = std::max<int64_t>(4 * num_sms / ((columns + 255) / 256), 1), each = (rows + blocks - 1) / blocks;
   return int(std::min<int64_t>(std::max<int64_t>((each + 7) / 8 * 8, 32), 1024));
 }
 
