@@ -134,7 +134,8 @@ namespace {
 // Up to 16 rows: the weights are read once and that bounds the call, or its latency does.  A warp takes one result column (a
 // value and a gate row of W for kGated), or two, four or eight warps do where there are few columns; its lanes run along k with
 // 16-byte loads, the rows' sums are exchanged so that each row's ends in a lane of its own.  128-row tiles of the tensor cores
-// would leave all but N / 64 SMs idle.
+// would leave all but N / 64 SMs idle.  (One row, 384 -> 1536 gated: 4.0 us from cold caches, 2.4 MB of weights; three rows, 1536 ->
+// 384: 5.2.  A launch of nothing takes some 2.5.)
 constexpr int kFewRows = 16;
 
 struct FewParams {
@@ -270,9 +271,9 @@ auto pick_few(int rows, bool vec, bool two) {
 
 // ---- dz from stored pre-activations ---------------------------------------------------------------------------------
 //
-// dz = dy act'(z), or [dy act(g) | dy v act'(g)], z kept in 32 bits: bound by HBM.  A block takes 256 columns
-// of some rows, a thread eight columns of every eighth of them, whose sums (db) it has on the way: part[block.y][column] (+)=
-// theirs, of the values before they are rounded.
+// dz = dy act'(z), or [dy act(g) | dy v act'(g)], z kept in 32 bits: bound by HBM (8192 rows of 4096, bf16: 42 us, 268 MB at 6.4
+// TB/s).  A block takes 256 columns of some rows, a thread eight columns of every eighth of them, whose sums (db) it has on the
+// way: part[block.y][column] (+)= theirs, of the values before they are rounded.
 struct SlopeParams {
   const void *dy, *saved;
   void* dz;
@@ -397,7 +398,8 @@ row_sum_kernel(const T* dz, long long pitch, long long rows, int N, long long pa
 }
 
 // out[r][c] = sum over the parts, in a fixed order; two such results (dW and db) in one launch, either of which may be empty.
-// A thread sums one value, or eight threads do where there are many parts of few values.
+// A thread sums one value, four where they lie together, or eight threads sum one where there are many parts of few values (18 parts of
+// 1024 x 128: 7.5 us, 9.4 MB mostly from L2; a launch and one round of loads bound it).
 struct JoinParams {
   const float* part;
   void* out;  // rows of `columns`, dense
@@ -457,7 +459,7 @@ join_kernel(const JoinParams a, const JoinParams b) {
 // no multiple of 16 bytes, columns that are not contiguous) pass through a padded copy, up to four in one launch.  A thread
 // makes a vector of eight columns, from two aligned loads shifted into place if they are contiguous, otherwise from eight
 // loads with neighbouring threads in neighbouring rows.  (An aligned 16-byte vector with a byte of the source in it lies in
-// the source's allocation.)
+// the source's allocation.)  2047 rows of 515 and 1283 rows of 515 in one launch take 4.4 us, with 2047 of 1283 besides 6.2.
 struct CopyParams {
   b200ta_copy job[B200TA_COPIES];
   long long end[B200TA_COPIES];  // vectors up to and with this job
@@ -508,8 +510,8 @@ int check_layer(const char* what, int dtype, int activation, int64_t rows, int K
 }
 
 // How dW = dz^T x is cut along the rows, and whether db comes from the same product (sums of dz by MMAs with ones, which only
-// tiles of up to 128 columns have room for) or from a pass over dz: its own, or the one that forms dz from kept values.  Parts are written and read once and sums read
-// dz once more at some 2400 bytes a clock; a launch more costs some 4000 clocks.
+// tiles of up to 128 columns have room for) or from a pass over dz: its own, or the one that forms dz from kept values.  Parts are
+// written and read once and sums read dz once more at some 2400 bytes a clock; a launch more costs some 4000 clocks.
 struct Split {
   int kblocks, parts;  // of a part; in all
   bool sums;           // db from the product

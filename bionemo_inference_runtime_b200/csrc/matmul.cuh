@@ -13,14 +13,21 @@
 // are zero-filled by the loads and clipped by the stores); base addresses and row pitches of what is read are multiples of 16
 // bytes.
 //
-// A persistent block walks [128 x tile_n] tiles; with kPair two blocks of a cluster walk [256 x 256] tiles together, each
-// with its 128 rows of A and half of B (cta_group::2), which halves what a tile of B costs in shared memory and from L2.
+// A persistent block walks [128 x tile_n] tiles; with kPair two blocks of a cluster walk [256 x tile_n] tiles together,
+// each with its 128 rows of A and half of B (cta_group::2), which halves what a tile of B costs in shared memory and from L2.
 // Warp roles (576 threads): warps 0-15 finish tiles (TMEM lane = row, groups of 32 columns), warp 16
 // loads [128 x 64] and [tile_n x 64] operand blocks by TMA into a ring, warp 17 issues tcgen05.mma into two accumulators of
 // 256 columns, one filled while the other is finished.  Where all of a column tile of B fits in half of the ring (64 KiB: 128
 // wide layers), it is loaded once and only A passes through the ring.  The finishing warps fetch what they read beside the
 // accumulators (residual, dy) by TMA a group ahead and store by TMA: a lane's own accesses to 32 rows occupy the load-store
 // unit for some 56 clocks.  Results whose rows TMA cannot address are stored from the same slabs, a row at a time.
+//
+// Measured (bf16): with long k the tensor cores bound it: 8192 rows, 1024 -> 4096 gated with silu 87 us (1580 TFLOP/s), 4096 -> 4096
+// dense 190 us (1450, at the power limit).  With short k finishing does, or HBM: 147456 rows of 128 -> 512: dense without an
+// activation 39 us (4.8 TB/s; a fill writes at 3.9), gated with relu 48, with silu 62, where a warp's loads from tensor memory, its
+// exponentials (42 % of that unit's rate) and its stores follow one another.  With the finishing warps in two sets, out of step, a
+// training step of the last took 330 us instead of 343; registers moved to them (setmaxnreg) gained nothing, and their code as a loop
+// over halves of a group lost 5 %.
 #pragma once
 
 #include <type_traits>
@@ -40,9 +47,9 @@ struct MatmulParams {
   int kblocks_split;                   // of one split
   int rows_inner;                      // valid rows of D for one outer index
   int columns;                         // valid result columns (kGated*: hidden units)
-  int tile_n;                          // accumulator columns of a tile: 64, 128 or 256
+  int tile_n;                          // accumulator columns of a tile: 64, 128 or 256 (pairs: 128, 256)
   int stages;
-  int pair;                            // two blocks on [256 x 256] tiles (tiles_m counts those)
+  int pair;                            // two blocks on [256 x tile_n] tiles (tiles_m counts those)
   int resident;                        // blocks keep their column tile of B (and walk the row tiles in steps of resident)
   const void* bias;                    // [columns] (kGated*: value biases, then gate biases), or NULL
   int activation;
@@ -571,7 +578,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         auto step = [&](auto first) {
           constexpr int kFirst = decltype(first)::value;
           float v[kStep], gate[kStep];
-          uint32_t bv[kStep / 2], bg[kStep / 2];
+          uint32_t bv[kStep / 2];
+          [[maybe_unused]] uint32_t bg[kStep / 2];
           if ((kForm == kDense || kForm == kGated) && bias != nullptr) {  // (the gradients' registers do not suffice)
             load_bias<T, kStep>(bv, bias, n + kFirst, p.columns);
             if constexpr (kTwo) load_bias<T, kStep>(bg, bias + p.columns, n + kFirst, p.columns);
