@@ -131,32 +131,30 @@ namespace {
 
 // ---- few rows ---------------------------------------------------------------------------------------------------
 //
-// Up to 16 rows: the weights are read once and that bounds the call, or its latency does.  A warp takes one result column (a
-// value and a gate row of W for kGated), or two, four or eight warps do where there are few columns; its lanes run along k with
-// 16-byte loads, the rows' sums are exchanged so that each row's ends in a lane of its own.  128-row tiles of the tensor cores
-// would leave all but N / 64 SMs idle.  (One row, 384 -> 1536 gated: 4.0 us from cold caches, 2.4 MB of weights; three rows, 1536 ->
-// 384: 5.2.  A launch of nothing takes some 2.5.)
+// Up to 16 rows: the weights are read once and that bounds the call, or its latency does.  A block takes 16 result columns (and
+// their gates for kGated), whose rows of W are the left operand of warp-wide products m16n8k16, eight rows of x the right one; its
+// warps take 32 of k in turn and add up in shared memory.  A lane reads 16 bytes of each of its rows, eight neighbouring k, which
+// serve as pairs 2t, 2t + 8 of two products: the order of k is the same in both operands and does not matter.  128-row tiles of
+// the tensor cores would leave all but N / 64 SMs idle and wait for tensor memory, and products by FMA want every row of x in
+// registers for each column (13 rows, 960 -> 4648 gated: 45 us so, now 8; 16 rows, 4096 -> 4096: 130 and 18; one row the same).
+// Rows that are not 16-byte aligned are shifted into place.
 constexpr int kFewRows = 16;
 
 struct FewParams {
   const void *x, *w, *bias, *residual;
   void *y, *saved;
   long long xs, ws, rs, ys, ss;
-  int rows, K, N, activation, warps;  // warps: of a column
+  int rows, K, N, activation;
 };
 
-template <typename T, int kVec>
+template <typename T>
 __device__ __forceinline__ void load_vec(const T* p, float* v) {
-  if constexpr (kVec == 1) {
-    v[0] = static_cast<float>(*p);
-  } else {
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = unpack2<T>(w[e]);
-      v[2 * e] = f.x, v[2 * e + 1] = f.y;
-    }
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = unpack2<T>(w[e]);
+    v[2 * e] = f.x, v[2 * e + 1] = f.y;
   }
 }
 
@@ -172,101 +170,100 @@ __device__ __forceinline__ void activate_any(int activation, float z, float& a, 
   }
 }
 
-// The sums over a warp of kRows values: lane l ends with that of row (l >> (5 - log2 kRows)).
-template <int kRows>
-__device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
-  int o = 16;
-#pragma unroll
-  for (int n = kRows; n > 1; n >>= 1, o >>= 1) {
-    const bool upper = lane & o;
-#pragma unroll
-    for (int i = 0; i < n / 2; ++i) {
-      const float keep = upper ? v[i + n / 2] : v[i], give = upper ? v[i] : v[i + n / 2];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-    }
-  }
-  for (; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
-  return v[0];
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (__is_same(T, __half))
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Eight elements of a row of K from k on, zeros behind it.
+template <typename T, bool kVec>
+__device__ __forceinline__ uint4 load_row(const T* row, int k, int K) {
+  if constexpr (kVec) return norm::load_if(k < K, row + k);
+  const uint4 v = norm::load_anywhere(row + k, row, K);
+  return K - k >= 8 ? v : norm::first<T>(v, K - k);
 }
 
-constexpr int kFewWarps = 8;  // of a block
-template <typename T, int kRows, int kVec, bool kTwo>
-__global__ void __launch_bounds__(kFewWarps * 32)
+constexpr int kFewWarps = 16, kFewColumns = 16;  // of a block, at most
+template <typename T, bool kTwo, int kEights, bool kVec>
+__global__ void __launch_bounds__(kFewWarps * 32, 1)
 few_rows_kernel(const FewParams p) {
-  __shared__ float joined[2][kFewWarps][32];
+  __shared__ float joined[kFewWarps][kTwo ? 2 : 1][kEights * 8][kFewColumns + 1];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % p.warps;
-  const int n = blockIdx.x * (kFewWarps / p.warps) + warp / p.warps;
-  const bool in = n < p.N;
-  float acc[kRows], gate[kRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, n0 = blockIdx.x * kFewColumns, warps = blockDim.x >> 5;
+  constexpr int kParts = kTwo ? 2 : 1;
+  const T *w[kParts][2], *x[kEights];
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) acc[r] = 0.f, gate[r] = 0.f;
-  if (in) {
-    const T* x = static_cast<const T*>(p.x);
-    const T* w = static_cast<const T*>(p.w) + n * p.ws;
-    const T* wg = static_cast<const T*>(p.w) + (long long)(n + p.N) * p.ws;
-#pragma unroll 2
-    for (int k = (part * 32 + lane) * kVec; k < p.K; k += p.warps * 32 * kVec) {
-      float a[kVec], b[kVec], c[kVec];
-      load_vec<T, kVec>(w + k, a);
-      if constexpr (kTwo) load_vec<T, kVec>(wg + k, b);
+  for (int h = 0; h < 2; ++h) {
+    const int n = min(n0 + g + 8 * h, p.N - 1);  // (rows past the last are read again, their results not stored)
+    w[0][h] = static_cast<const T*>(p.w) + n * p.ws;
+    if constexpr (kTwo) w[1][h] = static_cast<const T*>(p.w) + (long long)(n + p.N) * p.ws;
+  }
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        if (r < p.rows) {
-          load_vec<T, kVec>(x + r * p.xs + k, c);
+  for (int e = 0; e < kEights; ++e) x[e] = static_cast<const T*>(p.x) + min(g + 8 * e, p.rows - 1) * p.xs;
+  float acc[kParts][kEights][4] = {};
+#pragma unroll 4
+  for (int k = warp * 32; k < p.K; k += warps * 32) {
+    uint4 a[kParts][2], b[kEights];
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) {
-            acc[r] = fmaf(a[e], c[e], acc[r]);
-            if constexpr (kTwo) gate[r] = fmaf(b[e], c[e], gate[r]);
-          }
-        }
+    for (int i = 0; i < kParts; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) a[i][h] = load_row<T, kVec>(w[i][h], k + t * 8, p.K);
+#pragma unroll
+    for (int e = 0; e < kEights; ++e) b[e] = load_row<T, kVec>(x[e], k + t * 8, p.K);
+#pragma unroll
+    for (int i = 0; i < kParts; ++i)
+#pragma unroll
+      for (int e = 0; e < kEights; ++e) {
+        mma16816<T>(acc[i][e], a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b[e].x, b[e].y);
+        mma16816<T>(acc[i][e], a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b[e].z, b[e].w);
       }
-    }
   }
-  constexpr int kShift = kRows == 16 ? 1 : kRows == 8 ? 2 : kRows == 4 ? 3 : kRows == 2 ? 4 : 5;
-  float v = sum_rows<kRows>(acc, lane), g = 0.f;
-  if constexpr (kTwo) g = sum_rows<kRows>(gate, lane);
-  if (p.warps > 1) {
-    joined[0][warp][lane] = v;
-    if (kTwo) joined[1][warp][lane] = g;
-    __syncthreads();
-    if (part != 0) return;
-    for (int i = 1; i < p.warps; ++i) {
-      v += joined[0][warp + i][lane];
-      if (kTwo) g += joined[1][warp + i][lane];
-    }
+#pragma unroll
+  for (int i = 0; i < kParts; ++i)
+#pragma unroll
+    for (int e = 0; e < kEights; ++e)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) joined[warp][i][e * 8 + t * 2 + (j & 1)][g + 8 * (j >> 1)] = acc[i][e][j];
+  __syncthreads();
+  const int row = threadIdx.x / kFewColumns, c = threadIdx.x % kFewColumns, n = n0 + c;
+  if (row >= p.rows || n >= p.N) return;
+  float v = 0.f, gate = 0.f;
+  for (int i = 0; i < warps; ++i) {
+    v += joined[i][0][row][c];
+    if constexpr (kTwo) gate += joined[i][1][row][c];
   }
-  const int row = lane >> kShift;
-  if (!in || (lane & ((1 << kShift) - 1)) != 0 || row >= p.rows) return;
   const T* bias = static_cast<const T*>(p.bias);
   if (bias != nullptr) {
     v += static_cast<float>(bias[n]);
-    if (kTwo) g += static_cast<float>(bias[n + p.N]);
+    if (kTwo) gate += static_cast<float>(bias[n + p.N]);
   }
   if (p.saved != nullptr) {
     float* s = static_cast<float*>(p.saved) + row * p.ss + n;
     s[0] = v;
-    if (kTwo) s[p.ss / 2] = g;
+    if (kTwo) s[p.ss / 2] = gate;
   }
   float a, slope;
-  activate_any(p.activation, kTwo ? g : v, a, slope);
+  activate_any(p.activation, kTwo ? gate : v, a, slope);
   if (kTwo) a *= v;
   if (p.residual != nullptr) a += static_cast<float>(static_cast<const T*>(p.residual)[row * p.rs + n]);
   static_cast<T*>(p.y)[row * p.ys + n] = static_cast<T>(a);
 }
 
-template <typename T, int kVec, bool kTwo>
-auto pick_few(int rows) {
-  if (rows <= 1) return &few_rows_kernel<T, 1, kVec, kTwo>;
-  if (rows <= 2) return &few_rows_kernel<T, 2, kVec, kTwo>;
-  if (rows <= 4) return &few_rows_kernel<T, 4, kVec, kTwo>;
-  return rows <= 8 ? &few_rows_kernel<T, 8, kVec, kTwo> : &few_rows_kernel<T, 16, kVec, kTwo>;
+template <typename T, bool kTwo>
+auto pick_few(int rows, bool vec) {
+  if (rows <= 8) return vec ? &few_rows_kernel<T, kTwo, 1, true> : &few_rows_kernel<T, kTwo, 1, false>;
+  return vec ? &few_rows_kernel<T, kTwo, 2, true> : &few_rows_kernel<T, kTwo, 2, false>;
 }
 template <typename T>
 auto pick_few(int rows, bool vec, bool two) {
-  if (two) return vec ? pick_few<T, 8, true>(rows) : pick_few<T, 1, true>(rows);
-  return vec ? pick_few<T, 8, false>(rows) : pick_few<T, 1, false>(rows);
+  return two ? pick_few<T, true>(rows, vec) : pick_few<T, false>(rows, vec);
 }
 
 // ---- dz from stored pre-activations ---------------------------------------------------------------------------------
@@ -316,7 +313,7 @@ slope_kernel(const SlopeParams p) {
       T* dz = static_cast<T*>(p.dz) + row * p.zs + c;
       float d[8], v[8], g[8];
       if (c + 8 <= p.N) {
-        load_vec<T, 8>(dy, d);
+        load_vec<T>(dy, d);
         load_eight(z, v);
         if constexpr (kTwo) load_eight(z + p.ss / 2, g);
       } else {
@@ -385,7 +382,7 @@ row_sum_kernel(const T* dz, long long pitch, long long rows, int N, long long pa
     for (long long r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
       float v[8];
       if (c + 8 <= N) {
-        load_vec<T, 8>(dz + r * pitch + c, v);
+        load_vec<T>(dz + r * pitch + c, v);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = c + j < N ? static_cast<float>(dz[r * pitch + c + j]) : 0.f;
@@ -617,13 +614,11 @@ int b200ta_dense(const void* x, int64_t xs, const void* w, int64_t ws, const voi
     rc = get_device_state(&st);
     if (rc != B200TA_OK) return rc;
     const bool vec = K % 8 == 0 && rows_aligned(x, xs) && rows_aligned(w, ws), f16 = dtype == B200TA_DTYPE_F16;
-    // more warps a column while the device has room for them and each still has a vector a lane
-    int warps = 1;
-    while (warps < kFewWarps && int64_t(N) * warps < int64_t(st->num_sms) * 16 && K > warps * 32 * (vec ? 8 : 1)) warps *= 2;
-    const FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation, warps};
-    const int columns = kFewWarps / warps;
+    const FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation};
+    // sixteen warps where blocks are few (three rows, 1536 -> 384: 9 us instead of 11), eight otherwise, of which more blocks fit
+    const int blocks = (N + kFewColumns - 1) / kFewColumns, warps = blocks <= st->num_sms ? kFewWarps : kFewWarps / 2;
     return launch_kernel(st, kKernelDenseHelpers, f16 ? pick_few<__half>(int(rows), vec, gated) : pick_few<__nv_bfloat16>(int(rows), vec, gated),
-                         dim3(unsigned((N + columns - 1) / columns)), kFewWarps * 32, 0, stream, p);
+                         dim3(unsigned(blocks)), warps * 32, 0, stream, p);
   }
   B200TA_REQUIRE(rows_aligned(x, xs) && rows_aligned(w, ws) && (!residual || rows_aligned(residual, rs)) &&
                      (!saved || rows_aligned(saved, ss)),
