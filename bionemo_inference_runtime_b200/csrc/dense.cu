@@ -394,7 +394,7 @@ row_sum_kernel(const T* dz, long long pitch, long long rows, int N, long long pa
   store_sums(s, joined, part + (long long)blockIdx.y * part_pitch + blockIdx.x * 256, N - int(blockIdx.x) * 256, accumulate);
 }
 
-// out[r][c] = sum over the parts, in a fixed order; two such results (dW and db) in one launch, either of which may be empty.
+// out[r][c] = sum over the parts, in a fixed order; up to three such results (dW, db, dx) in one launch.
 // A thread sums one value, four where they lie together, or eight threads sum one where there are many parts of few values (18 parts of
 // 1024 x 128: 7.5 us, 9.4 MB mostly from L2; a launch and one round of loads bound it).
 struct JoinParams {
@@ -422,18 +422,19 @@ __device__ __forceinline__ void join_by_four(const JoinParams& p, long long firs
 }
 template <typename T>
 __global__ void __launch_bounds__(256)
-join_kernel(const JoinParams a, const JoinParams b) {
+join_kernel(const JoinParams a, const JoinParams b, const JoinParams c) {
   __shared__ float joined[8][33];
   pdl_trigger();
   pdl_wait();
-  const bool second = int(blockIdx.x) >= a.blocks;
-  const JoinParams& p = second ? b : a;
-  if (p.slices == 0) return join_by_four<T>(p, (blockIdx.x - (second ? a.blocks : 0)) * 256LL + threadIdx.x);
+  const int block = int(blockIdx.x);
+  const JoinParams& p = block < a.blocks ? a : block < a.blocks + b.blocks ? b : c;
+  const long long own = block - (block < a.blocks ? 0 : block < a.blocks + b.blocks ? a.blocks : a.blocks + b.blocks);
+  if (p.slices == 0) return join_by_four<T>(p, own * 256 + threadIdx.x);
   const int values = 256 / p.slices, slice = p.slices == 1 ? 0 : threadIdx.x >> 5, lane = p.slices == 1 ? threadIdx.x : threadIdx.x & 31;
   const long long total = p.rows * p.columns;
-  for (long long i0 = (blockIdx.x - (second ? a.blocks : 0)) * (long long)values; i0 < total; i0 += (long long)p.blocks * values) {
-    const long long i = i0 + lane, r = i / p.columns, c = i - r * p.columns;
-    const float* src = p.part + r * p.pitch + c;
+  for (long long i0 = own * values; i0 < total; i0 += (long long)p.blocks * values) {
+    const long long i = i0 + lane, r = i / p.columns;
+    const float* src = p.part + r * p.pitch + (i - r * p.columns);
     float sum = 0.f;
     if (i < total)
 #pragma unroll 8
@@ -529,6 +530,20 @@ Split split_rows(int64_t rows, int64_t n_rows, int64_t n_outer, int64_t columns,
   }
   return best;
 }
+// How dx = dz W is cut along the hidden units: in parts where few row tiles would walk many of them (1799 rows of 40, 5958 gated
+// units: 66 us in one, 20 in parts with their join).  Many rows have tiles enough.
+Split split_units(int64_t rows, int64_t units, int64_t outer, int64_t K, int num_sms) {
+  const int64_t kblocks = (units + matmul::kBK - 1) / matmul::kBK * outer;
+  Split best{int(kblocks), 1, false};
+  double least = 1e300;
+  for (int64_t tried = 1; tried <= 64 && tried <= kblocks && (tried == 1 || rows < int64_t(num_sms) * 64); tried += tried < 8 ? 1 : tried < 24 ? 2 : 8) {
+    const int64_t per = (kblocks + tried - 1) / tried, parts = (kblocks + per - 1) / per;
+    double cost = choose_tiling({parts > 1 ? kPartial : kPlain, false, false, rows, 1, K, int(per), int(parts)}, num_sms).clocks;
+    if (parts > 1) cost += 8000 + 8.0 * double(parts) * double(rows) * double(K) / 2400;
+    if (cost < least * 0.95) least = cost, best = {int(per), int(parts), false};
+  }
+  return best;
+}
 constexpr int kChunkRows = 256;  // chunks of the backward pass are multiples of this
 // Rows of a partial sum of db: enough blocks of 256 columns to fill the device a few times, at least 32 rows each.
 int sum_rows(int64_t rows, int64_t columns, int num_sms) {
@@ -542,8 +557,9 @@ struct BackwardPlan {
   int64_t dz_pitch;   // 0: dz is dy
   Split split;        // of a chunk's rows for dW
   bool direct;        // dW is written by its product
+  Split dx_split;     // of the units for dx
   int rows_sum;       // rows of a partial sum of db
-  int64_t dz, parts, sums, bytes;  // offsets, total
+  int64_t dz, parts, sums, dx_parts, bytes;  // offsets, total
 };
 // Whether dz and dx come from one kernel (narrow.cuh): its blocks take 256 rows each, so from a row tile for half of the SMs on.
 // (Backward pass of a gated layer 128 -> 512: 6000 rows 44 us so and 41 us otherwise, 9472 rows 46 and 44, 16384 rows 48 and 57,
@@ -572,6 +588,8 @@ BackwardPlan make_plan(bool gated, bool slope, bool kept, bool want_dbias, int64
   };
   p.dz = take(p.dz_pitch * (p.chunk < rows ? p.chunk : rows) * 2);
   p.parts = take(p.direct ? 0 : p.split.parts * outer * N * pad4(K) * int64_t(sizeof(float)));
+  p.dx_split = p.chunk >= rows ? split_units(rows, N, outer, K, num_sms) : Split{0, 1, false};
+  p.dx_parts = take(p.dx_split.parts == 1 ? 0 : p.dx_split.parts * rows * pad4(K) * int64_t(sizeof(float)));
   p.rows_sum = sum_rows(p.chunk, kept ? N : outer * N, num_sms);
   const int64_t slots = p.split.sums ? p.split.parts : (p.chunk + p.rows_sum - 1) / p.rows_sum;
   p.sums = take(!want_dbias || (p.split.sums && p.direct) ? 0 : slots * outer * pad8(N) * int64_t(sizeof(float)));
@@ -681,11 +699,12 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
     const int64_t need = (slices == 0 ? n_rows * columns / 4 + 255 : n_rows * columns * slices + 255) / 256, most = int64_t(st->num_sms) * 16;
     return JoinParams{part, out, stride, pitch, n_rows, int(count), columns, slices, wanted ? int(std::min(need, most)) : 0};
   };
-  auto join = [&](const JoinParams& a, const JoinParams& b) {
-    return launch_kernel(st, kKernelDenseHelpers, f16 ? join_kernel<__half> : join_kernel<__nv_bfloat16>, dim3(unsigned(a.blocks + b.blocks)),
-                         256, 0, stream, a, b);
+  auto join = [&](const JoinParams& a, const JoinParams& b, const JoinParams& c) {
+    return launch_kernel(st, kKernelDenseHelpers, f16 ? join_kernel<__half> : join_kernel<__nv_bfloat16>,
+                         dim3(unsigned(a.blocks + b.blocks + c.blocks)), 256, 0, stream, a, b, c);
   };
   const bool narrow = narrow_pays(own_dz, saved != nullptr, rows, K, dx, dxs, st->num_sms);
+  const bool dx_parts = dx != nullptr && !narrow && plan.dx_split.parts > 1 && dxs == K;  // (a join writes dense rows)
 
   for (int64_t r0 = 0; r0 < rows; r0 += plan.chunk) {
     const int64_t n = rows - r0 < plan.chunk ? rows - r0 : plan.chunk;
@@ -728,10 +747,15 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
     }
     if (dx != nullptr && !narrow) {
       Matmul m;
-      m.form = kPlain, m.b_mn = true, m.f16 = f16;
+      m.form = dx_parts ? kPartial : kPlain, m.b_mn = true, m.f16 = f16;
       m.a = {dz, n, N, zs, outer, zs / 2};
       m.b = {w, N, K, ws, outer, int64_t(N) * ws};
-      m.out = {static_cast<char*>(dx) + r0 * dxs * 2, n, K, dxs};
+      if (dx_parts) {
+        m.out = {ws_base + plan.dx_parts, n, K, pad4(K), plan.dx_split.parts, n * pad4(K)};
+        m.kblocks_split = plan.dx_split.kblocks;
+      } else {
+        m.out = {static_cast<char*>(dx) + r0 * dxs * 2, n, K, dxs};
+      }
       if (dw != nullptr) m.beside = kBesideFirst;
       m.what = "dense_backward dx";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
@@ -765,12 +789,13 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
     }
   }
   const bool parts_left = dw != nullptr && !direct, sums_left = dbias != nullptr && !(product_sums && direct);
-  if (!parts_left && !sums_left) return B200TA_OK;
+  if (!parts_left && !sums_left && !dx_parts) return B200TA_OK;
   const int64_t chunk = plan.chunk < rows ? plan.chunk : rows;
   const JoinParams a = join_of(parts_left, parts, plan.split.parts, outer * N * pad4(K), pad4(K), outer * N, K, dw);
   const JoinParams b = product_sums ? join_of(sums_left, sums, plan.split.parts, outer * N, N, outer, N, dbias)
                                     : join_of(sums_left, sums, (chunk + plan.rows_sum - 1) / plan.rows_sum, sum_pitch, sum_pitch / outer, outer, N, dbias);
-  return join(a, b);
+  const JoinParams c = join_of(dx_parts, reinterpret_cast<const float*>(ws_base + plan.dx_parts), plan.dx_split.parts, rows * pad4(K), pad4(K), rows, K, dx);
+  return join(a, b, c);
 }
 
 int b200ta_copy_rows(const b200ta_copy* jobs, int count, void* stream) {

@@ -322,6 +322,26 @@ def test_parts_of_the_weight_gradient():
     check_layer(**layer_inputs(20000, 64, 64, torch.bfloat16, False, True, True))
 
 
+@pytest.mark.parametrize("gated", [False, True], ids=["dense", "gated"])
+@pytest.mark.parametrize("rows,K,N", [(40, 33, 6000), (300, 130, 5001), (129, 1024, 4096)])
+def test_parts_of_the_input_gradient(rows, K, N, gated):
+    """Few rows and many hidden units: dx in parts of the units, with and without the other gradients beside it."""
+    given = layer_inputs(rows, K, N, torch.bfloat16, gated, True, False)
+    check_layer(activation="silu", **given)
+    back = ops.gated_dense_backward if gated else ops.dense_backward
+    both = back(given["dy"], given["x"], given["w"], given["bias"], activation="silu")
+    alone = back(given["dy"], given["x"], given["w"], given["bias"], activation="silu", want_dweight=False, want_dbias=False)
+    assert torch.equal(both[0], alone[0]) and alone[1] is None
+
+
+@pytest.mark.parametrize("gated", [False, True], ids=["dense", "gated"])
+@pytest.mark.parametrize("rows,K,N", [(1, 8, 16), (2, 33, 17), (7, 1703, 130), (8, 520, 15), (9, 100, 300), (13, 31, 257), (16, 1030, 64), (16, 4096, 40)])
+def test_few_rows(rows, K, N, gated):
+    """Up to 16 rows: one and two groups of eight, columns and inputs that fill the products and do not."""
+    for dtype in (torch.bfloat16, torch.float16):
+        check_layer(activation="gelu", **layer_inputs(rows, K, N, dtype, gated, True, not gated))
+
+
 def test_activations_far_out():
     """Slopes and values where exponentials overflow, and NaN, pass column by column."""
     z = torch.tensor([0.0, -0.0, 1e-3, -5, 5, -20, 20, -44, 44, -90, 90, -1e4, 1e4, -1e15, 1e15, -3e38, 3e38], device=DEV)
