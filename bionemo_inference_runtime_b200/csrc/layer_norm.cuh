@@ -30,7 +30,8 @@ struct NormParams {
   const void *x, *dy, *w, *b;
   void *y, *dx;
   float2* stats;   // {rstd, -mean * rstd} per row: written by the forward pass (if not NULL), read by the backward pass
-  float* partial;  // [blocks][2][width]
+  float* partial;  // [blocks][2][width], or NULL where sums are not wanted or one block has them all
+  void *dw, *db;   // of that block, each may be NULL
   long long xs, ys, dys, dxs, rows;
   int width;
   int lanes;           // threads that share a row, a power of two

@@ -9,6 +9,8 @@
 namespace b200ta {
 namespace {
 
+constexpr int64_t kOneBlock = 16384;  // elements of x
+
 // Blocks of a multiprocessor: 8 values a thread leave room for three of 256 threads, more (or single elements beside
 // them) for two.
 __host__ __device__ constexpr int grad_blocks_of(int threads, int values, bool shifted) {
@@ -174,7 +176,7 @@ norm_grad_kernel(const NormParams p) {
     }
     take = stage;
   }
-  if (p.partial == nullptr) return;
+  if (p.partial == nullptr && p.dw == nullptr && p.db == nullptr) return;
   norm::copy_wait<0>();
   __syncthreads();  // the slots are free
   // the groups' sums, joined in pairs: half of the groups that are left hand theirs to the other half
@@ -205,29 +207,54 @@ norm_grad_kernel(const NormParams p) {
     if (group < half) each(joined + group * 2 * p.width, true);
     __syncthreads();
   }
-  if (group == 0) each(p.partial + (long long)blockIdx.x * 2 * p.width, false);
+  if (group != 0) return;
+  if (p.partial != nullptr) return each(p.partial + (long long)blockIdx.x * 2 * p.width, false);
+  W *out_w = static_cast<W*>(p.dw), *out_b = static_cast<W*>(p.db);
+  auto put = [&](int c, float w_c, float b_c) {
+    if (out_w != nullptr) out_w[c] = static_cast<W>(w_c);
+    if (out_b != nullptr) out_b[c] = static_cast<W>(b_c);
+  };
+#pragma unroll
+  for (int i = 0; i < kItems; ++i)
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      const int c = place.column + i * lanes * kVec + 2 * j;
+      float w0, w1, b0, b1;
+      dw[i][j].to(w0, w1), db[i][j].to(b0, b1);
+      if (has(i)) put(c, w0, b0), put(c + 1, w1, b1);
+    }
+#pragma unroll
+  for (int i = 0; i < kSingles; ++i)
+    if (place.single[i] >= 0) put(place.single[i], single_dw[i], single_db[i]);
 }
 
-// dw and db: column sums of the blocks' partial sums.  A block takes 8 of the 2 * width columns, 128 threads a column.
-template <typename T>
+// dw and db: column sums of the blocks' partial sums.  A block takes kColumns of the 2 * width columns, 1024 / kColumns threads a
+// column: 8 columns while that gives no more blocks than run at once, then 32 or 128 (backward of 2000 rows of 16384 in bf16:
+// 124 us by eights alone, 103 so; of 8192 rows of 4096: 62 and 56).
+template <typename T, int kColumns>
 __global__ void __launch_bounds__(1024)
 norm_join_kernel(const float* partial, int blocks, int width, T* dw, T* db) {
-  __shared__ float part[32][8];
+  constexpr int kThreads = 1024 / kColumns, kRows = kColumns < 32 ? 32 : kThreads;  // rows of `part`
+  __shared__ float part[kRows][kColumns];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, k = threadIdx.x >> 3, c = blockIdx.x * 8 + (threadIdx.x & 7);
+  const int k = threadIdx.x / kColumns, c = blockIdx.x * kColumns + threadIdx.x % kColumns;
   float sum = 0.f;
   if (c < 2 * width)
 #pragma unroll 4
-    for (int b = k; b < blocks; b += 128) sum += __ldg(partial + (long long)b * 2 * width + c);
-  sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-  sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-  if (lane < 8) part[threadIdx.x >> 5][lane] = sum;
+    for (int b = k; b < blocks; b += kThreads) sum += __ldg(partial + (long long)b * 2 * width + c);
+  if constexpr (kColumns < 32) {
+#pragma unroll
+    for (int o = kColumns; o < 32; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) < kColumns) part[threadIdx.x >> 5][threadIdx.x & 31] = sum;
+  } else {
+    part[k][threadIdx.x % kColumns] = sum;
+  }
   __syncthreads();
-  if (threadIdx.x < 8 && c < 2 * width) {
+  if (threadIdx.x < kColumns && c < 2 * width) {
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) sum += part[i][threadIdx.x];
+    for (int i = 0; i < kRows; ++i) sum += part[i][threadIdx.x];
     T* dst = c < width ? dw : db;
     if (dst != nullptr) dst[c < width ? c : c - width] = static_cast<T>(sum);
   }
@@ -282,18 +309,26 @@ int b200ta_layer_norm_backward(const void* dy, int64_t dys, const void* x, int64
   const int joined = sums && groups > 1 ? groups / 2 * 2 * width * int(sizeof(float)) : 0;
   const int ring = norm::stages_of(2 * s.items, s.threads, resident) * 2 * s.items * s.threads * 16;
   const int smem = joined > ring ? joined : ring;
-  const int blocks = norm_blocks(rows, int64_t(st->num_sms) * resident, groups, vec, s.shifted);
+  // Little work is for one block, whose sums are dw and db (4 rows of 317 in fp32: 8.9 us in two launches, 6.4 in one;
+  // with twice the limit, 85 rows of 384 in bf16, 9.0 and 10.3), unless its step would not be a whole period of the rows' alignment.
+  const bool one = sums && rows * width <= kOneBlock && (!s.shifted || groups % vec == 0 || rows <= groups);
+  if (one) p.partial = nullptr, p.dw = dweight, p.db = dbias;
+  const int blocks = one ? 1 : norm_blocks(rows, int64_t(st->num_sms) * resident, groups, vec, s.shifted);
   const bool f32 = param_dtype == B200TA_DTYPE_F32;
   int (*launch)(DeviceState*, int, int, int, void*, const NormParams&);
   if (dtype == B200TA_DTYPE_BF16) launch = f32 ? pick<__nv_bfloat16, float>(s) : pick<__nv_bfloat16, __nv_bfloat16>(s);
   else if (dtype == B200TA_DTYPE_F16) launch = f32 ? pick<__half, float>(s) : pick<__half, __half>(s);
   else launch = pick<float, float>(s);
   rc = launch(st, blocks, s.threads, smem, stream, p);
-  if (rc != B200TA_OK || !sums) return rc;
-  const dim3 grid{unsigned((2 * width + 7) / 8)};
+  if (rc != B200TA_OK || !sums || one) return rc;
   auto join = [&](auto* dw, auto* db) {
-    return launch_kernel(st, kKernelNorm, norm_join_kernel<std::remove_pointer_t<decltype(dw)>>, grid, 1024, 0, stream, p.partial, blocks,
-                         width, dw, db);
+    using P = std::remove_pointer_t<decltype(dw)>;
+    auto launch_join = [&](auto* kernel, int columns) {
+      return launch_kernel(st, kKernelNorm, kernel, dim3(unsigned((2 * width + columns - 1) / columns)), 1024, 0, stream,
+                           static_cast<const float*>(p.partial), blocks, width, dw, db);
+    };
+    if (2 * width <= st->num_sms * 2 * 8) return launch_join(&norm_join_kernel<P, 8>, 8);
+    return 2 * width <= st->num_sms * 2 * 32 ? launch_join(&norm_join_kernel<P, 32>, 32) : launch_join(&norm_join_kernel<P, 128>, 128);
   };
   if (f32) return join(static_cast<float*>(dweight), static_cast<float*>(dbias));
   if (param_dtype == B200TA_DTYPE_F16) return join(static_cast<__half*>(dweight), static_cast<__half*>(dbias));
