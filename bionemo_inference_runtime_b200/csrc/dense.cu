@@ -591,8 +591,9 @@ BackwardPlan make_plan(bool gated, bool slope, bool kept, bool want_dbias, int64
   p.dx_split = p.chunk >= rows ? split_units(rows, N, outer, K, num_sms) : Split{0, 1, false};
   p.dx_parts = take(p.dx_split.parts == 1 ? 0 : p.dx_split.parts * rows * pad4(K) * int64_t(sizeof(float)));
   p.rows_sum = sum_rows(p.chunk, kept ? N : outer * N, num_sms);
-  const int64_t slots = p.split.sums ? p.split.parts : (p.chunk + p.rows_sum - 1) / p.rows_sum;
-  p.sums = take(!want_dbias || (p.split.sums && p.direct) ? 0 : slots * outer * pad8(N) * int64_t(sizeof(float)));
+  // Room for the sums of either way: db may be wanted without dW, whose product would have given them.
+  const int64_t by_product = p.split.sums && !p.direct ? p.split.parts : 0, by_rows = (p.chunk + p.rows_sum - 1) / p.rows_sum;
+  p.sums = take(want_dbias ? std::max(by_product, by_rows) * outer * pad8(N) * int64_t(sizeof(float)) : 0);
   return p;
 }
 // The plan is a function of the sizes; the last few of a thread are kept, since making one takes longer than a launch.

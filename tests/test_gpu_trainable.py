@@ -316,6 +316,33 @@ def test_narrow_layers_of_many_rows(rows, K, N, gated):
     assert torch.equal(both[0], alone[0]) and alone[1] is None
 
 
+@pytest.mark.parametrize("rows,K,N,gated", [(9600, 104, 1000, True), (3000, 64, 640, False), (1000, 40, 3000, True), (2047, 520, 1288, False), (300, 1600, 264, True)])
+def test_the_workspace_is_enough_for_every_choice_of_gradients(rows, K, N, gated):
+    """Each of dx, dW and db with and without the others: nothing is written behind the workspace, and what is wanted is the same."""
+    given = layer_inputs(rows, K, N, torch.bfloat16, gated, True, False)
+    x, w, bias, dy = given["x"], given["w"], given["bias"], given["dy"]
+    gelu, bf16, outer = 3, 0, 2 if gated else 1
+    needs = [_lib.load().b200ta_dense_backward_workspace_bytes(gelu, gated, 0, want_dbias, rows, K, N) for want_dbias in (0, 1)]
+    held = torch.empty(max(needs) + (64 << 20), device=DEV, dtype=torch.uint8)
+    wanted = {}
+    for want in [(1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (1, 0, 1), (0, 1, 1)]:
+        held.fill_(0x5A)
+        need = needs[want[2]]
+        dx, dw, db = torch.zeros_like(x), torch.zeros_like(w), torch.zeros(outer * N, device=DEV, dtype=x.dtype)
+        dx_p, dw_p, db_p = (t.data_ptr() if on else None for t, on in zip((dx, dw, db), want, strict=True))
+        _lib.call("b200ta_dense_backward", dy.data_ptr(), N, x.data_ptr(), K, w.data_ptr(), K, bias.data_ptr(), None, 0, dx_p, K, dw_p, db_p,
+                  held.data_ptr(), need, bf16, gelu, gated, rows, K, N, torch.cuda.current_stream().cuda_stream)
+        assert (held[need:] == 0x5A).all(), want
+        for name, t, on in zip(("dx", "dw", "db"), (dx, dw, db), want, strict=True):
+            if not on:
+                assert not t.any()
+            elif name == "dx":
+                assert torch.equal(t, wanted.setdefault(name, t)), want
+            else:  # their sums may run in another order: one rounding apart, and 32-bit sums of rows values of 1 or so
+                first = wanted.setdefault(name, t.double())
+                within(t, first, 2.02 * half_spacing(t.dtype) * first.abs() + 4 * SUM * rows, name)
+
+
 def test_parts_of_the_weight_gradient():
     """dW in one piece, and in parts of the rows."""
     check_layer(**layer_inputs(256, 2048, 2048, torch.bfloat16, False, True, True))
