@@ -561,11 +561,15 @@ struct BackwardPlan {
   int rows_sum;       // rows of a partial sum of db
   int64_t dz, parts, sums, dx_parts, bytes;  // offsets, total
 };
-// Whether dz and dx come from one kernel (narrow.cuh): its blocks take 256 rows each, so from a row tile for half of the SMs on.
-// (Backward pass of a gated layer 128 -> 512: 6000 rows 44 us so and 41 us otherwise, 9472 rows 46 and 44, 16384 rows 48 and 57,
-// 147456 rows 194 and 229; 64 -> 256, 147456 rows: 101 and 127.)
-bool narrow_pays(bool own_dz, bool kept, int64_t rows, int K, const void* dx, int64_t dxs, int num_sms) {
-  return own_dz && !kept && K <= 128 && dx != nullptr && rows_aligned(dx, dxs) && rows >= int64_t(num_sms) * 64;
+// Whether dz and dx come from one kernel (narrow.cuh).  Its blocks walk 64 units of 256 rows in some 6000 clocks (dense layers: 4800), one
+// item of 256 rows after the other, where two products take some 9000 (5500) for 128 units of 128 rows, shared evenly, and 25000 for
+// their launches and ends.  (Backward pass of a gated layer 128 -> 512: 9472 rows 46 us so and 44 otherwise, 16384 rows 48 and 57,
+// 147456 rows 194 and 229; 128 -> 128, 9472 rows: 32 and 39; 104 -> 3160, 14196 rows: 265 and 208.)
+bool narrow_pays(bool own_dz, bool kept, bool gated, int64_t rows, int K, int N, const void* dx, int64_t dxs, int num_sms) {
+  if (!own_dz || kept || K > 128 || dx == nullptr || !rows_aligned(dx, dxs) || rows <= kChunkRows) return false;
+  const double items = double((rows + 255) / 256), waves = double((int64_t(items) + num_sms - 1) / num_sms);
+  const double one = waves * double((N + 63) / 64) * (gated ? 6000 : 4800) + 8000;
+  return one < 25000 + (gated ? 9000 : 5500) * (double(rows) / 128) * (double(N) / 128) / num_sms;
 }
 BackwardPlan make_plan(bool gated, bool slope, bool kept, bool want_dbias, int64_t rows, int K, int N, int num_sms) {
   BackwardPlan p{};
@@ -704,7 +708,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
     return launch_kernel(st, kKernelDenseHelpers, f16 ? join_kernel<__half> : join_kernel<__nv_bfloat16>,
                          dim3(unsigned(a.blocks + b.blocks + c.blocks)), 256, 0, stream, a, b, c);
   };
-  const bool narrow = narrow_pays(own_dz, saved != nullptr, rows, K, dx, dxs, st->num_sms);
+  const bool narrow = narrow_pays(own_dz, saved != nullptr, gated != 0, rows, K, N, dx, dxs, st->num_sms);
   const bool dx_parts = dx != nullptr && !narrow && plan.dx_split.parts > 1 && dxs == K;  // (a join writes dense rows)
 
   for (int64_t r0 = 0; r0 < rows; r0 += plan.chunk) {
