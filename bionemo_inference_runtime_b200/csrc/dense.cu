@@ -536,7 +536,8 @@ Split split_units(int64_t rows, int64_t units, int64_t outer, int64_t K, int num
   const int64_t kblocks = (units + matmul::kBK - 1) / matmul::kBK * outer;
   Split best{int(kblocks), 1, false};
   double least = 1e300;
-  for (int64_t tried = 1; tried <= 64 && tried <= kblocks && (tried == 1 || rows < int64_t(num_sms) * 64); tried += tried < 8 ? 1 : tried < 24 ? 2 : 8) {
+  for (int64_t tried = 1; tried <= 64 && tried <= kblocks && (tried == 1 || rows < int64_t(num_sms) * 64);
+       tried += tried < 8 ? 1 : tried < 24 ? 2 : 8) {
     const int64_t per = (kblocks + tried - 1) / tried, parts = (kblocks + per - 1) / per;
     double cost = choose_tiling({parts > 1 ? kPartial : kPlain, false, false, rows, 1, K, int(per), int(parts)}, num_sms).clocks;
     if (parts > 1) cost += 8000 + 8.0 * double(parts) * double(rows) * double(K) / 2400;

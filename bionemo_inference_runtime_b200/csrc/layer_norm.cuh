@@ -9,8 +9,10 @@
 // the variance from centred values.  Issue slots come next (a first version with 64-bit index arithmetic and unpacked sums
 // needed 200 instructions for 16 values a lane and stayed at half the bandwidth), so addresses advance by constants, sums
 // and products are made in packed pairs, and groups of lanes have a size known at compile time.  Blocks are persistent; a
-// thread keeps its columns, and with them their parameters in registers (of up to 16 columns), and copies the next rows' vectors into its own slots
-// of shared memory while it works on one (registers alone hold too few bytes in flight).
+// thread keeps its columns, and with them their parameters in registers (of up to 16 columns), and copies the next rows'
+// vectors into its own slots of shared memory while it works on one (registers alone hold too few bytes in flight).
+// Measured: 262144 rows of 128 in bf16 forward 23 us (5.8 TB/s), backward 38 us from a cold L2 (5.2 TB/s) and 4.4 for its join;
+// 20000 rows of 1024 in fp32 28 and 46; 6001 of 8192 in fp16 45 and 87.
 //
 // Rows that are not 16-byte aligned (odd widths, odd pitches) take the same path: vectors lie on the 16-byte boundaries of the
 // row that is written, and the at most 2 * 7 elements (fp32: 3) before the first and behind the last whole vector are taken by

@@ -137,8 +137,8 @@ __host__ __device__ constexpr uint32_t idesc(bool f16, int m, int n, bool a_mn, 
   return make_idesc_bf16(m, n, a_mn, b_mn) & ~(f16 ? (1u << 7 | 1u << 10) : 0u);
 }
 
-// y / dz of kN of a group's 32 columns, from column kFirst, of one row, as 16-bit pairs.  v: accumulators (kGated*: of the values), g: of the gates, aux: residual
-// (with has_aux) or dy; kGatedGrad: y the gradients of the values, yg those of the gates.
+// y / dz of kN of a group's 32 columns, from column kFirst, of one row, as 16-bit pairs.  v: accumulators (kGated*: of the
+// values), g: of the gates, aux: residual (with has_aux) or dy; kGatedGrad: y the gradients of the values, yg those of the gates.
 template <typename T, MatmulForm kForm, int kAct, int kFirst, int kN>
 __device__ __forceinline__ void finish(const float (&v)[kN], const float (&g)[kN], bool has_aux, const uint32_t (&aux)[16],
                                        uint32_t (&y)[16], uint32_t (&yg)[16]) {
