@@ -139,6 +139,27 @@ def test_layer_norm_rows_on_other_boundaries(rows, width, dtype):
         assert not held.any()
 
 
+@pytest.mark.parametrize("rows,width", [(1, 300), (4, 317), (40, 384), (60, 200), (2000, 8), (1237, 1001), (500, 8192)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_layer_norm_gradients_one_by_one(rows, width, dtype):
+    """Each of dx, dweight and dbias with and without the others, and nothing written behind the workspace."""
+    x, dy, w = (randn(*shape, seed=i, dtype=dtype) for i, shape in enumerate(((rows, width), (rows, width), (width,))))
+    stats = ops.layer_norm(x, w, want_stats=True)[1]
+    code = _lib.DTYPE_BF16 if dtype == torch.bfloat16 else _lib.DTYPE_F32
+    need = _lib.load().b200ta_layer_norm_workspace_bytes(rows, width)
+    held = torch.empty(need + (1 << 20), device=DEV, dtype=torch.uint8)
+    wanted = {}
+    for want in [(1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1)]:
+        held.fill_(0x5A)
+        out = {"dx": torch.zeros_like(x), "dweight": torch.zeros_like(w), "dbias": torch.zeros_like(w)}
+        dx, dw, db = (t.data_ptr() if on else None for t, on in zip(out.values(), want, strict=True))
+        _lib.call("b200ta_layer_norm_backward", dy.data_ptr(), width, x.data_ptr(), width, stats.data_ptr(), w.data_ptr(), code, dx, width, dw, db,
+                  held.data_ptr(), need, code, rows, width, torch.cuda.current_stream().cuda_stream)
+        assert (held[need:] == 0x5A).all(), want
+        for (name, t), on in zip(out.items(), want, strict=True):
+            assert torch.equal(t, wanted.setdefault(name, t)) if on else not t.any(), (name, want)
+
+
 def test_layer_norm_strides_and_leading_shapes():
     base = randn(6, 5, 3, 160, seed=1)
     for x in (base[..., 7:107], base[:, 1:4, :, ::2], base.transpose(0, 2), base[:, :, 1], base.permute(0, 1, 3, 2), base[:0],
