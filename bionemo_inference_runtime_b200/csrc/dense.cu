@@ -119,9 +119,15 @@ int run_matmul(const Matmul& m, void* stream) {
   if (p.has_saved && (rc = map_of(&maps.saved, m.saved, 4, 16, 32, 1, SWZ_64, m.what)) != B200TA_OK) return rc;
   const int blocks = p.resident ? p.resident * p.tiles_n : std::min(p.work, p.pair ? st->num_sms / 2 : st->num_sms);
   const int grid = p.pair ? 2 * blocks : blocks;
-  // Two sets of finishing warps are out of step, so that one computes while the other loads and stores, and a warp's waits
-  // serve twice the columns; a block's only tile is for all of them.
-  p.alternate = p.resident ? p.tiles_m > p.resident : p.work > blocks;
+  // Sets of finishing warps are out of step, so that one computes while another loads and stores, and a warp's waits serve more
+  // columns; with a single group of 32 result columns to a tile, two sets would leave half of the warps without work.  A block's
+  // only tile is for all of them.  (Sums of A over k lie behind 128 accumulator columns.)
+  const bool several = p.resident ? p.tiles_m > p.resident : p.work > blocks;
+  p.buffers = p.tile_n <= 128 && p.sums == nullptr ? 2 : 1;
+  p.sets = !several ? 0 : units <= 32 || p.columns <= 32 ? 2 : 1;
+  // A set sees the phases of its own tiles alone, and a wait cannot tell a phase from the one after the next: every phase of an
+  // accumulator has to be the same set's, so there are as many accumulators as sets at least.
+  p.sets = std::min(p.sets, p.buffers);
   if (m.form == kDenseGrad || m.form == kGatedGrad) return launch_matmul_grad(st, m, maps, p, grid, stream);
   if (m.b_mn) return launch_matmul_product(st, m, maps, p, grid, stream);
   return launch_matmul_forward(st, m, maps, p, grid, stream);

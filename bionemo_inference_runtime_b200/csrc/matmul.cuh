@@ -17,7 +17,7 @@
 // each with its 128 rows of A and half of B (cta_group::2), which halves what a tile of B costs in shared memory and from L2.
 // Warp roles (576 threads): warps 0-15 finish tiles (TMEM lane = row, groups of 32 columns), warp 16
 // loads [128 x 64] and [tile_n x 64] operand blocks by TMA into a ring, warp 17 issues tcgen05.mma into two accumulators of
-// 256 columns, one filled while the other is finished.  Where all of a column tile of B fits in half of the ring (64 KiB: 128
+// 256 columns (four of 128 for tiles of that width), one filled while others are finished.  Where all of a column tile of B fits in half of the ring (64 KiB: 128
 // wide layers), it is loaded once and only A passes through the ring.  The finishing warps fetch what they read beside the
 // accumulators (residual, dy) by TMA a group ahead and store by TMA: a lane's own accesses to 32 rows occupy the load-store
 // unit for some 56 clocks.  Results whose rows TMA cannot address are stored from the same slabs, a row at a time.
@@ -56,7 +56,7 @@ struct MatmulParams {
   int has_aux;                         // kDense: a residual
   int has_saved;                       // kDense, kGated: D + bias is stored as well, in 32 bits
   int accumulate;                      // kPartial: add to what the parts hold
-  int alternate;                       // the finishing warps take tiles in two sets, in turn
+  int sets, buffers;                   // logarithms: sets of finishing warps that take tiles in turn (1, 2, 4); accumulators (2, 4)
   int beside;                          // kBesideFirst, kBesideSecond: see there
   void* sums;                          // kPlain, kPartial with MN-major A, tiles of up to 128: sums of A over k, [outer][rows] in
                                        // the operands' type (kPartial: [split][outer][rows] in 32 bits), or NULL
@@ -84,7 +84,7 @@ constexpr int kSmSlabs = kRingBytes;       // three for each finishing warp
 constexpr int kSmOnes = kSmSlabs + kFinishers * 3 * kSlab;  // an operand block of ones, [16 x 16]
 constexpr int kSmBars = kSmOnes + 512;
 enum Bar {
-  FULL = 0, EMPTY = kMaxStages, ACC_FULL = 2 * kMaxStages, ACC_EMPTY = ACC_FULL + 2, B_FULL = ACC_EMPTY + 2, AUX = B_FULL + 1,
+  FULL = 0, EMPTY = kMaxStages, ACC_FULL = 2 * kMaxStages, ACC_EMPTY = ACC_FULL + 4, B_FULL = ACC_EMPTY + 4, AUX = B_FULL + 1,
   NUM_BARS = AUX + kFinishers
 };
 constexpr int kSmTotal = kSmBars + NUM_BARS * 8 + 32;
@@ -313,9 +313,9 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       mbar_init(bars + (FULL + i) * 8, 1);
       mbar_init(bars + (EMPTY + i) * 8, 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(bars + (ACC_FULL + i) * 8, 1);
-      mbar_init(bars + (ACC_EMPTY + i) * 8, (kPair ? 2 * kFinishers : kFinishers) >> p.alternate);
+      mbar_init(bars + (ACC_EMPTY + i) * 8, (kPair ? 2 * kFinishers : kFinishers) >> p.sets);
     }
     mbar_init(bars + B_FULL * 8, 1);
     for (int i = 0; i < kFinishers; ++i) mbar_init(bars + (AUX + i) * 8, 1);
@@ -424,8 +424,9 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       if (p.resident) ok = mbar_wait_warp(bars + B_FULL * 8, 0, abort_flag);
       for (int i = 0; ok && i < items; ++i) {
         const Item t = item_of<kPair, kAMn>(p, i, units);
-        const uint32_t acc = tb + (i & 1) * 256;
-        ok = mbar_wait_warp(bars + (ACC_EMPTY + (i & 1)) * 8, ((i >> 1) & 1) ^ 1, abort_flag);
+        const int buffer = i & ((1 << p.buffers) - 1);
+        const uint32_t acc = tb + buffer * (512 >> p.buffers);
+        ok = mbar_wait_warp(bars + (ACC_EMPTY + buffer) * 8, ((i >> p.buffers) & 1) ^ 1, abort_flag);
         for (int kb = t.kb0; ok && kb < t.kb1; ++kb) {
           ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
           if (!ok) break;
@@ -453,17 +454,16 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (++stage == p.stages) stage = 0, phase ^= 1u;
         }
         if (!ok) break;
-        if constexpr (kPair) umma_commit_pair_warp(bars + (ACC_FULL + (i & 1)) * 8);
-        else umma_commit_warp(bars + (ACC_FULL + (i & 1)) * 8);
+        if constexpr (kPair) umma_commit_pair_warp(bars + (ACC_FULL + buffer) * 8);
+        else umma_commit_warp(bars + (ACC_FULL + buffer) * 8);
       }
     }
   } else {
     // ------------------------------------------------------------------ finishing warps
     if (p.beside != kBesideSecond) pdl_wait();
-    // All of them on every tile, each with every fourth group of 32 result columns; or (alternate) eight on the even tiles and
-    // eight on the odd ones, with every second group.
-    const int first_i = p.alternate ? warp >> 3 : 0, step_i = 1 + p.alternate;
-    const int first_g = p.alternate ? (warp >> 2) & 1 : warp >> 2, step_g = p.alternate ? 2 : 4;
+    // All of them on every tile, each with every fourth group of 32 result columns; or eight on the even tiles and eight on the
+    // odd ones, with every second group; or four on every fourth tile, with all groups.
+    const int first_i = warp >> (4 - p.sets), step_i = 1 << p.sets, step_g = 4 >> p.sets, first_g = (warp >> 2) & (step_g - 1);
     const int m = (warp & 3) * 32 + int(rank) * kBM;
     const uint32_t lane_acc = tmem_base + (uint32_t((warp & 3) * 32) << 16);
     const uint32_t slabs = base + kSmSlabs + warp * 3 * kSlab, out_slabs = slabs + (kAux ? kSlab : 0);
@@ -526,7 +526,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     auto release = [&](int i) {  // the accumulator is in registers
       tc_fence_before();
       __syncwarp();
-      const uint32_t bar = bars + (ACC_EMPTY + (i & 1)) * 8;
+      const uint32_t bar = bars + (ACC_EMPTY + (i & ((1 << p.buffers) - 1))) * 8;
       if (kPair) mbar_arrive_cluster_warp(in_first_block(bar));
       else mbar_arrive_warp(bar);
     };
@@ -535,10 +535,11 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     for (int i = first_i; ok && i < items; i += step_i) {
       const Item t = item_of<kPair, kAMn>(p, i, units);
       const int groups = groups_of(t), row = t.m0 + m;
-      ok = mbar_wait_warp(bars + (ACC_FULL + (i & 1)) * 8, (i >> 1) & 1, abort_flag);
+      const int buffer = i & ((1 << p.buffers) - 1);
+      ok = mbar_wait_warp(bars + (ACC_FULL + buffer) * 8, (i >> p.buffers) & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t acc = lane_acc + (i & 1) * 256;
+      const uint32_t acc = lane_acc + buffer * (512 >> p.buffers);
       if (kSums && p.sums != nullptr && t.n0 == 0 && first_g == 0 && groups > 0) {
         float sum[16];
         tmem_load(acc + 128, sum);

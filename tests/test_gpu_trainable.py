@@ -337,6 +337,11 @@ def test_narrow_layers_of_many_rows(rows, K, N, gated):
     assert torch.equal(both[0], alone[0]) and alone[1] is None
 
 
+def test_sums_of_many_parts_of_narrow_tiles():
+    """db from dW's product with few inputs: several tiles a block, with their sums beside them."""
+    check_layer(activation="relu", **layer_inputs(136787, 24, 160, torch.bfloat16, True, True, False))
+
+
 @pytest.mark.parametrize("rows,K,N,gated", [(9600, 104, 1000, True), (3000, 64, 640, False), (1000, 40, 3000, True), (2047, 520, 1288, False), (300, 1600, 264, True)])
 def test_the_workspace_is_enough_for_every_choice_of_gradients(rows, K, N, gated):
     """Each of dx, dW and db with and without the others: nothing is written behind the workspace, and what is wanted is the same."""
