@@ -34,6 +34,7 @@
 
 #include "activation.cuh"
 #include "common.cuh"
+#include "slab_ring.h"
 
 namespace b200ta {
 
@@ -234,6 +235,19 @@ __device__ __forceinline__ void tma_add_3d(const CUtensorMap* m, uint32_t src, i
                "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
+
+// A warp's groups of bulk stores, which its first lane commits and waits for.
+struct StoreGroups {
+  int lane;
+  template <int kNewest>
+  __device__ __forceinline__ void wait_read() const {
+    if (lane == 0) tma_store_wait_read<kNewest>();
+    __syncwarp();
+  }
+  __device__ __forceinline__ void commit() const {
+    if (lane == 0) tma_store_commit();
+  }
+};
 
 // ---- two blocks on one tile -------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -494,34 +508,38 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     };
     if (has_aux) load_aux();
 
-    uint32_t slot = 0;
+    SlabRing<kRing> ring_out;
+    const StoreGroups store_groups{lane};
     // writes a slab (32 columns in 16 bits or 16 in 32 bits, of the 32 rows) and stores it
     auto store = [&](const CUtensorMap& map, const uint32_t (&x)[16], int column, int row, int outer) {
-      const uint32_t slab = out_slabs + slot * kSlab;
-      if (lane == 0) tma_store_wait_read<kRing - 1>();  // the store that used this slab before has read it
-      __syncwarp();
+      const bool direct = (kForm == kDense || kForm == kGated || kForm == kPlain) && p.direct != nullptr && &map == &tm_out;
+      ring_out.pass(
+          store_groups,
+          [&](uint32_t slot) {
+            const uint32_t slab = out_slabs + slot * kSlab;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sts128(slab + sw64_offset(lane, j), make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
-      if ((kForm == kDense || kForm == kGated || kForm == kPlain) && p.direct != nullptr && &map == &tm_out) {
-        __syncwarp();
-        const int rows = p.rows_inner - row < 32 ? p.rows_inner - row : 32;
-        T* to = static_cast<T*>(p.direct) + outer * p.direct_outer + (long long)row * p.direct_pitch + column + lane;
-        if (column + lane < p.columns)
+            for (int j = 0; j < 4; ++j) sts128(slab + sw64_offset(lane, j), make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
+          },
+          [&](uint32_t slot) {
+            const uint32_t slab = out_slabs + slot * kSlab;
+            if (direct) {
+              __syncwarp();
+              const int rows = p.rows_inner - row < 32 ? p.rows_inner - row : 32;
+              T* to = static_cast<T*>(p.direct) + outer * p.direct_outer + (long long)row * p.direct_pitch + column + lane;
+              if (column + lane < p.columns)
 #pragma unroll 4
-          for (int i = 0; i < rows; ++i, to += p.direct_pitch)
-            *reinterpret_cast<uint16_t*>(to) = lds16(slab + sw64_offset(i, lane >> 3) + (lane & 7) * 2);
-        __syncwarp();
-        if (++slot == kRing) slot = 0;
-        return;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        if (kForm == kPartial && p.accumulate) tma_add_3d(&map, slab, column, row, outer);
-        else tma_store_3d(&map, slab, column, row, outer);
-        tma_store_commit();
-      }
-      if (++slot == kRing) slot = 0;
+                for (int i = 0; i < rows; ++i, to += p.direct_pitch)
+                  *reinterpret_cast<uint16_t*>(to) = lds16(slab + sw64_offset(i, lane >> 3) + (lane & 7) * 2);
+              __syncwarp();
+              return;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (kForm == kPartial && p.accumulate) tma_add_3d(&map, slab, column, row, outer);
+              else tma_store_3d(&map, slab, column, row, outer);
+            }
+          });
     };
     auto release = [&](int i) {  // the accumulator is in registers
       tc_fence_before();

@@ -1,0 +1,53 @@
+"""Pre-activations that a dense layer's forward pass keeps for its backward pass, and what the backward pass makes of them."""
+
+import pytest
+import torch
+
+from bionemo_inference_runtime_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+SUM = 2.0 ** -18  # of the sum of the absolute terms: sums of up to a few thousand terms in 32 bits
+
+
+@pytest.fixture(autouse=True)
+def _no_wait_ran_out():
+    _lib.reset_device_status()
+    yield
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+
+
+def randn(*shape, seed, dtype=torch.bfloat16, std=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=DEV) * std).to(dtype)
+
+
+def padded(n):
+    return (n + 7) // 8 * 8
+
+
+@pytest.mark.parametrize("gated", [False, True], ids=["dense", "gated"])
+@pytest.mark.parametrize("rows,K,N,first,pitch", [(4000, 1536, 1283, 0, 1283), (4000, 1536, 1280, 3, 1280), (9000, 1600, 70, 0, 70),
+                                                  (2100, 2048, 2047, 5, 2055)])
+def test_kept_values_beside_results_that_are_stored_in_place(rows, K, N, first, pitch, gated):
+    """Results that a TMA store cannot address (`first` elements off a boundary, rows `pitch` apart) leave row by row, between the
+    bulk stores of the kept values: these are the formula's, and the same bits as beside results that TMA takes."""
+    columns = 2 * N if gated else N
+    x, w, bias = randn(rows, K, seed=1), randn(columns, K, seed=2, std=K ** -0.5), randn(columns, seed=3, std=0.3)
+    layer = ops.gated_dense if gated else ops.dense
+    aligned = torch.empty(rows, padded(N), device=DEV, dtype=x.dtype)[:, :N]
+    y, kept = layer(x, w, bias, activation="gelu", want_saved=True, out=aligned)
+    z, size = x.double() @ w.double().t() + bias.double(), x.double().abs() @ w.double().abs().t() + bias.double().abs()
+    for part in range(2 if gated else 1):
+        got = kept[:, part * padded(N):][:, :N].double()
+        at = slice(part * N, (part + 1) * N)
+        assert ((got - z[:, at]).abs() <= SUM * size[:, at]).all()
+    for _ in range(4):
+        held = torch.empty(first + rows * pitch, device=DEV, dtype=x.dtype)
+        out = held[first:].as_strided((rows, N), (pitch, 1))
+        again, kept_again = layer(x, w, bias, activation="gelu", want_saved=True, out=out)
+        assert torch.equal(again, y)
+        for part in range(2 if gated else 1):
+            at = slice(part * padded(N), part * padded(N) + N)
+            assert torch.equal(kept_again[:, at], kept[:, at])
