@@ -607,6 +607,8 @@ BackwardPlan make_plan(bool gated, bool slope, bool kept, bool want_dbias, int64
   p.sums = take(want_dbias ? std::max(by_product, by_rows) * outer * pad8(N) * int64_t(sizeof(float)) : 0);
   return p;
 }
+// Whether kept pre-activations are read: a dense layer without an activation has dz = dy, whatever its caller kept.
+bool reads_kept(bool given, bool gated, int activation) { return given && (gated || activation != kActNone); }
 // The plan is a function of the sizes; the last few of a thread are kept, since making one takes longer than a launch.
 const BackwardPlan& plan_backward(bool gated, bool slope, bool kept, bool want_dbias, int64_t rows, int K, int N, int num_sms) {
   struct Entry {
@@ -676,7 +678,9 @@ size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int kept
   using namespace b200ta;
   DeviceState* st = nullptr;
   if (rows <= 0 || K <= 0 || N <= 0 || get_device_state(&st) != B200TA_OK) return 0;
-  return size_t(plan_backward(gated, activation != kActNone, kept != 0, want_dbias != 0, rows, K, N, st->num_sms).bytes);
+  return size_t(plan_backward(gated, activation != kActNone, reads_kept(kept != 0, gated != 0, activation), want_dbias != 0, rows, K, N,
+                              st->num_sms)
+                    .bytes);
 }
 
 int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias,
@@ -692,7 +696,8 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
   DeviceState* st = nullptr;
   rc = get_device_state(&st);
   if (rc != B200TA_OK) return rc;
-  const BackwardPlan& plan = plan_backward(gated, activation != kActNone, saved != nullptr, dbias != nullptr, rows, K, N, st->num_sms);
+  const bool kept = reads_kept(saved != nullptr, gated != 0, activation);
+  const BackwardPlan& plan = plan_backward(gated, activation != kActNone, kept, dbias != nullptr, rows, K, N, st->num_sms);
   B200TA_REQUIRE(plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
                                      workspace_bytes >= size_t(plan.bytes)),
                  "dense_backward: the workspace must be 256-byte aligned and of %lld bytes", (long long)plan.bytes);
@@ -715,7 +720,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
     return launch_kernel(st, kKernelDenseHelpers, f16 ? join_kernel<__half> : join_kernel<__nv_bfloat16>,
                          dim3(unsigned(a.blocks + b.blocks + c.blocks)), 256, 0, stream, a, b, c);
   };
-  const bool narrow = narrow_pays(own_dz, saved != nullptr, gated != 0, rows, K, N, dx, dxs, st->num_sms);
+  const bool narrow = narrow_pays(own_dz, kept, gated != 0, rows, K, N, dx, dxs, st->num_sms);
   const bool dx_parts = dx != nullptr && !narrow && plan.dx_split.parts > 1 && dxs == K;  // (a join writes dense rows)
 
   for (int64_t r0 = 0; r0 < rows; r0 += plan.chunk) {
@@ -737,7 +742,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
         if (dw != nullptr || dbias != nullptr) m.dz = {dst, n, N, zs, outer, zs / 2};
         m.bias = bias, m.activation = activation, m.what = "dense_backward dx";
         rc = run_narrow(m, stream);
-      } else if (saved != nullptr) {
+      } else if (kept) {
         const SlopeParams p{dy_c, static_cast<const float*>(saved) + r0 * ss, dst, dbias != nullptr && !product_sums ? sums : nullptr, dys, ss, zs, n,
                             sum_pitch, N, plan.rows_sum, r0 > 0};
         const dim3 grid{unsigned((N + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
@@ -789,7 +794,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       m.what = "dense_backward dW";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
     }
-    if (dbias != nullptr && !product_sums && saved == nullptr) {
+    if (dbias != nullptr && !product_sums && !kept) {
       const dim3 grid{unsigned((sum_columns + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
       if (f16)
         rc = launch_kernel(st, kKernelDenseHelpers, row_sum_kernel<__half>, grid, 256, 0, stream, static_cast<const __half*>(dz), zs, n,

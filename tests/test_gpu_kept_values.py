@@ -51,3 +51,33 @@ def test_kept_values_beside_results_that_are_stored_in_place(rows, K, N, first, 
         for part in range(2 if gated else 1):
             at = slice(part * padded(N), part * padded(N) + N)
             assert torch.equal(kept_again[:, at], kept[:, at])
+
+
+def backward(dy, x, w, bias, saved, activation, gated, want, held):
+    """The C entry point on a workspace inside `held`, whose rest is looked at by the caller; returns dx, dW, db and its size."""
+    rows, K = x.shape
+    N = dy.shape[1]
+    outer, code = 2 if gated else 1, ops.ACTIVATIONS[activation]
+    need = _lib.load().b200ta_dense_backward_workspace_bytes(code, gated, saved is not None, want[2], rows, K, N)
+    assert need <= held.numel()
+    dx, dw, db = torch.zeros_like(x), torch.zeros_like(w), torch.zeros(outer * N, device=DEV, dtype=x.dtype)
+    dx_p, dw_p, db_p = (t.data_ptr() if on else None for t, on in zip((dx, dw, db), want, strict=True))
+    _lib.call("b200ta_dense_backward", dy.data_ptr(), N, x.data_ptr(), K, w.data_ptr(), K, None if bias is None else bias.data_ptr(),
+              None if saved is None else saved.data_ptr(), 0 if saved is None else saved.stride(0), dx_p, K, dw_p, db_p, held.data_ptr(), need,
+              _lib.DTYPE_BF16, code, gated, rows, K, N, torch.cuda.current_stream().cuda_stream)
+    return dx, dw, db, need
+
+
+@pytest.mark.parametrize("rows,K,N", [(300, 64, 72), (5000, 64, 640), (700, 2048, 2048)])
+@pytest.mark.parametrize("want", [(1, 1, 1), (0, 1, 1), (0, 0, 1), (1, 0, 1)])
+def test_kept_values_of_a_layer_without_an_activation(rows, K, N, want):
+    """Its dz is dy and kept values are not read: with them, on a workspace full of NaN, all gradients are those without."""
+    x, w, dy = randn(rows, K, seed=1), randn(N, K, seed=2, std=K ** -0.5), randn(rows, N, seed=3, std=0.1)
+    saved = randn(rows, N, seed=4, dtype=torch.float32)
+    held = torch.full((1 << 25,), float("nan"), device=DEV).view(torch.uint8)
+    with_saved = backward(dy, x, w, None, saved, "none", False, want, held)[:3]
+    without = backward(dy, x, w, None, None, "none", False, want, held)[:3]
+    for a, b in zip(with_saved, without, strict=True):
+        assert torch.equal(a, b)
+    db = ops.dense_backward(dy, x, w, saved=saved, want_dx=bool(want[0]), want_dweight=bool(want[1]), want_dbias=True)[2]
+    assert torch.equal(db, with_saved[2])
