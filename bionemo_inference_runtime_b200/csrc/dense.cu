@@ -552,10 +552,12 @@ Split split_units(int64_t rows, int64_t units, int64_t outer, int64_t K, int num
   return best;
 }
 constexpr int kChunkRows = 256;  // chunks of the backward pass are multiples of this
-// Rows of a partial sum of db: enough blocks of 256 columns to fill the device a few times, at least 32 rows each.
+// Rows of a partial sum of db: enough blocks of 256 columns to fill the device a few times, 32 to 1024 rows each; more where the
+// second axis of a grid, on which the blocks of rows lie, has no room for so many blocks.
 int sum_rows(int64_t rows, int64_t columns, int num_sms) {
   const int64_t blocks = std::max<int64_t>(4 * num_sms / ((columns + 255) / 256), 1), each = (rows + blocks - 1) / blocks;
-  return int(std::min<int64_t>(std::max<int64_t>((each + 7) / 8 * 8, 32), 1024));
+  const int64_t wanted = std::min<int64_t>(std::max<int64_t>((each + 7) / 8 * 8, 32), 1024), least = (rows + 65534) / 65535;
+  return int(std::max(wanted, (least + 7) / 8 * 8));
 }
 
 // The backward pass: how many rows at a time, and where its intermediates lie in the workspace.
