@@ -113,10 +113,11 @@ Rows operand(const at::Tensor& t, bool few, Copies& copies) {
   return {copy, copy.data_ptr(), r.rows, r.columns, copy.stride(0), 1};
 }
 
-// Where a result goes: contiguous columns, rows with one stride.
+// Where a result goes: contiguous columns, rows with one stride that lie apart.
 Rows result_in(const at::Tensor& out) {
   Rows r = rows_of(out);
   if (r.held.data_ptr() != out.data_ptr() || r.column_stride != 1) refuse("out must have contiguous columns and rows with one stride");
+  if (r.rows > 1 && r.stride < r.columns) refuse("out must not overlap itself");
   return r;
 }
 at::Tensor empty_rows(const at::Tensor& x, int64_t columns) {
