@@ -63,7 +63,7 @@ def _host_made_for() -> str:
 def _host_stale() -> bool:
     """Whether _host.so is missing, older than its sources or made for another PyTorch, interpreter or toolkit."""
     made_for = OBJ_DIR / HOST_MADE_FOR
-    return (_stale(HOST, [*HOST_SOURCES, CSRC / "torch_host.h", PKG.parent / "include" / "b200ta.h"])
+    return (_stale(HOST, [*HOST_SOURCES, CSRC / "torch_host.h", CSRC / "rows_overlap.h", PKG.parent / "include" / "b200ta.h"])
             or not made_for.exists() or made_for.read_text() != _host_made_for())
 
 

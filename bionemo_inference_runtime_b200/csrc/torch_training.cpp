@@ -1,6 +1,7 @@
 // Host path of the trainable layers: layer norm, dense and gated dense layers and their gradients.  Checks the tensors, takes
 // outputs and workspaces from PyTorch's allocator on the tensors' own device and its current stream, and makes aligned copies
 // of what a TMA load cannot address (odd pitches, transposed or broadcast tensors).
+#include "rows_overlap.h"
 #include "torch_host.h"
 
 #include <ATen/cuda/EmptyTensor.h>
@@ -120,6 +121,21 @@ Rows result_in(const at::Tensor& out) {
   if (r.rows > 1 && r.stride < r.columns) refuse("out must not overlap itself");
   return r;
 }
+b200ta_host::RowSpan span_of(const Rows& r, int64_t element) {
+  return {int64_t(reinterpret_cast<uintptr_t>(r.ptr)), r.rows, r.columns * element, r.stride * element};
+}
+// Refuses a result of the caller's that shares memory with what the kernel reads where it lies: other blocks may read it after
+// it has been written.  With `in_place` the very rows that are read may be written, since each element is read by the threads
+// that write it, before they do.
+void require_apart(const Rows& to, const char* name, const Rows& from, const at::Tensor& out, const at::Tensor& read, bool in_place = false) {
+  const bool same = to.ptr == from.ptr && to.rows == from.rows && to.columns == from.columns && (to.rows == 1 || to.stride == from.stride);
+  if (in_place && same && out.scalar_type() == read.scalar_type()) return;
+  if (b200ta_host::overlaps(span_of(to, out.element_size()), span_of(from, read.element_size())))
+    refuse(std::string("out must not overlap ") + name);
+}
+void require_apart(const Rows& to, const char* name, const Maybe& vector, const at::Tensor& out) {
+  if (vector) require_apart(to, name, Rows{*vector, vector->data_ptr(), 1, vector->numel(), 0, 1}, out, *vector);
+}
 at::Tensor empty_rows(const at::Tensor& x, int64_t columns) {
   c10::SmallVector<int64_t, 8> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = columns;
@@ -167,6 +183,11 @@ std::pair<at::Tensor, Maybe> layer_norm(const at::Tensor& x, const Maybe& weight
   const Rows r = plain_rows(x);
   const Rows to = result_in(y);
   const Maybe w = weight ? Maybe(weight->contiguous()) : Maybe(), b = bias ? Maybe(bias->contiguous()) : Maybe();
+  if (out) {
+    require_apart(to, "x", r, y, r.held, true);
+    require_apart(to, "weight", w, y);
+    require_apart(to, "bias", b, y);
+  }
   check(lib.layer_norm(r.ptr, r.stride, pointer(w), pointer(b), params, to.ptr, to.stride, pointer(stats), dtype, rows, width,
                        float(eps), stream()),
         "b200ta_layer_norm");
@@ -237,8 +258,14 @@ std::pair<at::Tensor, Maybe> dense(const at::Tensor& x, const at::Tensor& w, con
   const Rows rx = operand(x, few, copies), rw = operand(w, few, copies), to = result_in(y);
   Rows rr{};
   if (residual) rr = operand(*residual, few, copies);
-  copies.make();
   const Maybe b = bias ? Maybe(bias->contiguous()) : Maybe();
+  if (out) {
+    require_apart(to, "x", rx, y, x);
+    require_apart(to, "weight", rw, y, w);
+    require_apart(to, "bias", b, y);
+    if (residual) require_apart(to, "residual", rr, y, *residual, true);
+  }
+  copies.make();
   check(lib.dense(rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), residual ? rr.ptr : nullptr, rr.stride, to.ptr, to.stride,
                   pointer(saved), pitch, l.dtype, int(activation), gated, l.rows, l.K, l.N, stream()),
         "b200ta_dense");

@@ -507,7 +507,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     """Layer norm over the last axis (1 to 16384 wide) of a bf16, fp16 or fp32 tensor of any leading shape and strides.
 
     ``weight`` and ``bias`` are in the dtype of ``x`` or fp32.  With ``want_stats`` returns ``(y, stats)``, ``stats``
-    being the fp32 ``[rows, 2]`` pairs ``{rstd, -mean * rstd}`` that :func:`layer_norm_backward` takes.
+    being the fp32 ``[rows, 2]`` pairs ``{rstd, -mean * rstd}`` that :func:`layer_norm_backward` takes.  ``out`` may be ``x``
+    itself, and must not share memory with it or the parameters otherwise.
     """
     y, stats = _host.layer_norm(x, weight, bias, float(eps), want_stats, out)
     return (y, stats) if want_stats else y
@@ -526,7 +527,8 @@ def dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = Non
     any sizes and strides; sums in fp32, one rounding at the end.
 
     With ``want_saved`` returns ``(y, saved)`` for :func:`dense_backward`: the values before the activation where a training
-    step is faster with them than by computing them again, otherwise None.
+    step is faster with them than by computing them again, otherwise None.  ``out`` may be ``residual`` itself, and must not
+    share memory with what is read otherwise.
     """
     y, saved = _host.dense(x, weight, bias, residual, _activation(activation), False, want_saved, out)
     return (y, saved) if want_saved else y
@@ -545,8 +547,8 @@ def dense_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias
 def gated_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str = "silu",
                 want_saved: bool = False, out: torch.Tensor | None = None):
     """``value * activation(gate)`` with ``[value | gate] = x @ weight.T + bias`` in one kernel: ``weight [2 * hidden, K]``
-    holds the value rows, then the gate rows (the order of the transitions' ``fused_fc2_fc1``).  Types, sizes and
-    ``want_saved`` as for :func:`dense`."""
+    holds the value rows, then the gate rows (the order of the transitions' ``fused_fc2_fc1``).  Types, sizes,
+    ``want_saved`` and ``out`` as for :func:`dense`."""
     y, saved = _host.dense(x, weight, bias, None, _activation(activation), True, want_saved, out)
     return (y, saved) if want_saved else y
 
