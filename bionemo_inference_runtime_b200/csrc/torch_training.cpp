@@ -151,6 +151,8 @@ at::Tensor or_out(const Maybe& out, const at::Tensor& x, int64_t columns) {
   c10::SmallVector<int64_t, 8> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = columns;
   require_like("out", *out, x, shape);
+  // Written behind PyTorch's back, but not unnoticed: a backward pass that has kept this tensor refuses to use it.
+  if (!out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
   return *out;
 }
 

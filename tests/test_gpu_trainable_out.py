@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+import bionemo_inference_runtime_b200 as b200
 from bionemo_inference_runtime_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
@@ -86,3 +87,19 @@ def test_results_beside_what_is_read_and_in_its_place(rows, width):
     out = torch.as_strided(swapped, (rows, width), (width, 1))  # the memory of x, which is copied first since its columns lie apart
     ops.dense(swapped, w, out=out)
     assert torch.equal(out, want)
+
+
+def test_a_result_over_what_a_backward_pass_needs_is_noticed():
+    """Automatic differentiation goes by a tensor's version: a result that is written to it counts as a change."""
+    w, norm = randn(64, 48, seed=2, std=0.1).requires_grad_(True), randn(48, seed=3)
+    z, square = randn(90, 48, seed=4), randn(48, 48, seed=5, std=0.1)
+    for call in (lambda out: ops.layer_norm(z, norm, out=out), lambda out: ops.dense(z, square, out=out),
+                 lambda out: ops.gated_dense(z, torch.cat([square, square]), out=out)):
+        x = randn(90, 48, seed=1)
+        loss = b200.dense(x, w, activation="silu").float().sum()
+        call(x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        x = torch.empty_like(z)
+        assert torch.equal(ops.layer_norm(z, norm, out=x), ops.layer_norm(z, norm))
