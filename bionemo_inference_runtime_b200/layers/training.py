@@ -40,7 +40,9 @@ class _LayerNorm(torch.autograd.Function):
 class _Dense(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        y, saved = ops.dense(x, weight, bias, activation=activation, residual=residual, want_saved=True)
+        keep = any(ctx.needs_input_grad[:3])  # the gradient of the residual is dy
+        y = ops.dense(x, weight, bias, activation=activation, residual=residual, want_saved=keep)
+        y, saved = y if keep else (y, None)
         ctx.save_for_backward(x, weight, bias, saved)
         ctx.activation = activation
         return y

@@ -54,3 +54,17 @@ def test_forward_mode_is_refused(kernels, name):
                 with torch.set_grad_enabled(on), pytest.raises(NotImplementedError, match="forward-mode"):
                     FUNCTIONS[name](*given)
     assert not FUNCTIONS[name](x, w, b, r).requires_grad
+
+
+def test_nothing_is_kept_for_gradients_that_do_not_need_it(kernels):
+    """The gradient of a residual is dy: where only that is wanted, the values before the activation are not kept."""
+    x, w, b, r = torch.randn(3, 4), torch.randn(6, 4), torch.randn(6), torch.randn(3, 6)
+    y = b200.dense(x, w, b, activation="gelu", residual=r.requires_grad_(True))
+    assert kernels.pop() == {"want_saved": False} and y.requires_grad
+    y.sum().backward()
+    assert torch.equal(r.grad, torch.ones_like(r))
+    for needs in (x, w, b):
+        needs.requires_grad_(True)
+        b200.dense(x, w, b, activation="gelu", residual=r)
+        assert kernels.pop() == {"want_saved": True}
+        needs.requires_grad_(False)
