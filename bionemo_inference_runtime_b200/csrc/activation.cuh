@@ -5,7 +5,8 @@
 // exponent is held below 62, so that the product of two terms stays finite, and what multiplies a sigmoid that small is held
 // above -44: the products are below 2^-56 where the formulas give zero.  NaN stays in its own value (the exponent's bound
 // drops it, the other factor keeps it).  Sums and products are made in packed pairs, which halves their issue slots.
-// Results agree with the formulas to a few units of the last place of 32 bits.
+// Results agree with the formulas to a few units of the last place of 32 bits; gelu's probability p(z) does in absolute terms
+// only (see normal2).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -58,7 +59,9 @@ __device__ __forceinline__ F2 held(float z0, float z1) { return F2(max_nan(z0, -
 // The normal distribution's p(z) = (1 + erf(z / sqrt 2)) / 2 and its density for two values: the rational approximation 7.1.26 of
 // Abramowitz and Stegun's handbook, erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2) with t = 1 / (1 + 0.3275911 x), whose error is below
 // 1.5e-7 (and falls with exp(-x^2)): one exponential, which is the density's, and a reciprocal for the pair.  (With erff() a
-// kernel of 15 million values took 41 us, with this 33.)  A NaN gives some number; z times it is NaN.
+// kernel of 15 million values took 41 us, with this 33.)  For p that is 7.5e-8 beside its roundings.  Below zero, where p itself
+// becomes small, its relative error grows: 3e-6 at z = -2, 6e-5 at -3, 5e-4 at -4 (where 1 + erf in 32 bits has 6e-4), 4e-3 at -6
+// (where that has lost every bit); half a spacing of fp16 is 5e-4, of bf16 4e-3.  A NaN gives some number; z times it is NaN.
 __device__ __forceinline__ void normal2(float z0, float z1, F2& p, F2& density) {
   constexpr float kP = 0.3275911f * 0.70710678118654752f, kHalfLog2e = 0.72134752044448170f, kDensity = 0.39894228040143268f;
   // a factor 1 / 2 is part of the coefficients
