@@ -5,6 +5,8 @@ import torch
 
 from bionemo_inference_runtime_b200 import _lib, ops
 
+from .test_gpu_trainable import half_spacing, layer_formula, layer_inputs, within
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 SUM = 2.0 ** -18  # of the sum of the absolute terms: sums of up to a few thousand terms in 32 bits
@@ -81,3 +83,60 @@ def test_kept_values_of_a_layer_without_an_activation(rows, K, N, want):
         assert torch.equal(a, b)
     db = ops.dense_backward(dy, x, w, saved=saved, want_dx=bool(want[0]), want_dweight=bool(want[1]), want_dbias=True)[2]
     assert torch.equal(db, with_saved[2])
+
+
+def forward_kept(x, w, bias, activation, gated):
+    """The pre-activations by the C entry point, which gives them for any width."""
+    rows, K = x.shape
+    outer = 2 if gated else 1
+    N = w.shape[0] // outer
+    y = torch.empty(rows, N, device=DEV, dtype=x.dtype)
+    saved = torch.full((rows, outer * padded(N)), float("nan"), device=DEV)
+    _lib.call("b200ta_dense", x.data_ptr(), K, w.data_ptr(), K, bias.data_ptr(), None, 0, y.data_ptr(), N, saved.data_ptr(), saved.shape[1],
+              _lib.DTYPE_BF16, ops.ACTIVATIONS[activation], gated, rows, K, N, torch.cuda.current_stream().cuda_stream)
+    return saved
+
+
+def check_gradients(got, want, x, w, bias, dy, activation, gated):
+    """dx, dW and db (those that were wanted) against the formulas in 64 bits: dz is rounded between the kernels."""
+    u, tiny = half_spacing(x.dtype), torch.finfo(x.dtype).smallest_normal
+    _, _, dz, sums = layer_formula(x, w, bias, None, activation, gated, dy)
+    off = SUM * sums + 1.01 * u * dz.abs() + tiny
+    xd, wd = x.double(), w.double()
+    for k, (name, exact, bound) in enumerate((("dx", lambda: dz @ wd, lambda: off @ wd.abs() + SUM * (dz.abs() @ wd.abs())),
+                                              ("dW", lambda: dz.t() @ xd, lambda: off.t() @ xd.abs() + SUM * (dz.abs().t() @ xd.abs())),
+                                              ("db", lambda: dz.sum(0), lambda: off.sum(0) + SUM * dz.abs().sum(0)))):
+        if want[k]:
+            result = exact()
+            within(got[k], result, 1.01 * u * result.abs() + bound() + tiny, name)
+
+
+CHOICES = [(1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (1, 0, 1), (0, 1, 1)]
+
+
+@pytest.mark.parametrize("rows,K,N,gated", [(1000, 104, 1000, True), (3000, 64, 640, False), (300, 1600, 264, True), (2047, 520, 1288, False)])
+def test_the_workspace_of_kept_values_is_enough_for_every_choice_of_gradients(rows, K, N, gated):
+    """Kept values give db on the way, a row of sums for each block of rows: nothing lies behind the workspace for any choice."""
+    given = layer_inputs(rows, K, N, torch.bfloat16, gated, True, False)
+    x, w, bias, dy = given["x"], given["w"], given["bias"], given["dy"]
+    saved = forward_kept(x, w, bias, "gelu", gated)
+    held = torch.empty(256 << 20, device=DEV, dtype=torch.uint8)
+    for want in CHOICES:
+        held.fill_(0xFF)  # (as numbers: NaN)
+        *got, need = backward(dy, x, w, bias, saved, "gelu", gated, want, held)
+        assert (held[need:] == 0xFF).all(), want
+        for t, on in zip(got, want, strict=True):
+            assert on or not t.any(), want
+        check_gradients(got, want, x, w, bias, dy, "gelu", gated)
+
+
+@pytest.mark.parametrize("rows,K,N,gated,want", [(250001, 64, 1024, True, (1, 1, 1)), (250001, 64, 1024, True, (0, 0, 1)),
+                                                 (300001, 24, 1000, False, (0, 1, 1))])
+def test_kept_values_in_chunks(rows, K, N, gated, want):
+    """More than half a gigabyte of dz: the backward pass takes the rows in several chunks, the last one a shorter one."""
+    given = layer_inputs(rows, K, N, torch.bfloat16, gated, True, False)
+    x, w, bias, dy = given["x"], given["w"], given["bias"], given["dy"]
+    saved = forward_kept(x, w, bias, "silu", gated)
+    held = torch.full((1 << 28,), float("nan"), device=DEV).view(torch.uint8)
+    *got, _ = backward(dy, x, w, bias, saved, "silu", gated, want, held)
+    check_gradients(got, want, x, w, bias, dy, "silu", gated)
