@@ -371,7 +371,8 @@ auto pick_slope(int activation) {
 
 // ---- sums over rows -------------------------------------------------------------------------------------------------
 //
-// part[block.y][n] (+)= sum over a block's rows of dz[., n].  32 lanes of eight columns, eight rows at a time, eight loads of a
+// part[block.y][n] (+)= sum over a block's rows of dz[., n], in 32 bits, of the values as they were rounded for dx and dW: the
+// roundings of many rows add up to about that of the result.  32 lanes of eight columns, eight rows at a time, eight loads of a
 // thread on their way: dz of 5003 rows and 6144 columns takes 14 us (61 MB).  (Blocks of half the rows with four loads: two waves
 // of them, 19 us.)
 template <typename T>

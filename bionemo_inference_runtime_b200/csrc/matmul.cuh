@@ -140,6 +140,9 @@ __host__ __device__ constexpr uint32_t idesc(bool f16, int m, int n, bool a_mn, 
 
 // y / dz of kN of a group's 32 columns, from column kFirst, of one row, as 16-bit pairs.  v: accumulators (kGated*: of the
 // values), g: of the gates, aux: residual (with has_aux) or dy; kGatedGrad: y the gradients of the values, yg those of the gates.
+// dz is formed in 32 bits and rounded once to the operands' type, since the products behind it take 16 bits: dx and dW are off by
+// two roundings instead of one (root mean square, bf16: 0.0023 of their size where a single rounding has 0.0017; fp16: 0.00029 and
+// 0.00021).  As a sum of two 16-bit numbers it would cost both products twice, and its way through memory.
 template <typename T, MatmulForm kForm, int kAct, int kFirst, int kN>
 __device__ __forceinline__ void finish(const float (&v)[kN], const float (&g)[kN], bool has_aux, const uint32_t (&aux)[16],
                                        uint32_t (&y)[16], uint32_t (&yg)[16]) {

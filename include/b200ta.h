@@ -447,9 +447,9 @@ int b200ta_dense(const void* x, int64_t x_row_stride, const void* w, int64_t w_r
 int b200ta_dense_keeps(int activation, int gated, int K);
 
 /* Gradients of the same: dx [rows, K], dw [N or 2 N, K] and dbias [N or 2 N], both dense; each may be NULL.  The
- * pre-activations are taken from `saved`, or computed again from x, w and bias if it is NULL.  Alignment of what is
- * read as above, results free; the workspace is 256-byte aligned; its
- * size depends on whether `saved` and `dbias` are given. */
+ * pre-activations are taken from `saved`, or computed again from x, w and bias if it is NULL (a layer that is not gated and has no
+ * activation needs none).  They give dz, which is rounded to `dtype` for the products behind it.  Alignment of what is read as
+ * above, results free; the workspace is 256-byte aligned; its size depends on whether `saved` and `dbias` are given. */
 size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, int64_t rows, int K, int N);
 int b200ta_dense_backward(const void* dy, int64_t dy_row_stride, const void* x, int64_t x_row_stride, const void* w,
                           int64_t w_row_stride, const void* bias, const void* saved, int64_t saved_row_stride, void* dx,
