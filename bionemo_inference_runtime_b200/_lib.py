@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p, POINTER
+from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p, POINTER
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -145,6 +145,10 @@ SIGNATURES: dict[str, tuple] = {
          c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int64, c_int, c_int, c_void_p],
     ),
     "b200ta_copy_rows": (c_int, [c_void_p, c_int, c_void_p]),
+    "b200ta_dropout": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_uint64, c_uint64, c_void_p, c_void_p],
+    ),
 }
 
 

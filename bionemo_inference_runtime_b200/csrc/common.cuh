@@ -44,13 +44,15 @@ struct DeviceState {
   int device = -1;
   int num_sms = 0;
   int* status_dev = nullptr;  // device word kernels write when they abandon a bounded wait
-  std::atomic<uint64_t> configured{0};  // bit per KernelId: its shared-memory limit has been raised on this device
+  std::atomic<uint64_t> configured[2] = {{0}, {0}};  // bit per KernelId: its shared-memory limit has been raised on this device
 };
 enum KernelId {
   kKernelPrologue, kKernelEpilogue, kKernelAttention, kKernelAttentionMasked, kKernelTransition, kKernelTransitionRelu,
   kKernelProject, kKernelContract, kKernelOutput, kKernelOutputF32, kKernelLinear, kKernelPairBias, kKernelRowStats,
   kKernelMaskRows, kKernelNorm, kKernelDenseHelpers, kKernelNarrow,
-  kKernelMatmul = kKernelNarrow + 4  // and one for each of the matmul kernels after it
+  kKernelMatmul = kKernelNarrow + 4,  // and one for each of the matmul kernels after it
+  kKernelDropout = 60, kKernelAdapter,
+  kKernelMatmulAdapters = 64  // and one for each of the matmul kernels with adapters after it
 };
 int get_device_state(DeviceState** out);
 
@@ -62,10 +64,11 @@ int get_device_state(DeviceState** out);
 template <typename... P, typename... A>
 int launch_clusters(DeviceState* st, KernelId id, void (*kernel)(P...), dim3 grid, unsigned cluster, int threads, int smem_bytes,
                     void* stream, A&&... args) {
-  const uint64_t bit = 1ull << id;
-  if (smem_bytes > 48 * 1024 && !(st->configured.load(std::memory_order_relaxed) & bit)) {
+  const uint64_t bit = 1ull << (id & 63);
+  std::atomic<uint64_t>& configured = st->configured[id >> 6];
+  if (smem_bytes > 48 * 1024 && !(configured.load(std::memory_order_relaxed) & bit)) {
     B200TA_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
-    st->configured.fetch_or(bit, std::memory_order_relaxed);
+    configured.fetch_or(bit, std::memory_order_relaxed);
   }
   cudaLaunchAttribute attrs[2];
   attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

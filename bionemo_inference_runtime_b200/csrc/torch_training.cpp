@@ -21,7 +21,7 @@ struct Library {
 #define B200TA_ENTRY(name) decltype(&b200ta_##name) name = nullptr;
 #define B200TA_ENTRIES(X)                                                                                                \
   X(layer_norm) X(layer_norm_workspace_bytes) X(layer_norm_backward) X(dense_few_rows) X(dense_keeps) X(dense)              \
-  X(dense_backward_workspace_bytes) X(dense_backward) X(copy_rows)
+  X(dense_backward_workspace_bytes) X(dense_backward) X(copy_rows) X(dropout)
   B200TA_ENTRIES(B200TA_ENTRY)
 #undef B200TA_ENTRY
 } lib;
@@ -308,6 +308,36 @@ std::tuple<Maybe, Maybe, Maybe> dense_backward(const at::Tensor& dy, const at::T
   return {dx, dweight, dbias};
 }
 
+// ---- dropout ----------------------------------------------------------------------------------------------------------
+
+at::Tensor dropout(const at::Tensor& x, int64_t dropped, uint64_t seed, uint64_t sequence, const Maybe& seed_at, const Maybe& residual,
+                   int64_t shared, const Maybe& out) {
+  const int dtype = dtype_code("x", x, true);
+  if (x.dim() < 1) refuse("dropout: x must have an axis at least");
+  if (shared < -1 || shared >= x.dim()) refuse("shared must be an axis of x " + shape_of(x) + " or None");
+  if (residual) require_like("residual", *residual, x, x.sizes());
+  if (seed_at && (seed_at->device() != x.device() || seed_at->scalar_type() != at::kLong || seed_at->numel() != 1))
+    refuse("a seed that is a tensor must be one int64 on the device of x");
+  if (out && !out->is_contiguous()) refuse("out must be contiguous");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const at::Tensor y = or_out(out, x, x.size(-1));
+  if (x.numel() == 0) return y;
+  const at::Tensor from = x.contiguous();
+  const Maybe added = residual ? Maybe(residual->contiguous()) : Maybe();
+  auto whole = [](const at::Tensor& t) { return Rows{t, t.data_ptr(), 1, t.numel(), 0, 1}; };
+  if (out) {
+    require_apart(whole(y), "x", whole(from), y, from, true);
+    if (added) require_apart(whole(y), "residual", whole(*added), y, *added, true);
+    if (seed_at) require_apart(whole(y), "seed", whole(*seed_at), y, *seed_at);
+  }
+  int64_t outer = 1, axis = 1, inner = 1;
+  for (int64_t d = 0; d < x.dim(); ++d) (d < shared ? outer : d == shared ? axis : inner) *= x.size(d);
+  check(lib.dropout(from.data_ptr(), pointer(added), y.data_ptr(), dtype, outer, axis, inner, int(dropped), seed, sequence,
+                    seed_at ? static_cast<const uint64_t*>(seed_at->data_ptr()) : nullptr, stream()),
+        "b200ta_dropout");
+  return y;
+}
+
 }  // namespace
 
 namespace b200ta_host {
@@ -325,6 +355,7 @@ void define_training(py::module_& m) {
   m.def("layer_norm_backward", &layer_norm_backward);
   m.def("dense", &dense);
   m.def("dense_backward", &dense_backward);
+  m.def("dropout", &dropout);
 }
 
 }  // namespace b200ta_host

@@ -77,6 +77,22 @@ class _GatedDense(torch.autograd.Function):
         return (*grads, None)
 
 
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, sequence, shared):
+        if isinstance(seed, torch.Tensor):
+            seed = seed.clone()  # a later step's seed may be written to the tensor before this step's backward pass
+        ctx.given = (p, seed, sequence)
+        ctx.shared = shared
+        return ops.dropout(x, p, seed, sequence, residual=residual, shared=shared)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        dx = ops.dropout_backward(dy, *ctx.given, shared=ctx.shared) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
+
+
 def _needs_grad(*tensors: torch.Tensor | None) -> bool:
     # A tensor with a tangent need not require a gradient: its result would silently have no tangent.  (Outside of a level there
     # are none; asking each tensor costs 0.4 us.)
@@ -107,6 +123,14 @@ def gated_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     if _needs_grad(x, weight, bias):
         return _GatedDense.apply(x, weight, bias, activation)
     return ops.gated_dense(x, weight, bias, activation=activation)
+
+
+def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, sequence: int = 0, *, residual: torch.Tensor | None = None,
+            shared: int | None = None) -> torch.Tensor:
+    """Differentiable :func:`ops.dropout <bionemo_inference_runtime_b200.ops.dropout>`: ``residual + keep * x / (1 - p)``."""
+    if _needs_grad(x, residual):
+        return _Dropout.apply(x, residual, p, seed, sequence, shared)
+    return ops.dropout(x, p, seed, sequence, residual=residual, shared=shared)
 
 
 class _Weight(nn.Module):

@@ -560,3 +560,36 @@ def gated_dense_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor
     """``(dx, dweight, dbias)`` of :func:`gated_dense`; see :func:`dense_backward`."""
     return _host.dense_backward(dy, x, weight, bias, saved, _activation(activation), True, want_dx, want_dweight,
                                            bias is not None if want_dbias is None else want_dbias)
+
+
+_WORD = (1 << 64) - 1
+
+
+def _dropout(x, p, seed, sequence, residual, shared, out):
+    if not 0 <= p <= 1:  # (NaN is neither)
+        raise ValueError(f"p must lie between 0 and 1, got {p}")
+    at = seed if isinstance(seed, torch.Tensor) else None
+    if shared is not None and not -x.dim() <= shared < x.dim():
+        raise ValueError(f"shared must be an axis of x {tuple(x.shape)} or None, got {shared}")
+    axis = -1 if shared is None else shared % x.dim()
+    return _host.dropout(x, round(p * 65536), 0 if at is not None else seed & _WORD, sequence & _WORD, at, residual, axis, out)
+
+
+def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, sequence: int = 0, *, residual: torch.Tensor | None = None,
+            shared: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``residual + keep * x / (1 - p)`` in one pass, for bf16, fp16 or fp32 of any shape.  ``keep`` is never stored: it is a function
+    of ``seed``, ``sequence`` and the element's number (Philox 4x32-10, 16 bits an element: ``p`` counts in steps of 2^-16), so
+    that :func:`dropout_backward` makes it again.
+
+    All entries along the axis ``shared`` have one draw (dropout of whole columns or rows of a pair tensor).  ``sequence`` tells the
+    layers of a step apart that have one ``seed``.  ``seed`` may be an int64 tensor of one element on the device, which is read when the
+    kernel runs: a captured graph then draws anew at each replay.  A dropped element is left out, whatever it is.  ``out`` may be ``x``
+    or ``residual`` themselves, and must not share memory with them otherwise.  (Tensors that are not contiguous are copied.)
+    """
+    return _dropout(x, p, seed, sequence, residual, shared, out)
+
+
+def dropout_backward(dy: torch.Tensor, p: float, seed: int | torch.Tensor, sequence: int = 0, *, shared: int | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of :func:`dropout` for ``x``: ``keep * dy / (1 - p)``.  That of its residual is ``dy``."""
+    return _dropout(dy, p, seed, sequence, None, shared, out)

@@ -469,6 +469,14 @@ typedef struct {
 } b200ta_copy;
 int b200ta_copy_rows(const b200ta_copy* jobs, int count, void* stream);
 
+/* y = residual + keep * x / (1 - p), p = dropped / 65536 (0 to 65536), for dense tensors of `dtype` that are seen as [outer, axis,
+ * inner]; residual may be NULL, y may be x or residual.  Element (o, a, i) has the number m = o * inner + i: the entries of `axis` share
+ * their draw (axis 1: none do).  It stays if the 16 bits u(m) >= dropped, where u(m) is half m % 2 (0: the low one) of word
+ * m % 8 / 2 of Philox 4x32-10 with the key `seed` and the counter {m / 8, sequence}, low words first.  The same call on dy without a
+ * residual is the gradient of x.  With `seed_at` (may be NULL) the seed is read from the device when the kernel runs. */
+int b200ta_dropout(const void* x, const void* residual, void* y, int dtype, int64_t outer, int64_t axis, int64_t inner, int dropped,
+                   uint64_t seed, uint64_t sequence, const uint64_t* seed_at, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
