@@ -1,0 +1,457 @@
+// The kernels of low-rank adapters beside the tensor-core products: low-rank values, their weights' gradients, small layouts.
+#include <algorithm>
+
+#include "adapters.cuh"
+#include "layer_norm.cuh"
+#include "warp_matmul.cuh"
+
+namespace b200ta {
+namespace {
+
+// Eight elements of a row of K from k on, zeros behind it.
+template <typename T, bool kVec>
+__device__ __forceinline__ uint4 load_eight_of(const T* row, int k, int K) {
+  const uint4 v = kVec ? norm::load_if(k < K, row + k) : norm::load_anywhere(row + k, row, K);
+  return K - k >= 8 ? v : norm::first<T>(v, K - k);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_low(const LowProduct& p, long long row, int r, float v) {
+  T* low = static_cast<T*>(p.low) + row * (2 * padded_rank(p.rank)) + r;
+  const T rounded = static_cast<T>(v);
+  *low = rounded;
+  low[padded_rank(p.rank)] = static_cast<T>(v - static_cast<float>(rounded));
+}
+
+// ---- low-rank values, a warp for each ------------------------------------------------------------------------------
+//
+// Few rows, or rows of many different adapters: a warp multiplies a row of x with one row of its adapter, 16 bytes a lane at a time.
+// Bound by latency, then by the adapters' way from L2 (each row reads its own).
+constexpr int kDotWarps = 8;
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kDotWarps * 32)
+low_dot_kernel(const LowProduct p, int groups) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, r = int(blockIdx.x % unsigned(groups)) * kDotWarps + (threadIdx.x >> 5);
+  const long long row = blockIdx.x / unsigned(groups);
+  if (r >= padded_rank(p.rank)) return;
+  const int g = adapter_of(p.index, uint32_t(row));
+  float sum = 0.f;
+  if (g != kNoAdapter && r < p.rank) {
+    for (int plane = 0; plane < p.planes; ++plane) {
+      const T* x = static_cast<const T*>(p.x) + row * p.xs + plane * p.x_plane;
+      const T* a = static_cast<const T*>(p.a) + ((long long)g * p.rank + r) * p.as + plane * p.a_plane;
+      float2 s = make_float2(0.f, 0.f);
+#pragma unroll 4
+      for (int k = lane * 8; k < p.K; k += 256) {
+        const uint4 u = load_eight_of<T, kVec>(x, k, p.K), v = load_eight_of<T, kVec>(a, k, p.K);
+        const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 c = unpack2<T>(uw[j]), d = unpack2<T>(vw[j]);
+          s.x = fmaf(c.x, d.x, s.x), s.y = fmaf(c.y, d.y, s.y);
+        }
+      }
+      sum += s.x + s.y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    sum *= p.scale != nullptr ? __ldg(p.scale + g) : p.scale_all;
+  }
+  if (lane == 0) store_low<T>(p, row, r, sum);
+}
+
+// ---- low-rank values by warp-wide products ---------------------------------------------------------------------------
+//
+// A warp takes 32 rows and kTiles * 8 ranks: products m16n8k16 with x as the left and the adapter's rows as the right operand, both read
+// as they lie: a lane reads 16 bytes of each of its rows, eight neighbouring k, that serve as the pairs of two products (the order of
+// k is the same in both operands and does not matter).  The warps of a block share the rows and take 32 of k in turn, or, where
+// there are many rows and few k, take rows of their own.  Rows of other adapters than the first are taken in further
+// passes; a pass stores the rows that are its own.  Bound by HBM (x once) or L2.
+constexpr int kLowRows = 32;
+__host__ __device__ constexpr int low_warps(int tiles) { return tiles == 8 ? 4 : 8; }
+template <typename T, int kTiles, bool kVec>
+__global__ void __launch_bounds__(low_warps(kTiles) * 32)
+low_product_kernel(const LowProduct p, int share) {
+  constexpr int kWarps = low_warps(kTiles), kRanks = kTiles * 8;
+  __shared__ float joined[kWarps][kLowRows][kRanks + 1];
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, t = lane & 3;
+  const long long row0 = ((long long)blockIdx.x * (share ? 1 : kWarps) + (share ? 0 : warp)) * kLowRows;
+  const int r0 = blockIdx.y * kRanks, first = share ? warp * 32 : 0, step = share ? kWarps * 32 : 32;
+  if (row0 >= p.rows) return;  // (of a block whose warps share rows: all of them)
+  TileAdapters<1> mine;
+  mine.load(p.index, row0, p.rows);
+  auto store = [&](int row, int r, float v) {  // a value of this warp's rows
+    if (r < padded_rank(p.rank)) store_low<T>(p, row0 + row, r, r < p.rank ? v : 0.f);
+  };
+  // rows without an adapter
+  for (int row = share ? warp : 0; row < kLowRows && row0 + row < p.rows; row += share ? kWarps : 1)
+    if (__shfl_sync(0xffffffffu, mine.g[0], row) == kNoAdapter)
+      for (int r = lane; r < kRanks; r += 32) store(row, r0 + r, 0.f);
+  for (int g = mine.next(-1); g != kNoAdapter; g = mine.next(g)) {
+    const uint32_t own = mine.rows_of(0, g);
+    const float scale = p.scale != nullptr ? __ldg(p.scale + g) : p.scale_all;
+    float acc[2][kTiles][4] = {};
+    for (int plane = 0; plane < p.planes; ++plane) {
+      const T *x[2][2], *a[kTiles];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long row = row0 + i * 8 + q;
+        x[i >> 1][i & 1] = static_cast<const T*>(p.x) + (row < p.rows ? row : p.rows - 1) * p.xs + plane * p.x_plane;
+      }
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+        const int r = r0 + j * 8 + q;
+        a[j] = static_cast<const T*>(p.a) + ((long long)g * p.rank + (r < p.rank ? r : p.rank - 1)) * p.as + plane * p.a_plane;
+      }
+#pragma unroll 2
+      for (int k = first + t * 8; k - t * 8 < p.K; k += step) {
+        uint4 u[2][2], v[kTiles];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i >> 1][i & 1] = load_eight_of<T, kVec>(x[i >> 1][i & 1], k, p.K);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) v[j] = load_eight_of<T, kVec>(a[j], k, p.K);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mma16816<T>(acc[i][j], u[i][0].x, u[i][1].x, u[i][0].y, u[i][1].y, v[j].x, v[j].y);
+            mma16816<T>(acc[i][j], u[i][0].z, u[i][1].z, u[i][0].w, u[i][1].w, v[j].z, v[j].w);
+          }
+      }
+    }
+    if (share) {
+      __syncthreads();  // (all warps have the same rows, and so the same passes)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) joined[warp][i * 16 + q + 8 * (e >> 1)][j * 8 + t * 2 + (e & 1)] = acc[i][j][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < kLowRows * kRanks; i += kWarps * 32) {
+        const int row = i / kRanks, r = i % kRanks;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) sum += joined[w][row][r];
+        if (own >> row & 1u) store(row, r0 + r, sum * scale);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = i * 16 + q + 8 * h, r = r0 + j * 8 + t * 2;
+            if (!(own >> row & 1u) || r >= padded_rank(p.rank)) continue;  // (padded to a multiple of eight)
+            const float v0 = r < p.rank ? acc[i][j][2 * h] * scale : 0.f, v1 = r + 1 < p.rank ? acc[i][j][2 * h + 1] * scale : 0.f;
+            T* to = static_cast<T*>(p.low) + (row0 + row) * (2 * padded_rank(p.rank)) + r;
+            const uint32_t rounded = pack2<T>(v0, v1);
+            const float2 f = unpack2<T>(rounded);
+            *reinterpret_cast<uint32_t*>(to) = rounded;
+            *reinterpret_cast<uint32_t*>(to + padded_rank(p.rank)) = pack2<T>(v0 - f.x, v1 - f.y);
+          }
+    }
+  }
+}
+
+template <typename T, bool kVec>
+int launch_low(DeviceState* st, const LowProduct& m, void* stream) {
+  // A pass over the rows' k for each adapter among 32 rows, or each row's own adapter read for it alone.
+  const bool own_warps = m.rows <= 16 || (m.index.index != nullptr && m.index.count > 1 && m.index.rows_per_index < 8 && m.rows <= 4096);
+  if (own_warps) {
+    const int groups = int((padded_rank(m.rank) + kDotWarps - 1) / kDotWarps);
+    return launch_kernel(st, kKernelAdapter, low_dot_kernel<T, kVec>, dim3(unsigned(m.rows * groups)), kDotWarps * 32, 0, stream, m, groups);
+  }
+  const int tiles = m.rank <= 16 ? 2 : m.rank <= 32 ? 4 : 8, warps = low_warps(tiles);
+  const int64_t groups = (m.rows + kLowRows - 1) / kLowRows;
+  const int share = groups < int64_t(st->num_sms) * warps * 2 || m.K > 512;
+  const dim3 grid{unsigned(share ? groups : (groups + warps - 1) / warps), unsigned((m.rank + tiles * 8 - 1) / (tiles * 8))};
+  auto* kernel = tiles == 2 ? low_product_kernel<T, 2, kVec> : tiles == 4 ? low_product_kernel<T, 4, kVec> : low_product_kernel<T, 8, kVec>;
+  return launch_kernel(st, kKernelAdapter, kernel, grid, warps * 32, 0, stream, m, share);
+}
+
+// ---- up matrices with their columns contiguous -----------------------------------------------------------------------
+
+struct TransposeParams {
+  const uint16_t* up;
+  uint16_t* out;
+  long long up_pitch, out_pitch;
+  int rank, N, planes;
+};
+__global__ void __launch_bounds__(256)
+transpose_up_kernel(const TransposeParams p) {
+  __shared__ uint16_t tile[32][34];
+  pdl_trigger();
+  pdl_wait();
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, n0 = blockIdx.x * 32, r0 = blockIdx.y * 32;
+  const long long g = blockIdx.z / p.planes, plane = blockIdx.z % p.planes;
+  const uint16_t* up = p.up + (g * p.planes + plane) * p.N * p.up_pitch;
+  uint16_t* out = p.out + (g * p.rank * p.planes + plane) * p.out_pitch;
+  for (int i = y; i < 32; i += 8)
+    if (n0 + i < p.N && r0 + x < p.rank) tile[i][x] = up[(n0 + i) * p.up_pitch + r0 + x];
+  __syncthreads();
+  for (int i = y; i < 32; i += 8)
+    if (r0 + i < p.rank && n0 + x < p.N) out[(long long)(r0 + i) * p.planes * p.out_pitch + n0 + x] = tile[x][i];
+}
+
+// ---- gradients of the adapters' weights ---------------------------------------------------------------------------------
+//
+// dD_g = sum over the rows of g of dt^T x, dU_g likewise of t and dz: bound by HBM or L2 (x and dz once; two operations a byte and rank
+// are nothing beside it).  A block takes 128 columns, one adapter, up to 64 ranks and a part of the rows, 64 at a time through a ring of
+// stages that cp.async fills: rows of other adapters, and what is behind the last column, are filled with zeros on the way, so
+// nothing of them is read.  Products m16n8k16 with ranks as rows and the tensor's rows along k: both operands lie with k across
+// and are transposed on their way from shared memory.  Of several adapters a block first lists the groups of 64 rows that hold
+// its own.  Parts are written in 32 bits and joined in a fixed order: results repeat bit by bit.
+constexpr int kGradRows = 64, kGradColumns = 128, kGradChunks = 1024;
+// (a block of up to 16, 32 or 64 ranks has its two terms beside each other in a row of 64, 128 or 256 bytes)
+constexpr int kGradV = kGradRows * kGradColumns * 2;
+__host__ __device__ constexpr int grad_stage(int tiles) { return kGradV + kGradRows * tiles * 64; }
+__host__ __device__ constexpr int grad_stages(int tiles) { return tiles == 4 ? 3 : 4; }
+
+struct GradParams {
+  LowGrad job[2];
+  AdapterIndex index;
+  long long rows;
+  int rank, rank_groups, slabs0, chunks_part, accumulate;
+};
+__device__ __forceinline__ void copy_or_zero(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename T, int kTiles>  // tiles of 16 ranks
+__global__ void __launch_bounds__(256, 2)
+low_grad_kernel(const GradParams p) {
+  constexpr int kStages = grad_stages(kTiles), kStage = grad_stage(kTiles), kTermVecs = kTiles * 2, kRowVecs = 2 * kTermVecs;
+  extern __shared__ __align__(128) uint8_t stages[];
+  __shared__ uint32_t masks[kGradChunks][2];
+  __shared__ uint16_t list[kGradChunks];
+  __shared__ int listed;
+  pdl_trigger();
+  pdl_wait();
+  const bool second = int(blockIdx.y) >= p.slabs0;
+  const LowGrad& job = second ? p.job[1] : p.job[0];
+  const int slab = int(blockIdx.y) - (second ? p.slabs0 : 0), slabs_plane = (job.columns + kGradColumns - 1) / kGradColumns;
+  const int plane = slab / slabs_plane, c0 = (slab - plane * slabs_plane) * kGradColumns;
+  const int g = blockIdx.z / p.rank_groups, r0 = int(blockIdx.z % unsigned(p.rank_groups)) * 64;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long first_row = (long long)blockIdx.x * p.chunks_part * kGradRows;
+  const long long rows = p.rows - first_row < (long long)p.chunks_part * kGradRows ? p.rows - first_row : (long long)p.chunks_part * kGradRows;
+  const int chunks = rows > 0 ? int((rows + kGradRows - 1) / kGradRows) : 0;
+
+  for (int c = warp; c < chunks; c += 8) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long row = c * kGradRows + h * 32 + lane;
+      const uint32_t own = __ballot_sync(0xffffffffu, row < rows && adapter_of(p.index, uint32_t(first_row + row)) == g);
+      if (lane == 0) masks[c][h] = own;
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int n = 0;
+    for (int c = 0; c < chunks; c += 32) {
+      const bool in = c + lane < chunks && (masks[c + lane < chunks ? c + lane : 0][0] | masks[c + lane < chunks ? c + lane : 0][1]) != 0;
+      const uint32_t vote = __ballot_sync(0xffffffffu, in);
+      if (in) list[n + __popc(vote & ((1u << lane) - 1u))] = uint16_t(c + lane);
+      n += __popc(vote);
+    }
+    if (lane == 0) listed = n;
+  }
+  __syncthreads();
+  const int count = listed;
+
+  const T* v = static_cast<const T*>(job.v) + plane * job.v_plane + c0;
+  const T* t = static_cast<const T*>(job.t) + r0;
+  const uint32_t base = smem_u32(stages);
+  const int v_column = (threadIdx.x & 15) * 8, v_bytes = max(0, min(16, (job.columns - c0 - v_column) * 2));
+  // vector threadIdx.x % kRowVecs of a row of t: first the first terms, then the second ones
+  const int t_vec = threadIdx.x % kRowVecs, t_column = t_vec % kTermVecs * 8;
+  const bool t_in = r0 + t_column < p.rank;  // (its padding to eight ranks is zeros)
+  const int t_from = t_column + (t_vec >= kTermVecs ? padded_rank(p.rank) : 0);
+  // (rows of 64 bytes: two of them to the 128 that the banks span)
+  auto t_at = [&](int row, int vec) { return kGradV + row * kRowVecs * 16 + ((kTiles == 1 ? vec ^ (row >> 1 & 3) : vec ^ (row & 7)) << 4); };
+  auto issue = [&](int i) {
+    if (i < count) {
+      const int c = list[i];
+      const uint32_t stage = base + (i % kStages) * kStage;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = (threadIdx.x >> 4) + 16 * j;
+        const bool own = masks[c][row >> 5] >> (row & 31) & 1u;
+        const int bytes = own ? v_bytes : 0;
+        const T* from = bytes > 0 ? v + (first_row + c * kGradRows + row) * job.v_pitch + v_column : static_cast<const T*>(job.v);
+        copy_or_zero(stage + row * 256 + (((threadIdx.x & 15) ^ (row & 7)) << 4), from, bytes);
+      }
+#pragma unroll
+      for (int row = threadIdx.x / kRowVecs; row < kGradRows; row += 256 / kRowVecs) {
+        const bool own = t_in && (masks[c][row >> 5] >> (row & 31) & 1u);
+        const T* from = own ? t + (first_row + c * kGradRows + row) * (2 * padded_rank(p.rank)) + t_from : static_cast<const T*>(job.t);
+        copy_or_zero(stage + t_at(row, t_vec), from, own ? 16 : 0);
+      }
+    }
+    norm::copy_commit();
+  };
+  float acc[kTiles][2][4] = {};
+  for (int i = 0; i < kStages - 1; ++i) issue(i);
+  for (int i = 0; i < count; ++i) {
+    norm::copy_wait<kStages - 2>();
+    __syncthreads();  // this group has arrived, and all warps are done with the one before, whose stage is filled again
+    issue(i + kStages - 1);
+    const uint32_t stage = base + (i % kStages) * kStage;
+#pragma unroll
+    for (int k = 0; k < kGradRows; k += 16) {
+      const int vr = k + (lane & 15), vc = warp * 2 + (lane >> 4);
+      uint32_t b[4];
+      ldmatrix4_t(stage + vr * 256 + ((vc ^ (vr & 7)) << 4), b);
+#pragma unroll
+      for (int m = 0; m < 2 * kTiles; ++m) {
+        const int tr = k + (lane >> 4) * 8 + (lane & 7);
+        uint32_t a[4];
+        ldmatrix4_t(stage + t_at(tr, m * 2 + (lane >> 3 & 1)), a);
+        mma16816<T>(acc[m % kTiles][0], a[0], a[1], a[2], a[3], b[0], b[1]);
+        mma16816<T>(acc[m % kTiles][1], a[0], a[1], a[2], a[3], b[2], b[3]);
+      }
+    }
+  }
+  norm::copy_wait<0>();
+  const long long pitch = low_grad_columns(job.columns, job.planes), plane_columns = pitch / job.planes;
+  const int adapters = gridDim.z / p.rank_groups;
+  float* part = job.part + ((long long)blockIdx.x * adapters + g) * p.rank * pitch + plane * plane_columns;
+#pragma unroll
+  for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = r0 + m * 16 + (lane >> 2) + 8 * (e >> 1), c = c0 + warp * 16 + n * 8 + (lane & 3) * 2 + (e & 1);
+        if (r >= p.rank || c >= job.columns) continue;
+        float* to = part + r * pitch + c;
+        *to = p.accumulate ? *to + acc[m][n][e] : acc[m][n][e];
+      }
+}
+
+template <typename T, int kTiles>
+int launch_grad(DeviceState* st, dim3 grid, void* stream, const GradParams& p) {
+  constexpr int kIndex = (kTiles == 4 ? 2 : kTiles - 1) + (__is_same(T, __half) ? 3 : 0);
+  return launch_kernel(st, KernelId(kKernelLowGrad + kIndex), low_grad_kernel<T, kTiles>, grid, 256, grad_stages(kTiles) * grad_stage(kTiles),
+                       stream, p);
+}
+
+struct LowJoinParams {
+  LowGrad job[2];
+  int rank, parts, adapters;
+  long long items0, items;  // of the first job, of both; an item is one value, or eight ranks of one column of a transposed result
+};
+template <typename T>
+__global__ void __launch_bounds__(256)
+low_join_kernel(const LowJoinParams p) {
+  pdl_trigger();
+  pdl_wait();
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < p.items; i += gridDim.x * 256LL) {
+    const bool second = i >= p.items0;
+    const LowGrad& job = second ? p.job[1] : p.job[0];
+    long long at = second ? i - p.items0 : i;
+    const int all = job.columns * job.planes, plane_columns = (job.columns + 3) / 4 * 4;
+    const long long pitch = (long long)plane_columns * job.planes, stride = (long long)p.adapters * p.rank * pitch;
+    const int column = int(at % all), plane = column / job.columns, ranks = job.transposed ? 8 : 1;
+    at /= all;
+    const int groups = (p.rank + ranks - 1) / ranks, r0 = int(at % groups) * ranks;
+    const long long g = at / groups;
+    const float* part = job.part + (g * p.rank + r0) * pitch + plane * plane_columns + (column - plane * job.columns);
+    float sum[8] = {};
+    const int n = p.rank - r0 < ranks ? p.rank - r0 : ranks;
+    if (job.transposed) {
+      for (int s = 0; s < p.parts; ++s)
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < n) sum[r] += __ldg(part + s * stride + r * pitch);
+      T* out = static_cast<T*>(job.out) + (g * all + column) * p.rank + r0;
+      if (n == 8 && p.rank % 8 == 0 && (reinterpret_cast<uintptr_t>(job.out) & 15u) == 0) {
+        *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]), pack2<T>(sum[4], sum[5]), pack2<T>(sum[6], sum[7]));
+      } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < n) out[r] = static_cast<T>(sum[r]);
+      }
+    } else {
+#pragma unroll 8
+      for (int s = 0; s < p.parts; ++s) sum[0] += __ldg(part + s * stride);
+      static_cast<T*>(job.out)[(g * p.rank + r0) * all + column] = static_cast<T>(sum[0]);
+    }
+  }
+}
+
+}  // namespace
+
+int run_low(const LowProduct& m, void* stream) {
+  DeviceState* st = nullptr;
+  const int rc = get_device_state(&st);
+  if (rc != B200TA_OK) return rc;
+  if (m.f16) return m.aligned ? launch_low<__half, true>(st, m, stream) : launch_low<__half, false>(st, m, stream);
+  return m.aligned ? launch_low<__nv_bfloat16, true>(st, m, stream) : launch_low<__nv_bfloat16, false>(st, m, stream);
+}
+
+int run_transpose_up(const void* up, int64_t up_pitch, void* out, int64_t out_pitch, int count, int rank, int N, int planes, void* stream) {
+  DeviceState* st = nullptr;
+  const int rc = get_device_state(&st);
+  if (rc != B200TA_OK) return rc;
+  const TransposeParams p{static_cast<const uint16_t*>(up), static_cast<uint16_t*>(out), up_pitch, out_pitch, rank, N, planes};
+  return launch_kernel(st, kKernelAdapter, transpose_up_kernel, dim3(unsigned((N + 31) / 32), unsigned((rank + 31) / 32), unsigned(count * planes)), 256,
+                       0, stream, p);
+}
+
+// Parts of the rows: two waves of two blocks on each multiprocessor if all adapters have their share of the rows, more (rows may be of
+// few of them) as long as the parts stay below 32 MiB.
+int low_grad_parts(int64_t rows, int64_t columns, int count, int rank, int num_sms) {
+  const int64_t chunks = (rows + kGradRows - 1) / kGradRows, slabs = (columns + kGradColumns - 1) / kGradColumns * ((rank + 63) / 64);
+  const int64_t wanted = (int64_t(num_sms) * 4 + slabs - 1) / slabs, shared = (wanted + count - 1) / count;
+  const int64_t by_bytes = (int64_t(1) << 25) / (int64_t(count) * rank * columns * 4);
+  const int64_t parts = std::max(std::min(std::max(shared, std::min(wanted, by_bytes)), (chunks + 3) / 4), (chunks + kGradChunks - 1) / kGradChunks);
+  const int64_t per = (chunks + parts - 1) / parts;
+  return int((chunks + per - 1) / per);
+}
+
+int run_low_grads(const LowGrads& m, void* stream) {
+  DeviceState* st = nullptr;
+  const int rc = get_device_state(&st);
+  if (rc != B200TA_OK) return rc;
+  GradParams p{};
+  auto slabs_of = [](const LowGrad& j) { return j.v == nullptr ? 0 : j.planes * ((j.columns + kGradColumns - 1) / kGradColumns); };
+  p.job[0] = m.job[0], p.job[1] = m.job[1], p.index = m.index, p.rows = m.rows, p.rank = m.rank, p.rank_groups = (m.rank + 63) / 64;
+  p.slabs0 = slabs_of(m.job[0]), p.accumulate = m.accumulate;
+  const int64_t chunks = (m.rows + kGradRows - 1) / kGradRows;
+  p.chunks_part = int((chunks + m.parts - 1) / m.parts);
+  B200TA_REQUIRE(p.chunks_part <= kGradChunks, "adapters: too many rows for %d parts", m.parts);
+  const dim3 grid{unsigned(m.parts), unsigned(p.slabs0 + slabs_of(m.job[1])), unsigned(m.index.count * p.rank_groups)};
+  const int tiles = m.rank <= 16 ? 1 : m.rank <= 32 ? 2 : 4;
+  int (*launch)(DeviceState*, dim3, void*, const GradParams&);
+  if (m.f16) launch = tiles == 1 ? launch_grad<__half, 1> : tiles == 2 ? launch_grad<__half, 2> : launch_grad<__half, 4>;
+  else launch = tiles == 1 ? launch_grad<__nv_bfloat16, 1> : tiles == 2 ? launch_grad<__nv_bfloat16, 2> : launch_grad<__nv_bfloat16, 4>;
+  return launch(st, grid, stream, p);
+}
+
+int run_low_join(const LowGrads& m, void* stream) {
+  DeviceState* st = nullptr;
+  const int rc = get_device_state(&st);
+  if (rc != B200TA_OK) return rc;
+  LowJoinParams p{};
+  auto items_of = [&](const LowGrad& j) {
+    return j.v == nullptr ? int64_t(0) : int64_t(m.index.count) * j.columns * j.planes * (j.transposed ? (m.rank + 7) / 8 : m.rank);
+  };
+  p.job[0] = m.job[0], p.job[1] = m.job[1], p.rank = m.rank, p.parts = m.parts, p.adapters = m.index.count;
+  p.items0 = items_of(m.job[0]), p.items = p.items0 + items_of(m.job[1]);
+  const int64_t blocks = std::min<int64_t>((p.items + 255) / 256, int64_t(st->num_sms) * 16);
+  return launch_kernel(st, kKernelAdapter, m.f16 ? low_join_kernel<__half> : low_join_kernel<__nv_bfloat16>, dim3(unsigned(blocks)), 256, 0, stream, p);
+}
+
+}  // namespace b200ta

@@ -51,8 +51,9 @@ enum KernelId {
   kKernelProject, kKernelContract, kKernelOutput, kKernelOutputF32, kKernelLinear, kKernelPairBias, kKernelRowStats,
   kKernelMaskRows, kKernelNorm, kKernelDenseHelpers, kKernelNarrow,
   kKernelMatmul = kKernelNarrow + 4,  // and one for each of the matmul kernels after it
-  kKernelDropout = 60, kKernelAdapter,
-  kKernelMatmulAdapters = 64  // and one for each of the matmul kernels with adapters after it
+  kKernelDropout = kKernelMatmul + 32, kKernelAdapter,
+  kKernelMatmulAdapters = 64,                        // and one for each of the matmul kernels with adapters after it
+  kKernelLowGrad = kKernelMatmulAdapters + 32        // six
 };
 int get_device_state(DeviceState** out);
 

@@ -5,6 +5,7 @@
 #include "layer_norm.cuh"
 #include "matmul.cuh"
 #include "narrow.cuh"
+#include "warp_matmul.cuh"
 
 namespace b200ta {
 
@@ -31,10 +32,12 @@ struct TilingOf {
   bool a_mn, sums;  // sums of A over k: tiles of up to 128 columns
   int64_t rows, outer, columns;
   int kblocks, splits;
+  double more = 0;  // blocks along k that adapters add to a tile, as parts of whole ones
 };
 Tiling choose_tiling(const TilingOf& m, int num_sms) {
   const bool two = m.form == kGated || m.form == kGatedGrad;
   const int64_t accumulated = two ? m.columns * 2 : m.columns;
+  const double kblocks = m.kblocks + m.more;
   const double finish = m.form == kGatedGrad ? 12 : two ? 8 : 6.5;  // clocks for an accumulator column of 128 rows
   Tiling best{128, 0, 0, 1e300};
   auto consider = [&](int n, int pair, int resident, double waves, double main) {
@@ -47,20 +50,29 @@ Tiling choose_tiling(const TilingOf& m, int num_sms) {
     if (n > 64 && n / 2 >= accumulated) continue;
     const int64_t tiles_n = (accumulated + n - 1) / n;
     const double mma = 4.0 * std::max(40.0, n * 0.54);
-    if (!m.a_mn && m.splits == 1 && m.kblocks * n * matmul::kBK * 2 <= matmul::kResidentBytes && tiles_n <= num_sms) {
+    if (!m.a_mn && m.splits == 1 && m.more == 0 && m.kblocks * n * matmul::kBK * 2 <= matmul::kResidentBytes && tiles_n <= num_sms) {
       const int64_t lanes = std::min(tiles_m, num_sms / tiles_n);
       consider(n, 0, int(lanes), waves_of(tiles_m, lanes), m.kblocks * std::max(mma, 356.0));
     } else {
       const double load = (n == 256 ? 1.2 : 1.0) * (16384 + n * 128) / 46;
-      consider(n, 0, 0, waves_of(tiles_m * tiles_n * m.splits, num_sms), m.kblocks * std::max(mma, load));
+      consider(n, 0, 0, waves_of(tiles_m * tiles_n * m.splits, num_sms), kblocks * std::max(mma, load));
     }
   }
   for (int n = 256; n >= 128 && m.rows > matmul::kBM && !m.sums; n /= 2) {
     if (n / 2 >= accumulated) continue;
     const int64_t tiles = (m.rows + 255) / 256 * m.outer * m.splits * ((accumulated + n - 1) / n);
-    consider(n, 1, 0, waves_of(tiles, num_sms / 2), m.kblocks * std::max(4.0 * n * 0.54, (16384 + n * 64) / 46.0));
+    consider(n, 1, 0, waves_of(tiles, num_sms / 2), kblocks * std::max(4.0 * n * 0.54, (16384 + n * 64) / 46.0));
   }
   return best;
+}
+
+// Ranks of a block along k, in rows of 32 or 64 bytes (a stage has room for two terms of the latter).
+int low_unit(int rank) { return rank <= 16 ? 16 : 32; }
+double low_blocks(const LowRank* a) {
+  if (a == nullptr) return 0;
+  const int unit = low_unit(a->rank);
+  const int64_t requests = a->index.index == nullptr ? 1 : 128 / int64_t(a->index.rows_per_index) + 1;
+  return double(std::min<int64_t>(a->index.count, requests)) * ((a->rank + unit - 1) / unit) * unit / 64;
 }
 
 }  // namespace
@@ -80,7 +92,8 @@ int run_matmul(const Matmul& m, void* stream) {
   p.kblocks_split = m.kblocks_split > 0 && m.kblocks_split < p.kblocks ? m.kblocks_split : p.kblocks;
   p.splits = (p.kblocks + p.kblocks_split - 1) / p.kblocks_split;
   p.rows_inner = int(rows), p.columns = int(columns);
-  const Tiling tiling = choose_tiling({m.form, m.a_mn, m.sums != nullptr, rows, m_outer, columns, p.kblocks_split, p.splits}, st->num_sms);
+  const Tiling tiling =
+      choose_tiling({m.form, m.a_mn, m.sums != nullptr, rows, m_outer, columns, p.kblocks_split, p.splits, low_blocks(m.adapters)}, st->num_sms);
   p.tile_n = tiling.tile_n, p.pair = tiling.pair, p.resident = tiling.resident;
   const int tile_m = p.pair ? 2 * matmul::kBM : matmul::kBM;
   p.tiles_m_inner = int((rows + tile_m - 1) / tile_m);
@@ -128,9 +141,24 @@ int run_matmul(const Matmul& m, void* stream) {
   // A set sees the phases of its own tiles alone, and a wait cannot tell a phase from the one after the next: every phase of an
   // accumulator has to be the same set's, so there are as many accumulators as sets at least.
   p.sets = std::min(p.sets, p.buffers);
-  if (m.form == kDenseGrad || m.form == kGatedGrad) return launch_matmul_grad(st, m, maps, p, grid, stream);
-  if (m.b_mn) return launch_matmul_product(st, m, maps, p, grid, stream);
-  return launch_matmul_forward(st, m, maps, p, grid, stream);
+  auto launch = [&](const auto& x) {
+    if (m.form == kDenseGrad || m.form == kGatedGrad) return launch_matmul_grad(st, m, maps, p, x, grid, stream);
+    if (m.b_mn) return launch_matmul_product(st, m, maps, p, x, grid, stream);
+    return launch_matmul_forward(st, m, maps, p, x, grid, stream);
+  };
+  if (m.adapters == nullptr) return launch(NoAdapters{});
+  const LowRank& a = *m.adapters;
+  MatmulAdapters x{};
+  x.index = a.index, x.rank = a.rank, x.unit = low_unit(a.rank), x.blocks = (a.rank + x.unit - 1) / x.unit;
+  const SwizzleMode swizzle = x.unit == 32 ? SWZ_64 : SWZ_32;
+  const Plane low{a.low, rows, a.rank, 2 * padded_rank(a.rank), 2, padded_rank(a.rank)};
+  if ((rc = map_of(&x.low, low, 2, uint32_t(x.unit), matmul::kBM, 2, swizzle, m.what)) != B200TA_OK) return rc;
+  const Plane high = m.b_mn ? Plane{a.high, a.rank, columns, a.high_pitch, a.index.count, a.rank * a.high_pitch}
+                            : Plane{a.high, columns, a.rank, a.high_pitch, a.index.count * (two ? 2 : 1), columns * a.high_pitch};
+  rc = m.b_mn ? map_of(&x.high, high, 2, 64, uint32_t(x.unit), 1, SWZ_128, m.what)
+              : map_of(&x.high, high, 2, uint32_t(x.unit), uint32_t(p.pair || !two ? b_rows : units), two && !p.pair ? 2 : 1, swizzle, m.what);
+  if (rc != B200TA_OK) return rc;
+  return launch(x);
 }
 
 namespace {
@@ -151,6 +179,7 @@ struct FewParams {
   void *y, *saved;
   long long xs, ws, rs, ys, ss;
   int rows, K, N, activation;
+  LowRank adapters;  // without `low`: none
 };
 
 template <typename T>
@@ -176,17 +205,6 @@ __device__ __forceinline__ void activate_any(int activation, float z, float& a, 
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (__is_same(T, __half))
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // Eight elements of a row of K from k on, zeros behind it.
 template <typename T, bool kVec>
 __device__ __forceinline__ uint4 load_row(const T* row, int k, int K) {
@@ -196,6 +214,25 @@ __device__ __forceinline__ uint4 load_row(const T* row, int k, int K) {
 }
 
 constexpr int kFewWarps = 16, kFewColumns = 16;  // of a block, at most
+// The sum of (low[r] + low2[r]) high[r] over the ranks.
+template <typename T>
+__device__ __forceinline__ float low_sum(const T* low, const T* low2, const T* high, int rank) {
+  float sum = 0.f;
+  if ((reinterpret_cast<uintptr_t>(high) & 15u) == 0 && rank % 8 == 0) {
+    for (int r = 0; r < rank; r += 8) {
+      float a[8], c[8], b[8];
+      load_vec<T>(low + r, a);
+      load_vec<T>(low2 + r, c);
+      load_vec<T>(high + r, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fmaf(a[j] + c[j], b[j], sum);
+    }
+  } else {
+    for (int r = 0; r < rank; ++r) sum = fmaf(static_cast<float>(low[r]) + static_cast<float>(low2[r]), static_cast<float>(high[r]), sum);
+  }
+  return sum;
+}
+
 template <typename T, bool kTwo, int kEights, bool kVec>
 __global__ void __launch_bounds__(kFewWarps * 32, 1)
 few_rows_kernel(const FewParams p) {
@@ -244,6 +281,16 @@ few_rows_kernel(const FewParams p) {
   for (int i = 0; i < warps; ++i) {
     v += joined[i][0][row][c];
     if constexpr (kTwo) gate += joined[i][1][row][c];
+  }
+  if (p.adapters.low != nullptr) {
+    const int a = adapter_of(p.adapters.index, uint32_t(row));
+    if (a != kNoAdapter) {
+      const int padded = padded_rank(p.adapters.rank);
+      const T* low = static_cast<const T*>(p.adapters.low) + row * 2 * padded;
+      const T* high = static_cast<const T*>(p.adapters.high) + ((long long)a * (kTwo ? 2 * p.N : p.N) + n) * p.adapters.high_pitch;
+      v += low_sum(low, low + padded, high, p.adapters.rank);
+      if constexpr (kTwo) gate += low_sum(low, low + padded, high + (long long)p.N * p.adapters.high_pitch, p.adapters.rank);
+    }
   }
   const T* bias = static_cast<const T*>(p.bias);
   if (bias != nullptr) {
@@ -629,16 +676,44 @@ const BackwardPlan& plan_backward(bool gated, bool slope, bool kept, bool want_d
   return e.plan;
 }
 
-}  // namespace
-}  // namespace b200ta
+// Where the adapters' intermediates of a backward pass lie behind the others in the workspace.
+struct LowPlan {
+  int parts;                          // of the rows for the adapters' gradients
+  int64_t up, low_grad, part[2], bytes;  // offsets: transposed up, dt of a chunk, parts of dD and dU
+};
+LowPlan plan_low(const BackwardPlan& plan, int count, int rank, int64_t rows, int K, int N, int outer, int num_sms) {
+  LowPlan p{};
+  const int64_t chunk = std::min(plan.chunk, rows), ad = low_grad_columns(K, 1), au = low_grad_columns(N, outer);
+  p.parts = low_grad_parts(chunk, int64_t(K) + int64_t(outer) * N, count, rank, num_sms);
+  p.bytes = (plan.bytes + 255) / 256 * 256;
+  auto take = [&](int64_t bytes) {
+    const int64_t at = p.bytes;
+    p.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  p.up = take(int64_t(count) * rank * outer * pad8(N) * 2);
+  p.low_grad = take(chunk * 2 * padded_rank(rank) * 2);
+  p.part[0] = take(int64_t(p.parts) * count * rank * ad * 4);
+  p.part[1] = take(int64_t(p.parts) * count * rank * au * 4);
+  return p;
+}
 
-extern "C" {
+int check_adapters(const char* what, const b200ta_adapters* a, const void* low) {
+  B200TA_REQUIRE(a != nullptr && a->down && a->up && low, "%s: NULL pointer", what);
+  B200TA_REQUIRE(a->count > 0 && a->count < 16384 && a->rank > 0 && a->rank <= kMaxRank, "%s: %d adapters of rank %d (up to 16383, up to %d)", what,
+                 a->count, a->rank, kMaxRank);
+  B200TA_REQUIRE(rows_aligned(low, 0), "%s: low must be 16-byte aligned", what);
+  B200TA_REQUIRE(a->index != nullptr || a->count == 1, "%s: several adapters need an index", what);
+  B200TA_REQUIRE(a->index == nullptr || ((a->index_bytes == 4 || a->index_bytes == 8) && a->rows_per_index > 0), "%s: index of %d bytes for %lld rows each",
+                 what, a->index_bytes, (long long)a->rows_per_index);
+  return B200TA_OK;
+}
+AdapterIndex index_of(const b200ta_adapters* a) {
+  return {a->index, a->index_bytes, uint32_t(std::min<int64_t>(std::max<int64_t>(a->rows_per_index, 1), int64_t(1) << 31)), 0, a->count};
+}
 
-int b200ta_dense_few_rows(void) { return b200ta::kFewRows; }
-
-int b200ta_dense(const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* residual, int64_t rs, void* y,
-                 int64_t ys, void* saved, int64_t ss, int dtype, int activation, int gated, int64_t rows, int K, int N, void* stream) {
-  using namespace b200ta;
+int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* residual, int64_t rs, void* y, int64_t ys,
+                  void* saved, int64_t ss, int dtype, int activation, int gated, int64_t rows, int K, int N, const LowRank* adapters, void* stream) {
   int rc = check_layer("dense", dtype, activation, rows, K, N);
   if (rc != B200TA_OK) return rc;
   B200TA_REQUIRE(x && w && y, "dense: NULL pointer");
@@ -649,7 +724,8 @@ int b200ta_dense(const void* x, int64_t xs, const void* w, int64_t ws, const voi
     rc = get_device_state(&st);
     if (rc != B200TA_OK) return rc;
     const bool vec = K % 8 == 0 && rows_aligned(x, xs) && rows_aligned(w, ws), f16 = dtype == B200TA_DTYPE_F16;
-    const FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation};
+    FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation, {}};
+    if (adapters != nullptr) p.adapters = *adapters;
     // sixteen warps where blocks are few (three rows, 1536 -> 384: 9 us instead of 11), eight otherwise, of which more blocks fit
     const int blocks = (N + kFewColumns - 1) / kFewColumns, warps = blocks <= st->num_sms ? kFewWarps : kFewWarps / 2;
     return launch_kernel(st, kKernelDenseHelpers, f16 ? pick_few<__half>(int(rows), vec, gated) : pick_few<__nv_bfloat16>(int(rows), vec, gated),
@@ -666,30 +742,13 @@ int b200ta_dense(const void* x, int64_t xs, const void* w, int64_t ws, const voi
   m.out = {y, rows, N, ys};
   if (residual) m.aux = {residual, rows, N, rs};
   if (saved) m.saved = {saved, rows, N, ss, gated ? 2 : 1, ss / 2};
-  m.bias = bias, m.activation = activation, m.what = gated ? "gated dense" : "dense";
+  m.bias = bias, m.activation = activation, m.adapters = adapters, m.what = gated ? "gated dense" : "dense";
   return run_matmul(m, stream);
 }
 
-int b200ta_dense_keeps(int activation, int gated, int K) {
-  // Kept values are written and read at 4 bytes each, computed ones cost 2 K operations each on the tensor cores: a training step
-  // of a gated layer takes 399 us either way for 8192 rows, 1024 -> 4096, and 361 us kept, 406 us computed again for 4096 rows,
-  // 2048 -> 4096.  (In 16 bits keeping would pay from 512 inputs on, but its rounding adds a third to the gradients' error.)
-  return (gated || activation != b200ta::kActNone) && K >= 1536;
-}
-
-size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, int64_t rows, int K, int N) {
-  using namespace b200ta;
-  DeviceState* st = nullptr;
-  if (rows <= 0 || K <= 0 || N <= 0 || get_device_state(&st) != B200TA_OK) return 0;
-  return size_t(plan_backward(gated, activation != kActNone, reads_kept(kept != 0, gated != 0, activation), want_dbias != 0, rows, K, N,
-                              st->num_sms)
-                    .bytes);
-}
-
-int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias,
-                          const void* saved, int64_t ss, void* dx, int64_t dxs, void* dw, void* dbias, void* workspace,
-                          size_t workspace_bytes, int dtype, int activation, int gated, int64_t rows, int K, int N, void* stream) {
-  using namespace b200ta;
+int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* saved,
+                    int64_t ss, void* dx, int64_t dxs, void* dw, void* dbias, void* workspace, size_t workspace_bytes, int dtype, int activation,
+                    int gated, int64_t rows, int K, int N, const b200ta_adapters* ad, const void* low, void* ddown, void* dup, void* stream) {
   int rc = check_layer("dense_backward", dtype, activation, rows, K, N);
   if (rc != B200TA_OK) return rc;
   B200TA_REQUIRE(dy && x && w, "dense_backward: NULL pointer");
@@ -701,11 +760,12 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
   if (rc != B200TA_OK) return rc;
   const bool kept = reads_kept(saved != nullptr, gated != 0, activation);
   const BackwardPlan& plan = plan_backward(gated, activation != kActNone, kept, dbias != nullptr, rows, K, N, st->num_sms);
-  B200TA_REQUIRE(plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
-                                     workspace_bytes >= size_t(plan.bytes)),
-                 "dense_backward: the workspace must be 256-byte aligned and of %lld bytes", (long long)plan.bytes);
-  const bool f16 = dtype == B200TA_DTYPE_F16, own_dz = plan.dz_pitch != 0;
   const int64_t outer = gated ? 2 : 1;
+  const LowPlan low_plan = ad != nullptr ? plan_low(plan, ad->count, ad->rank, rows, K, N, int(outer), st->num_sms) : LowPlan{0, 0, 0, {0, 0}, plan.bytes};
+  B200TA_REQUIRE(low_plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
+                                         workspace_bytes >= size_t(low_plan.bytes)),
+                 "dense_backward: the workspace must be 256-byte aligned and of %lld bytes", (long long)low_plan.bytes);
+  const bool f16 = dtype == B200TA_DTYPE_F16, own_dz = plan.dz_pitch != 0;
   char* ws_base = static_cast<char*>(workspace);
   float* parts = reinterpret_cast<float*>(ws_base + plan.parts);
   float* sums = reinterpret_cast<float*>(ws_base + plan.sums);
@@ -723,11 +783,31 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
     return launch_kernel(st, kKernelDenseHelpers, f16 ? join_kernel<__half> : join_kernel<__nv_bfloat16>,
                          dim3(unsigned(a.blocks + b.blocks + c.blocks)), 256, 0, stream, a, b, c);
   };
-  const bool narrow = narrow_pays(own_dz, kept, gated != 0, rows, K, N, dx, dxs, st->num_sms);
+  const bool narrow = ad == nullptr && narrow_pays(own_dz, kept, gated != 0, rows, K, N, dx, dxs, st->num_sms);
   const bool dx_parts = dx != nullptr && !narrow && plan.dx_split.parts > 1 && dxs == K;  // (a join writes dense rows)
+
+  // adapters: t (from the forward pass) with U for the pre-activations, dt with D for dx
+  const int64_t low_pitch = ad != nullptr ? 2 * padded_rank(ad->rank) : 0;
+  LowRank with_up{}, with_down{};
+  LowGrads low_grads{};
+  void* dt = ws_base + low_plan.low_grad;
+  if (ad != nullptr) {
+    with_up = {index_of(ad), ad->rank, nullptr, ad->up, ad->up_row_stride};
+    with_down = {index_of(ad), ad->rank, dt, ad->down, ad->down_row_stride};
+    low_grads.job[0] = {dt, nullptr, reinterpret_cast<float*>(ws_base + low_plan.part[0]), ddown, xs, 0, K, 1, 0};
+    low_grads.job[1] = {nullptr, nullptr, reinterpret_cast<float*>(ws_base + low_plan.part[1]), dup, 0, 0, N, int(outer), 1};
+    low_grads.rank = ad->rank, low_grads.parts = low_plan.parts, low_grads.f16 = f16;
+    if (dx != nullptr || ddown != nullptr) {
+      rc = run_transpose_up(ad->up, ad->up_row_stride, ws_base + low_plan.up, pad8(N), ad->count, ad->rank, N, int(outer), stream);
+      if (rc != B200TA_OK) return rc;
+    }
+  }
 
   for (int64_t r0 = 0; r0 < rows; r0 += plan.chunk) {
     const int64_t n = rows - r0 < plan.chunk ? rows - r0 : plan.chunk;
+    const char* low_c = static_cast<const char*>(low) + r0 * low_pitch * 2;
+    with_up.low = low_c;
+    with_up.index.first_row = with_down.index.first_row = uint32_t(r0);
     const char* dy_c = static_cast<const char*>(dy) + r0 * dys * 2;
     const char* x_c = static_cast<const char*>(x) + r0 * xs * 2;
     const void* dz = dy_c;
@@ -760,10 +840,16 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
         m.b = {w, N, K, ws, outer, int64_t(N) * ws};
         m.out = {dst, n, N, zs, outer, zs / 2};
         m.aux = {dy_c, n, N, dys};
-        m.bias = bias, m.activation = activation, m.what = "dense_backward dz";
+        m.bias = bias, m.activation = activation, m.adapters = ad != nullptr ? &with_up : nullptr, m.what = "dense_backward dz";
         rc = run_matmul(m, stream);
       }
       if (rc != B200TA_OK) return rc;
+    }
+    if (ad != nullptr && (dx != nullptr || ddown != nullptr)) {
+      LowProduct q{};
+      q.x = dz, q.a = ws_base + low_plan.up, q.low = dt, q.scale = ad->scale, q.scale_all = ad->scale_all;
+      q.xs = zs, q.x_plane = zs / outer, q.as = outer * pad8(N), q.a_plane = pad8(N), q.rows = n, q.K = N, q.planes = int(outer), q.rank = ad->rank, q.f16 = f16, q.aligned = true, q.index = with_down.index;
+      if ((rc = run_low(q, stream)) != B200TA_OK) return rc;
     }
     if (dx != nullptr && !narrow) {
       Matmul m;
@@ -777,6 +863,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
         m.out = {static_cast<char*>(dx) + r0 * dxs * 2, n, K, dxs};
       }
       if (dw != nullptr) m.beside = kBesideFirst;
+      if (ad != nullptr) m.adapters = &with_down;
       m.what = "dense_backward dx";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
     }
@@ -797,6 +884,13 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       m.what = "dense_backward dW";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
     }
+    if (ddown != nullptr || dup != nullptr) {
+      low_grads.job[0].v = ddown != nullptr ? x_c : nullptr;
+      low_grads.job[1].v = dup != nullptr ? dz : nullptr;
+      low_grads.job[1].t = low_c, low_grads.job[1].v_pitch = zs, low_grads.job[1].v_plane = zs / outer;
+      low_grads.index = with_down.index, low_grads.rows = n, low_grads.accumulate = r0 > 0;
+      if ((rc = run_low_grads(low_grads, stream)) != B200TA_OK) return rc;
+    }
     if (dbias != nullptr && !product_sums && !kept) {
       const dim3 grid{unsigned((sum_columns + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
       if (f16)
@@ -808,6 +902,7 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
       if (rc != B200TA_OK) return rc;
     }
   }
+  if ((ddown != nullptr || dup != nullptr) && (rc = run_low_join(low_grads, stream)) != B200TA_OK) return rc;
   const bool parts_left = dw != nullptr && !direct, sums_left = dbias != nullptr && !(product_sums && direct);
   if (!parts_left && !sums_left && !dx_parts) return B200TA_OK;
   const int64_t chunk = plan.chunk < rows ? plan.chunk : rows;
@@ -816,6 +911,84 @@ int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs
                                     : join_of(sums_left, sums, (chunk + plan.rows_sum - 1) / plan.rows_sum, sum_pitch, sum_pitch / outer, outer, N, dbias);
   const JoinParams c = join_of(dx_parts, reinterpret_cast<const float*>(ws_base + plan.dx_parts), plan.dx_split.parts, rows * pad4(K), pad4(K), rows, K, dx);
   return join(a, b, c);
+}
+
+}  // namespace
+}  // namespace b200ta
+
+extern "C" {
+
+int b200ta_dense_few_rows(void) { return b200ta::kFewRows; }
+
+int b200ta_dense(const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* residual, int64_t rs, void* y,
+                 int64_t ys, void* saved, int64_t ss, int dtype, int activation, int gated, int64_t rows, int K, int N, void* stream) {
+  return b200ta::dense_forward(x, xs, w, ws, bias, residual, rs, y, ys, saved, ss, dtype, activation, gated, rows, K, N, nullptr, stream);
+}
+
+int b200ta_dense_keeps(int activation, int gated, int K) {
+  // Kept values are written and read at 4 bytes each, computed ones cost 2 K operations each on the tensor cores: a training step
+  // of a gated layer takes 399 us either way for 8192 rows, 1024 -> 4096, and 361 us kept, 406 us computed again for 4096 rows,
+  // 2048 -> 4096.  (In 16 bits keeping would pay from 512 inputs on, but its rounding adds a third to the gradients' error.)
+  return (gated || activation != b200ta::kActNone) && K >= 1536;
+}
+
+size_t b200ta_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, int64_t rows, int K, int N) {
+  using namespace b200ta;
+  DeviceState* st = nullptr;
+  if (rows <= 0 || K <= 0 || N <= 0 || get_device_state(&st) != B200TA_OK) return 0;
+  return size_t(plan_backward(gated, activation != kActNone, reads_kept(kept != 0, gated != 0, activation), want_dbias != 0, rows, K, N,
+                              st->num_sms)
+                    .bytes);
+}
+
+int b200ta_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias,
+                          const void* saved, int64_t ss, void* dx, int64_t dxs, void* dw, void* dbias, void* workspace,
+                          size_t workspace_bytes, int dtype, int activation, int gated, int64_t rows, int K, int N, void* stream) {
+  return b200ta::dense_gradients(dy, dys, x, xs, w, ws, bias, saved, ss, dx, dxs, dw, dbias, workspace, workspace_bytes, dtype, activation, gated, rows,
+                                 K, N, nullptr, nullptr, nullptr, nullptr, stream);
+}
+
+int b200ta_adapter_dense(const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* residual, int64_t rs, void* y, int64_t ys,
+                         void* saved, int64_t ss, const b200ta_adapters* a, void* low, int dtype, int activation, int gated,
+                         int64_t rows, int K, int N, void* stream) {
+  using namespace b200ta;
+  int rc = check_layer("adapter_dense", dtype, activation, rows, K, N);
+  if (rc != B200TA_OK) return rc;
+  B200TA_REQUIRE(x && w && y, "adapter_dense: NULL pointer");
+  if ((rc = check_adapters("adapter_dense", a, low)) != B200TA_OK) return rc;
+  const bool aligned = rows_aligned(x, xs) && rows_aligned(a->down, a->down_row_stride);
+  B200TA_REQUIRE(rows <= kFewRows || (aligned && rows_aligned(a->up, a->up_row_stride)),
+                 "adapter_dense: what is read must be 16-byte aligned with row strides that are multiples of 8 elements");
+  LowProduct q{};
+  q.x = x, q.a = a->down, q.low = low, q.scale = a->scale, q.scale_all = a->scale_all;
+  q.xs = xs, q.as = a->down_row_stride, q.rows = rows, q.K = K, q.planes = 1, q.rank = a->rank;
+  q.f16 = dtype == B200TA_DTYPE_F16, q.aligned = aligned, q.index = index_of(a);
+  if ((rc = run_low(q, stream)) != B200TA_OK) return rc;
+  const LowRank adapters{q.index, a->rank, low, a->up, a->up_row_stride};
+  return dense_forward(x, xs, w, ws, bias, residual, rs, y, ys, saved, ss, dtype, activation, gated, rows, K, N, &adapters, stream);
+}
+
+size_t b200ta_adapter_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, int count, int rank, int64_t rows, int K, int N) {
+  using namespace b200ta;
+  DeviceState* st = nullptr;
+  if (rows <= 0 || K <= 0 || N <= 0 || count <= 0 || rank <= 0 || get_device_state(&st) != B200TA_OK) return 0;
+  const BackwardPlan& plan = plan_backward(gated, activation != kActNone, reads_kept(kept != 0, gated != 0, activation), want_dbias != 0, rows, K, N,
+                                           st->num_sms);
+  return size_t(plan_low(plan, count, rank, rows, K, N, gated ? 2 : 1, st->num_sms).bytes);
+}
+
+int b200ta_adapter_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* saved,
+                                  int64_t ss, const b200ta_adapters* a, const void* low, void* dx, int64_t dxs, void* dw, void* dbias,
+                                  void* ddown, void* dup, void* workspace, size_t workspace_bytes, int dtype, int activation, int gated, int64_t rows,
+                                  int K, int N, void* stream) {
+  using namespace b200ta;
+  int rc = check_layer("adapter_dense_backward", dtype, activation, rows, K, N);
+  if (rc != B200TA_OK) return rc;
+  if ((rc = check_adapters("adapter_dense_backward", a, low)) != B200TA_OK) return rc;
+  B200TA_REQUIRE(rows_aligned(a->down, a->down_row_stride) && rows_aligned(a->up, a->up_row_stride),
+                 "adapter_dense_backward: what is read must be 16-byte aligned with row strides that are multiples of 8 elements");
+  return dense_gradients(dy, dys, x, xs, w, ws, bias, saved, ss, dx, dxs, dw, dbias, workspace, workspace_bytes, dtype, activation, gated, rows, K, N, a,
+                         low, ddown, dup, stream);
 }
 
 int b200ta_copy_rows(const b200ta_copy* jobs, int count, void* stream) {

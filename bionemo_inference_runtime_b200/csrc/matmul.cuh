@@ -33,6 +33,7 @@
 #include <type_traits>
 
 #include "activation.cuh"
+#include "adapters.cuh"
 #include "common.cuh"
 #include "slab_ring.h"
 
@@ -69,6 +70,17 @@ struct MatmulParams {
 // Two products that read the same dz run beside each other: the first lets its successor start only when what came before both
 // is complete, so the second does not wait for it, except at its end (whatever follows them waits for the second alone).
 enum { kBesideNone = 0, kBesideFirst, kBesideSecond };
+
+// Adapters of the rows (see adapters.cuh), or none.  Behind the blocks of x and W along k, a tile takes for each adapter that its rows
+// have the blocks of t and U_g (for dx: of dt and D_g), `unit` ranks wide (as wide as the swizzle of their rows: 32 or 64
+// bytes, so that a stage holds both terms of t beside the one block of U_g that they share).  A block of t serves all of a tile's adapters: the MMA updates no lane (row) whose adapter is another, so nothing of
+// one request, infinities and NaN among it, reaches another's rows.
+struct NoAdapters {};
+struct MatmulAdapters {
+  CUtensorMap low, high;
+  AdapterIndex index;
+  int rank, unit, blocks;
+};
 
 #ifdef __CUDACC__
 
@@ -304,11 +316,29 @@ __device__ __forceinline__ void mbar_arrive_cluster_warp(uint32_t bar) {
       : "memory");
 }
 
-template <typename T, MatmulForm kForm, bool kAMn, bool kBMn, bool kPair>
+// The same for rows (lanes of tensor memory) whose bit in `off` is clear; the others keep what they hold.
+__device__ __forceinline__ void umma_ss_lanes_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t (&off)[4]) {
+  asm volatile(
+      "{\n.reg .pred p, e;\nsetp.eq.b32 p, 0, 0;\nelect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+      : "memory");
+}
+__device__ __forceinline__ void umma_ss_lanes_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t (&off)[8]) {
+  asm volatile(
+      "{\n.reg .pred p, e;\nsetp.eq.b32 p, 0, 0;\nelect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]), "r"(off[5]), "r"(off[6]),
+      "r"(off[7])
+      : "memory");
+}
+
+template <typename T, MatmulForm kForm, bool kAMn, bool kBMn, bool kPair, typename X>
 __global__ void __launch_bounds__(kThreads, 1)
 matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
               const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ CUtensorMap tm_aux,
-              const __grid_constant__ CUtensorMap tm_saved, const MatmulParams p) {
+              const __grid_constant__ CUtensorMap tm_saved, const MatmulParams p, const __grid_constant__ X x) {
+  constexpr bool kAdapt = !std::is_same<X, NoAdapters>::value;
   constexpr bool kTwo = kForm == kGated || kForm == kGatedGrad;  // value and gate columns in a tile
   constexpr bool kGrad = kForm == kDenseGrad || kForm == kGatedGrad;
   constexpr bool kAux = kGrad || kForm == kDense;                // a warp's first slab receives residual or dy
@@ -364,11 +394,14 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
 
   if (warp == 16) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      tma_prefetch_desc(&tm_a);
-      tma_prefetch_desc(&tm_b);
+    if (kAdapt || lane == 0) {  // (with adapters all lanes stay, to walk those of a tile's rows; the first one issues)
+      if (lane == 0) {
+        tma_prefetch_desc(&tm_a);
+        tma_prefetch_desc(&tm_b);
+      }
       if (p.beside != kBesideSecond) pdl_wait();
       auto load = [&](uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
+        if (kAdapt && lane != 0) return;
         if constexpr (kPair) tma_load_3d_pair(dst, m, bar, c0, c1, c2);
         else tma_load_3d(dst, m, bar, c0, c1, c2);
       };
@@ -383,7 +416,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       };
       if (p.resident) {
         const Item t = item_of<kPair, kAMn>(p, 0, units);
-        mbar_expect_tx(bars + B_FULL * 8, p.kblocks * b_bytes);
+        if (!kAdapt || lane == 0) mbar_expect_tx(bars + B_FULL * 8, p.kblocks * b_bytes);
         for (int kb = 0, ko = 0, ki = 0; kb < p.kblocks; ++kb) {
           load_b(base + kb * b_bytes, bars + B_FULL * 8, t.n0, ki * kBK, ko);
           if (++ki == p.kblocks_inner) ki = 0, ++ko;
@@ -392,21 +425,30 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       int stage = 0, issued = 0;
       uint32_t phase = 1;
       bool ok = true;
+      // The barrier that counts `bytes` of the next stage (of a pair: the first block's, which counts the loads of both).
+      uint32_t full = 0;
+      auto open_stage = [&](int bytes) {
+        if constexpr (kAdapt) ok = mbar_wait_warp(bars + (EMPTY + stage) * 8, phase, abort_flag);
+        else ok = mbar_wait(bars + (EMPTY + stage) * 8, phase, abort_flag);
+        if (!ok) return;
+        full = bars + (FULL + stage) * 8;
+        if (kPair) {
+          if (rank == 0 && (!kAdapt || lane == 0)) mbar_expect_tx(full, 2 * bytes);
+          full = in_first_block(full);
+        } else {
+          if (!kAdapt || lane == 0) mbar_expect_tx(full, bytes);
+        }
+      };
+      [[maybe_unused]] bool low_complete = p.beside != kBesideSecond;
       for (int i = 0; ok && i < items; ++i) {
         Item t = item_of<kPair, kAMn>(p, i, units);
+        [[maybe_unused]] TileAdapters<kPair ? 8 : 4> adapters;
+        if constexpr (kAdapt) adapters.load(x.index, t.m0, p.rows_inner);
         t.m0 += int(rank) * kBM;
         int ko = t.kb0 / p.kblocks_inner, ki = t.kb0 - ko * p.kblocks_inner;
         for (int kb = t.kb0; kb < t.kb1; ++kb) {
-          ok = mbar_wait(bars + (EMPTY + stage) * 8, phase, abort_flag);
+          open_stage(stage_bytes);
           if (!ok) break;
-          uint32_t full = bars + (FULL + stage) * 8;
-          // the first block's barrier counts the loads of both
-          if (kPair) {
-            if (rank == 0) mbar_expect_tx(full, 2 * stage_bytes);
-            full = in_first_block(full);
-          } else {
-            mbar_expect_tx(full, stage_bytes);
-          }
           const uint32_t sa = ring + stage * stage_bytes;
           const int k0 = ki * kBK;
           if constexpr (kAMn) {
@@ -420,10 +462,31 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (++stage == p.stages) stage = 0, phase ^= 1u;
           if (++ki == p.kblocks_inner) ki = 0, ++ko;
         }
+        if constexpr (kAdapt) {
+          for (int g = adapters.next(-1); ok && t.split == p.splits - 1 && g != kNoAdapter; g = adapters.next(g)) {
+            if (!low_complete) pdl_wait(), low_complete = true;
+            for (int block = 0; block < x.blocks; ++block) {
+              open_stage((2 * kBM + b_rows) * x.unit * 2);
+              if (!ok) break;
+              const uint32_t sa = ring + stage * stage_bytes, sb = sa + kABytes;
+              const int r0 = block * x.unit;
+              load(sa, &x.low, full, r0, t.m0, 0);
+              if constexpr (kBMn) {
+                for (int n = 0; n < b_rows; n += 64) load(sb + n * x.unit * 2, &x.high, full, t.n0 + int(rank) * b_rows + n, r0, g);
+              } else if constexpr (kTwo && kPair) {
+                load(sb, &x.high, full, r0, t.n0, 2 * g + int(rank));
+              } else {
+                load(sb, &x.high, full, r0, t.n0 + int(rank) * b_rows, kTwo ? 2 * g : g);
+              }
+              ++issued;
+              if (++stage == p.stages) stage = 0, phase ^= 1u;
+            }
+          }
+        }
       }
       // If the loop was abandoned, give copies still in flight a bounded chance to land (of a pair's first block: those of
       // both; its second block's copies are waited for there).
-      if (*abort_flag) {
+      if (*abort_flag && (!kAdapt || lane == 0)) {
         if (p.resident) mbar_wait(bars + B_FULL * 8, 0, abort_flag + 1);
         if (rank == 0)
           for (int j = issued > p.stages ? issued - p.stages : 0; j < issued; ++j)
@@ -439,8 +502,11 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       uint32_t phase = 0;
       bool ok = true;
       if (p.resident) ok = mbar_wait_warp(bars + B_FULL * 8, 0, abort_flag);
+      if (kAdapt && p.beside != kBesideSecond) pdl_wait();  // the index
       for (int i = 0; ok && i < items; ++i) {
         const Item t = item_of<kPair, kAMn>(p, i, units);
+        [[maybe_unused]] TileAdapters<kPair ? 8 : 4> adapters;
+        if constexpr (kAdapt) adapters.load(x.index, t.m0, p.rows_inner);
         const int buffer = i & ((1 << p.buffers) - 1);
         const uint32_t acc = tb + buffer * (512 >> p.buffers);
         ok = mbar_wait_warp(bars + (ACC_EMPTY + buffer) * 8, ((i >> p.buffers) & 1) ^ 1, abort_flag);
@@ -469,6 +535,29 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + stage) * 8);
           else umma_commit_warp(bars + (EMPTY + stage) * 8);
           if (++stage == p.stages) stage = 0, phase ^= 1u;
+        }
+        if constexpr (kAdapt) {
+          for (int g = adapters.next(-1); ok && t.split == p.splits - 1 && g != kNoAdapter; g = adapters.next(g)) {
+            uint32_t off[kPair ? 8 : 4];
+#pragma unroll
+            for (int j = 0; j < (kPair ? 8 : 4); ++j) off[j] = ~adapters.rows_of(j, g);
+            for (int block = 0; block < x.blocks; ++block) {
+              ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t sa = ring + stage * stage_bytes, sb = sa + kABytes;
+              // K-major: rows of 2 * unit bytes, groups of 8 rows apart as they lie.  MN-major: as above, `unit` rows (k) a block.
+              const uint64_t rows_hi = uint64_t(x.unit) | (1u << 14) | ((x.unit == 32 ? kLayoutSw64 : kLayoutSw32) << 29);
+              const uint64_t da = rows_hi << 32 | ((sa >> 4) | 1u << 16);
+              const uint64_t db = kBMn ? smem_desc<0, 1024, kLayoutSw128>(sb) | uint64_t(x.unit * 8) << 16 : rows_hi << 32 | ((sb >> 4) | 1u << 16);
+              const int left = x.rank - block * x.unit, steps = ((left < x.unit ? left : x.unit) + 15) / 16;
+              for (int term = 0; term < 2; ++term)  // (a term's block is 128 rows)
+                for (int k = 0; k < steps; ++k) umma_ss_lanes_warp(acc, da + term * x.unit * 16 + k * 2, db + k * (kBMn ? 128 : 2), id, off);
+              if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + stage) * 8);
+              else umma_commit_warp(bars + (EMPTY + stage) * 8);
+              if (++stage == p.stages) stage = 0, phase ^= 1u;
+            }
+          }
         }
         if (!ok) break;
         if constexpr (kPair) umma_commit_pair_warp(bars + (ACC_FULL + buffer) * 8);
@@ -692,27 +781,33 @@ struct Matmul {
   bool accumulate = false;
   int beside = kBesideNone;
   void* sums = nullptr;  // see MatmulParams
+  const LowRank* adapters = nullptr;
   const char* what = "matmul";
 };
 int run_matmul(const Matmul& m, void* stream);
 
-// The three sets of kernels, each compiled by itself; a set returns B200TA_ERR_UNSUPPORTED for a product that is not its own.
+// The three sets of kernels, each compiled by itself, without and with adapters; a set returns B200TA_ERR_UNSUPPORTED for a product
+// that is not its own.
 struct MatmulMaps {
   CUtensorMap a, b, out, aux, saved;
 };
-int launch_matmul_forward(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, int grid, void* stream);
-int launch_matmul_grad(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, int grid, void* stream);
-int launch_matmul_product(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, int grid, void* stream);
+int launch_matmul_forward(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const NoAdapters& x, int grid, void* stream);
+int launch_matmul_grad(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const NoAdapters& x, int grid, void* stream);
+int launch_matmul_product(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const NoAdapters& x, int grid, void* stream);
+int launch_matmul_forward(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const MatmulAdapters& x, int grid, void* stream);
+int launch_matmul_grad(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const MatmulAdapters& x, int grid, void* stream);
+int launch_matmul_product(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const MatmulAdapters& x, int grid, void* stream);
 
 #ifdef __CUDACC__
 namespace matmul {
-template <MatmulForm kForm, bool kAMn, bool kBMn>
-int launch(DeviceState* st, int id, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, int grid, void* stream) {
-  const KernelId kernel = KernelId(kKernelMatmul + 4 * id + (m.f16 ? 2 : 0) + (p.pair ? 1 : 0));
-  auto* function = p.pair ? (m.f16 ? matmul_kernel<__half, kForm, kAMn, kBMn, true> : matmul_kernel<__nv_bfloat16, kForm, kAMn, kBMn, true>)
-                          : (m.f16 ? matmul_kernel<__half, kForm, kAMn, kBMn, false> : matmul_kernel<__nv_bfloat16, kForm, kAMn, kBMn, false>);
+template <MatmulForm kForm, bool kAMn, bool kBMn, typename X>
+int launch(DeviceState* st, int id, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const X& x, int grid, void* stream) {
+  constexpr int kFirst = std::is_same<X, NoAdapters>::value ? kKernelMatmul : kKernelMatmulAdapters;
+  const KernelId kernel = KernelId(kFirst + 4 * id + (m.f16 ? 2 : 0) + (p.pair ? 1 : 0));
+  auto* function = p.pair ? (m.f16 ? matmul_kernel<__half, kForm, kAMn, kBMn, true, X> : matmul_kernel<__nv_bfloat16, kForm, kAMn, kBMn, true, X>)
+                          : (m.f16 ? matmul_kernel<__half, kForm, kAMn, kBMn, false, X> : matmul_kernel<__nv_bfloat16, kForm, kAMn, kBMn, false, X>);
   return launch_clusters(st, kernel, function, dim3(unsigned(grid)), p.pair ? 2 : 1, kThreads, kSmDynamic, stream, maps.a, maps.b,
-                         maps.out, maps.aux, maps.saved, p);
+                         maps.out, maps.aux, maps.saved, p, x);
 }
 }  // namespace matmul
 #endif

@@ -2,9 +2,9 @@
 #include "matmul.cuh"
 
 namespace b200ta {
-int launch_matmul_grad(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, int grid, void* stream) {
-  if (m.form == kDenseGrad) return matmul::launch<kDenseGrad, false, false>(st, 2, m, maps, p, grid, stream);
-  if (m.form == kGatedGrad) return matmul::launch<kGatedGrad, false, false>(st, 3, m, maps, p, grid, stream);
+int launch_matmul_grad(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const NoAdapters& x, int grid, void* stream) {
+  if (m.form == kDenseGrad) return matmul::launch<kDenseGrad, false, false>(st, 2, m, maps, p, x, grid, stream);
+  if (m.form == kGatedGrad) return matmul::launch<kGatedGrad, false, false>(st, 3, m, maps, p, x, grid, stream);
   return fail(B200TA_ERR_UNSUPPORTED, "%s: not a gradient of an activation", m.what);
 }
 }  // namespace b200ta

@@ -3,11 +3,11 @@
 #include "matmul.cuh"
 
 namespace b200ta {
-int launch_matmul_product(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, int grid, void* stream) {
-  if (m.form == kPlain && !m.a_mn) return matmul::launch<kPlain, false, true>(st, 4, m, maps, p, grid, stream);
-  if (m.form == kPlain) return matmul::launch<kPlain, true, true>(st, 5, m, maps, p, grid, stream);
-  if (m.form == kPartial && !m.a_mn) return matmul::launch<kPartial, false, true>(st, 7, m, maps, p, grid, stream);
-  if (m.form == kPartial) return matmul::launch<kPartial, true, true>(st, 6, m, maps, p, grid, stream);
+int launch_matmul_product(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const NoAdapters& x, int grid, void* stream) {
+  if (m.form == kPlain && !m.a_mn) return matmul::launch<kPlain, false, true>(st, 4, m, maps, p, x, grid, stream);
+  if (m.form == kPlain) return matmul::launch<kPlain, true, true>(st, 5, m, maps, p, x, grid, stream);
+  if (m.form == kPartial && !m.a_mn) return matmul::launch<kPartial, false, true>(st, 7, m, maps, p, x, grid, stream);
+  if (m.form == kPartial) return matmul::launch<kPartial, true, true>(st, 6, m, maps, p, x, grid, stream);
   return fail(B200TA_ERR_UNSUPPORTED, "%s: not a product of gradients", m.what);
 }
 }  // namespace b200ta

@@ -21,7 +21,8 @@ struct Library {
 #define B200TA_ENTRY(name) decltype(&b200ta_##name) name = nullptr;
 #define B200TA_ENTRIES(X)                                                                                                \
   X(layer_norm) X(layer_norm_workspace_bytes) X(layer_norm_backward) X(dense_few_rows) X(dense_keeps) X(dense)              \
-  X(dense_backward_workspace_bytes) X(dense_backward) X(copy_rows) X(dropout)
+  X(dense_backward_workspace_bytes) X(dense_backward) X(copy_rows) X(dropout)      \
+  X(adapter_dense) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
   B200TA_ENTRIES(B200TA_ENTRY)
 #undef B200TA_ENTRY
 } lib;
@@ -308,6 +309,133 @@ std::tuple<Maybe, Maybe, Maybe> dense_backward(const at::Tensor& dy, const at::T
   return {dx, dweight, dbias};
 }
 
+// ---- dense layers with adapters -----------------------------------------------------------------------------------------
+
+struct Adapting {
+  b200ta_adapters c{};
+  at::Tensor index, scale;  // held for the call
+  Rows down, up;
+};
+// The adapters of a layer of K inputs and `columns` outputs, checked; their matrices are made readable by `operand`.
+Adapting adapters_of(const at::Tensor& x, const Layer& l, int64_t columns, const at::Tensor& down, const at::Tensor& up, const Maybe& index,
+                     const Maybe& scale, double scale_all, bool few, Copies& copies) {
+  Adapting a;
+  if (down.dim() != 3 || down.size(2) != l.K || down.size(0) < 1 || down.size(1) < 1)
+    refuse("down must be [adapters, rank, " + std::to_string(l.K) + "], got " + shape_of(down));
+  const int64_t count = down.size(0), rank = down.size(1);
+  require_like("down", down, x, down.sizes());
+  require_like("up", up, x, {count, columns, rank});
+  if (rank > 256) refuse("the rank of adapters is up to 256, got " + std::to_string(rank));
+  if (count > 16383) refuse("up to 16383 adapters, got " + std::to_string(count));
+  a.c.rows_per_index = 1;
+  if (index) {
+    if (index->device() != x.device()) refuse("index must be on the device of x");
+    if (index->scalar_type() != at::kInt && index->scalar_type() != at::kLong) refuse("index must be int32 or int64");
+    bool prefix = index->dim() < x.dim();
+    for (int64_t d = 0; prefix && d < index->dim(); ++d) prefix = index->size(d) == x.size(d);
+    if (!prefix) refuse("index must have the leading axes of x " + shape_of(x) + " as its shape, got " + shape_of(*index));
+    a.index = index->contiguous();
+    a.c.index = a.index.data_ptr(), a.c.index_bytes = int(a.index.element_size());
+    a.c.rows_per_index = a.index.numel() > 0 ? std::max<int64_t>(l.rows / a.index.numel(), 1) : 1;
+  } else if (count != 1) {
+    refuse("several adapters need an index");
+  }
+  a.c.scale_all = float(scale_all);
+  if (scale) {
+    require_like("scale", *scale, x, {count}, true);
+    if (scale->scalar_type() != at::kFloat) refuse("scale must be a number or float32, one for each adapter");
+    a.scale = scale->contiguous();
+    a.c.scale = a.scale.data_ptr<float>();
+  }
+  a.c.count = int(count), a.c.rank = int(rank);
+  if (l.rows == 0) return a;
+  auto rows = [&](const at::Tensor& t) {  // (a matrix whose rows have one stride, adapters among them, is read where it lies)
+    return operand(t, few, copies);
+  };
+  a.down = rows(down), a.up = rows(up);
+  a.c.down = a.down.ptr, a.c.down_row_stride = a.down.stride, a.c.up = a.up.ptr, a.c.up_row_stride = a.up.stride;
+  return a;
+}
+
+std::tuple<at::Tensor, at::Tensor, Maybe> adapter_dense(const at::Tensor& x, const at::Tensor& w, const Maybe& bias, const at::Tensor& down,
+                                                        const at::Tensor& up, const Maybe& index, const Maybe& scale, double scale_all,
+                                                        const Maybe& residual, int64_t activation, bool gated, bool want_saved, const Maybe& out) {
+  const Layer l = layer_of(x, w, bias, activation, gated);
+  const c10::cuda::CUDAGuard guard(x.device());
+  Copies copies, low_copies;
+  const bool few = l.rows <= lib.dense_few_rows();
+  const Adapting a = adapters_of(x, l, w.size(0), down, up, index, scale, scale_all, few, low_copies);
+  const at::Tensor y = or_out(out, x, l.N);
+  if (residual) require_like("residual", *residual, x, y.sizes());
+  const int64_t low_pitch = 2 * pad8(a.c.rank), pitch = pad8(l.N) * (gated ? 2 : 1);
+  const at::Tensor low = empty({l.rows, low_pitch}, x.scalar_type(), x);
+  Maybe saved;
+  if (want_saved && lib.dense_keeps(int(activation), gated, l.K)) saved = empty({l.rows, pitch}, at::kFloat, x);
+  if (l.rows == 0) return {y, low, saved};
+  const Rows rx = operand(x, few, copies), rw = operand(w, few, copies), to = result_in(y);
+  Rows rr{};
+  if (residual) rr = operand(*residual, few, copies);
+  const Maybe b = bias ? Maybe(bias->contiguous()) : Maybe();
+  if (out) {
+    require_apart(to, "x", rx, y, x);
+    require_apart(to, "weight", rw, y, w);
+    require_apart(to, "bias", b, y);
+    require_apart(to, "down", a.down, y, down);
+    require_apart(to, "up", a.up, y, up);
+    if (index) require_apart(to, "index", Maybe(a.index), y);
+    if (scale) require_apart(to, "scale", Maybe(a.scale), y);
+    if (residual) require_apart(to, "residual", rr, y, *residual, true);
+  }
+  copies.make();
+  low_copies.make();
+  check(lib.adapter_dense(rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), residual ? rr.ptr : nullptr, rr.stride, to.ptr, to.stride,
+                          pointer(saved), pitch, &a.c, low.data_ptr(), l.dtype, int(activation), gated, l.rows, l.K, l.N, stream()),
+        "b200ta_adapter_dense");
+  return {y, low, saved};
+}
+
+std::tuple<Maybe, Maybe, Maybe, Maybe, Maybe> adapter_dense_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w, const Maybe& bias,
+                                                                     const at::Tensor& down, const at::Tensor& up, const Maybe& index,
+                                                                     const Maybe& scale, double scale_all, const at::Tensor& low, const Maybe& saved,
+                                                                     int64_t activation, bool gated, bool want_dx, bool want_dweight, bool want_dbias,
+                                                                     bool want_ddown, bool want_dup) {
+  const Layer l = layer_of(x, w, bias, activation, gated);
+  c10::SmallVector<int64_t, 8> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = l.N;
+  require_like("dy", dy, x, shape);
+  const int64_t pitch = pad8(l.N) * (gated ? 2 : 1);
+  const c10::cuda::CUDAGuard guard(x.device());
+  Copies copies, low_copies;
+  const Adapting a = adapters_of(x, l, w.size(0), down, up, index, scale, scale_all, false, low_copies);
+  const int64_t low_pitch = 2 * pad8(a.c.rank);
+  require_like("saved", low, x, {l.rows, low_pitch});
+  if (!low.is_contiguous()) refuse("saved must be what the forward pass returned");
+  if (saved) {
+    require_like("saved", *saved, x, {l.rows, pitch}, true);
+    if (!saved->is_contiguous() || saved->scalar_type() != at::kFloat) refuse("saved must be what the forward pass returned");
+  }
+  auto like = [&](bool want, const at::Tensor& t) { return want ? Maybe(empty(t.sizes(), t.scalar_type(), x)) : Maybe(); };
+  const Maybe dx = want_dx ? Maybe(empty_rows(x, l.K)) : Maybe(), dweight = like(want_dweight, w);
+  const Maybe dbias = want_dbias ? Maybe(empty({w.size(0)}, w.scalar_type(), x)) : Maybe(), ddown = like(want_ddown, down), dup = like(want_dup, up);
+  if (l.rows == 0) {
+    for (const Maybe* t : {&dweight, &dbias, &ddown, &dup})
+      if (*t) (*t)->zero_();
+    return {dx, dweight, dbias, ddown, dup};
+  }
+  const Rows rdy = operand(dy, false, copies), rx = operand(x, false, copies), rw = operand(w, false, copies);
+  copies.make();
+  low_copies.make();
+  const Maybe b = bias ? Maybe(bias->contiguous()) : Maybe();
+  const size_t need = lib.adapter_dense_backward_workspace_bytes(int(activation), gated, saved.has_value(), want_dbias, a.c.count, a.c.rank, l.rows,
+                                                                 l.K, l.N);
+  const at::Tensor workspace = bytes(x, need);
+  check(lib.adapter_dense_backward(rdy.ptr, rdy.stride, rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), pointer(saved), pitch, &a.c, low.data_ptr(),
+                                   pointer(dx), l.K, pointer(dweight), pointer(dbias), pointer(ddown), pointer(dup), workspace.data_ptr(),
+                                   need, l.dtype, int(activation), gated, l.rows, l.K, l.N, stream()),
+        "b200ta_adapter_dense_backward");
+  return {dx, dweight, dbias, ddown, dup};
+}
+
 // ---- dropout ----------------------------------------------------------------------------------------------------------
 
 at::Tensor dropout(const at::Tensor& x, int64_t dropped, uint64_t seed, uint64_t sequence, const Maybe& seed_at, const Maybe& residual,
@@ -355,6 +483,8 @@ void define_training(py::module_& m) {
   m.def("layer_norm_backward", &layer_norm_backward);
   m.def("dense", &dense);
   m.def("dense_backward", &dense_backward);
+  m.def("adapter_dense", &adapter_dense);
+  m.def("adapter_dense_backward", &adapter_dense_backward);
   m.def("dropout", &dropout);
 }
 

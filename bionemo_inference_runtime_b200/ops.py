@@ -562,6 +562,58 @@ def gated_dense_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor
                                            bias is not None if want_dbias is None else want_dbias)
 
 
+def _scale(scale) -> tuple:
+    return (scale, 1.0) if isinstance(scale, torch.Tensor) else (None, float(scale))
+
+
+def adapter_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, down: torch.Tensor, up: torch.Tensor,
+                  index: torch.Tensor | None = None, scale: float | torch.Tensor = 1.0, *, activation: str = "none",
+                  residual: torch.Tensor | None = None, want_saved: bool = False, out: torch.Tensor | None = None):
+    """:func:`dense` with low-rank adapters of many requests beside the shared weight:
+    ``activation(x @ weight.T + bias + scale[g] * (x @ down[g].T) @ up[g].T) + residual``.
+
+    ``down [adapters, rank, K]`` and ``up [adapters, N, rank]`` are in the dtype of ``x``, of ranks up to 256.  ``index`` (int32 or int64)
+    has the leading axes of ``x`` as its shape, one entry for each request or for each row; a row whose entry is none of
+    ``0 .. adapters - 1`` (-1, say) has no adapter.  Without an index all rows have the one adapter.  ``scale`` is a number or fp32,
+    one for each adapter.  Nothing of one request, infinities and NaN
+    among it, reaches another's rows.
+
+    With ``want_saved`` returns ``(y, saved)`` for :func:`adapter_dense_backward`.  Types, sizes, strides and ``out`` as for
+    :func:`dense`.
+    """
+    y, *saved = _host.adapter_dense(x, weight, bias, down, up, index, *_scale(scale), residual, _activation(activation), False, want_saved, out)
+    return (y, tuple(saved)) if want_saved else y
+
+
+def adapter_dense_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, down: torch.Tensor,
+                           up: torch.Tensor, index: torch.Tensor | None = None, scale: float | torch.Tensor = 1.0, *,
+                           activation: str = "none", saved: tuple, want_dx: bool = True, want_dweight: bool = False,
+                           want_dbias: bool = False, want_ddown: bool = True, want_dup: bool = True):
+    """``(dx, dweight, dbias, ddown, dup)`` of :func:`adapter_dense` (the gradient of its residual is ``dy``); ``saved`` is what the
+    forward pass returned.  The shared weight and bias are taken as frozen unless ``want_dweight`` and ``want_dbias`` say otherwise.
+    The gradient before the activation is rounded to the dtype of ``x`` between the kernels; sums over rows are in fp32 and in a fixed order, each adapter's over its own rows alone."""
+    return _host.adapter_dense_backward(dy, x, weight, bias, down, up, index, *_scale(scale), *saved, _activation(activation), False, want_dx,
+                                        want_dweight, want_dbias, want_ddown, want_dup)
+
+
+def adapter_gated_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, down: torch.Tensor, up: torch.Tensor,
+                        index: torch.Tensor | None = None, scale: float | torch.Tensor = 1.0, *, activation: str = "silu",
+                        want_saved: bool = False, out: torch.Tensor | None = None):
+    """:func:`gated_dense` with adapters (``up [adapters, 2 * hidden, rank]``): ``value * activation(gate)`` with
+    ``[value | gate] = x @ weight.T + bias + scale[g] * (x @ down[g].T) @ up[g].T``; see :func:`adapter_dense`."""
+    y, *saved = _host.adapter_dense(x, weight, bias, down, up, index, *_scale(scale), None, _activation(activation), True, want_saved, out)
+    return (y, tuple(saved)) if want_saved else y
+
+
+def adapter_gated_dense_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, down: torch.Tensor,
+                                 up: torch.Tensor, index: torch.Tensor | None = None, scale: float | torch.Tensor = 1.0, *,
+                                 activation: str = "silu", saved: tuple, want_dx: bool = True, want_dweight: bool = False,
+                                 want_dbias: bool = False, want_ddown: bool = True, want_dup: bool = True):
+    """``(dx, dweight, dbias, ddown, dup)`` of :func:`adapter_gated_dense`; see :func:`adapter_dense_backward`."""
+    return _host.adapter_dense_backward(dy, x, weight, bias, down, up, index, *_scale(scale), *saved, _activation(activation), True, want_dx,
+                                        want_dweight, want_dbias, want_ddown, want_dup)
+
+
 _WORD = (1 << 64) - 1
 
 

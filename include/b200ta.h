@@ -456,6 +456,37 @@ int b200ta_dense_backward(const void* dy, int64_t dy_row_stride, const void* x, 
                           int64_t dx_row_stride, void* dw, void* dbias, void* workspace, size_t workspace_bytes, int dtype,
                           int activation, int gated, int64_t rows, int K, int N, void* stream);
 
+/* The same layers with low-rank adapters of the rows' requests: x w^T + bias + low up_g^T before the activation, low = scale_g x down_g^T,
+ * where row r has the adapter g = index[r / rows_per_index]; rows whose index is none of 0 .. count - 1 have none.  down [count, rank, K] and up
+ * [count, N or 2 N, rank] lie with one row stride each; `scale` [count] on the device, or NULL for `scale_all`; index of 4 or 8 bytes an
+ * entry, or NULL for adapter 0 (of one) everywhere.  Ranks up to 256, up to 16383 adapters.  `low` [rows, 2, rank
+ * padded to 8] is written in `dtype` (second what the rounding of the first left out; padding included) and read again by the backward
+ * pass. */
+typedef struct {
+  const void *down, *up;
+  int64_t down_row_stride, up_row_stride;
+  const float* scale;
+  float scale_all;
+  const void* index;
+  int index_bytes;
+  int64_t rows_per_index;
+  int count, rank;
+} b200ta_adapters;
+int b200ta_adapter_dense(const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride, const void* bias, const void* residual,
+                         int64_t residual_row_stride, void* y, int64_t y_row_stride, void* saved, int64_t saved_row_stride,
+                         const b200ta_adapters* adapters, void* low, int dtype, int activation, int gated, int64_t rows,
+                         int K, int N, void* stream);
+
+/* Gradients of the same; ddown [count, rank, K] and dup [count, N or 2 N, rank] are dense and may be NULL.  dlow = scale_g dz up_g is held
+ * as low is, dz rounded to `dtype`. */
+size_t b200ta_adapter_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, int count, int rank, int64_t rows, int K,
+                                                     int N);
+int b200ta_adapter_dense_backward(const void* dy, int64_t dy_row_stride, const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride,
+                                  const void* bias, const void* saved, int64_t saved_row_stride, const b200ta_adapters* adapters, const void* low,
+                                  void* dx, int64_t dx_row_stride, void* dw, void* dbias, void* ddown, void* dup,
+                                  void* workspace, size_t workspace_bytes, int dtype, int activation, int gated, int64_t rows, int K, int N,
+                                  void* stream);
+
 /* dst[r, c] = src[r * row_stride + c * column_stride] for 16-bit elements: aligned copies of what the entry points above cannot
  * read as it lies, up to B200TA_COPIES of them in one launch.  dst is 16-byte aligned, its rows a multiple of 8 elements apart and
  * padded to 8 columns (the padding is written). */
