@@ -17,10 +17,10 @@ __device__ __forceinline__ uint4 load_eight_of(const T* row, int k, int K) {
 
 template <typename T>
 __device__ __forceinline__ void store_low(const LowProduct& p, long long row, int r, float v) {
-  T* low = static_cast<T*>(p.low) + row * (2 * padded_rank(p.rank)) + r;
+  T* low = static_cast<T*>(p.low) + row * low_pitch(p.rank) + low_place(p.rank, r);
   const T rounded = static_cast<T>(v);
   *low = rounded;
-  low[padded_rank(p.rank)] = static_cast<T>(v - static_cast<float>(rounded));
+  low[low_unit(p.rank)] = static_cast<T>(v - static_cast<float>(rounded));
 }
 
 // ---- low-rank values, a warp for each ------------------------------------------------------------------------------
@@ -35,13 +35,13 @@ low_dot_kernel(const LowProduct p, int groups) {
   pdl_trigger();
   const int lane = threadIdx.x & 31, r = int(blockIdx.x % unsigned(groups)) * kDotWarps + (threadIdx.x >> 5);
   const long long row = blockIdx.x / unsigned(groups);
-  if (r >= padded_rank(p.rank)) return;
+  if (r >= low_pitch(p.rank) / 2) return;
   const int g = adapter_of(p.index, uint32_t(row));
   float sum = 0.f;
   if (g != kNoAdapter && r < p.rank) {
     for (int plane = 0; plane < p.planes; ++plane) {
       const T* x = static_cast<const T*>(p.x) + row * p.xs + plane * p.x_plane;
-      const T* a = static_cast<const T*>(p.a) + ((long long)g * p.rank + r) * p.as + plane * p.a_plane;
+      const T* a = static_cast<const T*>(p.a) + ((long long)(g * p.planes + plane) * p.rank + r) * p.as;
       float2 s = make_float2(0.f, 0.f);
 #pragma unroll 4
       for (int k = lane * 8; k < p.K; k += 256) {
@@ -83,9 +83,10 @@ low_product_kernel(const LowProduct p, int share) {
   const int r0 = blockIdx.y * kRanks, first = share ? warp * 32 : 0, step = share ? kWarps * 32 : 32;
   if (row0 >= p.rows) return;  // (of a block whose warps share rows: all of them)
   TileAdapters<1> mine;
-  mine.load(p.index, row0, p.rows);
+  mine.fetch(p.index, int(row0), int(p.rows));
+  mine.arrived(p.index);
   auto store = [&](int row, int r, float v) {  // a value of this warp's rows
-    if (r < padded_rank(p.rank)) store_low<T>(p, row0 + row, r, r < p.rank ? v : 0.f);
+    if (r < low_pitch(p.rank) / 2) store_low<T>(p, row0 + row, r, r < p.rank ? v : 0.f);
   };
   // rows without an adapter
   for (int row = share ? warp : 0; row < kLowRows && row0 + row < p.rows; row += share ? kWarps : 1)
@@ -105,7 +106,7 @@ low_product_kernel(const LowProduct p, int share) {
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
         const int r = r0 + j * 8 + q;
-        a[j] = static_cast<const T*>(p.a) + ((long long)g * p.rank + (r < p.rank ? r : p.rank - 1)) * p.as + plane * p.a_plane;
+        a[j] = static_cast<const T*>(p.a) + ((long long)(g * p.planes + plane) * p.rank + (r < p.rank ? r : p.rank - 1)) * p.as;
       }
 #pragma unroll 2
       for (int k = first + t * 8; k - t * 8 < p.K; k += step) {
@@ -147,30 +148,32 @@ low_product_kernel(const LowProduct p, int share) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int row = i * 16 + q + 8 * h, r = r0 + j * 8 + t * 2;
-            if (!(own >> row & 1u) || r >= padded_rank(p.rank)) continue;  // (padded to a multiple of eight)
+            if (!(own >> row & 1u) || r >= low_pitch(p.rank) / 2) continue;
             const float v0 = r < p.rank ? acc[i][j][2 * h] * scale : 0.f, v1 = r + 1 < p.rank ? acc[i][j][2 * h + 1] * scale : 0.f;
-            T* to = static_cast<T*>(p.low) + (row0 + row) * (2 * padded_rank(p.rank)) + r;
+            T* to = static_cast<T*>(p.low) + (row0 + row) * low_pitch(p.rank) + low_place(p.rank, r);
             const uint32_t rounded = pack2<T>(v0, v1);
             const float2 f = unpack2<T>(rounded);
             *reinterpret_cast<uint32_t*>(to) = rounded;
-            *reinterpret_cast<uint32_t*>(to + padded_rank(p.rank)) = pack2<T>(v0 - f.x, v1 - f.y);
+            *reinterpret_cast<uint32_t*>(to + low_unit(p.rank)) = pack2<T>(v0 - f.x, v1 - f.y);
           }
     }
   }
 }
 
+// Each row's own adapter read for it alone, rather than a pass over the rows' k for each adapter among them.
+bool by_warps(const LowProduct& m) {
+  return m.rows <= 16 || (m.index.index != nullptr && m.index.count > 1 && m.index.rows_per_index < 8 && m.rows <= 4096);
+}
 template <typename T, bool kVec>
 int launch_low(DeviceState* st, const LowProduct& m, void* stream) {
-  // A pass over the rows' k for each adapter among 32 rows, or each row's own adapter read for it alone.
-  const bool own_warps = m.rows <= 16 || (m.index.index != nullptr && m.index.count > 1 && m.index.rows_per_index < 8 && m.rows <= 4096);
-  if (own_warps) {
-    const int groups = int((padded_rank(m.rank) + kDotWarps - 1) / kDotWarps);
+  if (by_warps(m)) {
+    const int groups = int((low_pitch(m.rank) / 2 + kDotWarps - 1) / kDotWarps);
     return launch_kernel(st, kKernelAdapter, low_dot_kernel<T, kVec>, dim3(unsigned(m.rows * groups)), kDotWarps * 32, 0, stream, m, groups);
   }
   const int tiles = m.rank <= 16 ? 2 : m.rank <= 32 ? 4 : 8, warps = low_warps(tiles);
   const int64_t groups = (m.rows + kLowRows - 1) / kLowRows;
   const int share = groups < int64_t(st->num_sms) * warps * 2 || m.K > 512;
-  const dim3 grid{unsigned(share ? groups : (groups + warps - 1) / warps), unsigned((m.rank + tiles * 8 - 1) / (tiles * 8))};
+  const dim3 grid{unsigned(share ? groups : (groups + warps - 1) / warps), unsigned((low_pitch(m.rank) / 2 + tiles * 8 - 1) / (tiles * 8))};
   auto* kernel = tiles == 2 ? low_product_kernel<T, 2, kVec> : tiles == 4 ? low_product_kernel<T, 4, kVec> : low_product_kernel<T, 8, kVec>;
   return launch_kernel(st, kKernelAdapter, kernel, grid, warps * 32, 0, stream, m, share);
 }
@@ -191,12 +194,12 @@ transpose_up_kernel(const TransposeParams p) {
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, n0 = blockIdx.x * 32, r0 = blockIdx.y * 32;
   const long long g = blockIdx.z / p.planes, plane = blockIdx.z % p.planes;
   const uint16_t* up = p.up + (g * p.planes + plane) * p.N * p.up_pitch;
-  uint16_t* out = p.out + (g * p.rank * p.planes + plane) * p.out_pitch;
+  uint16_t* out = p.out + (g * p.planes + plane) * p.rank * p.out_pitch;
   for (int i = y; i < 32; i += 8)
     if (n0 + i < p.N && r0 + x < p.rank) tile[i][x] = up[(n0 + i) * p.up_pitch + r0 + x];
   __syncthreads();
   for (int i = y; i < 32; i += 8)
-    if (r0 + i < p.rank && n0 + x < p.N) out[(long long)(r0 + i) * p.planes * p.out_pitch + n0 + x] = tile[x][i];
+    if (r0 + i < p.rank && n0 + x < p.N) out[(long long)(r0 + i) * p.out_pitch + n0 + x] = tile[x][i];
 }
 
 // ---- gradients of the adapters' weights ---------------------------------------------------------------------------------
@@ -208,7 +211,7 @@ transpose_up_kernel(const TransposeParams p) {
 // and are transposed on their way from shared memory.  Of several adapters a block first lists the groups of 64 rows that hold
 // its own.  Parts are written in 32 bits and joined in a fixed order: results repeat bit by bit.
 constexpr int kGradRows = 64, kGradColumns = 128, kGradChunks = 1024;
-// (a block of up to 16, 32 or 64 ranks has its two terms beside each other in a row of 64, 128 or 256 bytes)
+// (up to 16, 32 or 64 ranks with their two terms are a row of 64, 128 or 256 bytes)
 constexpr int kGradV = kGradRows * kGradColumns * 2;
 __host__ __device__ constexpr int grad_stage(int tiles) { return kGradV + kGradRows * tiles * 64; }
 __host__ __device__ constexpr int grad_stages(int tiles) { return tiles == 4 ? 3 : 4; }
@@ -231,23 +234,24 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t addr, uint32_t (&r)[4]) {
 template <typename T, int kTiles>  // tiles of 16 ranks
 __global__ void __launch_bounds__(256, 2)
 low_grad_kernel(const GradParams p) {
-  constexpr int kStages = grad_stages(kTiles), kStage = grad_stage(kTiles), kTermVecs = kTiles * 2, kRowVecs = 2 * kTermVecs;
+  constexpr int kStages = grad_stages(kTiles), kStage = grad_stage(kTiles), kRowVecs = 4 * kTiles;
   extern __shared__ __align__(128) uint8_t stages[];
   __shared__ uint32_t masks[kGradChunks][2];
   __shared__ uint16_t list[kGradChunks];
   __shared__ int listed;
   pdl_trigger();
   pdl_wait();
-  const bool second = int(blockIdx.y) >= p.slabs0;
+  const bool second = int(blockIdx.x) >= p.slabs0;
   const LowGrad& job = second ? p.job[1] : p.job[0];
-  const int slab = int(blockIdx.y) - (second ? p.slabs0 : 0), slabs_plane = (job.columns + kGradColumns - 1) / kGradColumns;
+  const int slab = int(blockIdx.x) - (second ? p.slabs0 : 0), slabs_plane = (job.columns + kGradColumns - 1) / kGradColumns;
   const int plane = slab / slabs_plane, c0 = (slab - plane * slabs_plane) * kGradColumns;
   const int g = blockIdx.z / p.rank_groups, r0 = int(blockIdx.z % unsigned(p.rank_groups)) * 64;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long first_row = (long long)blockIdx.x * p.chunks_part * kGradRows;
+  const long long first_row = (long long)blockIdx.y * p.chunks_part * kGradRows;
   const long long rows = p.rows - first_row < (long long)p.chunks_part * kGradRows ? p.rows - first_row : (long long)p.chunks_part * kGradRows;
   const int chunks = rows > 0 ? int((rows + kGradRows - 1) / kGradRows) : 0;
 
+#pragma unroll 4
   for (int c = warp; c < chunks; c += 8) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -271,13 +275,11 @@ low_grad_kernel(const GradParams p) {
   const int count = listed;
 
   const T* v = static_cast<const T*>(job.v) + plane * job.v_plane + c0;
-  const T* t = static_cast<const T*>(job.t) + r0;
+  const T* t = static_cast<const T*>(job.t) + r0 * 2;
   const uint32_t base = smem_u32(stages);
   const int v_column = (threadIdx.x & 15) * 8, v_bytes = max(0, min(16, (job.columns - c0 - v_column) * 2));
-  // vector threadIdx.x % kRowVecs of a row of t: first the first terms, then the second ones
-  const int t_vec = threadIdx.x % kRowVecs, t_column = t_vec % kTermVecs * 8;
-  const bool t_in = r0 + t_column < p.rank;  // (its padding to eight ranks is zeros)
-  const int t_from = t_column + (t_vec >= kTermVecs ? padded_rank(p.rank) : 0);
+  const int t_vec = threadIdx.x % kRowVecs, pitch_t = low_pitch(p.rank);
+  const bool t_in = r0 * 2 + t_vec * 8 < pitch_t;
   // (rows of 64 bytes: two of them to the 128 that the banks span)
   auto t_at = [&](int row, int vec) { return kGradV + row * kRowVecs * 16 + ((kTiles == 1 ? vec ^ (row >> 1 & 3) : vec ^ (row & 7)) << 4); };
   auto issue = [&](int i) {
@@ -295,7 +297,7 @@ low_grad_kernel(const GradParams p) {
 #pragma unroll
       for (int row = threadIdx.x / kRowVecs; row < kGradRows; row += 256 / kRowVecs) {
         const bool own = t_in && (masks[c][row >> 5] >> (row & 31) & 1u);
-        const T* from = own ? t + (first_row + c * kGradRows + row) * (2 * padded_rank(p.rank)) + t_from : static_cast<const T*>(job.t);
+        const T* from = own ? t + (first_row + c * kGradRows + row) * pitch_t + t_vec * 8 : static_cast<const T*>(job.t);
         copy_or_zero(stage + t_at(row, t_vec), from, own ? 16 : 0);
       }
     }
@@ -314,19 +316,20 @@ low_grad_kernel(const GradParams p) {
       uint32_t b[4];
       ldmatrix4_t(stage + vr * 256 + ((vc ^ (vr & 7)) << 4), b);
 #pragma unroll
-      for (int m = 0; m < 2 * kTiles; ++m) {
-        const int tr = k + (lane >> 4) * 8 + (lane & 7);
+      for (int m = 0; m < 2 * kTiles; ++m) {  // tiles of a block's first, then of its second terms
+        constexpr int kBlock = kTiles == 1 ? 1 : 2;
+        const int tr = k + (lane >> 4) * 8 + (lane & 7), tile = m / (2 * kBlock) * kBlock + m % kBlock;
         uint32_t a[4];
         ldmatrix4_t(stage + t_at(tr, m * 2 + (lane >> 3 & 1)), a);
-        mma16816<T>(acc[m % kTiles][0], a[0], a[1], a[2], a[3], b[0], b[1]);
-        mma16816<T>(acc[m % kTiles][1], a[0], a[1], a[2], a[3], b[2], b[3]);
+        mma16816<T>(acc[tile][0], a[0], a[1], a[2], a[3], b[0], b[1]);
+        mma16816<T>(acc[tile][1], a[0], a[1], a[2], a[3], b[2], b[3]);
       }
     }
   }
   norm::copy_wait<0>();
   const long long pitch = low_grad_columns(job.columns, job.planes), plane_columns = pitch / job.planes;
   const int adapters = gridDim.z / p.rank_groups;
-  float* part = job.part + ((long long)blockIdx.x * adapters + g) * p.rank * pitch + plane * plane_columns;
+  float* part = job.part + ((long long)blockIdx.y * adapters + g) * p.rank * pitch + plane * plane_columns;
 #pragma unroll
   for (int m = 0; m < kTiles; ++m)
 #pragma unroll
@@ -347,17 +350,23 @@ int launch_grad(DeviceState* st, dim3 grid, void* stream, const GradParams& p) {
                        stream, p);
 }
 
+// Sums over the parts: a thread takes one value, or eight ranks of a column whose results lie together, of every kSlices-th part; the
+// threads of an item are in different warps.
 struct LowJoinParams {
   LowGrad job[2];
   int rank, parts, adapters;
-  long long items0, items;  // of the first job, of both; an item is one value, or eight ranks of one column of a transposed result
+  long long items0, items;  // of the first job, of both
 };
-template <typename T>
+template <typename T, int kSlices>
 __global__ void __launch_bounds__(256)
 low_join_kernel(const LowJoinParams p) {
+  constexpr int kItems = 256 / kSlices;
+  __shared__ float joined[kSlices > 1 ? kSlices - 1 : 1][8][kItems];
   pdl_trigger();
   pdl_wait();
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < p.items; i += gridDim.x * 256LL) {
+  const int own = threadIdx.x % kItems, slice = threadIdx.x / kItems;
+  for (long long first = (long long)blockIdx.x * kItems; first < p.items; first += (long long)gridDim.x * kItems) {
+    const long long i = first + own;
     const bool second = i >= p.items0;
     const LowGrad& job = second ? p.job[1] : p.job[0];
     long long at = second ? i - p.items0 : i;
@@ -370,23 +379,42 @@ low_join_kernel(const LowJoinParams p) {
     const float* part = job.part + (g * p.rank + r0) * pitch + plane * plane_columns + (column - plane * job.columns);
     float sum[8] = {};
     const int n = p.rank - r0 < ranks ? p.rank - r0 : ranks;
-    if (job.transposed) {
-      for (int s = 0; s < p.parts; ++s)
+    if (i < p.items) {
+      if (job.transposed) {
+#pragma unroll 2
+        for (int s = slice; s < p.parts; s += kSlices)
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (r < n) sum[r] += __ldg(part + s * stride + r * pitch);
-      T* out = static_cast<T*>(job.out) + (g * all + column) * p.rank + r0;
-      if (n == 8 && p.rank % 8 == 0 && (reinterpret_cast<uintptr_t>(job.out) & 15u) == 0) {
-        *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]), pack2<T>(sum[4], sum[5]), pack2<T>(sum[6], sum[7]));
+          for (int r = 0; r < 8; ++r)
+            if (r < n) sum[r] += __ldg(part + s * stride + r * pitch);
       } else {
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (r < n) out[r] = static_cast<T>(sum[r]);
-      }
-    } else {
 #pragma unroll 8
-      for (int s = 0; s < p.parts; ++s) sum[0] += __ldg(part + s * stride);
+        for (int s = slice; s < p.parts; s += kSlices) sum[0] += __ldg(part + s * stride);
+      }
+    }
+    if constexpr (kSlices > 1) {
+      if (slice > 0)
+#pragma unroll
+        for (int r = 0; r < 8; ++r) joined[slice - 1][r][own] = sum[r];
+      __syncthreads();
+      if (slice == 0)
+#pragma unroll
+        for (int s = 0; s < kSlices - 1; ++s)
+#pragma unroll
+          for (int r = 0; r < 8; ++r) sum[r] += joined[s][r][own];
+      __syncthreads();
+    }
+    if (slice > 0 || i >= p.items) continue;
+    if (!job.transposed) {
       static_cast<T*>(job.out)[(g * p.rank + r0) * all + column] = static_cast<T>(sum[0]);
+      continue;
+    }
+    T* out = static_cast<T*>(job.out) + (g * all + column) * p.rank + r0;
+    if (n == 8 && p.rank % 8 == 0 && (reinterpret_cast<uintptr_t>(job.out) & 15u) == 0) {
+      *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]), pack2<T>(sum[4], sum[5]), pack2<T>(sum[6], sum[7]));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < n) out[r] = static_cast<T>(sum[r]);
     }
   }
 }
@@ -397,6 +425,7 @@ int run_low(const LowProduct& m, void* stream) {
   DeviceState* st = nullptr;
   const int rc = get_device_state(&st);
   if (rc != B200TA_OK) return rc;
+  if (m.rows > 512 && !by_warps(m)) return run_matmul_low(m, stream);
   if (m.f16) return m.aligned ? launch_low<__half, true>(st, m, stream) : launch_low<__half, false>(st, m, stream);
   return m.aligned ? launch_low<__nv_bfloat16, true>(st, m, stream) : launch_low<__nv_bfloat16, false>(st, m, stream);
 }
@@ -410,11 +439,11 @@ int run_transpose_up(const void* up, int64_t up_pitch, void* out, int64_t out_pi
                        0, stream, p);
 }
 
-// Parts of the rows: two waves of two blocks on each multiprocessor if all adapters have their share of the rows, more (rows may be of
+// Parts of the rows: one wave of two blocks on each multiprocessor if all adapters have their share of the rows, more (rows may be of
 // few of them) as long as the parts stay below 32 MiB.
 int low_grad_parts(int64_t rows, int64_t columns, int count, int rank, int num_sms) {
   const int64_t chunks = (rows + kGradRows - 1) / kGradRows, slabs = (columns + kGradColumns - 1) / kGradColumns * ((rank + 63) / 64);
-  const int64_t wanted = (int64_t(num_sms) * 4 + slabs - 1) / slabs, shared = (wanted + count - 1) / count;
+  const int64_t wanted = std::max<int64_t>(int64_t(num_sms) * 2 / slabs, 1), shared = std::max<int64_t>(int64_t(num_sms) * 2 / (slabs * count), 1);
   const int64_t by_bytes = (int64_t(1) << 25) / (int64_t(count) * rank * columns * 4);
   const int64_t parts = std::max(std::min(std::max(shared, std::min(wanted, by_bytes)), (chunks + 3) / 4), (chunks + kGradChunks - 1) / kGradChunks);
   const int64_t per = (chunks + parts - 1) / parts;
@@ -432,7 +461,8 @@ int run_low_grads(const LowGrads& m, void* stream) {
   const int64_t chunks = (m.rows + kGradRows - 1) / kGradRows;
   p.chunks_part = int((chunks + m.parts - 1) / m.parts);
   B200TA_REQUIRE(p.chunks_part <= kGradChunks, "adapters: too many rows for %d parts", m.parts);
-  const dim3 grid{unsigned(m.parts), unsigned(p.slabs0 + slabs_of(m.job[1])), unsigned(m.index.count * p.rank_groups)};
+  // (all columns of a part's rows at a time: memory is read in whole rows)
+  const dim3 grid{unsigned(p.slabs0 + slabs_of(m.job[1])), unsigned(m.parts), unsigned(m.index.count * p.rank_groups)};
   const int tiles = m.rank <= 16 ? 1 : m.rank <= 32 ? 2 : 4;
   int (*launch)(DeviceState*, dim3, void*, const GradParams&);
   if (m.f16) launch = tiles == 1 ? launch_grad<__half, 1> : tiles == 2 ? launch_grad<__half, 2> : launch_grad<__half, 4>;
@@ -450,8 +480,12 @@ int run_low_join(const LowGrads& m, void* stream) {
   };
   p.job[0] = m.job[0], p.job[1] = m.job[1], p.rank = m.rank, p.parts = m.parts, p.adapters = m.index.count;
   p.items0 = items_of(m.job[0]), p.items = p.items0 + items_of(m.job[1]);
-  const int64_t blocks = std::min<int64_t>((p.items + 255) / 256, int64_t(st->num_sms) * 16);
-  return launch_kernel(st, kKernelAdapter, m.f16 ? low_join_kernel<__half> : low_join_kernel<__nv_bfloat16>, dim3(unsigned(blocks)), 256, 0, stream, p);
+  // several threads to an item where there are many parts of few values
+  const bool sliced = m.parts >= 4 && p.items < int64_t(st->num_sms) * 256;
+  const int64_t each = sliced ? 32 : 256, blocks = std::min<int64_t>((p.items + each - 1) / each, int64_t(st->num_sms) * 16);
+  auto* kernel = m.f16 ? (sliced ? low_join_kernel<__half, 8> : low_join_kernel<__half, 1>)
+                       : (sliced ? low_join_kernel<__nv_bfloat16, 8> : low_join_kernel<__nv_bfloat16, 1>);
+  return launch_kernel(st, kKernelAdapter, kernel, dim3(unsigned(blocks)), 256, 0, stream, p);
 }
 
 }  // namespace b200ta

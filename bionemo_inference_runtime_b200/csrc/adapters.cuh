@@ -17,13 +17,26 @@ struct AdapterIndex {
   const void* index;
   int bytes;
   uint32_t rows_per_index, first_row;
+  uint32_t factor, shift;  // n / rows_per_index = n * factor >> shift for all n below 2^31
   int count;
 };
+inline AdapterIndex adapter_index(const void* index, int bytes, int64_t rows_per_index, int count) {
+  const uint64_t d = rows_per_index < 1 ? 1 : rows_per_index > (int64_t(1) << 31) ? uint64_t(1) << 31 : uint64_t(rows_per_index);
+  uint32_t s = 0;
+  while ((uint64_t(1) << s) < d) ++s;
+  // 2^(31 + s) / d, rounded up: what is added to it, times n, stays below 2^(31 + s)
+  return {index, bytes, uint32_t(d), 0, uint32_t(((uint64_t(1) << (31 + s)) + d - 1) / d), 31 + s, count};
+}
 constexpr int kNoAdapter = 0x7FFFFFFF;
 constexpr int kMaxRank = 256;
-__host__ __device__ constexpr int padded_rank(int rank) { return (rank + 7) / 8 * 8; }
+// How low-rank values lie: a row has blocks of 16 or 32 ranks, of each its first and then its second terms (64 or 128 bytes: a tensor
+// copy takes as long for a row of 32 bytes as for one of 128), zeros behind the last rank.
+__host__ __device__ constexpr int low_unit(int rank) { return rank <= 16 ? 16 : 32; }
+__host__ __device__ constexpr int low_blocks(int rank) { return (rank + low_unit(rank) - 1) / low_unit(rank); }
+__host__ __device__ constexpr int low_pitch(int rank) { return 2 * low_unit(rank) * low_blocks(rank); }
+__host__ __device__ constexpr int low_place(int rank, int r) { return r / low_unit(rank) * 2 * low_unit(rank) + r % low_unit(rank); }
 
-// An adapter's part of a product: low [rows][2][pad8(rank)] in 16 bits; high [count][planes of columns][rank], or [count][rank][columns] for a
+// An adapter's part of a product: low [rows][low_pitch] in 16 bits; high [count][planes of columns][rank], or [count][rank][columns] for a
 // product whose right operand has its rows along k.
 struct LowRank {
   AdapterIndex index;
@@ -33,24 +46,24 @@ struct LowRank {
   int64_t high_pitch;
 };
 
-// low[row][0][0 .. pad8(rank)) = scale[g] * sum over planes and k of x[row][plane][k] a[g][r][plane][k], zeros where there is no adapter and
-// behind the last rank; low[row][1] is what the rounding of low[row][0] left out.
+// low[row][r] = scale[g] * sum over planes and k of x[row][plane][k] a[g][plane][r][k], in two terms; zeros where there is no adapter.
 struct LowProduct {
   const void *x, *a;
   void* low;
-  const float* scale;  // per adapter on the device, or NULL:
+  const float* scale;  // of each adapter, on the device, or NULL: scale_all
   float scale_all;
-  long long xs, x_plane, as, a_plane, rows;  // adapter g begins at row g * rank of a
+  long long xs, x_plane, as, rows;
   int K, planes, rank;
   bool f16, aligned;  // aligned: 16-byte rows
   AdapterIndex index;
 };
 int run_low(const LowProduct& m, void* stream);
+int run_matmul_low(const LowProduct& m, void* stream);  // of it: on the tensor cores (dense.cu)
 
-// up [count][columns (two planes of N)][rank] as [count][rank][planes][pitch], for dz U.
+// up [count][columns (two planes of N)][rank] as [count][planes][rank][pitch], for dz U.
 int run_transpose_up(const void* up, int64_t up_pitch, void* out, int64_t out_pitch, int count, int rank, int N, int planes, void* stream);
 
-// part[p][g][r][column] (+)= sum over the rows of part p that have adapter g of (t[row][0][r] + t[row][1][r]) v[row][column], for one or two such sums, in
+// part[p][g][r][column] (+)= sum over the rows of part p that have adapter g of t[row][r] (both terms) v[row][column], for one or two such sums, in
 // 32 bits; then the parts joined, in their order, to [count][rank][columns] or (transposed) [count][columns][rank] in 16 bits.
 struct LowGrad {
   const void *t, *v;  // v NULL: not wanted
@@ -74,34 +87,71 @@ int run_low_join(const LowGrads& m, void* stream);
 
 #ifdef __CUDACC__
 // (Past the first-level cache: a kernel that starts beside the one before it reads what was complete before both.)
-__device__ __forceinline__ int adapter_of(const AdapterIndex& x, uint32_t row) {
-  if (x.index == nullptr) return 0;
-  const uint32_t i = (x.first_row + row) / x.rows_per_index;
-  const long long g = x.bytes == 8 ? __ldcg(static_cast<const long long*>(x.index) + i) : (long long)__ldcg(static_cast<const int*>(x.index) + i);
-  return g >= 0 && g < x.count ? int(g) : kNoAdapter;
+__device__ __forceinline__ long long index_entry(const AdapterIndex& x, uint32_t row) {
+  const uint32_t i = uint32_t(uint64_t(x.first_row + row) * x.factor >> x.shift);
+  return x.bytes == 8 ? __ldcg(static_cast<const long long*>(x.index) + i) : (long long)__ldcg(static_cast<const int*>(x.index) + i);
 }
-// The adapters of 32 * kWords rows, which a warp walks in ascending order: lane l has those of rows 32 j + l.
+__device__ __forceinline__ int adapter_of_entry(const AdapterIndex& x, long long entry) {
+  return entry >= 0 && entry < x.count ? int(entry) : kNoAdapter;
+}
+__device__ __forceinline__ int adapter_of(const AdapterIndex& x, uint32_t row) {
+  return x.index == nullptr ? 0 : adapter_of_entry(x, index_entry(x, row));
+}
+// The adapters of 32 * kWords rows, which a warp walks in ascending order: of rows that share an entry the one, of others lane l has
+// those of rows 32 j + l.  fetch() starts the loads, arrived() waits for them.  (The usual case is short: the warps that call this
+// share their issue slots with sixteen others.)
 template <int kWords>
 struct TileAdapters {
+  long long entry[kWords];
   int g[kWords];
-  __device__ __forceinline__ void load(const AdapterIndex& x, long long row0, long long rows) {
-    const int lane = threadIdx.x & 31;
+  uint32_t behind;  // bit j: this lane's row 32 j + l is behind the last one
+  bool same, next_same;
+  __device__ __forceinline__ void fetch(const AdapterIndex& x, int row0, int rows) {
+    next_same = true;
+    if (x.index == nullptr) return;
+    const uint32_t first = uint32_t(row0), last = uint32_t(min(row0 + 32 * kWords, rows) - 1);
+    next_same = (uint64_t(x.first_row + first) * x.factor >> x.shift) == (uint64_t(x.first_row + last) * x.factor >> x.shift);
+    if (next_same) {
+      entry[0] = index_entry(x, first);
+      return;
+    }
+    behind = 0;
 #pragma unroll
     for (int j = 0; j < kWords; ++j) {
-      const long long row = row0 + j * 32 + lane;
-      g[j] = row < rows ? adapter_of(x, uint32_t(row)) : kNoAdapter;
+      const int row = row0 + j * 32 + int(threadIdx.x & 31);
+      const bool in = row < rows;
+      entry[j] = in ? index_entry(x, uint32_t(row)) : -1;
+      behind |= in ? 0u : 1u << j;
     }
+  }
+  __device__ __forceinline__ void arrived(const AdapterIndex& x) {
+    same = next_same;
+    if (same) {
+      g[0] = x.index == nullptr ? 0 : adapter_of_entry(x, entry[0]);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) g[j] = adapter_of_entry(x, entry[j]);
   }
   // The first adapter behind `last` (-1: the first of all), kNoAdapter where there is none.
   __device__ __forceinline__ int next(int last) const {
+    if (same) return last < 0 ? g[0] : kNoAdapter;
     int least = kNoAdapter;
 #pragma unroll
     for (int j = 0; j < kWords; ++j)
       if (g[j] > last && g[j] < least) least = g[j];
     return int(__reduce_min_sync(0xffffffffu, unsigned(least)));
   }
+  // Whether no row has another adapter than a, or none.
+  __device__ __forceinline__ bool all_have(int a) const {
+    if (same) return true;
+    bool all = true;
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) all &= g[j] == a || behind >> j & 1;
+    return __all_sync(0xffffffffu, all);
+  }
   // Bit l: row 32 j + l has adapter a.
-  __device__ __forceinline__ uint32_t rows_of(int j, int a) const { return __ballot_sync(0xffffffffu, g[j] == a); }
+  __device__ __forceinline__ uint32_t rows_of(int j, int a) const { return same ? (a == g[0] ? ~0u : 0u) : __ballot_sync(0xffffffffu, g[j] == a); }
 };
 #endif
 

@@ -53,7 +53,8 @@ enum KernelId {
   kKernelMatmul = kKernelNarrow + 4,  // and one for each of the matmul kernels after it
   kKernelDropout = kKernelMatmul + 32, kKernelAdapter,
   kKernelMatmulAdapters = 64,                        // and one for each of the matmul kernels with adapters after it
-  kKernelLowGrad = kKernelMatmulAdapters + 32        // six
+  kKernelMatmulLow = kKernelMatmulAdapters + 32,     // two
+  kKernelLowGrad = kKernelMatmulLow + 2              // six
 };
 int get_device_state(DeviceState** out);
 

@@ -32,7 +32,8 @@ struct TilingOf {
   bool a_mn, sums;  // sums of A over k: tiles of up to 128 columns
   int64_t rows, outer, columns;
   int kblocks, splits;
-  double more = 0;  // blocks along k that adapters add to a tile, as parts of whole ones
+  double more = 0;  // blocks along k that adapters add to a tile
+  bool held = false;  // whether they may have room of their own
 };
 Tiling choose_tiling(const TilingOf& m, int num_sms) {
   const bool two = m.form == kGated || m.form == kGatedGrad;
@@ -50,9 +51,9 @@ Tiling choose_tiling(const TilingOf& m, int num_sms) {
     if (n > 64 && n / 2 >= accumulated) continue;
     const int64_t tiles_n = (accumulated + n - 1) / n;
     const double mma = 4.0 * std::max(40.0, n * 0.54);
-    if (!m.a_mn && m.splits == 1 && m.more == 0 && m.kblocks * n * matmul::kBK * 2 <= matmul::kResidentBytes && tiles_n <= num_sms) {
+    if (!m.a_mn && m.splits == 1 && (m.more == 0 || m.held) && m.kblocks * n * matmul::kBK * 2 <= matmul::kResidentBytes && tiles_n <= num_sms) {
       const int64_t lanes = std::min(tiles_m, num_sms / tiles_n);
-      consider(n, 0, int(lanes), waves_of(tiles_m, lanes), m.kblocks * std::max(mma, 356.0));
+      consider(n, 0, int(lanes), waves_of(tiles_m, lanes), m.kblocks * std::max(mma, 356.0) + m.more * 400);
     } else {
       const double load = (n == 256 ? 1.2 : 1.0) * (16384 + n * 128) / 46;
       consider(n, 0, 0, waves_of(tiles_m * tiles_n * m.splits, num_sms), kblocks * std::max(mma, load));
@@ -66,13 +67,9 @@ Tiling choose_tiling(const TilingOf& m, int num_sms) {
   return best;
 }
 
-// Ranks of a block along k, in rows of 32 or 64 bytes (a stage has room for two terms of the latter).
-int low_unit(int rank) { return rank <= 16 ? 16 : 32; }
-double low_blocks(const LowRank* a) {
-  if (a == nullptr) return 0;
-  const int unit = low_unit(a->rank);
-  const int64_t requests = a->index.index == nullptr ? 1 : 128 / int64_t(a->index.rows_per_index) + 1;
-  return double(std::min<int64_t>(a->index.count, requests)) * ((a->rank + unit - 1) / unit) * unit / 64;
+// Adapters that a tile of 128 rows is expected to have.
+double low_requests(const LowRank& a) {
+  return double(std::min<int64_t>(a.index.count, a.index.index == nullptr ? 1 : 127 / int64_t(a.index.rows_per_index) + 1));
 }
 
 }  // namespace
@@ -93,7 +90,9 @@ int run_matmul(const Matmul& m, void* stream) {
   p.splits = (p.kblocks + p.kblocks_split - 1) / p.kblocks_split;
   p.rows_inner = int(rows), p.columns = int(columns);
   const Tiling tiling =
-      choose_tiling({m.form, m.a_mn, m.sums != nullptr, rows, m_outer, columns, p.kblocks_split, p.splits, low_blocks(m.adapters)}, st->num_sms);
+      choose_tiling({m.form, m.a_mn, m.sums != nullptr, rows, m_outer, columns, p.kblocks_split, p.splits, m.adapters == nullptr ? 0 : low_requests(*m.adapters) * low_blocks(m.adapters->rank),
+                     m.adapters != nullptr && low_blocks(m.adapters->rank) == 1},
+                    st->num_sms);
   p.tile_n = tiling.tile_n, p.pair = tiling.pair, p.resident = tiling.resident;
   const int tile_m = p.pair ? 2 * matmul::kBM : matmul::kBM;
   p.tiles_m_inner = int((rows + tile_m - 1) / tile_m);
@@ -105,8 +104,9 @@ int run_matmul(const Matmul& m, void* stream) {
   p.work = int(work);
   p.group_m = p.pair ? 8 : 16;
   const int b_rows = p.pair ? p.tile_n / 2 : p.tile_n;
-  p.stages = p.resident ? (matmul::kRingBytes - matmul::kResidentBytes) / matmul::kABytes
-                        : matmul::kRingBytes / (matmul::kABytes + b_rows * matmul::kBK * 2);
+  const bool held = m.adapters != nullptr && low_blocks(m.adapters->rank) == 1 && (p.resident || low_requests(*m.adapters) >= 4);
+  const int ring = matmul::kRingBytes - (held ? matmul::held_bytes(low_unit(m.adapters->rank)) : 0);
+  p.stages = p.resident ? (ring - matmul::kResidentBytes) / matmul::kABytes : ring / (matmul::kABytes + b_rows * matmul::kBK * 2);
   if (p.stages > matmul::kMaxStages) p.stages = matmul::kMaxStages;
   p.bias = m.bias;
   p.activation = m.activation;
@@ -149,16 +149,46 @@ int run_matmul(const Matmul& m, void* stream) {
   if (m.adapters == nullptr) return launch(NoAdapters{});
   const LowRank& a = *m.adapters;
   MatmulAdapters x{};
-  x.index = a.index, x.rank = a.rank, x.unit = low_unit(a.rank), x.blocks = (a.rank + x.unit - 1) / x.unit;
+  x.index = a.index, x.rank = a.rank, x.unit = low_unit(a.rank), x.blocks = low_blocks(a.rank), x.held = held;
+  x.slots = std::min(matmul::kHighSlots, matmul::held_bytes(x.unit) / (b_rows * x.unit * 2));
   const SwizzleMode swizzle = x.unit == 32 ? SWZ_64 : SWZ_32;
-  const Plane low{a.low, rows, a.rank, 2 * padded_rank(a.rank), 2, padded_rank(a.rank)};
-  if ((rc = map_of(&x.low, low, 2, uint32_t(x.unit), matmul::kBM, 2, swizzle, m.what)) != B200TA_OK) return rc;
+  const Plane low{a.low, rows, low_pitch(a.rank), low_pitch(a.rank)};
+  if ((rc = map_of(&x.low, low, 2, uint32_t(2 * x.unit), matmul::kBM, 1, x.unit == 32 ? SWZ_128 : SWZ_64, m.what)) != B200TA_OK) return rc;
   const Plane high = m.b_mn ? Plane{a.high, a.rank, columns, a.high_pitch, a.index.count, a.rank * a.high_pitch}
                             : Plane{a.high, columns, a.rank, a.high_pitch, a.index.count * (two ? 2 : 1), columns * a.high_pitch};
   rc = m.b_mn ? map_of(&x.high, high, 2, 64, uint32_t(x.unit), 1, SWZ_128, m.what)
               : map_of(&x.high, high, 2, uint32_t(x.unit), uint32_t(p.pair || !two ? b_rows : units), two && !p.pair ? 2 : 1, swizzle, m.what);
   if (rc != B200TA_OK) return rc;
   return launch(x);
+}
+
+// Low-rank values of many rows on the tensor cores: tiles of 128 rows and all ranks.
+int run_matmul_low(const LowProduct& q, void* stream) {
+  DeviceState* st = nullptr;
+  int rc = get_device_state(&st);
+  if (rc != B200TA_OK) return rc;
+  const char* what = "adapters";
+  Matmul m;
+  m.form = kLow, m.f16 = q.f16, m.what = what;
+  MatmulParams p{};
+  p.tile_n = low_pitch(q.rank) / 2;
+  p.kblocks_inner = (q.K + matmul::kBK - 1) / matmul::kBK, p.kblocks = p.kblocks_split = p.kblocks_inner * q.planes;
+  p.splits = 1, p.rows_inner = int(q.rows), p.columns = p.tile_n;
+  p.tiles_m = p.tiles_m_inner = p.work = int((q.rows + matmul::kBM - 1) / matmul::kBM), p.tiles_n = 1, p.group_m = 16;
+  p.stages = std::min(matmul::kRingBytes / (matmul::kABytes + p.tile_n * matmul::kBK * 2), matmul::kMaxStages);
+  p.status = st->status_dev;
+  p.beside = kBesideFirst;
+  const int grid = std::min(p.work, st->num_sms);
+  p.buffers = p.tile_n <= 128 ? 2 : 1;
+  p.sets = p.work <= grid ? 0 : std::min(p.tile_n <= 16 ? 2 : 1, p.buffers);
+  MatmulMaps maps{};
+  if ((rc = map_of(&maps.a, {q.x, q.rows, q.K, q.xs, q.planes, q.x_plane}, 2, 64, matmul::kBM, 1, SWZ_128, what)) != B200TA_OK) return rc;
+  const Plane a{q.a, q.rank, q.K, q.as, q.index.count * q.planes, q.rank * q.as};
+  if ((rc = map_of(&maps.b, a, 2, 64, uint32_t(p.tile_n), 1, SWZ_128, what)) != B200TA_OK) return rc;
+  MatmulAdapters x{};
+  x.index = q.index, x.rank = q.rank, x.unit = low_unit(q.rank), x.blocks = low_blocks(q.rank);
+  x.scale = q.scale, x.scale_all = q.scale_all, x.low_out = q.low;
+  return launch_matmul_low(st, m, maps, p, x, grid, stream);
 }
 
 namespace {
@@ -214,21 +244,25 @@ __device__ __forceinline__ uint4 load_row(const T* row, int k, int K) {
 }
 
 constexpr int kFewWarps = 16, kFewColumns = 16;  // of a block, at most
-// The sum of (low[r] + low2[r]) high[r] over the ranks.
+// The sum of low[r] (both terms) high[r] over the ranks.
 template <typename T>
-__device__ __forceinline__ float low_sum(const T* low, const T* low2, const T* high, int rank) {
+__device__ __forceinline__ float low_sum(const T* low, const T* high, int rank) {
+  const int unit = low_unit(rank);
   float sum = 0.f;
   if ((reinterpret_cast<uintptr_t>(high) & 15u) == 0 && rank % 8 == 0) {
     for (int r = 0; r < rank; r += 8) {
       float a[8], c[8], b[8];
-      load_vec<T>(low + r, a);
-      load_vec<T>(low2 + r, c);
+      load_vec<T>(low + low_place(rank, r), a);
+      load_vec<T>(low + low_place(rank, r) + unit, c);
       load_vec<T>(high + r, b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum = fmaf(a[j] + c[j], b[j], sum);
     }
   } else {
-    for (int r = 0; r < rank; ++r) sum = fmaf(static_cast<float>(low[r]) + static_cast<float>(low2[r]), static_cast<float>(high[r]), sum);
+    for (int r = 0; r < rank; ++r) {
+      const T* t = low + low_place(rank, r);
+      sum = fmaf(static_cast<float>(t[0]) + static_cast<float>(t[unit]), static_cast<float>(high[r]), sum);
+    }
   }
   return sum;
 }
@@ -238,7 +272,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1)
 few_rows_kernel(const FewParams p) {
   __shared__ float joined[kFewWarps][kTwo ? 2 : 1][kEights * 8][kFewColumns + 1];
   pdl_trigger();
-  pdl_wait();
+  if (p.adapters.low == nullptr) pdl_wait();  // (otherwise what came before the kernel of the low-rank values is complete)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, n0 = blockIdx.x * kFewColumns, warps = blockDim.x >> 5;
   constexpr int kParts = kTwo ? 2 : 1;
   const T *w[kParts][2], *x[kEights];
@@ -283,13 +317,13 @@ few_rows_kernel(const FewParams p) {
     if constexpr (kTwo) gate += joined[i][1][row][c];
   }
   if (p.adapters.low != nullptr) {
+    pdl_wait();
     const int a = adapter_of(p.adapters.index, uint32_t(row));
     if (a != kNoAdapter) {
-      const int padded = padded_rank(p.adapters.rank);
-      const T* low = static_cast<const T*>(p.adapters.low) + row * 2 * padded;
+      const T* low = static_cast<const T*>(p.adapters.low) + row * low_pitch(p.adapters.rank);
       const T* high = static_cast<const T*>(p.adapters.high) + ((long long)a * (kTwo ? 2 * p.N : p.N) + n) * p.adapters.high_pitch;
-      v += low_sum(low, low + padded, high, p.adapters.rank);
-      if constexpr (kTwo) gate += low_sum(low, low + padded, high + (long long)p.N * p.adapters.high_pitch, p.adapters.rank);
+      v += low_sum(low, high, p.adapters.rank);
+      if constexpr (kTwo) gate += low_sum(low, high + (long long)p.N * p.adapters.high_pitch, p.adapters.rank);
     }
   }
   const T* bias = static_cast<const T*>(p.bias);
@@ -692,7 +726,7 @@ LowPlan plan_low(const BackwardPlan& plan, int count, int rank, int64_t rows, in
     return at;
   };
   p.up = take(int64_t(count) * rank * outer * pad8(N) * 2);
-  p.low_grad = take(chunk * 2 * padded_rank(rank) * 2);
+  p.low_grad = take(chunk * low_pitch(rank) * 2);
   p.part[0] = take(int64_t(p.parts) * count * rank * ad * 4);
   p.part[1] = take(int64_t(p.parts) * count * rank * au * 4);
   return p;
@@ -709,7 +743,7 @@ int check_adapters(const char* what, const b200ta_adapters* a, const void* low) 
   return B200TA_OK;
 }
 AdapterIndex index_of(const b200ta_adapters* a) {
-  return {a->index, a->index_bytes, uint32_t(std::min<int64_t>(std::max<int64_t>(a->rows_per_index, 1), int64_t(1) << 31)), 0, a->count};
+  return adapter_index(a->index, a->index_bytes, a->rows_per_index, a->count);
 }
 
 int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* residual, int64_t rs, void* y, int64_t ys,
@@ -743,6 +777,7 @@ int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const vo
   if (residual) m.aux = {residual, rows, N, rs};
   if (saved) m.saved = {saved, rows, N, ss, gated ? 2 : 1, ss / 2};
   m.bias = bias, m.activation = activation, m.adapters = adapters, m.what = gated ? "gated dense" : "dense";
+  if (adapters != nullptr) m.beside = kBesideSecond;  // (the kernel before is that of the low-rank values)
   return run_matmul(m, stream);
 }
 
@@ -787,7 +822,7 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
   const bool dx_parts = dx != nullptr && !narrow && plan.dx_split.parts > 1 && dxs == K;  // (a join writes dense rows)
 
   // adapters: t (from the forward pass) with U for the pre-activations, dt with D for dx
-  const int64_t low_pitch = ad != nullptr ? 2 * padded_rank(ad->rank) : 0;
+  const int64_t low_bytes = ad != nullptr ? low_pitch(ad->rank) * 2 : 0;
   LowRank with_up{}, with_down{};
   LowGrads low_grads{};
   void* dt = ws_base + low_plan.low_grad;
@@ -805,7 +840,7 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
 
   for (int64_t r0 = 0; r0 < rows; r0 += plan.chunk) {
     const int64_t n = rows - r0 < plan.chunk ? rows - r0 : plan.chunk;
-    const char* low_c = static_cast<const char*>(low) + r0 * low_pitch * 2;
+    const char* low_c = static_cast<const char*>(low) + r0 * low_bytes;
     with_up.low = low_c;
     with_up.index.first_row = with_down.index.first_row = uint32_t(r0);
     const char* dy_c = static_cast<const char*>(dy) + r0 * dys * 2;
@@ -848,7 +883,7 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
     if (ad != nullptr && (dx != nullptr || ddown != nullptr)) {
       LowProduct q{};
       q.x = dz, q.a = ws_base + low_plan.up, q.low = dt, q.scale = ad->scale, q.scale_all = ad->scale_all;
-      q.xs = zs, q.x_plane = zs / outer, q.as = outer * pad8(N), q.a_plane = pad8(N), q.rows = n, q.K = N, q.planes = int(outer), q.rank = ad->rank, q.f16 = f16, q.aligned = true, q.index = with_down.index;
+      q.xs = zs, q.x_plane = zs / outer, q.as = pad8(N), q.rows = n, q.K = N, q.planes = int(outer), q.rank = ad->rank, q.f16 = f16, q.aligned = true, q.index = with_down.index;
       if ((rc = run_low(q, stream)) != B200TA_OK) return rc;
     }
     if (dx != nullptr && !narrow) {
@@ -864,6 +899,7 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
       }
       if (dw != nullptr) m.beside = kBesideFirst;
       if (ad != nullptr) m.adapters = &with_down;
+      if (ad != nullptr && dw == nullptr) m.beside = kBesideSecond;  // (the kernel before is that of dt)
       m.what = "dense_backward dx";
       if ((rc = run_matmul(m, stream)) != B200TA_OK) return rc;
     }
@@ -967,6 +1003,8 @@ int b200ta_adapter_dense(const void* x, int64_t xs, const void* w, int64_t ws, c
   const LowRank adapters{q.index, a->rank, low, a->up, a->up_row_stride};
   return dense_forward(x, xs, w, ws, bias, residual, rs, y, ys, saved, ss, dtype, activation, gated, rows, K, N, &adapters, stream);
 }
+
+size_t b200ta_adapter_low_bytes(int rank) { return rank > 0 && rank <= b200ta::kMaxRank ? size_t(b200ta::low_pitch(rank)) * 2 : 0; }
 
 size_t b200ta_adapter_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, int count, int rank, int64_t rows, int K, int N) {
   using namespace b200ta;

@@ -1,5 +1,5 @@
 // The tensor-core products of the trainable dense layers (sm_100a): D[m, n] = sum_k A[m, k] B[n, k], finished in one of
-// six forms, for bf16 or fp16 operands with accumulators in 32 bits.
+// seven forms, for bf16 or fp16 operands with accumulators in 32 bits.
 //
 //   kDense      y = act(D + bias) + residual, and D + bias itself where the backward pass is to have it
 //   kGated      value and gate columns in one tile: y = (value + b) act(gate + b')
@@ -7,6 +7,7 @@
 //   kGatedGrad  dz = [dy act(gate) | dy value act'(gate)]
 //   kPlain      D                                                       products of gradients
 //   kPartial    D in 32 bits, over one of several parts of k            weight gradients, joined by another kernel
+//   kLow        scale D in two terms, each row with its own adapter's B low-rank values (see adapters.cuh)
 //
 // An operand lies with k contiguous (K-major) or with its rows contiguous (MN-major): x and W as they are make the forward
 // product, dz and W that of dx, dz and x that of dW; nothing is transposed in memory.  Sizes are free (tiles past the edge
@@ -39,7 +40,7 @@
 
 namespace b200ta {
 
-enum MatmulForm { kDense, kGated, kDenseGrad, kGatedGrad, kPlain, kPartial };
+enum MatmulForm { kDense, kGated, kDenseGrad, kGatedGrad, kPlain, kPartial, kLow };
 
 struct MatmulParams {
   int tiles_m, tiles_n, splits, work;  // work = tiles_m * tiles_n * splits items
@@ -72,14 +73,22 @@ struct MatmulParams {
 enum { kBesideNone = 0, kBesideFirst, kBesideSecond };
 
 // Adapters of the rows (see adapters.cuh), or none.  Behind the blocks of x and W along k, a tile takes for each adapter that its rows
-// have the blocks of t and U_g (for dx: of dt and D_g), `unit` ranks wide (as wide as the swizzle of their rows: 32 or 64
-// bytes, so that a stage holds both terms of t beside the one block of U_g that they share).  A block of t serves all of a tile's adapters: the MMA updates no lane (row) whose adapter is another, so nothing of
-// one request, infinities and NaN among it, reaches another's rows.
+// have the blocks of t and U_g (for dx: of dt and D_g), `unit` ranks wide; both terms of a block of t meet the same block of U_g.  The MMA
+// updates no lane (row) whose adapter is another, so nothing of one request, infinities and NaN among it, reaches another's rows.
+//
+// Usually each adapter's blocks pass through the ring like the others.  With `held` (a single block, few blocks of W or several
+// adapters a tile) a tile's t passes once, for all of its adapters, and U_g has room of its own behind the ring, where it stays until
+// an adapter or a column tile is another one.  Rows of one request after the other then load U_g hardly ever, and blocks keep
+// their tile of W (p.resident).  (147456 rows, 128 -> 512 gated, rank 16: 169 us through the ring.)
 struct NoAdapters {};
 struct MatmulAdapters {
   CUtensorMap low, high;
   AdapterIndex index;
   int rank, unit, blocks;
+  int held, slots;     // room for that many blocks of U_g
+  const float* scale;  // kLow: of each adapter, or NULL: scale_all; where the values go
+  float scale_all;
+  void* low_out;
 };
 
 #ifdef __CUDACC__
@@ -92,13 +101,16 @@ constexpr int kABytes = kBM * kBK * 2;
 constexpr int kRingBytes = 131072;         // operand stages
 constexpr int kResidentBytes = 65536;      // of them for a resident B
 constexpr int kMaxStages = 7;
+constexpr int kHighSlots = 4;              // of blocks of U_g, at most
+// The room for held blocks of U_g, the ring's last bytes: one of 256 rows.
+__host__ __device__ constexpr int held_bytes(int unit) { return 256 * unit * 2; }
 constexpr int kSlab = 2048;                // 32 rows of 64 bytes
 constexpr int kSmSlabs = kRingBytes;       // three for each finishing warp
 constexpr int kSmOnes = kSmSlabs + kFinishers * 3 * kSlab;  // an operand block of ones, [16 x 16]
 constexpr int kSmBars = kSmOnes + 512;
 enum Bar {
   FULL = 0, EMPTY = kMaxStages, ACC_FULL = 2 * kMaxStages, ACC_EMPTY = ACC_FULL + 4, B_FULL = ACC_EMPTY + 4, AUX = B_FULL + 1,
-  NUM_BARS = AUX + kFinishers
+  HIGH_FULL = AUX + kFinishers, HIGH_EMPTY = HIGH_FULL + kHighSlots, NUM_BARS = HIGH_EMPTY + kHighSlots
 };
 constexpr int kSmTotal = kSmBars + NUM_BARS * 8 + 32;
 constexpr int kSmDynamic = kSmTotal + 1024;
@@ -317,11 +329,12 @@ __device__ __forceinline__ void mbar_arrive_cluster_warp(uint32_t bar) {
 }
 
 // The same for rows (lanes of tensor memory) whose bit in `off` is clear; the others keep what they hold.
-__device__ __forceinline__ void umma_ss_lanes_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t (&off)[4]) {
+__device__ __forceinline__ void umma_ss_lanes_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t (&off)[4],
+                                                   uint32_t accumulate = 1) {
   asm volatile(
-      "{\n.reg .pred p, e;\nsetp.eq.b32 p, 0, 0;\nelect.sync _|e, 0xffffffff;\n"
+      "{\n.reg .pred p, e;\nsetp.ne.b32 p, %8, 0;\nelect.sync _|e, 0xffffffff;\n"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void umma_ss_lanes_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t (&off)[8]) {
@@ -366,6 +379,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     }
     mbar_init(bars + B_FULL * 8, 1);
     for (int i = 0; i < kFinishers; ++i) mbar_init(bars + (AUX + i) * 8, 1);
+    if constexpr (kAdapt)
+      for (int i = HIGH_FULL; i < NUM_BARS; ++i) mbar_init(bars + i * 8, 1);
     fence_mbar_init();
   }
   if (kSums && p.sums != nullptr && threadIdx.x < 128) {
@@ -391,6 +406,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   const int b_bytes = b_rows * kBK * 2;
   const int stage_bytes = p.resident ? kABytes : kABytes + b_bytes;
   const uint32_t ring = base + (p.resident ? kResidentBytes : 0);
+  uint32_t held = 0;  // the held blocks of adapters
+  if constexpr (kAdapt) held = base + kRingBytes - held_bytes(x.unit);
 
   if (warp == 16) {
     // ------------------------------------------------------------------ TMA producer
@@ -425,13 +442,13 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       int stage = 0, issued = 0;
       uint32_t phase = 1;
       bool ok = true;
-      // The barrier that counts `bytes` of the next stage (of a pair: the first block's, which counts the loads of both).
+      // The barrier that counts `bytes` of what is loaded next (of a pair: the first block's, which counts the loads of both).
       uint32_t full = 0;
-      auto open_stage = [&](int bytes) {
-        if constexpr (kAdapt) ok = mbar_wait_warp(bars + (EMPTY + stage) * 8, phase, abort_flag);
-        else ok = mbar_wait(bars + (EMPTY + stage) * 8, phase, abort_flag);
+      auto open = [&](int empty_bar, uint32_t empty_phase, int full_bar, int bytes) {
+        if constexpr (kAdapt) ok = mbar_wait_warp(bars + empty_bar * 8, empty_phase, abort_flag);
+        else ok = mbar_wait(bars + empty_bar * 8, empty_phase, abort_flag);
         if (!ok) return;
-        full = bars + (FULL + stage) * 8;
+        full = bars + full_bar * 8;
         if (kPair) {
           if (rank == 0 && (!kAdapt || lane == 0)) mbar_expect_tx(full, 2 * bytes);
           full = in_first_block(full);
@@ -439,12 +456,53 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (!kAdapt || lane == 0) mbar_expect_tx(full, bytes);
         }
       };
+      auto open_stage = [&](int bytes) { open(EMPTY + stage, phase, FULL + stage, bytes); };
       [[maybe_unused]] bool low_complete = p.beside != kBesideSecond;
+      // a block of U_g (D_g) of a tile
+      [[maybe_unused]] auto load_high = [&](uint32_t sb, int n0, int r0, int g) {
+        if constexpr (kAdapt) {
+          if constexpr (kBMn) {
+            for (int n = 0; n < b_rows; n += 64) load(sb + n * x.unit * 2, &x.high, full, n0 + int(rank) * b_rows + n, r0, g);
+          } else if constexpr (kTwo && kPair) {
+            load(sb, &x.high, full, r0, n0, 2 * g + int(rank));
+          } else {
+            load(sb, &x.high, full, r0, n0 + int(rank) * b_rows, kTwo ? 2 * g : g);
+          }
+        }
+      };
+      [[maybe_unused]] int highs = 0, held_g = -1, held_n = -1;  // held blocks loaded; what the last of them is
+      [[maybe_unused]] TileAdapters<kPair ? 8 : 4> adapters;
+      [[maybe_unused]] Item upcoming{};
+      [[maybe_unused]] auto look_ahead = [&](int i) {  // the adapters of the next item are on their way early
+        if constexpr (kAdapt) {
+          if (i >= items) return;
+          upcoming = item_of<kPair, kAMn>(p, i, units);
+          adapters.fetch(x.index, upcoming.m0, p.rows_inner);
+        }
+      };
+      look_ahead(0);
       for (int i = 0; ok && i < items; ++i) {
-        Item t = item_of<kPair, kAMn>(p, i, units);
-        [[maybe_unused]] TileAdapters<kPair ? 8 : 4> adapters;
-        if constexpr (kAdapt) adapters.load(x.index, t.m0, p.rows_inner);
+        Item t = upcoming;
+        if constexpr (!kAdapt) t = item_of<kPair, kAMn>(p, i, units);
         t.m0 += int(rank) * kBM;
+        if constexpr (kForm == kLow) {  // all of k for each adapter of the rows
+          adapters.arrived(x.index);
+          const int planes = p.kblocks / p.kblocks_inner;
+          for (int g = adapters.next(-1); ok && g != kNoAdapter; g = adapters.next(g)) {
+            for (int kb = 0, ko = 0, ki = 0; kb < p.kblocks; ++kb) {
+              open_stage(stage_bytes);
+              if (!ok) break;
+              const uint32_t sa = ring + stage * stage_bytes;
+              load(sa, &tm_a, full, ki * kBK, t.m0, ko);
+              load(sa + kABytes, &tm_b, full, ki * kBK, 0, g * planes + ko);
+              ++issued;
+              if (++stage == p.stages) stage = 0, phase ^= 1u;
+              if (++ki == p.kblocks_inner) ki = 0, ++ko;
+            }
+          }
+          look_ahead(i + 1);
+          continue;
+        }
         int ko = t.kb0 / p.kblocks_inner, ki = t.kb0 - ko * p.kblocks_inner;
         for (int kb = t.kb0; kb < t.kb1; ++kb) {
           open_stage(stage_bytes);
@@ -463,25 +521,38 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (++ki == p.kblocks_inner) ki = 0, ++ko;
         }
         if constexpr (kAdapt) {
+          adapters.arrived(x.index);
+          bool first = true;
           for (int g = adapters.next(-1); ok && t.split == p.splits - 1 && g != kNoAdapter; g = adapters.next(g)) {
             if (!low_complete) pdl_wait(), low_complete = true;
+            if (x.held) {
+              if (first) {
+                open_stage(2 * kBM * x.unit * 2);
+                if (!ok) break;
+                load(ring + stage * stage_bytes, &x.low, full, 0, t.m0, 0);
+                first = false, ++issued;
+                if (++stage == p.stages) stage = 0, phase ^= 1u;
+              }
+              if (g != held_g || t.n0 != held_n) {
+                const int slot = highs % x.slots, bytes = b_rows * x.unit * 2;
+                open(HIGH_EMPTY + slot, highs / x.slots & 1 ^ 1, HIGH_FULL + slot, bytes);
+                if (!ok) break;
+                load_high(held + slot * bytes, t.n0, 0, g);
+                ++highs, held_g = g, held_n = t.n0;
+              }
+              continue;
+            }
             for (int block = 0; block < x.blocks; ++block) {
               open_stage((2 * kBM + b_rows) * x.unit * 2);
               if (!ok) break;
-              const uint32_t sa = ring + stage * stage_bytes, sb = sa + kABytes;
-              const int r0 = block * x.unit;
-              load(sa, &x.low, full, r0, t.m0, 0);
-              if constexpr (kBMn) {
-                for (int n = 0; n < b_rows; n += 64) load(sb + n * x.unit * 2, &x.high, full, t.n0 + int(rank) * b_rows + n, r0, g);
-              } else if constexpr (kTwo && kPair) {
-                load(sb, &x.high, full, r0, t.n0, 2 * g + int(rank));
-              } else {
-                load(sb, &x.high, full, r0, t.n0 + int(rank) * b_rows, kTwo ? 2 * g : g);
-              }
+              const uint32_t sa = ring + stage * stage_bytes;
+              load(sa, &x.low, full, block * 2 * x.unit, t.m0, 0);
+              load_high(sa + kABytes, t.n0, block * x.unit, g);
               ++issued;
               if (++stage == p.stages) stage = 0, phase ^= 1u;
             }
           }
+          look_ahead(i + 1);
         }
       }
       // If the loop was abandoned, give copies still in flight a bounded chance to land (of a pair's first block: those of
@@ -491,6 +562,11 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         if (rank == 0)
           for (int j = issued > p.stages ? issued - p.stages : 0; j < issued; ++j)
             mbar_wait(bars + (FULL + j % p.stages) * 8, (j / p.stages) & 1, abort_flag + 1);
+        if constexpr (kAdapt) {
+          if (rank == 0)
+            for (int j = highs > x.slots ? highs - x.slots : 0; j < highs; ++j)
+              mbar_wait(bars + (HIGH_FULL + j % x.slots) * 8, (j / x.slots) & 1, abort_flag + 1);
+        }
       }
     }
   } else if (warp == 17) {
@@ -503,13 +579,53 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       bool ok = true;
       if (p.resident) ok = mbar_wait_warp(bars + B_FULL * 8, 0, abort_flag);
       if (kAdapt && p.beside != kBesideSecond) pdl_wait();  // the index
+      [[maybe_unused]] int highs = 0, held_g = -1, held_n = -1;
+      [[maybe_unused]] TileAdapters<kPair ? 8 : 4> adapters;
+      [[maybe_unused]] Item upcoming{};
+      [[maybe_unused]] auto look_ahead = [&](int i) {
+        if constexpr (kAdapt) {
+          if (i >= items) return;
+          upcoming = item_of<kPair, kAMn>(p, i, units);
+          adapters.fetch(x.index, upcoming.m0, p.rows_inner);
+        }
+      };
+      look_ahead(0);
       for (int i = 0; ok && i < items; ++i) {
-        const Item t = item_of<kPair, kAMn>(p, i, units);
-        [[maybe_unused]] TileAdapters<kPair ? 8 : 4> adapters;
-        if constexpr (kAdapt) adapters.load(x.index, t.m0, p.rows_inner);
+        Item t = upcoming;
+        if constexpr (!kAdapt) t = item_of<kPair, kAMn>(p, i, units);
         const int buffer = i & ((1 << p.buffers) - 1);
         const uint32_t acc = tb + buffer * (512 >> p.buffers);
         ok = mbar_wait_warp(bars + (ACC_EMPTY + buffer) * 8, ((i >> p.buffers) & 1) ^ 1, abort_flag);
+        if constexpr (kForm == kLow) {
+          adapters.arrived(x.index);
+          auto walk_k = [&](auto&& multiply) {
+            for (int kb = 0; kb < p.kblocks; ++kb) {
+              ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t sa = ring + stage * stage_bytes;
+              const uint64_t da = smem_desc<16, 1024, kLayoutSw128>(sa), db = smem_desc<16, 1024, kLayoutSw128>(sa + kABytes);
+#pragma unroll
+              for (int k = 0; k < kBK / 16; ++k) multiply(da + k * 2, db + k * 2, (kb > 0 || k > 0) ? 1u : 0u);
+              umma_commit_warp(bars + (EMPTY + stage) * 8);
+              if (++stage == p.stages) stage = 0, phase ^= 1u;
+            }
+          };
+          for (int g = adapters.next(-1); ok && g != kNoAdapter; g = adapters.next(g)) {
+            if (adapters.all_have(g)) {
+              walk_k([&](uint64_t da, uint64_t db, uint32_t add) { umma_ss_warp(acc, da, db, id, add); });
+            } else {
+              uint32_t off[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) off[j] = ~adapters.rows_of(j, g);
+              walk_k([&](uint64_t da, uint64_t db, uint32_t add) { umma_ss_lanes_warp(acc, da, db, id, off, add); });
+            }
+          }
+          if (!ok) break;
+          umma_commit_warp(bars + (ACC_FULL + buffer) * 8);
+          look_ahead(i + 1);
+          continue;
+        }
         for (int kb = t.kb0; ok && kb < t.kb1; ++kb) {
           ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
           if (!ok) break;
@@ -537,31 +653,83 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (++stage == p.stages) stage = 0, phase ^= 1u;
         }
         if constexpr (kAdapt) {
-          for (int g = adapters.next(-1); ok && t.split == p.splits - 1 && g != kNoAdapter; g = adapters.next(g)) {
-            uint32_t off[kPair ? 8 : 4];
+          adapters.arrived(x.index);
+          bool first = true;
+          uint32_t s_low = 0;  // the tile's block of t
+          int low_stage = 0;
+          // a block of t times one of U_g, for the lanes that are not off
+          int g;
+          auto multiply = [&](uint32_t sa, uint32_t sb, int ranks) {
+            // t: rows of 4 * unit bytes, its second terms 2 * unit bytes behind the first.  U_g: rows of 2 * unit bytes; D_g (MN-major) as
+            // above, with `unit` rows (k) to a block of 64 columns.  A step of 16 ranks is 32 bytes.
+            const bool wide = x.unit == 32;
+            const uint64_t da = (wide ? smem_desc<16, 1024, kLayoutSw128>(sa) : smem_desc<16, 512, kLayoutSw64>(sa));
+            uint64_t db;
+            if constexpr (kBMn) db = smem_desc<0, 1024, kLayoutSw128>(sb) | uint64_t(x.unit * 8) << 16;
+            else db = wide ? smem_desc<16, 512, kLayoutSw64>(sb) : smem_desc<16, 256, kLayoutSw32>(sb);
+            const bool two = wide && ranks > 16;
+            auto steps = [&](auto&& product) {
+              product(da, db);
+              product(da + x.unit / 8, db);
+              if (two) {
+                product(da + 2, db + (kBMn ? 128 : 2));
+                product(da + 6, db + (kBMn ? 128 : 2));
+              }
+            };
+            if (adapters.all_have(g)) {
+              steps([&](uint64_t a, uint64_t b) {
+                if constexpr (kPair) umma_ss_pair_warp(acc, a, b, id, 1u);
+                else umma_ss_warp(acc, a, b, id, 1u);
+              });
+            } else {
+              uint32_t off[kPair ? 8 : 4];
 #pragma unroll
-            for (int j = 0; j < (kPair ? 8 : 4); ++j) off[j] = ~adapters.rows_of(j, g);
+              for (int j = 0; j < (kPair ? 8 : 4); ++j) off[j] = ~adapters.rows_of(j, g);
+              steps([&](uint64_t a, uint64_t b) { umma_ss_lanes_warp(acc, a, b, id, off); });
+            }
+          };
+          for (g = adapters.next(-1); ok && t.split == p.splits - 1 && g != kNoAdapter; g = adapters.next(g)) {
+            if (x.held) {
+              if (first) {
+                ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+                if (!ok) break;
+                s_low = ring + stage * stage_bytes, low_stage = stage, first = false;
+                if (++stage == p.stages) stage = 0, phase ^= 1u;
+              }
+              if (g != held_g || t.n0 != held_n) {
+                if (highs > 0) {  // all that read the last one has been issued
+                  const uint32_t done = bars + (HIGH_EMPTY + (highs - 1) % x.slots) * 8;
+                  if constexpr (kPair) umma_commit_pair_warp(done);
+                  else umma_commit_warp(done);
+                }
+                ok = mbar_wait_warp(bars + (HIGH_FULL + highs % x.slots) * 8, highs / x.slots & 1, abort_flag);
+                if (!ok) break;
+                ++highs, held_g = g, held_n = t.n0;
+              }
+              tc_fence_after();
+              multiply(s_low, held + (highs - 1) % x.slots * (b_rows * x.unit * 2), x.rank);
+              continue;
+            }
             for (int block = 0; block < x.blocks; ++block) {
               ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
               if (!ok) break;
               tc_fence_after();
-              const uint32_t sa = ring + stage * stage_bytes, sb = sa + kABytes;
-              // K-major: rows of 2 * unit bytes, groups of 8 rows apart as they lie.  MN-major: as above, `unit` rows (k) a block.
-              const uint64_t rows_hi = uint64_t(x.unit) | (1u << 14) | ((x.unit == 32 ? kLayoutSw64 : kLayoutSw32) << 29);
-              const uint64_t da = rows_hi << 32 | ((sa >> 4) | 1u << 16);
-              const uint64_t db = kBMn ? smem_desc<0, 1024, kLayoutSw128>(sb) | uint64_t(x.unit * 8) << 16 : rows_hi << 32 | ((sb >> 4) | 1u << 16);
-              const int left = x.rank - block * x.unit, steps = ((left < x.unit ? left : x.unit) + 15) / 16;
-              for (int term = 0; term < 2; ++term)  // (a term's block is 128 rows)
-                for (int k = 0; k < steps; ++k) umma_ss_lanes_warp(acc, da + term * x.unit * 16 + k * 2, db + k * (kBMn ? 128 : 2), id, off);
+              const uint32_t sa = ring + stage * stage_bytes;
+              multiply(sa, sa + kABytes, x.rank - block * x.unit);
               if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + stage) * 8);
               else umma_commit_warp(bars + (EMPTY + stage) * 8);
               if (++stage == p.stages) stage = 0, phase ^= 1u;
             }
           }
+          if (!first) {
+            if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + low_stage) * 8);
+            else umma_commit_warp(bars + (EMPTY + low_stage) * 8);
+          }
         }
         if (!ok) break;
         if constexpr (kPair) umma_commit_pair_warp(bars + (ACC_FULL + buffer) * 8);
         else umma_commit_warp(bars + (ACC_FULL + buffer) * 8);
+        look_ahead(i + 1);
       }
     }
   } else {
@@ -650,6 +818,35 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       if (!ok) break;
       tc_fence_after();
       const uint32_t acc = lane_acc + buffer * (512 >> p.buffers);
+      if constexpr (kForm == kLow) {  // 16 ranks of a row at a time: two terms of 32 bytes
+        const bool in = row + lane < p.rows_inner;
+        const int g = in ? adapter_of(x.index, uint32_t(row + lane)) : kNoAdapter;
+        const float scale = g == kNoAdapter ? 0.f : x.scale != nullptr ? __ldg(x.scale + g) : x.scale_all;
+        if (first_g * 16 >= p.tile_n) release(i);
+        for (int r = first_g * 16; r < p.tile_n; r += step_g * 16) {
+          float v[16];
+          tmem_load(acc + r, v);
+          tmem_ld_wait();
+          if (r + step_g * 16 >= p.tile_n) release(i);
+          if (!in) continue;
+          uint32_t first[8], second[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            // (lanes without an adapter hold whatever was there)
+            const float v0 = g == kNoAdapter ? 0.f : v[2 * j] * scale, v1 = g == kNoAdapter ? 0.f : v[2 * j + 1] * scale;
+            first[j] = pack2<T>(v0, v1);
+            const float2 f = unpack2<T>(first[j]);
+            second[j] = pack2<T>(v0 - f.x, v1 - f.y);
+          }
+          T* to = static_cast<T*>(x.low_out) + (long long)(row + lane) * low_pitch(x.rank) + low_place(x.rank, r);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            reinterpret_cast<uint4*>(to)[h] = make_uint4(first[4 * h], first[4 * h + 1], first[4 * h + 2], first[4 * h + 3]);
+            reinterpret_cast<uint4*>(to + x.unit)[h] = make_uint4(second[4 * h], second[4 * h + 1], second[4 * h + 2], second[4 * h + 3]);
+          }
+        }
+        continue;
+      }
       if (kSums && p.sums != nullptr && t.n0 == 0 && first_g == 0 && groups > 0) {
         float sum[16];
         tmem_load(acc + 128, sum);
@@ -782,6 +979,7 @@ struct Matmul {
   int beside = kBesideNone;
   void* sums = nullptr;  // see MatmulParams
   const LowRank* adapters = nullptr;
+  const LowProduct* low = nullptr;  // kLow: everything else
   const char* what = "matmul";
 };
 int run_matmul(const Matmul& m, void* stream);
@@ -797,6 +995,7 @@ int launch_matmul_product(DeviceState* st, const Matmul& m, const MatmulMaps& ma
 int launch_matmul_forward(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const MatmulAdapters& x, int grid, void* stream);
 int launch_matmul_grad(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const MatmulAdapters& x, int grid, void* stream);
 int launch_matmul_product(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const MatmulAdapters& x, int grid, void* stream);
+int launch_matmul_low(DeviceState* st, const Matmul& m, const MatmulMaps& maps, const MatmulParams& p, const MatmulAdapters& x, int grid, void* stream);
 
 #ifdef __CUDACC__
 namespace matmul {

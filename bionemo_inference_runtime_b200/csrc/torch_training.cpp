@@ -22,7 +22,7 @@ struct Library {
 #define B200TA_ENTRIES(X)                                                                                                \
   X(layer_norm) X(layer_norm_workspace_bytes) X(layer_norm_backward) X(dense_few_rows) X(dense_keeps) X(dense)              \
   X(dense_backward_workspace_bytes) X(dense_backward) X(copy_rows) X(dropout)      \
-  X(adapter_dense) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
+  X(adapter_dense) X(adapter_low_bytes) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
   B200TA_ENTRIES(B200TA_ENTRY)
 #undef B200TA_ENTRY
 } lib;
@@ -367,7 +367,7 @@ std::tuple<at::Tensor, at::Tensor, Maybe> adapter_dense(const at::Tensor& x, con
   const Adapting a = adapters_of(x, l, w.size(0), down, up, index, scale, scale_all, few, low_copies);
   const at::Tensor y = or_out(out, x, l.N);
   if (residual) require_like("residual", *residual, x, y.sizes());
-  const int64_t low_pitch = 2 * pad8(a.c.rank), pitch = pad8(l.N) * (gated ? 2 : 1);
+  const int64_t low_pitch = int64_t(lib.adapter_low_bytes(a.c.rank)) / 2, pitch = pad8(l.N) * (gated ? 2 : 1);
   const at::Tensor low = empty({l.rows, low_pitch}, x.scalar_type(), x);
   Maybe saved;
   if (want_saved && lib.dense_keeps(int(activation), gated, l.K)) saved = empty({l.rows, pitch}, at::kFloat, x);
@@ -407,7 +407,7 @@ std::tuple<Maybe, Maybe, Maybe, Maybe, Maybe> adapter_dense_backward(const at::T
   const c10::cuda::CUDAGuard guard(x.device());
   Copies copies, low_copies;
   const Adapting a = adapters_of(x, l, w.size(0), down, up, index, scale, scale_all, false, low_copies);
-  const int64_t low_pitch = 2 * pad8(a.c.rank);
+  const int64_t low_pitch = int64_t(lib.adapter_low_bytes(a.c.rank)) / 2;
   require_like("saved", low, x, {l.rows, low_pitch});
   if (!low.is_contiguous()) refuse("saved must be what the forward pass returned");
   if (saved) {
