@@ -82,18 +82,19 @@ low_product_kernel(const LowProduct p, int share) {
   const long long row0 = ((long long)blockIdx.x * (share ? 1 : kWarps) + (share ? 0 : warp)) * kLowRows;
   const int r0 = blockIdx.y * kRanks, first = share ? warp * 32 : 0, step = share ? kWarps * 32 : 32;
   if (row0 >= p.rows) return;  // (of a block whose warps share rows: all of them)
-  TileAdapters<1> mine;
+  TileAdapters<1> mine(p.index);
   mine.fetch(p.index, int(row0), int(p.rows));
   mine.arrived(p.index);
   auto store = [&](int row, int r, float v) {  // a value of this warp's rows
     if (r < low_pitch(p.rank) / 2) store_low<T>(p, row0 + row, r, r < p.rank ? v : 0.f);
   };
+  const uint32_t in = p.rows - row0 < kLowRows ? (1u << (p.rows - row0)) - 1u : ~0u;  // rows that there are
   // rows without an adapter
-  for (int row = share ? warp : 0; row < kLowRows && row0 + row < p.rows; row += share ? kWarps : 1)
+  for (int row = share ? warp : 0; row < kLowRows && (in >> row & 1u); row += share ? kWarps : 1)
     if (__shfl_sync(0xffffffffu, mine.g[0], row) == kNoAdapter)
       for (int r = lane; r < kRanks; r += 32) store(row, r0 + r, 0.f);
   for (int g = mine.next(-1); g != kNoAdapter; g = mine.next(g)) {
-    const uint32_t own = mine.rows_of(0, g);
+    const uint32_t own = mine.rows_of(0, g) & in;
     const float scale = p.scale != nullptr ? __ldg(p.scale + g) : p.scale_all;
     float acc[2][kTiles][4] = {};
     for (int plane = 0; plane < p.planes; ++plane) {

@@ -98,23 +98,29 @@ __device__ __forceinline__ int adapter_of(const AdapterIndex& x, uint32_t row) {
   return x.index == nullptr ? 0 : adapter_of_entry(x, index_entry(x, row));
 }
 // The adapters of 32 * kWords rows, which a warp walks in ascending order: of rows that share an entry the one, of others lane l has
-// those of rows 32 j + l.  fetch() starts the loads, arrived() waits for them.  (The usual case is short: the warps that call this
-// share their issue slots with sixteen others.)
+// those of rows 32 j + l.  fetch() starts the loads, arrived() waits for them.  The usual case is short (rows of the same entry as
+// before: two comparisons), since the warps that call this share their issue slots with sixteen others and an instruction takes them
+// some ten clocks.
 template <int kWords>
 struct TileAdapters {
   long long entry[kWords];
   int g[kWords];
-  uint32_t behind;  // bit j: this lane's row 32 j + l is behind the last one
+  uint32_t behind;      // bit j: this lane's row 32 j + l is behind the last one
+  uint32_t begin, end;  // rows of the whole tensor that entry[0] is of
   bool same, next_same;
+  __device__ __forceinline__ explicit TileAdapters(const AdapterIndex& x) : begin(0), end(x.index == nullptr ? ~0u : 0u) { entry[0] = 0; }
   __device__ __forceinline__ void fetch(const AdapterIndex& x, int row0, int rows) {
-    next_same = true;
-    if (x.index == nullptr) return;
-    const uint32_t first = uint32_t(row0), last = uint32_t(min(row0 + 32 * kWords, rows) - 1);
-    next_same = (uint64_t(x.first_row + first) * x.factor >> x.shift) == (uint64_t(x.first_row + last) * x.factor >> x.shift);
+    const uint32_t first = x.first_row + uint32_t(row0), last = x.first_row + uint32_t(min(row0 + 32 * kWords, rows) - 1);
+    next_same = first >= begin && last < end;
+    if (next_same) return;
+    const uint32_t i = uint32_t(uint64_t(first) * x.factor >> x.shift);
+    begin = i * x.rows_per_index, end = begin + x.rows_per_index;
+    next_same = last < end;
     if (next_same) {
-      entry[0] = index_entry(x, first);
+      entry[0] = index_entry(x, uint32_t(row0));
       return;
     }
+    end = begin;
     behind = 0;
 #pragma unroll
     for (int j = 0; j < kWords; ++j) {
@@ -127,7 +133,7 @@ struct TileAdapters {
   __device__ __forceinline__ void arrived(const AdapterIndex& x) {
     same = next_same;
     if (same) {
-      g[0] = x.index == nullptr ? 0 : adapter_of_entry(x, entry[0]);
+      g[0] = adapter_of_entry(x, entry[0]);
       return;
     }
 #pragma unroll

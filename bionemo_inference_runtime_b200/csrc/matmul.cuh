@@ -158,6 +158,43 @@ __device__ __forceinline__ int items_of(const MatmulParams& p) {
   return (p.work - 1 - block) / blocks + 1;
 }
 
+// The items of a block one after the other, with adapters those of their rows as well, which are looked up an item ahead.
+template <bool kAdapt, bool kPair, bool kOuter>
+struct TileRows {
+  template <typename X>
+  __device__ __forceinline__ TileRows(const MatmulParams&, const X&, int) {}
+  __device__ __forceinline__ Item item(const MatmulParams& p, int i, int units) const { return item_of<kPair, kOuter>(p, i, units); }
+  template <typename X>
+  __device__ __forceinline__ void look(const MatmulParams&, const X&, int, int, int) {}
+};
+template <bool kPair, bool kOuter>
+struct TileRows<true, kPair, kOuter> {
+  Item upcoming;
+  TileAdapters<kPair ? 8 : 4> adapters;
+  __device__ __forceinline__ TileRows(const MatmulParams& p, const MatmulAdapters& x, int units)
+      : upcoming(item_of<kPair, kOuter>(p, 0, units)), adapters(x.index) {
+    adapters.fetch(x.index, upcoming.m0, p.rows_inner);
+  }
+  __device__ __forceinline__ Item item(const MatmulParams&, int, int) const { return upcoming; }
+  __device__ __forceinline__ void look(const MatmulParams& p, const MatmulAdapters& x, int i, int items, int units) {
+    if (i >= items) return;
+    if (p.resident) upcoming.m0 += p.resident * (kPair ? 2 * kBM : kBM);
+    else upcoming = item_of<kPair, kOuter>(p, i, units);
+    adapters.fetch(x.index, upcoming.m0, p.rows_inner);
+  }
+};
+// The held block of U_g that is used last: whose it is, where it lies, and the phase of its barriers.
+struct HeldHigh {
+  int g = -1, n0 = 0, slot = -1;
+  uint32_t phase = 1;
+  __device__ __forceinline__ bool differs(int to_g, int to_n) const { return to_g != g || to_n != n0; }
+  __device__ __forceinline__ void take(int slots, int to_g, int to_n) {
+    g = to_g, n0 = to_n;
+    if (slot < 0) slot = 0, phase = 0;
+    else if (++slot == slots) slot = 0, phase ^= 1u;
+  }
+};
+
 __host__ __device__ constexpr uint32_t idesc(bool f16, int m, int n, bool a_mn, bool b_mn) {
   return make_idesc_bf16(m, n, a_mn, b_mn) & ~(f16 ? (1u << 7 | 1u << 10) : 0u);
 }
@@ -470,22 +507,34 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           }
         }
       };
-      [[maybe_unused]] int highs = 0, held_g = -1, held_n = -1;  // held blocks loaded; what the last of them is
-      [[maybe_unused]] TileAdapters<kPair ? 8 : 4> adapters;
-      [[maybe_unused]] Item upcoming{};
-      [[maybe_unused]] auto look_ahead = [&](int i) {  // the adapters of the next item are on their way early
+      [[maybe_unused]] HeldHigh high;
+      [[maybe_unused]] int highs = 0;  // held blocks loaded
+      [[maybe_unused]] auto hold = [&](int g, int n0) {
         if constexpr (kAdapt) {
-          if (i >= items) return;
-          upcoming = item_of<kPair, kAMn>(p, i, units);
-          adapters.fetch(x.index, upcoming.m0, p.rows_inner);
+          if (!high.differs(g, n0)) return;
+          high.take(x.slots, g, n0);
+          const int bytes = b_rows * x.unit * 2;
+          open(HIGH_EMPTY + high.slot, high.phase ^ 1, HIGH_FULL + high.slot, bytes);
+          if (!ok) return;
+          load_high(held + high.slot * bytes, n0, 0, g);
+          ++highs;
         }
       };
-      look_ahead(0);
+      [[maybe_unused]] auto load_low = [&](int m0) {
+        if constexpr (kAdapt) {
+          open_stage(2 * kBM * x.unit * 2);
+          if (!ok) return;
+          load(ring + stage * stage_bytes, &x.low, full, 0, m0, 0);
+          ++issued;
+          if (++stage == p.stages) stage = 0, phase ^= 1u;
+        }
+      };
+      TileRows<kAdapt, kPair, kAMn> ahead(p, x, units);
       for (int i = 0; ok && i < items; ++i) {
-        Item t = upcoming;
-        if constexpr (!kAdapt) t = item_of<kPair, kAMn>(p, i, units);
+        Item t = ahead.item(p, i, units);
         t.m0 += int(rank) * kBM;
         if constexpr (kForm == kLow) {  // all of k for each adapter of the rows
+          auto& adapters = ahead.adapters;
           adapters.arrived(x.index);
           const int planes = p.kblocks / p.kblocks_inner;
           for (int g = adapters.next(-1); ok && g != kNoAdapter; g = adapters.next(g)) {
@@ -500,7 +549,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               if (++ki == p.kblocks_inner) ki = 0, ++ko;
             }
           }
-          look_ahead(i + 1);
+          ahead.look(p, x, i + 1, items, units);
           continue;
         }
         int ko = t.kb0 / p.kblocks_inner, ki = t.kb0 - ko * p.kblocks_inner;
@@ -521,25 +570,16 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (++ki == p.kblocks_inner) ki = 0, ++ko;
         }
         if constexpr (kAdapt) {
+          auto& adapters = ahead.adapters;
           adapters.arrived(x.index);
           bool first = true;
           for (int g = adapters.next(-1); ok && t.split == p.splits - 1 && g != kNoAdapter; g = adapters.next(g)) {
             if (!low_complete) pdl_wait(), low_complete = true;
             if (x.held) {
-              if (first) {
-                open_stage(2 * kBM * x.unit * 2);
-                if (!ok) break;
-                load(ring + stage * stage_bytes, &x.low, full, 0, t.m0, 0);
-                first = false, ++issued;
-                if (++stage == p.stages) stage = 0, phase ^= 1u;
-              }
-              if (g != held_g || t.n0 != held_n) {
-                const int slot = highs % x.slots, bytes = b_rows * x.unit * 2;
-                open(HIGH_EMPTY + slot, highs / x.slots & 1 ^ 1, HIGH_FULL + slot, bytes);
-                if (!ok) break;
-                load_high(held + slot * bytes, t.n0, 0, g);
-                ++highs, held_g = g, held_n = t.n0;
-              }
+              if (first) load_low(t.m0);
+              first = false;
+              if (ok) hold(g, t.n0);
+              if (adapters.same) break;
               continue;
             }
             for (int block = 0; block < x.blocks; ++block) {
@@ -552,7 +592,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               if (++stage == p.stages) stage = 0, phase ^= 1u;
             }
           }
-          look_ahead(i + 1);
+          ahead.look(p, x, i + 1, items, units);
         }
       }
       // If the loop was abandoned, give copies still in flight a bounded chance to land (of a pair's first block: those of
@@ -579,24 +619,49 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       bool ok = true;
       if (p.resident) ok = mbar_wait_warp(bars + B_FULL * 8, 0, abort_flag);
       if (kAdapt && p.beside != kBesideSecond) pdl_wait();  // the index
-      [[maybe_unused]] int highs = 0, held_g = -1, held_n = -1;
-      [[maybe_unused]] TileAdapters<kPair ? 8 : 4> adapters;
-      [[maybe_unused]] Item upcoming{};
-      [[maybe_unused]] auto look_ahead = [&](int i) {
-        if constexpr (kAdapt) {
-          if (i >= items) return;
-          upcoming = item_of<kPair, kAMn>(p, i, units);
-          adapters.fetch(x.index, upcoming.m0, p.rows_inner);
+      // Blocks of t: rows of 4 * unit bytes, the second terms 2 * unit bytes behind the first.  Of U_g: rows of 2 * unit bytes; of D_g
+      // (MN-major) as below, with `unit` rows (k) to a block of 64 columns.  A step of 16 ranks is 32 bytes.
+      [[maybe_unused]] uint64_t low_desc = 0, high_desc = 0;
+      [[maybe_unused]] uint32_t term = 0;
+      if constexpr (kAdapt) {
+        const bool wide = x.unit == 32;
+        low_desc = wide ? smem_desc<16, 1024, kLayoutSw128>(0) : smem_desc<16, 512, kLayoutSw64>(0);
+        if constexpr (kBMn) high_desc = smem_desc<0, 1024, kLayoutSw128>(0) | uint64_t(x.unit * 8) << 16;
+        else high_desc = wide ? smem_desc<16, 512, kLayoutSw64>(0) : smem_desc<16, 256, kLayoutSw32>(0);
+        term = x.unit / 8;
+      }
+      // t's block times that of U_g by `product`: both terms, and both again behind the first 16 ranks
+      [[maybe_unused]] auto steps = [&](uint64_t da, uint64_t db, int ranks, auto&& product) {
+        product(da, db);
+        product(da + term, db);
+        if (ranks > 16 && term == 4) {
+          product(da + 2, db + (kBMn ? 128 : 2));
+          product(da + 6, db + (kBMn ? 128 : 2));
         }
       };
-      look_ahead(0);
+      [[maybe_unused]] HeldHigh high;
+      [[maybe_unused]] uint64_t held_desc = 0;
+      [[maybe_unused]] auto hold = [&](int g, int n0) {  // waits for a held block of U_g
+        if constexpr (kAdapt) {
+          if (!high.differs(g, n0)) return;
+          if (high.g >= 0) {  // all that read the last one has been issued
+            const uint32_t done = bars + (HIGH_EMPTY + high.slot) * 8;
+            if constexpr (kPair) umma_commit_pair_warp(done);
+            else umma_commit_warp(done);
+          }
+          high.take(x.slots, g, n0);
+          ok = mbar_wait_warp(bars + (HIGH_FULL + high.slot) * 8, high.phase, abort_flag);
+          held_desc = high_desc | ((held + high.slot * (b_rows * x.unit * 2)) >> 4);
+        }
+      };
+      TileRows<kAdapt, kPair, kAMn> ahead(p, x, units);
       for (int i = 0; ok && i < items; ++i) {
-        Item t = upcoming;
-        if constexpr (!kAdapt) t = item_of<kPair, kAMn>(p, i, units);
+        const Item t = ahead.item(p, i, units);
         const int buffer = i & ((1 << p.buffers) - 1);
         const uint32_t acc = tb + buffer * (512 >> p.buffers);
         ok = mbar_wait_warp(bars + (ACC_EMPTY + buffer) * 8, ((i >> p.buffers) & 1) ^ 1, abort_flag);
         if constexpr (kForm == kLow) {
+          auto& adapters = ahead.adapters;
           adapters.arrived(x.index);
           auto walk_k = [&](auto&& multiply) {
             for (int kb = 0; kb < p.kblocks; ++kb) {
@@ -623,7 +688,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           }
           if (!ok) break;
           umma_commit_warp(bars + (ACC_FULL + buffer) * 8);
-          look_ahead(i + 1);
+          ahead.look(p, x, i + 1, items, units);
           continue;
         }
         for (int kb = t.kb0; ok && kb < t.kb1; ++kb) {
@@ -653,83 +718,70 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (++stage == p.stages) stage = 0, phase ^= 1u;
         }
         if constexpr (kAdapt) {
+          auto& adapters = ahead.adapters;
           adapters.arrived(x.index);
-          bool first = true;
-          uint32_t s_low = 0;  // the tile's block of t
-          int low_stage = 0;
-          // a block of t times one of U_g, for the lanes that are not off
-          int g;
-          auto multiply = [&](uint32_t sa, uint32_t sb, int ranks) {
-            // t: rows of 4 * unit bytes, its second terms 2 * unit bytes behind the first.  U_g: rows of 2 * unit bytes; D_g (MN-major) as
-            // above, with `unit` rows (k) to a block of 64 columns.  A step of 16 ranks is 32 bytes.
-            const bool wide = x.unit == 32;
-            const uint64_t da = (wide ? smem_desc<16, 1024, kLayoutSw128>(sa) : smem_desc<16, 512, kLayoutSw64>(sa));
-            uint64_t db;
-            if constexpr (kBMn) db = smem_desc<0, 1024, kLayoutSw128>(sb) | uint64_t(x.unit * 8) << 16;
-            else db = wide ? smem_desc<16, 512, kLayoutSw64>(sb) : smem_desc<16, 256, kLayoutSw32>(sb);
-            const bool two = wide && ranks > 16;
-            auto steps = [&](auto&& product) {
-              product(da, db);
-              product(da + x.unit / 8, db);
-              if (two) {
-                product(da + 2, db + (kBMn ? 128 : 2));
-                product(da + 6, db + (kBMn ? 128 : 2));
-              }
-            };
-            if (adapters.all_have(g)) {
-              steps([&](uint64_t a, uint64_t b) {
-                if constexpr (kPair) umma_ss_pair_warp(acc, a, b, id, 1u);
-                else umma_ss_warp(acc, a, b, id, 1u);
-              });
-            } else {
+          auto one = [&](uint64_t a, uint64_t b) {
+            if constexpr (kPair) umma_ss_pair_warp(acc, a, b, id, 1u);
+            else umma_ss_warp(acc, a, b, id, 1u);
+          };
+          auto release_stage = [&](int s) {
+            if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + s) * 8);
+            else umma_commit_warp(bars + (EMPTY + s) * 8);
+          };
+          const bool here = ok && t.split == p.splits - 1;
+          if (x.held && adapters.same) {
+            const int g = adapters.g[0];
+            if (here && g != kNoAdapter) {
+              hold(g, t.n0);
+              if (ok) ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              steps(low_desc | ((ring + stage * stage_bytes) >> 4), held_desc, x.rank, one);
+              release_stage(stage);
+              if (++stage == p.stages) stage = 0, phase ^= 1u;
+            }
+          } else {
+            uint64_t da = 0;  // the tile's block of t, if held
+            int low_stage = -1;
+            for (int g = adapters.next(-1); here && ok && g != kNoAdapter; g = adapters.next(g)) {
               uint32_t off[kPair ? 8 : 4];
 #pragma unroll
               for (int j = 0; j < (kPair ? 8 : 4); ++j) off[j] = ~adapters.rows_of(j, g);
-              steps([&](uint64_t a, uint64_t b) { umma_ss_lanes_warp(acc, a, b, id, off); });
-            }
-          };
-          for (g = adapters.next(-1); ok && t.split == p.splits - 1 && g != kNoAdapter; g = adapters.next(g)) {
-            if (x.held) {
-              if (first) {
+              const bool all = adapters.all_have(g);
+              auto multiply = [&](uint64_t a, uint64_t b, int ranks) {
+                if (all) steps(a, b, ranks, one);
+                else steps(a, b, ranks, [&](uint64_t ak, uint64_t bk) { umma_ss_lanes_warp(acc, ak, bk, id, off); });
+              };
+              if (x.held) {
+                if (low_stage < 0) {
+                  ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+                  if (!ok) break;
+                  da = low_desc | ((ring + stage * stage_bytes) >> 4), low_stage = stage;
+                  if (++stage == p.stages) stage = 0, phase ^= 1u;
+                }
+                hold(g, t.n0);
+                if (!ok) break;
+                tc_fence_after();
+                multiply(da, held_desc, x.rank);
+                continue;
+              }
+              for (int block = 0; block < x.blocks; ++block) {
                 ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
                 if (!ok) break;
-                s_low = ring + stage * stage_bytes, low_stage = stage, first = false;
+                tc_fence_after();
+                const uint32_t sa = ring + stage * stage_bytes;
+                multiply(low_desc | (sa >> 4), high_desc | ((sa + kABytes) >> 4), x.rank - block * x.unit);
+                release_stage(stage);
                 if (++stage == p.stages) stage = 0, phase ^= 1u;
               }
-              if (g != held_g || t.n0 != held_n) {
-                if (highs > 0) {  // all that read the last one has been issued
-                  const uint32_t done = bars + (HIGH_EMPTY + (highs - 1) % x.slots) * 8;
-                  if constexpr (kPair) umma_commit_pair_warp(done);
-                  else umma_commit_warp(done);
-                }
-                ok = mbar_wait_warp(bars + (HIGH_FULL + highs % x.slots) * 8, highs / x.slots & 1, abort_flag);
-                if (!ok) break;
-                ++highs, held_g = g, held_n = t.n0;
-              }
-              tc_fence_after();
-              multiply(s_low, held + (highs - 1) % x.slots * (b_rows * x.unit * 2), x.rank);
-              continue;
             }
-            for (int block = 0; block < x.blocks; ++block) {
-              ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t sa = ring + stage * stage_bytes;
-              multiply(sa, sa + kABytes, x.rank - block * x.unit);
-              if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + stage) * 8);
-              else umma_commit_warp(bars + (EMPTY + stage) * 8);
-              if (++stage == p.stages) stage = 0, phase ^= 1u;
-            }
-          }
-          if (!first) {
-            if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + low_stage) * 8);
-            else umma_commit_warp(bars + (EMPTY + low_stage) * 8);
+            if (ok && low_stage >= 0) release_stage(low_stage);
           }
         }
         if (!ok) break;
         if constexpr (kPair) umma_commit_pair_warp(bars + (ACC_FULL + buffer) * 8);
         else umma_commit_warp(bars + (ACC_FULL + buffer) * 8);
-        look_ahead(i + 1);
+        ahead.look(p, x, i + 1, items, units);
       }
     }
   } else {
