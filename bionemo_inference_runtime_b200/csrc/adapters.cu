@@ -205,14 +205,15 @@ transpose_up_kernel(const TransposeParams p) {
 
 // ---- gradients of the adapters' weights ---------------------------------------------------------------------------------
 //
-// dD_g = sum over the rows of g of dt^T x, dU_g likewise of t and dz: bound by HBM or L2 (x and dz once; two operations a byte and rank
-// are nothing beside it).  A block takes 128 columns, one adapter, up to 64 ranks and a part of the rows, 64 at a time through a ring of
-// stages that cp.async fills: rows of other adapters, and what is behind the last column, are filled with zeros on the way, so
-// nothing of them is read.  Products m16n8k16 with ranks as rows and the tensor's rows along k: both operands lie with k across
-// and are transposed on their way from shared memory.  Of several adapters a block first lists the groups of 64 rows that hold
-// its own.  Parts are written in 32 bits and joined in a fixed order: results repeat bit by bit.
-constexpr int kGradRows = 64, kGradColumns = 128, kGradChunks = 1024;
-// (up to 16, 32 or 64 ranks with their two terms are a row of 64, 128 or 256 bytes)
+// dD_g = sum over the rows of g of dt^T x, dU_g likewise of t and dz: bound by HBM or L2 (x and dz once), with 64 ranks by the warp-wide
+// products.  A block takes 128 columns, one adapter, up to 64 ranks and a part of the rows, 64 at a time through a ring of stages that a
+// ninth warp fills by TMA.  Products m16n8k16 with ranks as rows and the tensor's rows along k: both operands lie with k across and
+// are transposed on their way from shared memory.  Of several adapters a block first lists the groups of 64 rows that hold its own;
+// in a group that others have a part of, their rows are cleared in the operands' registers, so that infinities and NaN in them stay
+// out.  Parts are written in 32 bits and joined in a fixed order: results repeat bit by bit.  (Filled by cp.async from all threads,
+// 147456 rows of 128 and 1024 columns, rank 16: 89 us.)
+constexpr int kGradRows = 64, kGradColumns = 128, kGradChunks = 1024, kGradWarps = 8;
+// (up to 16, 32 or 64 ranks with their two terms are rows of 64 or 128 bytes, or two blocks of the latter)
 constexpr int kGradV = kGradRows * kGradColumns * 2;
 __host__ __device__ constexpr int grad_stage(int tiles) { return kGradV + kGradRows * tiles * 64; }
 __host__ __device__ constexpr int grad_stages(int tiles) { return tiles == 4 ? 3 : 4; }
@@ -220,52 +221,75 @@ __host__ __device__ constexpr int grad_stages(int tiles) { return tiles == 4 ? 3
 struct GradParams {
   LowGrad job[2];
   AdapterIndex index;
-  long long rows;
-  int rank, rank_groups, slabs0, chunks_part, accumulate;
+  int rows, rank, rank_groups, slabs0, chunks_part, accumulate;
+  int* status;
 };
-__device__ __forceinline__ void copy_or_zero(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
+struct GradMaps {
+  CUtensorMap t[2], v[2];
+};
 __device__ __forceinline__ void ldmatrix4_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
 }
+// Halves that stay of a pair of rows, whose bits are bits[0] and bits[1].
+__device__ __forceinline__ uint32_t pair_mask(uint32_t bits) { return ((bits & 1u) ? 0xFFFFu : 0u) | ((bits & 2u) ? 0xFFFF0000u : 0u); }
+
 template <typename T, int kTiles>  // tiles of 16 ranks
-__global__ void __launch_bounds__(256, 2)
-low_grad_kernel(const GradParams p) {
-  constexpr int kStages = grad_stages(kTiles), kStage = grad_stage(kTiles), kRowVecs = 4 * kTiles;
-  extern __shared__ __align__(128) uint8_t stages[];
+__global__ void __launch_bounds__((kGradWarps + 1) * 32, 2)
+low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
+  constexpr int kStages = grad_stages(kTiles), kStage = grad_stage(kTiles), kUnit = kTiles == 1 ? 16 : 32;
+  extern __shared__ uint8_t raw[];
   __shared__ uint32_t masks[kGradChunks][2];
   __shared__ uint16_t list[kGradChunks];
-  __shared__ int listed;
+  __shared__ __align__(8) uint64_t bars[2 * kStages];  // full, then empty
+  __shared__ int listed, aborted[2];
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u, bar0 = smem_u32(bars);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    aborted[0] = aborted[1] = 0;
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(bar0 + i * 8, 1);
+      mbar_init(bar0 + (kStages + i) * 8, kGradWarps);
+    }
+    fence_mbar_init();
+  }
   pdl_trigger();
   pdl_wait();
-  const bool second = int(blockIdx.x) >= p.slabs0;
+  const int second = int(blockIdx.x) >= p.slabs0;
   const LowGrad& job = second ? p.job[1] : p.job[0];
   const int slab = int(blockIdx.x) - (second ? p.slabs0 : 0), slabs_plane = (job.columns + kGradColumns - 1) / kGradColumns;
   const int plane = slab / slabs_plane, c0 = (slab - plane * slabs_plane) * kGradColumns;
   const int g = blockIdx.z / p.rank_groups, r0 = int(blockIdx.z % unsigned(p.rank_groups)) * 64;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long first_row = (long long)blockIdx.y * p.chunks_part * kGradRows;
-  const long long rows = p.rows - first_row < (long long)p.chunks_part * kGradRows ? p.rows - first_row : (long long)p.chunks_part * kGradRows;
-  const int chunks = rows > 0 ? int((rows + kGradRows - 1) / kGradRows) : 0;
+  const int first_row = int(blockIdx.y) * p.chunks_part * kGradRows;
+  const int rows = min(p.rows - first_row, p.chunks_part * kGradRows), chunks = rows > 0 ? (rows + kGradRows - 1) / kGradRows : 0;
 
-#pragma unroll 4
-  for (int c = warp; c < chunks; c += 8) {
+  // Bits of a group's rows that are g's.  (Rows behind the last one are zeros in shared memory, whoever's they are.)
+  for (int c0 = warp; c0 < chunks; c0 += 4 * (kGradWarps + 1)) {
+    int own[4][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const long long row = c * kGradRows + h * 32 + lane;
-      const uint32_t own = __ballot_sync(0xffffffffu, row < rows && adapter_of(p.index, uint32_t(first_row + row)) == g);
-      if (lane == 0) masks[c][h] = own;
-    }
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = (c0 + u * (kGradWarps + 1)) * kGradRows + h * 32 + lane;
+        own[u][h] = row < rows ? adapter_of(p.index, uint32_t(first_row + row)) : g;
+      }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t bits = __ballot_sync(0xffffffffu, own[u][h] == g);
+        const int c = c0 + u * (kGradWarps + 1);
+        if (lane == 0 && c < chunks) masks[c][h] = bits;
+      }
   }
   __syncthreads();
   if (warp == 0) {
     int n = 0;
     for (int c = 0; c < chunks; c += 32) {
-      const bool in = c + lane < chunks && (masks[c + lane < chunks ? c + lane : 0][0] | masks[c + lane < chunks ? c + lane : 0][1]) != 0;
+      const int at = c + lane < chunks ? c + lane : 0;
+      const bool in = c + lane < chunks && (masks[at][0] | masks[at][1]) != 0;
       const uint32_t vote = __ballot_sync(0xffffffffu, in);
       if (in) list[n + __popc(vote & ((1u << lane) - 1u))] = uint16_t(c + lane);
       n += __popc(vote);
@@ -274,81 +298,93 @@ low_grad_kernel(const GradParams p) {
   }
   __syncthreads();
   const int count = listed;
+  volatile int* abort_flag = aborted;
 
-  const T* v = static_cast<const T*>(job.v) + plane * job.v_plane + c0;
-  const T* t = static_cast<const T*>(job.t) + r0 * 2;
-  const uint32_t base = smem_u32(stages);
-  const int v_column = (threadIdx.x & 15) * 8, v_bytes = max(0, min(16, (job.columns - c0 - v_column) * 2));
-  const int t_vec = threadIdx.x % kRowVecs, pitch_t = low_pitch(p.rank);
-  const bool t_in = r0 * 2 + t_vec * 8 < pitch_t;
-  // (rows of 64 bytes: two of them to the 128 that the banks span)
-  auto t_at = [&](int row, int vec) { return kGradV + row * kRowVecs * 16 + ((kTiles == 1 ? vec ^ (row >> 1 & 3) : vec ^ (row & 7)) << 4); };
-  auto issue = [&](int i) {
-    if (i < count) {
-      const int c = list[i];
-      const uint32_t stage = base + (i % kStages) * kStage;
+  if (warp == kGradWarps) {
+    if (lane == 0) {
+      const CUtensorMap *tm_t = &maps.t[second], *tm_v = &maps.v[second];
+      bool ok = true;
+      int i = 0;
+      for (; i < count; ++i) {
+        const int s = i % kStages;
+        ok = mbar_wait(bar0 + (kStages + s) * 8, (i / kStages & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        const uint32_t stage = base + s * kStage, bar = bar0 + s * 8;
+        const int row = first_row + list[i] * kGradRows;
+        mbar_expect_tx(bar, kStage);
+        tma_load_3d(stage, tm_v, bar, c0, row, plane);
+        tma_load_3d(stage + kGradV / 2, tm_v, bar, c0 + 64, row, plane);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = (threadIdx.x >> 4) + 16 * j;
-        const bool own = masks[c][row >> 5] >> (row & 31) & 1u;
-        const int bytes = own ? v_bytes : 0;
-        const T* from = bytes > 0 ? v + (first_row + c * kGradRows + row) * job.v_pitch + v_column : static_cast<const T*>(job.v);
-        copy_or_zero(stage + row * 256 + (((threadIdx.x & 15) ^ (row & 7)) << 4), from, bytes);
+        for (int b = 0; b < (kTiles == 4 ? 2 : 1); ++b) tma_load_3d(stage + kGradV + b * kGradRows * 128, tm_t, bar, 2 * r0 + b * 64, row, 0);
       }
-#pragma unroll
-      for (int row = threadIdx.x / kRowVecs; row < kGradRows; row += 256 / kRowVecs) {
-        const bool own = t_in && (masks[c][row >> 5] >> (row & 31) & 1u);
-        const T* from = own ? t + (first_row + c * kGradRows + row) * pitch_t + t_vec * 8 : static_cast<const T*>(job.t);
-        copy_or_zero(stage + t_at(row, t_vec), from, own ? 16 : 0);
-      }
+      if (!ok)  // copies still in flight get a bounded chance to land
+        for (int j = i > kStages ? i - kStages : 0; j < i; ++j) mbar_wait(bar0 + j % kStages * 8, j / kStages & 1, abort_flag + 1);
     }
-    norm::copy_commit();
-  };
-  float acc[kTiles][2][4] = {};
-  for (int i = 0; i < kStages - 1; ++i) issue(i);
-  for (int i = 0; i < count; ++i) {
-    norm::copy_wait<kStages - 2>();
-    __syncthreads();  // this group has arrived, and all warps are done with the one before, whose stage is filled again
-    issue(i + kStages - 1);
-    const uint32_t stage = base + (i % kStages) * kStage;
+  } else {
+    float acc[kTiles][2][4] = {};
+    // rows of 128 bytes (t of 16 ranks: 64) whose 16-byte vectors are swizzled by the row
+    const int vr = lane & 15, tr = (lane >> 4) * 8 + (lane & 7);
+    const uint32_t v_at = (warp >> 2) * (kGradV / 2) + vr * 128 + ((((warp & 3) * 2 + (lane >> 4)) ^ (vr & 7)) << 4);
+    bool ok = true;
+    for (int i = 0; i < count; ++i) {
+      const int s = i % kStages;
+      ok = mbar_wait_warp(bar0 + s * 8, i / kStages & 1, abort_flag);
+      if (!ok) break;
+      const uint32_t stage = base + s * kStage;
+      const uint32_t bits0 = masks[list[i]][0], bits1 = masks[list[i]][1];
+      auto walk = [&](auto&& mask) {
 #pragma unroll
-    for (int k = 0; k < kGradRows; k += 16) {
-      const int vr = k + (lane & 15), vc = warp * 2 + (lane >> 4);
-      uint32_t b[4];
-      ldmatrix4_t(stage + vr * 256 + ((vc ^ (vr & 7)) << 4), b);
+        for (int k = 0; k < kGradRows; k += 16) {
+          uint32_t b[4];
+          ldmatrix4_t(stage + v_at + k * 128, b);
+          mask(k, b[0], b[2], b[1], b[3]);
 #pragma unroll
-      for (int m = 0; m < 2 * kTiles; ++m) {  // tiles of a block's first, then of its second terms
-        constexpr int kBlock = kTiles == 1 ? 1 : 2;
-        const int tr = k + (lane >> 4) * 8 + (lane & 7), tile = m / (2 * kBlock) * kBlock + m % kBlock;
-        uint32_t a[4];
-        ldmatrix4_t(stage + t_at(tr, m * 2 + (lane >> 3 & 1)), a);
-        mma16816<T>(acc[tile][0], a[0], a[1], a[2], a[3], b[0], b[1]);
-        mma16816<T>(acc[tile][1], a[0], a[1], a[2], a[3], b[2], b[3]);
+          for (int m = 0; m < 2 * kTiles; ++m) {  // tiles of a block's first, then of its second terms
+            constexpr int kBlock = kUnit / 16;
+            const int tile = m / (2 * kBlock) * kBlock + m % kBlock, row = k + tr;
+            const uint32_t t_at = kTiles == 1 ? row * 64 + ((m * 2 + (lane >> 3 & 1)) ^ (row >> 1 & 3)) * 16
+                                              : m / 4 * (kGradRows * 128) + row * 128 + ((m % 4 * 2 + (lane >> 3 & 1)) ^ (row & 7)) * 16;
+            uint32_t a[4];
+            ldmatrix4_t(stage + kGradV + t_at, a);
+            mask(k, a[0], a[1], a[2], a[3]);
+            mma16816<T>(acc[tile][0], a[0], a[1], a[2], a[3], b[0], b[1]);
+            mma16816<T>(acc[tile][1], a[0], a[1], a[2], a[3], b[2], b[3]);
+          }
+        }
+      };
+      if ((bits0 & bits1) == ~0u) {
+        walk([](int, uint32_t&, uint32_t&, uint32_t&, uint32_t&) {});
+      } else {
+        walk([&](int k, uint32_t& x0, uint32_t& x1, uint32_t& y0, uint32_t& y1) {  // rows k + 2 t, + 1, and those eight further
+          const uint32_t bits = (k < 32 ? bits0 : bits1) >> ((k & 31) + (lane & 3) * 2), lo = pair_mask(bits), hi = pair_mask(bits >> 8);
+          x0 &= lo, x1 &= lo, y0 &= hi, y1 &= hi;
+        });
       }
+      mbar_arrive_warp_after_reads(bar0 + (kStages + s) * 8);
     }
+    const int pitch = int(low_grad_columns(job.columns, job.planes)), plane_columns = pitch / job.planes, adapters = gridDim.z / p.rank_groups;
+    float* part = job.part + ((long long)blockIdx.y * adapters + g) * p.rank * pitch + plane * plane_columns;
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = r0 + m * 16 + (lane >> 2) + 8 * (e >> 1), c = c0 + warp * 16 + n * 8 + (lane & 3) * 2 + (e & 1);
+          if (r >= p.rank || c >= job.columns) continue;
+          float* to = part + (long long)r * pitch + c;
+          *to = p.accumulate ? *to + acc[m][n][e] : acc[m][n][e];
+        }
   }
-  norm::copy_wait<0>();
-  const long long pitch = low_grad_columns(job.columns, job.planes), plane_columns = pitch / job.planes;
-  const int adapters = gridDim.z / p.rank_groups;
-  float* part = job.part + ((long long)blockIdx.y * adapters + g) * p.rank * pitch + plane * plane_columns;
-#pragma unroll
-  for (int m = 0; m < kTiles; ++m)
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = r0 + m * 16 + (lane >> 2) + 8 * (e >> 1), c = c0 + warp * 16 + n * 8 + (lane & 3) * 2 + (e & 1);
-        if (r >= p.rank || c >= job.columns) continue;
-        float* to = part + r * pitch + c;
-        *to = p.accumulate ? *to + acc[m][n][e] : acc[m][n][e];
-      }
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) *p.status = B200TA_ERR_DEVICE_WAIT;
 }
 
 template <typename T, int kTiles>
-int launch_grad(DeviceState* st, dim3 grid, void* stream, const GradParams& p) {
+int launch_grad(DeviceState* st, dim3 grid, void* stream, const GradParams& p, const GradMaps& maps) {
   constexpr int kIndex = (kTiles == 4 ? 2 : kTiles - 1) + (__is_same(T, __half) ? 3 : 0);
-  return launch_kernel(st, KernelId(kKernelLowGrad + kIndex), low_grad_kernel<T, kTiles>, grid, 256, grad_stages(kTiles) * grad_stage(kTiles),
-                       stream, p);
+  return launch_kernel(st, KernelId(kKernelLowGrad + kIndex), low_grad_kernel<T, kTiles>, grid, (kGradWarps + 1) * 32,
+                       grad_stages(kTiles) * grad_stage(kTiles) + 1024, stream, p, maps);
 }
 
 // Sums over the parts: a thread takes one value, or eight ranks of a column whose results lie together, of every kSlices-th part; the
@@ -426,7 +462,10 @@ int run_low(const LowProduct& m, void* stream) {
   DeviceState* st = nullptr;
   const int rc = get_device_state(&st);
   if (rc != B200TA_OK) return rc;
-  if (m.rows > 512 && !by_warps(m)) return run_matmul_low(m, stream);
+  // tiles of 128 rows, unless those of several requests are too few to fill the device
+  const int64_t tiles = (m.rows + 127) / 128;
+  const bool mixed = m.index.index != nullptr && m.index.count > 1 && m.index.rows_per_index < 128;
+  if (m.rows > 512 && !by_warps(m) && !(mixed && tiles < st->num_sms)) return run_matmul_low(m, stream);
   if (m.f16) return m.aligned ? launch_low<__half, true>(st, m, stream) : launch_low<__half, false>(st, m, stream);
   return m.aligned ? launch_low<__nv_bfloat16, true>(st, m, stream) : launch_low<__nv_bfloat16, false>(st, m, stream);
 }
@@ -456,19 +495,34 @@ int run_low_grads(const LowGrads& m, void* stream) {
   const int rc = get_device_state(&st);
   if (rc != B200TA_OK) return rc;
   GradParams p{};
+  GradMaps maps{};
+  const int tiles = m.rank <= 16 ? 1 : m.rank <= 32 ? 2 : 4, t_row = tiles == 1 ? 32 : 64;
+  for (int i = 0; i < 2; ++i) {
+    const LowGrad& j = m.job[i];
+    if (j.v == nullptr) continue;
+    const uint64_t dims[3] = {uint64_t(j.columns), uint64_t(m.rows), uint64_t(j.planes)};
+    const uint64_t strides[2] = {uint64_t(j.v_pitch) * 2, uint64_t(j.planes > 1 ? j.v_plane : j.v_pitch) * 2};
+    const uint32_t box[3] = {64, kGradRows, 1};
+    int rc = encode_tensor_map(&maps.v[i], j.v, 2, 3, dims, strides, box, SWZ_128, "adapters");
+    if (rc != B200TA_OK) return rc;
+    const uint64_t t_dims[3] = {uint64_t(low_pitch(m.rank)), uint64_t(m.rows), 1};
+    const uint64_t t_strides[2] = {uint64_t(low_pitch(m.rank)) * 2, uint64_t(low_pitch(m.rank)) * 2};
+    const uint32_t t_box[3] = {uint32_t(t_row), kGradRows, 1};
+    rc = encode_tensor_map(&maps.t[i], j.t, 2, 3, t_dims, t_strides, t_box, tiles == 1 ? SWZ_64 : SWZ_128, "adapters");
+    if (rc != B200TA_OK) return rc;
+  }
   auto slabs_of = [](const LowGrad& j) { return j.v == nullptr ? 0 : j.planes * ((j.columns + kGradColumns - 1) / kGradColumns); };
-  p.job[0] = m.job[0], p.job[1] = m.job[1], p.index = m.index, p.rows = m.rows, p.rank = m.rank, p.rank_groups = (m.rank + 63) / 64;
-  p.slabs0 = slabs_of(m.job[0]), p.accumulate = m.accumulate;
+  p.job[0] = m.job[0], p.job[1] = m.job[1], p.index = m.index, p.rows = int(m.rows), p.rank = m.rank, p.rank_groups = (m.rank + 63) / 64;
+  p.slabs0 = slabs_of(m.job[0]), p.accumulate = m.accumulate, p.status = st->status_dev;
   const int64_t chunks = (m.rows + kGradRows - 1) / kGradRows;
   p.chunks_part = int((chunks + m.parts - 1) / m.parts);
   B200TA_REQUIRE(p.chunks_part <= kGradChunks, "adapters: too many rows for %d parts", m.parts);
   // (all columns of a part's rows at a time: memory is read in whole rows)
   const dim3 grid{unsigned(p.slabs0 + slabs_of(m.job[1])), unsigned(m.parts), unsigned(m.index.count * p.rank_groups)};
-  const int tiles = m.rank <= 16 ? 1 : m.rank <= 32 ? 2 : 4;
-  int (*launch)(DeviceState*, dim3, void*, const GradParams&);
+  int (*launch)(DeviceState*, dim3, void*, const GradParams&, const GradMaps&);
   if (m.f16) launch = tiles == 1 ? launch_grad<__half, 1> : tiles == 2 ? launch_grad<__half, 2> : launch_grad<__half, 4>;
   else launch = tiles == 1 ? launch_grad<__nv_bfloat16, 1> : tiles == 2 ? launch_grad<__nv_bfloat16, 2> : launch_grad<__nv_bfloat16, 4>;
-  return launch(st, grid, stream, p);
+  return launch(st, grid, stream, p, maps);
 }
 
 int run_low_join(const LowGrads& m, void* stream) {
