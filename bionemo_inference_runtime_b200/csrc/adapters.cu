@@ -163,7 +163,7 @@ low_product_kernel(const LowProduct p, int share) {
 
 // Each row's own adapter read for it alone, rather than a pass over the rows' k for each adapter among them.
 bool by_warps(const LowProduct& m) {
-  return m.rows <= 16 || (m.index.index != nullptr && m.index.count > 1 && m.index.rows_per_index < 8 && m.rows <= 4096);
+  return m.rows <= 32 || (m.index.index != nullptr && m.index.count > 1 && m.index.rows_per_index < 8 && m.rows <= 4096);
 }
 template <typename T, bool kVec>
 int launch_low(DeviceState* st, const LowProduct& m, void* stream) {

@@ -202,7 +202,11 @@ namespace {
 // the tensor cores would leave all but N / 64 SMs idle and wait for tensor memory, and products by FMA want every row of x in
 // registers for each column (13 rows, 960 -> 4648 gated: 45 us so, now 8; 16 rows, 4096 -> 4096: 130 and 18; one row the same).
 // Rows that are not 16-byte aligned are shifted into place.
-constexpr int kFewRows = 16;
+//
+// With adapters up to 64 rows: single tokens of many requests have as many adapters in a tile, and the tensor cores take them one after
+// the other (64 rows of 2048 -> 4096 with an adapter each, rank 16: 38 us).  Here a value's low-rank sum is its own thread's.  The kernel
+// of the low-rank values runs beside the products, which do not wait for it.
+constexpr int kFewRows = 16, kFewAdapterRows = 64;
 
 struct FewParams {
   const void *x, *w, *bias, *residual;
@@ -243,7 +247,8 @@ __device__ __forceinline__ uint4 load_row(const T* row, int k, int K) {
   return K - k >= 8 ? v : norm::first<T>(v, K - k);
 }
 
-constexpr int kFewWarps = 16, kFewColumns = 16;  // of a block, at most
+constexpr int kFewColumns = 16;  // of a block
+__host__ __device__ constexpr int few_warps(int eights, int parts) { return eights * parts <= 4 ? 16 : 64 / (eights * parts); }  // at most
 // The sum of low[r] (both terms) high[r] over the ranks.
 template <typename T>
 __device__ __forceinline__ float low_sum(const T* low, const T* high, int rank) {
@@ -268,9 +273,9 @@ __device__ __forceinline__ float low_sum(const T* low, const T* high, int rank) 
 }
 
 template <typename T, bool kTwo, int kEights, bool kVec>
-__global__ void __launch_bounds__(kFewWarps * 32, 1)
+__global__ void __launch_bounds__(few_warps(kEights, kTwo ? 2 : 1) * 32, 1)
 few_rows_kernel(const FewParams p) {
-  __shared__ float joined[kFewWarps][kTwo ? 2 : 1][kEights * 8][kFewColumns + 1];
+  __shared__ float joined[few_warps(kEights, kTwo ? 2 : 1)][kTwo ? 2 : 1][kEights * 8][kFewColumns + 1];
   pdl_trigger();
   if (p.adapters.low == nullptr) pdl_wait();  // (otherwise what came before the kernel of the low-rank values is complete)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, n0 = blockIdx.x * kFewColumns, warps = blockDim.x >> 5;
@@ -285,7 +290,7 @@ few_rows_kernel(const FewParams p) {
 #pragma unroll
   for (int e = 0; e < kEights; ++e) x[e] = static_cast<const T*>(p.x) + min(g + 8 * e, p.rows - 1) * p.xs;
   float acc[kParts][kEights][4] = {};
-#pragma unroll 4
+#pragma unroll(kEights > 2 ? 2 : 4)
   for (int k = warp * 32; k < p.K; k += warps * 32) {
     uint4 a[kParts][2], b[kEights];
 #pragma unroll
@@ -309,44 +314,48 @@ few_rows_kernel(const FewParams p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) joined[warp][i][e * 8 + t * 2 + (j & 1)][g + 8 * (j >> 1)] = acc[i][e][j];
   __syncthreads();
-  const int row = threadIdx.x / kFewColumns, c = threadIdx.x % kFewColumns, n = n0 + c;
-  if (row >= p.rows || n >= p.N) return;
-  float v = 0.f, gate = 0.f;
-  for (int i = 0; i < warps; ++i) {
-    v += joined[i][0][row][c];
-    if constexpr (kTwo) gate += joined[i][1][row][c];
-  }
-  if (p.adapters.low != nullptr) {
-    pdl_wait();
-    const int a = adapter_of(p.adapters.index, uint32_t(row));
-    if (a != kNoAdapter) {
-      const T* low = static_cast<const T*>(p.adapters.low) + row * low_pitch(p.adapters.rank);
-      const T* high = static_cast<const T*>(p.adapters.high) + ((long long)a * (kTwo ? 2 * p.N : p.N) + n) * p.adapters.high_pitch;
-      v += low_sum(low, high, p.adapters.rank);
-      if constexpr (kTwo) gate += low_sum(low, high + (long long)p.N * p.adapters.high_pitch, p.adapters.rank);
+  const int c = threadIdx.x % kFewColumns, n = n0 + c;
+  if (p.adapters.low != nullptr) pdl_wait();
+  for (int row = threadIdx.x / kFewColumns; row < p.rows && n < p.N; row += blockDim.x / kFewColumns) {
+    float v = 0.f, gate = 0.f;
+    for (int i = 0; i < warps; ++i) {
+      v += joined[i][0][row][c];
+      if constexpr (kTwo) gate += joined[i][1][row][c];
     }
+    if (p.adapters.low != nullptr) {
+      const int a = adapter_of(p.adapters.index, uint32_t(row));
+      if (a != kNoAdapter) {
+        const T* low = static_cast<const T*>(p.adapters.low) + row * low_pitch(p.adapters.rank);
+        const T* high = static_cast<const T*>(p.adapters.high) + ((long long)a * (kTwo ? 2 * p.N : p.N) + n) * p.adapters.high_pitch;
+        v += low_sum(low, high, p.adapters.rank);
+        if constexpr (kTwo) gate += low_sum(low, high + (long long)p.N * p.adapters.high_pitch, p.adapters.rank);
+      }
+    }
+    const T* bias = static_cast<const T*>(p.bias);
+    if (bias != nullptr) {
+      v += static_cast<float>(bias[n]);
+      if (kTwo) gate += static_cast<float>(bias[n + p.N]);
+    }
+    if (p.saved != nullptr) {
+      float* s = static_cast<float*>(p.saved) + row * p.ss + n;
+      s[0] = v;
+      if (kTwo) s[p.ss / 2] = gate;
+    }
+    float a, slope;
+    activate_any(p.activation, kTwo ? gate : v, a, slope);
+    if (kTwo) a *= v;
+    if (p.residual != nullptr) a += static_cast<float>(static_cast<const T*>(p.residual)[row * p.rs + n]);
+    static_cast<T*>(p.y)[row * p.ys + n] = static_cast<T>(a);
   }
-  const T* bias = static_cast<const T*>(p.bias);
-  if (bias != nullptr) {
-    v += static_cast<float>(bias[n]);
-    if (kTwo) gate += static_cast<float>(bias[n + p.N]);
-  }
-  if (p.saved != nullptr) {
-    float* s = static_cast<float*>(p.saved) + row * p.ss + n;
-    s[0] = v;
-    if (kTwo) s[p.ss / 2] = gate;
-  }
-  float a, slope;
-  activate_any(p.activation, kTwo ? gate : v, a, slope);
-  if (kTwo) a *= v;
-  if (p.residual != nullptr) a += static_cast<float>(static_cast<const T*>(p.residual)[row * p.rs + n]);
-  static_cast<T*>(p.y)[row * p.ys + n] = static_cast<T>(a);
 }
 
+template <typename T, bool kTwo, int kEights>
+auto pick_few(bool vec) {
+  return vec ? &few_rows_kernel<T, kTwo, kEights, true> : &few_rows_kernel<T, kTwo, kEights, false>;
+}
 template <typename T, bool kTwo>
 auto pick_few(int rows, bool vec) {
-  if (rows <= 8) return vec ? &few_rows_kernel<T, kTwo, 1, true> : &few_rows_kernel<T, kTwo, 1, false>;
-  return vec ? &few_rows_kernel<T, kTwo, 2, true> : &few_rows_kernel<T, kTwo, 2, false>;
+  return rows <= 8 ? pick_few<T, kTwo, 1>(vec) : rows <= 16 ? pick_few<T, kTwo, 2>(vec) : rows <= 32 ? pick_few<T, kTwo, 4>(vec) : pick_few<T, kTwo, 8>(vec);
 }
 template <typename T>
 auto pick_few(int rows, bool vec, bool two) {
@@ -753,7 +762,7 @@ int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const vo
   B200TA_REQUIRE(x && w && y, "dense: NULL pointer");
   B200TA_REQUIRE(!gated || residual == nullptr, "dense: a gated layer has no residual");
   B200TA_REQUIRE(!gated || saved == nullptr || ss % 16 == 0, "dense: the pitch of a gated layer's saved values must be a multiple of 16");
-  if (rows <= kFewRows) {
+  if (rows <= (adapters != nullptr ? kFewAdapterRows : kFewRows)) {
     DeviceState* st = nullptr;
     rc = get_device_state(&st);
     if (rc != B200TA_OK) return rc;
@@ -761,7 +770,8 @@ int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const vo
     FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation, {}};
     if (adapters != nullptr) p.adapters = *adapters;
     // sixteen warps where blocks are few (three rows, 1536 -> 384: 9 us instead of 11), eight otherwise, of which more blocks fit
-    const int blocks = (N + kFewColumns - 1) / kFewColumns, warps = blocks <= st->num_sms ? kFewWarps : kFewWarps / 2;
+    const int eights = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 8, blocks = (N + kFewColumns - 1) / kFewColumns;
+    const int warps = std::min(few_warps(eights, gated ? 2 : 1), blocks <= st->num_sms ? 16 : 8);
     return launch_kernel(st, kKernelDenseHelpers, f16 ? pick_few<__half>(int(rows), vec, gated) : pick_few<__nv_bfloat16>(int(rows), vec, gated),
                          dim3(unsigned(blocks)), warps * 32, 0, stream, p);
   }
@@ -993,7 +1003,7 @@ int b200ta_adapter_dense(const void* x, int64_t xs, const void* w, int64_t ws, c
   B200TA_REQUIRE(x && w && y, "adapter_dense: NULL pointer");
   if ((rc = check_adapters("adapter_dense", a, low)) != B200TA_OK) return rc;
   const bool aligned = rows_aligned(x, xs) && rows_aligned(a->down, a->down_row_stride);
-  B200TA_REQUIRE(rows <= kFewRows || (aligned && rows_aligned(a->up, a->up_row_stride)),
+  B200TA_REQUIRE(rows <= kFewAdapterRows || (aligned && rows_aligned(a->up, a->up_row_stride)),
                  "adapter_dense: what is read must be 16-byte aligned with row strides that are multiples of 8 elements");
   LowProduct q{};
   q.x = x, q.a = a->down, q.low = low, q.scale = a->scale, q.scale_all = a->scale_all;
@@ -1003,6 +1013,8 @@ int b200ta_adapter_dense(const void* x, int64_t xs, const void* w, int64_t ws, c
   const LowRank adapters{q.index, a->rank, low, a->up, a->up_row_stride};
   return dense_forward(x, xs, w, ws, bias, residual, rs, y, ys, saved, ss, dtype, activation, gated, rows, K, N, &adapters, stream);
 }
+
+int b200ta_adapter_few_rows(void) { return b200ta::kFewAdapterRows; }
 
 size_t b200ta_adapter_low_bytes(int rank) { return rank > 0 && rank <= b200ta::kMaxRank ? size_t(b200ta::low_pitch(rank)) * 2 : 0; }
 

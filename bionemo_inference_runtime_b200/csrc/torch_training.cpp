@@ -22,7 +22,7 @@ struct Library {
 #define B200TA_ENTRIES(X)                                                                                                \
   X(layer_norm) X(layer_norm_workspace_bytes) X(layer_norm_backward) X(dense_few_rows) X(dense_keeps) X(dense)              \
   X(dense_backward_workspace_bytes) X(dense_backward) X(copy_rows) X(dropout)      \
-  X(adapter_dense) X(adapter_low_bytes) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
+  X(adapter_dense) X(adapter_low_bytes) X(adapter_few_rows) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
   B200TA_ENTRIES(B200TA_ENTRY)
 #undef B200TA_ENTRY
 } lib;
@@ -363,7 +363,7 @@ std::tuple<at::Tensor, at::Tensor, Maybe> adapter_dense(const at::Tensor& x, con
   const Layer l = layer_of(x, w, bias, activation, gated);
   const c10::cuda::CUDAGuard guard(x.device());
   Copies copies, low_copies;
-  const bool few = l.rows <= lib.dense_few_rows();
+  const bool few = l.rows <= lib.adapter_few_rows();
   const Adapting a = adapters_of(x, l, w.size(0), down, up, index, scale, scale_all, few, low_copies);
   const at::Tensor y = or_out(out, x, l.N);
   if (residual) require_like("residual", *residual, x, y.sizes());
