@@ -205,15 +205,23 @@ namespace {
 //
 // With adapters up to 64 rows: single tokens of many requests have as many adapters in a tile, and the tensor cores take them one after
 // the other (64 rows of 2048 -> 4096 with an adapter each, rank 16: 38 us).  Here a value's low-rank sum is its own thread's.  The kernel
-// of the low-rank values runs beside the products, which do not wait for it.
+// of the low-rank values runs beside the products, which do not wait for it; a few of a row or two are made in each block instead (one
+// row, 384 -> 1536 gated, rank 16: one launch, 6 us with its way through the host, where two take 9).
 constexpr int kFewRows = 16, kFewAdapterRows = 64;
+constexpr int kOwnLow = 64, kOwnLowReads = 32768;  // values that a block makes itself, and elements of the adapters it reads for them
 
 struct FewParams {
   const void *x, *w, *bias, *residual;
   void *y, *saved;
   long long xs, ws, rs, ys, ss;
   int rows, K, N, activation;
-  LowRank adapters;  // without `low`: none
+  LowRank adapters;  // without `high`: none
+  // Without `low` each block makes the low-rank values itself, and the first one writes them to low_out (may be NULL).
+  const void* down;
+  const float* scale;
+  void* low_out;
+  long long ds;
+  float scale_all;
 };
 
 template <typename T>
@@ -249,24 +257,33 @@ __device__ __forceinline__ uint4 load_row(const T* row, int k, int K) {
 
 constexpr int kFewColumns = 16;  // of a block
 __host__ __device__ constexpr int few_warps(int eights, int parts) { return eights * parts <= 4 ? 16 : 64 / (eights * parts); }  // at most
-// The sum of low[r] (both terms) high[r] over the ranks.
+// The sum over the ranks of high[r] times low[r], both terms, or own[r].
 template <typename T>
-__device__ __forceinline__ float low_sum(const T* low, const T* high, int rank) {
+__device__ __forceinline__ float low_sum(const T* low, const float* own, const T* high, int rank) {
   const int unit = low_unit(rank);
   float sum = 0.f;
   if ((reinterpret_cast<uintptr_t>(high) & 15u) == 0 && rank % 8 == 0) {
     for (int r = 0; r < rank; r += 8) {
-      float a[8], c[8], b[8];
-      load_vec<T>(low + low_place(rank, r), a);
-      load_vec<T>(low + low_place(rank, r) + unit, c);
+      float a[8], b[8];
       load_vec<T>(high + r, b);
+      if (own != nullptr) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(a[j] + c[j], b[j], sum);
+        for (int j = 0; j < 8; ++j) a[j] = own[r + j];
+      } else {
+        float c[8];
+        load_vec<T>(low + low_place(rank, r), a);
+        load_vec<T>(low + low_place(rank, r) + unit, c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] += c[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fmaf(a[j], b[j], sum);
     }
   } else {
     for (int r = 0; r < rank; ++r) {
       const T* t = low + low_place(rank, r);
-      sum = fmaf(static_cast<float>(t[0]) + static_cast<float>(t[unit]), static_cast<float>(high[r]), sum);
+      const float a = own != nullptr ? own[r] : static_cast<float>(t[0]) + static_cast<float>(t[unit]);
+      sum = fmaf(a, static_cast<float>(high[r]), sum);
     }
   }
   return sum;
@@ -276,6 +293,7 @@ template <typename T, bool kTwo, int kEights, bool kVec>
 __global__ void __launch_bounds__(few_warps(kEights, kTwo ? 2 : 1) * 32, 1)
 few_rows_kernel(const FewParams p) {
   __shared__ float joined[few_warps(kEights, kTwo ? 2 : 1)][kTwo ? 2 : 1][kEights * 8][kFewColumns + 1];
+  __shared__ float own_low[kOwnLow];
   pdl_trigger();
   if (p.adapters.low == nullptr) pdl_wait();  // (otherwise what came before the kernel of the low-rank values is complete)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, n0 = blockIdx.x * kFewColumns, warps = blockDim.x >> 5;
@@ -289,6 +307,30 @@ few_rows_kernel(const FewParams p) {
   }
 #pragma unroll
   for (int e = 0; e < kEights; ++e) x[e] = static_cast<const T*>(p.x) + min(g + 8 * e, p.rows - 1) * p.xs;
+  if (p.down != nullptr) {  // a warp for each low-rank value
+    const int rank = p.adapters.rank;
+    for (int i = warp; i < p.rows * rank; i += warps) {
+      const int row = i / rank, r = i - row * rank, a = adapter_of(p.adapters.index, uint32_t(row));
+      float sum = 0.f;
+      if (a != kNoAdapter) {
+        const T *u = static_cast<const T*>(p.x) + row * p.xs, *d = static_cast<const T*>(p.down) + ((long long)a * rank + r) * p.ds;
+#pragma unroll 2
+        for (int k = lane * 8; k < p.K; k += 256) {
+          const uint4 m = load_row<T, kVec>(u, k, p.K), n = load_row<T, kVec>(d, k, p.K);
+          const uint32_t mw[4] = {m.x, m.y, m.z, m.w}, nw[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 e = unpack2<T>(mw[j]), f = unpack2<T>(nw[j]);
+            sum = fmaf(e.x, f.x, fmaf(e.y, f.y, sum));
+          }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        sum *= p.scale != nullptr ? __ldg(p.scale + a) : p.scale_all;
+      }
+      if (lane == 0) own_low[i] = sum;
+    }
+  }
   float acc[kParts][kEights][4] = {};
 #pragma unroll(kEights > 2 ? 2 : 4)
   for (int k = warp * 32; k < p.K; k += warps * 32) {
@@ -316,19 +358,30 @@ few_rows_kernel(const FewParams p) {
   __syncthreads();
   const int c = threadIdx.x % kFewColumns, n = n0 + c;
   if (p.adapters.low != nullptr) pdl_wait();
+  if (p.low_out != nullptr && blockIdx.x == 0) {  // as the backward pass reads them, zeros behind the last rank included
+    const int half = low_pitch(p.adapters.rank) / 2;
+    for (int i = threadIdx.x; i < p.rows * half; i += blockDim.x) {
+      const int row = i / half, r = i - row * half;
+      const float v = r < p.adapters.rank ? own_low[row * p.adapters.rank + r] : 0.f;
+      T* low = static_cast<T*>(p.low_out) + row * 2 * half + low_place(p.adapters.rank, r);
+      const T rounded = static_cast<T>(v);
+      low[0] = rounded, low[low_unit(p.adapters.rank)] = static_cast<T>(v - static_cast<float>(rounded));
+    }
+  }
   for (int row = threadIdx.x / kFewColumns; row < p.rows && n < p.N; row += blockDim.x / kFewColumns) {
     float v = 0.f, gate = 0.f;
     for (int i = 0; i < warps; ++i) {
       v += joined[i][0][row][c];
       if constexpr (kTwo) gate += joined[i][1][row][c];
     }
-    if (p.adapters.low != nullptr) {
+    if (p.adapters.high != nullptr) {
       const int a = adapter_of(p.adapters.index, uint32_t(row));
       if (a != kNoAdapter) {
-        const T* low = static_cast<const T*>(p.adapters.low) + row * low_pitch(p.adapters.rank);
         const T* high = static_cast<const T*>(p.adapters.high) + ((long long)a * (kTwo ? 2 * p.N : p.N) + n) * p.adapters.high_pitch;
-        v += low_sum(low, high, p.adapters.rank);
-        if constexpr (kTwo) gate += low_sum(low, high + (long long)p.N * p.adapters.high_pitch, p.adapters.rank);
+        const T* low = static_cast<const T*>(p.adapters.low) + row * low_pitch(p.adapters.rank);
+        const float* own = p.adapters.low == nullptr ? own_low + row * p.adapters.rank : nullptr;
+        v += low_sum(low, own, high, p.adapters.rank);
+        if constexpr (kTwo) gate += low_sum(low, own, high + (long long)p.N * p.adapters.high_pitch, p.adapters.rank);
       }
     }
     const T* bias = static_cast<const T*>(p.bias);
@@ -741,8 +794,9 @@ LowPlan plan_low(const BackwardPlan& plan, int count, int rank, int64_t rows, in
   return p;
 }
 
+bool own_low_pays(int64_t rows, int rank, int K) { return rows <= 8 && rows * rank <= kOwnLow && rows * rank * K <= kOwnLowReads; }
 int check_adapters(const char* what, const b200ta_adapters* a, const void* low) {
-  B200TA_REQUIRE(a != nullptr && a->down && a->up && low, "%s: NULL pointer", what);
+  B200TA_REQUIRE(a != nullptr && a->down && a->up, "%s: NULL pointer", what);
   B200TA_REQUIRE(a->count > 0 && a->count < 16384 && a->rank > 0 && a->rank <= kMaxRank, "%s: %d adapters of rank %d (up to 16383, up to %d)", what,
                  a->count, a->rank, kMaxRank);
   B200TA_REQUIRE(rows_aligned(low, 0), "%s: low must be 16-byte aligned", what);
@@ -756,7 +810,8 @@ AdapterIndex index_of(const b200ta_adapters* a) {
 }
 
 int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* residual, int64_t rs, void* y, int64_t ys,
-                  void* saved, int64_t ss, int dtype, int activation, int gated, int64_t rows, int K, int N, const LowRank* adapters, void* stream) {
+                  void* saved, int64_t ss, int dtype, int activation, int gated, int64_t rows, int K, int N, const LowRank* adapters, const LowProduct* own_low,
+                  void* stream) {
   int rc = check_layer("dense", dtype, activation, rows, K, N);
   if (rc != B200TA_OK) return rc;
   B200TA_REQUIRE(x && w && y, "dense: NULL pointer");
@@ -766,9 +821,15 @@ int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const vo
     DeviceState* st = nullptr;
     rc = get_device_state(&st);
     if (rc != B200TA_OK) return rc;
-    const bool vec = K % 8 == 0 && rows_aligned(x, xs) && rows_aligned(w, ws), f16 = dtype == B200TA_DTYPE_F16;
-    FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation, {}};
+    const bool f16 = dtype == B200TA_DTYPE_F16;
+    FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation, {}, nullptr, nullptr, nullptr, 0, 0.f};
+    bool vec_down = true;
     if (adapters != nullptr) p.adapters = *adapters;
+    if (own_low != nullptr) {
+      p.down = own_low->a, p.ds = own_low->as, p.scale = own_low->scale, p.scale_all = own_low->scale_all, p.low_out = own_low->low;
+      vec_down = rows_aligned(p.down, p.ds);
+    }
+    const bool vec = K % 8 == 0 && rows_aligned(x, xs) && rows_aligned(w, ws) && vec_down;
     // sixteen warps where blocks are few (three rows, 1536 -> 384: 9 us instead of 11), eight otherwise, of which more blocks fit
     const int eights = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 8, blocks = (N + kFewColumns - 1) / kFewColumns;
     const int warps = std::min(few_warps(eights, gated ? 2 : 1), blocks <= st->num_sms ? 16 : 8);
@@ -968,7 +1029,8 @@ int b200ta_dense_few_rows(void) { return b200ta::kFewRows; }
 
 int b200ta_dense(const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* residual, int64_t rs, void* y,
                  int64_t ys, void* saved, int64_t ss, int dtype, int activation, int gated, int64_t rows, int K, int N, void* stream) {
-  return b200ta::dense_forward(x, xs, w, ws, bias, residual, rs, y, ys, saved, ss, dtype, activation, gated, rows, K, N, nullptr, stream);
+  return b200ta::dense_forward(x, xs, w, ws, bias, residual, rs, y, ys, saved, ss, dtype, activation, gated, rows, K, N, nullptr, nullptr,
+                               stream);
 }
 
 int b200ta_dense_keeps(int activation, int gated, int K) {
@@ -1009,10 +1071,14 @@ int b200ta_adapter_dense(const void* x, int64_t xs, const void* w, int64_t ws, c
   q.x = x, q.a = a->down, q.low = low, q.scale = a->scale, q.scale_all = a->scale_all;
   q.xs = xs, q.as = a->down_row_stride, q.rows = rows, q.K = K, q.planes = 1, q.rank = a->rank;
   q.f16 = dtype == B200TA_DTYPE_F16, q.aligned = aligned, q.index = index_of(a);
-  if ((rc = run_low(q, stream)) != B200TA_OK) return rc;
-  const LowRank adapters{q.index, a->rank, low, a->up, a->up_row_stride};
-  return dense_forward(x, xs, w, ws, bias, residual, rs, y, ys, saved, ss, dtype, activation, gated, rows, K, N, &adapters, stream);
+  const bool own = own_low_pays(rows, a->rank, K);
+  B200TA_REQUIRE(low || own, "adapter_dense: NULL pointer");
+  if (!own && (rc = run_low(q, stream)) != B200TA_OK) return rc;
+  const LowRank adapters{q.index, a->rank, own ? nullptr : low, a->up, a->up_row_stride};
+  return dense_forward(x, xs, w, ws, bias, residual, rs, y, ys, saved, ss, dtype, activation, gated, rows, K, N, &adapters, own ? &q : nullptr, stream);
 }
+
+int b200ta_adapter_dense_needs_low(int64_t rows, int rank, int K) { return !b200ta::own_low_pays(rows, rank, K); }
 
 int b200ta_adapter_few_rows(void) { return b200ta::kFewAdapterRows; }
 
@@ -1035,6 +1101,7 @@ int b200ta_adapter_dense_backward(const void* dy, int64_t dys, const void* x, in
   int rc = check_layer("adapter_dense_backward", dtype, activation, rows, K, N);
   if (rc != B200TA_OK) return rc;
   if ((rc = check_adapters("adapter_dense_backward", a, low)) != B200TA_OK) return rc;
+  B200TA_REQUIRE(low, "adapter_dense_backward: NULL pointer");
   B200TA_REQUIRE(rows_aligned(a->down, a->down_row_stride) && rows_aligned(a->up, a->up_row_stride),
                  "adapter_dense_backward: what is read must be 16-byte aligned with row strides that are multiples of 8 elements");
   return dense_gradients(dy, dys, x, xs, w, ws, bias, saved, ss, dx, dxs, dw, dbias, workspace, workspace_bytes, dtype, activation, gated, rows, K, N, a,

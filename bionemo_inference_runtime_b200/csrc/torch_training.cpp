@@ -22,7 +22,7 @@ struct Library {
 #define B200TA_ENTRIES(X)                                                                                                \
   X(layer_norm) X(layer_norm_workspace_bytes) X(layer_norm_backward) X(dense_few_rows) X(dense_keeps) X(dense)              \
   X(dense_backward_workspace_bytes) X(dense_backward) X(copy_rows) X(dropout)      \
-  X(adapter_dense) X(adapter_low_bytes) X(adapter_few_rows) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
+  X(adapter_dense) X(adapter_low_bytes) X(adapter_few_rows) X(adapter_dense_needs_low) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
   B200TA_ENTRIES(B200TA_ENTRY)
 #undef B200TA_ENTRY
 } lib;
@@ -357,7 +357,7 @@ Adapting adapters_of(const at::Tensor& x, const Layer& l, int64_t columns, const
   return a;
 }
 
-std::tuple<at::Tensor, at::Tensor, Maybe> adapter_dense(const at::Tensor& x, const at::Tensor& w, const Maybe& bias, const at::Tensor& down,
+std::tuple<at::Tensor, Maybe, Maybe> adapter_dense(const at::Tensor& x, const at::Tensor& w, const Maybe& bias, const at::Tensor& down,
                                                         const at::Tensor& up, const Maybe& index, const Maybe& scale, double scale_all,
                                                         const Maybe& residual, int64_t activation, bool gated, bool want_saved, const Maybe& out) {
   const Layer l = layer_of(x, w, bias, activation, gated);
@@ -368,8 +368,8 @@ std::tuple<at::Tensor, at::Tensor, Maybe> adapter_dense(const at::Tensor& x, con
   const at::Tensor y = or_out(out, x, l.N);
   if (residual) require_like("residual", *residual, x, y.sizes());
   const int64_t low_pitch = int64_t(lib.adapter_low_bytes(a.c.rank)) / 2, pitch = pad8(l.N) * (gated ? 2 : 1);
-  const at::Tensor low = empty({l.rows, low_pitch}, x.scalar_type(), x);
-  Maybe saved;
+  Maybe low, saved;
+  if (want_saved || lib.adapter_dense_needs_low(l.rows, a.c.rank, l.K)) low = empty({l.rows, low_pitch}, x.scalar_type(), x);
   if (want_saved && lib.dense_keeps(int(activation), gated, l.K)) saved = empty({l.rows, pitch}, at::kFloat, x);
   if (l.rows == 0) return {y, low, saved};
   const Rows rx = operand(x, few, copies), rw = operand(w, few, copies), to = result_in(y);
@@ -389,9 +389,9 @@ std::tuple<at::Tensor, at::Tensor, Maybe> adapter_dense(const at::Tensor& x, con
   copies.make();
   low_copies.make();
   check(lib.adapter_dense(rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), residual ? rr.ptr : nullptr, rr.stride, to.ptr, to.stride,
-                          pointer(saved), pitch, &a.c, low.data_ptr(), l.dtype, int(activation), gated, l.rows, l.K, l.N, stream()),
+                          pointer(saved), pitch, &a.c, pointer(low), l.dtype, int(activation), gated, l.rows, l.K, l.N, stream()),
         "b200ta_adapter_dense");
-  return {y, low, saved};
+  return {y, want_saved ? low : Maybe(), saved};
 }
 
 std::tuple<Maybe, Maybe, Maybe, Maybe, Maybe> adapter_dense_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w, const Maybe& bias,

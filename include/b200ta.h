@@ -460,7 +460,8 @@ int b200ta_dense_backward(const void* dy, int64_t dy_row_stride, const void* x, 
  * where row r has the adapter g = index[r / rows_per_index]; rows whose index is none of 0 .. count - 1 have none.  down [count, rank, K] and up
  * [count, N or 2 N, rank] lie with one row stride each; `scale` [count] on the device, or NULL for `scale_all`; index of 4 or 8 bytes an
  * entry, or NULL for adapter 0 (of one) everywhere.  Ranks up to 256, up to 16383 adapters.  `low` has
- * b200ta_adapter_low_bytes(rank) bytes for each row, is 16-byte aligned, written here and read again by the backward pass.  Alignment as for
+ * b200ta_adapter_low_bytes(rank) bytes for each row, is 16-byte aligned, written here and read again by the backward pass; where
+ * b200ta_adapter_dense_needs_low() says no it may be NULL.  Alignment as for
  * b200ta_dense, with b200ta_adapter_few_rows() in the place of its few rows. */
 typedef struct {
   const void *down, *up;
@@ -474,6 +475,7 @@ typedef struct {
 } b200ta_adapters;
 size_t b200ta_adapter_low_bytes(int rank);
 int b200ta_adapter_few_rows(void);
+int b200ta_adapter_dense_needs_low(int64_t rows, int rank, int K);
 int b200ta_adapter_dense(const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride, const void* bias, const void* residual,
                          int64_t residual_row_stride, void* y, int64_t y_row_stride, void* saved, int64_t saved_row_stride,
                          const b200ta_adapters* adapters, void* low, int dtype, int activation, int gated, int64_t rows,
