@@ -185,13 +185,13 @@ struct TileRows<true, kPair, kOuter> {
 };
 // The held block of U_g that is used last: whose it is, where it lies, and the phase of its barriers.
 struct HeldHigh {
-  int g = -1, n0 = 0, slot = -1;
+  int g = -1, n0 = 0, place = -1;
   uint32_t phase = 1;
   __device__ __forceinline__ bool differs(int to_g, int to_n) const { return to_g != g || to_n != n0; }
   __device__ __forceinline__ void take(int slots, int to_g, int to_n) {
     g = to_g, n0 = to_n;
-    if (slot < 0) slot = 0, phase = 0;
-    else if (++slot == slots) slot = 0, phase ^= 1u;
+    if (place < 0) place = 0, phase = 0;
+    else if (++place == slots) place = 0, phase ^= 1u;
   }
 };
 
@@ -514,9 +514,9 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           if (!high.differs(g, n0)) return;
           high.take(x.slots, g, n0);
           const int bytes = b_rows * x.unit * 2;
-          open(HIGH_EMPTY + high.slot, high.phase ^ 1, HIGH_FULL + high.slot, bytes);
+          open(HIGH_EMPTY + high.place, high.phase ^ 1, HIGH_FULL + high.place, bytes);
           if (!ok) return;
-          load_high(held + high.slot * bytes, n0, 0, g);
+          load_high(held + high.place * bytes, n0, 0, g);
           ++highs;
         }
       };
@@ -645,13 +645,13 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         if constexpr (kAdapt) {
           if (!high.differs(g, n0)) return;
           if (high.g >= 0) {  // all that read the last one has been issued
-            const uint32_t done = bars + (HIGH_EMPTY + high.slot) * 8;
+            const uint32_t done = bars + (HIGH_EMPTY + high.place) * 8;
             if constexpr (kPair) umma_commit_pair_warp(done);
             else umma_commit_warp(done);
           }
           high.take(x.slots, g, n0);
-          ok = mbar_wait_warp(bars + (HIGH_FULL + high.slot) * 8, high.phase, abort_flag);
-          held_desc = high_desc | ((held + high.slot * (b_rows * x.unit * 2)) >> 4);
+          ok = mbar_wait_warp(bars + (HIGH_FULL + high.place) * 8, high.phase, abort_flag);
+          held_desc = high_desc | ((held + high.place * (b_rows * x.unit * 2)) >> 4);
         }
       };
       TileRows<kAdapt, kPair, kAMn> ahead(p, x, units);

@@ -11,7 +11,8 @@ from .buffers import PreallocatedBuffers, ensure_buffer
 from .linear import Linear, WeightMode, WeightsLoadingConfig
 from .pairformer import (PairformerLayerV1, PairformerLayerV2, PairformerModule, PairformerNoSeqLayer,
                          PairformerNoSeqModule)
-from .training import TrainableTransition, dense, dropout, gated_dense, layer_norm
+from .training import (TrainableTransition, adapter_dense, adapter_gated_dense, dense, dropout, gated_dense,
+                       layer_norm)
 from .transition import PairTransition, Transition
 from .triangle_multiplication import (TriangleMultiplicationMetadata, TriangleMultiplicationNode,
                                       TriangleMultiplicationNodeType, precompute_trimul_metadata,
@@ -29,5 +30,6 @@ __all__ = [
     "TriangleMultiplicationMetadata", "TriangleMultiplicationNode", "TriangleMultiplicationNodeType",
     "precompute_trimul_metadata", "set_trimul_token_padding", "PairformerNoSeqLayer", "PairformerNoSeqModule",
     "AttentionPairBias", "PairformerLayerV1", "PairformerLayerV2", "PairformerModule", "PrecomputedSingleMasks", "precompute_single_masks",
-    "register_precompute_single_masks", "TrainableTransition", "dense", "dropout", "gated_dense", "layer_norm",
+    "register_precompute_single_masks", "TrainableTransition", "adapter_dense", "adapter_gated_dense", "dense", "dropout",
+    "gated_dense", "layer_norm",
 ]
