@@ -145,14 +145,13 @@ SIGNATURES: dict[str, tuple] = {
          c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int64, c_int, c_int, c_void_p],
     ),
     "b200ta_adapter_low_bytes": (c_size_t, [c_int]),
-    "b200ta_adapter_few_rows": (c_int, []),
     "b200ta_adapter_dense_needs_low": (c_int, [c_int64, c_int, c_int]),
     "b200ta_adapter_dense": (
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
          c_int, c_int, c_int, c_int64, c_int, c_int, c_void_p],
     ),
-    "b200ta_adapter_dense_backward_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_int]),
+    "b200ta_adapter_dense_backward_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int, c_int]),
     "b200ta_adapter_dense_backward": (
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,

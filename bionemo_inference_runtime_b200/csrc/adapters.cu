@@ -161,13 +161,9 @@ low_product_kernel(const LowProduct p, int share) {
   }
 }
 
-// Each row's own adapter read for it alone, rather than a pass over the rows' k for each adapter among them.
-bool by_warps(const LowProduct& m) {
-  return m.rows <= 32 || (m.index.index != nullptr && m.index.count > 1 && m.index.rows_per_index < 8 && m.rows <= 4096);
-}
 template <typename T, bool kVec>
 int launch_low(DeviceState* st, const LowProduct& m, void* stream) {
-  if (by_warps(m)) {
+  if (low_by_rows(m.rows, m.rank, m.K * m.planes, m.index)) {
     const int groups = int((low_pitch(m.rank) / 2 + kDotWarps - 1) / kDotWarps);
     return launch_kernel(st, kKernelAdapter, low_dot_kernel<T, kVec>, dim3(unsigned(m.rows * groups)), kDotWarps * 32, 0, stream, m, groups);
   }
@@ -177,6 +173,57 @@ int launch_low(DeviceState* st, const LowProduct& m, void* stream) {
   const dim3 grid{unsigned(share ? groups : (groups + warps - 1) / warps), unsigned((low_pitch(m.rank) / 2 + tiles * 8 - 1) / (tiles * 8))};
   auto* kernel = tiles == 2 ? low_product_kernel<T, 2, kVec> : tiles == 4 ? low_product_kernel<T, 4, kVec> : low_product_kernel<T, 8, kVec>;
   return launch_kernel(st, kKernelAdapter, kernel, grid, warps * 32, 0, stream, m, share);
+}
+
+// The same of dz and U as it lies, [columns][rank]: a block for a row, whose threads take eight ranks of every so many columns.
+struct LowUpParams {
+  const void *dz, *up;
+  void* low;
+  const float* scale;
+  float scale_all;
+  long long zs, z_plane, us;
+  int N, planes, rank;
+  AdapterIndex index;
+};
+template <typename T>
+__global__ void __launch_bounds__(256)
+low_up_kernel(const LowUpParams p) {
+  __shared__ float joined[256][9];
+  pdl_wait();
+  pdl_trigger();
+  const long long row = blockIdx.x;
+  const int vectors = low_pitch(p.rank) / 16, ways = 256 / vectors, v = threadIdx.x % vectors, way = threadIdx.x / vectors;
+  const int g = adapter_of(p.index, uint32_t(row));
+  float sum[8] = {};
+  if (g != kNoAdapter && way < ways && v * 8 < p.rank) {
+    for (int plane = 0; plane < p.planes; ++plane) {
+      const T* dz = static_cast<const T*>(p.dz) + row * p.zs + plane * p.z_plane;
+      const T* up = static_cast<const T*>(p.up) + (long long)(g * p.planes + plane) * p.N * p.us + v * 8;
+#pragma unroll 8
+      for (int n = way; n < p.N; n += ways) {
+        const float d = static_cast<float>(dz[n]);
+        const uint4 x = norm::first<T>(__ldg(reinterpret_cast<const uint4*>(up + n * p.us)), p.rank - v * 8);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack2<T>(w[j]);
+          sum[2 * j] = fmaf(d, f.x, sum[2 * j]), sum[2 * j + 1] = fmaf(d, f.y, sum[2 * j + 1]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) joined[threadIdx.x][j] = sum[j];
+  __syncthreads();
+  const int r = threadIdx.x;
+  if (r >= low_pitch(p.rank) / 2) return;
+  float total = 0.f;
+  for (int w = 0; w < ways; ++w) total += joined[w * vectors + r / 8][r % 8];
+  if (r >= p.rank || g == kNoAdapter) total = 0.f;
+  else total *= p.scale != nullptr ? __ldg(p.scale + g) : p.scale_all;
+  T* low = static_cast<T*>(p.low) + row * low_pitch(p.rank) + low_place(p.rank, r);
+  const T rounded = static_cast<T>(total);
+  low[0] = rounded, low[low_unit(p.rank)] = static_cast<T>(total - static_cast<float>(rounded));
 }
 
 // ---- up matrices with their columns contiguous -----------------------------------------------------------------------
@@ -210,7 +257,8 @@ transpose_up_kernel(const TransposeParams p) {
 // ninth warp fills by TMA.  Products m16n8k16 with ranks as rows and the tensor's rows along k: both operands lie with k across and
 // are transposed on their way from shared memory.  Of several adapters a block first lists the groups of 64 rows that hold its own;
 // in a group that others have a part of, their rows are cleared in the operands' registers, so that infinities and NaN in them stay
-// out.  Parts are written in 32 bits and joined in a fixed order: results repeat bit by bit.  (Filled by cp.async from all threads,
+// out.  Parts are written in 32 bits, with a mark that they have been (a part of the rows may have none of an adapter's), and joined in
+// a fixed order: results repeat bit by bit.  A single part is the result.  (Filled by cp.async from all threads,
 // 147456 rows of 128 and 1024 columns, rank 16: 89 us.)
 constexpr int kGradRows = 64, kGradColumns = 128, kGradChunks = 1024, kGradWarps = 8;
 // (up to 16, 32 or 64 ranks with their two terms are rows of 64 or 128 bytes, or two blocks of the latter)
@@ -221,7 +269,8 @@ __host__ __device__ constexpr int grad_stages(int tiles) { return tiles == 4 ? 3
 struct GradParams {
   LowGrad job[2];
   AdapterIndex index;
-  int rows, rank, rank_groups, slabs0, chunks_part, accumulate;
+  int rows, rank, rank_groups, slabs0, chunks_part, accumulate, direct;
+  uint8_t* marks;  // of each block
   int* status;
 };
 struct GradMaps {
@@ -265,24 +314,43 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
   const int first_row = int(blockIdx.y) * p.chunks_part * kGradRows;
   const int rows = min(p.rows - first_row, p.chunks_part * kGradRows), chunks = rows > 0 ? (rows + kGradRows - 1) / kGradRows : 0;
 
-  // Bits of a group's rows that are g's.  (Rows behind the last one are zeros in shared memory, whoever's they are.)
-  for (int c0 = warp; c0 < chunks; c0 += 4 * (kGradWarps + 1)) {
-    int own[4][2];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = (c0 + u * (kGradWarps + 1)) * kGradRows + h * 32 + lane;
-        own[u][h] = row < rows ? adapter_of(p.index, uint32_t(first_row + row)) : g;
+  // Bits of a group's rows that are g's.  (Rows behind the last one are zeros in shared memory and count where others do.)
+  if (p.index.index == nullptr || p.index.rows_per_index >= 16) {  // a thread for a group, of a few entries
+    for (int c = threadIdx.x; c < chunks; c += (kGradWarps + 1) * 32) {
+      const int row0 = c * kGradRows, in = min(rows - row0, kGradRows);
+      uint64_t own = 0;
+      if (p.index.index == nullptr) {
+        own = ~0ull;
+      } else {
+        for (int row = 0; row < in;) {
+          const uint32_t at = p.index.first_row + uint32_t(first_row + row0 + row), next = (at / p.index.rows_per_index + 1) * p.index.rows_per_index;
+          const int end = int(min(uint32_t(in), row + (next - at)));
+          if (adapter_of(p.index, uint32_t(first_row + row0 + row)) == g) own |= (end - row >= 64 ? ~0ull : (1ull << (end - row)) - 1) << row;
+          row = end;
+        }
+        if (own != 0 && in < 64) own |= ~0ull << in;
       }
+      masks[c][0] = uint32_t(own), masks[c][1] = uint32_t(own >> 32);
+    }
+  } else {
+    for (int c0 = warp; c0 < chunks; c0 += 4 * (kGradWarps + 1)) {
+      int own[4][2];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t bits = __ballot_sync(0xffffffffu, own[u][h] == g);
-        const int c = c0 + u * (kGradWarps + 1);
-        if (lane == 0 && c < chunks) masks[c][h] = bits;
-      }
+        for (int h = 0; h < 2; ++h) {
+          const int row = (c0 + u * (kGradWarps + 1)) * kGradRows + h * 32 + lane;
+          own[u][h] = row < rows ? adapter_of(p.index, uint32_t(first_row + row)) : g;
+        }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t bits = __ballot_sync(0xffffffffu, own[u][h] == g);
+          const int c = c0 + u * (kGradWarps + 1);
+          if (lane == 0 && c < chunks) masks[c][h] = bits;
+        }
+    }
   }
   __syncthreads();
   if (warp == 0) {
@@ -299,6 +367,11 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
   __syncthreads();
   const int count = listed;
   volatile int* abort_flag = aborted;
+  uint8_t* mark = p.direct ? nullptr : p.marks + ((long long)blockIdx.y * gridDim.z + blockIdx.z) * gridDim.x + blockIdx.x;
+  if (count == 0 && !p.direct) {
+    if (threadIdx.x == 0 && !p.accumulate) *mark = 0;
+    return;
+  }
 
   if (warp == kGradWarps) {
     if (lane == 0) {
@@ -363,7 +436,10 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
       mbar_arrive_warp_after_reads(bar0 + (kStages + s) * 8);
     }
     const int pitch = int(low_grad_columns(job.columns, job.planes)), plane_columns = pitch / job.planes, adapters = gridDim.z / p.rank_groups;
+    const int all = job.columns * job.planes;
+    const bool add = !p.direct && p.accumulate && *mark;
     float* part = job.part + ((long long)blockIdx.y * adapters + g) * p.rank * pitch + plane * plane_columns;
+    T* out = static_cast<T*>(job.out) + (long long)g * p.rank * all;
 #pragma unroll
     for (int m = 0; m < kTiles; ++m)
 #pragma unroll
@@ -372,12 +448,20 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
         for (int e = 0; e < 4; ++e) {
           const int r = r0 + m * 16 + (lane >> 2) + 8 * (e >> 1), c = c0 + warp * 16 + n * 8 + (lane & 3) * 2 + (e & 1);
           if (r >= p.rank || c >= job.columns) continue;
-          float* to = part + (long long)r * pitch + c;
-          *to = p.accumulate ? *to + acc[m][n][e] : acc[m][n][e];
+          if (p.direct) {
+            const long long column = (long long)plane * job.columns + c;
+            out[job.transposed ? column * p.rank + r : (long long)r * all + column] = static_cast<T>(acc[m][n][e]);
+          } else {
+            float* to = part + (long long)r * pitch + c;
+            *to = add ? *to + acc[m][n][e] : acc[m][n][e];
+          }
         }
   }
   __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) *p.status = B200TA_ERR_DEVICE_WAIT;
+  if (threadIdx.x == 0) {
+    if (!p.direct) *mark = 1;
+    if (*abort_flag) *p.status = B200TA_ERR_DEVICE_WAIT;
+  }
 }
 
 template <typename T, int kTiles>
@@ -393,6 +477,8 @@ struct LowJoinParams {
   LowGrad job[2];
   int rank, parts, adapters;
   long long items0, items;  // of the first job, of both
+  const uint8_t* marks;     // [part][adapter, group of 64 ranks][slab of 128 columns]: parts that were written
+  int slabs, slabs0;
 };
 template <typename T, int kSlices>
 __global__ void __launch_bounds__(256)
@@ -414,18 +500,28 @@ low_join_kernel(const LowJoinParams p) {
     const int groups = (p.rank + ranks - 1) / ranks, r0 = int(at % groups) * ranks;
     const long long g = at / groups;
     const float* part = job.part + (g * p.rank + r0) * pitch + plane * plane_columns + (column - plane * job.columns);
+    const int rank_groups = (p.rank + 63) / 64, slabs_plane = (job.columns + kGradColumns - 1) / kGradColumns;
+    const uint8_t* mark = p.marks + (g * rank_groups + r0 / 64) * p.slabs + (second ? p.slabs0 : 0) + plane * slabs_plane + (column - plane * job.columns) / kGradColumns;
+    const long long mark_stride = (long long)p.adapters * rank_groups * p.slabs;
     float sum[8] = {};
     const int n = p.rank - r0 < ranks ? p.rank - r0 : ranks;
     if (i < p.items) {
       if (job.transposed) {
 #pragma unroll 2
-        for (int s = slice; s < p.parts; s += kSlices)
+        for (int s = slice; s < p.parts; s += kSlices) {
+          float x[8];
 #pragma unroll
-          for (int r = 0; r < 8; ++r)
-            if (r < n) sum[r] += __ldg(part + s * stride + r * pitch);
+          for (int r = 0; r < 8; ++r) x[r] = norm::element_if(r < n, part + s * stride + r * pitch);
+          const bool written = __ldg(mark + s * mark_stride);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) sum[r] += written ? x[r] : 0.f;
+        }
       } else {
 #pragma unroll 8
-        for (int s = slice; s < p.parts; s += kSlices) sum[0] += __ldg(part + s * stride);
+        for (int s = slice; s < p.parts; s += kSlices) {
+          const float x = norm::element_if(true, part + s * stride);  // (loaded whether it was written or not: loads overlap)
+          sum[0] += __ldg(mark + s * mark_stride) ? x : 0.f;
+        }
       }
     }
     if constexpr (kSlices > 1) {
@@ -458,6 +554,15 @@ low_join_kernel(const LowJoinParams p) {
 
 }  // namespace
 
+// Each row's own adapter read for it alone, from L2 at some 2 TB/s, rather than a pass over 32 rows' k for each adapter among them,
+// whose loads and products follow one another: 0.4 us for 256 of k and 2 us besides.  (288 rows of 1336, rank 32, 8 rows a request: 30 us
+// by passes, now 15.)
+bool low_by_rows(int64_t rows, int rank, int K, const AdapterIndex& index) {
+  const double adapters = index.index == nullptr ? 1 : std::min<double>(index.count, 31 / index.rows_per_index + 1);
+  const double each = 3 + double(rows) * rank * K * 2 / 2e6, passes = 4 + adapters * (2 + 0.4 * K / 256);
+  return rows <= 8192 && each < passes;
+}
+
 int run_low(const LowProduct& m, void* stream) {
   DeviceState* st = nullptr;
   const int rc = get_device_state(&st);
@@ -465,9 +570,17 @@ int run_low(const LowProduct& m, void* stream) {
   // tiles of 128 rows, unless those of several requests are too few to fill the device
   const int64_t tiles = (m.rows + 127) / 128;
   const bool mixed = m.index.index != nullptr && m.index.count > 1 && m.index.rows_per_index < 128;
-  if (m.rows > 512 && !by_warps(m) && !(mixed && tiles < st->num_sms)) return run_matmul_low(m, stream);
+  if (m.rows > 512 && !low_by_rows(m.rows, m.rank, m.K * m.planes, m.index) && !(mixed && tiles < st->num_sms)) return run_matmul_low(m, stream);
   if (m.f16) return m.aligned ? launch_low<__half, true>(st, m, stream) : launch_low<__half, false>(st, m, stream);
   return m.aligned ? launch_low<__nv_bfloat16, true>(st, m, stream) : launch_low<__nv_bfloat16, false>(st, m, stream);
+}
+
+int run_low_up(const LowProduct& m, const void* up, int64_t up_pitch, void* stream) {
+  DeviceState* st = nullptr;
+  const int rc = get_device_state(&st);
+  if (rc != B200TA_OK) return rc;
+  const LowUpParams p{m.x, up, m.low, m.scale, m.scale_all, m.xs, m.x_plane, up_pitch, m.K, m.planes, m.rank, m.index};
+  return launch_kernel(st, kKernelAdapter, m.f16 ? low_up_kernel<__half> : low_up_kernel<__nv_bfloat16>, dim3(unsigned(m.rows)), 256, 0, stream, p);
 }
 
 int run_transpose_up(const void* up, int64_t up_pitch, void* out, int64_t out_pitch, int count, int rank, int N, int planes, void* stream) {
@@ -479,15 +592,21 @@ int run_transpose_up(const void* up, int64_t up_pitch, void* out, int64_t out_pi
                        0, stream, p);
 }
 
-// Parts of the rows: one wave of two blocks on each multiprocessor if all adapters have their share of the rows, more (rows may be of
-// few of them) as long as the parts stay below 32 MiB.
-int low_grad_parts(int64_t rows, int64_t columns, int count, int rank, int num_sms) {
-  const int64_t chunks = (rows + kGradRows - 1) / kGradRows, slabs = (columns + kGradColumns - 1) / kGradColumns * ((rank + 63) / 64);
-  const int64_t wanted = std::max<int64_t>(int64_t(num_sms) * 2 / slabs, 1), shared = std::max<int64_t>(int64_t(num_sms) * 2 / (slabs * count), 1);
-  const int64_t by_bytes = (int64_t(1) << 25) / (int64_t(count) * rank * columns * 4);
-  const int64_t parts = std::max(std::min(std::max(shared, std::min(wanted, by_bytes)), (chunks + 3) / 4), (chunks + kGradChunks - 1) / kGradChunks);
+// Parts of the rows: one wave of two blocks on each multiprocessor if all adapters have their share of the rows, and up to four (rows may
+// be of few of them) as long as the parts stay below 16 MiB; blocks that have nothing to do end early.
+LowGradShape low_grad_shape(int64_t rows, int K, int N, int planes, int count, int rank, int num_sms) {
+  LowGradShape s{};
+  const int64_t chunks = (rows + kGradRows - 1) / kGradRows, columns = int64_t(K) + int64_t(planes) * N;
+  s.slabs = (K + kGradColumns - 1) / kGradColumns + planes * ((N + kGradColumns - 1) / kGradColumns);
+  const int64_t blocks = s.slabs * ((rank + 63) / 64), wave = int64_t(num_sms) * 2;
+  const int64_t wanted = std::max<int64_t>(wave / blocks, 1), shared = std::max<int64_t>(wave / (blocks * count), 1);
+  const int64_t by_bytes = (int64_t(1) << 24) / (int64_t(count) * rank * columns * 4), most = 4 * wave / (blocks * count);
+  const int64_t parts = std::max(std::min(std::max(shared, std::min(std::min(wanted, most), by_bytes)), (chunks + 3) / 4),
+                                 (chunks + kGradChunks - 1) / kGradChunks);
   const int64_t per = (chunks + parts - 1) / parts;
-  return int((chunks + per - 1) / per);
+  s.parts = int((chunks + per - 1) / per);
+  s.marks = s.slabs * s.parts * count * ((rank + 63) / 64);
+  return s;
 }
 
 int run_low_grads(const LowGrads& m, void* stream) {
@@ -513,7 +632,7 @@ int run_low_grads(const LowGrads& m, void* stream) {
   }
   auto slabs_of = [](const LowGrad& j) { return j.v == nullptr ? 0 : j.planes * ((j.columns + kGradColumns - 1) / kGradColumns); };
   p.job[0] = m.job[0], p.job[1] = m.job[1], p.index = m.index, p.rows = int(m.rows), p.rank = m.rank, p.rank_groups = (m.rank + 63) / 64;
-  p.slabs0 = slabs_of(m.job[0]), p.accumulate = m.accumulate, p.status = st->status_dev;
+  p.slabs0 = slabs_of(m.job[0]), p.accumulate = m.accumulate, p.direct = m.direct, p.marks = m.marks, p.status = st->status_dev;
   const int64_t chunks = (m.rows + kGradRows - 1) / kGradRows;
   p.chunks_part = int((chunks + m.parts - 1) / m.parts);
   B200TA_REQUIRE(p.chunks_part <= kGradChunks, "adapters: too many rows for %d parts", m.parts);
@@ -535,8 +654,10 @@ int run_low_join(const LowGrads& m, void* stream) {
   };
   p.job[0] = m.job[0], p.job[1] = m.job[1], p.rank = m.rank, p.parts = m.parts, p.adapters = m.index.count;
   p.items0 = items_of(m.job[0]), p.items = p.items0 + items_of(m.job[1]);
+  auto slabs_of = [](const LowGrad& j) { return j.v == nullptr ? 0 : j.planes * ((j.columns + kGradColumns - 1) / kGradColumns); };
+  p.marks = m.marks, p.slabs0 = slabs_of(m.job[0]), p.slabs = p.slabs0 + slabs_of(m.job[1]);
   // several threads to an item where there are many parts of few values
-  const bool sliced = m.parts >= 4 && p.items < int64_t(st->num_sms) * 256;
+  const bool sliced = m.parts >= 4 && p.items < int64_t(st->num_sms) * (m.parts >= 8 ? 1024 : 256);
   const int64_t each = sliced ? 32 : 256, blocks = std::min<int64_t>((p.items + each - 1) / each, int64_t(st->num_sms) * 16);
   auto* kernel = m.f16 ? (sliced ? low_join_kernel<__half, 8> : low_join_kernel<__half, 1>)
                        : (sliced ? low_join_kernel<__nv_bfloat16, 8> : low_join_kernel<__nv_bfloat16, 1>);

@@ -59,6 +59,9 @@ struct LowProduct {
 };
 int run_low(const LowProduct& m, void* stream);
 int run_matmul_low(const LowProduct& m, void* stream);  // of it: on the tensor cores (dense.cu)
+// dz U with U as it lies (for m.x = dz, its N columns as m.K; 16-byte rows), where low_by_rows() says so.
+bool low_by_rows(int64_t rows, int rank, int K, const AdapterIndex& index);
+int run_low_up(const LowProduct& m, const void* up, int64_t up_pitch, void* stream);
 
 // up [count][columns (two planes of N)][rank] as [count][planes][rank][pitch], for dz U.
 int run_transpose_up(const void* up, int64_t up_pitch, void* out, int64_t out_pitch, int count, int rank, int N, int planes, void* stream);
@@ -77,10 +80,15 @@ struct LowGrads {
   LowGrad job[2];
   AdapterIndex index;
   long long rows;
-  int rank, parts, accumulate;
+  int rank, parts, accumulate, direct;  // direct: one part of all rows, whose sums are the results (no join)
+  uint8_t* marks;
   bool f16;
 };
-int low_grad_parts(int64_t rows, int64_t columns, int count, int rank, int num_sms);
+struct LowGradShape {
+  int parts;
+  int64_t slabs, marks;  // marks: bytes
+};
+LowGradShape low_grad_shape(int64_t rows, int K, int N, int planes, int count, int rank, int num_sms);
 __host__ __device__ inline int64_t low_grad_columns(int columns, int planes) { return int64_t(planes) * ((columns + 3) / 4 * 4); }
 int run_low_grads(const LowGrads& m, void* stream);
 int run_low_join(const LowGrads& m, void* stream);

@@ -290,13 +290,14 @@ __device__ __forceinline__ float low_sum(const T* low, const float* own, const T
 }
 
 template <typename T, bool kTwo, int kEights, bool kVec>
-__global__ void __launch_bounds__(few_warps(kEights, kTwo ? 2 : 1) * 32, 1)
+__global__ void __launch_bounds__(few_warps(kEights, kTwo ? 2 : 1) * 32, kEights > 2 && few_warps(kEights, kTwo ? 2 : 1) <= 8 ? 2 : 1)
 few_rows_kernel(const FewParams p) {
   __shared__ float joined[few_warps(kEights, kTwo ? 2 : 1)][kTwo ? 2 : 1][kEights * 8][kFewColumns + 1];
   __shared__ float own_low[kOwnLow];
   pdl_trigger();
   if (p.adapters.low == nullptr) pdl_wait();  // (otherwise what came before the kernel of the low-rank values is complete)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, n0 = blockIdx.x * kFewColumns, warps = blockDim.x >> 5;
+  const int row0 = blockIdx.y * kFewAdapterRows, rows = min(p.rows - row0, kFewAdapterRows);
   constexpr int kParts = kTwo ? 2 : 1;
   const T *w[kParts][2], *x[kEights];
 #pragma unroll
@@ -306,7 +307,7 @@ few_rows_kernel(const FewParams p) {
     if constexpr (kTwo) w[1][h] = static_cast<const T*>(p.w) + (long long)(n + p.N) * p.ws;
   }
 #pragma unroll
-  for (int e = 0; e < kEights; ++e) x[e] = static_cast<const T*>(p.x) + min(g + 8 * e, p.rows - 1) * p.xs;
+  for (int e = 0; e < kEights; ++e) x[e] = static_cast<const T*>(p.x) + (row0 + min(g + 8 * e, rows - 1)) * p.xs;
   if (p.down != nullptr) {  // a warp for each low-rank value
     const int rank = p.adapters.rank;
     for (int i = warp; i < p.rows * rank; i += warps) {
@@ -368,20 +369,21 @@ few_rows_kernel(const FewParams p) {
       low[0] = rounded, low[low_unit(p.adapters.rank)] = static_cast<T>(v - static_cast<float>(rounded));
     }
   }
-  for (int row = threadIdx.x / kFewColumns; row < p.rows && n < p.N; row += blockDim.x / kFewColumns) {
+  for (int own = threadIdx.x / kFewColumns; own < rows && n < p.N; own += blockDim.x / kFewColumns) {
+    const int row = row0 + own;
     float v = 0.f, gate = 0.f;
     for (int i = 0; i < warps; ++i) {
-      v += joined[i][0][row][c];
-      if constexpr (kTwo) gate += joined[i][1][row][c];
+      v += joined[i][0][own][c];
+      if constexpr (kTwo) gate += joined[i][1][own][c];
     }
     if (p.adapters.high != nullptr) {
       const int a = adapter_of(p.adapters.index, uint32_t(row));
       if (a != kNoAdapter) {
         const T* high = static_cast<const T*>(p.adapters.high) + ((long long)a * (kTwo ? 2 * p.N : p.N) + n) * p.adapters.high_pitch;
         const T* low = static_cast<const T*>(p.adapters.low) + row * low_pitch(p.adapters.rank);
-        const float* own = p.adapters.low == nullptr ? own_low + row * p.adapters.rank : nullptr;
-        v += low_sum(low, own, high, p.adapters.rank);
-        if constexpr (kTwo) gate += low_sum(low, own, high + (long long)p.N * p.adapters.high_pitch, p.adapters.rank);
+        const float* made = p.adapters.low == nullptr ? own_low + row * p.adapters.rank : nullptr;
+        v += low_sum(low, made, high, p.adapters.rank);
+        if constexpr (kTwo) gate += low_sum(low, made, high + (long long)p.N * p.adapters.high_pitch, p.adapters.rank);
       }
     }
     const T* bias = static_cast<const T*>(p.bias);
@@ -604,7 +606,7 @@ join_kernel(const JoinParams a, const JoinParams b, const JoinParams c) {
 // ---- aligned copies ---------------------------------------------------------------------------------------------------
 //
 // dst[r][c] = src[r * rs + c * cs] for 16-bit elements: tensors whose rows a TMA load cannot address (a pitch or base that is
-// no multiple of 16 bytes, columns that are not contiguous) pass through a padded copy, up to four in one launch.  A thread
+// no multiple of 16 bytes, columns that are not contiguous) pass through a padded copy, up to six in one launch.  A thread
 // makes a vector of eight columns, from two aligned loads shifted into place if they are contiguous, otherwise from eight
 // loads with neighbouring threads in neighbouring rows.  (An aligned 16-byte vector with a byte of the source in it lies in
 // the source's allocation.)  2047 rows of 515 and 1283 rows of 515 in one launch take 4.4 us, with 2047 of 1283 besides 6.2.
@@ -774,23 +776,29 @@ const BackwardPlan& plan_backward(bool gated, bool slope, bool kept, bool want_d
 
 // Where the adapters' intermediates of a backward pass lie behind the others in the workspace.
 struct LowPlan {
-  int parts;                          // of the rows for the adapters' gradients
-  int64_t up, low_grad, part[2], bytes;  // offsets: transposed up, dt of a chunk, parts of dD and dU
+  int parts;       // of the rows for the adapters' gradients
+  bool direct;     // a single one
+  bool by_rows;    // dt from U as it lies
+  int64_t up, low_grad, part[2], marks, bytes;  // offsets: transposed up, dt of a chunk, parts of dD and dU, their marks
 };
-LowPlan plan_low(const BackwardPlan& plan, int count, int rank, int64_t rows, int K, int N, int outer, int num_sms) {
+LowPlan plan_low(const BackwardPlan& plan, const AdapterIndex& index, int rank, int64_t rows, int K, int N, int outer, int num_sms) {
   LowPlan p{};
+  const int count = index.count;
   const int64_t chunk = std::min(plan.chunk, rows), ad = low_grad_columns(K, 1), au = low_grad_columns(N, outer);
-  p.parts = low_grad_parts(chunk, int64_t(K) + int64_t(outer) * N, count, rank, num_sms);
+  const LowGradShape shape = low_grad_shape(chunk, K, N, outer, count, rank, num_sms);
+  p.parts = shape.parts, p.direct = shape.parts == 1 && chunk >= rows;
+  p.by_rows = low_by_rows(chunk, rank, outer * N, index);
   p.bytes = (plan.bytes + 255) / 256 * 256;
   auto take = [&](int64_t bytes) {
     const int64_t at = p.bytes;
     p.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  p.up = take(int64_t(count) * rank * outer * pad8(N) * 2);
+  p.up = take(p.by_rows ? 0 : int64_t(count) * rank * outer * pad8(N) * 2);
   p.low_grad = take(chunk * low_pitch(rank) * 2);
-  p.part[0] = take(int64_t(p.parts) * count * rank * ad * 4);
-  p.part[1] = take(int64_t(p.parts) * count * rank * au * 4);
+  p.part[0] = take(p.direct ? 0 : int64_t(p.parts) * count * rank * ad * 4);
+  p.part[1] = take(p.direct ? 0 : int64_t(p.parts) * count * rank * au * 4);
+  p.marks = take(p.direct ? 0 : shape.marks);
   return p;
 }
 
@@ -809,6 +817,12 @@ AdapterIndex index_of(const b200ta_adapters* a) {
   return adapter_index(a->index, a->index_bytes, a->rows_per_index, a->count);
 }
 
+// The few rows' kernel with adapters: up to 64 rows of several adapters, and a few times as many if they are single tokens of many
+// requests (230 rows of 3320 -> 704 with 55 adapters: 49 us on the tensor cores, 22 so; 64 rows of 128 -> 512 gated with one: 10 us there).
+bool few_with_adapters(int64_t rows, const AdapterIndex& index) {
+  const int64_t adapters = index.index == nullptr ? 1 : std::min<int64_t>(index.count, (std::min<int64_t>(rows, 128) - 1) / index.rows_per_index + 1);
+  return rows <= kFewRows || (rows <= kFewAdapterRows && adapters >= 4) || (rows <= 4 * kFewAdapterRows && adapters >= 16);
+}
 int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* residual, int64_t rs, void* y, int64_t ys,
                   void* saved, int64_t ss, int dtype, int activation, int gated, int64_t rows, int K, int N, const LowRank* adapters, const LowProduct* own_low,
                   void* stream) {
@@ -817,7 +831,7 @@ int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const vo
   B200TA_REQUIRE(x && w && y, "dense: NULL pointer");
   B200TA_REQUIRE(!gated || residual == nullptr, "dense: a gated layer has no residual");
   B200TA_REQUIRE(!gated || saved == nullptr || ss % 16 == 0, "dense: the pitch of a gated layer's saved values must be a multiple of 16");
-  if (rows <= (adapters != nullptr ? kFewAdapterRows : kFewRows)) {
+  if (rows <= kFewRows || (adapters != nullptr && few_with_adapters(rows, adapters->index))) {
     DeviceState* st = nullptr;
     rc = get_device_state(&st);
     if (rc != B200TA_OK) return rc;
@@ -832,9 +846,9 @@ int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const vo
     const bool vec = K % 8 == 0 && rows_aligned(x, xs) && rows_aligned(w, ws) && vec_down;
     // sixteen warps where blocks are few (three rows, 1536 -> 384: 9 us instead of 11), eight otherwise, of which more blocks fit
     const int eights = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 8, blocks = (N + kFewColumns - 1) / kFewColumns;
-    const int warps = std::min(few_warps(eights, gated ? 2 : 1), blocks <= st->num_sms ? 16 : 8);
+    const int warps = std::min(few_warps(eights, gated ? 2 : 1), blocks <= st->num_sms ? 16 : 8), row_blocks = int((rows + kFewAdapterRows - 1) / kFewAdapterRows);
     return launch_kernel(st, kKernelDenseHelpers, f16 ? pick_few<__half>(int(rows), vec, gated) : pick_few<__nv_bfloat16>(int(rows), vec, gated),
-                         dim3(unsigned(blocks)), warps * 32, 0, stream, p);
+                         dim3(unsigned(blocks), unsigned(row_blocks)), warps * 32, 0, stream, p);
   }
   B200TA_REQUIRE(rows_aligned(x, xs) && rows_aligned(w, ws) && (!residual || rows_aligned(residual, rs)) &&
                      (!saved || rows_aligned(saved, ss)),
@@ -867,7 +881,8 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
   const bool kept = reads_kept(saved != nullptr, gated != 0, activation);
   const BackwardPlan& plan = plan_backward(gated, activation != kActNone, kept, dbias != nullptr, rows, K, N, st->num_sms);
   const int64_t outer = gated ? 2 : 1;
-  const LowPlan low_plan = ad != nullptr ? plan_low(plan, ad->count, ad->rank, rows, K, N, int(outer), st->num_sms) : LowPlan{0, 0, 0, {0, 0}, plan.bytes};
+  const LowPlan low_plan = ad != nullptr ? plan_low(plan, index_of(ad), ad->rank, rows, K, N, int(outer), st->num_sms)
+                                            : LowPlan{0, false, false, 0, 0, {0, 0}, 0, plan.bytes};
   B200TA_REQUIRE(low_plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
                                          workspace_bytes >= size_t(low_plan.bytes)),
                  "dense_backward: the workspace must be 256-byte aligned and of %lld bytes", (long long)low_plan.bytes);
@@ -903,7 +918,8 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
     low_grads.job[0] = {dt, nullptr, reinterpret_cast<float*>(ws_base + low_plan.part[0]), ddown, xs, 0, K, 1, 0};
     low_grads.job[1] = {nullptr, nullptr, reinterpret_cast<float*>(ws_base + low_plan.part[1]), dup, 0, 0, N, int(outer), 1};
     low_grads.rank = ad->rank, low_grads.parts = low_plan.parts, low_grads.f16 = f16;
-    if (dx != nullptr || ddown != nullptr) {
+    low_grads.direct = low_plan.direct, low_grads.marks = reinterpret_cast<uint8_t*>(ws_base + low_plan.marks);
+    if ((dx != nullptr || ddown != nullptr) && !low_plan.by_rows) {
       rc = run_transpose_up(ad->up, ad->up_row_stride, ws_base + low_plan.up, pad8(N), ad->count, ad->rank, N, int(outer), stream);
       if (rc != B200TA_OK) return rc;
     }
@@ -955,7 +971,8 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
       LowProduct q{};
       q.x = dz, q.a = ws_base + low_plan.up, q.low = dt, q.scale = ad->scale, q.scale_all = ad->scale_all;
       q.xs = zs, q.x_plane = zs / outer, q.as = pad8(N), q.rows = n, q.K = N, q.planes = int(outer), q.rank = ad->rank, q.f16 = f16, q.aligned = true, q.index = with_down.index;
-      if ((rc = run_low(q, stream)) != B200TA_OK) return rc;
+      rc = low_plan.by_rows ? run_low_up(q, ad->up, ad->up_row_stride, stream) : run_low(q, stream);
+      if (rc != B200TA_OK) return rc;
     }
     if (dx != nullptr && !narrow) {
       Matmul m;
@@ -1009,7 +1026,7 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
       if (rc != B200TA_OK) return rc;
     }
   }
-  if ((ddown != nullptr || dup != nullptr) && (rc = run_low_join(low_grads, stream)) != B200TA_OK) return rc;
+  if ((ddown != nullptr || dup != nullptr) && !low_plan.direct && (rc = run_low_join(low_grads, stream)) != B200TA_OK) return rc;
   const bool parts_left = dw != nullptr && !direct, sums_left = dbias != nullptr && !(product_sums && direct);
   if (!parts_left && !sums_left && !dx_parts) return B200TA_OK;
   const int64_t chunk = plan.chunk < rows ? plan.chunk : rows;
@@ -1065,7 +1082,7 @@ int b200ta_adapter_dense(const void* x, int64_t xs, const void* w, int64_t ws, c
   B200TA_REQUIRE(x && w && y, "adapter_dense: NULL pointer");
   if ((rc = check_adapters("adapter_dense", a, low)) != B200TA_OK) return rc;
   const bool aligned = rows_aligned(x, xs) && rows_aligned(a->down, a->down_row_stride);
-  B200TA_REQUIRE(rows <= kFewAdapterRows || (aligned && rows_aligned(a->up, a->up_row_stride)),
+  B200TA_REQUIRE(rows <= kFewRows || (aligned && rows_aligned(a->up, a->up_row_stride)),
                  "adapter_dense: what is read must be 16-byte aligned with row strides that are multiples of 8 elements");
   LowProduct q{};
   q.x = x, q.a = a->down, q.low = low, q.scale = a->scale, q.scale_all = a->scale_all;
@@ -1080,17 +1097,15 @@ int b200ta_adapter_dense(const void* x, int64_t xs, const void* w, int64_t ws, c
 
 int b200ta_adapter_dense_needs_low(int64_t rows, int rank, int K) { return !b200ta::own_low_pays(rows, rank, K); }
 
-int b200ta_adapter_few_rows(void) { return b200ta::kFewAdapterRows; }
-
 size_t b200ta_adapter_low_bytes(int rank) { return rank > 0 && rank <= b200ta::kMaxRank ? size_t(b200ta::low_pitch(rank)) * 2 : 0; }
 
-size_t b200ta_adapter_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, int count, int rank, int64_t rows, int K, int N) {
+size_t b200ta_adapter_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, const b200ta_adapters* a, int64_t rows, int K, int N) {
   using namespace b200ta;
   DeviceState* st = nullptr;
-  if (rows <= 0 || K <= 0 || N <= 0 || count <= 0 || rank <= 0 || get_device_state(&st) != B200TA_OK) return 0;
+  if (a == nullptr || rows <= 0 || K <= 0 || N <= 0 || a->count <= 0 || a->rank <= 0 || get_device_state(&st) != B200TA_OK) return 0;
   const BackwardPlan& plan = plan_backward(gated, activation != kActNone, reads_kept(kept != 0, gated != 0, activation), want_dbias != 0, rows, K, N,
                                            st->num_sms);
-  return size_t(plan_low(plan, count, rank, rows, K, N, gated ? 2 : 1, st->num_sms).bytes);
+  return size_t(plan_low(plan, index_of(a), a->rank, rows, K, N, gated ? 2 : 1, st->num_sms).bytes);
 }
 
 int b200ta_adapter_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* saved,

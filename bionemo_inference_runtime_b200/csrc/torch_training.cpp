@@ -22,7 +22,7 @@ struct Library {
 #define B200TA_ENTRIES(X)                                                                                                \
   X(layer_norm) X(layer_norm_workspace_bytes) X(layer_norm_backward) X(dense_few_rows) X(dense_keeps) X(dense)              \
   X(dense_backward_workspace_bytes) X(dense_backward) X(copy_rows) X(dropout)      \
-  X(adapter_dense) X(adapter_low_bytes) X(adapter_few_rows) X(adapter_dense_needs_low) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
+  X(adapter_dense) X(adapter_low_bytes) X(adapter_dense_needs_low) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
   B200TA_ENTRIES(B200TA_ENTRY)
 #undef B200TA_ENTRY
 } lib;
@@ -362,9 +362,9 @@ std::tuple<at::Tensor, Maybe, Maybe> adapter_dense(const at::Tensor& x, const at
                                                         const Maybe& residual, int64_t activation, bool gated, bool want_saved, const Maybe& out) {
   const Layer l = layer_of(x, w, bias, activation, gated);
   const c10::cuda::CUDAGuard guard(x.device());
-  Copies copies, low_copies;
-  const bool few = l.rows <= lib.adapter_few_rows();
-  const Adapting a = adapters_of(x, l, w.size(0), down, up, index, scale, scale_all, few, low_copies);
+  Copies copies;
+  const bool few = l.rows <= lib.dense_few_rows();
+  const Adapting a = adapters_of(x, l, w.size(0), down, up, index, scale, scale_all, few, copies);
   const at::Tensor y = or_out(out, x, l.N);
   if (residual) require_like("residual", *residual, x, y.sizes());
   const int64_t low_pitch = int64_t(lib.adapter_low_bytes(a.c.rank)) / 2, pitch = pad8(l.N) * (gated ? 2 : 1);
@@ -387,7 +387,6 @@ std::tuple<at::Tensor, Maybe, Maybe> adapter_dense(const at::Tensor& x, const at
     if (residual) require_apart(to, "residual", rr, y, *residual, true);
   }
   copies.make();
-  low_copies.make();
   check(lib.adapter_dense(rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), residual ? rr.ptr : nullptr, rr.stride, to.ptr, to.stride,
                           pointer(saved), pitch, &a.c, pointer(low), l.dtype, int(activation), gated, l.rows, l.K, l.N, stream()),
         "b200ta_adapter_dense");
@@ -405,8 +404,8 @@ std::tuple<Maybe, Maybe, Maybe, Maybe, Maybe> adapter_dense_backward(const at::T
   require_like("dy", dy, x, shape);
   const int64_t pitch = pad8(l.N) * (gated ? 2 : 1);
   const c10::cuda::CUDAGuard guard(x.device());
-  Copies copies, low_copies;
-  const Adapting a = adapters_of(x, l, w.size(0), down, up, index, scale, scale_all, false, low_copies);
+  Copies copies;
+  const Adapting a = adapters_of(x, l, w.size(0), down, up, index, scale, scale_all, false, copies);
   const int64_t low_pitch = int64_t(lib.adapter_low_bytes(a.c.rank)) / 2;
   require_like("saved", low, x, {l.rows, low_pitch});
   if (!low.is_contiguous()) refuse("saved must be what the forward pass returned");
@@ -424,10 +423,8 @@ std::tuple<Maybe, Maybe, Maybe, Maybe, Maybe> adapter_dense_backward(const at::T
   }
   const Rows rdy = operand(dy, false, copies), rx = operand(x, false, copies), rw = operand(w, false, copies);
   copies.make();
-  low_copies.make();
   const Maybe b = bias ? Maybe(bias->contiguous()) : Maybe();
-  const size_t need = lib.adapter_dense_backward_workspace_bytes(int(activation), gated, saved.has_value(), want_dbias, a.c.count, a.c.rank, l.rows,
-                                                                 l.K, l.N);
+  const size_t need = lib.adapter_dense_backward_workspace_bytes(int(activation), gated, saved.has_value(), want_dbias, &a.c, l.rows, l.K, l.N);
   const at::Tensor workspace = bytes(x, need);
   check(lib.adapter_dense_backward(rdy.ptr, rdy.stride, rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), pointer(saved), pitch, &a.c, low.data_ptr(),
                                    pointer(dx), l.K, pointer(dweight), pointer(dbias), pointer(ddown), pointer(dup), workspace.data_ptr(),

@@ -462,7 +462,7 @@ int b200ta_dense_backward(const void* dy, int64_t dy_row_stride, const void* x, 
  * entry, or NULL for adapter 0 (of one) everywhere.  Ranks up to 256, up to 16383 adapters.  `low` has
  * b200ta_adapter_low_bytes(rank) bytes for each row, is 16-byte aligned, written here and read again by the backward pass; where
  * b200ta_adapter_dense_needs_low() says no it may be NULL.  Alignment as for
- * b200ta_dense, with b200ta_adapter_few_rows() in the place of its few rows. */
+ * b200ta_dense. */
 typedef struct {
   const void *down, *up;
   int64_t down_row_stride, up_row_stride;
@@ -474,7 +474,6 @@ typedef struct {
   int count, rank;
 } b200ta_adapters;
 size_t b200ta_adapter_low_bytes(int rank);
-int b200ta_adapter_few_rows(void);
 int b200ta_adapter_dense_needs_low(int64_t rows, int rank, int K);
 int b200ta_adapter_dense(const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride, const void* bias, const void* residual,
                          int64_t residual_row_stride, void* y, int64_t y_row_stride, void* saved, int64_t saved_row_stride,
@@ -483,8 +482,8 @@ int b200ta_adapter_dense(const void* x, int64_t x_row_stride, const void* w, int
 
 /* Gradients of the same; ddown [count, rank, K] and dup [count, N or 2 N, rank] are dense and may be NULL.  dlow = scale_g dz up_g is held
  * as low is, dz rounded to `dtype`. */
-size_t b200ta_adapter_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, int count, int rank, int64_t rows, int K,
-                                                     int N);
+size_t b200ta_adapter_dense_backward_workspace_bytes(int activation, int gated, int kept, int want_dbias, const b200ta_adapters* adapters,
+                                                     int64_t rows, int K, int N);
 int b200ta_adapter_dense_backward(const void* dy, int64_t dy_row_stride, const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride,
                                   const void* bias, const void* saved, int64_t saved_row_stride, const b200ta_adapters* adapters, const void* low,
                                   void* dx, int64_t dx_row_stride, void* dw, void* dbias, void* ddown, void* dup,
@@ -494,7 +493,7 @@ int b200ta_adapter_dense_backward(const void* dy, int64_t dy_row_stride, const v
 /* dst[r, c] = src[r * row_stride + c * column_stride] for 16-bit elements: aligned copies of what the entry points above cannot
  * read as it lies, up to B200TA_COPIES of them in one launch.  dst is 16-byte aligned, its rows a multiple of 8 elements apart and
  * padded to 8 columns (the padding is written). */
-#define B200TA_COPIES 4
+#define B200TA_COPIES 6
 typedef struct {
   const void* src;
   int64_t row_stride, column_stride;

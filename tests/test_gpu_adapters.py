@@ -283,7 +283,7 @@ def test_nothing_is_written_behind_the_results(rows, K, N, count, rank, n, gated
     a = Adapters(down.data_ptr(), up.data_ptr(), down.shape[-1], up.shape[-1], given["scale"].data_ptr(), 1.0, index.data_ptr(), 4, rows // n, count, rank)
     stream = torch.cuda.current_stream().cuda_stream
     sizes = {"y": rows * N * 2, "low": rows * lib.b200ta_adapter_low_bytes(rank), "dx": rows * K * 2, "ddown": count * rank * K * 2, "dup": count * columns * rank * 2}
-    need = lib.b200ta_adapter_dense_backward_workspace_bytes(act, gated, 0, 0, count, rank, rows, K, N)
+    need = lib.b200ta_adapter_dense_backward_workspace_bytes(act, gated, 0, 0, _lib.ctypes.byref(a), rows, K, N)
     sizes["workspace"] = need
     got = {k: held(v) for k, v in sizes.items()}
     x, w, dy = given["x"], given["w"], given["dy"]
