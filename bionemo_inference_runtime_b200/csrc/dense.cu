@@ -104,7 +104,7 @@ int run_matmul(const Matmul& m, void* stream) {
   p.work = int(work);
   p.group_m = p.pair ? 8 : 16;
   const int b_rows = p.pair ? p.tile_n / 2 : p.tile_n;
-  const bool held = m.adapters != nullptr && low_blocks(m.adapters->rank) == 1 && (p.resident || low_requests(*m.adapters) >= 4);
+  const bool held = m.adapters != nullptr && low_blocks(m.adapters->rank) == 1 && p.resident;
   const int ring = matmul::kRingBytes - (held ? matmul::held_bytes(low_unit(m.adapters->rank)) : 0);
   p.stages = p.resident ? (ring - matmul::kResidentBytes) / matmul::kABytes : ring / (matmul::kABytes + b_rows * matmul::kBK * 2);
   if (p.stages > matmul::kMaxStages) p.stages = matmul::kMaxStages;

@@ -76,10 +76,10 @@ enum { kBesideNone = 0, kBesideFirst, kBesideSecond };
 // have the blocks of t and U_g (for dx: of dt and D_g), `unit` ranks wide; both terms of a block of t meet the same block of U_g.  The MMA
 // updates no lane (row) whose adapter is another, so nothing of one request, infinities and NaN among it, reaches another's rows.
 //
-// Usually each adapter's blocks pass through the ring like the others.  With `held` (a single block, few blocks of W or several
-// adapters a tile) a tile's t passes once, for all of its adapters, and U_g has room of its own behind the ring, where it stays until
-// an adapter or a column tile is another one.  Rows of one request after the other then load U_g hardly ever, and blocks keep
-// their tile of W (p.resident).  (147456 rows, 128 -> 512 gated, rank 16: 169 us through the ring.)
+// Usually each adapter's blocks pass through the ring like the others.  With `held` (a single block of ranks, and blocks that keep their
+// tile of W) a tile's t passes once, for all of its adapters, and U_g has room of its own behind the ring, where it stays until an
+// adapter is another one: rows of one request after the other load it hardly ever.  (147456 rows, 128 -> 512 gated, rank 16: 82 us so,
+// without adapters 64, through the ring 110.  For tiles of many adapters the ring is better: it looks further ahead.)
 struct NoAdapters {};
 struct MatmulAdapters {
   CUtensorMap low, high;
