@@ -93,8 +93,9 @@ low_product_kernel(const LowProduct p, int share) {
   for (int row = share ? warp : 0; row < kLowRows && (in >> row & 1u); row += share ? kWarps : 1)
     if (__shfl_sync(0xffffffffu, mine.g[0], row) == kNoAdapter)
       for (int r = lane; r < kRanks; r += 32) store(row, r0 + r, 0.f);
-  for (int g = mine.next(-1); g != kNoAdapter; g = mine.next(g)) {
-    const uint32_t own = mine.rows_of(0, g) & in;
+  for (uint32_t taken[1]; mine.more();) {
+    const int g = mine.take(taken);
+    const uint32_t own = taken[0] & in;
     const float scale = p.scale != nullptr ? __ldg(p.scale + g) : p.scale_all;
     float acc[2][kTiles][4] = {};
     for (int plane = 0; plane < p.planes; ++plane) {

@@ -105,16 +105,17 @@ __device__ __forceinline__ int adapter_of_entry(const AdapterIndex& x, long long
 __device__ __forceinline__ int adapter_of(const AdapterIndex& x, uint32_t row) {
   return x.index == nullptr ? 0 : adapter_of_entry(x, index_entry(x, row));
 }
-// The adapters of 32 * kWords rows, which a warp walks in ascending order: of rows that share an entry the one, of others lane l has
-// those of rows 32 j + l.  fetch() starts the loads, arrived() waits for them.  The usual case is short (rows of the same entry as
+// The adapters of 32 * kWords rows, which a warp takes in the order of their first rows: of rows that share an entry the one, of others
+// lane l has those of rows 32 j + l.  fetch() starts the loads, arrived() waits for them.  The usual case is short (rows of the same entry as
 // before: two comparisons), since the warps that call this share their issue slots with sixteen others and an instruction takes them
 // some ten clocks.
 template <int kWords>
 struct TileAdapters {
   long long entry[kWords];
   int g[kWords];
-  uint32_t behind;      // bit j: this lane's row 32 j + l is behind the last one
-  uint32_t begin, end;  // rows of the whole tensor that entry[0] is of
+  uint32_t left[kWords];  // rows whose adapter has not been taken
+  int count;              // rows that there are
+  uint32_t begin, end;    // rows of the whole tensor that entry[0] is of
   bool same, next_same;
   __device__ __forceinline__ explicit TileAdapters(const AdapterIndex& x) : begin(0), end(x.index == nullptr ? ~0u : 0u) { entry[0] = 0; }
   __device__ __forceinline__ void fetch(const AdapterIndex& x, int row0, int rows) {
@@ -129,43 +130,60 @@ struct TileAdapters {
       return;
     }
     end = begin;
-    behind = 0;
+    count = rows - row0;
 #pragma unroll
     for (int j = 0; j < kWords; ++j) {
-      const int row = row0 + j * 32 + int(threadIdx.x & 31);
-      const bool in = row < rows;
-      entry[j] = in ? index_entry(x, uint32_t(row)) : -1;
-      behind |= in ? 0u : 1u << j;
+      const int row = j * 32 + int(threadIdx.x & 31);
+      entry[j] = row < count ? index_entry(x, uint32_t(row0 + row)) : -1;
     }
   }
   __device__ __forceinline__ void arrived(const AdapterIndex& x) {
     same = next_same;
     if (same) {
       g[0] = adapter_of_entry(x, entry[0]);
+      left[0] = g[0] != kNoAdapter;
       return;
     }
 #pragma unroll
-    for (int j = 0; j < kWords; ++j) g[j] = adapter_of_entry(x, entry[j]);
+    for (int j = 0; j < kWords; ++j) {
+      g[j] = adapter_of_entry(x, entry[j]);
+      left[j] = __ballot_sync(0xffffffffu, g[j] != kNoAdapter);
+    }
   }
-  // The first adapter behind `last` (-1: the first of all), kNoAdapter where there is none.
-  __device__ __forceinline__ int next(int last) const {
-    if (same) return last < 0 ? g[0] : kNoAdapter;
-    int least = kNoAdapter;
+  // Whether rows are left whose adapter has not been taken.
+  __device__ __forceinline__ bool more() const {
+    uint32_t any = left[0];
+    if (!same)
 #pragma unroll
-    for (int j = 0; j < kWords; ++j)
-      if (g[j] > last && g[j] < least) least = g[j];
-    return int(__reduce_min_sync(0xffffffffu, unsigned(least)));
+      for (int j = 1; j < kWords; ++j) any |= left[j];
+    return any != 0;
   }
-  // Whether no row has another adapter than a, or none.
-  __device__ __forceinline__ bool all_have(int a) const {
+  // Takes the adapter of the first row that is left; bit l of rows[j]: row 32 j + l has it.
+  __device__ __forceinline__ int take(uint32_t (&rows)[kWords]) {
+    if (same) {
+      left[0] = 0;
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) rows[j] = ~0u;
+      return g[0];
+    }
+    int value = g[0];
+    uint32_t bits = left[0];
+#pragma unroll
+    for (int j = 1; j < kWords; ++j)
+      if (bits == 0) value = g[j], bits = left[j];
+    const int a = __shfl_sync(0xffffffffu, value, __ffs(bits) - 1);
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) rows[j] = __ballot_sync(0xffffffffu, g[j] == a), left[j] &= ~rows[j];
+    return a;
+  }
+  // Whether these are all rows that there are.
+  __device__ __forceinline__ bool all(const uint32_t (&rows)[kWords]) const {
     if (same) return true;
-    bool all = true;
+    bool every = true;
 #pragma unroll
-    for (int j = 0; j < kWords; ++j) all &= g[j] == a || behind >> j & 1;
-    return __all_sync(0xffffffffu, all);
+    for (int j = 0; j < kWords; ++j) every &= rows[j] == (count >= 32 * (j + 1) ? ~0u : count > 32 * j ? (1u << (count - 32 * j)) - 1u : 0u);
+    return every;
   }
-  // Bit l: row 32 j + l has adapter a.
-  __device__ __forceinline__ uint32_t rows_of(int j, int a) const { return same ? (a == g[0] ? ~0u : 0u) : __ballot_sync(0xffffffffu, g[j] == a); }
 };
 #endif
 

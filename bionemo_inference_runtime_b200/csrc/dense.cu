@@ -149,7 +149,7 @@ int run_matmul(const Matmul& m, void* stream) {
   if (m.adapters == nullptr) return launch(NoAdapters{});
   const LowRank& a = *m.adapters;
   MatmulAdapters x{};
-  x.index = a.index, x.rank = a.rank, x.unit = low_unit(a.rank), x.blocks = low_blocks(a.rank), x.held = held;
+  x.index = a.index, x.rank = a.rank, x.unit = low_unit(a.rank), x.blocks = low_blocks(a.rank), x.held = held, x.share = 64 / x.unit;
   x.slots = std::min(matmul::kHighSlots, matmul::held_bytes(x.unit) / (b_rows * x.unit * 2));
   const SwizzleMode swizzle = x.unit == 32 ? SWZ_64 : SWZ_32;
   const Plane low{a.low, rows, low_pitch(a.rank), low_pitch(a.rank)};

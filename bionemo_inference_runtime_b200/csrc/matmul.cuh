@@ -86,6 +86,7 @@ struct MatmulAdapters {
   AdapterIndex index;
   int rank, unit, blocks;
   int held, slots;     // room for that many blocks of U_g
+  int share;           // adapters that share a stage of the ring (with a single block of ranks)
   const float* scale;  // kLow: of each adapter, or NULL: scale_all; where the values go
   float scale_all;
   void* low_out;
@@ -537,7 +538,8 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           auto& adapters = ahead.adapters;
           adapters.arrived(x.index);
           const int planes = p.kblocks / p.kblocks_inner;
-          for (int g = adapters.next(-1); ok && g != kNoAdapter; g = adapters.next(g)) {
+          for (uint32_t rows[kPair ? 8 : 4]; ok && adapters.more();) {
+            const int g = adapters.take(rows);
             for (int kb = 0, ko = 0, ki = 0; kb < p.kblocks; ++kb) {
               open_stage(stage_bytes);
               if (!ok) break;
@@ -573,13 +575,30 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           auto& adapters = ahead.adapters;
           adapters.arrived(x.index);
           bool first = true;
-          for (int g = adapters.next(-1); ok && t.split == p.splits - 1 && g != kNoAdapter; g = adapters.next(g)) {
+          for (uint32_t rows[kPair ? 8 : 4]; ok && t.split == p.splits - 1 && adapters.more();) {
             if (!low_complete) pdl_wait(), low_complete = true;
+            int g[4] = {adapters.take(rows)};
             if (x.held) {
               if (first) load_low(t.m0);
               first = false;
-              if (ok) hold(g, t.n0);
-              if (adapters.same) break;
+              if (ok) hold(g[0], t.n0);
+              continue;
+            }
+            if (x.blocks == 1) {  // blocks of U_g as wide as one of W, of as many adapters, share a stage and a block of t
+              int count = 1;
+#pragma unroll
+              for (int j = 1; j < 4; ++j)
+                if (j < x.share && adapters.more()) g[j] = adapters.take(rows), count = j + 1;
+              const int bytes = b_rows * x.unit * 2;
+              open_stage(2 * kBM * x.unit * 2 + count * bytes);
+              if (!ok) break;
+              const uint32_t sa = ring + stage * stage_bytes;
+              load(sa, &x.low, full, 0, t.m0, 0);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (j < count) load_high(sa + kABytes + j * bytes, t.n0, 0, g[j]);
+              ++issued;
+              if (++stage == p.stages) stage = 0, phase ^= 1u;
               continue;
             }
             for (int block = 0; block < x.blocks; ++block) {
@@ -587,7 +606,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               if (!ok) break;
               const uint32_t sa = ring + stage * stage_bytes;
               load(sa, &x.low, full, block * 2 * x.unit, t.m0, 0);
-              load_high(sa + kABytes, t.n0, block * x.unit, g);
+              load_high(sa + kABytes, t.n0, block * x.unit, g[0]);
               ++issued;
               if (++stage == p.stages) stage = 0, phase ^= 1u;
             }
@@ -676,13 +695,14 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               if (++stage == p.stages) stage = 0, phase ^= 1u;
             }
           };
-          for (int g = adapters.next(-1); ok && g != kNoAdapter; g = adapters.next(g)) {
-            if (adapters.all_have(g)) {
+          bool first = true;
+          for (uint32_t off[4]; ok && adapters.more(); first = false) {
+            adapters.take(off);
+            if (first && !adapters.more() && adapters.all(off)) {
               walk_k([&](uint64_t da, uint64_t db, uint32_t add) { umma_ss_warp(acc, da, db, id, add); });
             } else {
-              uint32_t off[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) off[j] = ~adapters.rows_of(j, g);
+              for (int j = 0; j < 4; ++j) off[j] = ~off[j];
               walk_k([&](uint64_t da, uint64_t db, uint32_t add) { umma_ss_lanes_warp(acc, da, db, id, off, add); });
             }
           }
@@ -742,16 +762,22 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
             }
           } else {
             uint64_t da = 0;  // the tile's block of t, if held
-            int low_stage = -1;
-            for (int g = adapters.next(-1); here && ok && g != kNoAdapter; g = adapters.next(g)) {
-              uint32_t off[kPair ? 8 : 4];
+            int low_stage = -1, g = kNoAdapter;
+            uint32_t off[kPair ? 8 : 4];
+            bool all = false, low_first = true;
+            auto take = [&]() {
+              g = adapters.take(off);
+              all = low_first && !adapters.more() && adapters.all(off);
+              low_first = false;
 #pragma unroll
-              for (int j = 0; j < (kPair ? 8 : 4); ++j) off[j] = ~adapters.rows_of(j, g);
-              const bool all = adapters.all_have(g);
-              auto multiply = [&](uint64_t a, uint64_t b, int ranks) {
-                if (all) steps(a, b, ranks, one);
-                else steps(a, b, ranks, [&](uint64_t ak, uint64_t bk) { umma_ss_lanes_warp(acc, ak, bk, id, off); });
-              };
+              for (int j = 0; j < (kPair ? 8 : 4); ++j) off[j] = ~off[j];
+            };
+            auto multiply = [&](uint64_t a, uint64_t b, int ranks) {
+              if (all) steps(a, b, ranks, one);
+              else steps(a, b, ranks, [&](uint64_t ak, uint64_t bk) { umma_ss_lanes_warp(acc, ak, bk, id, off); });
+            };
+            for (; here && ok && adapters.more();) {
+              take();
               if (x.held) {
                 if (low_stage < 0) {
                   ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
@@ -763,6 +789,21 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
                 if (!ok) break;
                 tc_fence_after();
                 multiply(da, held_desc, x.rank);
+                continue;
+              }
+              if (x.blocks == 1) {
+                ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t sa = ring + stage * stage_bytes, bytes = b_rows * x.unit * 2;
+                const uint64_t low = low_desc | (sa >> 4);
+                multiply(low, high_desc | ((sa + kABytes) >> 4), x.rank);
+                for (int j = 1; j < x.share && adapters.more(); ++j) {
+                  take();
+                  multiply(low, high_desc | ((sa + kABytes + j * bytes) >> 4), x.rank);
+                }
+                release_stage(stage);
+                if (++stage == p.stages) stage = 0, phase ^= 1u;
                 continue;
               }
               for (int block = 0; block < x.blocks; ++block) {
