@@ -20,7 +20,7 @@ __device__ __forceinline__ void store_low(const LowProduct& p, long long row, in
   T* low = static_cast<T*>(p.low) + row * low_pitch(p.rank) + low_place(p.rank, r);
   const T rounded = static_cast<T>(v);
   *low = rounded;
-  low[low_unit(p.rank)] = static_cast<T>(v - static_cast<float>(rounded));
+  low[low_unit(p.rank)] = static_cast<T>(second_term(v, static_cast<float>(rounded)));
 }
 
 // ---- low-rank values, a warp for each ------------------------------------------------------------------------------
@@ -156,7 +156,7 @@ low_product_kernel(const LowProduct p, int share) {
             const uint32_t rounded = pack2<T>(v0, v1);
             const float2 f = unpack2<T>(rounded);
             *reinterpret_cast<uint32_t*>(to) = rounded;
-            *reinterpret_cast<uint32_t*>(to + low_unit(p.rank)) = pack2<T>(v0 - f.x, v1 - f.y);
+            *reinterpret_cast<uint32_t*>(to + low_unit(p.rank)) = pack2<T>(second_term(v0, f.x), second_term(v1, f.y));
           }
     }
   }
@@ -224,7 +224,7 @@ low_up_kernel(const LowUpParams p) {
   else total *= p.scale != nullptr ? __ldg(p.scale + g) : p.scale_all;
   T* low = static_cast<T*>(p.low) + row * low_pitch(p.rank) + low_place(p.rank, r);
   const T rounded = static_cast<T>(total);
-  low[0] = rounded, low[low_unit(p.rank)] = static_cast<T>(total - static_cast<float>(rounded));
+  low[0] = rounded, low[low_unit(p.rank)] = static_cast<T>(second_term(total, static_cast<float>(rounded)));
 }
 
 // ---- up matrices with their columns contiguous -----------------------------------------------------------------------

@@ -94,6 +94,11 @@ int run_low_grads(const LowGrads& m, void* stream);
 int run_low_join(const LowGrads& m, void* stream);
 
 #ifdef __CUDACC__
+// What the rounding of v to `rounded` left out; nothing of what has no number in 16 bits, so that infinities stay infinities.
+__device__ __forceinline__ float second_term(float v, float rounded) {
+  const float rest = v - rounded;
+  return fabsf(rest) <= 3.402823466e38f ? rest : 0.f;
+}
 // (Past the first-level cache: a kernel that starts beside the one before it reads what was complete before both.)
 __device__ __forceinline__ long long index_entry(const AdapterIndex& x, uint32_t row) {
   const uint32_t i = uint32_t(uint64_t(x.first_row + row) * x.factor >> x.shift);

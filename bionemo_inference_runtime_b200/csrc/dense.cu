@@ -366,7 +366,7 @@ few_rows_kernel(const FewParams p) {
       const float v = r < p.adapters.rank ? own_low[row * p.adapters.rank + r] : 0.f;
       T* low = static_cast<T*>(p.low_out) + row * 2 * half + low_place(p.adapters.rank, r);
       const T rounded = static_cast<T>(v);
-      low[0] = rounded, low[low_unit(p.adapters.rank)] = static_cast<T>(v - static_cast<float>(rounded));
+      low[0] = rounded, low[low_unit(p.adapters.rank)] = static_cast<T>(second_term(v, static_cast<float>(rounded)));
     }
   }
   for (int own = threadIdx.x / kFewColumns; own < rows && n < p.N; own += blockDim.x / kFewColumns) {

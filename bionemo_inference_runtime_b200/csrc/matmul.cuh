@@ -929,7 +929,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
             const float v0 = g == kNoAdapter ? 0.f : v[2 * j] * scale, v1 = g == kNoAdapter ? 0.f : v[2 * j + 1] * scale;
             first[j] = pack2<T>(v0, v1);
             const float2 f = unpack2<T>(first[j]);
-            second[j] = pack2<T>(v0 - f.x, v1 - f.y);
+            second[j] = pack2<T>(second_term(v0, f.x), second_term(v1, f.y));
           }
           T* to = static_cast<T*>(x.low_out) + (long long)(row + lane) * low_pitch(x.rank) + low_place(x.rank, r);
 #pragma unroll

@@ -9,6 +9,7 @@ on the transposed view by swapping the two pair strides (no copy).
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 
@@ -624,7 +625,8 @@ def _dropout(x, p, seed, sequence, residual, shared, out):
     if shared is not None and not -x.dim() <= shared < x.dim():
         raise ValueError(f"shared must be an axis of x {tuple(x.shape)} or None, got {shared}")
     axis = -1 if shared is None else shared % x.dim()
-    return _host.dropout(x, round(p * 65536), 0 if at is not None else seed & _WORD, sequence & _WORD, at, residual, axis, out)
+    number = 0 if at is not None else operator.index(seed) & _WORD
+    return _host.dropout(x, round(p * 65536), number, operator.index(sequence) & _WORD, at, residual, axis, out)
 
 
 def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, sequence: int = 0, *, residual: torch.Tensor | None = None,

@@ -237,6 +237,15 @@ def test_nothing_of_a_request_reaches_another(n, each, gated):
     assert all(a is None if c is None else torch.equal(a, c) for a, c in zip(again, clean, strict=True))  # the same bits each time
 
 
+@pytest.mark.parametrize("rows", [2, 40, 300, 700])
+def test_what_leaves_the_range_of_16_bits_is_infinite(rows):
+    """A low-rank value past 65504 in fp16 is an infinity there, not the NaN of what it lacks."""
+    given = layer(rows, 64, 40, 1, 8, torch.float16, residual=False, bias=False)
+    x = given["x"].abs() * 100
+    y = ops.adapter_dense(x, given["w"], None, given["down"].abs() + 20, given["up"].abs() + 0.01)
+    assert torch.isinf(y).all() and (y > 0).all()
+
+
 def test_strides():
     """Operands that no aligned load takes as they lie: odd pitches, transposed, broadcast and single-column tensors."""
     for n, each in ((6, 1), (60, 1), (10, 40)):
