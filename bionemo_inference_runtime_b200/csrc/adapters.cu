@@ -289,7 +289,7 @@ __device__ __forceinline__ uint32_t pair_mask(uint32_t bits) { return ((bits & 1
 template <typename T, int kTiles>  // tiles of 16 ranks
 __global__ void __launch_bounds__((kGradWarps + 1) * 32, 2)
 low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
-  constexpr int kStages = grad_stages(kTiles), kStage = grad_stage(kTiles), kUnit = kTiles == 1 ? 16 : 32;
+  constexpr int kStages = grad_stages(kTiles), kStage = grad_stage(kTiles);
   extern __shared__ uint8_t raw[];
   __shared__ uint32_t masks[kGradChunks][2];
   __shared__ uint16_t list[kGradChunks];
@@ -395,10 +395,19 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
         for (int j = i > kStages ? i - kStages : 0; j < i; ++j) mbar_wait(bar0 + j % kStages * 8, j / kStages & 1, abort_flag + 1);
     }
   } else {
-    float acc[kTiles][2][4] = {};
+    // A warp has 16 columns and all ranks, or of 64 ranks half and 32 columns: fewer operands for as many products (each warp reads its
+    // part of t from shared memory, which bounds it; 8192 rows of 8192 columns: 61 us with all ranks, now 50).
+    constexpr int kWays = kTiles == 4 ? 2 : 1, kOwn = kTiles / kWays;
+    const int way = kWays == 2 ? warp >> 2 : 0, columns0 = kWays == 2 ? (warp & 3) * 32 : warp * 16;
+    float acc[kOwn][2 * kWays][4] = {};
     // rows of 128 bytes (t of 16 ranks: 64) whose 16-byte vectors are swizzled by the row
     const int vr = lane & 15, tr = (lane >> 4) * 8 + (lane & 7);
-    const uint32_t v_at = (warp >> 2) * (kGradV / 2) + vr * 128 + ((((warp & 3) * 2 + (lane >> 4)) ^ (vr & 7)) << 4);
+    uint32_t v_at[kWays];
+#pragma unroll
+    for (int j = 0; j < kWays; ++j) {
+      const int vec = columns0 / 8 + j * 2 + (lane >> 4);
+      v_at[j] = (vec >> 3) * (kGradV / 2) + vr * 128 + (((vec & 7) ^ (vr & 7)) << 4);
+    }
     bool ok = true;
     for (int i = 0; i < count; ++i) {
       const int s = i % kStages;
@@ -409,20 +418,25 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
       auto walk = [&](auto&& mask) {
 #pragma unroll
         for (int k = 0; k < kGradRows; k += 16) {
-          uint32_t b[4];
-          ldmatrix4_t(stage + v_at + k * 128, b);
-          mask(k, b[0], b[2], b[1], b[3]);
+          uint32_t b[kWays][4];
 #pragma unroll
-          for (int m = 0; m < 2 * kTiles; ++m) {  // tiles of a block's first, then of its second terms
-            constexpr int kBlock = kUnit / 16;
-            const int tile = m / (2 * kBlock) * kBlock + m % kBlock, row = k + tr;
+          for (int j = 0; j < kWays; ++j) {
+            ldmatrix4_t(stage + v_at[j] + k * 128, b[j]);
+            mask(k, b[j][0], b[j][2], b[j][1], b[j][3]);
+          }
+#pragma unroll
+          for (int m = 0; m < 2 * kOwn; ++m) {  // tiles of the block's first, then of its second terms
+            const int row = k + tr;
             const uint32_t t_at = kTiles == 1 ? row * 64 + ((m * 2 + (lane >> 3 & 1)) ^ (row >> 1 & 3)) * 16
-                                              : m / 4 * (kGradRows * 128) + row * 128 + ((m % 4 * 2 + (lane >> 3 & 1)) ^ (row & 7)) * 16;
+                                              : way * (kGradRows * 128) + row * 128 + ((m * 2 + (lane >> 3 & 1)) ^ (row & 7)) * 16;
             uint32_t a[4];
             ldmatrix4_t(stage + kGradV + t_at, a);
             mask(k, a[0], a[1], a[2], a[3]);
-            mma16816<T>(acc[tile][0], a[0], a[1], a[2], a[3], b[0], b[1]);
-            mma16816<T>(acc[tile][1], a[0], a[1], a[2], a[3], b[2], b[3]);
+#pragma unroll
+            for (int j = 0; j < kWays; ++j) {
+              mma16816<T>(acc[m % kOwn][2 * j], a[0], a[1], a[2], a[3], b[j][0], b[j][1]);
+              mma16816<T>(acc[m % kOwn][2 * j + 1], a[0], a[1], a[2], a[3], b[j][2], b[j][3]);
+            }
           }
         }
       };
@@ -442,12 +456,12 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
     float* part = job.part + ((long long)blockIdx.y * adapters + g) * p.rank * pitch + plane * plane_columns;
     T* out = static_cast<T*>(job.out) + (long long)g * p.rank * all;
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m)
+    for (int m = 0; m < kOwn; ++m)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < 2 * kWays; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int r = r0 + m * 16 + (lane >> 2) + 8 * (e >> 1), c = c0 + warp * 16 + n * 8 + (lane & 3) * 2 + (e & 1);
+          const int r = r0 + (way * kOwn + m) * 16 + (lane >> 2) + 8 * (e >> 1), c = c0 + columns0 + n * 8 + (lane & 3) * 2 + (e & 1);
           if (r >= p.rank || c >= job.columns) continue;
           if (p.direct) {
             const long long column = (long long)plane * job.columns + c;
