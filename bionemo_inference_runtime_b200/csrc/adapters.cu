@@ -495,32 +495,35 @@ struct LowJoinParams {
   const uint8_t* marks;     // [part][adapter, group of 64 ranks][slab of 128 columns]: parts that were written
   int slabs, slabs0;
 };
-template <typename T, int kSlices>
-__global__ void __launch_bounds__(256)
+template <typename T, int kSlices, typename Int>  // Int: unsigned, wide enough for all items
+__global__ void __launch_bounds__(256, 4)
 low_join_kernel(const LowJoinParams p) {
   constexpr int kItems = 256 / kSlices;
   __shared__ float joined[kSlices > 1 ? kSlices - 1 : 1][8][kItems];
   pdl_trigger();
   pdl_wait();
   const int own = threadIdx.x % kItems, slice = threadIdx.x / kItems;
-  for (long long first = (long long)blockIdx.x * kItems; first < p.items; first += (long long)gridDim.x * kItems) {
-    const long long i = first + own;
-    const bool second = i >= p.items0;
+  const Int items = Int(p.items), items0 = Int(p.items0);
+  for (Int first = Int(blockIdx.x) * kItems; first < items; first += Int(gridDim.x) * kItems) {
+    const Int i = first + own;
+    const bool second = i >= items0;
     const LowGrad& job = second ? p.job[1] : p.job[0];
-    long long at = second ? i - p.items0 : i;
-    const int all = job.columns * job.planes, plane_columns = (job.columns + 3) / 4 * 4;
+    const Int at = second ? i - items0 : i;
+    const uint32_t all = uint32_t(job.columns) * job.planes;
+    const int plane_columns = (job.columns + 3) / 4 * 4, ranks = job.transposed ? 8 : 1;
     const long long pitch = (long long)plane_columns * job.planes, stride = (long long)p.adapters * p.rank * pitch;
-    const int column = int(at % all), plane = column / job.columns, ranks = job.transposed ? 8 : 1;
-    at /= all;
-    const int groups = (p.rank + ranks - 1) / ranks, r0 = int(at % groups) * ranks;
-    const long long g = at / groups;
+    const Int row = at / all;
+    const int column = int(at - row * all), plane = column >= job.columns;
+    const uint32_t groups = uint32_t(p.rank + ranks - 1) / ranks;
+    const long long g = row / groups;
+    const int r0 = int(row - Int(g) * groups) * ranks;
     const float* part = job.part + (g * p.rank + r0) * pitch + plane * plane_columns + (column - plane * job.columns);
     const int rank_groups = (p.rank + 63) / 64, slabs_plane = (job.columns + kGradColumns - 1) / kGradColumns;
     const uint8_t* mark = p.marks + (g * rank_groups + r0 / 64) * p.slabs + (second ? p.slabs0 : 0) + plane * slabs_plane + (column - plane * job.columns) / kGradColumns;
     const long long mark_stride = (long long)p.adapters * rank_groups * p.slabs;
     float sum[8] = {};
     const int n = p.rank - r0 < ranks ? p.rank - r0 : ranks;
-    if (i < p.items) {
+    if (i < items) {
       if (job.transposed) {
 #pragma unroll 2
         for (int s = slice; s < p.parts; s += kSlices) {
@@ -551,7 +554,7 @@ low_join_kernel(const LowJoinParams p) {
           for (int r = 0; r < 8; ++r) sum[r] += joined[s][r][own];
       __syncthreads();
     }
-    if (slice > 0 || i >= p.items) continue;
+    if (slice > 0 || i >= items) continue;
     if (!job.transposed) {
       static_cast<T*>(job.out)[(g * p.rank + r0) * all + column] = static_cast<T>(sum[0]);
       continue;
@@ -677,8 +680,11 @@ int run_low_join(const LowGrads& m, void* stream) {
   // several threads to an item where there are many parts of few values
   const bool sliced = m.parts >= 4 && p.items < int64_t(st->num_sms) * (m.parts >= 8 ? 1024 : 256);
   const int64_t each = sliced ? 32 : 256, blocks = std::min<int64_t>((p.items + each - 1) / each, int64_t(st->num_sms) * 16);
-  auto* kernel = m.f16 ? (sliced ? low_join_kernel<__half, 8> : low_join_kernel<__half, 1>)
-                       : (sliced ? low_join_kernel<__nv_bfloat16, 8> : low_join_kernel<__nv_bfloat16, 1>);
+  void (*kernel)(LowJoinParams);
+  if (p.items < (int64_t(1) << 31))
+    kernel = m.f16 ? (sliced ? low_join_kernel<__half, 8, uint32_t> : low_join_kernel<__half, 1, uint32_t>)
+                   : (sliced ? low_join_kernel<__nv_bfloat16, 8, uint32_t> : low_join_kernel<__nv_bfloat16, 1, uint32_t>);
+  else kernel = m.f16 ? low_join_kernel<__half, 1, uint64_t> : low_join_kernel<__nv_bfloat16, 1, uint64_t>;
   return launch_kernel(st, kKernelAdapter, kernel, dim3(unsigned(blocks)), 256, 0, stream, p);
 }
 
