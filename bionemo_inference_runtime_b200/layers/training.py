@@ -249,6 +249,8 @@ class TrainableTransition(nn.Module):
         state = {k: v for k, v in self.state_dict().items() if "_adapters." not in k}
         if self.fc3_adapters is None:
             return state
+        if not 0 <= adapter < self.fc3_adapters.down.shape[0]:
+            raise ValueError(f"there is no adapter {adapter} of {self.fc3_adapters.down.shape[0]}")
         for name, adapters in (("fused_fc2_fc1", self.fused_fc2_fc1_adapters), ("fc3", self.fc3_adapters)):
             weight = state[f"{name}.weight"]
             added = adapters.up[adapter].detach().double() @ adapters.down[adapter].detach().double()
@@ -269,7 +271,8 @@ class TrainableTransition(nn.Module):
 
     def forward(self, x: torch.Tensor, mask: torch.Tensor | None = None, *, residual: bool = False,
                 index: torch.Tensor | None = None, seed: int | torch.Tensor | None = None, sequence: int = 0) -> torch.Tensor:
-        """``seed`` and ``sequence`` are those of :func:`dropout`; without a seed one is drawn from PyTorch's CPU generator."""
+        """``seed`` and ``sequence`` are those of :func:`dropout`; without a seed one is drawn from PyTorch's CPU generator (a step that
+        is captured into a graph needs one, on the device if it is to be another one at each replay)."""
         if residual and self.out_dim != self.dim:
             raise ValueError(f"a residual needs out_dim == dim, got {self.out_dim} and {self.dim}")
         if index is not None and self.fc3_adapters is None:
@@ -283,6 +286,9 @@ class TrainableTransition(nn.Module):
         if mask is not None:
             update = update * _row_mask(x, mask).unsqueeze(-1).to(x.dtype)
         if drops:
-            seed = int(torch.randint(1 << 62, ())) if seed is None else seed
+            if seed is None:
+                if x.is_cuda and torch.cuda.is_current_stream_capturing():
+                    raise ValueError("a captured step needs a seed: one drawn now would drop the same elements at every replay")
+                seed = int(torch.randint(1 << 62, ()))
             return dropout(update, self.dropout, seed, sequence, residual=x if residual else None, shared=self.dropout_shared)
         return x + update if residual else update

@@ -86,3 +86,6 @@ def test_state_of_an_adapted_transition_merges_into_a_plain_one():
     want = layer.fc3.weight.double() + 0.5 * layer.fc3_adapters.up[1].double() @ layer.fc3_adapters.down[1].double()
     assert torch.equal(merged, want.to(torch.bfloat16))
     assert torch.equal(plain.merged_state_dict()["fc3.weight"], plain.fc3.weight)
+    for none in (-1, 2):  # (-1 stands for no adapter elsewhere)
+        with pytest.raises(ValueError, match="adapter"):
+            layer.merged_state_dict(none)

@@ -137,6 +137,22 @@ def test_captured_training_step():
         assert all(torch.equal(a, b) for a, b in zip(out, want, strict=True))
 
 
+def test_a_captured_step_needs_a_seed():
+    layer, x = adapted(64, 96, 2, dropout=0.2), randn(4, 50, 64, seed=1)
+    index = torch.tensor([0, 1, -1, 1], device=DEV)
+    with torch.no_grad():
+        layer(x, index=index)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()), pytest.raises(ValueError, match="seed"):
+            layer(x, index=index)
+        layer.eval()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = layer(x, index=index)
+        graph.replay()
+        assert torch.equal(y, layer(x, index=index))
+
+
 def test_example():
     path = Path(__file__).resolve().parent.parent / "examples" / "finetune_adapters.py"
     spec = importlib.util.spec_from_file_location("finetune_adapters", path)
