@@ -395,7 +395,7 @@ std::tuple<at::Tensor, Maybe, Maybe> adapter_dense(const at::Tensor& x, const at
 
 std::tuple<Maybe, Maybe, Maybe, Maybe, Maybe> adapter_dense_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w, const Maybe& bias,
                                                                      const at::Tensor& down, const at::Tensor& up, const Maybe& index,
-                                                                     const Maybe& scale, double scale_all, const at::Tensor& low, const Maybe& saved,
+                                                                     const Maybe& scale, double scale_all, const Maybe& low, const Maybe& saved,
                                                                      int64_t activation, bool gated, bool want_dx, bool want_dweight, bool want_dbias,
                                                                      bool want_ddown, bool want_dup) {
   const Layer l = layer_of(x, w, bias, activation, gated);
@@ -407,8 +407,9 @@ std::tuple<Maybe, Maybe, Maybe, Maybe, Maybe> adapter_dense_backward(const at::T
   Copies copies;
   const Adapting a = adapters_of(x, l, w.size(0), down, up, index, scale, scale_all, false, copies);
   const int64_t low_pitch = int64_t(lib.adapter_low_bytes(a.c.rank)) / 2;
-  require_like("saved", low, x, {l.rows, low_pitch});
-  if (!low.is_contiguous()) refuse("saved must be what the forward pass returned");
+  if (!low) refuse("saved must be what the forward pass returned with want_saved");
+  require_like("saved", *low, x, {l.rows, low_pitch});
+  if (!low->is_contiguous()) refuse("saved must be what the forward pass returned");
   if (saved) {
     require_like("saved", *saved, x, {l.rows, pitch}, true);
     if (!saved->is_contiguous() || saved->scalar_type() != at::kFloat) refuse("saved must be what the forward pass returned");
@@ -426,7 +427,7 @@ std::tuple<Maybe, Maybe, Maybe, Maybe, Maybe> adapter_dense_backward(const at::T
   const Maybe b = bias ? Maybe(bias->contiguous()) : Maybe();
   const size_t need = lib.adapter_dense_backward_workspace_bytes(int(activation), gated, saved.has_value(), want_dbias, &a.c, l.rows, l.K, l.N);
   const at::Tensor workspace = bytes(x, need);
-  check(lib.adapter_dense_backward(rdy.ptr, rdy.stride, rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), pointer(saved), pitch, &a.c, low.data_ptr(),
+  check(lib.adapter_dense_backward(rdy.ptr, rdy.stride, rx.ptr, rx.stride, rw.ptr, rw.stride, pointer(b), pointer(saved), pitch, &a.c, pointer(low),
                                    pointer(dx), l.K, pointer(dweight), pointer(dbias), pointer(ddown), pointer(dup), workspace.data_ptr(),
                                    need, l.dtype, int(activation), gated, l.rows, l.K, l.N, stream()),
         "b200ta_adapter_dense_backward");

@@ -355,7 +355,7 @@ def test_empty_and_refused():
     with pytest.raises(ValueError, match="rank"):
         ops.adapter_dense(wide["x"], wide["w"], None, wide["down"], wide["up"])
     y, saved = call(want_saved=True)
-    for kept in ((saved[0][:5], None), (saved[0].half(), None), (saved[0], torch.zeros(12, 8, device=DEV))):
+    for kept in ((saved[0][:5], None), (saved[0].half(), None), (saved[0], torch.zeros(12, 8, device=DEV)), (None, None)):
         with pytest.raises(ValueError, match="saved"):
             ops.adapter_dense_backward(y, g["x"], g["w"], None, g["down"], g["up"], g["index"], saved=kept)
 
