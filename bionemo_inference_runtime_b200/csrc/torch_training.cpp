@@ -8,6 +8,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include "../../include/b200ta.h"
 
@@ -434,6 +436,19 @@ std::tuple<Maybe, Maybe, Maybe, Maybe, Maybe> adapter_dense_backward(const at::T
   return {dx, dweight, dbias, ddown, dup};
 }
 
+// Whether a leaf among these tensors has a node that accumulates its gradients on the default stream, which an eager graph of the leaf
+// that is alive keeps: a backward pass that is being captured cannot reach that stream, and PyTorch would end the capture with an error
+// that names neither.
+bool accumulated_elsewhere(const std::vector<Maybe>& tensors) {
+  for (const Maybe& t : tensors) {
+    if (!t || !t->is_cuda() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto on = node ? node->stream() : std::nullopt;
+    if (on && *on == c10::cuda::getDefaultCUDAStream(t->device().index()).unwrap()) return true;
+  }
+  return false;
+}
+
 // ---- dropout ----------------------------------------------------------------------------------------------------------
 
 at::Tensor dropout(const at::Tensor& x, int64_t dropped, uint64_t seed, uint64_t sequence, const Maybe& seed_at, const Maybe& residual,
@@ -484,6 +499,7 @@ void define_training(py::module_& m) {
   m.def("adapter_dense", &adapter_dense);
   m.def("adapter_dense_backward", &adapter_dense_backward);
   m.def("dropout", &dropout);
+  m.def("accumulated_elsewhere", &accumulated_elsewhere);
 }
 
 }  // namespace b200ta_host

@@ -78,6 +78,12 @@ class _GatedDense(torch.autograd.Function):
         return (*grads, None)
 
 
+def _refuse_capture(*inputs: torch.Tensor | None) -> None:
+    if torch.cuda.is_current_stream_capturing() and ops._host.accumulated_elsewhere(inputs):
+        raise RuntimeError("a backward pass is captured into a graph while an eager graph of the same leaves is alive, whose gradients are "
+                           "accumulated on the default stream: release that graph first")
+
+
 class _AdapterDense(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, down, up, residual, index, scale, activation, gated):
@@ -95,6 +101,7 @@ class _AdapterDense(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, down, up, index, scale, *saved = ctx.saved_tensors
+        _refuse_capture(x, weight, bias, down, up)
         wanted = ctx.needs_input_grad
         grads = (None,) * 5
         if any(wanted[:5]):

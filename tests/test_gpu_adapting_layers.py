@@ -137,6 +137,33 @@ def test_captured_training_step():
         assert all(torch.equal(a, b) for a, b in zip(out, want, strict=True))
 
 
+def test_a_backward_pass_is_not_captured_beside_an_eager_graph_of_its_leaves():
+    """Their gradients' nodes lie on the default stream while that graph lives; without it, or with one of another stream, capture works."""
+    x, w, dy = randn(32, 64, seed=1), randn(48, 64, seed=2), randn(32, 48, seed=3)
+    down, up = (t.requires_grad_(True) for t in (randn(1, 8, 64, seed=4), randn(1, 48, 8, seed=5)))
+    want = torch.autograd.grad(b200.adapter_dense(x, w, None, down, up), (down, up), dy)
+
+    def captured():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(b200.adapter_dense(x, w, None, down, up), (down, up), dy)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+
+    alive = b200.adapter_dense(x, w, None, down, up)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        captured()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(alive, (down, up), dy), want, strict=True))
+    del alive
+    captured()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        alive = b200.adapter_dense(x, w, None, down, up)
+    side.synchronize()
+    captured()
+    del alive
+
+
 def test_a_captured_step_needs_a_seed():
     layer, x = adapted(64, 96, 2, dropout=0.2), randn(4, 50, 64, seed=1)
     index = torch.tensor([0, 1, -1, 1], device=DEV)
