@@ -160,8 +160,12 @@ def gated_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
 
 
 def _adapter_dense(x, weight, bias, down, up, residual, index, scale, activation, gated):
-    if isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
+    if isinstance(scale, torch.Tensor) and _needs_grad(scale):
         raise NotImplementedError("the scale of adapters has no gradient")
+    if not _needs_grad(x, weight, bias, down, up, residual):
+        if gated:
+            return ops.adapter_gated_dense(x, weight, bias, down, up, index, scale, activation=activation)
+        return ops.adapter_dense(x, weight, bias, down, up, index, scale, activation=activation, residual=residual)
     return _AdapterDense.apply(x, weight, bias, down, up, residual, index, scale, activation, gated)
 
 
@@ -170,9 +174,7 @@ def adapter_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
                   residual: torch.Tensor | None = None) -> torch.Tensor:
     """Differentiable :func:`ops.adapter_dense <bionemo_inference_runtime_b200.ops.adapter_dense>`:
     ``activation(x @ weight.T + bias + scale[g] * (x @ down[g].T) @ up[g].T) + residual``."""
-    if _needs_grad(x, weight, bias, down, up, residual):
-        return _adapter_dense(x, weight, bias, down, up, residual, index, scale, activation, False)
-    return ops.adapter_dense(x, weight, bias, down, up, index, scale, activation=activation, residual=residual)
+    return _adapter_dense(x, weight, bias, down, up, residual, index, scale, activation, False)
 
 
 def adapter_gated_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, down: torch.Tensor, up: torch.Tensor,
@@ -180,9 +182,7 @@ def adapter_gated_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
                         activation: str = "silu") -> torch.Tensor:
     """Differentiable :func:`ops.adapter_gated_dense <bionemo_inference_runtime_b200.ops.adapter_gated_dense>`:
     ``value * activation(gate)``, both with their part of the adapter."""
-    if _needs_grad(x, weight, bias, down, up):
-        return _adapter_dense(x, weight, bias, down, up, None, index, scale, activation, True)
-    return ops.adapter_gated_dense(x, weight, bias, down, up, index, scale, activation=activation)
+    return _adapter_dense(x, weight, bias, down, up, None, index, scale, activation, True)
 
 
 def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, sequence: int = 0, *, residual: torch.Tensor | None = None,

@@ -5,6 +5,7 @@ from pathlib import Path
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import bionemo_inference_runtime_b200 as b200
 from bionemo_inference_runtime_b200 import _lib, ops
@@ -56,6 +57,28 @@ def test_host_tensors_and_bad_probabilities_are_refused():
     for rank in (-1, 257):
         with pytest.raises(ValueError, match="rank"):
             b200.TrainableTransition(8, 16, adapter_rank=rank, device="cpu")
+
+
+@pytest.mark.parametrize("function", [b200.adapter_dense, b200.adapter_gated_dense])
+def test_derivatives_that_there_are_not_are_refused(function):
+    """The gradient of a scale, asked for alone too, and forward-mode derivatives of any argument."""
+    x, w, b = torch.zeros(4, 8), torch.zeros(6, 8), torch.zeros(6)
+    down, up, scale = torch.zeros(2, 2, 8), torch.zeros(2, 6, 2), torch.ones(2)
+    index = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(NotImplementedError, match="scale"):
+        function(x, w, b, down, up, index, scale.requires_grad_(True))
+    scale.requires_grad_(False)
+    with forward_ad.dual_level():
+        for k in (0, 1, 2, 3, 4, 6):
+            given = [x, w, b, down, up, index, scale]
+            given[k] = forward_ad.make_dual(given[k], torch.ones_like(given[k]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                function(*given)
+        for k in (0, 1):
+            given = [x, x]
+            given[k] = forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                b200.dropout(given[0], 0.5, 1, residual=given[1])
 
 
 def test_rows_find_their_entry_by_a_product():
