@@ -259,8 +259,8 @@ transpose_up_kernel(const TransposeParams p) {
 // are transposed on their way from shared memory.  Of several adapters a block first lists the groups of 64 rows that hold its own;
 // in a group that others have a part of, their rows are cleared in the operands' registers, so that infinities and NaN in them stay
 // out.  Parts are written in 32 bits, with a mark that they have been (a part of the rows may have none of an adapter's), and joined in
-// a fixed order: results repeat bit by bit.  A single part is the result.  (Filled by cp.async from all threads,
-// 147456 rows of 128 and 1024 columns, rank 16: 89 us.)
+// a fixed order: results repeat bit by bit.  A single part is the result.  147456 rows of 128 and 1024 columns, rank 16: 57 us (359 MB at
+// 6.3 TB/s; filled by cp.async from all threads 89); 8192 rows of 8192 columns, rank 64: 50 us (the products' pipe 0.73 full).
 constexpr int kGradRows = 64, kGradColumns = 128, kGradChunks = 1024, kGradWarps = 8;
 // (up to 16, 32 or 64 ranks with their two terms are rows of 64 or 128 bytes, or two blocks of the latter)
 constexpr int kGradV = kGradRows * kGradColumns * 2;
@@ -586,8 +586,8 @@ int run_low(const LowProduct& m, void* stream) {
   const int rc = get_device_state(&st);
   if (rc != B200TA_OK) return rc;
   // Tiles of 128 rows on the tensor cores, unless those of several requests are too few to fill the device, or few ranks of a few
-  // thousand rows are done sooner by blocks of 32 (a layer of 3072 rows, 1536 -> 384, rank 16: 18.0 us so and 20.5 by tiles; of 768 rows
-  // with rank 64: 18.6 and 15.5; 2048 rows of 4096, rank 64: 75 and 57).
+  // thousand rows are done sooner by blocks of 32 (a layer of 4 x 768 rows, 1536 -> 384, rank 16: 18.0 us so and 20.5 by tiles; of 768
+  // rows with rank 64: 18.6 and 15.5; 2048 rows of 4096, rank 64: 75 and 57).
   const int64_t tiles = (m.rows + 127) / 128;
   const bool mixed = m.index.index != nullptr && m.index.count > 1 && m.index.rows_per_index < 128;
   const bool small = m.rows <= 512 || (mixed && tiles < st->num_sms) || (m.rank <= 16 && m.rows <= 8192 && m.K * m.planes <= 2048);
