@@ -162,14 +162,22 @@ low_product_kernel(const LowProduct p, int share) {
   }
 }
 
+int dot_groups(int rank) { return (low_pitch(rank) / 2 + kDotWarps - 1) / kDotWarps; }
+bool low_by_dots(const LowProduct& m, int num_sms) {
+  return low_by_rows(m.rows, m.rank, m.K * m.planes, m.index, dot_groups(m.rank), num_sms);
+}
 template <typename T, bool kVec>
 int launch_low(DeviceState* st, const LowProduct& m, void* stream) {
-  if (low_by_rows(m.rows, m.rank, m.K * m.planes, m.index)) {
-    const int groups = int((low_pitch(m.rank) / 2 + kDotWarps - 1) / kDotWarps);
+  if (low_by_dots(m, st->num_sms)) {
+    const int groups = dot_groups(m.rank);
     return launch_kernel(st, kKernelAdapter, low_dot_kernel<T, kVec>, dim3(unsigned(m.rows * groups)), kDotWarps * 32, 0, stream, m, groups);
   }
-  const int tiles = m.rank <= 16 ? 2 : m.rank <= 32 ? 4 : 8, warps = low_warps(tiles);
   const int64_t groups = (m.rows + kLowRows - 1) / kLowRows;
+  // All ranks in a block, up to 64, or more blocks of fewer where these leave multiprocessors idle (158 rows of 1448, rank 76, two adapters
+  // in turn: 10 us for 30; a gated training step of 300 rows of 2048, rank 64: 115 for 175).
+  int tiles = m.rank <= 16 ? 2 : m.rank <= 32 ? 4 : 8;
+  while (tiles > 2 && groups * ((low_pitch(m.rank) / 2 + tiles * 8 - 1) / (tiles * 8)) * 2 <= st->num_sms) tiles /= 2;
+  const int warps = low_warps(tiles);
   const int share = groups < int64_t(st->num_sms) * warps * 2 || m.K > 512;
   const dim3 grid{unsigned(share ? groups : (groups + warps - 1) / warps), unsigned((low_pitch(m.rank) / 2 + tiles * 8 - 1) / (tiles * 8))};
   auto* kernel = tiles == 2 ? low_product_kernel<T, 2, kVec> : tiles == 4 ? low_product_kernel<T, 4, kVec> : low_product_kernel<T, 8, kVec>;
@@ -219,6 +227,7 @@ low_up_kernel(const LowUpParams p) {
   const int r = threadIdx.x;
   if (r >= low_pitch(p.rank) / 2) return;
   float total = 0.f;
+#pragma unroll 8
   for (int w = 0; w < ways; ++w) total += joined[w * vectors + r / 8][r % 8];
   if (r >= p.rank || g == kNoAdapter) total = 0.f;
   else total *= p.scale != nullptr ? __ldg(p.scale + g) : p.scale_all;
@@ -574,10 +583,11 @@ low_join_kernel(const LowJoinParams p) {
 
 // Each row's own adapter read for it alone, from L2 at some 2 TB/s, rather than a pass over 32 rows' k for each adapter among them,
 // whose loads and products follow one another: 0.4 us for 256 of k and 2 us besides.  (288 rows of 1336, rank 32, 8 rows a request: 30 us
-// by passes, now 15.)
-bool low_by_rows(int64_t rows, int rank, int K, const AdapterIndex& index) {
+// by passes, now 15.)  Blocks (`blocks_row` for each row) come in rounds of eight on each multiprocessor (1310 rows of 88, rank 20, 10
+// rows a request: 16 us so, 8 by passes).
+bool low_by_rows(int64_t rows, int rank, int K, const AdapterIndex& index, int blocks_row, int num_sms) {
   const double adapters = index.index == nullptr ? 1 : std::min<double>(index.count, 31 / index.rows_per_index + 1);
-  const double each = 3 + double(rows) * rank * K * 2 / 2e6, passes = 4 + adapters * (2 + 0.4 * K / 256);
+  const double each = 3 + double(rows) * rank * K * 2 / 2e6 + 2.5 * double(rows * blocks_row / (num_sms * 8)), passes = 4 + adapters * (2 + 0.4 * K / 256);
   return rows <= 8192 && each < passes;
 }
 
@@ -591,7 +601,7 @@ int run_low(const LowProduct& m, void* stream) {
   const int64_t tiles = (m.rows + 127) / 128;
   const bool mixed = m.index.index != nullptr && m.index.count > 1 && m.index.rows_per_index < 128;
   const bool small = m.rows <= 512 || (mixed && tiles < st->num_sms) || (m.rank <= 16 && m.rows <= 8192 && m.K * m.planes <= 2048);
-  if (!small && !low_by_rows(m.rows, m.rank, m.K * m.planes, m.index)) return run_matmul_low(m, stream);
+  if (!small && !low_by_dots(m, st->num_sms)) return run_matmul_low(m, stream);
   if (m.f16) return m.aligned ? launch_low<__half, true>(st, m, stream) : launch_low<__half, false>(st, m, stream);
   return m.aligned ? launch_low<__nv_bfloat16, true>(st, m, stream) : launch_low<__nv_bfloat16, false>(st, m, stream);
 }
@@ -678,7 +688,8 @@ int run_low_join(const LowGrads& m, void* stream) {
   auto slabs_of = [](const LowGrad& j) { return j.v == nullptr ? 0 : j.planes * ((j.columns + kGradColumns - 1) / kGradColumns); };
   p.marks = m.marks, p.slabs0 = slabs_of(m.job[0]), p.slabs = p.slabs0 + slabs_of(m.job[1]);
   // several threads to an item where there are many parts of few values
-  const bool sliced = m.parts >= 4 && p.items < int64_t(st->num_sms) * (m.parts >= 8 ? 1024 : 256);
+  // (170000 values of 24 parts: 24 us sliced, 19 otherwise; 46000 of 29: 8 and 10)
+  const bool sliced = m.parts >= 4 && p.items < int64_t(st->num_sms) * 28 * m.parts;
   const int64_t each = sliced ? 32 : 256, blocks = std::min<int64_t>((p.items + each - 1) / each, int64_t(st->num_sms) * 16);
   void (*kernel)(LowJoinParams);
   if (p.items < (int64_t(1) << 31))

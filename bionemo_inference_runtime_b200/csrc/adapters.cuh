@@ -60,7 +60,7 @@ struct LowProduct {
 int run_low(const LowProduct& m, void* stream);
 int run_matmul_low(const LowProduct& m, void* stream);  // of it: on the tensor cores (dense.cu)
 // dz U with U as it lies (for m.x = dz, its N columns as m.K; 16-byte rows), where low_by_rows() says so.
-bool low_by_rows(int64_t rows, int rank, int K, const AdapterIndex& index);
+bool low_by_rows(int64_t rows, int rank, int K, const AdapterIndex& index, int blocks_row, int num_sms);
 int run_low_up(const LowProduct& m, const void* up, int64_t up_pitch, void* stream);
 
 // up [count][columns (two planes of N)][rank] as [count][planes][rank][pitch], for dz U.

@@ -203,8 +203,8 @@ namespace {
 // registers for each column (13 rows, 960 -> 4648 gated: 45 us so, now 8; 16 rows, 4096 -> 4096: 130 and 18; one row the same).
 // Rows that are not 16-byte aligned are shifted into place.
 //
-// With adapters up to 64 rows: single tokens of many requests have as many adapters in a tile, and the tensor cores take them one after
-// the other (64 rows of 2048 -> 4096 with an adapter each, rank 16: 38 us).  Here a value's low-rank sum is its own thread's.  The kernel
+// With adapters also some hundred rows, 64 to a block: single tokens of many requests have as many adapters in a tile, and the tensor cores
+// take them one after the other (64 rows of 2048 -> 4096 with an adapter each, rank 16: 38 us, now 16).  Here a value's low-rank sum is its own thread's.  The kernel
 // of the low-rank values runs beside the products, which do not wait for it; a few of a row or two are made in each block instead (one
 // row, 384 -> 1536 gated, rank 16: one launch, 6 us with its way through the host, where two take 9).
 constexpr int kFewRows = 16, kFewAdapterRows = 64;
@@ -787,7 +787,7 @@ LowPlan plan_low(const BackwardPlan& plan, const AdapterIndex& index, int rank, 
   const int64_t chunk = std::min(plan.chunk, rows), ad = low_grad_columns(K, 1), au = low_grad_columns(N, outer);
   const LowGradShape shape = low_grad_shape(chunk, K, N, outer, count, rank, num_sms);
   p.parts = shape.parts, p.direct = shape.parts == 1 && chunk >= rows;
-  p.by_rows = low_by_rows(chunk, rank, outer * N, index);
+  p.by_rows = low_by_rows(chunk, rank, outer * N, index, 1, num_sms);
   p.bytes = (plan.bytes + 255) / 256 * 256;
   auto take = [&](int64_t bytes) {
     const int64_t at = p.bytes;
@@ -817,11 +817,19 @@ AdapterIndex index_of(const b200ta_adapters* a) {
   return adapter_index(a->index, a->index_bytes, a->rows_per_index, a->count);
 }
 
-// The few rows' kernel with adapters: up to 64 rows of several adapters, and a few times as many if they are single tokens of many
-// requests (230 rows of 3320 -> 704 with 55 adapters: 49 us on the tensor cores, 22 so; 64 rows of 128 -> 512 gated with one: 10 us there).
-bool few_with_adapters(int64_t rows, const AdapterIndex& index) {
-  const int64_t adapters = index.index == nullptr ? 1 : std::min<int64_t>(index.count, (std::min<int64_t>(rows, 128) - 1) / index.rows_per_index + 1);
-  return rows <= kFewRows || (rows <= kFewAdapterRows && adapters >= 4) || (rows <= 4 * kFewAdapterRows && adapters >= 16);
+// The few rows' kernel with adapters, where rows are single tokens of many requests: on the tensor cores each adapter of a tile is an MMA of
+// its own for every 32 ranks (some 0.4 us), here its weights pass through each block's registers once for 64 rows.  Microseconds; a round is two
+// blocks on each multiprocessor.  (320 tokens of 100 adapters, rank 16: 512 -> 512 12 us so and 40 on the tensor cores, 1024 -> 1024 23 and
+// 31, 2048 -> 4096 70 and 50; of 20 adapters 12 and 20, 23 and 18, 70 and 28; 24 tokens of 6 adapters, 512 -> 512, 6 and 11; 64 rows of 128 -> 512
+// with one adapter 9 and 8.)
+bool few_with_adapters(int64_t rows, const AdapterIndex& index, int rank, int K, int64_t columns, int num_sms) {
+  if (rows <= kFewRows) return true;
+  if (rows > 1024) return false;
+  const double adapters = index.index == nullptr ? 1 : double(std::min<int64_t>(index.count, (std::min<int64_t>(rows, 128) - 1) / index.rows_per_index + 1));
+  const double tiles = double((rows + 127) / 128) * double(columns) / (256.0 * num_sms);
+  const double rounds = double((rows + kFewAdapterRows - 1) / kFewAdapterRows) * double((columns + kFewColumns - 1) / kFewColumns) / (2.0 * num_sms);
+  const double here = rows <= 32 ? 4 + std::max(rounds, 1.0) * (0.5 + 0.1 * rank + 0.0025 * K) : 10 + std::max(rounds, 1.0) * (1 + 0.28 * rank + 0.0043 * K);
+  return here < 10 + std::max(tiles, 1.0) * (0.003 * K + 0.42 * adapters * low_blocks(rank));
 }
 int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* residual, int64_t rs, void* y, int64_t ys,
                   void* saved, int64_t ss, int dtype, int activation, int gated, int64_t rows, int K, int N, const LowRank* adapters, const LowProduct* own_low,
@@ -831,10 +839,9 @@ int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const vo
   B200TA_REQUIRE(x && w && y, "dense: NULL pointer");
   B200TA_REQUIRE(!gated || residual == nullptr, "dense: a gated layer has no residual");
   B200TA_REQUIRE(!gated || saved == nullptr || ss % 16 == 0, "dense: the pitch of a gated layer's saved values must be a multiple of 16");
-  if (rows <= kFewRows || (adapters != nullptr && few_with_adapters(rows, adapters->index))) {
-    DeviceState* st = nullptr;
-    rc = get_device_state(&st);
-    if (rc != B200TA_OK) return rc;
+  DeviceState* st = nullptr;
+  if ((rows <= kFewRows || adapters != nullptr) && (rc = get_device_state(&st)) != B200TA_OK) return rc;
+  if (rows <= kFewRows || (adapters != nullptr && few_with_adapters(rows, adapters->index, adapters->rank, K, int64_t(N) * (gated ? 2 : 1), st->num_sms))) {
     const bool f16 = dtype == B200TA_DTYPE_F16;
     FewParams p{x, w, bias, residual, y, saved, xs, ws, rs, ys, ss, int(rows), K, N, activation, {}, nullptr, nullptr, nullptr, 0, 0.f};
     bool vec_down = true;
