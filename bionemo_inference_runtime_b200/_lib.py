@@ -145,6 +145,7 @@ SIGNATURES: dict[str, tuple] = {
          c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int64, c_int, c_int, c_void_p],
     ),
     "b200ta_adapter_low_bytes": (c_size_t, [c_int]),
+    "b200ta_adapter_dense_keeps": (c_int, [c_int, c_int, c_int64, c_int, c_int]),
     "b200ta_adapter_dense_needs_low": (c_int, [c_int64, c_int, c_int]),
     "b200ta_adapter_dense": (
         c_int,

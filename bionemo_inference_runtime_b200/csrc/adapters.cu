@@ -1,5 +1,6 @@
 // The kernels of low-rank adapters beside the tensor-core products: low-rank values, their weights' gradients, small layouts.
 #include <algorithm>
+#include <type_traits>
 
 #include "adapters.cuh"
 #include "layer_norm.cuh"
@@ -71,7 +72,7 @@ low_dot_kernel(const LowProduct p, int groups) {
 // passes; a pass stores the rows that are its own.  Bound by HBM (x once) or L2.
 constexpr int kLowRows = 32;
 __host__ __device__ constexpr int low_warps(int tiles) { return tiles == 8 ? 4 : 8; }
-template <typename T, int kTiles, bool kVec>
+template <typename T, int kTiles, bool kVec, bool kExact>  // kExact: x in two terms
 __global__ void __launch_bounds__(low_warps(kTiles) * 32)
 low_product_kernel(const LowProduct p, int share) {
   constexpr int kWarps = low_warps(kTiles), kRanks = kTiles * 8;
@@ -100,6 +101,7 @@ low_product_kernel(const LowProduct p, int share) {
     float acc[2][kTiles][4] = {};
     for (int plane = 0; plane < p.planes; ++plane) {
       const T *x[2][2], *a[kTiles];
+      const long long second = kExact ? static_cast<const T*>(p.x2) - static_cast<const T*>(p.x) : 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const long long row = row0 + i * 8 + q;
@@ -117,13 +119,24 @@ low_product_kernel(const LowProduct p, int share) {
         for (int i = 0; i < 4; ++i) u[i >> 1][i & 1] = load_eight_of<T, kVec>(x[i >> 1][i & 1], k, p.K);
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) v[j] = load_eight_of<T, kVec>(a[j], k, p.K);
+        auto multiply = [&]() {
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j)
+          for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mma16816<T>(acc[i][j], u[i][0].x, u[i][1].x, u[i][0].y, u[i][1].y, v[j].x, v[j].y);
-            mma16816<T>(acc[i][j], u[i][0].z, u[i][1].z, u[i][0].w, u[i][1].w, v[j].z, v[j].w);
-          }
+            for (int i = 0; i < 2; ++i) {
+              mma16816<T>(acc[i][j], u[i][0].x, u[i][1].x, u[i][0].y, u[i][1].y, v[j].x, v[j].y);
+              mma16816<T>(acc[i][j], u[i][0].z, u[i][1].z, u[i][0].w, u[i][1].w, v[j].z, v[j].w);
+            }
+        };
+        if constexpr (kExact) {
+          uint4 rest[2][2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rest[i >> 1][i & 1] = load_eight_of<T, kVec>(x[i >> 1][i & 1] + second, k, p.K);
+          multiply();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u[i >> 1][i & 1] = rest[i >> 1][i & 1];
+        }
+        multiply();
       }
     }
     if (share) {
@@ -166,6 +179,7 @@ int dot_groups(int rank) { return (low_pitch(rank) / 2 + kDotWarps - 1) / kDotWa
 bool low_by_dots(const LowProduct& m, int num_sms) {
   return low_by_rows(m.rows, m.rank, m.K * m.planes, m.index, dot_groups(m.rank), num_sms);
 }
+// (Of dz with second terms by products alone: run_low_up() takes what low_by_rows() says, which comprises what low_by_dots() would.)
 template <typename T, bool kVec>
 int launch_low(DeviceState* st, const LowProduct& m, void* stream) {
   if (low_by_dots(m, st->num_sms)) {
@@ -180,13 +194,18 @@ int launch_low(DeviceState* st, const LowProduct& m, void* stream) {
   const int warps = low_warps(tiles);
   const int share = groups < int64_t(st->num_sms) * warps * 2 || m.K > 512;
   const dim3 grid{unsigned(share ? groups : (groups + warps - 1) / warps), unsigned((low_pitch(m.rank) / 2 + tiles * 8 - 1) / (tiles * 8))};
-  auto* kernel = tiles == 2 ? low_product_kernel<T, 2, kVec> : tiles == 4 ? low_product_kernel<T, 4, kVec> : low_product_kernel<T, 8, kVec>;
+  auto pick = [&](auto exact) {
+    constexpr bool kExact = decltype(exact)::value;
+    return tiles == 2 ? low_product_kernel<T, 2, kVec, kExact> : tiles == 4 ? low_product_kernel<T, 4, kVec, kExact> : low_product_kernel<T, 8, kVec, kExact>;
+  };
+  // (dz with its second terms is aligned)
+  auto* kernel = kVec && m.x2 != nullptr ? pick(std::integral_constant<bool, kVec>()) : pick(std::false_type());
   return launch_kernel(st, kKernelAdapter, kernel, grid, warps * 32, 0, stream, m, share);
 }
 
 // The same of dz and U as it lies, [columns][rank]: a block for a row, whose threads take eight ranks of every so many columns.
 struct LowUpParams {
-  const void *dz, *up;
+  const void *dz, *dz2, *up;
   void* low;
   const float* scale;
   float scale_all;
@@ -207,10 +226,11 @@ low_up_kernel(const LowUpParams p) {
   if (g != kNoAdapter && way < ways && v * 8 < p.rank) {
     for (int plane = 0; plane < p.planes; ++plane) {
       const T* dz = static_cast<const T*>(p.dz) + row * p.zs + plane * p.z_plane;
+      const T* dz2 = p.dz2 == nullptr ? nullptr : static_cast<const T*>(p.dz2) + row * p.zs + plane * p.z_plane;
       const T* up = static_cast<const T*>(p.up) + (long long)(g * p.planes + plane) * p.N * p.us + v * 8;
 #pragma unroll 8
       for (int n = way; n < p.N; n += ways) {
-        const float d = static_cast<float>(dz[n]);
+        const float d = dz2 == nullptr ? static_cast<float>(dz[n]) : static_cast<float>(dz[n]) + static_cast<float>(dz2[n]);
         const uint4 x = norm::first<T>(__ldg(reinterpret_cast<const uint4*>(up + n * p.us)), p.rank - v * 8);
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -280,11 +300,12 @@ struct GradParams {
   LowGrad job[2];
   AdapterIndex index;
   int rows, rank, rank_groups, slabs0, chunks_part, accumulate, direct;
+  int terms;  // of the second job's tensor: logarithm
   uint8_t* marks;  // of each block
   int* status;
 };
 struct GradMaps {
-  CUtensorMap t[2], v[2];
+  CUtensorMap t[2], v[2], v2;
 };
 __device__ __forceinline__ void ldmatrix4_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -375,7 +396,7 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
     if (lane == 0) listed = n;
   }
   __syncthreads();
-  const int count = listed;
+  const int terms = second ? p.terms : 0, count = listed << terms;
   volatile int* abort_flag = aborted;
   uint8_t* mark = p.direct ? nullptr : p.marks + ((long long)blockIdx.y * gridDim.z + blockIdx.z) * gridDim.x + blockIdx.x;
   if (count == 0 && !p.direct) {
@@ -385,7 +406,7 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
 
   if (warp == kGradWarps) {
     if (lane == 0) {
-      const CUtensorMap *tm_t = &maps.t[second], *tm_v = &maps.v[second];
+      const CUtensorMap *tm_t = &maps.t[second], *tm_first = &maps.v[second];
       bool ok = true;
       int i = 0;
       for (; i < count; ++i) {
@@ -393,7 +414,8 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
         ok = mbar_wait(bar0 + (kStages + s) * 8, (i / kStages & 1) ^ 1, abort_flag);
         if (!ok) break;
         const uint32_t stage = base + s * kStage, bar = bar0 + s * 8;
-        const int row = first_row + list[i] * kGradRows;
+        const int row = first_row + list[i >> terms] * kGradRows;
+        const CUtensorMap* tm_v = i & terms ? &maps.v2 : tm_first;
         mbar_expect_tx(bar, kStage);
         tma_load_3d(stage, tm_v, bar, c0, row, plane);
         tma_load_3d(stage + kGradV / 2, tm_v, bar, c0 + 64, row, plane);
@@ -423,7 +445,7 @@ low_grad_kernel(const GradParams p, const __grid_constant__ GradMaps maps) {
       ok = mbar_wait_warp(bar0 + s * 8, i / kStages & 1, abort_flag);
       if (!ok) break;
       const uint32_t stage = base + s * kStage;
-      const uint32_t bits0 = masks[list[i]][0], bits1 = masks[list[i]][1];
+      const uint32_t bits0 = masks[list[i >> terms]][0], bits1 = masks[list[i >> terms]][1];
       auto walk = [&](auto&& mask) {
 #pragma unroll
         for (int k = 0; k < kGradRows; k += 16) {
@@ -610,7 +632,7 @@ int run_low_up(const LowProduct& m, const void* up, int64_t up_pitch, void* stre
   DeviceState* st = nullptr;
   const int rc = get_device_state(&st);
   if (rc != B200TA_OK) return rc;
-  const LowUpParams p{m.x, up, m.low, m.scale, m.scale_all, m.xs, m.x_plane, up_pitch, m.K, m.planes, m.rank, m.index};
+  const LowUpParams p{m.x, m.x2, up, m.low, m.scale, m.scale_all, m.xs, m.x_plane, up_pitch, m.K, m.planes, m.rank, m.index};
   return launch_kernel(st, kKernelAdapter, m.f16 ? low_up_kernel<__half> : low_up_kernel<__nv_bfloat16>, dim3(unsigned(m.rows)), 256, 0, stream, p);
 }
 
@@ -655,6 +677,7 @@ int run_low_grads(const LowGrads& m, void* stream) {
     const uint32_t box[3] = {64, kGradRows, 1};
     int rc = encode_tensor_map(&maps.v[i], j.v, 2, 3, dims, strides, box, SWZ_128, "adapters");
     if (rc != B200TA_OK) return rc;
+    if (i == 1 && j.v2 != nullptr && (rc = encode_tensor_map(&maps.v2, j.v2, 2, 3, dims, strides, box, SWZ_128, "adapters")) != B200TA_OK) return rc;
     const uint64_t t_dims[3] = {uint64_t(low_pitch(m.rank)), uint64_t(m.rows), 1};
     const uint64_t t_strides[2] = {uint64_t(low_pitch(m.rank)) * 2, uint64_t(low_pitch(m.rank)) * 2};
     const uint32_t t_box[3] = {uint32_t(t_row), kGradRows, 1};
@@ -664,6 +687,7 @@ int run_low_grads(const LowGrads& m, void* stream) {
   auto slabs_of = [](const LowGrad& j) { return j.v == nullptr ? 0 : j.planes * ((j.columns + kGradColumns - 1) / kGradColumns); };
   p.job[0] = m.job[0], p.job[1] = m.job[1], p.index = m.index, p.rows = int(m.rows), p.rank = m.rank, p.rank_groups = (m.rank + 63) / 64;
   p.slabs0 = slabs_of(m.job[0]), p.accumulate = m.accumulate, p.direct = m.direct, p.marks = m.marks, p.status = st->status_dev;
+  p.terms = m.job[1].v2 != nullptr;
   const int64_t chunks = (m.rows + kGradRows - 1) / kGradRows;
   p.chunks_part = int((chunks + m.parts - 1) / m.parts);
   B200TA_REQUIRE(p.chunks_part <= kGradChunks, "adapters: too many rows for %d parts", m.parts);

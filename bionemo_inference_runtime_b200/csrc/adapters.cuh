@@ -49,6 +49,7 @@ struct LowRank {
 // low[row][r] = scale[g] * sum over planes and k of x[row][plane][k] a[g][plane][r][k], in two terms; zeros where there is no adapter.
 struct LowProduct {
   const void *x, *a;
+  const void* x2;  // what the rounding of x left out, laid out alike (up to kExactRows rows), or NULL
   void* low;
   const float* scale;  // of each adapter, on the device, or NULL: scale_all
   float scale_all;
@@ -57,6 +58,7 @@ struct LowProduct {
   bool f16, aligned;  // aligned: 16-byte rows
   AdapterIndex index;
 };
+constexpr int64_t kExactRows = 512;  // (run_low() takes as many without tensor cores)
 int run_low(const LowProduct& m, void* stream);
 int run_matmul_low(const LowProduct& m, void* stream);  // of it: on the tensor cores (dense.cu)
 // dz U with U as it lies (for m.x = dz, its N columns as m.K; 16-byte rows), where low_by_rows() says so.
@@ -70,6 +72,7 @@ int run_transpose_up(const void* up, int64_t up_pitch, void* out, int64_t out_pi
 // 32 bits; then the parts joined, in their order, to [count][rank][columns] or (transposed) [count][columns][rank] in 16 bits.
 struct LowGrad {
   const void *t, *v;  // v NULL: not wanted
+  const void* v2;     // second terms of v, laid out alike, or NULL
   float* part;
   void* out;
   long long v_pitch, v_plane;

@@ -424,8 +424,8 @@ auto pick_few(int rows, bool vec, bool two) {
 // way: part[block.y][column] (+)= theirs, of the values before they are rounded.
 struct SlopeParams {
   const void *dy, *saved;
-  void* dz;
-  float* part;  // or NULL
+  void *dz, *dz2;  // dz2: what the rounding of dz left out, or NULL
+  float* part;     // or NULL
   long long dys, ss, zs, rows, part_pitch;
   int N, rows_block, accumulate;
 };
@@ -446,6 +446,17 @@ __device__ __forceinline__ void store_sums(const float (&s)[8], float (&joined)[
     part[threadIdx.x] = accumulate ? part[threadIdx.x] + sum : sum;
   }
   __syncthreads();
+}
+// What the rounding of eight values to 16 bits leaves out.
+template <typename T>
+__device__ __forceinline__ uint4 rests(const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = unpack2<T>(pack2<T>(v[2 * j], v[2 * j + 1]));
+    w[j] = pack2<T>(second_term(v[2 * j], f.x), second_term(v[2 * j + 1], f.y));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <typename T, int kAct, bool kTwo>
 __global__ void __launch_bounds__(256, kTwo ? 3 : 4)
@@ -494,6 +505,11 @@ slope_kernel(const SlopeParams p) {
       if constexpr (kTwo)
         *reinterpret_cast<uint4*>(dz + p.zs / 2) =
             make_uint4(pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3]), pack2<T>(g[4], g[5]), pack2<T>(g[6], g[7]));
+      if (p.dz2 != nullptr) {
+        T* to = static_cast<T*>(p.dz2) + row * p.zs + c;
+        *reinterpret_cast<uint4*>(to) = rests<T>(v);
+        if constexpr (kTwo) *reinterpret_cast<uint4*>(to + p.zs / 2) = rests<T>(g);
+      }
     }
   }
   if (p.part == nullptr) return;
@@ -779,9 +795,10 @@ struct LowPlan {
   int parts;       // of the rows for the adapters' gradients
   bool direct;     // a single one
   bool by_rows;    // dt from U as it lies
-  int64_t up, low_grad, part[2], marks, bytes;  // offsets: transposed up, dt of a chunk, parts of dD and dU, their marks
+  bool exact;      // dz in two terms for dt and dU
+  int64_t up, low_grad, part[2], marks, dz2, bytes;  // offsets: transposed up, dt of a chunk, parts of dD and dU, their marks, dz's second terms
 };
-LowPlan plan_low(const BackwardPlan& plan, const AdapterIndex& index, int rank, int64_t rows, int K, int N, int outer, int num_sms) {
+LowPlan plan_low(const BackwardPlan& plan, const AdapterIndex& index, bool kept, int rank, int64_t rows, int K, int N, int outer, int num_sms) {
   LowPlan p{};
   const int count = index.count;
   const int64_t chunk = std::min(plan.chunk, rows), ad = low_grad_columns(K, 1), au = low_grad_columns(N, outer);
@@ -799,6 +816,12 @@ LowPlan plan_low(const BackwardPlan& plan, const AdapterIndex& index, int rank, 
   p.part[0] = take(p.direct ? 0 : int64_t(p.parts) * count * rank * ad * 4);
   p.part[1] = take(p.direct ? 0 : int64_t(p.parts) * count * rank * au * 4);
   p.marks = take(p.direct ? 0 : shape.marks);
+  // Of few values of dt, or of dz, each is a large part of dD (dU), whose error would be that of a few roundings of dz (12 tokens of 13
+  // adapters: 0.0027 of dD's size in bf16, where its own rounding is 0.0017, now 0.0017): kept pre-activations give dz's second terms, and
+  // the products of dt and dU take both.  Of many values the roundings average (0.0024), and the second terms' time counts (300 rows,
+  // 2048 -> 2048 gated, rank 64: a training step 115 us, 141 with them).
+  p.exact = kept && rows <= kExactRows && rows * std::min(rank, outer * N) <= 4096;
+  p.dz2 = take(p.exact ? rows * plan.dz_pitch * 2 : 0);
   return p;
 }
 
@@ -888,8 +911,8 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
   const bool kept = reads_kept(saved != nullptr, gated != 0, activation);
   const BackwardPlan& plan = plan_backward(gated, activation != kActNone, kept, dbias != nullptr, rows, K, N, st->num_sms);
   const int64_t outer = gated ? 2 : 1;
-  const LowPlan low_plan = ad != nullptr ? plan_low(plan, index_of(ad), ad->rank, rows, K, N, int(outer), st->num_sms)
-                                            : LowPlan{0, false, false, 0, 0, {0, 0}, 0, plan.bytes};
+  const LowPlan low_plan = ad != nullptr ? plan_low(plan, index_of(ad), kept, ad->rank, rows, K, N, int(outer), st->num_sms)
+                                            : LowPlan{0, false, false, false, 0, 0, {0, 0}, 0, 0, plan.bytes};
   B200TA_REQUIRE(low_plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
                                          workspace_bytes >= size_t(low_plan.bytes)),
                  "dense_backward: the workspace must be 256-byte aligned and of %lld bytes", (long long)low_plan.bytes);
@@ -919,11 +942,12 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
   LowRank with_up{}, with_down{};
   LowGrads low_grads{};
   void* dt = ws_base + low_plan.low_grad;
+  void* dz2 = low_plan.exact ? ws_base + low_plan.dz2 : nullptr;
   if (ad != nullptr) {
     with_up = {index_of(ad), ad->rank, nullptr, ad->up, ad->up_row_stride};
     with_down = {index_of(ad), ad->rank, dt, ad->down, ad->down_row_stride};
-    low_grads.job[0] = {dt, nullptr, reinterpret_cast<float*>(ws_base + low_plan.part[0]), ddown, xs, 0, K, 1, 0};
-    low_grads.job[1] = {nullptr, nullptr, reinterpret_cast<float*>(ws_base + low_plan.part[1]), dup, 0, 0, N, int(outer), 1};
+    low_grads.job[0] = {dt, nullptr, nullptr, reinterpret_cast<float*>(ws_base + low_plan.part[0]), ddown, xs, 0, K, 1, 0};
+    low_grads.job[1] = {nullptr, nullptr, nullptr, reinterpret_cast<float*>(ws_base + low_plan.part[1]), dup, 0, 0, N, int(outer), 1};
     low_grads.rank = ad->rank, low_grads.parts = low_plan.parts, low_grads.f16 = f16;
     low_grads.direct = low_plan.direct, low_grads.marks = reinterpret_cast<uint8_t*>(ws_base + low_plan.marks);
     if ((dx != nullptr || ddown != nullptr) && !low_plan.by_rows) {
@@ -955,7 +979,7 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
         m.bias = bias, m.activation = activation, m.what = "dense_backward dx";
         rc = run_narrow(m, stream);
       } else if (kept) {
-        const SlopeParams p{dy_c, static_cast<const float*>(saved) + r0 * ss, dst, dbias != nullptr && !product_sums ? sums : nullptr, dys, ss, zs, n,
+        const SlopeParams p{dy_c, static_cast<const float*>(saved) + r0 * ss, dst, dz2, dbias != nullptr && !product_sums ? sums : nullptr, dys, ss, zs, n,
                             sum_pitch, N, plan.rows_sum, r0 > 0};
         const dim3 grid{unsigned((N + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
         void (*kernel)(SlopeParams);
@@ -976,7 +1000,7 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
     }
     if (ad != nullptr && (dx != nullptr || ddown != nullptr)) {
       LowProduct q{};
-      q.x = dz, q.a = ws_base + low_plan.up, q.low = dt, q.scale = ad->scale, q.scale_all = ad->scale_all;
+      q.x = dz, q.x2 = dz2, q.a = ws_base + low_plan.up, q.low = dt, q.scale = ad->scale, q.scale_all = ad->scale_all;
       q.xs = zs, q.x_plane = zs / outer, q.as = pad8(N), q.rows = n, q.K = N, q.planes = int(outer), q.rank = ad->rank, q.f16 = f16, q.aligned = true, q.index = with_down.index;
       rc = low_plan.by_rows ? run_low_up(q, ad->up, ad->up_row_stride, stream) : run_low(q, stream);
       if (rc != B200TA_OK) return rc;
@@ -1018,6 +1042,7 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
     if (ddown != nullptr || dup != nullptr) {
       low_grads.job[0].v = ddown != nullptr ? x_c : nullptr;
       low_grads.job[1].v = dup != nullptr ? dz : nullptr;
+      low_grads.job[1].v2 = dup != nullptr ? dz2 : nullptr;
       low_grads.job[1].t = low_c, low_grads.job[1].v_pitch = zs, low_grads.job[1].v_plane = zs / outer;
       low_grads.index = with_down.index, low_grads.rows = n, low_grads.accumulate = r0 > 0;
       if ((rc = run_low_grads(low_grads, stream)) != B200TA_OK) return rc;
@@ -1102,6 +1127,14 @@ int b200ta_adapter_dense(const void* x, int64_t xs, const void* w, int64_t ws, c
   return dense_forward(x, xs, w, ws, bias, residual, rs, y, ys, saved, ss, dtype, activation, gated, rows, K, N, &adapters, own ? &q : nullptr, stream);
 }
 
+int b200ta_adapter_dense_keeps(int activation, int gated, int64_t rows, int K, int N) {
+  // Computed again, values take their adapters' blocks once more; a few million are written and read sooner from K = 1 on, and any number
+  // of them from some 768 on.  A training step with 5 adapters, computed again and kept: 100 rows, 1024 -> 1024, 49 and 40 us; 2000 rows,
+  // 512 -> 1024 gated, 98 and 86; 8000 rows, 128 -> 512 gated, 108 and 99; 60000 rows of it 249 and 298; 30000 rows, 1024 -> 1024, 300
+  // and 283; 512 -> 512 gated 208 and 204.
+  return (gated || activation != b200ta::kActNone) && (K >= 768 || double(rows) * N * (gated ? 2 : 1) <= 16777216.);
+}
+
 int b200ta_adapter_dense_needs_low(int64_t rows, int rank, int K) { return !b200ta::own_low_pays(rows, rank, K); }
 
 size_t b200ta_adapter_low_bytes(int rank) { return rank > 0 && rank <= b200ta::kMaxRank ? size_t(b200ta::low_pitch(rank)) * 2 : 0; }
@@ -1112,7 +1145,7 @@ size_t b200ta_adapter_dense_backward_workspace_bytes(int activation, int gated, 
   if (a == nullptr || rows <= 0 || K <= 0 || N <= 0 || a->count <= 0 || a->rank <= 0 || get_device_state(&st) != B200TA_OK) return 0;
   const BackwardPlan& plan = plan_backward(gated, activation != kActNone, reads_kept(kept != 0, gated != 0, activation), want_dbias != 0, rows, K, N,
                                            st->num_sms);
-  return size_t(plan_low(plan, index_of(a), a->rank, rows, K, N, gated ? 2 : 1, st->num_sms).bytes);
+  return size_t(plan_low(plan, index_of(a), reads_kept(kept != 0, gated != 0, activation), a->rank, rows, K, N, gated ? 2 : 1, st->num_sms).bytes);
 }
 
 int b200ta_adapter_dense_backward(const void* dy, int64_t dys, const void* x, int64_t xs, const void* w, int64_t ws, const void* bias, const void* saved,

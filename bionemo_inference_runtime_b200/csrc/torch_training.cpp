@@ -24,7 +24,7 @@ struct Library {
 #define B200TA_ENTRIES(X)                                                                                                \
   X(layer_norm) X(layer_norm_workspace_bytes) X(layer_norm_backward) X(dense_few_rows) X(dense_keeps) X(dense)              \
   X(dense_backward_workspace_bytes) X(dense_backward) X(copy_rows) X(dropout)      \
-  X(adapter_dense) X(adapter_low_bytes) X(adapter_dense_needs_low) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
+  X(adapter_dense) X(adapter_low_bytes) X(adapter_dense_keeps) X(adapter_dense_needs_low) X(adapter_dense_backward_workspace_bytes) X(adapter_dense_backward)
   B200TA_ENTRIES(B200TA_ENTRY)
 #undef B200TA_ENTRY
 } lib;
@@ -372,7 +372,7 @@ std::tuple<at::Tensor, Maybe, Maybe> adapter_dense(const at::Tensor& x, const at
   const int64_t low_pitch = int64_t(lib.adapter_low_bytes(a.c.rank)) / 2, pitch = pad8(l.N) * (gated ? 2 : 1);
   Maybe low, saved;
   if (want_saved || lib.adapter_dense_needs_low(l.rows, a.c.rank, l.K)) low = empty({l.rows, low_pitch}, x.scalar_type(), x);
-  if (want_saved && lib.dense_keeps(int(activation), gated, l.K)) saved = empty({l.rows, pitch}, at::kFloat, x);
+  if (want_saved && lib.adapter_dense_keeps(int(activation), gated, l.rows, l.K, l.N)) saved = empty({l.rows, pitch}, at::kFloat, x);
   if (l.rows == 0) return {y, low, saved};
   const Rows rx = operand(x, few, copies), rw = operand(w, few, copies), to = result_in(y);
   Rows rr{};

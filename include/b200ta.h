@@ -474,6 +474,8 @@ typedef struct {
   int count, rank;
 } b200ta_adapters;
 size_t b200ta_adapter_low_bytes(int rank);
+/* Whether a training step is faster with `saved` (of few rows its gradients are also more exact with it). */
+int b200ta_adapter_dense_keeps(int activation, int gated, int64_t rows, int K, int N);
 int b200ta_adapter_dense_needs_low(int64_t rows, int rank, int K);
 int b200ta_adapter_dense(const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride, const void* bias, const void* residual,
                          int64_t residual_row_stride, void* y, int64_t y_row_stride, void* saved, int64_t saved_row_stride,

@@ -129,21 +129,23 @@ def check(x, w, bias, residual, down, up, scale, index, gated, dy, activation="n
         near = pre.detach().abs() <= (z_off[:, N:] if gated else z_off)
         jump = near * d.abs() * (value.abs() if gated else 1)
         off = off + (torch.cat([near * d.abs() * z_off[:, N:], jump], 1) if gated else jump)
+    off_low = off  # of dz for the adapters' gradients: in two terms where rows are few
     if activation != "none" or gated:
         off = off + 1.01 * u * dz.abs() + tiny
+        off_low = off_low + 1.01 * u * u * dz.abs() + least if rows <= 512 and rows * min(down.shape[1], dz.shape[1]) <= 4096 else off
     dx, dx_off = dz @ wd, off @ wd.abs() + SUM * (dz.abs() @ wd.abs())
     ddown, ddown_off, dup, dup_off = torch.zeros_like(dd), torch.zeros_like(dd), torch.zeros_like(ud), torch.zeros_like(ud)
     for g, r in enumerate(has):
         s = float(scale[g])
         dt = s * (dz[r] @ ud[g])
         sums = s * (dz[r].abs() @ ud[g].abs())
-        dt_off = s * (off[r] @ ud[g].abs()) + SUM * sums + 1.01 * u * u * dt.abs() + least
+        dt_off = s * (off_low[r] @ ud[g].abs()) + SUM * sums + 1.01 * u * u * dt.abs() + least
         dx[r] += dt @ dd[g]
         dx_off[r] += dt_off @ dd[g].abs() + SUM * (sums @ dd[g].abs())
         ddown[g] = dt.t() @ xd[r]
         ddown_off[g] = dt_off.t() @ xd[r].abs() + SUM * (dt.abs().t() @ xd[r].abs())
         dup[g] = dz[r].t() @ t[r]
-        dup_off[g] = off[r].t() @ (t[r].abs() + t_off[r]) + dz[r].abs().t() @ t_off[r] + SUM * (dz[r].abs().t() @ t[r].abs())
+        dup_off[g] = off_low[r].t() @ (t[r].abs() + t_off[r]) + dz[r].abs().t() @ t_off[r] + SUM * (dz[r].abs().t() @ t[r].abs())
     wanted = [("dx", got[0].view(rows, K), dx, dx_off), ("ddown", got[3], ddown, ddown_off), ("dup", got[4], dup, dup_off)]
     if whole:
         wanted.append(("dweight", got[1], dz.t() @ xd, off.t() @ xd.abs() + SUM * (dz.abs().t() @ xd.abs())))
