@@ -190,7 +190,8 @@ int launch_low(DeviceState* st, const LowProduct& m, void* stream) {
   // All ranks in a block, up to 64, or more blocks of fewer where these leave multiprocessors idle (158 rows of 1448, rank 76, two adapters
   // in turn: 10 us for 30; a gated training step of 300 rows of 2048, rank 64: 115 for 175).
   int tiles = m.rank <= 16 ? 2 : m.rank <= 32 ? 4 : 8;
-  while (tiles > 2 && groups * ((low_pitch(m.rank) / 2 + tiles * 8 - 1) / (tiles * 8)) * 2 <= st->num_sms) tiles /= 2;
+  for (int i = 0; i < 2; ++i)
+    if (tiles > 2 && groups * ((low_pitch(m.rank) / 2 + tiles * 8 - 1) / (tiles * 8)) * 2 <= st->num_sms) tiles /= 2;
   const int warps = low_warps(tiles);
   const int share = groups < int64_t(st->num_sms) * warps * 2 || m.K > 512;
   const dim3 grid{unsigned(share ? groups : (groups + warps - 1) / warps), unsigned((low_pitch(m.rank) / 2 + tiles * 8 - 1) / (tiles * 8))};
