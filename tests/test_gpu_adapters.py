@@ -274,7 +274,8 @@ def test_strides():
 @pytest.mark.parametrize("rows,K,N,count,rank,n", [(3, 64, 40, 2, 8, 3), (40, 64, 40, 3, 16, 40), (200, 72, 136, 2, 12, 4), (521, 64, 40, 1, 20, 1), (1311, 40, 520, 5, 16, 19),
                                                    (9479, 128, 64, 1, 16, 1)])
 @pytest.mark.parametrize("gated", [0, 1])
-def test_nothing_is_written_behind_the_results(rows, K, N, count, rank, n, gated):
+@pytest.mark.parametrize("kept", [0, 1])
+def test_nothing_is_written_behind_the_results(rows, K, N, count, rank, n, gated, kept):
     """Through the C entry points, with canaries behind y, the low-rank values, every gradient and the workspace."""
     index = requests(count, n)
     given = layer(rows, K, N, count, rank, gated=bool(gated), residual=False, bias=False, index=index)
@@ -294,14 +295,17 @@ def test_nothing_is_written_behind_the_results(rows, K, N, count, rank, n, gated
     a = Adapters(down.data_ptr(), up.data_ptr(), down.shape[-1], up.shape[-1], given["scale"].data_ptr(), 1.0, index.data_ptr(), 4, rows // n, count, rank)
     stream = torch.cuda.current_stream().cuda_stream
     sizes = {"y": rows * N * 2, "low": rows * lib.b200ta_adapter_low_bytes(rank), "dx": rows * K * 2, "ddown": count * rank * K * 2, "dup": count * columns * rank * 2}
-    need = lib.b200ta_adapter_dense_backward_workspace_bytes(act, gated, 0, 0, _lib.ctypes.byref(a), rows, K, N)
+    need = lib.b200ta_adapter_dense_backward_workspace_bytes(act, gated, kept, 0, _lib.ctypes.byref(a), rows, K, N)
     sizes["workspace"] = need
+    pitch = (N + 7) // 8 * 8 * (1 + gated)
+    sizes["saved"] = rows // n * n * pitch * 4
     got = {k: held(v) for k, v in sizes.items()}
     x, w, dy = given["x"], given["w"], given["dy"]
     rows = rows // n * n
-    _lib.call("b200ta_adapter_dense", x.data_ptr(), K, w.data_ptr(), K, None, None, 0, got["y"].data_ptr(), N, None, 0, _lib.ctypes.byref(a),
+    saved = got["saved"].data_ptr() if kept else None
+    _lib.call("b200ta_adapter_dense", x.data_ptr(), K, w.data_ptr(), K, None, None, 0, got["y"].data_ptr(), N, saved, pitch, _lib.ctypes.byref(a),
               got["low"].data_ptr(), 0, act, gated, rows, K, N, stream)
-    _lib.call("b200ta_adapter_dense_backward", dy.data_ptr(), N, x.data_ptr(), K, w.data_ptr(), K, None, None, 0, _lib.ctypes.byref(a),
+    _lib.call("b200ta_adapter_dense_backward", dy.data_ptr(), N, x.data_ptr(), K, w.data_ptr(), K, None, saved, pitch, _lib.ctypes.byref(a),
               got["low"].data_ptr(), got["dx"].data_ptr(), K, None, None, got["ddown"].data_ptr(), got["dup"].data_ptr(), got["workspace"].data_ptr(), need, 0,
               act, gated, rows, K, N, stream)
     torch.cuda.synchronize()
