@@ -118,41 +118,43 @@ def check(x, w, bias, residual, down, up, scale, index, gated, dy, activation="n
     within(y.view(rows, N), want, 1.01 * u * want.abs() + off + tiny, "y")
     if not backward:
         return
-    got = back(shaped(dy), shaped(x), *given, activation=activation, saved=saved, want_dweight=whole, want_dbias=whole and bias is not None)
-    d = dy.double()
-    if gated:
-        dz = torch.cat([d * a, d * value * slope], 1)
-        off = torch.cat([1.2 * d.abs() * off_g, 1.02 * d.abs() * (1.2 * off_v + 0.8 * value.abs() * off_g)], 1)
-    else:
-        dz, off = d * slope, 0.8 * d.abs() * z_off
-    if activation == "relu":  # its slope jumps: where the sum may have the other sign, either is right
-        near = pre.detach().abs() <= (z_off[:, N:] if gated else z_off)
-        jump = near * d.abs() * (value.abs() if gated else 1)
-        off = off + (torch.cat([near * d.abs() * z_off[:, N:], jump], 1) if gated else jump)
-    off_low = off  # of dz for the adapters' gradients: in two terms where rows are few
-    if activation != "none" or gated:
-        off = off + 1.01 * u * dz.abs() + tiny
-        off_low = off_low + 1.01 * u * u * dz.abs() + least if rows <= 512 and rows * min(down.shape[1], dz.shape[1]) <= 4096 else off
-    dx, dx_off = dz @ wd, off @ wd.abs() + SUM * (dz.abs() @ wd.abs())
-    ddown, ddown_off, dup, dup_off = torch.zeros_like(dd), torch.zeros_like(dd), torch.zeros_like(ud), torch.zeros_like(ud)
-    for g, r in enumerate(has):
-        s = float(scale[g])
-        dt = s * (dz[r] @ ud[g])
-        sums = s * (dz[r].abs() @ ud[g].abs())
-        dt_off = s * (off_low[r] @ ud[g].abs()) + SUM * sums + 1.01 * u * u * dt.abs() + least
-        dx[r] += dt @ dd[g]
-        dx_off[r] += dt_off @ dd[g].abs() + SUM * (sums @ dd[g].abs())
-        ddown[g] = dt.t() @ xd[r]
-        ddown_off[g] = dt_off.t() @ xd[r].abs() + SUM * (dt.abs().t() @ xd[r].abs())
-        dup[g] = dz[r].t() @ t[r]
-        dup_off[g] = off_low[r].t() @ (t[r].abs() + t_off[r]) + dz[r].abs().t() @ t_off[r] + SUM * (dz[r].abs().t() @ t[r].abs())
-    wanted = [("dx", got[0].view(rows, K), dx, dx_off), ("ddown", got[3], ddown, ddown_off), ("dup", got[4], dup, dup_off)]
-    if whole:
-        wanted.append(("dweight", got[1], dz.t() @ xd, off.t() @ xd.abs() + SUM * (dz.abs().t() @ xd.abs())))
-        if bias is not None:
-            wanted.append(("dbias", got[2], dz.sum(0), off.sum(0) + SUM * dz.abs().sum(0)))
-    for name, have, want, bound in wanted:
-        within(have, want, 1.01 * u * want.abs() + bound + tiny, name)
+    # with the values before the activation kept, where they are, and computed again
+    for kept in (saved,) if saved[1] is None else (saved, (saved[0], None)):
+        got = back(shaped(dy), shaped(x), *given, activation=activation, saved=kept, want_dweight=whole, want_dbias=whole and bias is not None)
+        d = dy.double()
+        if gated:
+            dz = torch.cat([d * a, d * value * slope], 1)
+            off = torch.cat([1.2 * d.abs() * off_g, 1.02 * d.abs() * (1.2 * off_v + 0.8 * value.abs() * off_g)], 1)
+        else:
+            dz, off = d * slope, 0.8 * d.abs() * z_off
+        if activation == "relu":  # its slope jumps: where the sum may have the other sign, either is right
+            near = pre.detach().abs() <= (z_off[:, N:] if gated else z_off)
+            jump = near * d.abs() * (value.abs() if gated else 1)
+            off = off + (torch.cat([near * d.abs() * z_off[:, N:], jump], 1) if gated else jump)
+        off_low = off  # of dz for the adapters' gradients: in two terms where rows are few
+        if activation != "none" or gated:
+            off = off + 1.01 * u * dz.abs() + tiny
+            off_low = off_low + 1.01 * u * u * dz.abs() + least if kept[1] is not None and rows <= 512 and rows * min(down.shape[1], dz.shape[1]) <= 4096 else off
+        dx, dx_off = dz @ wd, off @ wd.abs() + SUM * (dz.abs() @ wd.abs())
+        ddown, ddown_off, dup, dup_off = torch.zeros_like(dd), torch.zeros_like(dd), torch.zeros_like(ud), torch.zeros_like(ud)
+        for g, r in enumerate(has):
+            s = float(scale[g])
+            dt = s * (dz[r] @ ud[g])
+            sums = s * (dz[r].abs() @ ud[g].abs())
+            dt_off = s * (off_low[r] @ ud[g].abs()) + SUM * sums + 1.01 * u * u * dt.abs() + least
+            dx[r] += dt @ dd[g]
+            dx_off[r] += dt_off @ dd[g].abs() + SUM * (sums @ dd[g].abs())
+            ddown[g] = dt.t() @ xd[r]
+            ddown_off[g] = dt_off.t() @ xd[r].abs() + SUM * (dt.abs().t() @ xd[r].abs())
+            dup[g] = dz[r].t() @ t[r]
+            dup_off[g] = off_low[r].t() @ (t[r].abs() + t_off[r]) + dz[r].abs().t() @ t_off[r] + SUM * (dz[r].abs().t() @ t[r].abs())
+        wanted = [("dx", got[0].view(rows, K), dx, dx_off), ("ddown", got[3], ddown, ddown_off), ("dup", got[4], dup, dup_off)]
+        if whole:
+            wanted.append(("dweight", got[1], dz.t() @ xd, off.t() @ xd.abs() + SUM * (dz.abs().t() @ xd.abs())))
+            if bias is not None:
+                wanted.append(("dbias", got[2], dz.sum(0), off.sum(0) + SUM * dz.abs().sum(0)))
+        for name, have, want, bound in wanted:
+            within(have, want, 1.01 * u * want.abs() + bound + tiny, name)
 
 
 # rows around a block's own values (8), the few rows (16, 64), the kernels by 32 rows and the tiles of 128 and 256
@@ -186,7 +188,7 @@ def test_adapters_of_many_requests(n, each, gated):
 @pytest.mark.parametrize("activation", list(ACTS))
 @pytest.mark.parametrize("rows,K", [(6, 64), (50, 64), (150, 64), (150, 1544)])
 def test_activations(rows, K, activation, gated):
-    """Few rows, pre-activations computed again, pre-activations kept."""
+    """Few rows, tiles of rows, few inputs and many."""
     for dtype in (torch.bfloat16, torch.float16):
         check(activation=activation, **layer(rows, K, 72, 3, 16, dtype, gated, True, True, requests(3, rows // 2)))
 
