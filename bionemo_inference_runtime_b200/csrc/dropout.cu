@@ -19,6 +19,7 @@
 
 #include "activation.cuh"
 #include "common.cuh"
+#include "dropout_windows.h"
 
 namespace b200ta {
 namespace {
@@ -184,6 +185,7 @@ dropout_kernel(const DropoutParams p) {
 // bits of 2048 numbered elements of one outer index; a row's whole vectors find their eight (fp32: four) bits at any place, and the
 // elements before and behind them are taken one by one.  `lanes` threads share a row.
 constexpr int kOdd = kThreads * 8;
+static_assert(kOdd == kDropoutBits, "a byte of bits from each thread");
 template <typename T, bool kResidual>
 __global__ void __launch_bounds__(kThreads)
 dropout_rows_kernel(const DropoutParams p, int windows, int lanes) {
@@ -191,9 +193,9 @@ dropout_rows_kernel(const DropoutParams p, int windows, int lanes) {
   __shared__ uint32_t bits[kOdd / 32 + 2];  // (the numbered elements from the last multiple of eight before the window on)
   pdl_trigger();
   pdl_wait();
-  const long long outer = blockIdx.x / unsigned(windows);
-  const int window = int(blockIdx.x % unsigned(windows)) * (kOdd - 8), width = int(p.inner - window < kOdd - 8 ? p.inner - window : kOdd - 8);
-  const long long m0 = outer * p.inner + window;
+  const DropoutWindow window = dropout_window(blockIdx.x, unsigned(windows), p.inner);
+  const int width = window.width;
+  const long long m0 = window.outer * p.inner + window.first;
   reinterpret_cast<uint8_t*>(bits)[threadIdx.x] = uint8_t(keep_bits(m0 / 8 + threadIdx.x, p.sequence, seed_of(p), p.dropped));
   if (threadIdx.x < 2) bits[kOdd / 32 + threadIdx.x] = 0;
   __syncthreads();
@@ -210,7 +212,7 @@ dropout_rows_kernel(const DropoutParams p, int windows, int lanes) {
     int head[kRows];       // elements before its first whole vector
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      row[r] = (outer * p.axis + a + r * step) * p.inner + window;
+      row[r] = (window.outer * p.axis + a + r * step) * p.inner + window.first;
       head[r] = min(int(-row[r] & (kVec - 1)), width);
     }
     for (int v = lane; v * kVec < width; v += lanes) {
@@ -286,12 +288,12 @@ int launch(DeviceState* st, DropoutParams p, void* stream) {
   auto aligned = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
   const bool shared = p.axis > 1, based = aligned(p.x) && aligned(p.residual) && aligned(p.y);
   const bool whole = based && (shared ? p.inner % 8 == 0 : p.dropped < 65536), rows = based && shared && !whole && p.inner >= 16;
-  const int64_t windows = (p.inner + kOdd - 9) / (kOdd - 8);
+  const int64_t windows = dropout_windows(p.inner);
   const int64_t each = !whole ? kOdd : shared ? kThreads * 8 : kThreads * 8 * kUnroll<T>;
   const int64_t blocks = rows ? p.count / p.inner * windows : (p.count + each - 1) / each;
   B200TA_REQUIRE(blocks < (int64_t(1) << 31), "dropout: too many elements");
   int lanes = 4;  // as many threads as take a row's window at a time
-  while (lanes < kThreads && lanes * (16 / int(sizeof(T))) < std::min<int64_t>(p.inner, kOdd - 8)) lanes *= 2;
+  while (lanes < kThreads && lanes * (16 / int(sizeof(T))) < std::min<int64_t>(p.inner, kDropoutWindow)) lanes *= 2;
   // Two waves of eight blocks on each multiprocessor, as long as a thread has several entries of the axis.
   const int64_t wanted = std::max<int64_t>((int64_t(st->num_sms) * 16 + blocks - 1) / blocks, 1);
   p.chunk = std::max<int64_t>((p.axis + wanted - 1) / wanted, std::min<int64_t>(p.axis, rows ? 4 * (kThreads / lanes) : kUnroll<T>));
