@@ -915,6 +915,7 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         const bool in = row + lane < p.rows_inner;
         const int g = in ? adapter_of(x.index, uint32_t(row + lane)) : kNoAdapter;
         const float scale = g == kNoAdapter ? 0.f : x.scale != nullptr ? __ldg(x.scale + g) : x.scale_all;
+        const int ranks = g == kNoAdapter ? 0 : x.rank;
         if (first_g * 16 >= p.tile_n) release(i);
         for (int r = first_g * 16; r < p.tile_n; r += step_g * 16) {
           float v[16];
@@ -925,8 +926,9 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           uint32_t first[8], second[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            // (lanes without an adapter hold whatever was there)
-            const float v0 = g == kNoAdapter ? 0.f : v[2 * j] * scale, v1 = g == kNoAdapter ? 0.f : v[2 * j + 1] * scale;
+            // (Lanes without an adapter hold whatever was there, and columns behind the last rank NaN where the row has an infinity,
+            // which would reach the row's results through the zeros behind U's last rank.)
+            const float v0 = r + 2 * j < ranks ? v[2 * j] * scale : 0.f, v1 = r + 2 * j + 1 < ranks ? v[2 * j + 1] * scale : 0.f;
             first[j] = pack2<T>(v0, v1);
             const float2 f = unpack2<T>(first[j]);
             second[j] = pack2<T>(second_term(v0, f.x), second_term(v1, f.y));
