@@ -1,0 +1,62 @@
+"""Adapters' gradients in fp16 within what is rounded, and many more adapters than tiles.
+
+The bounds of the adapters' tests add the smallest normal number to each value that is rounded, 2^-14 in fp16, several times a rounding of
+gradients around 0.1.  Here gradients are 512 times as large (a power of two: they keep their bits), so that it is below a tenth of the
+roundings of most of them."""
+
+import pytest
+import torch
+
+from bionemo_inference_runtime_b200 import _lib, ops
+from tests.test_gpu_adapters import check, layer, requests
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def _no_wait_ran_out():
+    _lib.reset_device_status()
+    yield
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("gated", [False, True], ids=["dense", "gated"])
+@pytest.mark.parametrize("activation", ["none", "relu", "silu", "gelu", "gelu_tanh", "sigmoid"])
+@pytest.mark.parametrize("n,each,K,N,rank", [(6, 1, 64, 72, 16), (50, 1, 64, 72, 12), (30, 5, 200, 72, 20), (3, 300, 136, 96, 16), (3, 300, 520, 40, 40),
+                                             (4, 2500, 72, 64, 16)])
+def test_fp16_gradients_within_their_roundings(n, each, K, N, rank, activation, gated):
+    given = layer(n * each, K, N, 3, rank, torch.float16, gated, True, True, requests(3, n))
+    given["dy"] = given["dy"] * 512
+    check(activation=activation, **given)
+
+
+@pytest.mark.parametrize("rows,count", [(50, 16383), (3000, 5000), (10000, 2000)])
+@pytest.mark.parametrize("gated", [False, True], ids=["dense", "gated"])
+def test_thousands_of_adapters(rows, count, gated):
+    """Each row its own adapter, from anywhere among them: relative to the size of each result, in bf16 with at most three roundings on the
+    way (2^-9 each in the root mean square).  The last adapter and the one behind it are asked for as well; adapters without rows
+    have gradients of zero."""
+    K, N, rank = 40, 24, 6
+    g = torch.Generator(device=DEV).manual_seed(1)
+    index = torch.randint(0, count, (rows,), generator=g, device=DEV)
+    index[0], index[1], index[2] = count - 1, count, -1
+    p = layer(rows, K, N, count, rank, gated=gated, residual=False, index=index)
+    forward, back = (ops.adapter_gated_dense, ops.adapter_gated_dense_backward) if gated else (ops.adapter_dense, ops.adapter_dense_backward)
+    args = (p["w"], p["bias"], p["down"], p["up"], index, p["scale"])
+    y, saved = forward(p["x"], *args, activation="silu", want_saved=True)
+    dx, _, _, ddown, dup = back(p["dy"], p["x"], *args, activation="silu", saved=saved)
+
+    x, w, b, down, up = (p[k].double().requires_grad_(True) for k in ("x", "w", "bias", "down", "up"))
+    has = index.clamp(0, count - 1)
+    share = (p["scale"].double()[has] * ((index >= 0) & (index < count))).unsqueeze(1)
+    t = share * torch.einsum("rk,rjk->rj", x, down[has])
+    z = x @ w.t() + b + torch.einsum("rj,rnj->rn", t, up[has])
+    want = z[:, :N] * torch.nn.functional.silu(z[:, N:]) if gated else torch.nn.functional.silu(z)
+    grads = torch.autograd.grad(want, (x, down, up), p["dy"].double())
+    for name, got, ref in zip(("y", "dx", "ddown", "dup"), (y, dx, ddown, dup), (want.detach(), *grads), strict=True):
+        assert torch.isfinite(got).all() and ((got.double() - ref).norm() / ref.norm()).item() < 3 * 2 ** -9, name
+    idle = torch.ones(count, dtype=torch.bool, device=DEV)
+    idle[index[(index >= 0) & (index < count)]] = False
+    assert idle.any() and not ddown[idle].any() and not dup[idle].any()
