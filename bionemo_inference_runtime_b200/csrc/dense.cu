@@ -207,6 +207,8 @@ namespace {
 // take them one after the other (64 rows of 2048 -> 4096 with an adapter each, rank 16: 38 us, now 16).  Here a value's low-rank sum is its own thread's.  The kernel
 // of the low-rank values runs beside the products, which do not wait for it; a few of a row or two are made in each block instead (one
 // row, 384 -> 1536 gated, rank 16: one launch, 6 us with its way through the host, where two take 9).
+// Without adapters the kernel is one of its own: their branches would take the aligned form from 48 registers a thread to 72 (up to 16 rows
+// from 64), and a multiprocessor from five blocks to three (one row, 8192 -> 28672: 104 us, with them 139; 4096 -> 16384: 43 and 55).
 constexpr int kFewRows = 16, kFewAdapterRows = 64;
 constexpr int kOwnLow = 64, kOwnLowReads = 32768;  // values that a block makes itself, and elements of the adapters it reads for them
 
@@ -215,7 +217,7 @@ struct FewParams {
   void *y, *saved;
   long long xs, ws, rs, ys, ss;
   int rows, K, N, activation;
-  LowRank adapters;  // without `high`: none
+  LowRank adapters;  // (of the form with adapters)
   // Without `low` each block makes the low-rank values itself, and the first one writes them to low_out (may be NULL).
   const void* down;
   const float* scale;
@@ -289,15 +291,15 @@ __device__ __forceinline__ float low_sum(const T* low, const float* own, const T
   return sum;
 }
 
-template <typename T, bool kTwo, int kEights, bool kVec>
+template <typename T, bool kTwo, int kEights, bool kVec, bool kAdapt>
 __global__ void __launch_bounds__(few_warps(kEights, kTwo ? 2 : 1) * 32, kEights > 2 && few_warps(kEights, kTwo ? 2 : 1) <= 8 ? 2 : 1)
 few_rows_kernel(const FewParams p) {
   __shared__ float joined[few_warps(kEights, kTwo ? 2 : 1)][kTwo ? 2 : 1][kEights * 8][kFewColumns + 1];
-  __shared__ float own_low[kOwnLow];
+  __shared__ float own_low[kAdapt ? kOwnLow : 1];
   pdl_trigger();
-  if (p.adapters.low == nullptr) pdl_wait();  // (otherwise what came before the kernel of the low-rank values is complete)
+  if (!kAdapt || p.adapters.low == nullptr) pdl_wait();  // (otherwise what came before the kernel of the low-rank values is complete)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, n0 = blockIdx.x * kFewColumns, warps = blockDim.x >> 5;
-  const int row0 = blockIdx.y * kFewAdapterRows, rows = min(p.rows - row0, kFewAdapterRows);
+  const int row0 = kAdapt ? blockIdx.y * kFewAdapterRows : 0, rows = kAdapt ? min(p.rows - row0, kFewAdapterRows) : p.rows;
   constexpr int kParts = kTwo ? 2 : 1;
   const T *w[kParts][2], *x[kEights];
 #pragma unroll
@@ -308,7 +310,7 @@ few_rows_kernel(const FewParams p) {
   }
 #pragma unroll
   for (int e = 0; e < kEights; ++e) x[e] = static_cast<const T*>(p.x) + (row0 + min(g + 8 * e, rows - 1)) * p.xs;
-  if (p.down != nullptr) {  // a warp for each low-rank value
+  if (kAdapt && p.down != nullptr) {  // a warp for each low-rank value
     const int rank = p.adapters.rank;
     for (int i = warp; i < p.rows * rank; i += warps) {
       const int row = i / rank, r = i - row * rank, a = adapter_of(p.adapters.index, uint32_t(row));
@@ -358,8 +360,8 @@ few_rows_kernel(const FewParams p) {
       for (int j = 0; j < 4; ++j) joined[warp][i][e * 8 + t * 2 + (j & 1)][g + 8 * (j >> 1)] = acc[i][e][j];
   __syncthreads();
   const int c = threadIdx.x % kFewColumns, n = n0 + c;
-  if (p.adapters.low != nullptr) pdl_wait();
-  if (p.low_out != nullptr && blockIdx.x == 0) {  // as the backward pass reads them, zeros behind the last rank included
+  if (kAdapt && p.adapters.low != nullptr) pdl_wait();
+  if (kAdapt && p.low_out != nullptr && blockIdx.x == 0) {  // as the backward pass reads them, zeros behind the last rank included
     const int half = low_pitch(p.adapters.rank) / 2;
     for (int i = threadIdx.x; i < p.rows * half; i += blockDim.x) {
       const int row = i / half, r = i - row * half;
@@ -376,7 +378,7 @@ few_rows_kernel(const FewParams p) {
       v += joined[i][0][own][c];
       if constexpr (kTwo) gate += joined[i][1][own][c];
     }
-    if (p.adapters.high != nullptr) {
+    if constexpr (kAdapt) {
       const int a = adapter_of(p.adapters.index, uint32_t(row));
       if (a != kNoAdapter) {
         const T* high = static_cast<const T*>(p.adapters.high) + ((long long)a * (kTwo ? 2 * p.N : p.N) + n) * p.adapters.high_pitch;
@@ -401,20 +403,25 @@ few_rows_kernel(const FewParams p) {
     if (kTwo) a *= v;
     if (p.residual != nullptr) a += static_cast<float>(static_cast<const T*>(p.residual)[row * p.rs + n]);
     static_cast<T*>(p.y)[row * p.ys + n] = static_cast<T>(a);
+    if (!kAdapt) break;  // (as many threads as values)
   }
 }
 
-template <typename T, bool kTwo, int kEights>
+template <typename T, bool kTwo, int kEights, bool kAdapt>
 auto pick_few(bool vec) {
-  return vec ? &few_rows_kernel<T, kTwo, kEights, true> : &few_rows_kernel<T, kTwo, kEights, false>;
+  return vec ? &few_rows_kernel<T, kTwo, kEights, true, kAdapt> : &few_rows_kernel<T, kTwo, kEights, false, kAdapt>;
 }
 template <typename T, bool kTwo>
-auto pick_few(int rows, bool vec) {
-  return rows <= 8 ? pick_few<T, kTwo, 1>(vec) : rows <= 16 ? pick_few<T, kTwo, 2>(vec) : rows <= 32 ? pick_few<T, kTwo, 4>(vec) : pick_few<T, kTwo, 8>(vec);
+auto pick_few(int rows, bool vec, bool adapt) {
+  if (!adapt) return rows <= 8 ? pick_few<T, kTwo, 1, false>(vec) : pick_few<T, kTwo, 2, false>(vec);
+  return rows <= 8    ? pick_few<T, kTwo, 1, true>(vec)
+         : rows <= 16 ? pick_few<T, kTwo, 2, true>(vec)
+         : rows <= 32 ? pick_few<T, kTwo, 4, true>(vec)
+                      : pick_few<T, kTwo, 8, true>(vec);
 }
 template <typename T>
-auto pick_few(int rows, bool vec, bool two) {
-  return two ? pick_few<T, true>(rows, vec) : pick_few<T, false>(rows, vec);
+auto pick_few(int rows, bool vec, bool two, bool adapt) {
+  return two ? pick_few<T, true>(rows, vec, adapt) : pick_few<T, false>(rows, vec, adapt);
 }
 
 // ---- dz from stored pre-activations ---------------------------------------------------------------------------------
@@ -877,7 +884,8 @@ int dense_forward(const void* x, int64_t xs, const void* w, int64_t ws, const vo
     // sixteen warps where blocks are few (three rows, 1536 -> 384: 9 us instead of 11), eight otherwise, of which more blocks fit
     const int eights = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 8, blocks = (N + kFewColumns - 1) / kFewColumns;
     const int warps = std::min(few_warps(eights, gated ? 2 : 1), blocks <= st->num_sms ? 16 : 8), row_blocks = int((rows + kFewAdapterRows - 1) / kFewAdapterRows);
-    return launch_kernel(st, kKernelDenseHelpers, f16 ? pick_few<__half>(int(rows), vec, gated) : pick_few<__nv_bfloat16>(int(rows), vec, gated),
+    const bool adapt = adapters != nullptr;
+    return launch_kernel(st, kKernelDenseHelpers, f16 ? pick_few<__half>(int(rows), vec, gated, adapt) : pick_few<__nv_bfloat16>(int(rows), vec, gated, adapt),
                          dim3(unsigned(blocks), unsigned(row_blocks)), warps * 32, 0, stream, p);
   }
   B200TA_REQUIRE(rows_aligned(x, xs) && rows_aligned(w, ws) && (!residual || rows_aligned(residual, rs)) &&
