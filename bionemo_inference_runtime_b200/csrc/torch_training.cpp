@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include "../../include/b200ta.h"
@@ -436,15 +437,20 @@ std::tuple<Maybe, Maybe, Maybe, Maybe, Maybe> adapter_dense_backward(const at::T
   return {dx, dweight, dbias, ddown, dup};
 }
 
-// Whether a leaf among these tensors has a node that accumulates its gradients on the default stream, which an eager graph of the leaf
-// that is alive keeps: a backward pass that is being captured cannot reach that stream, and PyTorch would end the capture with an error
-// that names neither.
-bool accumulated_elsewhere(const std::vector<Maybe>& tensors) {
-  for (const Maybe& t : tensors) {
-    if (!t || !t->is_cuda() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+// Whether a leaf among these has a node that accumulates its gradients on the default stream, which an eager graph of the leaf that is
+// alive keeps, and the backward pass that is running sends a gradient there: being captured, it cannot reach that stream, and PyTorch
+// would end the capture with an error that names neither.
+bool accumulated_elsewhere(const std::vector<at::Tensor>& leaves) {
+  const auto* running = torch::autograd::get_current_graph_task_exec_info();  // (empty: all nodes take part)
+  for (const at::Tensor& t : leaves) {
+    if (!t.is_cuda()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (node && running != nullptr && !running->empty()) {
+      const auto part = running->find(node.get());
+      if (part == running->end() || !part->second.should_execute()) continue;
+    }
     const auto on = node ? node->stream() : std::nullopt;
-    if (on && *on == c10::cuda::getDefaultCUDAStream(t->device().index()).unwrap()) return true;
+    if (on && *on == c10::cuda::getDefaultCUDAStream(t.device().index()).unwrap()) return true;
   }
   return false;
 }

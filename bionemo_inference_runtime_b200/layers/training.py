@@ -21,6 +21,15 @@ from .. import ops
 from .transition import _row_mask
 
 
+def _refuse_capture(ctx, dy: torch.Tensor) -> None:
+    """Refuses, by name, a captured backward pass whose gradients go to leaves that an eager graph holds on the default stream."""
+    if dy.is_cuda and torch.cuda.is_current_stream_capturing():
+        leaves = [f.variable for f, _ in ctx.next_functions if f is not None and f.name() == "torch::autograd::AccumulateGrad"]
+        if ops._host.accumulated_elsewhere(leaves):
+            raise RuntimeError("a backward pass is captured into a graph while an eager graph of the same leaves is alive, whose gradients are "
+                               "accumulated on the default stream: release that graph first")
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -31,6 +40,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _refuse_capture(ctx, dy)
         x, stats, weight = ctx.saved_tensors
         wanted = ctx.needs_input_grad
         dx, dweight, dbias = ops.layer_norm_backward(dy, x, stats, weight, want_dx=wanted[0], want_dweight=wanted[1],
@@ -51,6 +61,7 @@ class _Dense(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _refuse_capture(ctx, dy)
         x, weight, bias, saved = ctx.saved_tensors
         wanted = ctx.needs_input_grad
         grads = (None, None, None)
@@ -71,17 +82,12 @@ class _GatedDense(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _refuse_capture(ctx, dy)
         x, weight, bias, saved = ctx.saved_tensors
         wanted = ctx.needs_input_grad
         grads = ops.gated_dense_backward(dy, x, weight, bias, activation=ctx.activation, saved=saved, want_dx=wanted[0],
                                          want_dweight=wanted[1], want_dbias=wanted[2])
         return (*grads, None)
-
-
-def _refuse_capture(*inputs: torch.Tensor | None) -> None:
-    if torch.cuda.is_current_stream_capturing() and ops._host.accumulated_elsewhere(inputs):
-        raise RuntimeError("a backward pass is captured into a graph while an eager graph of the same leaves is alive, whose gradients are "
-                           "accumulated on the default stream: release that graph first")
 
 
 class _AdapterDense(torch.autograd.Function):
@@ -100,8 +106,8 @@ class _AdapterDense(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _refuse_capture(ctx, dy)
         x, weight, bias, down, up, index, scale, *saved = ctx.saved_tensors
-        _refuse_capture(x, weight, bias, down, up)
         wanted = ctx.needs_input_grad
         grads = (None,) * 5
         if any(wanted[:5]):
@@ -123,6 +129,7 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _refuse_capture(ctx, dy)
         dx = ops.dropout_backward(dy, *ctx.given, shared=ctx.shared) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
 
