@@ -465,7 +465,7 @@ __device__ __forceinline__ uint4 rests(const float (&v)[8]) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-template <typename T, int kAct, bool kTwo>
+template <typename T, int kAct, bool kTwo, bool kRests>  // kRests: dz2 is wanted
 __global__ void __launch_bounds__(256, kTwo ? 3 : 4)
 slope_kernel(const SlopeParams p) {
   __shared__ float joined[8][256 + 4];
@@ -512,7 +512,7 @@ slope_kernel(const SlopeParams p) {
       if constexpr (kTwo)
         *reinterpret_cast<uint4*>(dz + p.zs / 2) =
             make_uint4(pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3]), pack2<T>(g[4], g[5]), pack2<T>(g[6], g[7]));
-      if (p.dz2 != nullptr) {
+      if constexpr (kRests) {
         T* to = static_cast<T*>(p.dz2) + row * p.zs + c;
         *reinterpret_cast<uint4*>(to) = rests<T>(v);
         if constexpr (kTwo) *reinterpret_cast<uint4*>(to + p.zs / 2) = rests<T>(g);
@@ -525,16 +525,21 @@ slope_kernel(const SlopeParams p) {
   store_sums(sv, joined, part, columns, p.accumulate);
   if constexpr (kTwo) store_sums(sg, joined, part + p.zs / 2, columns, p.accumulate);
 }
-template <typename T, bool kTwo>
+template <typename T, bool kTwo, bool kRests>
 auto pick_slope(int activation) {
   switch (activation) {
-    case kActNone: return &slope_kernel<T, kActNone, kTwo>;
-    case kActRelu: return &slope_kernel<T, kActRelu, kTwo>;
-    case kActSilu: return &slope_kernel<T, kActSilu, kTwo>;
-    case kActGelu: return &slope_kernel<T, kActGelu, kTwo>;
-    case kActGeluTanh: return &slope_kernel<T, kActGeluTanh, kTwo>;
-    default: return &slope_kernel<T, kActSigmoid, kTwo>;
+    case kActNone: return &slope_kernel<T, kActNone, kTwo, kRests>;
+    case kActRelu: return &slope_kernel<T, kActRelu, kTwo, kRests>;
+    case kActSilu: return &slope_kernel<T, kActSilu, kTwo, kRests>;
+    case kActGelu: return &slope_kernel<T, kActGelu, kTwo, kRests>;
+    case kActGeluTanh: return &slope_kernel<T, kActGeluTanh, kTwo, kRests>;
+    default: return &slope_kernel<T, kActSigmoid, kTwo, kRests>;
   }
+}
+template <typename T>
+auto pick_slope(int activation, bool two, bool rests) {
+  if (two) return rests ? pick_slope<T, true, true>(activation) : pick_slope<T, true, false>(activation);
+  return rests ? pick_slope<T, false, true>(activation) : pick_slope<T, false, false>(activation);
 }
 
 // ---- sums over rows -------------------------------------------------------------------------------------------------
@@ -991,8 +996,8 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
                             sum_pitch, N, plan.rows_sum, r0 > 0};
         const dim3 grid{unsigned((N + 255) / 256), unsigned((n + plan.rows_sum - 1) / plan.rows_sum)};
         void (*kernel)(SlopeParams);
-        if (f16) kernel = gated ? pick_slope<__half, true>(activation) : pick_slope<__half, false>(activation);
-        else kernel = gated ? pick_slope<__nv_bfloat16, true>(activation) : pick_slope<__nv_bfloat16, false>(activation);
+        if (f16) kernel = pick_slope<__half>(activation, gated, dz2 != nullptr);
+        else kernel = pick_slope<__nv_bfloat16>(activation, gated, dz2 != nullptr);
         rc = launch_kernel(st, kKernelDenseHelpers, kernel, grid, 256, 0, stream, p);
       } else {
         Matmul m;
