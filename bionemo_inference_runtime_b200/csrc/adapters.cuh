@@ -27,6 +27,11 @@ inline AdapterIndex adapter_index(const void* index, int bytes, int64_t rows_per
   // 2^(31 + s) / d, rounded up: what is added to it, times n, stays below 2^(31 + s)
   return {index, bytes, uint32_t(d), 0, uint32_t(((uint64_t(1) << (31 + s)) + d - 1) / d), 31 + s, count};
 }
+// Adapters that a tile of `tile` of `rows` rows is expected to have: of the entries of its index, one each.
+inline int64_t adapters_of_tile(const AdapterIndex& x, int64_t rows, int tile) {
+  const int64_t entries = x.index == nullptr ? 1 : ((rows < tile ? rows : tile) - 1) / x.rows_per_index + 1;
+  return entries < x.count ? entries : x.count;
+}
 constexpr int kNoAdapter = 0x7FFFFFFF;
 constexpr int kMaxRank = 256;
 // How low-rank values lie: a row has blocks of 16 or 32 ranks, of each its first and then its second terms (64 or 128 bytes: a tensor

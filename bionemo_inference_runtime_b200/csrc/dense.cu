@@ -32,13 +32,12 @@ struct TilingOf {
   bool a_mn, sums;  // sums of A over k: tiles of up to 128 columns
   int64_t rows, outer, columns;
   int kblocks, splits;
-  double more = 0;  // blocks along k that adapters add to a tile
+  double more = 0, more_pair = 0;  // blocks along k that adapters add to a tile of 128 rows, to one of 256
   bool held = false;  // whether they may have room of their own
 };
 Tiling choose_tiling(const TilingOf& m, int num_sms) {
   const bool two = m.form == kGated || m.form == kGatedGrad;
   const int64_t accumulated = two ? m.columns * 2 : m.columns;
-  const double kblocks = m.kblocks + m.more;
   const double finish = m.form == kGatedGrad ? 12 : two ? 8 : 6.5;  // clocks for an accumulator column of 128 rows
   Tiling best{128, 0, 0, 1e300};
   auto consider = [&](int n, int pair, int resident, double waves, double main) {
@@ -51,25 +50,23 @@ Tiling choose_tiling(const TilingOf& m, int num_sms) {
     if (n > 64 && n / 2 >= accumulated) continue;
     const int64_t tiles_n = (accumulated + n - 1) / n;
     const double mma = 4.0 * std::max(40.0, n * 0.54);
-    if (!m.a_mn && m.splits == 1 && (m.more == 0 || m.held) && m.kblocks * n * matmul::kBK * 2 <= matmul::kResidentBytes && tiles_n <= num_sms) {
+    const bool keeps = !m.a_mn && m.splits == 1 && (m.more == 0 || m.held) && m.kblocks * n * matmul::kBK * 2 <= matmul::kResidentBytes && tiles_n <= num_sms;
+    if (keeps) {
       const int64_t lanes = std::min(tiles_m, num_sms / tiles_n);
-      consider(n, 0, int(lanes), waves_of(tiles_m, lanes), m.kblocks * std::max(mma, 356.0) + m.more * 400);
-    } else {
+      // (a first adapter 400 clocks, each further one of a tile 800: its U arrives when the one before it is done with)
+      consider(n, 0, int(lanes), waves_of(tiles_m, lanes), m.kblocks * std::max(mma, 356.0) + (m.more > 0 ? m.more * 800 - 400 : 0));
+    }
+    if (!keeps || m.more > 0) {  // (many adapters: 20000 tokens of 100, 128 -> 512 gated, 387 us held, 268 through the ring)
       const double load = (n == 256 ? 1.2 : 1.0) * (16384 + n * 128) / 46;
-      consider(n, 0, 0, waves_of(tiles_m * tiles_n * m.splits, num_sms), kblocks * std::max(mma, load));
+      consider(n, 0, 0, waves_of(tiles_m * tiles_n * m.splits, num_sms), (m.kblocks + m.more) * std::max(mma, load));
     }
   }
   for (int n = 256; n >= 128 && m.rows > matmul::kBM && !m.sums; n /= 2) {
     if (n / 2 >= accumulated) continue;
     const int64_t tiles = (m.rows + 255) / 256 * m.outer * m.splits * ((accumulated + n - 1) / n);
-    consider(n, 1, 0, waves_of(tiles, num_sms / 2), kblocks * std::max(4.0 * n * 0.54, (16384 + n * 64) / 46.0));
+    consider(n, 1, 0, waves_of(tiles, num_sms / 2), (m.kblocks + m.more_pair) * std::max(4.0 * n * 0.54, (16384 + n * 64) / 46.0));
   }
   return best;
-}
-
-// Adapters that a tile of 128 rows is expected to have.
-double low_requests(const LowRank& a) {
-  return double(std::min<int64_t>(a.index.count, a.index.index == nullptr ? 1 : 127 / int64_t(a.index.rows_per_index) + 1));
 }
 
 }  // namespace
@@ -89,10 +86,14 @@ int run_matmul(const Matmul& m, void* stream) {
   p.kblocks_split = m.kblocks_split > 0 && m.kblocks_split < p.kblocks ? m.kblocks_split : p.kblocks;
   p.splits = (p.kblocks + p.kblocks_split - 1) / p.kblocks_split;
   p.rows_inner = int(rows), p.columns = int(columns);
-  const Tiling tiling =
-      choose_tiling({m.form, m.a_mn, m.sums != nullptr, rows, m_outer, columns, p.kblocks_split, p.splits, m.adapters == nullptr ? 0 : low_requests(*m.adapters) * low_blocks(m.adapters->rank),
-                     m.adapters != nullptr && low_blocks(m.adapters->rank) == 1},
-                    st->num_sms);
+  TilingOf tiles{m.form, m.a_mn, m.sums != nullptr, rows, m_outer, columns, p.kblocks_split, p.splits};
+  if (m.adapters != nullptr) {
+    const int blocks = low_blocks(m.adapters->rank);
+    tiles.more = double(adapters_of_tile(m.adapters->index, rows, matmul::kBM) * blocks);
+    tiles.more_pair = double(adapters_of_tile(m.adapters->index, rows, 2 * matmul::kBM) * blocks);
+    tiles.held = blocks == 1;
+  }
+  const Tiling tiling = choose_tiling(tiles, st->num_sms);
   p.tile_n = tiling.tile_n, p.pair = tiling.pair, p.resident = tiling.resident;
   const int tile_m = p.pair ? 2 * matmul::kBM : matmul::kBM;
   p.tiles_m_inner = int((rows + tile_m - 1) / tile_m);
