@@ -706,117 +706,114 @@ matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               walk_k([&](uint64_t da, uint64_t db, uint32_t add) { umma_ss_lanes_warp(acc, da, db, id, off, add); });
             }
           }
-          if (!ok) break;
-          umma_commit_warp(bars + (ACC_FULL + buffer) * 8);
-          ahead.look(p, x, i + 1, items, units);
-          continue;
-        }
-        for (int kb = t.kb0; ok && kb < t.kb1; ++kb) {
-          ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t sa = ring + stage * stage_bytes, sb = p.resident ? base + kb * b_bytes : sa + kABytes;
-          // K-major: rows of 128 bytes, groups of 8 rows 1 KiB apart, a step of 16 k is 32 bytes.  MN-major: rows (k) of 64
-          // elements, blocks of 64 elements 8 KiB apart, a step of 16 k is 2 KiB.
-          const uint64_t da = kAMn ? smem_desc<8192, 1024, kLayoutSw128>(sa) : smem_desc<16, 1024, kLayoutSw128>(sa);
-          const uint64_t db = kBMn ? smem_desc<8192, 1024, kLayoutSw128>(sb) : smem_desc<16, 1024, kLayoutSw128>(sb);
-#pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) {
-            const uint64_t dak = da + k * (kAMn ? 128 : 2), dbk = db + k * (kBMn ? 128 : 2);
-            const uint32_t add = (kb > t.kb0 || k > 0) ? 1u : 0u;
-            if constexpr (kPair) umma_ss_pair_warp(acc, dak, dbk, id, add);
-            else umma_ss_warp(acc, dak, dbk, id, add);
-          }
-          if (kSums && p.sums != nullptr && t.n0 == 0) {  // A times a block of ones, into 16 columns of their own
-            const uint32_t id_ones = idesc(__is_same(T, __half), kBM, 16, kAMn, false);
-            const uint64_t ones = smem_desc<16, 256, kLayoutSw32>(base + kSmOnes);
-#pragma unroll
-            for (int k = 0; k < kBK / 16; ++k) umma_ss_warp(acc + 128, da + k * 128, ones, id_ones, (kb > t.kb0 || k > 0) ? 1u : 0u);
-          }
-          if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + stage) * 8);
-          else umma_commit_warp(bars + (EMPTY + stage) * 8);
-          if (++stage == p.stages) stage = 0, phase ^= 1u;
-        }
-        if constexpr (kAdapt) {
-          auto& adapters = ahead.adapters;
-          adapters.arrived(x.index);
-          auto one = [&](uint64_t a, uint64_t b) {
-            if constexpr (kPair) umma_ss_pair_warp(acc, a, b, id, 1u);
-            else umma_ss_warp(acc, a, b, id, 1u);
-          };
-          auto release_stage = [&](int s) {
-            if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + s) * 8);
-            else umma_commit_warp(bars + (EMPTY + s) * 8);
-          };
-          const bool here = ok && t.split == p.splits - 1;
-          if (x.held && adapters.same) {
-            const int g = adapters.g[0];
-            if (here && g != kNoAdapter) {
-              hold(g, t.n0);
-              if (ok) ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
-              if (!ok) break;
-              tc_fence_after();
-              steps(low_desc | ((ring + stage * stage_bytes) >> 4), held_desc, x.rank, one);
-              release_stage(stage);
-              if (++stage == p.stages) stage = 0, phase ^= 1u;
+        } else {
+          for (int kb = t.kb0; ok && kb < t.kb1; ++kb) {
+            ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t sa = ring + stage * stage_bytes, sb = p.resident ? base + kb * b_bytes : sa + kABytes;
+            // K-major: rows of 128 bytes, groups of 8 rows 1 KiB apart, a step of 16 k is 32 bytes.  MN-major: rows (k) of 64
+            // elements, blocks of 64 elements 8 KiB apart, a step of 16 k is 2 KiB.
+            const uint64_t da = kAMn ? smem_desc<8192, 1024, kLayoutSw128>(sa) : smem_desc<16, 1024, kLayoutSw128>(sa);
+            const uint64_t db = kBMn ? smem_desc<8192, 1024, kLayoutSw128>(sb) : smem_desc<16, 1024, kLayoutSw128>(sb);
+  #pragma unroll
+            for (int k = 0; k < kBK / 16; ++k) {
+              const uint64_t dak = da + k * (kAMn ? 128 : 2), dbk = db + k * (kBMn ? 128 : 2);
+              const uint32_t add = (kb > t.kb0 || k > 0) ? 1u : 0u;
+              if constexpr (kPair) umma_ss_pair_warp(acc, dak, dbk, id, add);
+              else umma_ss_warp(acc, dak, dbk, id, add);
             }
-          } else {
-            uint64_t da = 0;  // the tile's block of t, if held
-            int low_stage = -1, g = kNoAdapter;
-            uint32_t off[kPair ? 8 : 4];
-            bool all = false, low_first = true;
-            auto take = [&]() {
-              g = adapters.take(off);
-              all = low_first && !adapters.more() && adapters.all(off);
-              low_first = false;
-#pragma unroll
-              for (int j = 0; j < (kPair ? 8 : 4); ++j) off[j] = ~off[j];
+            if (kSums && p.sums != nullptr && t.n0 == 0) {  // A times a block of ones, into 16 columns of their own
+              const uint32_t id_ones = idesc(__is_same(T, __half), kBM, 16, kAMn, false);
+              const uint64_t ones = smem_desc<16, 256, kLayoutSw32>(base + kSmOnes);
+  #pragma unroll
+              for (int k = 0; k < kBK / 16; ++k) umma_ss_warp(acc + 128, da + k * 128, ones, id_ones, (kb > t.kb0 || k > 0) ? 1u : 0u);
+            }
+            if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + stage) * 8);
+            else umma_commit_warp(bars + (EMPTY + stage) * 8);
+            if (++stage == p.stages) stage = 0, phase ^= 1u;
+          }
+          if constexpr (kAdapt) {
+            auto& adapters = ahead.adapters;
+            adapters.arrived(x.index);
+            auto one = [&](uint64_t a, uint64_t b) {
+              if constexpr (kPair) umma_ss_pair_warp(acc, a, b, id, 1u);
+              else umma_ss_warp(acc, a, b, id, 1u);
             };
-            auto multiply = [&](uint64_t a, uint64_t b, int ranks) {
-              if (all) steps(a, b, ranks, one);
-              else steps(a, b, ranks, [&](uint64_t ak, uint64_t bk) { umma_ss_lanes_warp(acc, ak, bk, id, off); });
+            auto release_stage = [&](int s) {
+              if constexpr (kPair) umma_commit_pair_warp(bars + (EMPTY + s) * 8);
+              else umma_commit_warp(bars + (EMPTY + s) * 8);
             };
-            for (; here && ok && adapters.more();) {
-              take();
-              if (x.held) {
-                if (low_stage < 0) {
+            const bool here = ok && t.split == p.splits - 1;
+            if (x.held && adapters.same) {
+              const int g = adapters.g[0];
+              if (here && g != kNoAdapter) {
+                hold(g, t.n0);
+                if (ok) ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                steps(low_desc | ((ring + stage * stage_bytes) >> 4), held_desc, x.rank, one);
+                release_stage(stage);
+                if (++stage == p.stages) stage = 0, phase ^= 1u;
+              }
+            } else {
+              uint64_t da = 0;  // the tile's block of t, if held
+              int low_stage = -1, g = kNoAdapter;
+              uint32_t off[kPair ? 8 : 4];
+              bool all = false, low_first = true;
+              auto take = [&]() {
+                g = adapters.take(off);
+                all = low_first && !adapters.more() && adapters.all(off);
+                low_first = false;
+  #pragma unroll
+                for (int j = 0; j < (kPair ? 8 : 4); ++j) off[j] = ~off[j];
+              };
+              auto multiply = [&](uint64_t a, uint64_t b, int ranks) {
+                if (all) steps(a, b, ranks, one);
+                else steps(a, b, ranks, [&](uint64_t ak, uint64_t bk) { umma_ss_lanes_warp(acc, ak, bk, id, off); });
+              };
+              for (; here && ok && adapters.more();) {
+                take();
+                if (x.held) {
+                  if (low_stage < 0) {
+                    ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+                    if (!ok) break;
+                    da = low_desc | ((ring + stage * stage_bytes) >> 4), low_stage = stage;
+                    if (++stage == p.stages) stage = 0, phase ^= 1u;
+                  }
+                  hold(g, t.n0);
+                  if (!ok) break;
+                  tc_fence_after();
+                  multiply(da, held_desc, x.rank);
+                  continue;
+                }
+                if (x.blocks == 1) {
                   ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
                   if (!ok) break;
-                  da = low_desc | ((ring + stage * stage_bytes) >> 4), low_stage = stage;
+                  tc_fence_after();
+                  const uint32_t sa = ring + stage * stage_bytes, bytes = b_rows * x.unit * 2;
+                  const uint64_t low = low_desc | (sa >> 4);
+                  multiply(low, high_desc | ((sa + kABytes) >> 4), x.rank);
+                  for (int j = 1; j < x.share && adapters.more(); ++j) {
+                    take();
+                    multiply(low, high_desc | ((sa + kABytes + j * bytes) >> 4), x.rank);
+                  }
+                  release_stage(stage);
+                  if (++stage == p.stages) stage = 0, phase ^= 1u;
+                  continue;
+                }
+                for (int block = 0; block < x.blocks; ++block) {
+                  ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
+                  if (!ok) break;
+                  tc_fence_after();
+                  const uint32_t sa = ring + stage * stage_bytes;
+                  multiply(low_desc | (sa >> 4), high_desc | ((sa + kABytes) >> 4), x.rank - block * x.unit);
+                  release_stage(stage);
                   if (++stage == p.stages) stage = 0, phase ^= 1u;
                 }
-                hold(g, t.n0);
-                if (!ok) break;
-                tc_fence_after();
-                multiply(da, held_desc, x.rank);
-                continue;
               }
-              if (x.blocks == 1) {
-                ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t sa = ring + stage * stage_bytes, bytes = b_rows * x.unit * 2;
-                const uint64_t low = low_desc | (sa >> 4);
-                multiply(low, high_desc | ((sa + kABytes) >> 4), x.rank);
-                for (int j = 1; j < x.share && adapters.more(); ++j) {
-                  take();
-                  multiply(low, high_desc | ((sa + kABytes + j * bytes) >> 4), x.rank);
-                }
-                release_stage(stage);
-                if (++stage == p.stages) stage = 0, phase ^= 1u;
-                continue;
-              }
-              for (int block = 0; block < x.blocks; ++block) {
-                ok = mbar_wait_warp(bars + (FULL + stage) * 8, phase, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t sa = ring + stage * stage_bytes;
-                multiply(low_desc | (sa >> 4), high_desc | ((sa + kABytes) >> 4), x.rank - block * x.unit);
-                release_stage(stage);
-                if (++stage == p.stages) stage = 0, phase ^= 1u;
-              }
+              if (ok && low_stage >= 0) release_stage(low_stage);
             }
-            if (ok && low_stage >= 0) release_stage(low_stage);
           }
         }
         if (!ok) break;
@@ -1074,7 +1071,6 @@ struct Matmul {
   int beside = kBesideNone;
   void* sums = nullptr;  // see MatmulParams
   const LowRank* adapters = nullptr;
-  const LowProduct* low = nullptr;  // kLow: everything else
   const char* what = "matmul";
 };
 int run_matmul(const Matmul& m, void* stream);
