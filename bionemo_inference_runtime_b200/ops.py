@@ -576,8 +576,10 @@ def adapter_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     ``down [adapters, rank, K]`` and ``up [adapters, N, rank]`` are in the dtype of ``x``, of ranks up to 256.  ``index`` (int32 or int64)
     has the leading axes of ``x`` as its shape, one entry for each request or for each row; a row whose entry is none of
     ``0 .. adapters - 1`` (-1, say) has no adapter.  Without an index all rows have the one adapter.  ``scale`` is a number or fp32,
-    one for each adapter.  Nothing of one request, infinities and NaN
-    among it, reaches another's rows.
+    one for each adapter.  Nothing of one request, infinities and NaN among it, reaches another's rows.  What the formula makes
+    infinite in a row because of infinities in its own adapter (or scale) is an infinity or NaN, here and in the gradients: the low-rank
+    values are held as two numbers, whose products with an infinity may differ in sign.  Infinities in ``x`` alone come out as the
+    formula has them.  In fp16 a low-rank value beyond 65504 is an infinity.
 
     With ``want_saved`` returns ``(y, saved)`` for :func:`adapter_dense_backward`.  Types, sizes, strides and ``out`` as for
     :func:`dense`.

@@ -461,8 +461,8 @@ int b200ta_dense_backward(const void* dy, int64_t dy_row_stride, const void* x, 
  * [count, N or 2 N, rank] lie with one row stride each; `scale` [count] on the device, or NULL for `scale_all`; index of 4 or 8 bytes an
  * entry, or NULL for adapter 0 (of one) everywhere.  Ranks up to 256, up to 16383 adapters.  `low` has
  * b200ta_adapter_low_bytes(rank) bytes for each row, is 16-byte aligned, written here and read again by the backward pass; where
- * b200ta_adapter_dense_needs_low() says no it may be NULL.  Alignment as for
- * b200ta_dense. */
+ * b200ta_adapter_dense_needs_low() says no it may be NULL.  Infinities in a row's own adapter make infinite or NaN what the formula
+ * makes infinite with them.  Alignment as for b200ta_dense. */
 typedef struct {
   const void *down, *up;
   int64_t down_row_stride, up_row_stride;
