@@ -609,7 +609,7 @@ low_join_kernel(const LowJoinParams p) {
 // by passes, now 15.)  Blocks (`blocks_row` for each row) come in rounds of eight on each multiprocessor (1310 rows of 88, rank 20, 10
 // rows a request: 16 us so, 8 by passes).
 bool low_by_rows(int64_t rows, int rank, int K, const AdapterIndex& index, int blocks_row, int num_sms) {
-  const double adapters = index.index == nullptr ? 1 : std::min<double>(index.count, 31 / index.rows_per_index + 1);
+  const double adapters = double(adapters_of_tile(index, rows, 32));
   const double each = 3 + double(rows) * rank * K * 2 / 2e6 + 2.5 * double(rows * blocks_row / (num_sms * 8)), passes = 4 + adapters * (2 + 0.4 * K / 256);
   return rows <= 8192 && each < passes;
 }

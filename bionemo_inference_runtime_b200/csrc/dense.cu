@@ -205,7 +205,7 @@ namespace {
 // Rows that are not 16-byte aligned are shifted into place.
 //
 // With adapters also some hundred rows, 64 to a block: single tokens of many requests have as many adapters in a tile, and the tensor cores
-// take them one after the other (64 rows of 2048 -> 4096 with an adapter each, rank 16: 38 us, now 16).  Here a value's low-rank sum is its own thread's.  The kernel
+// take them one after the other (64 rows of 2048 -> 4096 with an adapter each, rank 16: 23 us, so 17).  Here a value's low-rank sum is its own thread's.  The kernel
 // of the low-rank values runs beside the products, which do not wait for it; a few of a row or two are made in each block instead (one
 // row, 384 -> 1536 gated, rank 16: one launch, 6 us with its way through the host, where two take 9).
 // Without adapters the kernel is one of its own: their branches would take the aligned form from 48 registers a thread to 72 (up to 16 rows
@@ -855,13 +855,13 @@ AdapterIndex index_of(const b200ta_adapters* a) {
 
 // The few rows' kernel with adapters, where rows are single tokens of many requests: on the tensor cores each adapter of a tile is an MMA of
 // its own for every 32 ranks (some 0.4 us), here its weights pass through each block's registers once for 64 rows.  Microseconds; a round is two
-// blocks on each multiprocessor.  (320 tokens of 100 adapters, rank 16: 512 -> 512 12 us so and 40 on the tensor cores, 1024 -> 1024 23 and
-// 31, 2048 -> 4096 70 and 50; of 20 adapters 12 and 20, 23 and 18, 70 and 28; 24 tokens of 6 adapters, 512 -> 512, 6 and 11; 64 rows of 128 -> 512
-// with one adapter 9 and 8.)
+// blocks on each multiprocessor.  (320 tokens of 100 adapters, rank 16: 512 -> 512 12 us so and 29 on the tensor cores, 1024 -> 1024 22 and
+// 32, 2048 -> 4096 70 and 50; of 20 adapters 12 and 16, 22 and 18, 70 and 28; 24 tokens of 6 adapters, 512 -> 512, 5 and 11; 64 rows of 128 -> 512
+// with one adapter 8.5 and 6.5.)
 bool few_with_adapters(int64_t rows, const AdapterIndex& index, int rank, int K, int64_t columns, int num_sms) {
   if (rows <= kFewRows) return true;
   if (rows > 1024) return false;
-  const double adapters = index.index == nullptr ? 1 : double(std::min<int64_t>(index.count, (std::min<int64_t>(rows, 128) - 1) / index.rows_per_index + 1));
+  const double adapters = double(adapters_of_tile(index, rows, matmul::kBM));
   const double tiles = double((rows + 127) / 128) * double(columns) / (256.0 * num_sms);
   const double rounds = double((rows + kFewAdapterRows - 1) / kFewAdapterRows) * double((columns + kFewColumns - 1) / kFewColumns) / (2.0 * num_sms);
   const double here = rows <= 32 ? 4 + std::max(rounds, 1.0) * (0.5 + 0.1 * rank + 0.0025 * K) : 10 + std::max(rounds, 1.0) * (1 + 0.28 * rank + 0.0043 * K);

@@ -11,10 +11,10 @@
 //
 // Bound: HBM (x and residual are read, y is written, once), or issue slots where the generator runs for every element of 16 bits: a
 // block of it serves eight elements, 60 slots of the 32 bytes' 140.  A thread takes several vectors, whose loads are on their way while
-// the generator runs; along a shared axis it makes one block of the generator for all of them.  Measured: 262144 rows of 128 in
-// bf16 with a residual and a shared axis 28.5 us (7.1 TB/s, some of it from L2; loads and stores that mark their lines as used once:
-// 31.5 without), 16384 rows of 2048 in fp16 without either 23 us (5.8
-// TB/s; 28 with a mask of bits between the generator and the elements), in fp32 41 us (6.6 TB/s).
+// the generator runs; along a shared axis it makes one block of the generator for all of them.  Measured back to back: 262144 rows of
+// 128 in bf16 with a residual and a shared axis 31 us (6.5 TB/s), 16384 rows of 2048 in fp16 without either 23 us (5.8 TB/s; 28 with a
+// mask of bits between the generator and the elements), in fp32 41 us (6.6 TB/s).  Loads and stores mark their lines as used once, for
+// the sake of what else is in L2: alone the kernel takes as long without.
 #include <algorithm>
 
 #include "activation.cuh"
