@@ -45,6 +45,7 @@ __host__ __device__ constexpr int low_place(int rank, int r) { return r / low_un
 // product whose right operand has its rows along k.
 struct LowRank {
   AdapterIndex index;
+  int64_t rows;
   int rank;
   const void* low;
   const void* high;

@@ -89,8 +89,8 @@ int run_matmul(const Matmul& m, void* stream) {
   TilingOf tiles{m.form, m.a_mn, m.sums != nullptr, rows, m_outer, columns, p.kblocks_split, p.splits};
   if (m.adapters != nullptr) {
     const int blocks = low_blocks(m.adapters->rank);
-    tiles.more = double(adapters_of_tile(m.adapters->index, rows, matmul::kBM) * blocks);
-    tiles.more_pair = double(adapters_of_tile(m.adapters->index, rows, 2 * matmul::kBM) * blocks);
+    tiles.more = double(adapters_of_tile(m.adapters->index, m.adapters->rows, matmul::kBM) * blocks);
+    tiles.more_pair = double(adapters_of_tile(m.adapters->index, m.adapters->rows, 2 * matmul::kBM) * blocks);
     tiles.held = blocks == 1;
   }
   const Tiling tiling = choose_tiling(tiles, st->num_sms);
@@ -150,10 +150,10 @@ int run_matmul(const Matmul& m, void* stream) {
   if (m.adapters == nullptr) return launch(NoAdapters{});
   const LowRank& a = *m.adapters;
   MatmulAdapters x{};
-  x.index = a.index, x.rank = a.rank, x.unit = low_unit(a.rank), x.blocks = low_blocks(a.rank), x.held = held, x.share = 64 / x.unit;
+  x.index = a.index, x.rows = int(a.rows), x.rank = a.rank, x.unit = low_unit(a.rank), x.blocks = low_blocks(a.rank), x.held = held, x.share = 64 / x.unit;
   x.slots = std::min(matmul::kHighSlots, matmul::held_bytes(x.unit) / (b_rows * x.unit * 2));
   const SwizzleMode swizzle = x.unit == 32 ? SWZ_64 : SWZ_32;
-  const Plane low{a.low, rows, low_pitch(a.rank), low_pitch(a.rank)};
+  const Plane low{a.low, a.rows, low_pitch(a.rank), low_pitch(a.rank)};
   if ((rc = map_of(&x.low, low, 2, uint32_t(2 * x.unit), matmul::kBM, 1, x.unit == 32 ? SWZ_128 : SWZ_64, m.what)) != B200TA_OK) return rc;
   const Plane high = m.b_mn ? Plane{a.high, a.rank, columns, a.high_pitch, a.index.count, a.rank * a.high_pitch}
                             : Plane{a.high, columns, a.rank, a.high_pitch, a.index.count * (two ? 2 : 1), columns * a.high_pitch};
@@ -187,7 +187,7 @@ int run_matmul_low(const LowProduct& q, void* stream) {
   const Plane a{q.a, q.rank, q.K, q.as, q.index.count * q.planes, q.rank * q.as};
   if ((rc = map_of(&maps.b, a, 2, 64, uint32_t(p.tile_n), 1, SWZ_128, what)) != B200TA_OK) return rc;
   MatmulAdapters x{};
-  x.index = q.index, x.rank = q.rank, x.unit = low_unit(q.rank), x.blocks = low_blocks(q.rank);
+  x.index = q.index, x.rows = int(q.rows), x.rank = q.rank, x.unit = low_unit(q.rank), x.blocks = low_blocks(q.rank);
   x.scale = q.scale, x.scale_all = q.scale_all, x.low_out = q.low;
   return launch_matmul_low(st, m, maps, p, x, grid, stream);
 }
@@ -804,12 +804,15 @@ const BackwardPlan& plan_backward(bool gated, bool slope, bool kept, bool want_d
 }
 
 // Where the adapters' intermediates of a backward pass lie behind the others in the workspace.
+constexpr int64_t kExactDxRows = 16;
 struct LowPlan {
   int parts;       // of the rows for the adapters' gradients
   bool direct;     // a single one
   bool by_rows;    // dt from U as it lies
   bool exact;      // dz in two terms for dt and dU
-  int64_t up, low_grad, part[2], marks, dz2, bytes;  // offsets: transposed up, dt of a chunk, parts of dD and dU, their marks, dz's second terms
+  bool exact_dx;   // and for dx
+  // Offsets: transposed up, dt of a chunk, parts of dD and dU, their marks, dz's first terms and behind their rows its second ones, parts of dx.
+  int64_t up, low_grad, part[2], marks, dz, dx_parts, bytes;
 };
 LowPlan plan_low(const BackwardPlan& plan, const AdapterIndex& index, bool kept, int rank, int64_t rows, int K, int N, int outer, int num_sms) {
   LowPlan p{};
@@ -834,7 +837,12 @@ LowPlan plan_low(const BackwardPlan& plan, const AdapterIndex& index, bool kept,
   // the products of dt and dU take both.  Of many values the roundings average (0.0024), and the second terms' time counts (300 rows,
   // 2048 -> 2048 gated, rank 64: a training step 115 us, 141 with them).
   p.exact = kept && rows <= kExactRows && rows * std::min(rank, outer * N) <= 4096;
-  p.dz2 = take(p.exact ? rows * plan.dz_pitch * 2 : 0);
+  p.dz = take(p.exact ? 2 * rows * plan.dz_pitch * 2 : 0);
+  // A row of dx is a sum over the columns, of a few large ones in effect, and of few rows all of them may be off alike (a row of 46 columns,
+  // 16 inputs: 0.0036 of dx's size, now 0.0012, as its own rounding).  Both terms' rows fit into one tile; the join of its parts is at most a
+  // launch more (a row, 1536 -> 384: a backward pass of 15.4 us instead of 13.5).  Of more rows the errors are of all sizes (0.0024).
+  p.exact_dx = p.exact && rows <= kExactDxRows;
+  p.dx_parts = take(p.exact_dx ? 2 * plan.dx_split.parts * rows * pad4(K) * int64_t(sizeof(float)) : 0);
   return p;
 }
 
@@ -926,7 +934,7 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
   const BackwardPlan& plan = plan_backward(gated, activation != kActNone, kept, dbias != nullptr, rows, K, N, st->num_sms);
   const int64_t outer = gated ? 2 : 1;
   const LowPlan low_plan = ad != nullptr ? plan_low(plan, index_of(ad), kept, ad->rank, rows, K, N, int(outer), st->num_sms)
-                                            : LowPlan{0, false, false, false, 0, 0, {0, 0}, 0, 0, plan.bytes};
+                                            : LowPlan{0, false, false, false, false, 0, 0, {0, 0}, 0, 0, 0, plan.bytes};
   B200TA_REQUIRE(low_plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0 &&
                                          workspace_bytes >= size_t(low_plan.bytes)),
                  "dense_backward: the workspace must be 256-byte aligned and of %lld bytes", (long long)low_plan.bytes);
@@ -936,7 +944,10 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
   float* sums = reinterpret_cast<float*>(ws_base + plan.sums);
   const int64_t sum_pitch = own_dz ? plan.dz_pitch : pad8(N);  // columns of dz that are summed, padding included
   const int sum_columns = int(own_dz ? plan.dz_pitch : N);
-  const bool direct = plan.direct, product_sums = plan.split.sums && dw != nullptr && dbias != nullptr;
+  // (With adapters and few rows db is summed before dz is rounded: of a few columns its error would be that of dz's roundings, 13 x 4 rows,
+  // 80 -> 16, 0.0030 of db's size, now 0.0011.  The join is up to 2 us more.)
+  const bool exact_sums = ad != nullptr && kept && rows <= 2 * kExactRows;
+  const bool direct = plan.direct, product_sums = plan.split.sums && dw != nullptr && dbias != nullptr && !exact_sums;
 
   auto join_of = [&](bool wanted, const float* part, int64_t count, int64_t stride, int64_t pitch, int64_t n_rows, int columns, void* out) {
     const bool four = columns % 4 == 0 && pitch % 4 == 0 && stride % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7u) == 0;
@@ -949,17 +960,20 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
                          dim3(unsigned(a.blocks + b.blocks + c.blocks)), 256, 0, stream, a, b, c);
   };
   const bool narrow = ad == nullptr && narrow_pays(own_dz, kept, gated != 0, rows, K, N, dx, dxs, st->num_sms);
-  const bool dx_parts = dx != nullptr && !narrow && plan.dx_split.parts > 1 && dxs == K;  // (a join writes dense rows)
+  const bool dx_dense = dx != nullptr && !narrow && dxs == K;  // (a join writes dense rows)
+  const bool exact_dx = dx_dense && low_plan.exact_dx, dx_parts = exact_dx || (dx_dense && plan.dx_split.parts > 1);
+  const int64_t dx_terms = exact_dx ? 2 : 1;
+  char* dx_part = ws_base + (exact_dx ? low_plan.dx_parts : plan.dx_parts);
 
   // adapters: t (from the forward pass) with U for the pre-activations, dt with D for dx
   const int64_t low_bytes = ad != nullptr ? low_pitch(ad->rank) * 2 : 0;
   LowRank with_up{}, with_down{};
   LowGrads low_grads{};
   void* dt = ws_base + low_plan.low_grad;
-  void* dz2 = low_plan.exact ? ws_base + low_plan.dz2 : nullptr;
+  void* dz2 = low_plan.exact ? ws_base + low_plan.dz + rows * plan.dz_pitch * 2 : nullptr;
   if (ad != nullptr) {
-    with_up = {index_of(ad), ad->rank, nullptr, ad->up, ad->up_row_stride};
-    with_down = {index_of(ad), ad->rank, dt, ad->down, ad->down_row_stride};
+    with_up = {index_of(ad), 0, ad->rank, nullptr, ad->up, ad->up_row_stride};
+    with_down = {index_of(ad), 0, ad->rank, dt, ad->down, ad->down_row_stride};
     low_grads.job[0] = {dt, nullptr, nullptr, reinterpret_cast<float*>(ws_base + low_plan.part[0]), ddown, xs, 0, K, 1, 0};
     low_grads.job[1] = {nullptr, nullptr, nullptr, reinterpret_cast<float*>(ws_base + low_plan.part[1]), dup, 0, 0, N, int(outer), 1};
     low_grads.rank = ad->rank, low_grads.parts = low_plan.parts, low_grads.f16 = f16;
@@ -974,13 +988,14 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
     const int64_t n = rows - r0 < plan.chunk ? rows - r0 : plan.chunk;
     const char* low_c = static_cast<const char*>(low) + r0 * low_bytes;
     with_up.low = low_c;
+    with_up.rows = with_down.rows = n;
     with_up.index.first_row = with_down.index.first_row = uint32_t(r0);
     const char* dy_c = static_cast<const char*>(dy) + r0 * dys * 2;
     const char* x_c = static_cast<const char*>(x) + r0 * xs * 2;
     const void* dz = dy_c;
     int64_t zs = dys;
     if (own_dz) {
-      void* dst = ws_base + plan.dz;
+      void* dst = ws_base + (low_plan.exact ? low_plan.dz : plan.dz);
       dz = dst, zs = plan.dz_pitch;
       if (narrow) {
         Narrow m;
@@ -1022,10 +1037,10 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
     if (dx != nullptr && !narrow) {
       Matmul m;
       m.form = dx_parts ? kPartial : kPlain, m.b_mn = true, m.f16 = f16;
-      m.a = {dz, n, N, zs, outer, zs / 2};
+      m.a = {dz, dx_terms * n, N, zs, outer, zs / 2};
       m.b = {w, N, K, ws, outer, int64_t(N) * ws};
       if (dx_parts) {
-        m.out = {ws_base + plan.dx_parts, n, K, pad4(K), plan.dx_split.parts, n * pad4(K)};
+        m.out = {dx_part, dx_terms * n, K, pad4(K), plan.dx_split.parts, dx_terms * n * pad4(K)};
         m.kblocks_split = plan.dx_split.kblocks;
       } else {
         m.out = {static_cast<char*>(dx) + r0 * dxs * 2, n, K, dxs};
@@ -1079,7 +1094,7 @@ int dense_gradients(const void* dy, int64_t dys, const void* x, int64_t xs, cons
   const JoinParams a = join_of(parts_left, parts, plan.split.parts, outer * N * pad4(K), pad4(K), outer * N, K, dw);
   const JoinParams b = product_sums ? join_of(sums_left, sums, plan.split.parts, outer * N, N, outer, N, dbias)
                                     : join_of(sums_left, sums, (chunk + plan.rows_sum - 1) / plan.rows_sum, sum_pitch, sum_pitch / outer, outer, N, dbias);
-  const JoinParams c = join_of(dx_parts, reinterpret_cast<const float*>(ws_base + plan.dx_parts), plan.dx_split.parts, rows * pad4(K), pad4(K), rows, K, dx);
+  const JoinParams c = join_of(dx_parts, reinterpret_cast<const float*>(dx_part), dx_terms * plan.dx_split.parts, rows * pad4(K), pad4(K), rows, K, dx);
   return join(a, b, c);
 }
 
@@ -1137,7 +1152,7 @@ int b200ta_adapter_dense(const void* x, int64_t xs, const void* w, int64_t ws, c
   const bool own = own_low_pays(rows, a->rank, K);
   B200TA_REQUIRE(low || own, "adapter_dense: NULL pointer");
   if (!own && (rc = run_low(q, stream)) != B200TA_OK) return rc;
-  const LowRank adapters{q.index, a->rank, own ? nullptr : low, a->up, a->up_row_stride};
+  const LowRank adapters{q.index, rows, a->rank, own ? nullptr : low, a->up, a->up_row_stride};
   return dense_forward(x, xs, w, ws, bias, residual, rs, y, ys, saved, ss, dtype, activation, gated, rows, K, N, &adapters, own ? &q : nullptr, stream);
 }
 

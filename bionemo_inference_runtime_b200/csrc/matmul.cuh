@@ -84,6 +84,7 @@ struct NoAdapters {};
 struct MatmulAdapters {
   CUtensorMap low, high;
   AdapterIndex index;
+  int rows;            // of D that may have an adapter
   int rank, unit, blocks;
   int held, slots;     // room for that many blocks of U_g
   int share;           // adapters that share a stage of the ring (with a single block of ranks)
@@ -174,14 +175,14 @@ struct TileRows<true, kPair, kOuter> {
   TileAdapters<kPair ? 8 : 4> adapters;
   __device__ __forceinline__ TileRows(const MatmulParams& p, const MatmulAdapters& x, int units)
       : upcoming(item_of<kPair, kOuter>(p, 0, units)), adapters(x.index) {
-    adapters.fetch(x.index, upcoming.m0, p.rows_inner);
+    adapters.fetch(x.index, upcoming.m0, x.rows);
   }
   __device__ __forceinline__ Item item(const MatmulParams&, int, int) const { return upcoming; }
   __device__ __forceinline__ void look(const MatmulParams& p, const MatmulAdapters& x, int i, int items, int units) {
     if (i >= items) return;
     if (p.resident) upcoming.m0 += p.resident * (kPair ? 2 * kBM : kBM);
     else upcoming = item_of<kPair, kOuter>(p, i, units);
-    adapters.fetch(x.index, upcoming.m0, p.rows_inner);
+    adapters.fetch(x.index, upcoming.m0, x.rows);
   }
 };
 // The held block of U_g that is used last: whose it is, where it lies, and the phase of its barriers.

@@ -577,8 +577,9 @@ def adapter_dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     has the leading axes of ``x`` as its shape, one entry for each request or for each row; a row whose entry is none of
     ``0 .. adapters - 1`` (-1, say) has no adapter.  Without an index all rows have the one adapter.  ``scale`` is a number or fp32,
     one for each adapter.  Nothing of one request, infinities and NaN among it, reaches another's rows.  What the formula makes
-    infinite in a row because of infinities in its own adapter (or scale) is an infinity or NaN, here and in the gradients: the low-rank
-    values are held as two numbers, whose products with an infinity may differ in sign.  Infinities in ``x`` alone come out as the
+    infinite because of infinities in a row's own adapter or scale, or in a gradient because of infinities in the shared weight, is an
+    infinity or NaN: low-rank values are held as two numbers, gradients of few rows as well, whose products with an infinity may differ in
+    sign.  Infinities in ``x`` alone come out as the
     formula has them.  In fp16 a low-rank value beyond 65504 is an infinity.
 
     With ``want_saved`` returns ``(y, saved)`` for :func:`adapter_dense_backward`.  Types, sizes, strides and ``out`` as for
@@ -594,7 +595,9 @@ def adapter_dense_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tens
                            want_dbias: bool = False, want_ddown: bool = True, want_dup: bool = True):
     """``(dx, dweight, dbias, ddown, dup)`` of :func:`adapter_dense` (the gradient of its residual is ``dy``); ``saved`` is what the
     forward pass returned.  The shared weight and bias are taken as frozen unless ``want_dweight`` and ``want_dbias`` say otherwise.
-    The gradient before the activation is rounded to the dtype of ``x`` between the kernels; sums over rows are in fp32 and in a fixed order, each adapter's over its own rows alone."""
+    The gradient before the activation is rounded to the dtype of ``x`` between the kernels (of few rows it is held in two numbers for
+    ``dx``, ``ddown`` and ``dup``, and summed before it is rounded for ``dbias``); sums over rows are in fp32 and in a fixed order, each
+    adapter's over its own rows alone."""
     return _host.adapter_dense_backward(dy, x, weight, bias, down, up, index, *_scale(scale), *saved, _activation(activation), False, want_dx,
                                         want_dweight, want_dbias, want_ddown, want_dup)
 
